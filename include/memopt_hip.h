@@ -296,6 +296,98 @@ int memopt_paged_attention_noalloc(const memopt_attn_desc *desc, void *stream);
 #define MEMOPT_PATH_DIRECT 2  /* attended straight from the cache (csrc/direct.hip)       */
 int memopt_multi_query_path(int32_t path);
 
+/* ------------------------------------------------------------------------ */
+/* Packed batches: grouped heads, sequences of different lengths            */
+/* ------------------------------------------------------------------------ */
+/* No counterparts in the reference, whose attention takes one query head per
+ * cached head and the same number of queries from every sequence, and whose
+ * callers build block tables and slots on the host.
+ *
+ * A packed tensor holds the rows of `batch` sequences one behind the other:
+ * query_starts (int32 [batch + 1], device, ascending from >= 0 to <= tokens)
+ * gives sequence b the rows query_starts[b] .. query_starts[b + 1] - 1.
+ * Entries outside [0, tokens] are clamped; rows of no sequence are neither
+ * read nor written. Query head h reads key head h / (num_heads /
+ * num_kv_heads). Strides are in elements; a row's head_dim elements are
+ * contiguous, rows are 16-byte aligned. */
+
+/* Element types of memopt_prompt_desc. */
+#define MEMOPT_FP16 0
+#define MEMOPT_BF16 1
+
+/* Causal attention over whole prompts from q, k and v as a layer's
+ * projections leave them (views of a fused projection included): row i of a
+ * sequence sees its rows j <= i with j < num_sink_tokens or j > i -
+ * window_size (window_size <= 0: all j <= i), scale 1/sqrt(head_dim).
+ * Elements of hidden rows never reach a result, inf and NaN included.
+ * head_dim 64 or 128. `out` must not overlap the inputs. */
+typedef struct memopt_prompt_desc {
+  const void *query, *key, *value;   /* [tokens, heads, head_dim]              */
+  void *out;                         /* [tokens, num_heads, head_dim]          */
+  int32_t dtype;                     /* MEMOPT_FP16 / MEMOPT_BF16              */
+  int32_t tokens, batch, num_heads, num_kv_heads, head_dim;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride, o_token_stride, o_head_stride;
+  const int32_t *query_starts;
+  int32_t window_size, num_sink_tokens;
+} memopt_prompt_desc;
+int memopt_prompt_attention(const memopt_prompt_desc *desc, void *stream);
+
+/* Attention of packed queries over a paged cache: sequence b's rows are the
+ * last positions of its context_lens[b] tokens (row i of n at position
+ * context_lens[b] - n + i), and see what the causal rule of
+ * memopt_paged_attention shows them (window, sinks, unlinked pages skipped,
+ * window_size <= 0 or > max_seq_len: max_seq_len; a row that sees nothing
+ * gives 0). Sequences may bring different numbers of rows, none included.
+ * Caches: MEMOPT_KV_INT4 page buffers (key_cache; value_cache unused) and
+ * contiguous MEMOPT_KV_FP16 pools with block_size a multiple of 16, both with
+ * num_kv_heads heads; head_dim 64 or 128; INT4 values are (code - 8) * scale.
+ * max_query_len bounds the rows of any one sequence (rows past it may be left
+ * unwritten). */
+typedef struct memopt_packed_desc {
+  const void *query;                 /* fp16 [tokens, num_heads, head_dim]     */
+  void *out;                         /* fp16 [tokens, num_heads, head_dim]     */
+  int32_t tokens, batch, num_heads, num_kv_heads, head_dim;
+  int64_t q_token_stride, q_head_stride, o_token_stride, o_head_stride;
+  int32_t kv_format;                 /* MEMOPT_KV_FP16 / MEMOPT_KV_INT4        */
+  const void *key_cache, *value_cache;
+  int32_t block_size;
+  int64_t num_kv_blocks;
+  const int32_t *block_tables;       /* [batch, max_blocks_per_seq]            */
+  int32_t max_blocks_per_seq;
+  const int32_t *context_lens;       /* [batch]                                */
+  const int32_t *query_starts;       /* [batch + 1]                            */
+  int32_t max_query_len, max_seq_len, window_size, num_sink_tokens;
+  void *workspace;                   /* >= memopt_packed_workspace_size bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+} memopt_packed_desc;
+int memopt_packed_workspace_size(const memopt_packed_desc *desc, int64_t *bytes);
+int memopt_packed_attention(const memopt_packed_desc *desc, void *stream);
+
+/* The index tensors of a batch's next step, built on the device. Request b
+ * holds context_lens[b] tokens in the pages of its block table row and asks
+ * for new_tokens[b] more. Free pages are a ring: free_pages[(free_span[0] +
+ * i) % num_free_pages] for i < free_span[1], taken from the front in request
+ * order (the FIFO order of memopt_allocate_block). Requests are served in
+ * order while the sums of what the valid requests so far ask for stay within
+ * the free pages and num_rows (one that needs no page is not refused for
+ * pages). Written: the new entries of block_tables; context_lens_out and
+ * free_span_out (which may be the inputs); query_starts [num_requests + 1];
+ * slots and positions [num_rows], request by request, -1 behind the last row
+ * (memopt_write_cache skips those); status [num_requests]: */
+#define MEMOPT_STEP_SERVED   0
+#define MEMOPT_STEP_INVALID  1  /* a negative count, or more tokens than the table's row holds */
+#define MEMOPT_STEP_UNLINKED 2  /* the page that holds its last token was evicted               */
+#define MEMOPT_STEP_NO_PAGES 3
+#define MEMOPT_STEP_NO_ROWS  4
+/* A request that is not served stays as it was and gets no rows. At most 4096
+ * requests; calls on one batch must not overlap. */
+int memopt_advance_batch(const int32_t *new_tokens, const int32_t *context_lens, int32_t num_requests,
+                         int32_t *block_tables, int32_t max_blocks_per_seq, const int32_t *free_pages,
+                         int32_t num_free_pages, const int32_t *free_span, int32_t block_size, int32_t num_rows,
+                         int32_t *context_lens_out, int32_t *free_span_out, int32_t *query_starts, int32_t *slots,
+                         int32_t *positions, int32_t *status, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

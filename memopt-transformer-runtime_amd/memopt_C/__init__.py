@@ -21,7 +21,10 @@ reference behaviour):
     key_scales=None, value_scales=None, kv_layout=None)`` — INT4 caches are
     dequantized just in time inside the kernel;
   * ``free_evicted_blocks(is_block_free)`` — the post-eviction sweep the
-    reference documents but never implements (src/csrc/kv_cache.cu:1033-1036).
+    reference documents but never implements (src/csrc/kv_cache.cu:1033-1036);
+  * ``prompt_attention``, ``packed_attention`` / ``PreparedPackedAttention``
+    and ``advance_batch`` — packed batches with grouped heads: whole prompts
+    straight from q, k and v, the paged cache, and a step's index tensors.
 
 The library is loaded at import; a missing or unloadable library raises
 ``ImportError`` naming the path (there is no CPU fallback).
@@ -32,7 +35,7 @@ import contextlib
 import ctypes
 import os
 import threading
-from typing import List, Optional, Sequence, Tuple
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch  # must precede the HIP library so both share one HIP runtime
 
@@ -41,7 +44,8 @@ __all__ = [
     "get_key_pool", "get_value_pool", "get_pool_scales", "get_int4_pages", "int4_layout", "free_blocks_count",
     "write_cache", "evict_cache", "evict_tokens", "free_evicted_blocks",
     "dynamic_sparse_attention", "PreparedAttention", "quantize_kv_cache_int4", "dequantize_kv_cache_int4",
-    "library_path",
+    "prompt_attention", "packed_attention", "PreparedPackedAttention", "advance_batch", "advance_batch_buffers",
+    "BatchStep", "library_path",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -72,6 +76,33 @@ class AttnDesc(ctypes.Structure):
         ("sc_page_stride", _i64), ("sc_head_stride", _i64), ("sc_token_stride", _i64),
         ("block_tables", _vp), ("max_blocks_per_seq", _i32), ("context_lens", _vp),
         ("max_seq_len", _i32), ("window_size", _i32), ("num_sink_tokens", _i32), ("causal", _i32),
+        ("workspace", _vp), ("workspace_bytes", _i64),
+    ]
+
+
+class PromptDesc(ctypes.Structure):
+    """Mirror of ``memopt_prompt_desc`` (include/memopt_hip.h)."""
+
+    _fields_ = [
+        ("query", _vp), ("key", _vp), ("value", _vp), ("out", _vp),
+        ("dtype", _i32), ("tokens", _i32), ("batch", _i32), ("num_heads", _i32), ("num_kv_heads", _i32),
+        ("head_dim", _i32),
+        ("q_token_stride", _i64), ("q_head_stride", _i64), ("k_token_stride", _i64), ("k_head_stride", _i64),
+        ("v_token_stride", _i64), ("v_head_stride", _i64), ("o_token_stride", _i64), ("o_head_stride", _i64),
+        ("query_starts", _vp), ("window_size", _i32), ("num_sink_tokens", _i32),
+    ]
+
+
+class PackedDesc(ctypes.Structure):
+    """Mirror of ``memopt_packed_desc`` (include/memopt_hip.h)."""
+
+    _fields_ = [
+        ("query", _vp), ("out", _vp),
+        ("tokens", _i32), ("batch", _i32), ("num_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32),
+        ("q_token_stride", _i64), ("q_head_stride", _i64), ("o_token_stride", _i64), ("o_head_stride", _i64),
+        ("kv_format", _i32), ("key_cache", _vp), ("value_cache", _vp), ("block_size", _i32), ("num_kv_blocks", _i64),
+        ("block_tables", _vp), ("max_blocks_per_seq", _i32), ("context_lens", _vp), ("query_starts", _vp),
+        ("max_query_len", _i32), ("max_seq_len", _i32), ("window_size", _i32), ("num_sink_tokens", _i32),
         ("workspace", _vp), ("workspace_bytes", _i64),
     ]
 
@@ -107,6 +138,11 @@ _c_dsa = _sig("memopt_dynamic_sparse_attention",
 _c_ws = _sig("memopt_attention_workspace_size", [ctypes.POINTER(AttnDesc), ctypes.POINTER(_i64)])
 _c_attn = _sig("memopt_paged_attention", [ctypes.POINTER(AttnDesc), _vp])
 _c_attn_noalloc = _sig("memopt_paged_attention_noalloc", [ctypes.POINTER(AttnDesc), _vp])
+_c_prompt = _sig("memopt_prompt_attention", [ctypes.POINTER(PromptDesc), _vp])
+_c_packed_ws = _sig("memopt_packed_workspace_size", [ctypes.POINTER(PackedDesc), ctypes.POINTER(_i64)])
+_c_packed = _sig("memopt_packed_attention", [ctypes.POINTER(PackedDesc), _vp])
+_c_advance = _sig("memopt_advance_batch",
+                  [_vp, _vp, _i32, _vp, _i32, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp])
 
 KV_FP16, KV_INT4, KV_INT4_ROWS = 0, 1, 2
 _FORMATS = {"fp16": KV_FP16, "int4": KV_INT4}
@@ -732,3 +768,265 @@ class PreparedAttention:
             s = stream if stream is not None else torch._C._cuda_getCurrentRawStream(self.device.index)
             _check(self._fn(self._dp, s))
         return self.out
+
+
+# ---------------------------------------------------------------------------
+# Packed batches: grouped heads, sequences of different lengths (no
+# counterparts in the reference)
+# ---------------------------------------------------------------------------
+
+def _device_tensors(fn: str, device: torch.device, *tensors) -> None:
+    for t, n in tensors:
+        if not (isinstance(t, torch.Tensor) and t.is_cuda):
+            raise RuntimeError(f"{fn}: {n} must be a CUDA tensor")
+        if t.device != device:
+            raise RuntimeError(f"{fn}: {n} on a different device")
+
+
+def _int32(fn: str, t: torch.Tensor, name: str, shape: Tuple[int, ...]) -> None:
+    if not (t.dtype == torch.int32 and tuple(t.shape) == shape and t.is_contiguous()):
+        raise RuntimeError(f"{fn}: {name} must be a contiguous int32 tensor of shape {list(shape)}")
+
+
+def _no_grad(fn: str, *tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{fn}: no gradients are computed; call it under torch.no_grad()")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself where its last dimension is contiguous and its rows are
+    16-byte aligned (views of a fused projection are), else a contiguous copy."""
+    s = t.stride()
+    if s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0 and s[0] >= t.shape[2]:
+        return t
+    return t.contiguous()
+
+
+def _out_rows(fn: str, out: Optional[torch.Tensor], query: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    s = out.stride()
+    if not (out.shape == query.shape and out.dtype == query.dtype and out.device == query.device and s[2] == 1 and
+            s[0] % 8 == 0 and s[1] % 8 == 0 and out.data_ptr() % 16 == 0):
+        raise RuntimeError(f"{fn}: out must be shaped like query, with contiguous 16-byte aligned rows")
+    return out
+
+
+def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, cu_seqlens: torch.Tensor,
+                     window_size: int = -1, *, num_sink_tokens: int = 0,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention over whole prompts packed one behind the other; returns ``[T, Hq, D]``.
+
+    ``query`` ``[T, Hq, D]``, ``keys`` / ``values`` ``[T, Hkv, D]``: fp16 or
+    bf16, D 64 or 128, Hq a multiple of Hkv (query head h reads key head
+    ``h // (Hq / Hkv)``); any strides whose rows are contiguous and 16-byte
+    aligned, such as views of a fused projection, are read in place.
+    ``cu_seqlens``: int32 ``[B + 1]`` on the device, ascending; sequence b is
+    rows ``cu_seqlens[b] .. cu_seqlens[b + 1] - 1``. Row i of a sequence sees
+    its rows ``j <= i`` with ``j < num_sink_tokens`` or ``j > i -
+    window_size`` (``window_size <= 0``: all of them), scale 1/sqrt(D).
+    Rows of no sequence are left as they are in ``out`` (a fresh ``out`` is
+    not initialized there). ``out`` must not overlap the inputs.
+    """
+    fn = "prompt_attention"
+    _require(isinstance(query, torch.Tensor) and query.is_cuda, "prompt_attention: query must be a CUDA tensor")
+    _device_tensors(fn, query.device, (keys, "keys"), (values, "values"), (cu_seqlens, "cu_seqlens"))
+    _no_grad(fn, query, keys, values)
+    _require(query.dim() == 3 and keys.dim() == 3 and values.dim() == 3,
+             "prompt_attention: query, keys and values must be 3-D [tokens, heads, head_dim]")
+    T, Hq, D = query.shape
+    Hk = keys.shape[1]
+    _require(query.dtype in (torch.float16, torch.bfloat16), "prompt_attention: query must be fp16 or bf16")
+    _require(keys.dtype == query.dtype and values.dtype == query.dtype,
+             "prompt_attention: keys and values must have query's dtype")
+    if not (tuple(keys.shape) == (T, Hk, D) and keys.shape == values.shape):
+        raise RuntimeError(f"{fn}: keys and values must be [{T}, kv heads, {D}], got {list(keys.shape)} and "
+                           f"{list(values.shape)}")
+    _require(cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1, "prompt_attention: cu_seqlens must be 1-D [batch + 1]")
+    B = cu_seqlens.shape[0] - 1
+    _int32(fn, cu_seqlens, "cu_seqlens", (B + 1,))
+    out = _out_rows(fn, out, query)
+    q, k, v = _rows(query), _rows(keys), _rows(values)
+    with _on(query.device):
+        d = PromptDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), int(q.dtype == torch.bfloat16), T, B,
+                       Hq, Hk, D, q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                       out.stride(0), out.stride(1), cu_seqlens.data_ptr(), int(window_size), int(num_sink_tokens))
+        _check(_c_prompt(ctypes.byref(d), _stream(query)))
+    return out
+
+
+def _packed_desc(query, key_cache, value_cache, block_tables, context_lens, cu_seqlens, max_query_len, max_seq_len,
+                 window_size, num_sink_tokens, out):
+    """Validated PackedDesc: (desc, out, workspace, keepalive)."""
+    fn = "packed_attention"
+    _device_tensors(fn, query.device, (key_cache, "key_cache"), (value_cache, "value_cache"),
+                    (block_tables, "block_tables"), (context_lens, "context_lens"), (cu_seqlens, "cu_seqlens"))
+    _no_grad(fn, query)
+    _require(query.dim() == 3, "packed_attention: query must be 3-D [tokens, heads, head_dim]")
+    _require(query.dtype == torch.float16, "packed_attention: query must be fp16")
+    T, Hq, D = query.shape
+    _require(cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1, "packed_attention: cu_seqlens must be 1-D [batch + 1]")
+    B = cu_seqlens.shape[0] - 1
+    _int32(fn, cu_seqlens, "cu_seqlens", (B + 1,))
+    _int32(fn, context_lens, "context_lens", (B,))
+    _require(block_tables.dim() == 2, "packed_attention: block_tables must be 2-D [batch, max_blocks_per_seq]")
+    _int32(fn, block_tables, "block_tables", (B, block_tables.shape[1]))
+    _require(max_query_len >= 0, "packed_attention: max_query_len must not be negative")
+    keep = (query, key_cache, value_cache, block_tables, context_lens, cu_seqlens)
+    if key_cache.dtype == torch.uint8:
+        _require(D in (64, 128), "packed_attention: head_dim must be 64 or 128")
+        _require(key_cache.dim() == 3 and value_cache.dim() == 3 and key_cache.shape[1] > 0,
+                 "packed_attention: INT4 caches are the pool's code views or its page buffer [pages, heads, bytes]")
+        Hk = key_cache.shape[1]
+        pages = _int4_pages_base(key_cache, value_cache, Hk, D)
+        _require(pages is not None, "packed_attention: not an INT4 page buffer of this head_dim")
+        base_k, nb, buf = pages
+        _require(buf.device == query.device, "packed_attention: key_cache on a different device")
+        fmt, bs, base_v, keep = KV_INT4, 16, None, keep + (buf,)
+    else:
+        _require(key_cache.dtype == torch.float16 and value_cache.dtype == torch.float16,
+                 "packed_attention: caches must be fp16 or INT4 pages")
+        _require(key_cache.dim() == 4 and key_cache.shape == value_cache.shape and key_cache.shape[3] == D,
+                 "packed_attention: caches must be 4-D [num_kv_blocks, block_size, kv heads, head_dim]")
+        _require(key_cache.is_contiguous() and value_cache.is_contiguous(),
+                 "packed_attention: caches must be contiguous")
+        nb, bs, Hk = key_cache.shape[:3]
+        fmt, base_k, base_v = KV_FP16, key_cache.data_ptr(), value_cache.data_ptr()
+    out = _out_rows(fn, out, query)
+    q = _rows(query)
+    d = PackedDesc(q.data_ptr(), out.data_ptr(), T, B, Hq, Hk, D, q.stride(0), q.stride(1), out.stride(0),
+                   out.stride(1), fmt, base_k, base_v, bs, nb, block_tables.data_ptr(), block_tables.shape[1],
+                   context_lens.data_ptr(), cu_seqlens.data_ptr(), int(max_query_len), int(max_seq_len),
+                   int(window_size), int(num_sink_tokens))
+    need = _i64()
+    _check(_c_packed_ws(ctypes.byref(d), ctypes.byref(need)))
+    ws = None
+    if need.value > 0:
+        ws = torch.empty(need.value, dtype=torch.uint8, device=query.device)
+        d.workspace, d.workspace_bytes = ws.data_ptr(), need.value
+    return d, out, ws, keep + (q,)
+
+
+def packed_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                     block_tables: torch.Tensor, context_lens: torch.Tensor, cu_seqlens: torch.Tensor,
+                     max_query_len: int, max_seq_len: int, window_size: int = -1, *, num_sink_tokens: int = 0,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of packed queries over the paged cache with grouped heads; returns fp16 ``[T, Hq, D]``.
+
+    Sequence b's queries are rows ``cu_seqlens[b] .. cu_seqlens[b + 1] - 1``
+    of ``query`` ``[T, Hq, D]`` (fp16; strides as in ``prompt_attention``):
+    the last positions of its ``context_lens[b]`` tokens, whose K/V are in the
+    cache already. Each sequence may bring any number of them (decode: one);
+    ``max_query_len`` bounds it. Caches: INT4 pages (the pool's code views,
+    or a page buffer passed as both) or fp16 pools, with Hkv heads that divide
+    Hq. Masks, windows and sinks are those of ``dynamic_sparse_attention(...,
+    causal=True)``; a row that sees no key gives 0. Rows of no sequence are
+    left as they are in ``out``.
+    """
+    _require(isinstance(query, torch.Tensor) and query.is_cuda, "packed_attention: query must be a CUDA tensor")
+    with _on(query.device):
+        d, out, ws, _keep = _packed_desc(query, key_cache, value_cache, block_tables, context_lens, cu_seqlens,
+                                         max_query_len, max_seq_len, window_size, num_sink_tokens, out)
+        _check(_c_packed(ctypes.byref(d), _stream(query)))
+    return out
+
+
+class PreparedPackedAttention:
+    """A validated ``packed_attention`` call bound to fixed tensors.
+
+    Construction checks the arguments and allocates the workspace; each call
+    launches on the current stream and returns ``out`` (overwritten in place).
+    For loops in which only the tensors' contents change. Calls of one plan
+    share its workspace and must not overlap.
+    """
+
+    def __init__(self, query, key_cache, value_cache, block_tables, context_lens, cu_seqlens, max_query_len,
+                 max_seq_len, window_size=-1, *, num_sink_tokens=0, out=None):
+        _require(isinstance(query, torch.Tensor) and query.is_cuda, "packed_attention: query must be a CUDA tensor")
+        self.device = query.device
+        _require(_rows(query) is query,
+                 "PreparedPackedAttention: query's rows must be contiguous and 16-byte aligned (it is read in place)")
+        with _on(self.device):
+            self._d, self.out, self._ws, self._keep = _packed_desc(
+                query, key_cache, value_cache, block_tables, context_lens, cu_seqlens, max_query_len, max_seq_len,
+                window_size, num_sink_tokens, out)
+        self._dp = ctypes.byref(self._d)
+
+    @property
+    def workspace_bytes(self) -> int:
+        return 0 if self._ws is None else self._ws.numel()
+
+    def __call__(self, stream: Optional[int] = None) -> torch.Tensor:
+        with _on(self.device):
+            s = stream if stream is not None else torch._C._cuda_getCurrentRawStream(self.device.index)
+            _check(_c_packed(self._dp, s))
+        return self.out
+
+
+class BatchStep(NamedTuple):
+    """What ``advance_batch`` writes (int32): ``context_lens`` ``[B]``,
+    ``free_span`` ``[2]``, ``cu_seqlens`` ``[B + 1]``, ``slots`` and
+    ``positions`` ``[rows]``, ``status`` ``[B]``."""
+    context_lens: torch.Tensor
+    free_span: torch.Tensor
+    cu_seqlens: torch.Tensor
+    slots: torch.Tensor
+    positions: torch.Tensor
+    status: torch.Tensor
+
+
+def advance_batch_buffers(num_requests: int, num_rows: int, device) -> BatchStep:
+    """Buffers for ``advance_batch(..., out=)``."""
+    sizes = (num_requests, 2, num_requests + 1, num_rows, num_rows, num_requests)
+    return BatchStep(*(torch.empty(n, dtype=torch.int32, device=device) for n in sizes))
+
+
+def advance_batch(new_tokens: torch.Tensor, context_lens: torch.Tensor, block_tables: torch.Tensor,
+                  free_pages: torch.Tensor, free_span: torch.Tensor, block_size: int, num_rows: Optional[int] = None, *,
+                  out: Optional[BatchStep] = None) -> BatchStep:
+    """The index tensors of a batch's next step, built on the GPU (nothing is read back).
+
+    Request b holds ``context_lens[b]`` tokens in the pages of
+    ``block_tables[b]`` (int32 ``[B, M]``, its new entries are written in
+    place) and asks for ``new_tokens[b]`` more. ``free_pages`` int32 ``[C]``
+    is a ring whose free pages start at ``free_span[0]``, ``free_span[1]`` of
+    them; they are taken in request order. Requests are served in order while
+    what the valid ones so far ask for fits the free pages and ``num_rows``
+    (one that needs no page is not refused for pages); the others stay as
+    they were. ``status`` is 0 for a served request, 1 for an invalid count,
+    2 where the page of its last token was evicted, 3 and 4 where pages or
+    rows did not last. ``slots`` (for ``write_cache``) and ``positions`` hold
+    the rows request by request, -1 behind the last.
+
+    ``out``: buffers to write into (``advance_batch_buffers``); its
+    ``context_lens`` and ``free_span`` may be the inputs, which are then
+    advanced in place. Calls on one batch must not overlap.
+    """
+    fn = "advance_batch"
+    _require(isinstance(new_tokens, torch.Tensor) and new_tokens.is_cuda,
+             "advance_batch: new_tokens must be a CUDA tensor")
+    dev = new_tokens.device
+    _device_tensors(fn, dev, (context_lens, "context_lens"), (block_tables, "block_tables"),
+                    (free_pages, "free_pages"), (free_span, "free_span"))
+    _require(new_tokens.dim() == 1 and block_tables.dim() == 2 and free_pages.dim() == 1,
+             "advance_batch: new_tokens and free_pages must be 1-D, block_tables 2-D")
+    B, M, C = new_tokens.shape[0], block_tables.shape[1], free_pages.shape[0]
+    _int32(fn, new_tokens, "new_tokens", (B,))
+    _int32(fn, context_lens, "context_lens", (B,))
+    _int32(fn, block_tables, "block_tables", (B, M))
+    _int32(fn, free_pages, "free_pages", (C,))
+    _int32(fn, free_span, "free_span", (2,))
+    if out is None:
+        _require(num_rows is not None, "advance_batch: num_rows or out must be given")
+        out = advance_batch_buffers(B, num_rows, dev)
+    rows = out.slots.shape[0]
+    _require(num_rows is None or num_rows == rows, "advance_batch: num_rows differs from out's rows")
+    _device_tensors(fn, dev, *zip(out, BatchStep._fields))
+    for t, n, k in zip(out, BatchStep._fields, (B, 2, B + 1, rows, rows, B)):
+        _int32(fn, t, n, (k,))
+    with _on(dev):
+        _check(_c_advance(new_tokens.data_ptr(), context_lens.data_ptr(), B, block_tables.data_ptr(), M,
+                          free_pages.data_ptr(), C, free_span.data_ptr(), int(block_size), rows,
+                          out.context_lens.data_ptr(), out.free_span.data_ptr(), out.cu_seqlens.data_ptr(),
+                          out.slots.data_ptr(), out.positions.data_ptr(), out.status.data_ptr(), _stream(new_tokens)))
+    return out
