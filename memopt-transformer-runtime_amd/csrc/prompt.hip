@@ -67,11 +67,14 @@ __device__ __forceinline__ float both_halves_max(float v) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// Sum of a wave's lanes, in every lane.
+// Sum of a wave's lanes, wave-uniform (lane exchanges in registers).
 __device__ __forceinline__ int32_t wave_sum(int32_t v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  return __builtin_amdgcn_readfirstlane(v);
+  v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, true);   // quad_perm: lane ^ 1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, true);   // quad_perm: lane ^ 2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, true);  // row_half_mirror
+  v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, true);  // row_mirror
+  return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) + __builtin_amdgcn_readlane(v, 32) +
+         __builtin_amdgcn_readlane(v, 48);
 }
 
 // The query tile (R rows of one sequence) that comes rank-th when the tiles of
@@ -87,6 +90,11 @@ struct Tile {
 template <int R>
 __device__ __forceinline__ bool find_tile(const int32_t *cu, int32_t B, int32_t T, int32_t rank, Tile &out) {
   const int lane = threadIdx.x & 63;
+  if (B == 1) {
+    const int32_t lo = min(max(cu[0], 0), T), n = (min(max(cu[1], lo), T) - lo + R - 1) / R;
+    out = {0, n - 1 - rank};
+    return rank < n;
+  }
   auto tiles_of = [&](int32_t b) {
     if (b >= B) return 0;
     const int32_t lo = min(max(cu[b], 0), T), hi = min(max(cu[b + 1], lo), T);
@@ -154,25 +162,26 @@ __device__ __forceinline__ u32x2p_t v_read(const uint8_t *tile, uint32_t off) {
   return __builtin_bit_cast(u32x2p_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t *)(tile + off)));
 }
 
-// Zeroes the elements of four operands that are inf or NaN; whether any lane had one.
+// A pair of elements with inf and NaN replaced by the largest finite value of
+// their sign; `odd` collects a nonzero bit wherever that changed one.
 template <class E>
-__device__ __forceinline__ bool drop_odd(u32x4p_t (&v)[4]) {
-  constexpr uint32_t m = E::kExponent * 0x10001u, step = 0x80008000u - m;  // a full exponent carries into bit 15
-  uint32_t any = 0;
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) any |= (v[c][i] & m) + step;
-  if (!__any((any & 0x80008000u) != 0)) return false;
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t f = (v[c][i] & m) + step;
-      v[c][i] &= ((f & 0x8000u) ? 0u : 0xFFFFu) | ((f & 0x80000000u) ? 0u : 0xFFFF0000u);
-    }
-  return true;
+__device__ __forceinline__ uint32_t tame(uint32_t w, uint32_t &odd) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  constexpr unsigned short most = (unsigned short)(E::kExponent - 1);
+  const u16x2 m = __builtin_elementwise_min(__builtin_bit_cast(u16x2, w & 0x7FFF7FFFu), u16x2{most, most});
+  const uint32_t y = bfi(0x7FFF7FFFu, __builtin_bit_cast(uint32_t, m), w);
+  odd |= y ^ w;
+  return y;
 }
+
+template <int N>
+struct IntConst {
+  static constexpr int value = N;
+};
+
+// `n` instructions of class `mask` here in the schedule (0x002 VALU, 0x008
+// MFMA, 0x100 LDS read, 0x400 transcendental).
+#define SCHED(mask, n) __builtin_amdgcn_sched_group_barrier(mask, n, 0)
 
 template <class E, int D, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p) {
@@ -180,7 +189,8 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
   constexpr int RB = 2 * D, CPR = RB / 16;         // bytes and 16-byte pieces of an LDS row
   constexpr int NCH = D / 16, NDB = D / 32;
   constexpr int RPC = 1024 / RB, NC = TK / RPC / NW;  // rows per copy; copies per wave of K (and of V)
-  __shared__ __attribute__((aligned(16))) uint8_t lds_k[2][TK * RB], lds_v[2][TK * RB];
+  __shared__ __attribute__((aligned(16))) uint8_t lds_k0[TK * RB], lds_k1[TK * RB], lds_v0[TK * RB],
+      lds_v1[TK * RB];
 
   const int lane = threadIdx.x & 63, n = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -232,8 +242,8 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
   const uint8_t *k_base = reinterpret_cast<const uint8_t *>(p.k + (int64_t)s0 * p.k_ts + kvh * p.k_hs);
   const uint8_t *v_base = reinterpret_cast<const uint8_t *>(p.v + (int64_t)s0 * p.v_ts + kvh * p.v_hs);
   const uint32_t wave_lds = (uint32_t)wave * NC * 1024;
-  const uint32_t mk[2] = {lds_u32(lds_k[0]) + wave_lds, lds_u32(lds_k[1]) + wave_lds};
-  const uint32_t mv[2] = {lds_u32(lds_v[0]) + wave_lds, lds_u32(lds_v[1]) + wave_lds};
+  const uint32_t mk[2] = {lds_u32(lds_k0) + wave_lds, lds_u32(lds_k1) + wave_lds};
+  const uint32_t mv[2] = {lds_u32(lds_v0) + wave_lds, lds_u32(lds_v1) + wave_lds};
   // A tile's rows through a descriptor of their own: 64-bit bases, and rows
   // past the sequence lie outside its range and read as zeros.
   auto rows_at = [&](const uint8_t *base, uint32_t rb, int32_t key0) __attribute__((always_inline)) {
@@ -241,10 +251,11 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
     return __builtin_amdgcn_make_buffer_rsrc((void *)(base + (int64_t)key0 * rb), (short)0,
                                              (int)((rows - 1) * rb + RB), 0x00020000);
   };
-  auto load_tile = [&](int32_t it, int buf) __attribute__((always_inline)) {
-    const int32_t key0 = tile_base(it);
-    lds_dma_range<0, NC>(rows_at(k_base, k_rb, key0), mk[buf], k_off, 0);
-    lds_dma_range<0, NC>(rows_at(v_base, v_rb, key0), mv[buf], v_off, 0);
+  auto load_k = [&](int32_t it, int buf) __attribute__((always_inline)) {
+    lds_dma_range<0, NC>(rows_at(k_base, k_rb, tile_base(it)), mk[buf], k_off, 0);
+  };
+  auto load_v = [&](int32_t it, int buf) __attribute__((always_inline)) {
+    lds_dma_range<0, NC>(rows_at(v_base, v_rb, tile_base(it)), mv[buf], v_off, 0);
   };
 
   uint32_t ka[NCH], va[NDB];
@@ -263,118 +274,294 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
   // probabilities lie in (0, 2^15] and fp16 holds those down to 2^-21 of the
   // largest as normal numbers.
   constexpr float kTop = 7.0f;
-  float ncm = 0.0f, thr = -INFINITY, lsum = 0.0f;
-  const int32_t w_last = min(qw0 + 31, len - 1);  // the wave's last row
+  float ncm = 0.0f, thr = -INFINITY, lsum = 0.0f, lsum1 = 0.0f;
 
-  if (n_tiles > 0) load_tile(0, 0);
-  for (int32_t it = 0; it < n_tiles; ++it) {
-    const int P = it & 1;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();  // tile it is in LDS; every wave has read tile it - 1
-    if (it + 1 < n_tiles) load_tile(it + 1, P ^ 1);
-    const int32_t tb = tile_base(it);
-    if (qw0 >= len || tb > w_last || (tb + TK <= qw0 - p.W + 1 && tb >= p.sinks)) continue;  // nothing to see
-    const bool full = tb + TK - 1 <= qw0 && (tb >= qw0 + 31 - p.W + 1 || tb + TK <= p.sinks);
+  // What this wave sees: the sink tiles and window iterations [v0, v1); of
+  // those, iterations [f0, f1) hold window tiles that all its rows see whole.
+  const bool any = qw0 < len;
+  const int32_t w_last = min(qw0 + 31, len - 1);
+  int32_t v0 = sink_tiles, v1 = sink_tiles, f0 = 0, f1 = 0;
+  if (any) {
+    const int32_t off = sink_tiles - t_first;  // iteration of tile t: t + off
+    v0 = max(sink_tiles, max(0, qw0 - p.W + 1) / TK + off);
+    v1 = max(v0, w_last / TK + 1 + off);
+    f0 = max(sink_tiles, (max(0, qw0 + 31 - p.W + 1) + TK - 1) / TK + off);
+    f1 = max(f0, (qw0 + 1) / TK + off);
+  }
+  auto sees = [&](int32_t it) { return it < sink_tiles ? any : it >= v0 && it < v1; };
 
-    f32x16_t s[2];
-#pragma unroll
-    for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-      for (int c = 0; c < NCH; ++c) {
-        const u32x4p_t a = *reinterpret_cast<const u32x4p_t *>(&lds_k[P][32 * blk * RB + ka[c]]);
-        s[blk] = E::mfma(a, qf[c], c == 0 ? (f32x16_t){} : s[blk]);
-      }
-    // Register r of block blk holds key tb + 32 blk + 8 (r / 4) + 4 hl + r % 4.
-#pragma unroll
-    for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[blk][r] = fmaf(s[blk][r], p.qk_scale_log2, ncm);
+  // Register r of block blk holds key tb + 32 blk + 8 (r / 4) + 4 hl + r % 4.
+  auto apply_mask = [&](f32x16_t (&s)[2], int32_t tb) __attribute__((always_inline)) {
     const int32_t key0 = tb + 4 * hl;
-    if (!full) {
-      const int32_t last = q_ok ? qi - key0 : -1, first = qi - p.W + 1 - key0, sink = p.sinks - key0;
+    const int32_t last = q_ok ? qi - key0 : -1, first = qi - p.W + 1 - key0, sink = p.sinks - key0;
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk)
+    for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int32_t c = 32 * blk + 8 * (r >> 2) + (r & 3);
-          s[blk][r] = (c <= last) & ((c >= first) | (c < sink)) ? s[blk][r] : -INFINITY;
-        }
-    }
+      for (int r = 0; r < 16; ++r) {
+        const int32_t c = 32 * blk + 8 * (r >> 2) + (r & 3);
+        s[blk][r] = (c <= last) & ((c >= first) | (c < sink)) ? s[blk][r] : -INFINITY;
+      }
+  };
+  auto row_max = [&](const f32x16_t (&s)[2]) __attribute__((always_inline)) {
     float t = s[0][0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) t = fmaxf(t, s[0][r]);
 #pragma unroll
     for (int r = 0; r < 16; ++r) t = fmaxf(t, s[1][r]);
-    t = both_halves_max(t);
+    return both_halves_max(t);
+  };
+  auto to_x = [&](f32x16_t &s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], p.qk_scale_log2, ncm);
+  };
+  auto raise_max = [&](float t, f32x16_t (&s)[2]) __attribute__((always_inline)) {
     if (__any(t > thr)) {
       const bool start = thr == -INFINITY, found = t > -INFINITY;
       const float shift = start ? (found ? t - kTop : 0.0f) : fmaxf(t - kTop, 0.0f);
       const float alpha = start ? (found ? 0.0f : 1.0f) : (shift > 0.0f ? fast_exp2(-shift) : 1.0f);
       lsum *= alpha;
+      lsum1 *= alpha;
 #pragma unroll
-      for (int db = 0; db < NDB; ++db) o[db] *= alpha;
+      for (int db = 0; db < NDB; ++db)
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk) s[blk] -= shift;
+        for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[blk][r] -= shift;
       ncm -= shift;
       thr = (start && !found) ? thr : kTop + 8.0f;
     }
-    u32x4p_t pf[4];
+  };
+  // Probabilities of one block, which two register quads each make an operand
+  // of the second product as they are; their sum, from the rounded pairs.
+  auto probs = [&](f32x16_t &s, u32x4p_t (&pb)[2], float &sum) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 8 * (c & 1) + 2 * i;
-        s[c >> 1][r] = fast_exp2(s[c >> 1][r]);
-        s[c >> 1][r + 1] = fast_exp2(s[c >> 1][r + 1]);
-        pf[c][i] = E::pack(s[c >> 1][r], s[c >> 1][r + 1]);
-        lsum = E::add2(pf[c][i], lsum);
-      }
-    // Probabilities of 16 keys (two register quads) are the second product's
-    // operand as they are; V^T comes transposed from LDS in the same order.
-    bool odd = false;
-#pragma unroll
-    for (int db = 0; db < NDB; ++db) {
-      u32x4p_t vf[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const u32x2p_t lo = v_read(lds_v[P], va[db] + 16 * c * RB), hi8 = v_read(lds_v[P], va[db] + (16 * c + 8) * RB);
-        vf[c] = u32x4p_t{lo[0], lo[1], hi8[0], hi8[1]};
-      }
-      if (!full) odd |= drop_odd<E>(vf);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) o[db] = E::mfma(vf[c], pf[c], o[db]);
+    for (int i = 0; i < 8; ++i) {
+      s[2 * i] = fast_exp2(s[2 * i]);
+      s[2 * i + 1] = fast_exp2(s[2 * i + 1]);
+      pb[i >> 2][i & 3] = E::pack(s[2 * i], s[2 * i + 1]);
     }
-    if (!full && odd) {  // wave-uniform
-      // Elements of V that are inf or NaN were left out above, as they must not
-      // meet the weight 0 of a row that does not see them; each is added here
-      // to the rows that do.
-      const int32_t last = q_ok ? qi - tb : -1, first = qi - p.W + 1 - tb, sink = p.sinks - tb;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum = E::add2(pb[i >> 2][i & 3], sum);
+  };
+  // Operands: K piece c of a 32-key block; V of 16 keys (half i % 2 of a
+  // 32-key block) and dims 32 (i / 2) .. + 31, transposed from four-row reads.
+  auto kfrag = [&](const uint8_t *kt, int blk, int c) __attribute__((always_inline)) {
+    return *reinterpret_cast<const u32x4p_t *>(kt + 32 * blk * RB + ka[c]);
+  };
+  auto vfrag = [&](const uint8_t *vt, int blk, int i) __attribute__((always_inline)) {
+    const uint8_t *src = vt + (32 * blk + 16 * (i & 1)) * RB;
+    const u32x2p_t a = v_read(src, va[i >> 1]), b8 = v_read(src + 8 * RB, va[i >> 1]);
+    return u32x4p_t{a[0], a[1], b8[0], b8[1]};
+  };
+  auto qk_block = [&](const uint8_t *kt, int blk, f32x16_t &acc, auto prec, const u32x4p_t (&pre)[4])
+                      __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < NCH; ++c)
+      acc = E::mfma((decltype(prec)::value && c < 4) ? pre[c] : kfrag(kt, blk, c), qf[c], c == 0 ? (f32x16_t){} : acc);
+  };
+  auto pv_block = [&](const uint8_t *vt, int blk, const u32x4p_t (&pb)[2], const u32x4p_t (&pre)[4])
+                      __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2 * NDB; ++i)
+      o[i >> 1] = E::mfma(i < 4 ? pre[i] : vfrag(vt, blk, i), pb[i & 1], o[i >> 1]);
+  };
+  // End of an iteration: this wave's copies have arrived and its reads are
+  // done; the barrier says so for all waves.
+  auto publish = [&]() __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+
+  // Iteration `it` of parity P takes the exp2 arguments x(it) in sc and leaves
+  // x(it + 1) in sn. K(it + 1) is read from buffer P ^ 1 while K(it + 2) is
+  // copied into buffer P; V(it) is read from buffer P while V(it + 1) is
+  // copied into buffer P ^ 1.
+  // Pipelined form, for tiles seen whole: four segments of matrix
+  // instructions, each with vector work of another tile or block beside it,
+  // operands read ahead (a segment's first four under the segment before).
+  auto iter_full = [&](int32_t it, f32x16_t (&sc)[2], f32x16_t (&sn)[2], auto pc) __attribute__((always_inline)) {
+    constexpr int P = decltype(pc)::value;
+    const uint8_t *const kt = P ? lds_k0 : lds_k1, *const vt = P ? lds_v1 : lds_v0;
+    const u32x4p_t none[4] = {};
+    u32x4p_t pre_k[4], pre_a[4], pre_b[4], pa[2], pb[2];
+    if (it + 2 < n_tiles) load_k(it + 2, P);
+    __builtin_amdgcn_s_setprio(1);
+    // QK(it + 1) block 0 | maximum of x(it)
+    qk_block(kt, 0, sn[0], IntConst<0>{}, none);
+    const float t = row_max(sc);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) pre_k[c] = kfrag(kt, 1, c);
+    SCHED(0x100, 4);
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      SCHED(0x008, 1);
+      SCHED(0x100, 1);
+      SCHED(0x002, 2);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    raise_max(t, sc);
+    // QK(it + 1) block 1 | probabilities of block 0
+    qk_block(kt, 1, sn[1], IntConst<1>{}, pre_k);
+    probs(sc[0], pa, lsum);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pre_a[i] = vfrag(vt, 0, i);
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      SCHED(0x008, 1);
+      if (NCH == 8 && c < 4) SCHED(0x100, 1);
+      else SCHED(0x100, 2);
+      SCHED(0x002, 16 / NCH);
+      SCHED(0x400, 16 / NCH);
+    }
+    asm volatile("" ::"v"(pa[0]), "v"(pa[1]));  // (keeps the exp2s in this segment)
+    __builtin_amdgcn_sched_barrier(0);
+    if (it + 1 < n_tiles) load_v(it + 1, P ^ 1);
+    // PV(it) block 0 | probabilities of block 1
+    pv_block(vt, 0, pa, pre_a);
+    probs(sc[1], pb, lsum1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pre_b[i] = vfrag(vt, 1, i);
+#pragma unroll
+    for (int c = 0; c < 2 * NDB; ++c) {
+      SCHED(0x008, 1);
+      SCHED(0x100, 2);
+      SCHED(0x002, 16 / (2 * NDB));
+      SCHED(0x400, 16 / (2 * NDB));
+    }
+    asm volatile("" ::"v"(pb[0]), "v"(pb[1]));
+    __builtin_amdgcn_sched_barrier(0);
+    // PV(it) block 1 | x(it + 1)
+    pv_block(vt, 1, pb, pre_b);
+    to_x(sn[0]);
+    to_x(sn[1]);
+#pragma unroll
+    for (int c = 0; c < 2 * NDB; ++c) {
+      SCHED(0x008, 1);
+      if (c < 2 * NDB - 4) SCHED(0x100, 2);
+      SCHED(0x002, 32 / (2 * NDB));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
+    publish();
+  };
+  // Plain form, for tiles that are masked, not seen, or followed by one that
+  // is not.
+  uint32_t odd = 0;  // nonzero where a masked tile's V held inf or NaN
+  auto iter_edge = [&](int32_t it, f32x16_t (&sc)[2], f32x16_t (&sn)[2], auto pc) __attribute__((always_inline)) {
+    constexpr int P = decltype(pc)::value;
+    const uint8_t *const kt = P ? lds_k0 : lds_k1, *const vt = P ? lds_v1 : lds_v0;
+    const u32x4p_t none[4] = {};
+    if (it + 2 < n_tiles) load_k(it + 2, P);
+    if (it + 1 < n_tiles) load_v(it + 1, P ^ 1);
+    if (sees(it)) {
+      const int32_t tb = tile_base(it);
+      const bool full = it >= f0 && it < f1;
+      if (!full) apply_mask(sc, tb);
+      raise_max(row_max(sc), sc);
+      u32x4p_t pf[2][2];
+      probs(sc[0], pf[0], lsum);
+      probs(sc[1], pf[1], lsum1);
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) {
+        u32x4p_t vf[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) vf[c] = vfrag(vt, c >> 1, 2 * db + (c & 1));
+        if (!full) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vf[c][i] = tame<E>(vf[c][i], odd);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[db] = E::mfma(vf[c], pf[c >> 1][c & 1], o[db]);
+      }
+    }
+    if (it + 1 < n_tiles && sees(it + 1)) {
+      qk_block(kt, 0, sn[0], IntConst<0>{}, none);
+      qk_block(kt, 1, sn[1], IntConst<0>{}, none);
+      to_x(sn[0]);
+      to_x(sn[1]);
+    } else {
+      sn[0] = (f32x16_t){};
+      sn[1] = (f32x16_t){};
+    }
+    publish();
+  };
+
+  f32x16_t sx[2], sy[2];
+  if (n_tiles > 0) {
+    load_k(0, 0);
+    load_v(0, 0);
+    if (n_tiles > 1) load_k(1, 1);
+    publish();
+    const u32x4p_t none[4] = {};
+    if (sees(0)) {
+      qk_block(lds_k0, 0, sx[0], IntConst<0>{}, none);
+      qk_block(lds_k0, 1, sx[1], IntConst<0>{}, none);
+      to_x(sx[0]);
+      to_x(sx[1]);
+    } else {
+      sx[0] = (f32x16_t){};
+      sx[1] = (f32x16_t){};
+    }
+    __syncthreads();  // K(0)'s buffer is refilled by the first iteration
+  }
+  // Iterations [m0, m1) are pipelined: this tile seen whole, the next seen.
+  // Two iterations per trip keep buffers and score registers constant. (One
+  // loop for the plain iterations before and behind, with the buffer as a
+  // variable, spilled operand addresses into the pipelined loop: twice as long.)
+  const int32_t m0 = min(n_tiles, f0 + (f0 & 1)), m1 = max(m0, min(f1, v1 - 1));
+  int32_t it = 0;
+  for (; it < m0; it += 2) {
+    iter_edge(it, sx, sy, IntConst<0>{});
+    if (it + 1 >= m0) {
+      ++it;
+      break;
+    }
+    iter_edge(it + 1, sy, sx, IntConst<1>{});
+  }
+  for (; it < m1; it += 2) {
+    iter_full(it, sx, sy, IntConst<0>{});
+    if (it + 1 >= m1) {
+      ++it;
+      break;
+    }
+    iter_full(it + 1, sy, sx, IntConst<1>{});
+  }
+  if (it < n_tiles && (it & 1)) {
+    iter_edge(it, sy, sx, IntConst<1>{});
+    ++it;
+  }
+  for (; it < n_tiles; it += 2) {
+    iter_edge(it, sx, sy, IntConst<0>{});
+    if (it + 1 >= n_tiles) break;
+    iter_edge(it + 1, sy, sx, IntConst<1>{});
+  }
+
+  if (__any(odd != 0)) {
+    // inf and NaN in V entered the masked tiles as finite values, since the
+    // weight 0 of a row that does not see them would make NaN of them. Rows
+    // that do see one have inf or NaN in that column whatever its weight.
 #pragma unroll 1
-      for (int key = 0; key < TK; ++key) {
-        const int reg = 16 * (key >> 5) + 4 * ((key >> 3) & 3) + (key & 3);
-        float pk = 0.0f;
+    for (int32_t i = 0; i < n_tiles; ++i) {
+      if (!sees(i) || (i >= f0 && i < f1)) continue;
+      const int32_t tb = tile_base(i);
+#pragma unroll 1
+      for (int32_t key = tb; key < min(tb + TK, len); ++key) {
+        const uint16_t *row = reinterpret_cast<const uint16_t *>(v_base + (int64_t)key * v_rb) + 4 * hl;
+        const bool see = q_ok && key <= qi && (key < p.sinks || key > qi - p.W);
 #pragma unroll
-        for (int x = 0; x < 32; ++x) pk = x == reg ? s[x >> 4][x & 15] : pk;
-        pk = __shfl(pk, n + 32 * ((key >> 2) & 1), 64);
-        const bool see = (key <= last) & ((key >= first) | (key < sink));
-#pragma unroll
-        for (int db = 0; db < NDB; ++db)
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const uint8_t *src = &lds_v[P][key * RB + 16 * ((4 * db + g) ^ v_swz(key)) + 8 * hl];
-            const u32x2p_t w = *reinterpret_cast<const u32x2p_t *>(src);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint16_t bits = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-              if (see && (bits & E::kExponent) == E::kExponent)
-                o[db][4 * g + e] = fmaf(pk, E::value(bits), o[db][4 * g + e]);
-            }
-          }
+        for (int r = 0; r < 16 * NDB; ++r) {
+          const uint16_t bits = row[8 * (r >> 2) + (r & 3)];
+          if (see && (bits & E::kExponent) == E::kExponent) o[r >> 4][r & 15] += E::value(bits);
+        }
       }
     }
   }
 
-  const float l = xor32_sum(lsum);
+  const float l = xor32_sum(lsum + lsum1);
   if (!q_ok) return;
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
   uint16_t *dst = p.out + (int64_t)(s0 + qi) * p.o_ts + h * p.o_hs + 4 * hl;
