@@ -361,7 +361,10 @@ typedef struct memopt_packed_desc {
   void *workspace;                   /* >= memopt_packed_workspace_size bytes, 16-byte aligned */
   int64_t workspace_bytes;
 } memopt_packed_desc;
-int memopt_packed_workspace_size(const memopt_packed_desc *desc, int64_t *bytes);
+/* The workspace's first `zeroed` bytes (arrival counters) must be zero before
+ * its first use; every call leaves them zero. The rest may hold anything.
+ * Calls sharing a workspace must not overlap. */
+int memopt_packed_workspace_size(const memopt_packed_desc *desc, int64_t *bytes, int64_t *zeroed);
 int memopt_packed_attention(const memopt_packed_desc *desc, void *stream);
 
 /* The index tensors of a batch's next step, built on the device. Request b

@@ -14,9 +14,13 @@
 // block of 16 rows fills a matrix instruction that a lone query head would
 // leave 15/16 empty. Every cached byte is read once per block of rows.
 //
-// Work: a workgroup of 4 waves owns QN = 16 * QB rows of one (sequence, key
-// head) and one split of its visible 16-token chunks; a wave takes two chunks
-// (32 tokens) per step. Layout, as in direct.hip:
+// Work: QN = 16 * QB rows of one (sequence, key head) are a block; a wave takes
+// two 16-token chunks (32 tokens) of a block's visible ones per step. The steps
+// of all blocks of a key head form one list, which is dealt to its workgroups
+// of 4 waves in equal runs, whatever the sequences' lengths (by sequence and
+// split, a batch of 2700 to 8192 tokens ran as long as its longest part). A
+// block whose steps fall to one workgroup is finished there; else each
+// leaves partial sums, and the last to arrive adds them up. Layout, as in direct.hip:
 //  * S^T = K Q^T on v_mfma_f32_16x16x32_f16, one product per token half t: row
 //    r of the A operand is token r % 8 + 8 t of chunk r / 8, which is how a
 //    page interleaves its tokens. Over pages each product covers dims of one
@@ -52,56 +56,64 @@ struct PackedParams {
   int64_t kv_ps, kv_hs, kv_ts;   // bytes
   int32_t W, sinks;
   float qk_scale_log2;
-  int32_t one_block;             // every sequence has at most one block of rows
-  int32_t items, splits;
-  float *ws_o, *ws_ml;           // [items * Hk][splits][QN][D], [items * Hk][splits][QN][2]
+  int32_t wgs, blocks;           // workgroups per key head; blocks that ws_cnt has counters for
+  uint32_t *ws_cnt;              // [blocks * Hk] arrivals; zero between calls
+  float *ws_o, *ws_ml;           // [2 * wgs * Hk][QN][D], [2 * wgs * Hk][QN][2]: see partial_slot
 };
 
-// A block of rows: sequence b, rows [row0, row0 + QN) of its `rows`.
-struct RowBlock {
-  int32_t b, row0, rows, start, n, ctx;  // start, n: the sequence's first query row and their number
-};
+// Workgroups per key head, so partial sums of a block, at most: their weights
+// take the place of the waves' sums in LDS.
+static constexpr int max_workgroups(int D) { return 4 * D; }
 
+// Inclusive prefix sum over the wave (DPP row shifts, then row broadcasts),
+// saturating: query starts that do not ascend can count rows more than once.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t scan_step(uint32_t v) {
+  return __builtin_elementwise_add_sat(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, ROWS == 0xF));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v = scan_step<0x111, 0xF>(v);
+  v = scan_step<0x112, 0xF>(v);
+  v = scan_step<0x114, 0xF>(v);
+  v = scan_step<0x118, 0xF>(v);
+  v = scan_step<0x142, 0xA>(v);
+  return scan_step<0x143, 0xC>(v);
+}
+
+// What rows at positions pos_lo .. pos_hi of a context see, in 16-token
+// chunks: the sinks [0, sc), then the window [wc0, wc0 + n - sc).
+struct Visible {
+  int32_t sc, wc0, n;
+};
+__device__ __forceinline__ Visible visible_chunks(const PackedParams &p, int32_t kv_lim, int32_t pos_lo,
+                                                  int32_t pos_hi) {
+  const int32_t hi = max(0, min(kv_lim, pos_hi + 1));
+  Visible v;
+  v.sc = (min(p.sinks, hi) + 15) >> 4;
+  v.wc0 = max(max(0, pos_lo - p.W + 1) >> 4, v.sc);
+  v.n = v.sc + max(0, ((hi + 15) >> 4) - v.wc0);
+  return v;
+}
+
+// A sequence's rows and, in the list of steps, its blocks: each takes `steps`
+// places, as many as its widest block can need (at least one, so that rows
+// which see nothing are written, too).
+struct Seq {
+  int32_t start, n, ctx, kv_lim, blocks, steps;
+};
 template <int QN>
-__device__ __forceinline__ bool find_block(const PackedParams &p, int32_t item, RowBlock &out) {
-  const int lane = threadIdx.x & 63;
-  auto first_row = [&](int32_t b) { return min(max(p.cu[b], 0), p.T); };
-  int32_t b = item, block = 0;
-  if (!p.one_block) {
-    int32_t before = 0;
-    bool found = false;
-    for (int32_t b0 = 0; b0 < p.B && !found; b0 += 64) {
-      const int32_t i = b0 + lane;
-      int32_t c = 0;
-      if (i < p.B) {
-        const int32_t lo = first_row(i), hi = max(lo, first_row(i + 1));
-        c = (int32_t)(((int64_t)(hi - lo) * p.G + QN - 1) / QN);
-      }
-      int32_t incl = c;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const int32_t u = __shfl_up(incl, off, 64);
-        if (lane >= off) incl += u;
-      }
-      const int32_t total = __builtin_amdgcn_readlane(incl, 63);
-      if (item < before + total) {
-        const int src = __builtin_ctzll(__ballot(item < before + incl));
-        b = b0 + src;
-        block = item - before - (__builtin_amdgcn_readlane(incl, src) - __builtin_amdgcn_readlane(c, src));
-        found = true;
-      }
-      before += total;
-    }
-    if (!found) return false;
-  }
-  b = __builtin_amdgcn_readfirstlane(b);
-  out.b = b;
-  out.start = first_row(b);
-  out.n = max(out.start, first_row(b + 1)) - out.start;
-  out.rows = out.n * p.G;
-  out.row0 = QN * __builtin_amdgcn_readfirstlane(block);
-  out.ctx = p.ctx[b];
-  return out.row0 < out.rows;
+__device__ __forceinline__ Seq sequence(const PackedParams &p, int32_t b) {
+  Seq q;
+  q.start = min(max(p.cu[b], 0), p.T);
+  q.n = min(max(p.cu[b + 1], q.start), p.T) - q.start;
+  q.ctx = p.ctx[b];
+  q.kv_lim = (int32_t)min((int64_t)q.ctx, (int64_t)p.M * p.bs);
+  q.blocks = (q.n * p.G + QN - 1) / QN;
+  const int32_t pos0 = q.ctx - q.n;
+  int32_t n = visible_chunks(p, q.kv_lim, pos0, q.ctx - 1).n;
+  if (q.blocks > 1) n = min(n, ((min(p.sinks, max(q.kv_lim, 0)) + 15) >> 4) + ((p.W + QN / p.G + 1) >> 4) + 2);
+  q.steps = max(1, (n + 1) >> 1);
+  return q;
 }
 
 // Raw registers of one step, by cache format.
@@ -129,34 +141,82 @@ struct PackedV<D, MEMOPT_KV_FP16> {
 };
 
 template <int D, int FMT, int QB>
-__global__ __launch_bounds__(256, QB == 1 && (FMT == MEMOPT_KV_INT4 || D == 64) ? 3 : 2) void packed_kernel(const PackedParams p) {
-  constexpr int NW = 4, KK = D / 32, ND = D / 16, QN = 16 * QB;
+__global__ __launch_bounds__(256, QB == 1 ? (FMT == MEMOPT_KV_INT4 || D == 64 ? 4 : 2) : 2) void packed_kernel(
+    const PackedParams p) {
+  constexpr int NW = 4, NT = 64 * NW, KK = D / 32, ND = D / 16, QN = 16 * QB;
   constexpr bool PAGES = FMT == MEMOPT_KV_INT4;
   constexpr int NG = PAGES ? D / 64 : 1;  // score sums per (row, token)
   constexpr int OS = D + 4;               // row stride of s_o: 16 rows of D floats would share a bank
   __shared__ __attribute__((aligned(16))) float s_o[NW][QN][OS];
   __shared__ float s_ml[NW][QN][2];
+  __shared__ int s_last;
+  static_assert(NW * OS >= max_workgroups(D), "the weights of a merge fit s_o");
 
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int32_t split = blockIdx.x % p.splits, unit = blockIdx.x / p.splits;
-  const int32_t kvh = unit % p.Hk, item = unit / p.Hk;
-  RowBlock rb;
-  if (!find_block<QN>(p, item, rb)) return;  // workgroup-uniform
-  const int32_t ctx = rb.ctx, kv_lim = (int32_t)min((int64_t)ctx, (int64_t)p.M * p.bs);
-  const int32_t last_row = min(rb.row0 + QN, rb.rows) - 1;
-  const int32_t pos0 = ctx - rb.n;  // position of the sequence's first query
-  const int32_t pos_lo = pos0 + rb.row0 / p.G, pos_hi = pos0 + last_row / p.G;
+  const int32_t kvh = blockIdx.x % p.Hk, wg = blockIdx.x / p.Hk;
 
-  // Visible chunks: sinks [0, sc), then the window [wc0, hc).
-  const int32_t hi = max(0, min(kv_lim, pos_hi + 1));
-  const int32_t win_lo = max(0, pos_lo - p.W + 1);
-  const int32_t hc = (hi + 15) >> 4;
-  const int32_t sc = (min(p.sinks, hi) + 15) >> 4;
-  const int32_t wc0 = max(win_lo >> 4, sc);
-  const int32_t n_vis = sc + max(0, hc - wc0);
-  const SplitRange sr = split_range((n_vis + 1) >> 1, split, p.splits);
-  const int32_t begin = sr.begin, end = sr.end;
+  // The list's length; then the sequence that holds this workgroup's first place.
+  uint32_t sum = 0;
+  for (int32_t b0 = 0; b0 < p.B; b0 += 64) {
+    uint32_t c = 0;
+    if (b0 + lane < p.B) {
+      const Seq q = sequence<QN>(p, b0 + lane);
+      c = (uint32_t)q.blocks * (uint32_t)q.steps;
+    }
+    sum = __builtin_elementwise_add_sat(sum, (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(c), 63));
+  }
+  // (past 2^31 only where sequences overlap: nothing is computed then)
+  const int32_t total = (int32_t)sum;
+  // Runs of one step per wave at least: shorter ones cost more to merge than they save.
+  const int32_t wgs = min(p.wgs, max(1, total / NW));
+  if (total <= 0 || wg >= wgs) return;
+  const int32_t run = total / wgs, longer = total - run * wgs;  // the first `longer` runs have one place more
+  int32_t at = wg * run + min(wg, longer);
+  const int32_t stop = at + run + (wg < longer ? 1 : 0);
+  auto wg_of = [&](int32_t x) {
+    const int32_t edge = longer * (run + 1);
+    return x < edge ? x / (run + 1) : longer + (x - edge) / run;
+  };
+  int32_t seq_at = 0, seq_blocks = 0, b = 0;  // places and blocks before sequence b
+  for (int32_t b0 = 0; b0 < p.B; b0 += 64) {
+    uint32_t c = 0, nb = 0;
+    if (b0 + lane < p.B) {
+      const Seq q = sequence<QN>(p, b0 + lane);
+      nb = q.blocks;
+      c = nb * (uint32_t)q.steps;
+    }
+    const int32_t incl = (int32_t)wave_scan(c), blocks = (int32_t)wave_scan(nb);
+    const int32_t sum64 = __builtin_amdgcn_readlane(incl, 63);
+    if (at < seq_at + sum64) {
+      const int src = __builtin_ctzll(__ballot(at < seq_at + incl));
+      b = b0 + src;
+      seq_at += __builtin_amdgcn_readlane(incl, src) - __builtin_amdgcn_readlane((int)c, src);
+      seq_blocks += __builtin_amdgcn_readlane(blocks, src) - __builtin_amdgcn_readlane((int)nb, src);
+      break;
+    }
+    seq_at += sum64;
+    seq_blocks += __builtin_amdgcn_readlane(blocks, 63);
+  }
+
+  // Block by block of this workgroup's run.
+  Seq seq = sequence<QN>(p, b);
+  while (at < stop) {
+  while (at >= seq_at + seq.blocks * seq.steps) {  // (sequences without rows take no place)
+    seq_at += seq.blocks * seq.steps;
+    seq_blocks += seq.blocks;
+    seq = sequence<QN>(p, ++b);
+  }
+  const int32_t block = (at - seq_at) / seq.steps;
+  if (seq_blocks + block >= p.blocks) return;  // sequences overlap: past the counters
+  const int32_t block_at = seq_at + block * seq.steps;
+  const int32_t row0 = block * QN, rows = seq.n * p.G, ctx = seq.ctx, kv_lim = seq.kv_lim;
+  const int32_t pos0 = ctx - seq.n;  // position of the sequence's first query
+  const int32_t pos_lo = pos0 + row0 / p.G, pos_hi = pos0 + (min(row0 + QN, rows) - 1) / p.G;
+  const Visible vis = visible_chunks(p, kv_lim, pos_lo, pos_hi);
+  const int32_t sc = vis.sc, wc0 = vis.wc0, n_vis = vis.n;
+  const int32_t begin = at - block_at, end = min(min(stop - block_at, seq.steps), (n_vis + 1) >> 1);
+  at = min(stop, block_at + seq.steps);
 
   // Q as the B operand: column r = row, k-group g; dims of product kk as the K
   // operand holds them (pages: 16 g + 8 (kk % 2) of scale group kk / 2, in
@@ -165,15 +225,15 @@ __global__ __launch_bounds__(256, QB == 1 && (FMT == MEMOPT_KV_INT4 || D == 64) 
   int32_t row_pos[QB];
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
-    const int32_t row = rb.row0 + 16 * qb + r, tok = row / p.G;
+    const int32_t row = row0 + 16 * qb + r, tok = row / p.G;
     row_pos[qb] = pos0 + tok;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       h8_t x = {};
-      if (row < rb.rows) {
+      if (row < rows) {
         const int d0 = PAGES ? 64 * (kk >> 1) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g;
         const h8_t y = __builtin_bit_cast(
-            h8_t, *reinterpret_cast<const u32x4_t *>(p.q + (int64_t)(rb.start + tok) * p.q_ts +
+            h8_t, *reinterpret_cast<const u32x4_t *>(p.q + (int64_t)(seq.start + tok) * p.q_ts +
                                                      (int64_t)(kvh * p.G + row - tok * p.G) * p.q_hs + d0));
         if (PAGES) {
           x[0] = y[0]; x[1] = y[4]; x[2] = y[1]; x[3] = y[5];
@@ -204,7 +264,7 @@ __global__ __launch_bounds__(256, QB == 1 && (FMT == MEMOPT_KV_INT4 || D == 64) 
     bool ok;
     int64_t kv;
   };
-  const int32_t *btrow = p.bt + (int64_t)rb.b * p.M;
+  const int32_t *btrow = p.bt + (int64_t)b * p.M;
   const int32_t cpp = PAGES ? 1 : p.bs >> 4;
   const int32_t nb32 = (int32_t)min(p.nb, (int64_t)INT32_MAX);
   struct Entry {  // a chunk's block-table entry, not yet waited for
@@ -537,10 +597,22 @@ __global__ __launch_bounds__(256, QB == 1 && (FMT == MEMOPT_KV_INT4 || D == 64) 
     }
   }
   __syncthreads();
-  for (int idx = tid; idx < QN * (D / 4); idx += NW * 64) {
+  // A block whose steps lie in one run is finished here.
+  const int32_t w0 = wg_of(block_at), w1 = wg_of(block_at + seq.steps - 1), live = min(QN, rows - row0);
+  auto write_row = [&](int row, int d, f32x4_t x, float l) __attribute__((always_inline)) {
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const int32_t rr = row0 + row, tok = rr / p.G;
+    *reinterpret_cast<u32x2_t *>(p.out + (int64_t)(seq.start + tok) * p.o_ts +
+                                 (int64_t)(kvh * p.G + rr - tok * p.G) * p.o_hs + d) =
+        u32x2_t{as_u32(half2_t{(half_t)(x[0] * inv), (half_t)(x[1] * inv)}),
+                as_u32(half2_t{(half_t)(x[2] * inv), (half_t)(x[3] * inv)})};
+  };
+  // A run holds at most two blocks in part: one that began before it (slot 0),
+  // one that begins in it and goes on behind it (slot 1).
+  auto partial_slot = [&](int32_t w) { return ((int64_t)w * 2 + (w == w0 ? 1 : 0)) * p.Hk + kvh; };
+  const int64_t mine = partial_slot(wg) * QN;
+  for (int idx = tid; idx < live * (D / 4); idx += NT) {
     const int row = idx / (D / 4), d = 4 * (idx % (D / 4));
-    const int32_t rr = rb.row0 + row;
-    if (rr >= rb.rows) break;  // rows grow with idx
     float mx = s_ml[0][row][0];
 #pragma unroll
     for (int w = 1; w < NW; ++w) mx = fmaxf(mx, s_ml[w][row][0]);
@@ -552,92 +624,119 @@ __global__ __launch_bounds__(256, QB == 1 && (FMT == MEMOPT_KV_INT4 || D == 64) 
       l += s_ml[w][row][1] * fw;
       x += *reinterpret_cast<const f32x4_t *>(&s_o[w][row][d]) * fw;
     }
-    if (p.splits == 1) {
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-      const int32_t tok = rr / p.G;
-      *reinterpret_cast<u32x2_t *>(p.out + (int64_t)(rb.start + tok) * p.o_ts +
-                                   (int64_t)(kvh * p.G + rr - tok * p.G) * p.o_hs + d) =
-          u32x2_t{as_u32(half2_t{(half_t)(x[0] * inv), (half_t)(x[1] * inv)}),
-                  as_u32(half2_t{(half_t)(x[2] * inv), (half_t)(x[3] * inv)})};
+    if (w0 == w1) {
+      write_row(row, d, x, l);
     } else {
-      const int64_t at = ((int64_t)unit * p.splits + split) * QN + row;
-      *reinterpret_cast<f32x4_t *>(p.ws_o + at * D + d) = x;
-      if (d == 0) {
-        p.ws_ml[2 * at] = mx;
-        p.ws_ml[2 * at + 1] = l;
+      // (agent scope: the other workgroups of the block may run on other XCDs)
+      uint64_t *dst = reinterpret_cast<uint64_t *>(p.ws_o + (mine + row) * D + d);
+      __hip_atomic_store(dst, __builtin_bit_cast(uint64_t, u32x2_t{__float_as_uint(x[0]), __float_as_uint(x[1])}),
+                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(dst + 1, __builtin_bit_cast(uint64_t, u32x2_t{__float_as_uint(x[2]), __float_as_uint(x[3])}),
+                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (d == 0)
+        __hip_atomic_store(reinterpret_cast<uint64_t *>(p.ws_ml + 2 * (mine + row)),
+                           __builtin_bit_cast(uint64_t, u32x2_t{__float_as_uint(mx), __float_as_uint(l)}),
+                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  if (w0 != w1) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's partial stores are complete
+    __syncthreads();
+    if (tid == 0) {
+      uint32_t *cnt = p.ws_cnt + (int64_t)(seq_blocks + block) * p.Hk + kvh;
+      const uint32_t n = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
+      s_last = n == (uint32_t)(w1 - w0 + 1);
+      if (s_last) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (s_last) {
+      // Weights of the partials, row by row (a wave per row), in s_o; the row's
+      // sum in s_ml. Then each thread adds four dims of a row over them.
+      auto load2 = [&](const float *src) __attribute__((always_inline)) {
+        const u32x2_t u = __builtin_bit_cast(
+            u32x2_t, __hip_atomic_load(reinterpret_cast<const uint64_t *>(src), __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT));
+        return float2{__uint_as_float(u[0]), __uint_as_float(u[1])};
+      };
+      const int32_t parts = w1 - w0 + 1;
+      float *wgt = &s_o[0][0][0];
+      constexpr int WS = NW * OS;  // weights of a row
+      for (int row = wave; row < live; row += NW) {
+        float mx = -INFINITY, l = 0.0f;
+        for (int32_t i = lane; i < parts; i += 64) {
+          const float2 ml = load2(p.ws_ml + 2 * (partial_slot(w0 + i) * QN + row));
+          wgt[row * WS + i] = ml.x;
+          mx = fmaxf(mx, ml.x);
+        }
+        mx = wave_max(mx);
+        for (int32_t i = lane; i < parts; i += 64) {
+          const float m = wgt[row * WS + i], f = m == -INFINITY ? 0.0f : fast_exp2(m - mx);
+          wgt[row * WS + i] = f;
+          l += f * load2(p.ws_ml + 2 * (partial_slot(w0 + i) * QN + row)).y;
+        }
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) l += shfl_xor(l, off);
+        if (lane == 0) s_ml[0][row][1] = l;
+      }
+      __syncthreads();
+      for (int idx = tid; idx < live * (D / 4); idx += NT) {
+        const int row = idx / (D / 4), d = 4 * (idx % (D / 4));
+        f32x4_t x = {};
+        for (int32_t i0 = 0; i0 < parts; i0 += 8) {
+          float2 y[8][2];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float *src = p.ws_o + (partial_slot(w0 + min(i0 + k, parts - 1)) * QN + row) * D + d;
+            y[k][0] = load2(src);
+            y[k][1] = load2(src + 2);
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float f = i0 + k < parts ? wgt[row * WS + i0 + k] : 0.0f;
+            x += f32x4_t{y[k][0].x, y[k][0].y, y[k][1].x, y[k][1].y} * f;
+          }
+        }
+        write_row(row, d, x, s_ml[0][row][1]);
       }
     }
   }
-}
-
-// Sums the splits of a unit's rows, one wave per row: lane s takes split s's
-// (m, l) (splits <= 64); every lane then adds D / 64 dims over the splits,
-// eight loads in flight.
-template <int D, int QN>
-__global__ __launch_bounds__(256) void packed_merge_kernel(const PackedParams p) {
-  constexpr int R = 8, E = D / 64;
-  typedef float vec_t __attribute__((ext_vector_type(E)));
-  const int lane = threadIdx.x & 63;
-  const int32_t unit = (int32_t)(blockIdx.x / (QN / 4));
-  const int row = 4 * (int)(blockIdx.x % (QN / 4)) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int32_t kvh = unit % p.Hk;
-  RowBlock rb;
-  if (!find_block<QN>(p, unit / p.Hk, rb) || rb.row0 + row >= rb.rows) return;
-  const int64_t at = (int64_t)unit * p.splits * QN + row;
-  const float *ml = p.ws_ml + 2 * (at + (int64_t)min(lane, p.splits - 1) * QN);
-  const float *src = p.ws_o + at * D + E * lane;
-  const float m = lane < p.splits ? ml[0] : -INFINITY, l = ml[1];
-  const float mx = wave_max(m);
-  const float wgt = m == -INFINITY ? 0.0f : fast_exp2(m - mx);
-  float lt = lane < p.splits ? l * wgt : 0.0f;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) lt += shfl_xor(lt, off);
-  vec_t o = {};
-  for (int s0 = 0; s0 < p.splits; s0 += R) {
-    vec_t x[R];
-#pragma unroll
-    for (int k = 0; k < R; ++k)
-      x[k] = *reinterpret_cast<const vec_t *>(src + (int64_t)min(s0 + k, p.splits - 1) * QN * D);
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wgt), min(s0 + k, 63)));
-      if (s0 + k < p.splits) o += x[k] * fs;
-    }
+  __syncthreads();  // s_o and s_ml are free for the next block
   }
-  const float inv = lt > 0.0f ? 1.0f / lt : 0.0f;
-  const int32_t rr = rb.row0 + row, tok = rr / p.G;
-  half_t *dst = p.out + (int64_t)(rb.start + tok) * p.o_ts + (int64_t)(kvh * p.G + rr - tok * p.G) * p.o_hs + E * lane;
-  if constexpr (E == 2) *reinterpret_cast<uint32_t *>(dst) = as_u32(half2_t{(half_t)(o[0] * inv), (half_t)(o[1] * inv)});
-  else *dst = (half_t)(o[0] * inv);
 }
 
 // Query rows per block: 16 where a sequence has no more than that.
 struct PackedPlan {
-  int32_t qn, one_block, splits;
-  int64_t items;
+  int32_t qn, wgs;
+  int64_t blocks;  // at most this many
 };
 
 static PackedPlan packed_plan(const memopt_packed_desc &d) {
   PackedPlan pl;
   const int64_t G = d.num_heads / d.num_kv_heads, most = (int64_t)std::min(d.max_query_len, d.tokens) * G;
   pl.qn = most <= 16 ? 16 : 32;
-  pl.one_block = most <= pl.qn;
-  // blocks: sum over sequences of ceil(rows / qn)
-  pl.items = pl.one_block ? d.batch : (d.tokens * G + (int64_t)(pl.qn - 1) * std::min(d.batch, d.tokens)) / pl.qn;
-  const int64_t units = pl.items * d.num_kv_heads;
-  // Splits: about two workgroups per CU, at least two steps (64 tokens) per
-  // wave of the longest context the call allows, at most 64.
-  const int64_t W = effective_window(d.window_size, d.max_seq_len);
-  int64_t tokens = W + pl.qn + std::max(0, d.num_sink_tokens) + 32;
-  tokens = std::min<int64_t>(tokens, (int64_t)d.max_blocks_per_seq * d.block_size);
-  int64_t s = (2LL * compute_units() + units - 1) / units;
-  s = std::min<int64_t>(std::min(s, tokens / (4 * 2 * 32)), 64);
-  pl.splits = (int32_t)(s < 2 ? 1 : s);
+  // sum over the sequences of ceil(rows / qn)
+  pl.blocks = (d.tokens * G + (int64_t)(pl.qn - 1) * std::min(d.batch, d.tokens)) / pl.qn;
+  const int64_t resident = pl.qn == 16 && (d.kv_format == MEMOPT_KV_INT4 || d.head_dim == 64) ? 3 : 2;
+  pl.wgs = (int32_t)std::max<int64_t>(1, std::min<int64_t>(resident * compute_units() / d.num_kv_heads,
+                                                           max_workgroups(d.head_dim)));
   return pl;
 }
 
-static int64_t packed_workspace(const memopt_packed_desc &d, const PackedPlan &pl) {
-  return pl.splits > 1 ? pl.items * d.num_kv_heads * pl.splits * pl.qn * (d.head_dim + 2) * 4 : 0;
+// Steps (32 tokens) that a block can need.
+static int64_t packed_steps(const memopt_packed_desc &d) {
+  return ((int64_t)d.max_blocks_per_seq * d.block_size + 31) / 32;
+}
+
+struct PackedWorkspace {
+  int64_t counters, ml, total;  // bytes of the counters, offset of the (m, l) pairs
+};
+static PackedWorkspace packed_workspace(const memopt_packed_desc &d, const PackedPlan &pl) {
+  PackedWorkspace w;
+  w.counters = (pl.blocks * d.num_kv_heads * 4 + 255) / 256 * 256;
+  const int64_t rows = 2LL * pl.wgs * d.num_kv_heads * pl.qn;
+  w.ml = w.counters + rows * d.head_dim * 4;
+  w.total = w.ml + rows * 8;
+  return w;
 }
 
 static int validate_packed(const memopt_packed_desc &d) {
@@ -665,7 +764,7 @@ static int validate_packed(const memopt_packed_desc &d) {
 
 template <int D, int FMT>
 static void launch_packed(const PackedParams &p, int qn, hipStream_t stream) {
-  const dim3 grid((unsigned)((int64_t)p.items * p.Hk * p.splits));
+  const dim3 grid((unsigned)((int64_t)p.wgs * p.Hk));
   if (qn == 16) hipLaunchKernelGGL((packed_kernel<D, FMT, 1>), grid, dim3(256), 0, stream, p);
   else hipLaunchKernelGGL((packed_kernel<D, FMT, 2>), grid, dim3(256), 0, stream, p);
 }
@@ -674,12 +773,14 @@ static void launch_packed(const PackedParams &p, int qn, hipStream_t stream) {
 
 using namespace memopt;
 
-extern "C" int memopt_packed_workspace_size(const memopt_packed_desc *desc, int64_t *bytes) {
-  MEMOPT_REQUIRE(desc && bytes, MEMOPT_ERR_INVALID, "packed_workspace_size: null pointer");
-  *bytes = 0;
+extern "C" int memopt_packed_workspace_size(const memopt_packed_desc *desc, int64_t *bytes, int64_t *zeroed) {
+  MEMOPT_REQUIRE(desc && bytes && zeroed, MEMOPT_ERR_INVALID, "packed_workspace_size: null pointer");
+  *bytes = *zeroed = 0;
   int rc = validate_packed(*desc);
   if (rc != MEMOPT_OK || desc->tokens == 0 || desc->batch == 0 || desc->max_query_len == 0) return rc;
-  *bytes = packed_workspace(*desc, packed_plan(*desc));
+  const PackedWorkspace w = packed_workspace(*desc, packed_plan(*desc));
+  *bytes = w.total;
+  *zeroed = w.counters;
   return MEMOPT_OK;
 }
 
@@ -692,12 +793,11 @@ extern "C" int memopt_packed_attention(const memopt_packed_desc *desc, void *str
                      d.block_tables && d.context_lens && d.query_starts,
                  MEMOPT_ERR_INVALID, "packed_attention: null pointer");
   const PackedPlan pl = packed_plan(d);
-  const int64_t need = packed_workspace(d, pl);
-  MEMOPT_REQUIRE(need == 0 || (d.workspace && d.workspace_bytes >= need), MEMOPT_ERR_INVALID,
-                 "packed_attention: workspace needs " + std::to_string(need) + " bytes");
-  MEMOPT_REQUIRE(pl.items * d.num_kv_heads * std::max<int64_t>(pl.splits, pl.qn / 4) < (1LL << 31) &&
-                     (int64_t)d.tokens * d.num_heads < (1LL << 31),
-                 MEMOPT_ERR_UNSUPPORTED, "packed_attention: too many rows");
+  const PackedWorkspace w = packed_workspace(d, pl);
+  MEMOPT_REQUIRE(d.workspace && d.workspace_bytes >= w.total, MEMOPT_ERR_INVALID,
+                 "packed_attention: workspace needs " + std::to_string(w.total) + " bytes");
+  MEMOPT_REQUIRE((int64_t)d.tokens * d.num_heads < (1LL << 31) && pl.blocks * packed_steps(d) < (1LL << 31),
+                 MEMOPT_ERR_UNSUPPORTED, "packed_attention: too many (row, page) pairs for one call");
   PackedParams p = {};
   p.q = (const half_t *)d.query;
   p.out = (half_t *)d.out;
@@ -729,13 +829,11 @@ extern "C" int memopt_packed_attention(const memopt_packed_desc *desc, void *str
   p.W = std::min(effective_window(d.window_size, d.max_seq_len), 1 << 30);  // (position - W stays in 32 bits)
   p.sinks = std::max(0, d.num_sink_tokens);
   p.qk_scale_log2 = 1.4426950408889634f / sqrtf((float)d.head_dim);
-  p.one_block = pl.one_block;
-  p.items = (int32_t)pl.items;
-  p.splits = pl.splits;
-  if (pl.splits > 1) {
-    p.ws_o = (float *)d.workspace;
-    p.ws_ml = p.ws_o + pl.items * d.num_kv_heads * pl.splits * pl.qn * d.head_dim;
-  }
+  p.wgs = pl.wgs;
+  p.blocks = (int32_t)pl.blocks;
+  p.ws_cnt = (uint32_t *)d.workspace;
+  p.ws_o = (float *)((uint8_t *)d.workspace + w.counters);
+  p.ws_ml = (float *)((uint8_t *)d.workspace + w.ml);
   hipStream_t s = (hipStream_t)stream;
   if (d.head_dim == 128) {
     if (d.kv_format == MEMOPT_KV_INT4) launch_packed<128, MEMOPT_KV_INT4>(p, pl.qn, s);
@@ -744,15 +842,5 @@ extern "C" int memopt_packed_attention(const memopt_packed_desc *desc, void *str
     if (d.kv_format == MEMOPT_KV_INT4) launch_packed<64, MEMOPT_KV_INT4>(p, pl.qn, s);
     else launch_packed<64, MEMOPT_KV_FP16>(p, pl.qn, s);
   }
-  rc = check_launch("packed_attention");
-  if (rc != MEMOPT_OK || pl.splits == 1) return rc;
-  const dim3 grid((unsigned)(pl.items * d.num_kv_heads * (pl.qn / 4)));
-  if (d.head_dim == 128) {
-    if (pl.qn == 16) hipLaunchKernelGGL((packed_merge_kernel<128, 16>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((packed_merge_kernel<128, 32>), grid, dim3(256), 0, s, p);
-  } else {
-    if (pl.qn == 16) hipLaunchKernelGGL((packed_merge_kernel<64, 16>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((packed_merge_kernel<64, 32>), grid, dim3(256), 0, s, p);
-  }
-  return check_launch("packed_attention(merge)");
+  return check_launch("packed_attention");
 }

@@ -90,6 +90,7 @@ struct Tile {
 template <int R>
 __device__ __forceinline__ bool find_tile(const int32_t *cu, int32_t B, int32_t T, int32_t rank, Tile &out) {
   const int lane = threadIdx.x & 63;
+  out = {0, 0};
   if (B == 1) {
     const int32_t lo = min(max(cu[0], 0), T), n = (min(max(cu[1], lo), T) - lo + R - 1) / R;
     out = {0, n - 1 - rank};

@@ -35,7 +35,7 @@ import contextlib
 import ctypes
 import os
 import threading
-from typing import List, NamedTuple, Optional, Sequence, Tuple
+from typing import List, Optional, Sequence, Tuple
 
 import torch  # must precede the HIP library so both share one HIP runtime
 
@@ -139,7 +139,8 @@ _c_ws = _sig("memopt_attention_workspace_size", [ctypes.POINTER(AttnDesc), ctype
 _c_attn = _sig("memopt_paged_attention", [ctypes.POINTER(AttnDesc), _vp])
 _c_attn_noalloc = _sig("memopt_paged_attention_noalloc", [ctypes.POINTER(AttnDesc), _vp])
 _c_prompt = _sig("memopt_prompt_attention", [ctypes.POINTER(PromptDesc), _vp])
-_c_packed_ws = _sig("memopt_packed_workspace_size", [ctypes.POINTER(PackedDesc), ctypes.POINTER(_i64)])
+_c_packed_ws = _sig("memopt_packed_workspace_size",
+                    [ctypes.POINTER(PackedDesc), ctypes.POINTER(_i64), ctypes.POINTER(_i64)])
 _c_packed = _sig("memopt_packed_attention", [ctypes.POINTER(PackedDesc), _vp])
 _c_advance = _sig("memopt_advance_batch",
                   [_vp, _vp, _i32, _vp, _i32, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp])
@@ -162,7 +163,7 @@ _SAME_DEVICE = contextlib.nullcontext()
 
 def _on(device: torch.device):
     """``torch.cuda.device(device)``, or nothing to enter where it is current already."""
-    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _SAME_DEVICE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def _require(cond: bool, msg: str) -> None:
@@ -775,8 +776,12 @@ class PreparedAttention:
 # counterparts in the reference)
 # ---------------------------------------------------------------------------
 
-def _device_tensors(fn: str, device: torch.device, *tensors) -> None:
-    for t, n in tensors:
+# (On the smallest calls the host side takes longer than the kernels, so the
+# checks below read each property of a tensor once and format messages only
+# when they raise.)
+def _device_tensors(fn: str, device: torch.device, **tensors) -> None:
+    """Raises for the first of ``tensors`` that is not a CUDA tensor on ``device``."""
+    for n, t in tensors.items():
         if not (isinstance(t, torch.Tensor) and t.is_cuda):
             raise RuntimeError(f"{fn}: {n} must be a CUDA tensor")
         if t.device != device:
@@ -784,7 +789,7 @@ def _device_tensors(fn: str, device: torch.device, *tensors) -> None:
 
 
 def _int32(fn: str, t: torch.Tensor, name: str, shape: Tuple[int, ...]) -> None:
-    if not (t.dtype == torch.int32 and tuple(t.shape) == shape and t.is_contiguous()):
+    if not (t.dtype is torch.int32 and t.shape == shape and t.is_contiguous()):
         raise RuntimeError(f"{fn}: {name} must be a contiguous int32 tensor of shape {list(shape)}")
 
 
@@ -793,23 +798,33 @@ def _no_grad(fn: str, *tensors: torch.Tensor) -> None:
         raise RuntimeError(f"{fn}: no gradients are computed; call it under torch.no_grad()")
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` itself where its last dimension is contiguous and its rows are
-    16-byte aligned (views of a fused projection are), else a contiguous copy."""
-    s = t.stride()
-    if s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0 and s[0] >= t.shape[2]:
-        return t
-    return t.contiguous()
+def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int, int, int]:
+    """(tensor, address, token stride, head stride) of ``t`` itself where its
+    last dimension is contiguous and its rows are 16-byte aligned (views of a
+    fused projection are), else of a contiguous copy."""
+    ts, hs, ds = t.stride()
+    p = t.data_ptr()
+    if ds == 1 and not (ts % 8 or hs % 8 or p % 16) and ts >= t.shape[2]:
+        return t, p, ts, hs
+    t = t.contiguous()
+    return t, t.data_ptr(), t.shape[1] * t.shape[2], t.shape[2]
 
 
-def _out_rows(fn: str, out: Optional[torch.Tensor], query: torch.Tensor) -> torch.Tensor:
+def _out_rows(fn: str, out: Optional[torch.Tensor], query: torch.Tensor) -> Tuple[torch.Tensor, int, int, int]:
+    """(out, address, token stride, head stride); a fresh tensor for ``None``."""
     if out is None:
-        return torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    s = out.stride()
-    if not (out.shape == query.shape and out.dtype == query.dtype and out.device == query.device and s[2] == 1 and
-            s[0] % 8 == 0 and s[1] % 8 == 0 and out.data_ptr() % 16 == 0):
-        raise RuntimeError(f"{fn}: out must be shaped like query, with contiguous 16-byte aligned rows")
-    return out
+        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+        return out, out.data_ptr(), out.shape[1] * out.shape[2], out.shape[2]
+    _device_tensors(fn, query.device, out=out)
+    if not (out.shape == query.shape and out.dtype == query.dtype):
+        raise RuntimeError(f"{fn}: out must be shaped like query, with its dtype")
+    ts, hs, ds = out.stride()
+    p = out.data_ptr()
+    # (a row stride of 0 would have rows overwrite each other)
+    if not (ds == 1 and not (ts % 8 or hs % 8 or p % 16) and ts >= out.shape[2] and (hs >= out.shape[2] or
+                                                                                     out.shape[1] == 1)):
+        raise RuntimeError(f"{fn}: out must have contiguous 16-byte aligned rows that do not overlap")
+    return out, p, ts, hs
 
 
 def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -829,28 +844,34 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     not initialized there). ``out`` must not overlap the inputs.
     """
     fn = "prompt_attention"
-    _require(isinstance(query, torch.Tensor) and query.is_cuda, "prompt_attention: query must be a CUDA tensor")
-    _device_tensors(fn, query.device, (keys, "keys"), (values, "values"), (cu_seqlens, "cu_seqlens"))
+    if not (isinstance(query, torch.Tensor) and query.is_cuda):
+        raise RuntimeError(f"{fn}: query must be a CUDA tensor")
+    device, dtype, shape = query.device, query.dtype, query.shape
+    _device_tensors(fn, device, keys=keys, values=values, cu_seqlens=cu_seqlens)
     _no_grad(fn, query, keys, values)
-    _require(query.dim() == 3 and keys.dim() == 3 and values.dim() == 3,
-             "prompt_attention: query, keys and values must be 3-D [tokens, heads, head_dim]")
-    T, Hq, D = query.shape
-    Hk = keys.shape[1]
-    _require(query.dtype in (torch.float16, torch.bfloat16), "prompt_attention: query must be fp16 or bf16")
-    _require(keys.dtype == query.dtype and values.dtype == query.dtype,
-             "prompt_attention: keys and values must have query's dtype")
-    if not (tuple(keys.shape) == (T, Hk, D) and keys.shape == values.shape):
-        raise RuntimeError(f"{fn}: keys and values must be [{T}, kv heads, {D}], got {list(keys.shape)} and "
+    kshape = keys.shape
+    if not (len(shape) == 3 and len(kshape) == 3 and values.dim() == 3):
+        raise RuntimeError(f"{fn}: query, keys and values must be 3-D [tokens, heads, head_dim]")
+    T, Hq, D = shape
+    Hk = kshape[1]
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
+        raise RuntimeError(f"{fn}: query must be fp16 or bf16")
+    if not (keys.dtype is dtype and values.dtype is dtype):
+        raise RuntimeError(f"{fn}: keys and values must have query's dtype")
+    if not (kshape == (T, Hk, D) and values.shape == kshape):
+        raise RuntimeError(f"{fn}: keys and values must be [{T}, kv heads, {D}], got {list(kshape)} and "
                            f"{list(values.shape)}")
-    _require(cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1, "prompt_attention: cu_seqlens must be 1-D [batch + 1]")
-    B = cu_seqlens.shape[0] - 1
-    _int32(fn, cu_seqlens, "cu_seqlens", (B + 1,))
-    out = _out_rows(fn, out, query)
-    q, k, v = _rows(query), _rows(keys), _rows(values)
-    with _on(query.device):
-        d = PromptDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), int(q.dtype == torch.bfloat16), T, B,
-                       Hq, Hk, D, q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                       out.stride(0), out.stride(1), cu_seqlens.data_ptr(), int(window_size), int(num_sink_tokens))
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
+        raise RuntimeError(f"{fn}: cu_seqlens must be 1-D [batch + 1]")
+    n = cu_seqlens.shape[0]
+    _int32(fn, cu_seqlens, "cu_seqlens", (n,))
+    with _on(device):
+        out, po, ots, ohs = _out_rows(fn, out, query)
+        q, pq, qts, qhs = _rows(query)
+        k, pk, kts, khs = _rows(keys)
+        v, pv, vts, vhs = _rows(values)
+        d = PromptDesc(pq, pk, pv, po, 1 if dtype is torch.bfloat16 else 0, T, n - 1, Hq, Hk, D, qts, qhs, kts, khs,
+                       vts, vhs, ots, ohs, cu_seqlens.data_ptr(), int(window_size), int(num_sink_tokens))
         _check(_c_prompt(ctypes.byref(d), _stream(query)))
     return out
 
@@ -859,8 +880,8 @@ def _packed_desc(query, key_cache, value_cache, block_tables, context_lens, cu_s
                  window_size, num_sink_tokens, out):
     """Validated PackedDesc: (desc, out, workspace, keepalive)."""
     fn = "packed_attention"
-    _device_tensors(fn, query.device, (key_cache, "key_cache"), (value_cache, "value_cache"),
-                    (block_tables, "block_tables"), (context_lens, "context_lens"), (cu_seqlens, "cu_seqlens"))
+    _device_tensors(fn, query.device, key_cache=key_cache, value_cache=value_cache, block_tables=block_tables,
+                    context_lens=context_lens, cu_seqlens=cu_seqlens)
     _no_grad(fn, query)
     _require(query.dim() == 3, "packed_attention: query must be 3-D [tokens, heads, head_dim]")
     _require(query.dtype == torch.float16, "packed_attention: query must be fp16")
@@ -892,17 +913,19 @@ def _packed_desc(query, key_cache, value_cache, block_tables, context_lens, cu_s
                  "packed_attention: caches must be contiguous")
         nb, bs, Hk = key_cache.shape[:3]
         fmt, base_k, base_v = KV_FP16, key_cache.data_ptr(), value_cache.data_ptr()
-    out = _out_rows(fn, out, query)
-    q = _rows(query)
-    d = PackedDesc(q.data_ptr(), out.data_ptr(), T, B, Hq, Hk, D, q.stride(0), q.stride(1), out.stride(0),
-                   out.stride(1), fmt, base_k, base_v, bs, nb, block_tables.data_ptr(), block_tables.shape[1],
-                   context_lens.data_ptr(), cu_seqlens.data_ptr(), int(max_query_len), int(max_seq_len),
-                   int(window_size), int(num_sink_tokens))
-    need = _i64()
-    _check(_c_packed_ws(ctypes.byref(d), ctypes.byref(need)))
+    out, po, ots, ohs = _out_rows(fn, out, query)
+    q, pq, qts, qhs = _rows(query)
+    # (the C side holds 32-bit sizes)
+    d = PackedDesc(pq, po, T, B, Hq, Hk, D, qts, qhs, ots, ohs, fmt, base_k, base_v, bs, nb, block_tables.data_ptr(),
+                   block_tables.shape[1], context_lens.data_ptr(), cu_seqlens.data_ptr(),
+                   min(int(max_query_len), 2 ** 31 - 1), min(int(max_seq_len), 2 ** 31 - 1), int(window_size),
+                   int(num_sink_tokens))
+    need, zeroed = _i64(), _i64()
+    _check(_c_packed_ws(ctypes.byref(d), ctypes.byref(need), ctypes.byref(zeroed)))
     ws = None
     if need.value > 0:
         ws = torch.empty(need.value, dtype=torch.uint8, device=query.device)
+        ws[:zeroed.value].zero_()  # arrival counters; the partial sums may hold anything
         d.workspace, d.workspace_bytes = ws.data_ptr(), need.value
     return d, out, ws, keep + (q,)
 
@@ -944,7 +967,7 @@ class PreparedPackedAttention:
                  max_seq_len, window_size=-1, *, num_sink_tokens=0, out=None):
         _require(isinstance(query, torch.Tensor) and query.is_cuda, "packed_attention: query must be a CUDA tensor")
         self.device = query.device
-        _require(_rows(query) is query,
+        _require(query.dim() == 3 and _rows(query)[0] is query,
                  "PreparedPackedAttention: query's rows must be contiguous and 16-byte aligned (it is read in place)")
         with _on(self.device):
             self._d, self.out, self._ws, self._keep = _packed_desc(
@@ -963,16 +986,30 @@ class PreparedPackedAttention:
         return self.out
 
 
-class BatchStep(NamedTuple):
-    """What ``advance_batch`` writes (int32): ``context_lens`` ``[B]``,
-    ``free_span`` ``[2]``, ``cu_seqlens`` ``[B + 1]``, ``slots`` and
-    ``positions`` ``[rows]``, ``status`` ``[B]``."""
-    context_lens: torch.Tensor
-    free_span: torch.Tensor
-    cu_seqlens: torch.Tensor
-    slots: torch.Tensor
-    positions: torch.Tensor
-    status: torch.Tensor
+class BatchStep:
+    """What ``advance_batch`` writes (int32, contiguous, on one device):
+    ``context_lens`` ``[B]``, ``free_span`` ``[2]``, ``cu_seqlens`` ``[B +
+    1]``, ``slots`` and ``positions`` ``[rows]``, ``status`` ``[B]``. The
+    tensors are checked here once, and kept."""
+
+    FIELDS = ("context_lens", "free_span", "cu_seqlens", "slots", "positions", "status")
+    __slots__ = FIELDS + ("device", "_args")
+
+    def __init__(self, context_lens, free_span, cu_seqlens, slots, positions, status):
+        fn = "advance_batch"
+        tensors = (context_lens, free_span, cu_seqlens, slots, positions, status)
+        self.device = getattr(context_lens, "device", None)
+        _device_tensors(fn, self.device, **dict(zip(self.FIELDS, tensors)))
+        _require(context_lens.dim() == 1 and slots.dim() == 1, "advance_batch: context_lens and slots must be 1-D")
+        B, rows = context_lens.shape[0], slots.shape[0]
+        for n, t, k in zip(self.FIELDS, tensors, (B, 2, B + 1, rows, rows, B)):
+            _int32(fn, t, n, (k,))
+            setattr(self, n, t)
+        self._args = (rows, *(t.data_ptr() for t in tensors))
+
+    def replace(self, **tensors) -> "BatchStep":
+        """The same buffers with some of them exchanged."""
+        return BatchStep(**{**{n: getattr(self, n) for n in self.FIELDS}, **tensors})
 
 
 def advance_batch_buffers(num_requests: int, num_rows: int, device) -> BatchStep:
@@ -1003,13 +1040,13 @@ def advance_batch(new_tokens: torch.Tensor, context_lens: torch.Tensor, block_ta
     advanced in place. Calls on one batch must not overlap.
     """
     fn = "advance_batch"
-    _require(isinstance(new_tokens, torch.Tensor) and new_tokens.is_cuda,
-             "advance_batch: new_tokens must be a CUDA tensor")
-    dev = new_tokens.device
-    _device_tensors(fn, dev, (context_lens, "context_lens"), (block_tables, "block_tables"),
-                    (free_pages, "free_pages"), (free_span, "free_span"))
-    _require(new_tokens.dim() == 1 and block_tables.dim() == 2 and free_pages.dim() == 1,
-             "advance_batch: new_tokens and free_pages must be 1-D, block_tables 2-D")
+    if not (isinstance(new_tokens, torch.Tensor) and new_tokens.is_cuda):
+        raise RuntimeError(f"{fn}: new_tokens must be a CUDA tensor")
+    device = new_tokens.device
+    _device_tensors(fn, device, context_lens=context_lens, block_tables=block_tables, free_pages=free_pages,
+                    free_span=free_span)
+    if not (new_tokens.dim() == 1 and block_tables.dim() == 2 and free_pages.dim() == 1):
+        raise RuntimeError(f"{fn}: new_tokens and free_pages must be 1-D, block_tables 2-D")
     B, M, C = new_tokens.shape[0], block_tables.shape[1], free_pages.shape[0]
     _int32(fn, new_tokens, "new_tokens", (B,))
     _int32(fn, context_lens, "context_lens", (B,))
@@ -1017,16 +1054,15 @@ def advance_batch(new_tokens: torch.Tensor, context_lens: torch.Tensor, block_ta
     _int32(fn, free_pages, "free_pages", (C,))
     _int32(fn, free_span, "free_span", (2,))
     if out is None:
-        _require(num_rows is not None, "advance_batch: num_rows or out must be given")
-        out = advance_batch_buffers(B, num_rows, dev)
-    rows = out.slots.shape[0]
-    _require(num_rows is None or num_rows == rows, "advance_batch: num_rows differs from out's rows")
-    _device_tensors(fn, dev, *zip(out, BatchStep._fields))
-    for t, n, k in zip(out, BatchStep._fields, (B, 2, B + 1, rows, rows, B)):
-        _int32(fn, t, n, (k,))
-    with _on(dev):
+        _require(num_rows is not None and num_rows >= 0, "advance_batch: num_rows or out must be given")
+        out = advance_batch_buffers(B, num_rows, device)
+    rows, *pointers = out._args
+    if num_rows is not None and num_rows != rows:
+        raise RuntimeError(f"{fn}: num_rows differs from out's rows")
+    if out.device != device or out.context_lens.shape[0] != B:
+        raise RuntimeError(f"{fn}: out holds buffers of another device or number of requests")
+    with _on(device):
         _check(_c_advance(new_tokens.data_ptr(), context_lens.data_ptr(), B, block_tables.data_ptr(), M,
-                          free_pages.data_ptr(), C, free_span.data_ptr(), int(block_size), rows,
-                          out.context_lens.data_ptr(), out.free_span.data_ptr(), out.cu_seqlens.data_ptr(),
-                          out.slots.data_ptr(), out.positions.data_ptr(), out.status.data_ptr(), _stream(new_tokens)))
+                          free_pages.data_ptr(), C, free_span.data_ptr(), int(block_size), rows, *pointers,
+                          _stream(new_tokens)))
     return out

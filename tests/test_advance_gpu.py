@@ -103,7 +103,7 @@ def test_in_place_steps_in_a_graph():
     new = np.ones(B, np.int32)
     dn, dc, dt, dr, ds = (torch.from_numpy(x).to(dev()) for x in (new, ctx, tables, ring, span))
     buf = memopt_C.advance_batch_buffers(B, B + 4, dev())
-    buf = buf._replace(context_lens=dc, free_span=ds)
+    buf = buf.replace(context_lens=dc, free_span=ds)
     memopt_C.advance_batch(dn, dc, dt, dr, ds, bs, out=buf)
     for d, x in ((dc, ctx), (dt, tables), (ds, span)):
         d.copy_(torch.from_numpy(x))
@@ -151,4 +151,10 @@ def test_refusals():
     refused("4096 requests", [z(4097), z(4097), z(4097, 4), z(9), z(2)], 16, 4)
     refused("2\\^31", ok, 2 ** 30, 4)
     refused("differs", ok, 16, 4, out=memopt_C.advance_batch_buffers(3, 5, dev()))
-    refused("status", ok, 16, out=memopt_C.advance_batch_buffers(3, 5, dev())._replace(status=z(2)))
+    refused("another device or number", ok, 16, out=memopt_C.advance_batch_buffers(4, 5, dev()))
+    for field, t, match in [("status", z(2), "status"), ("slots", z(6), "positions"), ("slots", z(5).cpu(), "CUDA"),
+                            ("positions", z(10)[::2], "positions"), ("context_lens", z(3).long(), "context_lens")]:
+        with pytest.raises(RuntimeError, match=match):
+            memopt_C.advance_batch_buffers(3, 5, dev()).replace(**{field: t})
+    with pytest.raises(TypeError):
+        memopt_C.advance_batch_buffers(3, 5, dev()).replace(rows=z(5))

@@ -203,7 +203,9 @@ def test_refusals():
     refused("1-D", q, k, v, cu[None])
     refused("head_dim must be", q[..., :32].contiguous(), k[..., :32].contiguous(), v[..., :32].contiguous(), cu)
     refused("out must be", q, k, v, cu, out=torch.empty_like(q).bfloat16())
-    refused("out must be", q, k, v, cu, out=torch.empty((20, 4, 65), dtype=q.dtype, device=dev())[..., 1:])
+    refused("out must have", q, k, v, cu, out=torch.empty((20, 4, 65), dtype=q.dtype, device=dev())[..., 1:])
+    refused("overlap", q, k, v, cu, out=torch.empty((20, 1, 64), dtype=q.dtype, device=dev()).expand(20, 4, 64))
+    refused("out must be a CUDA", q, k, v, cu, out=q.cpu())
     refused("gradients", q.requires_grad_(), k, v, cu)
     with torch.no_grad():
         memopt_C.prompt_attention(q, k, v, cu)
