@@ -36,6 +36,7 @@
 #include <cmath>
 
 #include "attention.hpp"
+#include "lds_dma.hpp"
 #include "page_format.hpp"
 
 namespace memopt {
@@ -45,12 +46,29 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
+// x / d for 0 <= x < 2^31 by a product: with 2^l >= d and m = floor(2^(31 + l)
+// / d) + 1, floor(m x / 2^(31 + l)) = floor(x / d) (the classic round-up
+// multiplier; a division takes some 25 vector instructions, and a workgroup
+// that takes ten steps per wave felt them).
+struct Divisor {
+  uint32_t d, mul, shift;
+  static Divisor of(uint32_t d) {
+    uint32_t l = 0;
+    while ((1ull << l) < d) ++l;
+    return {d, d > 1 ? (uint32_t)((1ull << (31 + l)) / d + 1) : 0, l > 0 ? l - 1 : 0};
+  }
+  __device__ __forceinline__ int32_t operator()(int32_t x) const {
+    return d == 1 ? x : (int32_t)(__umulhi((uint32_t)x, mul) >> shift);
+  }
+};
+
 struct PackedParams {
   const half_t *q;
   half_t *out;
   int64_t q_ts, q_hs, o_ts, o_hs;  // elements
-  const int32_t *cu, *ctx, *bt;
   int32_t T, B, Hq, Hk, G, M, bs;
+  Divisor by_g;                  // rows to tokens
+  int32_t span;                  // positions that a block of rows can spread over, less one
   int64_t nb;
   const uint8_t *k, *v;          // INT4 pages: k = the page buffer
   int64_t kv_ps, kv_hs, kv_ts;   // bytes
@@ -61,9 +79,9 @@ struct PackedParams {
   float *ws_o, *ws_ml;           // [2 * wgs * Hk][QN][D], [2 * wgs * Hk][QN][2]: see partial_slot
 };
 
-// Workgroups per key head, so partial sums of a block, at most: their weights
-// take the place of the waves' sums in LDS.
-static constexpr int max_workgroups(int D) { return 4 * D; }
+// Workgroups per key head, so partial sums of a block, at most (their weights
+// are held in LDS).
+static constexpr int kMaxParts = 256;
 
 // Inclusive prefix sum over the wave (DPP row shifts, then row broadcasts),
 // saturating: query starts that do not ascend can count rows more than once.
@@ -102,16 +120,17 @@ struct Seq {
   int32_t start, n, ctx, kv_lim, blocks, steps;
 };
 template <int QN>
-__device__ __forceinline__ Seq sequence(const PackedParams &p, int32_t b) {
+__device__ __forceinline__ Seq sequence(const PackedParams &p, const int32_t *__restrict__ starts,
+                                        const int32_t *__restrict__ ctxs, int32_t b) {
   Seq q;
-  q.start = min(max(p.cu[b], 0), p.T);
-  q.n = min(max(p.cu[b + 1], q.start), p.T) - q.start;
-  q.ctx = p.ctx[b];
+  q.start = min(max(starts[b], 0), p.T);
+  q.n = min(max(starts[b + 1], q.start), p.T) - q.start;
+  q.ctx = ctxs[b];
   q.kv_lim = (int32_t)min((int64_t)q.ctx, (int64_t)p.M * p.bs);
   q.blocks = (q.n * p.G + QN - 1) / QN;
   const int32_t pos0 = q.ctx - q.n;
   int32_t n = visible_chunks(p, q.kv_lim, pos0, q.ctx - 1).n;
-  if (q.blocks > 1) n = min(n, ((min(p.sinks, max(q.kv_lim, 0)) + 15) >> 4) + ((p.W + QN / p.G + 1) >> 4) + 2);
+  if (q.blocks > 1) n = min(n, ((min(p.sinks, max(q.kv_lim, 0)) + 15) >> 4) + ((p.W + p.span) >> 4) + 2);
   q.steps = max(1, (n + 1) >> 1);
   return q;
 }
@@ -140,30 +159,66 @@ struct PackedV<D, MEMOPT_KV_FP16> {
   uint32_t w[8][D / 32];  // token e: D / 16 halves
 };
 
-template <int D, int FMT, int QB>
-__global__ __launch_bounds__(256, QB == 1 ? (FMT == MEMOPT_KV_INT4 || D == 64 ? 4 : 2) : 2) void packed_kernel(
-    const PackedParams p) {
-  constexpr int NW = 4, NT = 64 * NW, KK = D / 32, ND = D / 16, QN = 16 * QB;
+// 16 bytes per lane from buffer offset IMM + off into LDS byte m0v + IMM + 16 *
+// lane, not waited for (the compiler does not track it; the immediate counts
+// for both addresses, and the s_nop is the wait state between a write of m0
+// and its use, as in lds_dma.hpp). STREAM: data read once per launch
+// (kStreamLoad).
+template <bool STREAM, int IMM>
+__device__ __forceinline__ void ring_copy(__amdgpu_buffer_rsrc_t r, uint32_t m0v, uint32_t off) {
+  static_assert(IMM < 4096, "immediate offsets are 12 bits");
+  if constexpr (STREAM)
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen offset:%3 nt lds"
+                 ::"v"(off), "s"(r), "{m0}"(m0v), "i"(IMM) : "memory");
+  else
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen offset:%3 lds"
+                 ::"v"(off), "s"(r), "{m0}"(m0v), "i"(IMM) : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ T lds_at(uint32_t a) {
+  return *(const __attribute__((address_space(3))) T *)(uintptr_t)a;
+}
+
+static constexpr int kRingSteps = 2;
+
+// Workgroups per CU that the kernels' registers and LDS are meant for.
+__host__ __device__ static constexpr int resident(int NW, int QB) { return QB == 2 ? 2 : NW == 4 ? 3 : 1; }
+
+template <int D, int FMT, int QB, int NW>
+__global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_kernel(
+    const PackedParams p, const int32_t *__restrict__ starts, const int32_t *__restrict__ ctxs,
+    const int32_t *__restrict__ tables) {
+  constexpr int NT = 64 * NW, KK = D / 32, ND = D / 16, QN = 16 * QB;
   constexpr bool PAGES = FMT == MEMOPT_KV_INT4;
   constexpr int NG = PAGES ? D / 64 : 1;  // score sums per (row, token)
   constexpr int OS = D + 4;               // row stride of s_o: 16 rows of D floats would share a bank
-  __shared__ __attribute__((aligned(16))) float s_o[NW][QN][OS];
+  // Pages stream through a ring of raw blocks per wave (see copy_step), which
+  // the merge of the waves takes over when the steps are done.
+  constexpr int BLK = 16 * D + 64 * (D / 64), STG = 2 * BLK, NS = kRingSteps;
+  constexpr int OBYTES = NW * QN * OS * 4, RBYTES = PAGES ? NW * NS * STG : 0, MBYTES = QN * kMaxParts * 4 + NT * 16;
+  __shared__ __attribute__((aligned(16))) uint8_t smem[std::max({OBYTES, RBYTES, MBYTES})];
+  float(*const s_o)[QN][OS] = reinterpret_cast<float(*)[QN][OS]>(smem);
   __shared__ float s_ml[NW][QN][2];
   __shared__ int s_last;
-  static_assert(NW * OS >= max_workgroups(D), "the weights of a merge fit s_o");
 
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int32_t kvh = blockIdx.x % p.Hk, wg = blockIdx.x / p.Hk;
 
-  // The list's length; then the sequence that holds this workgroup's first place.
-  uint32_t sum = 0;
-  for (int32_t b0 = 0; b0 < p.B; b0 += 64) {
-    uint32_t c = 0;
+  // The list's length; then the sequence that holds this workgroup's first
+  // place. Lane i takes sequence b0 + i; up to 64 sequences are counted once.
+  uint32_t sum = 0, c = 0, nb = 0;
+  auto count = [&](int32_t b0) __attribute__((always_inline)) {
+    c = nb = 0;
     if (b0 + lane < p.B) {
-      const Seq q = sequence<QN>(p, b0 + lane);
-      c = (uint32_t)q.blocks * (uint32_t)q.steps;
+      const Seq q = sequence<QN>(p, starts, ctxs, b0 + lane);
+      nb = q.blocks;
+      c = nb * (uint32_t)q.steps;
     }
+  };
+  for (int32_t b0 = 0; b0 < p.B; b0 += 64) {
+    count(b0);
     sum = __builtin_elementwise_add_sat(sum, (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(c), 63));
   }
   // (past 2^31 only where sequences overlap: nothing is computed then)
@@ -172,20 +227,17 @@ __global__ __launch_bounds__(256, QB == 1 ? (FMT == MEMOPT_KV_INT4 || D == 64 ? 
   const int32_t wgs = min(p.wgs, max(1, total / NW));
   if (total <= 0 || wg >= wgs) return;
   const int32_t run = total / wgs, longer = total - run * wgs;  // the first `longer` runs have one place more
-  int32_t at = wg * run + min(wg, longer);
+  const int32_t first = wg * run + min(wg, longer);
+  int32_t at = first;
   const int32_t stop = at + run + (wg < longer ? 1 : 0);
   auto wg_of = [&](int32_t x) {
     const int32_t edge = longer * (run + 1);
-    return x < edge ? x / (run + 1) : longer + (x - edge) / run;
+    const bool head = x < edge;
+    return (head ? 0 : longer) + (head ? x : x - edge) / (head ? run + 1 : run);
   };
   int32_t seq_at = 0, seq_blocks = 0, b = 0;  // places and blocks before sequence b
   for (int32_t b0 = 0; b0 < p.B; b0 += 64) {
-    uint32_t c = 0, nb = 0;
-    if (b0 + lane < p.B) {
-      const Seq q = sequence<QN>(p, b0 + lane);
-      nb = q.blocks;
-      c = nb * (uint32_t)q.steps;
-    }
+    if (p.B > 64) count(b0);
     const int32_t incl = (int32_t)wave_scan(c), blocks = (int32_t)wave_scan(nb);
     const int32_t sum64 = __builtin_amdgcn_readlane(incl, 63);
     if (at < seq_at + sum64) {
@@ -200,51 +252,23 @@ __global__ __launch_bounds__(256, QB == 1 ? (FMT == MEMOPT_KV_INT4 || D == 64 ? 
   }
 
   // Block by block of this workgroup's run.
-  Seq seq = sequence<QN>(p, b);
+  Seq seq = sequence<QN>(p, starts, ctxs, b);
   while (at < stop) {
   while (at >= seq_at + seq.blocks * seq.steps) {  // (sequences without rows take no place)
     seq_at += seq.blocks * seq.steps;
     seq_blocks += seq.blocks;
-    seq = sequence<QN>(p, ++b);
+    seq = sequence<QN>(p, starts, ctxs, ++b);
   }
-  const int32_t block = (at - seq_at) / seq.steps;
+  const int32_t block = seq.blocks == 1 ? 0 : (at - seq_at) / seq.steps;
   if (seq_blocks + block >= p.blocks) return;  // sequences overlap: past the counters
   const int32_t block_at = seq_at + block * seq.steps;
   const int32_t row0 = block * QN, rows = seq.n * p.G, ctx = seq.ctx, kv_lim = seq.kv_lim;
   const int32_t pos0 = ctx - seq.n;  // position of the sequence's first query
-  const int32_t pos_lo = pos0 + row0 / p.G, pos_hi = pos0 + (min(row0 + QN, rows) - 1) / p.G;
+  const int32_t pos_lo = pos0 + p.by_g(row0), pos_hi = pos0 + p.by_g(min(row0 + QN, rows) - 1);
   const Visible vis = visible_chunks(p, kv_lim, pos_lo, pos_hi);
   const int32_t sc = vis.sc, wc0 = vis.wc0, n_vis = vis.n;
   const int32_t begin = at - block_at, end = min(min(stop - block_at, seq.steps), (n_vis + 1) >> 1);
   at = min(stop, block_at + seq.steps);
-
-  // Q as the B operand: column r = row, k-group g; dims of product kk as the K
-  // operand holds them (pages: 16 g + 8 (kk % 2) of scale group kk / 2, in
-  // nibble-unpack order; fp16: 32 kk + 8 g).
-  h8_t qf[QB][KK];
-  int32_t row_pos[QB];
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    const int32_t row = row0 + 16 * qb + r, tok = row / p.G;
-    row_pos[qb] = pos0 + tok;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      h8_t x = {};
-      if (row < rows) {
-        const int d0 = PAGES ? 64 * (kk >> 1) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g;
-        const h8_t y = __builtin_bit_cast(
-            h8_t, *reinterpret_cast<const u32x4_t *>(p.q + (int64_t)(seq.start + tok) * p.q_ts +
-                                                     (int64_t)(kvh * p.G + row - tok * p.G) * p.q_hs + d0));
-        if (PAGES) {
-          x[0] = y[0]; x[1] = y[4]; x[2] = y[1]; x[3] = y[5];
-          x[4] = y[2]; x[5] = y[6]; x[6] = y[3]; x[7] = y[7];
-        } else {
-          x = y;
-        }
-      }
-      qf[qb][kk] = x;
-    }
-  }
 
   f32x4_t o[QB][ND];
   float ncm[QB], thr[QB], lsum[QB];
@@ -257,124 +281,210 @@ __global__ __launch_bounds__(256, QB == 1 ? (FMT == MEMOPT_KV_INT4 || D == 64 ? 
     lsum[qb] = 0.0f;
   }
 
-  // Chunk i of the visible list: logical chunk, and its byte offset in the
-  // cache (chunk 0 of page 0, always mapped, if there is none).
-  struct Chunk {
-    int32_t lc;
-    bool ok;
-    int64_t kv;
-  };
-  const int32_t *btrow = p.bt + (int64_t)b * p.M;
+  // Chunk i of the visible list is logical chunk i, or i + skip behind the
+  // sinks. A step is the chunks 2 i and 2 i + 1; those of steps [full0, full1)
+  // lie where every row sees all their tokens, so they need no mask once both
+  // pages are there.
+  const int32_t *btrow = tables + (int64_t)b * p.M;
   const int32_t cpp = PAGES ? 1 : p.bs >> 4;
   const int32_t nb32 = (int32_t)min(p.nb, (int64_t)INT32_MAX);
-  struct Entry {  // a chunk's block-table entry, not yet waited for
-    int32_t lc, page, phys;
-    bool in;
+  const int32_t skip = wc0 - sc;
+  auto logical = [&](int32_t i) { return i + (i < sc ? 0 : skip); };
+  const int32_t full0 = (max(skip > 0 ? sc : 0, ((max(0, pos_hi - p.W + 1) + 15) >> 4) - skip) + 1) >> 1;
+  const int32_t full1 = ((max(0, min(kv_lim, pos_lo + 1)) >> 4) - skip) >> 1;
+  struct Step {  // its block-table entries, not yet waited for
+    int32_t i, a, b;
   };
   auto fetch = [&](int32_t i) __attribute__((always_inline)) {
-    Entry e;
-    e.lc = i < sc ? i : wc0 + (i - sc);
-    e.in = i < n_vis;
-    e.page = cpp == 1 ? e.lc : e.lc / cpp;
-    e.phys = btrow[e.in ? e.page : 0];  // n_vis > 0 here, so the row has an entry 0
+    Step e;
+    e.i = i;
+    const int32_t ca = 2 * i, cb = 2 * i + 1;
+    const int32_t la = ca < n_vis ? logical(ca) : 0, lb = cb < n_vis ? logical(cb) : 0;  // (a row has an entry 0)
+    e.a = btrow[cpp == 1 ? la : la / cpp];
+    e.b = btrow[cpp == 1 ? lb : lb / cpp];
+    if (cb >= n_vis) e.b = -1;
     return e;
   };
-  auto resolve = [&](const Entry &e) __attribute__((always_inline)) {
-    Chunk c;
-    c.lc = e.lc;
-    c.ok = e.in && e.phys >= 0 && e.phys < nb32;
-    c.kv = (int64_t)(c.ok ? e.phys : 0) * p.kv_ps + (int64_t)kvh * p.kv_hs +
-           (int64_t)(c.ok ? 16 * (e.lc - e.page * cpp) : 0) * p.kv_ts;
-    return c;
+  auto mapped = [&](int32_t phys) { return phys >= 0 && phys < nb32; };
+  // Byte offset of chunk `lc` (chunk 0 of page 0, always mapped, if its page is not).
+  auto offset_of = [&](int32_t phys, int32_t lc) __attribute__((always_inline)) {
+    const bool ok = mapped(phys);
+    int64_t x = (int64_t)(ok ? phys : 0) * p.kv_ps;
+    if constexpr (!PAGES) x += (int64_t)(ok ? 16 * (lc - lc / cpp * cpp) : 0) * p.kv_ts;
+    return x;
   };
 
   const Int4Page f(D);
   PackedK<D, FMT> kr;
   PackedV<D, FMT> vr;
-  // K of two chunks: lane row r is tokens r % 8 and r % 8 + 8 of chunk r / 8.
-  auto load_k = [&](const Chunk &ca, const Chunk &cb) __attribute__((always_inline)) {
-    const int pr = r & 7;
-    const uint8_t *base = p.k + (r < 8 ? ca.kv : cb.kv);
+  const int p0 = 4 * (g & 1);  // this lane's score tokens: p0 + i and p0 + i + 8 of chunk g / 2
+  // Pages: the two blocks of a step as they are, 1 KiB per copy, straight into
+  // the wave's ring: kRingSteps steps are in flight without holding registers.
+  const uint32_t ring = lds_u32(smem) + wave * NS * STG;
+  const uint8_t *const kbase = p.k + (int64_t)kvh * p.kv_hs, *const vbase = p.v + (int64_t)kvh * p.kv_hs;
+  auto copy_block = [&](int64_t kv, uint32_t dst) __attribute__((always_inline)) {
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc((void *)(kbase + kv), (short)0, BLK, 0x00020000);
+    constexpr int TAIL = BLK / 1024 * 1024;
+    ring_copy<QB == 1, 0>(rs, dst, 16 * lane);
+    if constexpr (D == 128) ring_copy<QB == 1, 1024>(rs, dst, 16 * lane);
+    if (lane < (BLK - TAIL) / 16) ring_copy<QB == 1, TAIL>(rs, dst, 16 * lane);
+  };
+  auto copy_step = [&](const Step &e, int stage) __attribute__((always_inline)) {
+    copy_block(offset_of(e.a, 0), ring + stage * STG);
+    copy_block(offset_of(e.b, 0), ring + stage * STG + BLK);
+  };
+  // K of a step: lane row r is tokens r % 8 and r % 8 + 8 of chunk r / 8.
+  // V: lane (r, g) holds dims [D/16 r, D/16 (r + 1)) of its score tokens.
+  auto read_k = [&](int stage) __attribute__((always_inline)) {
     if constexpr (PAGES) {
+      const uint32_t at = ring + stage * STG;
+      const uint32_t kb = at + (r < 8 ? 0 : BLK) + (uint32_t)f.kcodes + (8 * (r & 7) + (D == 128 ? g : 2 * g)) * (D / 8);
+      const uint32_t tb = at + (g < 2 ? 0 : BLK);
 #pragma unroll
       for (int j = 0; j < D / 64; ++j) {
-        // D = 128: lane group 4 j + g of the page (16 dims of scale group j); D = 64: groups 2 g and 2 g + 1
-        const int c = D == 128 ? 4 * j + g : 2 * g;
-        const u32x4_t x = *reinterpret_cast<const u32x4_t *>(base + f.kcodes + (8 * pr + c) * f.BPL);
+        // (D = 128: lane group 4 j + g of the page, 16 dims of scale group j; D = 64: groups 2 g and 2 g + 1)
+        const u32x4_t x = lds_at<u32x4_t>(kb + 4 * j * (D / 8));
 #pragma unroll
         for (int w = 0; w < 4; ++w) kr.w[4 * j + w] = x[w];
-        kr.sc[j] = *reinterpret_cast<const u32x4_t *>(p.k + (g < 2 ? ca.kv : cb.kv) + f.kscales +
-                                                      2 * (16 * j + 8 * (g & 1)));
+        kr.sc[j] = lds_at<u32x4_t>(tb + (uint32_t)f.kscales + 2 * (16 * j + 2 * p0));
       }
-    } else {
+    }
+  };
+  auto read_v = [&](int stage) __attribute__((always_inline)) {
+    if constexpr (PAGES) {
+      const uint32_t tb = ring + stage * STG + (g < 2 ? 0 : BLK);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t src = tb + (uint32_t)f.vcodes + 8 * (p0 + i) * (D / 8) + (D / 16) * r;
+        if constexpr (D == 128) {
+          const u32x2_t x = lds_at<u32x2_t>(src);
+          vr.w[i][0] = x[0];
+          vr.w[i][1] = x[1];
+        } else {
+          vr.w[i][0] = lds_at<uint32_t>(src);
+        }
+      }
+      vr.sc = lds_at<u32x4_t>(tb + (uint32_t)f.vscales + 2 * ((r * (D / 16) / 64) * 16 + 2 * p0));
+    }
+  };
+  // fp16 pools: the same from global memory into registers.
+  auto load_k = [&](const Step &e) __attribute__((always_inline)) {
+    if constexpr (!PAGES) {
+      const uint8_t *base = kbase + (r < 8 ? offset_of(e.a, logical(2 * e.i)) : offset_of(e.b, logical(2 * e.i + 1)));
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk)
-          kr.w[t][kk] = *reinterpret_cast<const u32x4_t *>(base + (int64_t)(pr + 8 * t) * p.kv_ts +
+          kr.w[t][kk] = *reinterpret_cast<const u32x4_t *>(base + (int64_t)((r & 7) + 8 * t) * p.kv_ts +
                                                            2 * (32 * kk + 8 * g));
     }
   };
-  // V of two chunks: lane (r, g) holds dims [D/16 r, D/16 (r + 1)) of tokens
-  // p_i, p_i + 8, p_i = 4 (g % 2) + i, of chunk g / 2 (element 2 i + t).
-  auto load_v = [&](const Chunk &ca, const Chunk &cb) __attribute__((always_inline)) {
-    const int p0 = 4 * (g & 1);
-    const int64_t cbase = g < 2 ? ca.kv : cb.kv;
-    if constexpr (PAGES) {
-      const uint8_t *base = p.k + cbase;
+  auto load_v = [&](const Step &e) __attribute__((always_inline)) {
+    if constexpr (!PAGES) {
+      const uint8_t *base = vbase + (g < 2 ? offset_of(e.a, logical(2 * e.i)) : offset_of(e.b, logical(2 * e.i + 1)));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t *src = base + f.vcodes + 8 * (p0 + i) * f.BPL + (D / 16) * r;
+      for (int x = 0; x < 8; ++x) {  // element 2 i + t: token p0 + i + 8 t
+        const uint8_t *src = base + (int64_t)(p0 + (x >> 1) + 8 * (x & 1)) * p.kv_ts + (D / 8) * r;
         if constexpr (D == 128) {
-          const u32x2_t x = *reinterpret_cast<const u32x2_t *>(src);
-          vr.w[i][0] = x[0];
-          vr.w[i][1] = x[1];
-        } else {
-          vr.w[i][0] = *reinterpret_cast<const uint32_t *>(src);
-        }
-      }
-      vr.sc = *reinterpret_cast<const u32x4_t *>(base + f.vscales + 2 * ((r * (D / 16) / 64) * 16 + 2 * p0));
-    } else {
-      const uint8_t *base = p.v + cbase;
+          const u32x4_t y = *reinterpret_cast<const u32x4_t *>(src);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint8_t *src = base + (int64_t)(p0 + (e >> 1) + 8 * (e & 1)) * p.kv_ts + (D / 8) * r;
-        if constexpr (D == 128) {
-          const u32x4_t x = *reinterpret_cast<const u32x4_t *>(src);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) vr.w[e][j] = x[j];
+          for (int j = 0; j < 4; ++j) vr.w[x][j] = y[j];
         } else {
-          const u32x2_t x = *reinterpret_cast<const u32x2_t *>(src);
-          vr.w[e][0] = x[0];
-          vr.w[e][1] = x[1];
+          const u32x2_t y = *reinterpret_cast<const u32x2_t *>(src);
+          vr.w[x][0] = y[0];
+          vr.w[x][1] = y[1];
         }
       }
     }
   };
 
+  // (w & mask) | bits as one v_and_or_b32: the constants are hidden from the
+  // compiler, which would make two instructions of them. (As inline assembly,
+  // the instruction escapes the compiler's wait states: one that overwrote
+  // the start of a sum while its matrix instruction still read it gave NaN.)
+  uint32_t m_lo = 0x000F000Fu, m_hi = 0x00F000F0u, e1024 = 0x64006400u, e64 = 0x54005400u;
+  asm("" : "+s"(m_lo), "+s"(m_hi));
+  asm("" : "+v"(e1024), "+v"(e64));
   const half2_t b1032 = {(half_t)1032.0f, (half_t)1032.0f}, b72 = {(half_t)72.0f, (half_t)72.0f};
   // The eight codes of a word, less 8, in nibble-unpack order (exact).
   auto codes = [&](uint32_t w) __attribute__((always_inline)) {
     const uint32_t w8 = w >> 8;
-    return u32x4_t{as_u32(as_half2(bfi(0x000F000Fu, w, 0x64006400u)) - b1032),
-                   as_u32(as_half2(bfi(0x00F000F0u, w, 0x54005400u)) - b72),
-                   as_u32(as_half2(bfi(0x000F000Fu, w8, 0x64006400u)) - b1032),
-                   as_u32(as_half2(bfi(0x00F000F0u, w8, 0x54005400u)) - b72)};
+    return u32x4_t{as_u32(as_half2((w & m_lo) | e1024) - b1032), as_u32(as_half2((w & m_hi) | e64) - b72),
+                   as_u32(as_half2((w8 & m_lo) | e1024) - b1032), as_u32(as_half2((w8 & m_hi) | e64) - b72)};
+  };
+  // The same without the subtractions, so plus 1032 in the even pairs and 72
+  // in the odd ones: K's sums start at minus those times the sums of q
+  // (kstart). Their 32-bit roundings grow to about 2^-24 * 1032 of the sum of
+  // |q| * scale, a tenth of what rounding K to fp16 would cost, and far below
+  // the rounding of the probabilities.
+  auto biased = [&](uint32_t w) __attribute__((always_inline)) {
+    const uint32_t w8 = w >> 8;
+    return u32x4_t{(w & m_lo) | e1024, (w & m_hi) | e64, (w8 & m_lo) | e1024, (w8 & m_hi) | e64};
+  };
+  const half2_t ones = {(half_t)1.0f, (half_t)1.0f};
+  h8_t qf[QB][KK];
+  f32x4_t kstart[QB][NG];
+  int32_t row_pos[QB];
+  auto load_q = [&]() __attribute__((always_inline)) {
+    // Q as the B operand: column r = row, k-group g; dims of product kk as the K
+    // operand holds them (pages: 16 g + 8 (kk % 2) of scale group kk / 2, in
+    // nibble-unpack order; fp16: 32 kk + 8 g).
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+      const int32_t row = row0 + 16 * qb + r, tok = p.by_g(row);
+      row_pos[qb] = pos0 + tok;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        h8_t x = {};
+        if (row < rows) {
+          const int d0 = PAGES ? 64 * (kk >> 1) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g;
+          const h8_t y = __builtin_bit_cast(
+              h8_t, *reinterpret_cast<const u32x4_t *>(p.q + (int64_t)(seq.start + tok) * p.q_ts +
+                                                       (int64_t)(kvh * p.G + row - tok * p.G) * p.q_hs + d0));
+          if (PAGES) {
+            x[0] = y[0]; x[1] = y[4]; x[2] = y[1]; x[3] = y[5];
+            x[4] = y[2]; x[5] = y[6]; x[6] = y[3]; x[7] = y[7];
+          } else {
+            x = y;
+          }
+        }
+        qf[qb][kk] = x;
+      }
+    }
+
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        float x = 0.0f;
+        if constexpr (PAGES) {
+          float even = 0.0f, odd_q = 0.0f;  // operand pairs 0, 2 and 1, 3
+#pragma unroll
+          for (int kk = j * (KK / NG); kk < (j + 1) * (KK / NG); ++kk) {
+            const u32x4_t y = __builtin_bit_cast(u32x4_t, qf[qb][kk]);
+            even = __builtin_amdgcn_fdot2(as_half2(y[2]), ones, __builtin_amdgcn_fdot2(as_half2(y[0]), ones, even, false), false);
+            odd_q = __builtin_amdgcn_fdot2(as_half2(y[3]), ones, __builtin_amdgcn_fdot2(as_half2(y[1]), ones, odd_q, false), false);
+          }
+          x = xor32_sum(xor16_sum(-1032.0f * even - 72.0f * odd_q));
+        }
+        kstart[qb][j] = f32x4_t{x, x, x, x};
+      }
   };
   auto k_operand = [&](int t, int kk) __attribute__((always_inline)) {
     if constexpr (PAGES) {
-      return __builtin_bit_cast(h8_t, codes(D == 128 ? kr.w[4 * (kk >> 1) + 2 * t + (kk & 1)] : kr.w[2 * kk + t]));
+      return __builtin_bit_cast(h8_t, biased(D == 128 ? kr.w[4 * (kk >> 1) + 2 * t + (kk & 1)] : kr.w[2 * kk + t]));
     } else {
       return __builtin_bit_cast(h8_t, kr.w[t][kk]);
     }
   };
 
-  const half2_t ones = {(half_t)1.0f, (half_t)1.0f};
   // exp2 argument of a new maximum: probabilities lie in (0, 2^15], so fp16
   // holds those down to 2^-21 of the largest as normal numbers.
   constexpr float kTop = 7.0f;
-  auto step = [&](const Chunk &ca, const Chunk &cb, const Chunk &na, const Chunk &nb_, bool more)
-                  __attribute__((always_inline)) {
+  uint32_t odd = 0;  // nonzero: a masked step held inf or NaN in V
+  // One step; `between` runs when K has been used and V has not.
+  auto step = [&](const Step &e, auto between) __attribute__((always_inline)) {
     f32x4_t s[QB][NG][2];
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
@@ -385,7 +495,7 @@ __global__ __launch_bounds__(256, QB == 1 ? (FMT == MEMOPT_KV_INT4 || D == 64 ? 
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb)
           s[qb][kk / PG][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              a, qf[qb][kk], kk % PG == 0 ? (f32x4_t){} : s[qb][kk / PG][t], 0, 0, 0);
+              a, qf[qb][kk], kk % PG == 0 ? kstart[qb][kk / PG] : s[qb][kk / PG][t], 0, 0, 0);
       }
     }
     // exp2 arguments; element 2 i + t: token key0 + i + 8 t
@@ -396,21 +506,18 @@ __global__ __launch_bounds__(256, QB == 1 ? (FMT == MEMOPT_KV_INT4 || D == 64 ? 
       for (int e = 0; e < 8; ++e) {
         float y = s[qb][0][e & 1][e >> 1];
         if constexpr (PAGES) {
-          y *= (float)as_half2(kr.sc[0][e >> 1])[e & 1];
+          y = fmaf(y, (float)as_half2(kr.sc[0][e >> 1])[e & 1], 0.0f);  // (one mixed-precision instruction)
           if constexpr (NG == 2) y = fmaf(s[qb][1][e & 1][e >> 1], (float)as_half2(kr.sc[1][e >> 1])[e & 1], y);
         }
         x[qb][e] = fmaf(y, p.qk_scale_log2, ncm[qb]);
       }
-    if (more) load_k(na, nb_);
+    between();
 
-    // Every (token, row) of the step visible: no mask (wave-uniform).
-    const int32_t ta = ca.lc * 16, tb = cb.lc * 16;
-    auto chunk_full = [&](const Chunk &c, int32_t t0) {
-      return c.ok && t0 + 16 <= kv_lim && t0 + 15 <= pos_lo && (t0 >= pos_hi - p.W + 1 || t0 + 16 <= p.sinks);
-    };
-    const bool full = chunk_full(ca, ta) && chunk_full(cb, tb);
+    const bool ok_a = mapped(e.a), ok_b = mapped(e.b);
+    const bool full = e.i >= full0 && e.i < full1 && ok_a && ok_b;  // (wave-uniform)
+    const int32_t ta = 16 * logical(2 * e.i), tb = 16 * logical(2 * e.i + 1);
     const int32_t key0 = (g < 2 ? ta : tb) + 4 * (g & 1);
-    const bool c_ok = g < 2 ? ca.ok : cb.ok;
+    const bool c_ok = g < 2 ? ok_a : ok_b;
     h8_t pf[QB];
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
@@ -456,38 +563,34 @@ __global__ __launch_bounds__(256, QB == 1 ? (FMT == MEMOPT_KV_INT4 || D == 64 ? 
 
     // A weight of 0 must not meet an inf or NaN of V. Tokens that no row of the
     // block sees (behind the context, unlinked, outside the window) become
-    // zeros; among those that only some rows see, odd values are left out
-    // and added below to the rows that see them.
-    bool odd = false;
-    uint32_t odd_e = 0;
+    // zeros; so do inf and NaN among those that only some rows see, which
+    // get them back at the end (`odd`).
     if (!full) {
       const int32_t last = c_ok ? min(pos_hi, kv_lim - 1) - key0 : -1;
       const int32_t first_w = pos_lo - p.W + 1 - key0, end_s = p.sinks - key0;
+      const bool several = pos_lo != pos_hi;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int32_t c = (e >> 1) + 8 * (e & 1);
-        bool live = (c <= last) & ((c >= first_w) | (c < end_s));
-        bool bad = false;
-        if constexpr (PAGES) {  // 8 * scale past the fp16 range
-          bad = ((vr.sc[e >> 1] >> (16 * (e & 1))) & 0x7FFFu) >= 0x7000u;
-        } else {
-          uint32_t any = 0;
-#pragma unroll
-          for (int j = 0; j < D / 32; ++j) any |= (vr.w[e][j] & 0x7C007C00u) + 0x04000400u;
-          bad = (any & 0x80008000u) != 0;
-        }
-        bad = bad && live && pos_lo != pos_hi;
-        odd |= bad;
-        odd_e |= bad ? 1u << e : 0u;
-        live = live && !bad;
+        const bool live = (c <= last) & ((c >= first_w) | (c < end_s));
         if constexpr (PAGES) {
-          vr.sc[e >> 1] &= live ? ~0u : (e & 1) ? 0x0000FFFFu : 0xFFFF0000u;
+          const uint32_t half = (e & 1) ? 0xFFFF0000u : 0x0000FFFFu;
+          const bool bad = several && live && (vr.sc[e >> 1] & half & 0x7C007C00u) == (half & 0x7C007C00u);
+          odd |= bad ? 1u : 0u;
+          vr.sc[e >> 1] &= live && !bad ? ~0u : ~half;
         } else {
 #pragma unroll
-          for (int j = 0; j < D / 32; ++j) vr.w[e][j] = live ? vr.w[e][j] : 0u;
+          for (int j = 0; j < D / 32; ++j) {
+            uint32_t w = live ? vr.w[e][j] : 0u;
+            if (several) {
+              const uint32_t f = ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u;  // a full exponent carries
+              odd |= f;
+              w &= ~((f << 1) - (f >> 15));
+            }
+            vr.w[e][j] = w;
+          }
         }
       }
-      odd = __any(odd);
     }
     auto pv = [&](int i, u32x4_t a) __attribute__((always_inline)) {
 #pragma unroll
@@ -517,65 +620,87 @@ __global__ __launch_bounds__(256, QB == 1 ? (FMT == MEMOPT_KV_INT4 || D == 64 ? 
         pv(i, a);
       }
     }
-    if (odd) {
-      // Token by token; a lane adds its quarter of the dims.
-#pragma unroll 1
-      for (int tk = 0; tk < 32; ++tk) {
-        const int t = tk & 15, pp = t & 7, half = t >> 3;
-        const int owner = 2 * (tk >> 4) + (pp >> 2), elem = 2 * (pp & 3) + half;  // lane group, element
-        // (over pages the two scale groups of a token are odd apart from each other, so any lane of the group counts)
-        if ((__ballot((odd_e >> elem) & 1) & (0xFFFFull << (16 * owner))) == 0) continue;
-        const Chunk &c = tk < 16 ? ca : cb;
-        const int32_t key = c.lc * 16 + t;
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) {
-          float pe = 0.0f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) pe = e == elem ? x[qb][e] : pe;
-          pe = __shfl(pe, r + 16 * owner, 64);
-          const bool see = key <= min(row_pos[qb], kv_lim - 1) &&
-                           (key < p.sinks || key >= row_pos[qb] - p.W + 1);
-#pragma unroll
-          for (int d = 0; d < D / 4; ++d) {
-            const int dim = (D / 4) * g + d;
-            float y;
-            bool bad;
-            if constexpr (PAGES) {
-              const uint8_t *blk = p.k + c.kv;
-              const half_t sv = reinterpret_cast<const half_t *>(blk + f.vscales)[f.scale_idx(t, dim / 64)];
-              bad = (__builtin_bit_cast(uint16_t, sv) & 0x7FFFu) >= 0x7000u;
-              y = (float)(int)((blk[f.vcodes + f.v_byte(t, dim)] >> (4 * (dim & 1))) & 15) - 8.0f;
-              y *= (float)sv;
-            } else {
-              // the whole token's row was left out on the lanes that found something odd in it
-              const half_t *rowp = reinterpret_cast<const half_t *>(p.v + c.kv + (int64_t)t * p.kv_ts);
-              bad = false;
-#pragma unroll
-              for (int z = 0; z < ND; ++z)
-                bad |= (__builtin_bit_cast(uint16_t, rowp[dim / ND * ND + z]) & 0x7C00u) == 0x7C00u;
-              y = (float)rowp[dim];
-            }
-            if (see && bad) o[qb][d % ND][d / ND] = fmaf(pe, y, o[qb][d % ND][d / ND]);
-          }
-        }
-      }
-    }
-    if (more) load_v(na, nb_);
   };
 
-  int32_t st = begin + wave;
-  if (st < end) {
-    Entry ea = fetch(2 * (st + NW)), eb = fetch(2 * (st + NW) + 1);
-    Chunk ca = resolve(fetch(2 * st)), cb = resolve(fetch(2 * st + 1));
-    load_k(ca, cb);
-    load_v(ca, cb);
-    for (; st < end; st += NW) {
-      const Chunk na = resolve(ea), nb_ = resolve(eb);
-      ea = fetch(2 * (st + 2 * NW));
-      eb = fetch(2 * (st + 2 * NW) + 1);
-      step(ca, cb, na, nb_, st + NW < end);
-      ca = na;
-      cb = nb_;
+  // Wave w takes steps begin + w, begin + w + NW, ...
+  if constexpr (PAGES) {
+    constexpr int CPS = 2 * ((BLK + 1023) / 1024);  // copies per step
+    Step queue[NS];                                 // the steps in flight, then the next
+#pragma unroll
+    for (int k = 0; k < NS; ++k) {
+      queue[k] = fetch(begin + wave + k * NW);
+      if (queue[k].i < end) copy_step(queue[k], k);
+    }
+    Step next = fetch(begin + wave + NS * NW);
+    load_q();  // (behind the first copies, which take longer)
+    int stage = 0;
+#pragma unroll 1
+    for (int32_t round = begin; round < end; round += NW) {
+      if (queue[0].i >= end) continue;
+      // this step's copies are the oldest: wait until no more than the later steps' are left
+      if (queue[NS - 1].i < end) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * CPS) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      const Step e = queue[0];
+      read_k(stage);
+      step(e, [&]() __attribute__((always_inline)) {
+        read_v(stage);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the stage is filled again
+        if (next.i < end) copy_step(next, stage);
+#pragma unroll
+        for (int k = 0; k + 1 < NS; ++k) queue[k] = queue[k + 1];
+        queue[NS - 1] = next;
+        next = fetch(next.i + NW);
+      });
+      stage = stage + 1 == NS ? 0 : stage + 1;
+    }
+    __syncthreads();  // every wave has read its ring: the sums take its place
+  } else {
+    Step e = fetch(begin + wave), next = fetch(begin + wave + NW);
+    if (e.i < end) {
+      load_k(e);
+      load_v(e);
+    }
+    load_q();
+    while (e.i < end) {
+      const Step after = fetch(next.i + NW);
+      step(e, [&]() __attribute__((always_inline)) {
+        if (next.i < end) load_k(next);
+      });
+      if (next.i < end) load_v(next);
+      e = next;
+      next = after;
+    }
+  }
+
+  if (__any(odd != 0)) {
+    // Rows that see an inf or NaN of V have inf or NaN in its column whatever
+    // its weight; a lane looks through its quarter of the dims.
+#pragma unroll 1
+    for (int32_t i = begin + wave; i < end; i += NW) {
+      if (i >= full0 && i < full1) continue;  // (a whole chunk there is unlinked: all zeros)
+      const Step e = fetch(i);
+#pragma unroll 1
+      for (int tk = 0; tk < 32; ++tk) {
+        const int32_t phys = tk < 16 ? e.a : e.b, lc = logical(2 * i + (tk >> 4)), t = tk & 15, key = 16 * lc + t;
+        if (!mapped(phys) || key >= kv_lim) continue;
+        const int64_t at = offset_of(phys, lc);
+#pragma unroll
+        for (int d = 0; d < D / 4; ++d) {
+          const int dim = (D / 4) * g + d;
+          float y;
+          if constexpr (PAGES) {
+            const uint8_t *blk = kbase + at;
+            const half_t sv = reinterpret_cast<const half_t *>(blk + f.vscales)[f.scale_idx(t, dim / 64)];
+            y = ((float)((blk[f.vcodes + f.v_byte(t, dim)] >> (4 * (dim & 1))) & 15) - 8.0f) * (float)sv;
+          } else {
+            y = (float)reinterpret_cast<const half_t *>(vbase + at + (int64_t)t * p.kv_ts)[dim];
+          }
+          const bool bad = (__float_as_uint(y) & 0x7F800000u) == 0x7F800000u;
+#pragma unroll
+          for (int qb = 0; qb < QB; ++qb)
+            if (bad && key <= row_pos[qb] && (key < p.sinks || key >= row_pos[qb] - p.W + 1)) o[qb][d % ND][d / ND] += y;
+        }
+      }
     }
   }
 
@@ -585,6 +710,7 @@ __global__ __launch_bounds__(256, QB == 1 ? (FMT == MEMOPT_KV_INT4 || D == 64 ? 
   for (int qb = 0; qb < QB; ++qb) {
     const float l = xor32_sum(xor16_sum(lsum[qb]));
     const int row = 16 * qb + r;
+    if (row0 + row >= rows) continue;
 #pragma unroll
     for (int reg = 0; reg < 4; ++reg)
 #pragma unroll
@@ -598,10 +724,12 @@ __global__ __launch_bounds__(256, QB == 1 ? (FMT == MEMOPT_KV_INT4 || D == 64 ? 
   }
   __syncthreads();
   // A block whose steps lie in one run is finished here.
-  const int32_t w0 = wg_of(block_at), w1 = wg_of(block_at + seq.steps - 1), live = min(QN, rows - row0);
+  const int32_t w0 = block_at >= first ? wg : wg_of(block_at);
+  const int32_t w1 = block_at + seq.steps <= stop ? wg : wg_of(block_at + seq.steps - 1);
+  const int32_t live = min(QN, rows - row0);
   auto write_row = [&](int row, int d, f32x4_t x, float l) __attribute__((always_inline)) {
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    const int32_t rr = row0 + row, tok = rr / p.G;
+    const int32_t rr = row0 + row, tok = p.by_g(rr);
     *reinterpret_cast<u32x2_t *>(p.out + (int64_t)(seq.start + tok) * p.o_ts +
                                  (int64_t)(kvh * p.G + rr - tok * p.G) * p.o_hs + d) =
         u32x2_t{as_u32(half2_t{(half_t)(x[0] * inv), (half_t)(x[1] * inv)}),
@@ -650,8 +778,9 @@ __global__ __launch_bounds__(256, QB == 1 ? (FMT == MEMOPT_KV_INT4 || D == 64 ? 
     }
     __syncthreads();
     if (s_last) {
-      // Weights of the partials, row by row (a wave per row), in s_o; the row's
-      // sum in s_ml. Then each thread adds four dims of a row over them.
+      // Weights of the partials, row by row (a wave per row), in LDS; the row's
+      // sum in s_ml. Then the partials are dealt to parts of the workgroup, four
+      // dims of a row per thread, loads first; the parts' sums meet in LDS.
       auto load2 = [&](const float *src) __attribute__((always_inline)) {
         const u32x2_t u = __builtin_bit_cast(
             u32x2_t, __hip_atomic_load(reinterpret_cast<const uint64_t *>(src), __ATOMIC_RELAXED,
@@ -659,44 +788,63 @@ __global__ __launch_bounds__(256, QB == 1 ? (FMT == MEMOPT_KV_INT4 || D == 64 ? 
         return float2{__uint_as_float(u[0]), __uint_as_float(u[1])};
       };
       const int32_t parts = w1 - w0 + 1;
-      float *wgt = &s_o[0][0][0];
-      constexpr int WS = NW * OS;  // weights of a row
-      for (int row = wave; row < live; row += NW) {
-        float mx = -INFINITY, l = 0.0f;
-        for (int32_t i = lane; i < parts; i += 64) {
-          const float2 ml = load2(p.ws_ml + 2 * (partial_slot(w0 + i) * QN + row));
-          wgt[row * WS + i] = ml.x;
-          mx = fmaxf(mx, ml.x);
-        }
-        mx = wave_max(mx);
-        for (int32_t i = lane; i < parts; i += 64) {
-          const float m = wgt[row * WS + i], f = m == -INFINITY ? 0.0f : fast_exp2(m - mx);
-          wgt[row * WS + i] = f;
-          l += f * load2(p.ws_ml + 2 * (partial_slot(w0 + i) * QN + row)).y;
-        }
+      float *const wgt = reinterpret_cast<float *>(smem);
+      f32x4_t *const sums = reinterpret_cast<f32x4_t *>(smem + QN * kMaxParts * 4);
+      const int32_t cells = live * (D / 4), groups = max(1, NT / cells);
+      constexpr int R = 8;
+      float2 y[R][2];
+      auto load_parts = [&](int32_t i0, int row, int d) __attribute__((always_inline)) {
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) l += shfl_xor(l, off);
-        if (lane == 0) s_ml[0][row][1] = l;
-      }
-      __syncthreads();
-      for (int idx = tid; idx < live * (D / 4); idx += NT) {
-        const int row = idx / (D / 4), d = 4 * (idx % (D / 4));
-        f32x4_t x = {};
-        for (int32_t i0 = 0; i0 < parts; i0 += 8) {
-          float2 y[8][2];
+        for (int k = 0; k < R; ++k) {
+          const float *src = p.ws_o + (partial_slot(w0 + min(i0 + k * groups, parts - 1)) * QN + row) * D + d;
+          y[k][0] = load2(src);
+          y[k][1] = load2(src + 2);
+        }
+      };
+      for (int c0 = 0; c0 < cells; c0 += NT) {  // (once where the cells fit the workgroup)
+        const int cell = groups > 1 ? tid % cells : c0 + tid, part = groups > 1 ? tid / cells : 0;
+        const bool on = cell < cells && part < groups;
+        const int row = on ? cell / (D / 4) : 0, d = 4 * (cell % (D / 4));
+        load_parts(part, row, d);  // in flight while the weights are computed
+        if (c0 == 0) {
+          for (int row = wave; row < live; row += NW) {
+            float m[kMaxParts / 64], l[kMaxParts / 64], mx = -INFINITY, lt = 0.0f;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float *src = p.ws_o + (partial_slot(w0 + min(i0 + k, parts - 1)) * QN + row) * D + d;
-            y[k][0] = load2(src);
-            y[k][1] = load2(src + 2);
+            for (int i = 0; i < kMaxParts / 64; ++i) {
+              const int32_t w = lane + 64 * i;
+              const float2 ml = load2(p.ws_ml + 2 * (partial_slot(w0 + min(w, parts - 1)) * QN + row));
+              m[i] = w < parts ? ml.x : -INFINITY;
+              l[i] = ml.y;
+              mx = fmaxf(mx, m[i]);
+            }
+            mx = wave_max(mx);
+#pragma unroll
+            for (int i = 0; i < kMaxParts / 64; ++i) {
+              const float f = m[i] == -INFINITY ? 0.0f : fast_exp2(m[i] - mx);
+              lt += f * l[i];
+              if (lane + 64 * i < parts) wgt[row * kMaxParts + lane + 64 * i] = f;
+            }
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) lt += shfl_xor(lt, off);
+            if (lane == 0) s_ml[0][row][1] = lt;
           }
+          __syncthreads();
+        }
+        f32x4_t x = {};
+        for (int32_t i0 = part; i0 < parts && on; i0 += R * groups) {
+          if (i0 != part) load_parts(i0, row, d);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float f = i0 + k < parts ? wgt[row * WS + i0 + k] : 0.0f;
+          for (int k = 0; k < R; ++k) {
+            const float f = i0 + k * groups < parts ? wgt[row * kMaxParts + i0 + k * groups] : 0.0f;
             x += f32x4_t{y[k][0].x, y[k][0].y, y[k][1].x, y[k][1].y} * f;
           }
         }
-        write_row(row, d, x, s_ml[0][row][1]);
+        if (groups > 1) {
+          sums[tid] = x;
+          __syncthreads();
+          for (int k = 1; k < groups && part == 0 && on; ++k) x += sums[tid + k * cells];
+        }
+        if (on && part == 0) write_row(row, d, x, s_ml[0][row][1]);
       }
     }
   }
@@ -704,9 +852,14 @@ __global__ __launch_bounds__(256, QB == 1 ? (FMT == MEMOPT_KV_INT4 || D == 64 ? 
   }
 }
 
+// Steps (32 tokens) that a block can need.
+static int64_t packed_steps(const memopt_packed_desc &d) {
+  return ((int64_t)d.max_blocks_per_seq * d.block_size + 31) / 32;
+}
+
 // Query rows per block: 16 where a sequence has no more than that.
 struct PackedPlan {
-  int32_t qn, wgs;
+  int32_t qn, waves, wgs;
   int64_t blocks;  // at most this many
 };
 
@@ -716,15 +869,22 @@ static PackedPlan packed_plan(const memopt_packed_desc &d) {
   pl.qn = most <= 16 ? 16 : 32;
   // sum over the sequences of ceil(rows / qn)
   pl.blocks = (d.tokens * G + (int64_t)(pl.qn - 1) * std::min(d.batch, d.tokens)) / pl.qn;
-  const int64_t resident = pl.qn == 16 && (d.kv_format == MEMOPT_KV_INT4 || d.head_dim == 64) ? 3 : 2;
-  pl.wgs = (int32_t)std::max<int64_t>(1, std::min<int64_t>(resident * compute_units() / d.num_kv_heads,
-                                                           max_workgroups(d.head_dim)));
+  // Workgroups of 4 waves, three to a CU: they hide each other's starts and
+  // ends. Where a sequence would fall to more than 24 of them, its last
+  // workgroup adds up as many partial sums one round trip after another: there
+  // 12 waves in one workgroup per CU leave a third as many (one sequence of
+  // 131072 tokens x 8 key heads: 42.0 us, now 35.4; 32 sequences of 2700 to
+  // 8192: 47.9 with 4 waves, 51.9 with 12; one of 1024: 8.7 and 11.6). fp16
+  // rows take their registers from the ring's share: 8 waves, one workgroup.
+  auto wgs = [&](int waves) {
+    const int64_t n = (int64_t)resident(waves, pl.qn / 16) * compute_units() / d.num_kv_heads;
+    return (int32_t)std::max<int64_t>(1, std::min<int64_t>(n, kMaxParts));
+  };
+  pl.waves = pl.qn == 32 ? 4 : d.kv_format == MEMOPT_KV_FP16 ? 8 : 4;
+  if (pl.waves == 4 && pl.qn == 16 && std::min<int64_t>(wgs(4), packed_steps(d) * d.batch / 4) > 24LL * d.batch)
+    pl.waves = 12;
+  pl.wgs = wgs(pl.waves);
   return pl;
-}
-
-// Steps (32 tokens) that a block can need.
-static int64_t packed_steps(const memopt_packed_desc &d) {
-  return ((int64_t)d.max_blocks_per_seq * d.block_size + 31) / 32;
 }
 
 struct PackedWorkspace {
@@ -762,11 +922,21 @@ static int validate_packed(const memopt_packed_desc &d) {
   return MEMOPT_OK;
 }
 
-template <int D, int FMT>
-static void launch_packed(const PackedParams &p, int qn, hipStream_t stream) {
-  const dim3 grid((unsigned)((int64_t)p.wgs * p.Hk));
-  if (qn == 16) hipLaunchKernelGGL((packed_kernel<D, FMT, 1>), grid, dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((packed_kernel<D, FMT, 2>), grid, dim3(256), 0, stream, p);
+template <int D, int FMT, int QB, int NW>
+static void launch_packed(const PackedParams &p, const memopt_packed_desc &d, hipStream_t stream) {
+  hipLaunchKernelGGL((packed_kernel<D, FMT, QB, NW>), dim3((unsigned)((int64_t)p.wgs * p.Hk)), dim3(64 * NW), 0, stream,
+                     p, d.query_starts, d.context_lens, d.block_tables);
+}
+template <int D>
+static void launch_packed(const PackedParams &p, const memopt_packed_desc &d, const PackedPlan &pl, hipStream_t s) {
+  if (d.kv_format == MEMOPT_KV_INT4) {
+    if (pl.qn == 32) launch_packed<D, MEMOPT_KV_INT4, 2, 4>(p, d, s);
+    else if (pl.waves == 12) launch_packed<D, MEMOPT_KV_INT4, 1, 12>(p, d, s);
+    else launch_packed<D, MEMOPT_KV_INT4, 1, 4>(p, d, s);
+  } else {
+    if (pl.qn == 32) launch_packed<D, MEMOPT_KV_FP16, 2, 4>(p, d, s);
+    else launch_packed<D, MEMOPT_KV_FP16, 1, 8>(p, d, s);
+  }
 }
 
 }  // namespace memopt
@@ -805,14 +975,13 @@ extern "C" int memopt_packed_attention(const memopt_packed_desc *desc, void *str
   p.q_hs = d.q_head_stride;
   p.o_ts = d.o_token_stride;
   p.o_hs = d.o_head_stride;
-  p.cu = d.query_starts;
-  p.ctx = d.context_lens;
-  p.bt = d.block_tables;
   p.T = d.tokens;
   p.B = d.batch;
   p.Hq = d.num_heads;
   p.Hk = d.num_kv_heads;
   p.G = d.num_heads / d.num_kv_heads;
+  p.by_g = Divisor::of((uint32_t)p.G);
+  p.span = pl.qn / p.G + 1;
   p.M = d.max_blocks_per_seq;
   p.bs = d.block_size;
   p.nb = d.num_kv_blocks;
@@ -835,12 +1004,7 @@ extern "C" int memopt_packed_attention(const memopt_packed_desc *desc, void *str
   p.ws_o = (float *)((uint8_t *)d.workspace + w.counters);
   p.ws_ml = (float *)((uint8_t *)d.workspace + w.ml);
   hipStream_t s = (hipStream_t)stream;
-  if (d.head_dim == 128) {
-    if (d.kv_format == MEMOPT_KV_INT4) launch_packed<128, MEMOPT_KV_INT4>(p, pl.qn, s);
-    else launch_packed<128, MEMOPT_KV_FP16>(p, pl.qn, s);
-  } else {
-    if (d.kv_format == MEMOPT_KV_INT4) launch_packed<64, MEMOPT_KV_INT4>(p, pl.qn, s);
-    else launch_packed<64, MEMOPT_KV_FP16>(p, pl.qn, s);
-  }
+  if (d.head_dim == 128) launch_packed<128>(p, d, pl, s);
+  else launch_packed<64>(p, d, pl, s);
   return check_launch("packed_attention");
 }

@@ -170,7 +170,7 @@ __device__ __forceinline__ uint32_t tame(uint32_t w, uint32_t &odd) {
   typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
   constexpr unsigned short most = (unsigned short)(E::kExponent - 1);
   const u16x2 m = __builtin_elementwise_min(__builtin_bit_cast(u16x2, w & 0x7FFF7FFFu), u16x2{most, most});
-  const uint32_t y = bfi(0x7FFF7FFFu, __builtin_bit_cast(uint32_t, m), w);
+  const uint32_t y = (w & 0x80008000u) | __builtin_bit_cast(uint32_t, m);
   odd |= y ^ w;
   return y;
 }
