@@ -14,6 +14,11 @@
 // block of 16 rows fills a matrix instruction that a lone query head would
 // leave 15/16 empty. Every cached byte is read once per block of rows.
 //
+// Long chunks: enough of them to fill the GPU with 128-row tiles attend from a
+// staged copy of what they see instead (stage_kernel here, then the tiles of
+// prompt.hip): a block of 32 rows unpacks each page once more, and from 512
+// rows on that costs more than writing the copy. What follows is the rest.
+//
 // Work: QN = 16 * QB rows of one (sequence, key head) are a block; a wave takes
 // two 16-token chunks (32 tokens) of a block's visible ones per step. The steps
 // of all blocks of a key head form one list, which is dealt to its workgroups
@@ -32,11 +37,19 @@
 //    their lane, and a page's V word unpacks into one register of four
 //    operands.
 // Output row rr of V^T product i is dim (D / 16) rr + i.
+//
+// Bound by vector instructions: about 200 per step of 32 tokens and 16 rows
+// (D = 128, INT4), four cycles each, most of them the unpacking of V; a copy
+// without them streams 131072 tokens of 8 key heads in 18 us, the kernel takes
+// 35. 32 sequences of 2700 to 8192 tokens, 32 query over 8 key heads: 48 us, 4.1
+// TB/s of pages; one of 131072: 35 us, 4.0 TB/s. A card's large copy reaches
+// 5.1.
 #include <algorithm>
 #include <cmath>
 
 #include "attention.hpp"
 #include "lds_dma.hpp"
+#include "packed.hpp"
 #include "page_format.hpp"
 
 namespace memopt {
@@ -45,22 +58,6 @@ typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
-
-// x / d for 0 <= x < 2^31 by a product: with 2^l >= d and m = floor(2^(31 + l)
-// / d) + 1, floor(m x / 2^(31 + l)) = floor(x / d) (the classic round-up
-// multiplier; a division takes some 25 vector instructions, and a workgroup
-// that takes ten steps per wave felt them).
-struct Divisor {
-  uint32_t d, mul, shift;
-  static Divisor of(uint32_t d) {
-    uint32_t l = 0;
-    while ((1ull << l) < d) ++l;
-    return {d, d > 1 ? (uint32_t)((1ull << (31 + l)) / d + 1) : 0, l > 0 ? l - 1 : 0};
-  }
-  __device__ __forceinline__ int32_t operator()(int32_t x) const {
-    return d == 1 ? x : (int32_t)(__umulhi((uint32_t)x, mul) >> shift);
-  }
-};
 
 struct PackedParams {
   const half_t *q;
@@ -77,6 +74,7 @@ struct PackedParams {
   int32_t wgs, blocks;           // workgroups per key head; blocks that ws_cnt has counters for
   uint32_t *ws_cnt;              // [blocks * Hk] arrivals; zero between calls
   float *ws_o, *ws_ml;           // [2 * wgs * Hk][QN][D], [2 * wgs * Hk][QN][2]: see partial_slot
+  Staged st;                     // sequences that attend from a staged copy instead
 };
 
 // Workgroups per key head, so partial sums of a block, at most (their weights
@@ -123,11 +121,12 @@ template <int QN>
 __device__ __forceinline__ Seq sequence(const PackedParams &p, const int32_t *__restrict__ starts,
                                         const int32_t *__restrict__ ctxs, int32_t b) {
   Seq q;
-  q.start = min(max(starts[b], 0), p.T);
-  q.n = min(max(starts[b + 1], q.start), p.T) - q.start;
+  const Rows rows = rows_of(starts, p.T, b);
+  q.start = rows.start;
+  q.n = rows.n;
   q.ctx = ctxs[b];
   q.kv_lim = (int32_t)min((int64_t)q.ctx, (int64_t)p.M * p.bs);
-  q.blocks = (q.n * p.G + QN - 1) / QN;
+  q.blocks = is_staged(p.st, q.n, p.G) ? 0 : (q.n * p.G + QN - 1) / QN;
   const int32_t pos0 = q.ctx - q.n;
   int32_t n = visible_chunks(p, q.kv_lim, pos0, q.ctx - 1).n;
   if (q.blocks > 1) n = min(n, ((min(p.sinks, max(q.kv_lim, 0)) + 15) >> 4) + ((p.W + p.span) >> 4) + 2);
@@ -254,601 +253,726 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
   // Block by block of this workgroup's run.
   Seq seq = sequence<QN>(p, starts, ctxs, b);
   while (at < stop) {
-  while (at >= seq_at + seq.blocks * seq.steps) {  // (sequences without rows take no place)
-    seq_at += seq.blocks * seq.steps;
-    seq_blocks += seq.blocks;
-    seq = sequence<QN>(p, starts, ctxs, ++b);
-  }
-  const int32_t block = seq.blocks == 1 ? 0 : (at - seq_at) / seq.steps;
-  if (seq_blocks + block >= p.blocks) return;  // sequences overlap: past the counters
-  const int32_t block_at = seq_at + block * seq.steps;
-  const int32_t row0 = block * QN, rows = seq.n * p.G, ctx = seq.ctx, kv_lim = seq.kv_lim;
-  const int32_t pos0 = ctx - seq.n;  // position of the sequence's first query
-  const int32_t pos_lo = pos0 + p.by_g(row0), pos_hi = pos0 + p.by_g(min(row0 + QN, rows) - 1);
-  const Visible vis = visible_chunks(p, kv_lim, pos_lo, pos_hi);
-  const int32_t sc = vis.sc, wc0 = vis.wc0, n_vis = vis.n;
-  const int32_t begin = at - block_at, end = min(min(stop - block_at, seq.steps), (n_vis + 1) >> 1);
-  at = min(stop, block_at + seq.steps);
-
-  f32x4_t o[QB][ND];
-  float ncm[QB], thr[QB], lsum[QB];
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-#pragma unroll
-    for (int i = 0; i < ND; ++i) o[qb][i] = (f32x4_t){};
-    ncm[qb] = 0.0f;
-    thr[qb] = -INFINITY;
-    lsum[qb] = 0.0f;
-  }
-
-  // Chunk i of the visible list is logical chunk i, or i + skip behind the
-  // sinks. A step is the chunks 2 i and 2 i + 1; those of steps [full0, full1)
-  // lie where every row sees all their tokens, so they need no mask once both
-  // pages are there.
-  const int32_t *btrow = tables + (int64_t)b * p.M;
-  const int32_t cpp = PAGES ? 1 : p.bs >> 4;
-  const int32_t nb32 = (int32_t)min(p.nb, (int64_t)INT32_MAX);
-  const int32_t skip = wc0 - sc;
-  auto logical = [&](int32_t i) { return i + (i < sc ? 0 : skip); };
-  const int32_t full0 = (max(skip > 0 ? sc : 0, ((max(0, pos_hi - p.W + 1) + 15) >> 4) - skip) + 1) >> 1;
-  const int32_t full1 = ((max(0, min(kv_lim, pos_lo + 1)) >> 4) - skip) >> 1;
-  struct Step {  // its block-table entries, not yet waited for
-    int32_t i, a, b;
-  };
-  auto fetch = [&](int32_t i) __attribute__((always_inline)) {
-    Step e;
-    e.i = i;
-    const int32_t ca = 2 * i, cb = 2 * i + 1;
-    const int32_t la = ca < n_vis ? logical(ca) : 0, lb = cb < n_vis ? logical(cb) : 0;  // (a row has an entry 0)
-    e.a = btrow[cpp == 1 ? la : la / cpp];
-    e.b = btrow[cpp == 1 ? lb : lb / cpp];
-    if (cb >= n_vis) e.b = -1;
-    return e;
-  };
-  auto mapped = [&](int32_t phys) { return phys >= 0 && phys < nb32; };
-  // Byte offset of chunk `lc` (chunk 0 of page 0, always mapped, if its page is not).
-  auto offset_of = [&](int32_t phys, int32_t lc) __attribute__((always_inline)) {
-    const bool ok = mapped(phys);
-    int64_t x = (int64_t)(ok ? phys : 0) * p.kv_ps;
-    if constexpr (!PAGES) x += (int64_t)(ok ? 16 * (lc - lc / cpp * cpp) : 0) * p.kv_ts;
-    return x;
-  };
-
-  const Int4Page f(D);
-  PackedK<D, FMT> kr;
-  PackedV<D, FMT> vr;
-  const int p0 = 4 * (g & 1);  // this lane's score tokens: p0 + i and p0 + i + 8 of chunk g / 2
-  // Pages: the two blocks of a step as they are, 1 KiB per copy, straight into
-  // the wave's ring: kRingSteps steps are in flight without holding registers.
-  const uint32_t ring = lds_u32(smem) + wave * NS * STG;
-  const uint8_t *const kbase = p.k + (int64_t)kvh * p.kv_hs, *const vbase = p.v + (int64_t)kvh * p.kv_hs;
-  auto copy_block = [&](int64_t kv, uint32_t dst) __attribute__((always_inline)) {
-    const __amdgpu_buffer_rsrc_t rs =
-        __builtin_amdgcn_make_buffer_rsrc((void *)(kbase + kv), (short)0, BLK, 0x00020000);
-    constexpr int TAIL = BLK / 1024 * 1024;
-    ring_copy<QB == 1, 0>(rs, dst, 16 * lane);
-    if constexpr (D == 128) ring_copy<QB == 1, 1024>(rs, dst, 16 * lane);
-    if (lane < (BLK - TAIL) / 16) ring_copy<QB == 1, TAIL>(rs, dst, 16 * lane);
-  };
-  auto copy_step = [&](const Step &e, int stage) __attribute__((always_inline)) {
-    copy_block(offset_of(e.a, 0), ring + stage * STG);
-    copy_block(offset_of(e.b, 0), ring + stage * STG + BLK);
-  };
-  // K of a step: lane row r is tokens r % 8 and r % 8 + 8 of chunk r / 8.
-  // V: lane (r, g) holds dims [D/16 r, D/16 (r + 1)) of its score tokens.
-  auto read_k = [&](int stage) __attribute__((always_inline)) {
-    if constexpr (PAGES) {
-      const uint32_t at = ring + stage * STG;
-      const uint32_t kb = at + (r < 8 ? 0 : BLK) + (uint32_t)f.kcodes + (8 * (r & 7) + (D == 128 ? g : 2 * g)) * (D / 8);
-      const uint32_t tb = at + (g < 2 ? 0 : BLK);
-#pragma unroll
-      for (int j = 0; j < D / 64; ++j) {
-        // (D = 128: lane group 4 j + g of the page, 16 dims of scale group j; D = 64: groups 2 g and 2 g + 1)
-        const u32x4_t x = lds_at<u32x4_t>(kb + 4 * j * (D / 8));
-#pragma unroll
-        for (int w = 0; w < 4; ++w) kr.w[4 * j + w] = x[w];
-        kr.sc[j] = lds_at<u32x4_t>(tb + (uint32_t)f.kscales + 2 * (16 * j + 2 * p0));
-      }
+    while (at >= seq_at + seq.blocks * seq.steps) {  // (sequences without rows take no place)
+      seq_at += seq.blocks * seq.steps;
+      seq_blocks += seq.blocks;
+      seq = sequence<QN>(p, starts, ctxs, ++b);
     }
-  };
-  auto read_v = [&](int stage) __attribute__((always_inline)) {
-    if constexpr (PAGES) {
-      const uint32_t tb = ring + stage * STG + (g < 2 ? 0 : BLK);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t src = tb + (uint32_t)f.vcodes + 8 * (p0 + i) * (D / 8) + (D / 16) * r;
-        if constexpr (D == 128) {
-          const u32x2_t x = lds_at<u32x2_t>(src);
-          vr.w[i][0] = x[0];
-          vr.w[i][1] = x[1];
-        } else {
-          vr.w[i][0] = lds_at<uint32_t>(src);
-        }
-      }
-      vr.sc = lds_at<u32x4_t>(tb + (uint32_t)f.vscales + 2 * ((r * (D / 16) / 64) * 16 + 2 * p0));
-    }
-  };
-  // fp16 pools: the same from global memory into registers.
-  auto load_k = [&](const Step &e) __attribute__((always_inline)) {
-    if constexpr (!PAGES) {
-      const uint8_t *base = kbase + (r < 8 ? offset_of(e.a, logical(2 * e.i)) : offset_of(e.b, logical(2 * e.i + 1)));
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk)
-          kr.w[t][kk] = *reinterpret_cast<const u32x4_t *>(base + (int64_t)((r & 7) + 8 * t) * p.kv_ts +
-                                                           2 * (32 * kk + 8 * g));
-    }
-  };
-  auto load_v = [&](const Step &e) __attribute__((always_inline)) {
-    if constexpr (!PAGES) {
-      const uint8_t *base = vbase + (g < 2 ? offset_of(e.a, logical(2 * e.i)) : offset_of(e.b, logical(2 * e.i + 1)));
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {  // element 2 i + t: token p0 + i + 8 t
-        const uint8_t *src = base + (int64_t)(p0 + (x >> 1) + 8 * (x & 1)) * p.kv_ts + (D / 8) * r;
-        if constexpr (D == 128) {
-          const u32x4_t y = *reinterpret_cast<const u32x4_t *>(src);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) vr.w[x][j] = y[j];
-        } else {
-          const u32x2_t y = *reinterpret_cast<const u32x2_t *>(src);
-          vr.w[x][0] = y[0];
-          vr.w[x][1] = y[1];
-        }
-      }
-    }
-  };
+    const int32_t block = seq.blocks == 1 ? 0 : (at - seq_at) / seq.steps;
+    if (seq_blocks + block >= p.blocks) return;  // sequences overlap: past the counters
+    const int32_t block_at = seq_at + block * seq.steps;
+    const int32_t row0 = block * QN, rows = seq.n * p.G, ctx = seq.ctx, kv_lim = seq.kv_lim;
+    const int32_t pos0 = ctx - seq.n;  // position of the sequence's first query
+    const int32_t pos_lo = pos0 + p.by_g(row0), pos_hi = pos0 + p.by_g(min(row0 + QN, rows) - 1);
+    const Visible vis = visible_chunks(p, kv_lim, pos_lo, pos_hi);
+    const int32_t sc = vis.sc, wc0 = vis.wc0, n_vis = vis.n;
+    const int32_t begin = at - block_at, end = min(min(stop - block_at, seq.steps), (n_vis + 1) >> 1);
+    at = min(stop, block_at + seq.steps);
 
-  // (w & mask) | bits as one v_and_or_b32: the constants are hidden from the
-  // compiler, which would make two instructions of them. (As inline assembly,
-  // the instruction escapes the compiler's wait states: one that overwrote
-  // the start of a sum while its matrix instruction still read it gave NaN.)
-  uint32_t m_lo = 0x000F000Fu, m_hi = 0x00F000F0u, e1024 = 0x64006400u, e64 = 0x54005400u;
-  asm("" : "+s"(m_lo), "+s"(m_hi));
-  asm("" : "+v"(e1024), "+v"(e64));
-  const half2_t b1032 = {(half_t)1032.0f, (half_t)1032.0f}, b72 = {(half_t)72.0f, (half_t)72.0f};
-  // The eight codes of a word, less 8, in nibble-unpack order (exact).
-  auto codes = [&](uint32_t w) __attribute__((always_inline)) {
-    const uint32_t w8 = w >> 8;
-    return u32x4_t{as_u32(as_half2((w & m_lo) | e1024) - b1032), as_u32(as_half2((w & m_hi) | e64) - b72),
-                   as_u32(as_half2((w8 & m_lo) | e1024) - b1032), as_u32(as_half2((w8 & m_hi) | e64) - b72)};
-  };
-  // The same without the subtractions, so plus 1032 in the even pairs and 72
-  // in the odd ones: K's sums start at minus those times the sums of q
-  // (kstart). Their 32-bit roundings grow to about 2^-24 * 1032 of the sum of
-  // |q| * scale, a tenth of what rounding K to fp16 would cost, and far below
-  // the rounding of the probabilities.
-  auto biased = [&](uint32_t w) __attribute__((always_inline)) {
-    const uint32_t w8 = w >> 8;
-    return u32x4_t{(w & m_lo) | e1024, (w & m_hi) | e64, (w8 & m_lo) | e1024, (w8 & m_hi) | e64};
-  };
-  const half2_t ones = {(half_t)1.0f, (half_t)1.0f};
-  h8_t qf[QB][KK];
-  f32x4_t kstart[QB][NG];
-  int32_t row_pos[QB];
-  auto load_q = [&]() __attribute__((always_inline)) {
-    // Q as the B operand: column r = row, k-group g; dims of product kk as the K
-    // operand holds them (pages: 16 g + 8 (kk % 2) of scale group kk / 2, in
-    // nibble-unpack order; fp16: 32 kk + 8 g).
+    f32x4_t o[QB][ND];
+    float ncm[QB], thr[QB], lsum[QB];
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
-      const int32_t row = row0 + 16 * qb + r, tok = p.by_g(row);
-      row_pos[qb] = pos0 + tok;
+#pragma unroll
+      for (int i = 0; i < ND; ++i) o[qb][i] = (f32x4_t){};
+      ncm[qb] = 0.0f;
+      thr[qb] = -INFINITY;
+      lsum[qb] = 0.0f;
+    }
+
+    // Chunk i of the visible list is logical chunk i, or i + skip behind the
+    // sinks. A step is the chunks 2 i and 2 i + 1; those of steps [full0, full1)
+    // lie where every row sees all their tokens, so they need no mask once both
+    // pages are there.
+    const int32_t *btrow = tables + (int64_t)b * p.M;
+    const int32_t cpp = PAGES ? 1 : p.bs >> 4;
+    const int32_t nb32 = (int32_t)min(p.nb, (int64_t)INT32_MAX);
+    const int32_t skip = wc0 - sc;
+    auto logical = [&](int32_t i) { return i + (i < sc ? 0 : skip); };
+    const int32_t full0 = (max(skip > 0 ? sc : 0, ((max(0, pos_hi - p.W + 1) + 15) >> 4) - skip) + 1) >> 1;
+    const int32_t full1 = ((max(0, min(kv_lim, pos_lo + 1)) >> 4) - skip) >> 1;
+    struct Step {  // its block-table entries, not yet waited for
+      int32_t i, a, b;
+    };
+    auto fetch = [&](int32_t i) __attribute__((always_inline)) {
+      Step e;
+      e.i = i;
+      const int32_t ca = 2 * i, cb = 2 * i + 1;
+      const int32_t la = ca < n_vis ? logical(ca) : 0, lb = cb < n_vis ? logical(cb) : 0;  // (a row has an entry 0)
+      e.a = btrow[cpp == 1 ? la : la / cpp];
+      e.b = btrow[cpp == 1 ? lb : lb / cpp];
+      if (cb >= n_vis) e.b = -1;
+      return e;
+    };
+    auto mapped = [&](int32_t phys) { return phys >= 0 && phys < nb32; };
+    // Byte offset of chunk `lc` (chunk 0 of page 0, always mapped, if its page is not).
+    auto offset_of = [&](int32_t phys, int32_t lc) __attribute__((always_inline)) {
+      const bool ok = mapped(phys);
+      int64_t x = (int64_t)(ok ? phys : 0) * p.kv_ps;
+      if constexpr (!PAGES) x += (int64_t)(ok ? 16 * (lc - lc / cpp * cpp) : 0) * p.kv_ts;
+      return x;
+    };
+
+    const Int4Page f(D);
+    PackedK<D, FMT> kr;
+    PackedV<D, FMT> vr;
+    const int p0 = 4 * (g & 1);  // this lane's score tokens: p0 + i and p0 + i + 8 of chunk g / 2
+    // Pages: the two blocks of a step as they are, 1 KiB per copy, straight into
+    // the wave's ring: kRingSteps steps are in flight without holding registers.
+    const uint32_t ring = lds_u32(smem) + wave * NS * STG;
+    const uint8_t *const kbase = p.k + (int64_t)kvh * p.kv_hs, *const vbase = p.v + (int64_t)kvh * p.kv_hs;
+    auto copy_block = [&](int64_t kv, uint32_t dst) __attribute__((always_inline)) {
+      const __amdgpu_buffer_rsrc_t rs =
+          __builtin_amdgcn_make_buffer_rsrc((void *)(kbase + kv), (short)0, BLK, 0x00020000);
+      constexpr int TAIL = BLK / 1024 * 1024;
+      ring_copy<QB == 1, 0>(rs, dst, 16 * lane);
+      if constexpr (D == 128) ring_copy<QB == 1, 1024>(rs, dst, 16 * lane);
+      if (lane < (BLK - TAIL) / 16) ring_copy<QB == 1, TAIL>(rs, dst, 16 * lane);
+    };
+    auto copy_step = [&](const Step &e, int stage) __attribute__((always_inline)) {
+      copy_block(offset_of(e.a, 0), ring + stage * STG);
+      copy_block(offset_of(e.b, 0), ring + stage * STG + BLK);
+    };
+    // K of a step: lane row r is tokens r % 8 and r % 8 + 8 of chunk r / 8.
+    // V: lane (r, g) holds dims [D/16 r, D/16 (r + 1)) of its score tokens.
+    auto read_k = [&](int stage) __attribute__((always_inline)) {
+      if constexpr (PAGES) {
+        const uint32_t at = ring + stage * STG;
+        const uint32_t kb = at + (r < 8 ? 0 : BLK) + (uint32_t)f.kcodes + (8 * (r & 7) + (D == 128 ? g : 2 * g)) * (D / 8);
+        const uint32_t tb = at + (g < 2 ? 0 : BLK);
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) {
+          // (D = 128: lane group 4 j + g of the page, 16 dims of scale group j; D = 64: groups 2 g and 2 g + 1)
+          const u32x4_t x = lds_at<u32x4_t>(kb + 4 * j * (D / 8));
+#pragma unroll
+          for (int w = 0; w < 4; ++w) kr.w[4 * j + w] = x[w];
+          kr.sc[j] = lds_at<u32x4_t>(tb + (uint32_t)f.kscales + 2 * (16 * j + 2 * p0));
+        }
+      }
+    };
+    auto read_v = [&](int stage) __attribute__((always_inline)) {
+      if constexpr (PAGES) {
+        const uint32_t tb = ring + stage * STG + (g < 2 ? 0 : BLK);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t src = tb + (uint32_t)f.vcodes + 8 * (p0 + i) * (D / 8) + (D / 16) * r;
+          if constexpr (D == 128) {
+            const u32x2_t x = lds_at<u32x2_t>(src);
+            vr.w[i][0] = x[0];
+            vr.w[i][1] = x[1];
+          } else {
+            vr.w[i][0] = lds_at<uint32_t>(src);
+          }
+        }
+        vr.sc = lds_at<u32x4_t>(tb + (uint32_t)f.vscales + 2 * ((r * (D / 16) / 64) * 16 + 2 * p0));
+      }
+    };
+    // fp16 pools: the same from global memory into registers.
+    auto load_k = [&](const Step &e) __attribute__((always_inline)) {
+      if constexpr (!PAGES) {
+        const uint8_t *base = kbase + (r < 8 ? offset_of(e.a, logical(2 * e.i)) : offset_of(e.b, logical(2 * e.i + 1)));
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk)
+            kr.w[t][kk] = *reinterpret_cast<const u32x4_t *>(base + (int64_t)((r & 7) + 8 * t) * p.kv_ts +
+                                                             2 * (32 * kk + 8 * g));
+      }
+    };
+    auto load_v = [&](const Step &e) __attribute__((always_inline)) {
+      if constexpr (!PAGES) {
+        const uint8_t *base = vbase + (g < 2 ? offset_of(e.a, logical(2 * e.i)) : offset_of(e.b, logical(2 * e.i + 1)));
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {  // element 2 i + t: token p0 + i + 8 t
+          const uint8_t *src = base + (int64_t)(p0 + (x >> 1) + 8 * (x & 1)) * p.kv_ts + (D / 8) * r;
+          if constexpr (D == 128) {
+            const u32x4_t y = *reinterpret_cast<const u32x4_t *>(src);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) vr.w[x][j] = y[j];
+          } else {
+            const u32x2_t y = *reinterpret_cast<const u32x2_t *>(src);
+            vr.w[x][0] = y[0];
+            vr.w[x][1] = y[1];
+          }
+        }
+      }
+    };
+
+    // (w & mask) | bits as one v_and_or_b32: the constants are hidden from the
+    // compiler, which would make two instructions of them. (As inline assembly,
+    // the instruction escapes the compiler's wait states: one that overwrote
+    // the start of a sum while its matrix instruction still read it gave NaN.)
+    uint32_t m_lo = 0x000F000Fu, m_hi = 0x00F000F0u, e1024 = 0x64006400u, e64 = 0x54005400u;
+    asm("" : "+s"(m_lo), "+s"(m_hi));
+    asm("" : "+v"(e1024), "+v"(e64));
+    const half2_t b1032 = {(half_t)1032.0f, (half_t)1032.0f}, b72 = {(half_t)72.0f, (half_t)72.0f};
+    // The eight codes of a word, less 8, in nibble-unpack order (exact).
+    auto codes = [&](uint32_t w) __attribute__((always_inline)) {
+      const uint32_t w8 = w >> 8;
+      return u32x4_t{as_u32(as_half2((w & m_lo) | e1024) - b1032), as_u32(as_half2((w & m_hi) | e64) - b72),
+                     as_u32(as_half2((w8 & m_lo) | e1024) - b1032), as_u32(as_half2((w8 & m_hi) | e64) - b72)};
+    };
+    // The same without the subtractions, so plus 1032 in the even pairs and 72
+    // in the odd ones: K's sums start at minus those times the sums of q
+    // (kstart). Their 32-bit roundings grow to about 2^-24 * 1032 of the sum of
+    // |q| * scale, a tenth of what rounding K to fp16 would cost, and far below
+    // the rounding of the probabilities.
+    auto biased = [&](uint32_t w) __attribute__((always_inline)) {
+      const uint32_t w8 = w >> 8;
+      return u32x4_t{(w & m_lo) | e1024, (w & m_hi) | e64, (w8 & m_lo) | e1024, (w8 & m_hi) | e64};
+    };
+    const half2_t ones = {(half_t)1.0f, (half_t)1.0f};
+    h8_t qf[QB][KK];
+    f32x4_t kstart[QB][NG];
+    int32_t row_pos[QB];
+    auto load_q = [&]() __attribute__((always_inline)) {
+      // Q as the B operand: column r = row, k-group g; dims of product kk as the K
+      // operand holds them (pages: 16 g + 8 (kk % 2) of scale group kk / 2, in
+      // nibble-unpack order; fp16: 32 kk + 8 g).
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) {
+        const int32_t row = row0 + 16 * qb + r, tok = p.by_g(row);
+        row_pos[qb] = pos0 + tok;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          h8_t x = {};
+          if (row < rows) {
+            const int d0 = PAGES ? 64 * (kk >> 1) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g;
+            const h8_t y = __builtin_bit_cast(
+                h8_t, *reinterpret_cast<const u32x4_t *>(p.q + (int64_t)(seq.start + tok) * p.q_ts +
+                                                         (int64_t)(kvh * p.G + row - tok * p.G) * p.q_hs + d0));
+            if (PAGES) {
+              x[0] = y[0]; x[1] = y[4]; x[2] = y[1]; x[3] = y[5];
+              x[4] = y[2]; x[5] = y[6]; x[6] = y[3]; x[7] = y[7];
+            } else {
+              x = y;
+            }
+          }
+          qf[qb][kk] = x;
+        }
+      }
+
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          float x = 0.0f;
+          if constexpr (PAGES) {
+            float even = 0.0f, odd_q = 0.0f;  // operand pairs 0, 2 and 1, 3
+#pragma unroll
+            for (int kk = j * (KK / NG); kk < (j + 1) * (KK / NG); ++kk) {
+              const u32x4_t y = __builtin_bit_cast(u32x4_t, qf[qb][kk]);
+              even = __builtin_amdgcn_fdot2(as_half2(y[2]), ones, __builtin_amdgcn_fdot2(as_half2(y[0]), ones, even, false), false);
+              odd_q = __builtin_amdgcn_fdot2(as_half2(y[3]), ones, __builtin_amdgcn_fdot2(as_half2(y[1]), ones, odd_q, false), false);
+            }
+            x = xor32_sum(xor16_sum(-1032.0f * even - 72.0f * odd_q));
+          }
+          kstart[qb][j] = f32x4_t{x, x, x, x};
+        }
+    };
+    auto k_operand = [&](int t, int kk) __attribute__((always_inline)) {
+      if constexpr (PAGES) {
+        return __builtin_bit_cast(h8_t, biased(D == 128 ? kr.w[4 * (kk >> 1) + 2 * t + (kk & 1)] : kr.w[2 * kk + t]));
+      } else {
+        return __builtin_bit_cast(h8_t, kr.w[t][kk]);
+      }
+    };
+
+    // exp2 argument of a new maximum: probabilities lie in (0, 2^15], so fp16
+    // holds those down to 2^-21 of the largest as normal numbers.
+    constexpr float kTop = 7.0f;
+    uint32_t odd = 0;  // nonzero: a masked step held inf or NaN in V
+    // One step; `between` runs when K has been used and V has not.
+    auto step = [&](const Step &e, auto between) __attribute__((always_inline)) {
+      f32x4_t s[QB][NG][2];
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
-        h8_t x = {};
-        if (row < rows) {
-          const int d0 = PAGES ? 64 * (kk >> 1) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g;
-          const h8_t y = __builtin_bit_cast(
-              h8_t, *reinterpret_cast<const u32x4_t *>(p.q + (int64_t)(seq.start + tok) * p.q_ts +
-                                                       (int64_t)(kvh * p.G + row - tok * p.G) * p.q_hs + d0));
-          if (PAGES) {
-            x[0] = y[0]; x[1] = y[4]; x[2] = y[1]; x[3] = y[5];
-            x[4] = y[2]; x[5] = y[6]; x[6] = y[3]; x[7] = y[7];
-          } else {
-            x = y;
+        constexpr int PG = KK / NG;  // products per sum
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const h8_t a = k_operand(t, kk);
+#pragma unroll
+          for (int qb = 0; qb < QB; ++qb)
+            s[qb][kk / PG][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                a, qf[qb][kk], kk % PG == 0 ? kstart[qb][kk / PG] : s[qb][kk / PG][t], 0, 0, 0);
+        }
+      }
+      // exp2 arguments; element 2 i + t: token key0 + i + 8 t
+      float x[QB][8];
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float y = s[qb][0][e & 1][e >> 1];
+          if constexpr (PAGES) {
+            y = fmaf(y, (float)as_half2(kr.sc[0][e >> 1])[e & 1], 0.0f);  // (one mixed-precision instruction)
+            if constexpr (NG == 2) y = fmaf(s[qb][1][e & 1][e >> 1], (float)as_half2(kr.sc[1][e >> 1])[e & 1], y);
+          }
+          x[qb][e] = fmaf(y, p.qk_scale_log2, ncm[qb]);
+        }
+      between();
+
+      const bool ok_a = mapped(e.a), ok_b = mapped(e.b);
+      const bool full = e.i >= full0 && e.i < full1 && ok_a && ok_b;  // (wave-uniform)
+      const int32_t ta = 16 * logical(2 * e.i), tb = 16 * logical(2 * e.i + 1);
+      const int32_t key0 = (g < 2 ? ta : tb) + 4 * (g & 1);
+      const bool c_ok = g < 2 ? ok_a : ok_b;
+      h8_t pf[QB];
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) {
+        if (!full) {
+          const int32_t last = c_ok ? min(row_pos[qb], kv_lim - 1) - key0 : -1;
+          const int32_t first_w = row_pos[qb] - p.W + 1 - key0, end_s = p.sinks - key0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int32_t c = (e >> 1) + 8 * (e & 1);
+            x[qb][e] = (c <= last) & ((c >= first_w) | (c < end_s)) ? x[qb][e] : -INFINITY;
           }
         }
-        qf[qb][kk] = x;
-      }
-    }
-
+        float t = x[qb][0];
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb)
+        for (int e = 1; e < 8; ++e) t = fmaxf(t, x[qb][e]);
+        if (__any(t > thr[qb])) {  // wave-uniform, rare after the first steps
+          // the row's four lanes agree on the new maximum
+          auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(t), __float_as_uint(t), false, false);
+          t = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+          sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(t), __float_as_uint(t), false, false);
+          t = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+          const bool first = thr[qb] == -INFINITY, found = t > -INFINITY;
+          const float shift = first ? (found ? t - kTop : 0.0f) : fmaxf(t - kTop, 0.0f);
+          const float alpha = first ? (found ? 0.0f : 1.0f) : (shift > 0.0f ? fast_exp2(-shift) : 1.0f);
+          lsum[qb] *= alpha;
 #pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        float x = 0.0f;
-        if constexpr (PAGES) {
-          float even = 0.0f, odd_q = 0.0f;  // operand pairs 0, 2 and 1, 3
+          for (int i = 0; i < ND; ++i) o[qb][i] *= alpha;
 #pragma unroll
-          for (int kk = j * (KK / NG); kk < (j + 1) * (KK / NG); ++kk) {
-            const u32x4_t y = __builtin_bit_cast(u32x4_t, qf[qb][kk]);
-            even = __builtin_amdgcn_fdot2(as_half2(y[2]), ones, __builtin_amdgcn_fdot2(as_half2(y[0]), ones, even, false), false);
-            odd_q = __builtin_amdgcn_fdot2(as_half2(y[3]), ones, __builtin_amdgcn_fdot2(as_half2(y[1]), ones, odd_q, false), false);
-          }
-          x = xor32_sum(xor16_sum(-1032.0f * even - 72.0f * odd_q));
+          for (int e = 0; e < 8; ++e) x[qb][e] -= shift;
+          ncm[qb] -= shift;
+          thr[qb] = (first && !found) ? thr[qb] : kTop + 8.0f;
         }
-        kstart[qb][j] = f32x4_t{x, x, x, x};
-      }
-  };
-  auto k_operand = [&](int t, int kk) __attribute__((always_inline)) {
-    if constexpr (PAGES) {
-      return __builtin_bit_cast(h8_t, biased(D == 128 ? kr.w[4 * (kk >> 1) + 2 * t + (kk & 1)] : kr.w[2 * kk + t]));
-    } else {
-      return __builtin_bit_cast(h8_t, kr.w[t][kk]);
-    }
-  };
-
-  // exp2 argument of a new maximum: probabilities lie in (0, 2^15], so fp16
-  // holds those down to 2^-21 of the largest as normal numbers.
-  constexpr float kTop = 7.0f;
-  uint32_t odd = 0;  // nonzero: a masked step held inf or NaN in V
-  // One step; `between` runs when K has been used and V has not.
-  auto step = [&](const Step &e, auto between) __attribute__((always_inline)) {
-    f32x4_t s[QB][NG][2];
+        uint32_t w[4];
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      constexpr int PG = KK / NG;  // products per sum
+        for (int e = 0; e < 8; ++e) x[qb][e] = fast_exp2(x[qb][e]);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const h8_t a = k_operand(t, kk);
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb)
-          s[qb][kk / PG][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              a, qf[qb][kk], kk % PG == 0 ? kstart[qb][kk / PG] : s[qb][kk / PG][t], 0, 0, 0);
-      }
-    }
-    // exp2 arguments; element 2 i + t: token key0 + i + 8 t
-    float x[QB][8];
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float y = s[qb][0][e & 1][e >> 1];
-        if constexpr (PAGES) {
-          y = fmaf(y, (float)as_half2(kr.sc[0][e >> 1])[e & 1], 0.0f);  // (one mixed-precision instruction)
-          if constexpr (NG == 2) y = fmaf(s[qb][1][e & 1][e >> 1], (float)as_half2(kr.sc[1][e >> 1])[e & 1], y);
+        for (int i = 0; i < 4; ++i) {
+          w[i] = as_u32(half2_t{(half_t)x[qb][2 * i], (half_t)x[qb][2 * i + 1]});
+          lsum[qb] = __builtin_amdgcn_fdot2(as_half2(w[i]), ones, lsum[qb], false);
         }
-        x[qb][e] = fmaf(y, p.qk_scale_log2, ncm[qb]);
+        pf[qb] = __builtin_bit_cast(h8_t, u32x4_t{w[0], w[1], w[2], w[3]});
       }
-    between();
 
-    const bool ok_a = mapped(e.a), ok_b = mapped(e.b);
-    const bool full = e.i >= full0 && e.i < full1 && ok_a && ok_b;  // (wave-uniform)
-    const int32_t ta = 16 * logical(2 * e.i), tb = 16 * logical(2 * e.i + 1);
-    const int32_t key0 = (g < 2 ? ta : tb) + 4 * (g & 1);
-    const bool c_ok = g < 2 ? ok_a : ok_b;
-    h8_t pf[QB];
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
+      // A weight of 0 must not meet an inf or NaN of V. Tokens that no row of the
+      // block sees (behind the context, unlinked, outside the window) become
+      // zeros; so do inf and NaN among those that only some rows see, which
+      // get them back at the end (`odd`).
       if (!full) {
-        const int32_t last = c_ok ? min(row_pos[qb], kv_lim - 1) - key0 : -1;
-        const int32_t first_w = row_pos[qb] - p.W + 1 - key0, end_s = p.sinks - key0;
+        const int32_t last = c_ok ? min(pos_hi, kv_lim - 1) - key0 : -1;
+        const int32_t first_w = pos_lo - p.W + 1 - key0, end_s = p.sinks - key0;
+        const bool several = pos_lo != pos_hi;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int32_t c = (e >> 1) + 8 * (e & 1);
-          x[qb][e] = (c <= last) & ((c >= first_w) | (c < end_s)) ? x[qb][e] : -INFINITY;
-        }
-      }
-      float t = x[qb][0];
-#pragma unroll
-      for (int e = 1; e < 8; ++e) t = fmaxf(t, x[qb][e]);
-      if (__any(t > thr[qb])) {  // wave-uniform, rare after the first steps
-        // the row's four lanes agree on the new maximum
-        auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(t), __float_as_uint(t), false, false);
-        t = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-        sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(t), __float_as_uint(t), false, false);
-        t = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-        const bool first = thr[qb] == -INFINITY, found = t > -INFINITY;
-        const float shift = first ? (found ? t - kTop : 0.0f) : fmaxf(t - kTop, 0.0f);
-        const float alpha = first ? (found ? 0.0f : 1.0f) : (shift > 0.0f ? fast_exp2(-shift) : 1.0f);
-        lsum[qb] *= alpha;
-#pragma unroll
-        for (int i = 0; i < ND; ++i) o[qb][i] *= alpha;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[qb][e] -= shift;
-        ncm[qb] -= shift;
-        thr[qb] = (first && !found) ? thr[qb] : kTop + 8.0f;
-      }
-      uint32_t w[4];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[qb][e] = fast_exp2(x[qb][e]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[i] = as_u32(half2_t{(half_t)x[qb][2 * i], (half_t)x[qb][2 * i + 1]});
-        lsum[qb] = __builtin_amdgcn_fdot2(as_half2(w[i]), ones, lsum[qb], false);
-      }
-      pf[qb] = __builtin_bit_cast(h8_t, u32x4_t{w[0], w[1], w[2], w[3]});
-    }
-
-    // A weight of 0 must not meet an inf or NaN of V. Tokens that no row of the
-    // block sees (behind the context, unlinked, outside the window) become
-    // zeros; so do inf and NaN among those that only some rows see, which
-    // get them back at the end (`odd`).
-    if (!full) {
-      const int32_t last = c_ok ? min(pos_hi, kv_lim - 1) - key0 : -1;
-      const int32_t first_w = pos_lo - p.W + 1 - key0, end_s = p.sinks - key0;
-      const bool several = pos_lo != pos_hi;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int32_t c = (e >> 1) + 8 * (e & 1);
-        const bool live = (c <= last) & ((c >= first_w) | (c < end_s));
-        if constexpr (PAGES) {
-          const uint32_t half = (e & 1) ? 0xFFFF0000u : 0x0000FFFFu;
-          const bool bad = several && live && (vr.sc[e >> 1] & half & 0x7C007C00u) == (half & 0x7C007C00u);
-          odd |= bad ? 1u : 0u;
-          vr.sc[e >> 1] &= live && !bad ? ~0u : ~half;
-        } else {
-#pragma unroll
-          for (int j = 0; j < D / 32; ++j) {
-            uint32_t w = live ? vr.w[e][j] : 0u;
-            if (several) {
-              const uint32_t f = ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u;  // a full exponent carries
-              odd |= f;
-              w &= ~((f << 1) - (f >> 15));
-            }
-            vr.w[e][j] = w;
-          }
-        }
-      }
-    }
-    auto pv = [&](int i, u32x4_t a) __attribute__((always_inline)) {
-#pragma unroll
-      for (int qb = 0; qb < QB; ++qb)
-        o[qb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), pf[qb], o[qb][i], 0, 0, 0);
-    };
-    if constexpr (PAGES) {
-#pragma unroll
-      for (int u = 0; u < D / 64; ++u) {
-        u32x4_t y[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          y[i] = codes(vr.w[i][u]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) y[i][j] = as_u32(as_half2(y[i][j]) * as_half2(vr.sc[i]));
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) pv(4 * u + j, u32x4_t{y[0][j], y[1][j], y[2][j], y[3][j]});
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < ND; ++i) {
-        u32x4_t a;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          a[j] = __builtin_amdgcn_perm(vr.w[2 * j + 1][i >> 1], vr.w[2 * j][i >> 1], (i & 1) ? 0x07060302u : 0x05040100u);
-        pv(i, a);
-      }
-    }
-  };
-
-  // Wave w takes steps begin + w, begin + w + NW, ...
-  if constexpr (PAGES) {
-    constexpr int CPS = 2 * ((BLK + 1023) / 1024);  // copies per step
-    Step queue[NS];                                 // the steps in flight, then the next
-#pragma unroll
-    for (int k = 0; k < NS; ++k) {
-      queue[k] = fetch(begin + wave + k * NW);
-      if (queue[k].i < end) copy_step(queue[k], k);
-    }
-    Step next = fetch(begin + wave + NS * NW);
-    load_q();  // (behind the first copies, which take longer)
-    int stage = 0;
-#pragma unroll 1
-    for (int32_t round = begin; round < end; round += NW) {
-      if (queue[0].i >= end) continue;
-      // this step's copies are the oldest: wait until no more than the later steps' are left
-      if (queue[NS - 1].i < end) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * CPS) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      const Step e = queue[0];
-      read_k(stage);
-      step(e, [&]() __attribute__((always_inline)) {
-        read_v(stage);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the stage is filled again
-        if (next.i < end) copy_step(next, stage);
-#pragma unroll
-        for (int k = 0; k + 1 < NS; ++k) queue[k] = queue[k + 1];
-        queue[NS - 1] = next;
-        next = fetch(next.i + NW);
-      });
-      stage = stage + 1 == NS ? 0 : stage + 1;
-    }
-    __syncthreads();  // every wave has read its ring: the sums take its place
-  } else {
-    Step e = fetch(begin + wave), next = fetch(begin + wave + NW);
-    if (e.i < end) {
-      load_k(e);
-      load_v(e);
-    }
-    load_q();
-    while (e.i < end) {
-      const Step after = fetch(next.i + NW);
-      step(e, [&]() __attribute__((always_inline)) {
-        if (next.i < end) load_k(next);
-      });
-      if (next.i < end) load_v(next);
-      e = next;
-      next = after;
-    }
-  }
-
-  if (__any(odd != 0)) {
-    // Rows that see an inf or NaN of V have inf or NaN in its column whatever
-    // its weight; a lane looks through its quarter of the dims.
-#pragma unroll 1
-    for (int32_t i = begin + wave; i < end; i += NW) {
-      if (i >= full0 && i < full1) continue;  // (a whole chunk there is unlinked: all zeros)
-      const Step e = fetch(i);
-#pragma unroll 1
-      for (int tk = 0; tk < 32; ++tk) {
-        const int32_t phys = tk < 16 ? e.a : e.b, lc = logical(2 * i + (tk >> 4)), t = tk & 15, key = 16 * lc + t;
-        if (!mapped(phys) || key >= kv_lim) continue;
-        const int64_t at = offset_of(phys, lc);
-#pragma unroll
-        for (int d = 0; d < D / 4; ++d) {
-          const int dim = (D / 4) * g + d;
-          float y;
+          const bool live = (c <= last) & ((c >= first_w) | (c < end_s));
           if constexpr (PAGES) {
-            const uint8_t *blk = kbase + at;
-            const half_t sv = reinterpret_cast<const half_t *>(blk + f.vscales)[f.scale_idx(t, dim / 64)];
-            y = ((float)((blk[f.vcodes + f.v_byte(t, dim)] >> (4 * (dim & 1))) & 15) - 8.0f) * (float)sv;
+            const uint32_t half = (e & 1) ? 0xFFFF0000u : 0x0000FFFFu;
+            const bool bad = several && live && (vr.sc[e >> 1] & half & 0x7C007C00u) == (half & 0x7C007C00u);
+            odd |= bad ? 1u : 0u;
+            vr.sc[e >> 1] &= live && !bad ? ~0u : ~half;
           } else {
-            y = (float)reinterpret_cast<const half_t *>(vbase + at + (int64_t)t * p.kv_ts)[dim];
-          }
-          const bool bad = (__float_as_uint(y) & 0x7F800000u) == 0x7F800000u;
 #pragma unroll
-          for (int qb = 0; qb < QB; ++qb)
-            if (bad && key <= row_pos[qb] && (key < p.sinks || key >= row_pos[qb] - p.W + 1)) o[qb][d % ND][d / ND] += y;
+            for (int j = 0; j < D / 32; ++j) {
+              uint32_t w = live ? vr.w[e][j] : 0u;
+              if (several) {
+                const uint32_t f = ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u;  // a full exponent carries
+                odd |= f;
+                w &= ~((f << 1) - (f >> 15));
+              }
+              vr.w[e][j] = w;
+            }
+          }
+        }
+      }
+      auto pv = [&](int i, u32x4_t a) __attribute__((always_inline)) {
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb)
+          o[qb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), pf[qb], o[qb][i], 0, 0, 0);
+      };
+      if constexpr (PAGES) {
+#pragma unroll
+        for (int u = 0; u < D / 64; ++u) {
+          u32x4_t y[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            y[i] = codes(vr.w[i][u]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[i][j] = as_u32(as_half2(y[i][j]) * as_half2(vr.sc[i]));
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) pv(4 * u + j, u32x4_t{y[0][j], y[1][j], y[2][j], y[3][j]});
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+          u32x4_t a;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            a[j] = __builtin_amdgcn_perm(vr.w[2 * j + 1][i >> 1], vr.w[2 * j][i >> 1], (i & 1) ? 0x07060302u : 0x05040100u);
+          pv(i, a);
+        }
+      }
+    };
+
+    // Wave w takes steps begin + w, begin + w + NW, ...
+    if constexpr (PAGES) {
+      constexpr int CPS = 2 * ((BLK + 1023) / 1024);  // copies per step
+      Step queue[NS];                                 // the steps in flight, then the next
+#pragma unroll
+      for (int k = 0; k < NS; ++k) {
+        queue[k] = fetch(begin + wave + k * NW);
+        if (queue[k].i < end) copy_step(queue[k], k);
+      }
+      Step next = fetch(begin + wave + NS * NW);
+      load_q();  // (behind the first copies, which take longer)
+      int stage = 0;
+#pragma unroll 1
+      for (int32_t round = begin; round < end; round += NW) {
+        if (queue[0].i >= end) continue;
+        // this step's copies are the oldest: wait until no more than the later steps' are left
+        if (queue[NS - 1].i < end) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * CPS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const Step e = queue[0];
+        read_k(stage);
+        step(e, [&]() __attribute__((always_inline)) {
+          read_v(stage);
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the stage is filled again
+          if (next.i < end) copy_step(next, stage);
+#pragma unroll
+          for (int k = 0; k + 1 < NS; ++k) queue[k] = queue[k + 1];
+          queue[NS - 1] = next;
+          next = fetch(next.i + NW);
+        });
+        stage = stage + 1 == NS ? 0 : stage + 1;
+      }
+      __syncthreads();  // every wave has read its ring: the sums take its place
+    } else {
+      Step e = fetch(begin + wave), next = fetch(begin + wave + NW);
+      if (e.i < end) {
+        load_k(e);
+        load_v(e);
+      }
+      load_q();
+      while (e.i < end) {
+        const Step after = fetch(next.i + NW);
+        step(e, [&]() __attribute__((always_inline)) {
+          if (next.i < end) load_k(next);
+        });
+        if (next.i < end) load_v(next);
+        e = next;
+        next = after;
+      }
+    }
+
+    if (__any(odd != 0)) {
+      // Rows that see an inf or NaN of V have inf or NaN in its column whatever
+      // its weight; a lane looks through its quarter of the dims.
+#pragma unroll 1
+      for (int32_t i = begin + wave; i < end; i += NW) {
+        if (i >= full0 && i < full1) continue;  // (a whole chunk there is unlinked: all zeros)
+        const Step e = fetch(i);
+#pragma unroll 1
+        for (int tk = 0; tk < 32; ++tk) {
+          const int32_t phys = tk < 16 ? e.a : e.b, lc = logical(2 * i + (tk >> 4)), t = tk & 15, key = 16 * lc + t;
+          if (!mapped(phys) || key >= kv_lim) continue;
+          const int64_t at = offset_of(phys, lc);
+#pragma unroll
+          for (int d = 0; d < D / 4; ++d) {
+            const int dim = (D / 4) * g + d;
+            float y;
+            if constexpr (PAGES) {
+              const uint8_t *blk = kbase + at;
+              const half_t sv = reinterpret_cast<const half_t *>(blk + f.vscales)[f.scale_idx(t, dim / 64)];
+              y = ((float)((blk[f.vcodes + f.v_byte(t, dim)] >> (4 * (dim & 1))) & 15) - 8.0f) * (float)sv;
+            } else {
+              y = (float)reinterpret_cast<const half_t *>(vbase + at + (int64_t)t * p.kv_ts)[dim];
+            }
+            const bool bad = (__float_as_uint(y) & 0x7F800000u) == 0x7F800000u;
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb)
+              if (bad && key <= row_pos[qb] && (key < p.sinks || key >= row_pos[qb] - p.W + 1)) o[qb][d % ND][d / ND] += y;
+          }
         }
       }
     }
-  }
 
-  // Merge of the waves. Lane (n, g) holds dims [D/4 g, D/4 (g + 1)) of row n:
-  // row 4 g + reg of V^T product i is dim D/16 (4 g + reg) + i.
+    // Merge of the waves. Lane (n, g) holds dims [D/4 g, D/4 (g + 1)) of row n:
+    // row 4 g + reg of V^T product i is dim D/16 (4 g + reg) + i.
 #pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    const float l = xor32_sum(xor16_sum(lsum[qb]));
-    const int row = 16 * qb + r;
-    if (row0 + row >= rows) continue;
+    for (int qb = 0; qb < QB; ++qb) {
+      const float l = xor32_sum(xor16_sum(lsum[qb]));
+      const int row = 16 * qb + r;
+      if (row0 + row >= rows) continue;
 #pragma unroll
-    for (int reg = 0; reg < 4; ++reg)
+      for (int reg = 0; reg < 4; ++reg)
 #pragma unroll
-      for (int i = 0; i < ND; i += 4)
-        *reinterpret_cast<f32x4_t *>(&s_o[wave][row][ND * (4 * g + reg) + i]) =
-            f32x4_t{o[qb][i][reg], o[qb][i + 1][reg], o[qb][i + 2][reg], o[qb][i + 3][reg]};
-    if (g == 0) {
-      s_ml[wave][row][0] = thr[qb] == -INFINITY ? -INFINITY : -ncm[qb];
-      s_ml[wave][row][1] = l;
+        for (int i = 0; i < ND; i += 4)
+          *reinterpret_cast<f32x4_t *>(&s_o[wave][row][ND * (4 * g + reg) + i]) =
+              f32x4_t{o[qb][i][reg], o[qb][i + 1][reg], o[qb][i + 2][reg], o[qb][i + 3][reg]};
+      if (g == 0) {
+        s_ml[wave][row][0] = thr[qb] == -INFINITY ? -INFINITY : -ncm[qb];
+        s_ml[wave][row][1] = l;
+      }
     }
-  }
-  __syncthreads();
-  // A block whose steps lie in one run is finished here.
-  const int32_t w0 = block_at >= first ? wg : wg_of(block_at);
-  const int32_t w1 = block_at + seq.steps <= stop ? wg : wg_of(block_at + seq.steps - 1);
-  const int32_t live = min(QN, rows - row0);
-  auto write_row = [&](int row, int d, f32x4_t x, float l) __attribute__((always_inline)) {
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    const int32_t rr = row0 + row, tok = p.by_g(rr);
-    *reinterpret_cast<u32x2_t *>(p.out + (int64_t)(seq.start + tok) * p.o_ts +
-                                 (int64_t)(kvh * p.G + rr - tok * p.G) * p.o_hs + d) =
-        u32x2_t{as_u32(half2_t{(half_t)(x[0] * inv), (half_t)(x[1] * inv)}),
-                as_u32(half2_t{(half_t)(x[2] * inv), (half_t)(x[3] * inv)})};
-  };
-  // A run holds at most two blocks in part: one that began before it (slot 0),
-  // one that begins in it and goes on behind it (slot 1).
-  auto partial_slot = [&](int32_t w) { return ((int64_t)w * 2 + (w == w0 ? 1 : 0)) * p.Hk + kvh; };
-  const int64_t mine = partial_slot(wg) * QN;
-  for (int idx = tid; idx < live * (D / 4); idx += NT) {
-    const int row = idx / (D / 4), d = 4 * (idx % (D / 4));
-    float mx = s_ml[0][row][0];
+    __syncthreads();
+    // A block whose steps lie in one run is finished here.
+    const int32_t w0 = block_at >= first ? wg : wg_of(block_at);
+    const int32_t w1 = block_at + seq.steps <= stop ? wg : wg_of(block_at + seq.steps - 1);
+    const int32_t live = min(QN, rows - row0);
+    auto write_row = [&](int row, int d, f32x4_t x, float l) __attribute__((always_inline)) {
+      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      const int32_t rr = row0 + row, tok = p.by_g(rr);
+      *reinterpret_cast<u32x2_t *>(p.out + (int64_t)(seq.start + tok) * p.o_ts +
+                                   (int64_t)(kvh * p.G + rr - tok * p.G) * p.o_hs + d) =
+          u32x2_t{as_u32(half2_t{(half_t)(x[0] * inv), (half_t)(x[1] * inv)}),
+                  as_u32(half2_t{(half_t)(x[2] * inv), (half_t)(x[3] * inv)})};
+    };
+    // A run holds at most two blocks in part: one that began before it (slot 0),
+    // one that begins in it and goes on behind it (slot 1).
+    auto partial_slot = [&](int32_t w) { return ((int64_t)w * 2 + (w == w0 ? 1 : 0)) * p.Hk + kvh; };
+    const int64_t mine = partial_slot(wg) * QN;
+    for (int idx = tid; idx < live * (D / 4); idx += NT) {
+      const int row = idx / (D / 4), d = 4 * (idx % (D / 4));
+      float mx = s_ml[0][row][0];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) mx = fmaxf(mx, s_ml[w][row][0]);
-    float l = 0.0f;
-    f32x4_t x = {};
+      for (int w = 1; w < NW; ++w) mx = fmaxf(mx, s_ml[w][row][0]);
+      float l = 0.0f;
+      f32x4_t x = {};
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float mw = s_ml[w][row][0], fw = mw == -INFINITY ? 0.0f : fast_exp2(mw - mx);
-      l += s_ml[w][row][1] * fw;
-      x += *reinterpret_cast<const f32x4_t *>(&s_o[w][row][d]) * fw;
-    }
-    if (w0 == w1) {
-      write_row(row, d, x, l);
-    } else {
-      // (agent scope: the other workgroups of the block may run on other XCDs)
-      uint64_t *dst = reinterpret_cast<uint64_t *>(p.ws_o + (mine + row) * D + d);
-      __hip_atomic_store(dst, __builtin_bit_cast(uint64_t, u32x2_t{__float_as_uint(x[0]), __float_as_uint(x[1])}),
-                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __hip_atomic_store(dst + 1, __builtin_bit_cast(uint64_t, u32x2_t{__float_as_uint(x[2]), __float_as_uint(x[3])}),
-                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (d == 0)
-        __hip_atomic_store(reinterpret_cast<uint64_t *>(p.ws_ml + 2 * (mine + row)),
-                           __builtin_bit_cast(uint64_t, u32x2_t{__float_as_uint(mx), __float_as_uint(l)}),
+      for (int w = 0; w < NW; ++w) {
+        const float mw = s_ml[w][row][0], fw = mw == -INFINITY ? 0.0f : fast_exp2(mw - mx);
+        l += s_ml[w][row][1] * fw;
+        x += *reinterpret_cast<const f32x4_t *>(&s_o[w][row][d]) * fw;
+      }
+      if (w0 == w1) {
+        write_row(row, d, x, l);
+      } else {
+        // (agent scope: the other workgroups of the block may run on other XCDs)
+        uint64_t *dst = reinterpret_cast<uint64_t *>(p.ws_o + (mine + row) * D + d);
+        __hip_atomic_store(dst, __builtin_bit_cast(uint64_t, u32x2_t{__float_as_uint(x[0]), __float_as_uint(x[1])}),
                            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(dst + 1, __builtin_bit_cast(uint64_t, u32x2_t{__float_as_uint(x[2]), __float_as_uint(x[3])}),
+                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (d == 0)
+          __hip_atomic_store(reinterpret_cast<uint64_t *>(p.ws_ml + 2 * (mine + row)),
+                             __builtin_bit_cast(uint64_t, u32x2_t{__float_as_uint(mx), __float_as_uint(l)}),
+                             __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
     }
-  }
-  if (w0 != w1) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's partial stores are complete
-    __syncthreads();
-    if (tid == 0) {
-      uint32_t *cnt = p.ws_cnt + (int64_t)(seq_blocks + block) * p.Hk + kvh;
-      const uint32_t n = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
-      s_last = n == (uint32_t)(w1 - w0 + 1);
-      if (s_last) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (s_last) {
-      // Weights of the partials, row by row (a wave per row), in LDS; the row's
-      // sum in s_ml. Then the partials are dealt to parts of the workgroup, four
-      // dims of a row per thread, loads first; the parts' sums meet in LDS.
-      auto load2 = [&](const float *src) __attribute__((always_inline)) {
-        const u32x2_t u = __builtin_bit_cast(
-            u32x2_t, __hip_atomic_load(reinterpret_cast<const uint64_t *>(src), __ATOMIC_RELAXED,
-                                       __HIP_MEMORY_SCOPE_AGENT));
-        return float2{__uint_as_float(u[0]), __uint_as_float(u[1])};
-      };
-      const int32_t parts = w1 - w0 + 1;
-      float *const wgt = reinterpret_cast<float *>(smem);
-      f32x4_t *const sums = reinterpret_cast<f32x4_t *>(smem + QN * kMaxParts * 4);
-      const int32_t cells = live * (D / 4), groups = max(1, NT / cells);
-      constexpr int R = 8;
-      float2 y[R][2];
-      auto load_parts = [&](int32_t i0, int row, int d) __attribute__((always_inline)) {
-#pragma unroll
-        for (int k = 0; k < R; ++k) {
-          const float *src = p.ws_o + (partial_slot(w0 + min(i0 + k * groups, parts - 1)) * QN + row) * D + d;
-          y[k][0] = load2(src);
-          y[k][1] = load2(src + 2);
-        }
-      };
-      for (int c0 = 0; c0 < cells; c0 += NT) {  // (once where the cells fit the workgroup)
-        const int cell = groups > 1 ? tid % cells : c0 + tid, part = groups > 1 ? tid / cells : 0;
-        const bool on = cell < cells && part < groups;
-        const int row = on ? cell / (D / 4) : 0, d = 4 * (cell % (D / 4));
-        load_parts(part, row, d);  // in flight while the weights are computed
-        if (c0 == 0) {
-          for (int row = wave; row < live; row += NW) {
-            float m[kMaxParts / 64], l[kMaxParts / 64], mx = -INFINITY, lt = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kMaxParts / 64; ++i) {
-              const int32_t w = lane + 64 * i;
-              const float2 ml = load2(p.ws_ml + 2 * (partial_slot(w0 + min(w, parts - 1)) * QN + row));
-              m[i] = w < parts ? ml.x : -INFINITY;
-              l[i] = ml.y;
-              mx = fmaxf(mx, m[i]);
-            }
-            mx = wave_max(mx);
-#pragma unroll
-            for (int i = 0; i < kMaxParts / 64; ++i) {
-              const float f = m[i] == -INFINITY ? 0.0f : fast_exp2(m[i] - mx);
-              lt += f * l[i];
-              if (lane + 64 * i < parts) wgt[row * kMaxParts + lane + 64 * i] = f;
-            }
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) lt += shfl_xor(lt, off);
-            if (lane == 0) s_ml[0][row][1] = lt;
-          }
-          __syncthreads();
-        }
-        f32x4_t x = {};
-        for (int32_t i0 = part; i0 < parts && on; i0 += R * groups) {
-          if (i0 != part) load_parts(i0, row, d);
+    if (w0 != w1) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's partial stores are complete
+      __syncthreads();
+      if (tid == 0) {
+        uint32_t *cnt = p.ws_cnt + (int64_t)(seq_blocks + block) * p.Hk + kvh;
+        const uint32_t n = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
+        s_last = n == (uint32_t)(w1 - w0 + 1);
+        if (s_last) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      __syncthreads();
+      if (s_last) {
+        // Weights of the partials, row by row (a wave per row), in LDS; the row's
+        // sum in s_ml. Then the partials are dealt to parts of the workgroup, four
+        // dims of a row per thread, loads first; the parts' sums meet in LDS.
+        auto load2 = [&](const float *src) __attribute__((always_inline)) {
+          const u32x2_t u = __builtin_bit_cast(
+              u32x2_t, __hip_atomic_load(reinterpret_cast<const uint64_t *>(src), __ATOMIC_RELAXED,
+                                         __HIP_MEMORY_SCOPE_AGENT));
+          return float2{__uint_as_float(u[0]), __uint_as_float(u[1])};
+        };
+        const int32_t parts = w1 - w0 + 1;
+        float *const wgt = reinterpret_cast<float *>(smem);
+        f32x4_t *const sums = reinterpret_cast<f32x4_t *>(smem + QN * kMaxParts * 4);
+        const int32_t cells = live * (D / 4), groups = max(1, NT / cells);
+        constexpr int R = 8;
+        float2 y[R][2];
+        auto load_parts = [&](int32_t i0, int row, int d) __attribute__((always_inline)) {
 #pragma unroll
           for (int k = 0; k < R; ++k) {
-            const float f = i0 + k * groups < parts ? wgt[row * kMaxParts + i0 + k * groups] : 0.0f;
-            x += f32x4_t{y[k][0].x, y[k][0].y, y[k][1].x, y[k][1].y} * f;
+            const float *src = p.ws_o + (partial_slot(w0 + min(i0 + k * groups, parts - 1)) * QN + row) * D + d;
+            y[k][0] = load2(src);
+            y[k][1] = load2(src + 2);
           }
+        };
+        for (int c0 = 0; c0 < cells; c0 += NT) {  // (once where the cells fit the workgroup)
+          const int cell = groups > 1 ? tid % cells : c0 + tid, part = groups > 1 ? tid / cells : 0;
+          const bool on = cell < cells && part < groups;
+          const int row = on ? cell / (D / 4) : 0, d = 4 * (cell % (D / 4));
+          load_parts(part, row, d);  // in flight while the weights are computed
+          if (c0 == 0) {
+            for (int row = wave; row < live; row += NW) {
+              float m[kMaxParts / 64], l[kMaxParts / 64], mx = -INFINITY, lt = 0.0f;
+#pragma unroll
+              for (int i = 0; i < kMaxParts / 64; ++i) {
+                const int32_t w = lane + 64 * i;
+                const float2 ml = load2(p.ws_ml + 2 * (partial_slot(w0 + min(w, parts - 1)) * QN + row));
+                m[i] = w < parts ? ml.x : -INFINITY;
+                l[i] = ml.y;
+                mx = fmaxf(mx, m[i]);
+              }
+              mx = wave_max(mx);
+#pragma unroll
+              for (int i = 0; i < kMaxParts / 64; ++i) {
+                const float f = m[i] == -INFINITY ? 0.0f : fast_exp2(m[i] - mx);
+                lt += f * l[i];
+                if (lane + 64 * i < parts) wgt[row * kMaxParts + lane + 64 * i] = f;
+              }
+#pragma unroll
+              for (int off = 32; off > 0; off >>= 1) lt += shfl_xor(lt, off);
+              if (lane == 0) s_ml[0][row][1] = lt;
+            }
+            __syncthreads();
+          }
+          f32x4_t x = {};
+          for (int32_t i0 = part; i0 < parts && on; i0 += R * groups) {
+            if (i0 != part) load_parts(i0, row, d);
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+              const float f = i0 + k * groups < parts ? wgt[row * kMaxParts + i0 + k * groups] : 0.0f;
+              x += f32x4_t{y[k][0].x, y[k][0].y, y[k][1].x, y[k][1].y} * f;
+            }
+          }
+          if (groups > 1) {
+            sums[tid] = x;
+            __syncthreads();
+            for (int k = 1; k < groups && part == 0 && on; ++k) x += sums[tid + k * cells];
+          }
+          if (on && part == 0) write_row(row, d, x, s_ml[0][row][1]);
         }
-        if (groups > 1) {
-          sums[tid] = x;
-          __syncthreads();
-          for (int k = 1; k < groups && part == 0 && on; ++k) x += sums[tid + k * cells];
-        }
-        if (on && part == 0) write_row(row, d, x, s_ml[0][row][1]);
       }
     }
+    __syncthreads();  // s_o and s_ml are free for the next block
   }
-  __syncthreads();  // s_o and s_ml are free for the next block
+}
+
+// The staged copies: K and V of what the staged sequences see, as fp16 rows.
+// The 64-token tiles of all of them form one list; workgroup i of a key head
+// takes tiles i, i + gridDim, ..., each wave 16 tokens of them, which lie in
+// one page. A wave reads a block of a page as it is (lane l: the 16 dims (D =
+// 64: 8) of tokens p = l / 8 and p + 8 that start at D / 8 * (l % 8)) and writes
+// fp16((code - 8) * scale): one rounding, as in the V operands above.
+template <int D, int FMT>
+__global__ __launch_bounds__(256) void stage_kernel(const PackedParams p, const int32_t *__restrict__ starts,
+                                                    const int32_t *__restrict__ ctxs,
+                                                    const int32_t *__restrict__ tables) {
+  constexpr bool PAGES = FMT == MEMOPT_KV_INT4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int32_t kvh = blockIdx.x % p.Hk, wg = blockIdx.x / p.Hk, wgs = gridDim.x / p.Hk;
+  const Int4Page f(D);
+  int32_t item = wg, before = 0, slots = 0;
+  for (int32_t b0 = 0; b0 < p.B; b0 += 64) {
+    // lane i: sequence b0 + i
+    bool on = false;
+    int32_t n = 0, kv_lim = 0, tiles = 0;
+    StagedMap m = {};
+    if (b0 + lane < p.B) {
+      n = rows_of(starts, p.T, b0 + lane).n;
+      const int32_t ctx = ctxs[b0 + lane];
+      kv_lim = (int32_t)min((int64_t)ctx, (int64_t)p.M * p.bs);
+      on = is_staged(p.st, n, p.G);
+      m = staged_map(kv_lim, ctx - n, p.W, p.sinks);
+      if (on) tiles = (m.sink_end + max(0, (max(kv_lim, 0) + 63) / 64 * 64 - max(m.lo, m.sink_end))) / 64;
+    }
+    const uint64_t staged = __ballot(on);
+    const int32_t incl = (int32_t)wave_scan((uint32_t)tiles), total = __builtin_amdgcn_readlane(incl, 63);
+    for (; item < before + total; item += wgs) {
+      const int src = __builtin_ctzll(__ballot(item < before + incl));
+      const int32_t slot = slots + (int32_t)__popcll(staged & ((1ull << src) - 1));
+      if (slot >= p.st.slots) return;  // sequences overlap
+      const int32_t lim = __builtin_amdgcn_readlane(kv_lim, src), sink_end = __builtin_amdgcn_readlane(m.sink_end, src);
+      const int32_t skip = __builtin_amdgcn_readlane(m.skip, src);
+      const int32_t row = 64 * (item - before - __builtin_amdgcn_readlane(incl, src) + __builtin_amdgcn_readlane(tiles, src)) +
+                          16 * wave;
+      if (row >= p.st.cap) return;  // (a chunk longer than announced)
+      const int32_t pos = row < sink_end ? row : row + skip, chunk = pos >> 4, cpp = PAGES ? 1 : p.bs >> 4;
+      const bool inside = pos < lim;
+      const int32_t phys = inside ? tables[(int64_t)(b0 + src) * p.M + (cpp == 1 ? chunk : chunk / cpp)] : 0;
+      const bool ok = phys >= 0 && phys < p.nb;
+      if (kvh == 0 && lane == 0) p.st.links[((int64_t)slot * p.st.cap + row) / 16] = ok ? 1 : 0;
+      if (!inside) continue;
+      const int64_t out = (((int64_t)slot * p.st.cap + row) * p.Hk + kvh) * D, ts = (int64_t)p.Hk * D;
+      if constexpr (PAGES) {
+        constexpr int DL = D / 8, W = D / 64;  // dims and words of a token per lane
+        const int t = lane >> 3, d0 = DL * (lane & 7);
+        uint32_t kw[2][W], vw[2 * W];  // K words of tokens t and t + 8; V words hold four dims of both
+        uint32_t ks = 0, vs = 0;
+#pragma unroll
+        for (int j = 0; j < 2 * W; ++j) kw[j / W][j % W] = vw[j] = 0x88888888u;
+        if (ok) {
+          const uint8_t *blk = p.k + (int64_t)phys * p.kv_ps + kvh * p.kv_hs;
+          const uint32_t *kc = reinterpret_cast<const uint32_t *>(blk + f.kcodes) + 2 * W * lane;
+          const uint32_t *vc = reinterpret_cast<const uint32_t *>(blk + f.vcodes) + 2 * W * lane;
+#pragma unroll
+          for (int j = 0; j < 2 * W; ++j) {
+            kw[j / W][j % W] = kc[j];
+            vw[j] = vc[j];
+          }
+          ks = *reinterpret_cast<const uint32_t *>(blk + f.kscales + 2 * f.scale_idx(t, d0 / 64));
+          vs = *reinterpret_cast<const uint32_t *>(blk + f.vscales + 2 * f.scale_idx(t, d0 / 64));
+        }
+        auto unpack = [&](uint32_t w, uint32_t s, uint32_t (&y)[4]) __attribute__((always_inline)) {
+          const half2_t b1032 = {(half_t)1032.0f, (half_t)1032.0f}, b72 = {(half_t)72.0f, (half_t)72.0f};
+          const uint32_t w8 = w >> 8;
+          y[0] = as_u32((as_half2((w & 0x000F000Fu) | 0x64006400u) - b1032) * as_half2(s));
+          y[1] = as_u32((as_half2((w & 0x00F000F0u) | 0x54005400u) - b72) * as_half2(s));
+          y[2] = as_u32((as_half2((w8 & 0x000F000Fu) | 0x64006400u) - b1032) * as_half2(s));
+          y[3] = as_u32((as_half2((w8 & 0x00F000F0u) | 0x54005400u) - b72) * as_half2(s));
+        };
+        constexpr uint32_t LO = 0x05040100u, HI = 0x07060302u;
+        half_t *const ko = p.st.k + out + t * ts + d0, *const vo = p.st.v + out + t * ts + d0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int j = 0; j < W; ++j) {
+            uint32_t y[4];
+            unpack(kw[h][j], __builtin_amdgcn_perm(ks, ks, h ? 0x03020302u : 0x01000100u), y);
+            *reinterpret_cast<u32x4_t *>(ko + 8 * h * ts + 8 * j) =
+                u32x4_t{__builtin_amdgcn_perm(y[1], y[0], LO), __builtin_amdgcn_perm(y[3], y[2], LO),
+                        __builtin_amdgcn_perm(y[1], y[0], HI), __builtin_amdgcn_perm(y[3], y[2], HI)};
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+          uint32_t y[4], z[4];
+          unpack(vw[2 * j], vs, y);
+          unpack(vw[2 * j + 1], vs, z);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t sel = h ? HI : LO;
+            *reinterpret_cast<u32x4_t *>(vo + 8 * h * ts + 8 * j) =
+                u32x4_t{__builtin_amdgcn_perm(y[1], y[0], sel), __builtin_amdgcn_perm(y[3], y[2], sel),
+                        __builtin_amdgcn_perm(z[1], z[0], sel), __builtin_amdgcn_perm(z[3], z[2], sel)};
+          }
+        }
+      } else {
+        constexpr int PPR = D / 8, NP = 16 * PPR / 64;  // 16-byte pieces of a row, and per lane
+        const int64_t at = (int64_t)phys * p.kv_ps + (int64_t)(16 * (chunk - chunk / cpp * cpp)) * p.kv_ts + kvh * p.kv_hs;
+        u32x4_t kx[NP], vx[NP];
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          const int t = (64 * j + lane) / PPR, d = 8 * (lane % PPR);
+          kx[j] = vx[j] = (u32x4_t){};
+          if (ok) {
+            kx[j] = *reinterpret_cast<const u32x4_t *>(p.k + at + t * p.kv_ts + 2 * d);
+            vx[j] = *reinterpret_cast<const u32x4_t *>(p.v + at + t * p.kv_ts + 2 * d);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          const int t = (64 * j + lane) / PPR, d = 8 * (lane % PPR);
+          *reinterpret_cast<u32x4_t *>(p.st.k + out + t * ts + d) = kx[j];
+          *reinterpret_cast<u32x4_t *>(p.st.v + out + t * ts + d) = vx[j];
+        }
+      }
+    }
+    before += total;
+    slots += (int32_t)__popcll(staged);
   }
 }
 
@@ -861,10 +985,23 @@ static int64_t packed_steps(const memopt_packed_desc &d) {
 struct PackedPlan {
   int32_t qn, waves, wgs;
   int64_t blocks;  // at most this many
+  int32_t min_rows, slots;  // staged sequences
+  int64_t cap;
 };
 
+// Rows from which a sequence's chunk attends from a staged copy, and rows of
+// the whole batch and all key heads, as tiles of 128, from which any does: one
+// per CU, since those tiles are not split along the keys (some 17 us for 1024
+// of them) as the blocks here are. 32 query over 8 key heads of 128, us staged
+// and not: 8 chunks of 1024 rows over contexts of 4096 162 and 262; 8 of 512
+// (256 tiles) 110 and 133; 32 of 512 455 and 521; but 32 of 256 314 and 264,
+// one of 1024 (64 tiles) 72 and 53.
+static constexpr int kStagedRows = 512;
+// Of staged copies at most this much.
+static constexpr int64_t kStagedBytes = 2LL << 30;
+
 static PackedPlan packed_plan(const memopt_packed_desc &d) {
-  PackedPlan pl;
+  PackedPlan pl = {};
   const int64_t G = d.num_heads / d.num_kv_heads, most = (int64_t)std::min(d.max_query_len, d.tokens) * G;
   pl.qn = most <= 16 ? 16 : 32;
   // sum over the sequences of ceil(rows / qn)
@@ -884,18 +1021,35 @@ static PackedPlan packed_plan(const memopt_packed_desc &d) {
   if (pl.waves == 4 && pl.qn == 16 && std::min<int64_t>(wgs(4), packed_steps(d) * d.batch / 4) > 24LL * d.batch)
     pl.waves = 12;
   pl.wgs = wgs(pl.waves);
+  pl.min_rows = kStagedRows;
+  if (most >= pl.min_rows && (int64_t)d.tokens * d.num_heads >= 128LL * compute_units()) {
+    const int64_t W = std::min(effective_window(d.window_size, d.max_seq_len), 1 << 30), sinks = std::max(0, d.num_sink_tokens);
+    auto up64 = [](int64_t x) { return (x + 63) / 64 * 64; };
+    pl.cap = std::min(up64((int64_t)d.max_blocks_per_seq * d.block_size),
+                      up64(W + std::min(d.max_query_len, d.tokens)) + 128 + up64(sinks));
+    const int64_t fit = kStagedBytes / (pl.cap * d.num_kv_heads * d.head_dim * 4);
+    const int64_t most_seqs = std::min<int64_t>(d.batch, d.tokens * G / pl.min_rows);
+    pl.slots = (int32_t)std::min(most_seqs, fit);
+    // Room for fewer than could come: chunks of which no more than that fit into the batch.
+    if (fit < most_seqs) pl.min_rows = (int32_t)(d.tokens * G / (fit + 1) + 1);
+  }
   return pl;
 }
 
 struct PackedWorkspace {
-  int64_t counters, ml, total;  // bytes of the counters, offset of the (m, l) pairs
+  int64_t counters, ml, links, k, v, total;  // bytes of the counters; offsets of the (m, l) pairs and the staged copies
 };
 static PackedWorkspace packed_workspace(const memopt_packed_desc &d, const PackedPlan &pl) {
   PackedWorkspace w;
   w.counters = (pl.blocks * d.num_kv_heads * 4 + 255) / 256 * 256;
   const int64_t rows = 2LL * pl.wgs * d.num_kv_heads * pl.qn;
   w.ml = w.counters + rows * d.head_dim * 4;
-  w.total = w.ml + rows * 8;
+  auto up256 = [](int64_t x) { return (x + 255) / 256 * 256; };
+  w.links = up256(w.ml + rows * 8);
+  w.k = up256(w.links + pl.slots * pl.cap / 16);
+  const int64_t staged = pl.slots * pl.cap * d.num_kv_heads * d.head_dim * 2;
+  w.v = w.k + staged;
+  w.total = w.v + staged;
   return w;
 }
 
@@ -939,6 +1093,16 @@ static void launch_packed(const PackedParams &p, const memopt_packed_desc &d, co
   }
 }
 
+template <int D>
+static void launch_stage(const PackedParams &p, const memopt_packed_desc &d, dim3 grid, hipStream_t s) {
+  if (d.kv_format == MEMOPT_KV_INT4)
+    hipLaunchKernelGGL((stage_kernel<D, MEMOPT_KV_INT4>), grid, dim3(256), 0, s, p, d.query_starts, d.context_lens,
+                       d.block_tables);
+  else
+    hipLaunchKernelGGL((stage_kernel<D, MEMOPT_KV_FP16>), grid, dim3(256), 0, s, p, d.query_starts, d.context_lens,
+                       d.block_tables);
+}
+
 }  // namespace memopt
 
 using namespace memopt;
@@ -962,6 +1126,8 @@ extern "C" int memopt_packed_attention(const memopt_packed_desc *desc, void *str
   MEMOPT_REQUIRE(d.query && d.out && d.key_cache && (d.value_cache || d.kv_format == MEMOPT_KV_INT4) &&
                      d.block_tables && d.context_lens && d.query_starts,
                  MEMOPT_ERR_INVALID, "packed_attention: null pointer");
+  MEMOPT_REQUIRE((int64_t)d.max_blocks_per_seq * d.block_size <= INT32_MAX - 127, MEMOPT_ERR_UNSUPPORTED,
+                 "packed_attention: positions must fit 32 bits");
   const PackedPlan pl = packed_plan(d);
   const PackedWorkspace w = packed_workspace(d, pl);
   MEMOPT_REQUIRE(d.workspace && d.workspace_bytes >= w.total, MEMOPT_ERR_INVALID,
@@ -1004,6 +1170,20 @@ extern "C" int memopt_packed_attention(const memopt_packed_desc *desc, void *str
   p.ws_o = (float *)((uint8_t *)d.workspace + w.counters);
   p.ws_ml = (float *)((uint8_t *)d.workspace + w.ml);
   hipStream_t s = (hipStream_t)stream;
+  if (pl.slots > 0) {
+    uint8_t *const ws = (uint8_t *)d.workspace;
+    p.st = {pl.min_rows, std::min(d.max_query_len, d.tokens), pl.slots, (int32_t)pl.cap, (half_t *)(ws + w.k),
+            (half_t *)(ws + w.v), ws + w.links};
+    const unsigned wgs = (unsigned)std::max<int64_t>(1, std::min<int64_t>(8LL * compute_units() / p.Hk, pl.slots * pl.cap / 64));
+    const dim3 grid(wgs * p.Hk);
+    if (d.head_dim == 128) launch_stage<128>(p, d, grid, s);
+    else launch_stage<64>(p, d, grid, s);
+    if ((rc = check_launch("packed_attention(stage)")) != MEMOPT_OK) return rc;
+    const PagedTiles t = {p.q, p.out, p.q_ts, p.q_hs, p.o_ts, p.o_hs, d.query_starts, d.context_lens, p.T, p.B, p.Hk, p.G,
+                          d.head_dim, (int32_t)std::min<int64_t>((int64_t)p.M * p.bs, INT32_MAX), p.W, p.sinks,
+                          p.qk_scale_log2, p.st};
+    if ((rc = launch_paged_tiles(t, s)) != MEMOPT_OK) return rc;
+  }
   if (d.head_dim == 128) launch_packed<128>(p, d, pl, s);
   else launch_packed<64>(p, d, pl, s);
   return check_launch("packed_attention");

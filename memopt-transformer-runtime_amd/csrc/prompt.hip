@@ -13,6 +13,7 @@
 
 #include "attention.hpp"
 #include "lds_dma.hpp"
+#include "packed.hpp"
 
 namespace memopt {
 
@@ -25,9 +26,14 @@ struct PromptParams {
   const uint16_t *q, *k, *v;  // 16-bit elements; strides in elements
   uint16_t *out;
   int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs;
-  const int32_t *cu;
-  int32_t T, B, Hq, Hk, W, sinks;
+  const int32_t *starts;
+  int32_t T, B, Hk, G, W, sinks;
+  Divisor by_g;
   float qk_scale_log2;
+  // chunks over a cache: k and v are the staged copies
+  const int32_t *ctx;
+  int32_t max_tokens;
+  Staged st;
 };
 
 // 16-bit operand types. Products of two elements are exact in the 32-bit
@@ -77,34 +83,37 @@ __device__ __forceinline__ int32_t wave_sum(int32_t v) {
          __builtin_amdgcn_readlane(v, 48);
 }
 
-// The query tile (R rows of one sequence) that comes rank-th when the tiles of
-// all sequences are ordered by their place in their sequence, last places
-// first: under the causal mask those see the most keys, and a grid that ends
-// with its longest workgroups leaves the GPU idle behind them. Each lane holds
-// the tile counts of up to four sequences; the tiles at place >= x are
-// counted with one sum over the wave, x found by bisection. More than 256
-// sequences are taken in order instead. Returns false past the last tile.
+// The tile (R rows of one sequence) that comes rank-th when the tiles of all
+// sequences are ordered by their place in their sequence, last places first:
+// under the causal mask those see the most keys, and a grid that ends with its
+// longest workgroups leaves the GPU idle behind them. Each lane holds the
+// tile counts of up to four sequences; the tiles at place >= x are counted
+// with one sum over the wave, x found by bisection. More than 256 sequences
+// are taken in order instead. Returns false past the last tile. Over a cache
+// only staged sequences have tiles; slot is their rank.
 struct Tile {
-  int32_t b, t;
+  int32_t b, t, slot;
 };
-template <int R>
-__device__ __forceinline__ bool find_tile(const int32_t *cu, int32_t B, int32_t T, int32_t rank, Tile &out) {
+template <int R, bool PAGED>
+__device__ __forceinline__ bool find_tile(const PromptParams &p, int32_t rank, Tile &out) {
   const int lane = threadIdx.x & 63;
-  out = {0, 0};
-  if (B == 1) {
-    const int32_t lo = min(max(cu[0], 0), T), n = (min(max(cu[1], lo), T) - lo + R - 1) / R;
-    out = {0, n - 1 - rank};
+  out = {0, 0, 0};
+  auto tiles_of = [&](int32_t b) {
+    if (b >= p.B) return 0;
+    const int32_t n = rows_of(p.starts, p.T, b).n;
+    if (PAGED && !is_staged(p.st, n, p.G)) return 0;
+    return (n * p.G + R - 1) / R;
+  };
+  if (p.B == 1) {
+    const int32_t n = tiles_of(0);
+    out.t = n - 1 - rank;
     return rank < n;
   }
-  auto tiles_of = [&](int32_t b) {
-    if (b >= B) return 0;
-    const int32_t lo = min(max(cu[b], 0), T), hi = min(max(cu[b + 1], lo), T);
-    return (hi - lo + R - 1) / R;
-  };
-  if (B <= 256) {
+  const uint64_t below = (1ull << lane) - 1;
+  if (p.B <= 256) {
     int32_t n[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) n[k] = 64 * k < B ? tiles_of(64 * k + lane) : 0;
+    for (int k = 0; k < 4; ++k) n[k] = 64 * k < p.B ? tiles_of(64 * k + lane) : 0;
     auto at_or_past = [&](int32_t x) {
       int32_t s = 0;
 #pragma unroll
@@ -112,7 +121,7 @@ __device__ __forceinline__ bool find_tile(const int32_t *cu, int32_t B, int32_t 
       return wave_sum(s);
     };
     if (rank >= at_or_past(0)) return false;
-    int32_t lo = 0, hi = (T + R - 1) / R;  // at_or_past(lo) > rank >= at_or_past(hi)
+    int32_t lo = 0, hi = (p.T * p.G + R - 1) / R;  // at_or_past(lo) > rank >= at_or_past(hi)
     while (hi - lo > 1) {
       const int32_t mid = (lo + hi) >> 1;
       if (at_or_past(mid) > rank) lo = mid;
@@ -122,20 +131,23 @@ __device__ __forceinline__ bool find_tile(const int32_t *cu, int32_t B, int32_t 
     out.t = lo;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const uint64_t m = __ballot(n[k] > lo);
+      const uint64_t m = __ballot(n[k] > lo), staged = PAGED ? __ballot(n[k] > 0) : 0;
       const int32_t c = __popcll(m);
-      if (r >= 0 && r < c) {
-        const bool mine = n[k] > lo && (int32_t)__popcll(m & ((1ull << lane) - 1)) == r;
-        out.b = 64 * k + (int32_t)__builtin_ctzll(__ballot(mine));
+      if (r < c) {
+        const int src = __builtin_ctzll(__ballot(n[k] > lo && (int32_t)__popcll(m & below) == r));
+        out.b = 64 * k + src;
+        out.slot += (int32_t)__popcll(staged & ((1ull << src) - 1));
+        return true;
       }
-      r = r < c ? -1 : r - c;
-      if (r < 0) break;
+      r -= c;
+      out.slot += (int32_t)__popcll(staged);
     }
-    return true;
+    return false;
   }
   int32_t before = 0;
-  for (int32_t b0 = 0; b0 < B; b0 += 64) {
+  for (int32_t b0 = 0; b0 < p.B; b0 += 64) {
     const int32_t n = tiles_of(b0 + lane);
+    const uint64_t staged = PAGED ? __ballot(n > 0) : 0;
     int32_t incl = n;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -148,9 +160,11 @@ __device__ __forceinline__ bool find_tile(const int32_t *cu, int32_t B, int32_t 
       out.b = b0 + src;
       const int32_t count = __builtin_amdgcn_readlane(n, src), end = __builtin_amdgcn_readlane(incl, src);
       out.t = count - 1 - (rank - (before + end - count));
+      out.slot += (int32_t)__popcll(staged & ((1ull << src) - 1));
       return true;
     }
     before += total;
+    out.slot += (int32_t)__popcll(staged);
   }
   return false;
 }
@@ -184,7 +198,7 @@ struct IntConst {
 // MFMA, 0x100 LDS read, 0x400 transcendental).
 #define SCHED(mask, n) __builtin_amdgcn_sched_group_barrier(mask, n, 0)
 
-template <class E, int D, int NW>
+template <class E, int D, int NW, bool PAGED>
 __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p) {
   constexpr int TK = 64, R = 32 * NW;             // keys per tile, query rows per workgroup
   constexpr int RB = 2 * D, CPR = RB / 16;         // bytes and 16-byte pieces of an LDS row
@@ -195,35 +209,39 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
 
   const int lane = threadIdx.x & 63, n = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int32_t slot = (int32_t)(blockIdx.x % p.Hq);
+  // Workgroup i runs on XCD i % 8: a key head's workgroups share an XCD and its
+  // L2 where the heads deal out evenly.
+  const int32_t kvh = (int32_t)(blockIdx.x % p.Hk);
   Tile tile;
-  if (!find_tile<R>(p.cu, p.B, p.T, (int32_t)(blockIdx.x / p.Hq), tile)) return;
-  const int32_t b = __builtin_amdgcn_readfirstlane(tile.b);
-  const int32_t G = p.Hq / p.Hk;
-  // Workgroup i runs on XCD i % 8: the query heads of one key head share an
-  // XCD and its L2 where the heads deal out evenly.
-  int32_t kvh = slot / G, h = slot;
-  if (p.Hk % 8 == 0) {
-    kvh = (slot & 7) + 8 * ((slot >> 3) / G);
-    h = kvh * G + (slot >> 3) % G;
-  }
-  const int32_t s0 = min(max(p.cu[b], 0), p.T), len = min(max(p.cu[b + 1], s0), p.T) - s0;
+  if (!find_tile<R, PAGED>(p, (int32_t)(blockIdx.x / p.Hk), tile)) return;
+  const int32_t b = __builtin_amdgcn_readfirstlane(tile.b), slot = __builtin_amdgcn_readfirstlane(tile.slot);
+  if (PAGED && slot >= p.st.slots) return;  // sequences overlap
+  // The rows of a sequence and a key head: token i's G query heads are rows
+  // G i .. G i + G - 1. (So a tile spans few positions, its waves end with the
+  // same key tile, and short prompts fill tiles.) Positions: of the sequence,
+  // or over a cache the last ones of the context.
+  const Rows seq = rows_of(p.starts, p.T, b);
+  const int32_t rows = seq.n * p.G, ctx = PAGED ? p.ctx[b] : seq.n, pos0 = ctx - seq.n;
+  const int32_t len = PAGED ? min(ctx, p.max_tokens) : seq.n;  // keys
   const int32_t q0 = R * __builtin_amdgcn_readfirstlane(tile.t), qw0 = q0 + 32 * wave, qi = qw0 + n;
-  const bool q_ok = qi < len;
+  const bool q_ok = qi < rows;
+  const int32_t tok = p.by_g(min(qi, rows - 1)), qp = pos0 + tok;
+  const int64_t q_head = (int64_t)kvh * p.G + (min(qi, rows - 1) - tok * p.G);
+  auto pos_of = [&](int32_t row) { return pos0 + p.by_g(min(row, rows - 1)); };
 
   u32x4p_t qf[NCH];
 #pragma unroll
   for (int c = 0; c < NCH; ++c) qf[c] = (u32x4p_t){};
   if (q_ok) {
-    const uint16_t *src = p.q + (int64_t)(s0 + qi) * p.q_ts + h * p.q_hs + 8 * hl;
+    const uint16_t *src = p.q + (int64_t)(seq.start + tok) * p.q_ts + q_head * p.q_hs + 8 * hl;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) qf[c] = *reinterpret_cast<const u32x4p_t *>(src + 16 * c);
   }
 
   // Tiles of the workgroup: sinks, then the window of its rows.
-  const int32_t q_last = min(q0 + R, len) - 1, hi = q_last + 1;
+  const int32_t hi = max(0, min(len, pos_of(q0 + R - 1) + 1));
   const int32_t sink_tiles = (min(p.sinks, hi) + TK - 1) / TK;
-  const int32_t t_first = max(max(0, q0 - p.W + 1) / TK, sink_tiles), t_last = (hi + TK - 1) / TK;
+  const int32_t t_first = max(max(0, pos_of(q0) - p.W + 1) / TK, sink_tiles), t_last = (hi + TK - 1) / TK;
   const int32_t n_tiles = sink_tiles + max(0, t_last - t_first);
   auto tile_base = [&](int32_t it) { return (it < sink_tiles ? it : t_first + (it - sink_tiles)) * TK; };
 
@@ -240,8 +258,12 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
     k_off[c] = row * k_rb + 16 * (j ^ k_swz(row)) - c * 1024;
     v_off[c] = row * v_rb + 16 * (j ^ v_swz(row)) - c * 1024;
   }
-  const uint8_t *k_base = reinterpret_cast<const uint8_t *>(p.k + (int64_t)s0 * p.k_ts + kvh * p.k_hs);
-  const uint8_t *v_base = reinterpret_cast<const uint8_t *>(p.v + (int64_t)s0 * p.v_ts + kvh * p.v_hs);
+  const int64_t key_row = PAGED ? (int64_t)slot * p.st.cap : seq.start;
+  const uint8_t *k_base = reinterpret_cast<const uint8_t *>(p.k + key_row * p.k_ts + kvh * p.k_hs);
+  const uint8_t *v_base = reinterpret_cast<const uint8_t *>(p.v + key_row * p.v_ts + kvh * p.v_hs);
+  // Row of a position: staged copies leave out what lies between sinks and window.
+  const StagedMap sm = staged_map(len, pos0, p.W, p.sinks);
+  auto key_at = [&](int32_t pos) { return PAGED && pos >= sm.sink_end ? pos - sm.skip : pos; };
   const uint32_t wave_lds = (uint32_t)wave * NC * 1024;
   const uint32_t mk[2] = {lds_u32(lds_k0) + wave_lds, lds_u32(lds_k1) + wave_lds};
   const uint32_t mv[2] = {lds_u32(lds_v0) + wave_lds, lds_u32(lds_v1) + wave_lds};
@@ -249,7 +271,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
   // past the sequence lie outside its range and read as zeros.
   auto rows_at = [&](const uint8_t *base, uint32_t rb, int32_t key0) __attribute__((always_inline)) {
     const int32_t rows = min(TK, len - key0);
-    return __builtin_amdgcn_make_buffer_rsrc((void *)(base + (int64_t)key0 * rb), (short)0,
+    return __builtin_amdgcn_make_buffer_rsrc((void *)(base + (int64_t)key_at(key0) * rb), (short)0,
                                              (int)((rows - 1) * rb + RB), 0x00020000);
   };
   auto load_k = [&](int32_t it, int buf) __attribute__((always_inline)) {
@@ -279,28 +301,42 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
 
   // What this wave sees: the sink tiles and window iterations [v0, v1); of
   // those, iterations [f0, f1) hold window tiles that all its rows see whole.
-  const bool any = qw0 < len;
-  const int32_t w_last = min(qw0 + 31, len - 1);
+  const bool any = qw0 < rows;
   int32_t v0 = sink_tiles, v1 = sink_tiles, f0 = 0, f1 = 0;
   if (any) {
     const int32_t off = sink_tiles - t_first;  // iteration of tile t: t + off
-    v0 = max(sink_tiles, max(0, qw0 - p.W + 1) / TK + off);
-    v1 = max(v0, w_last / TK + 1 + off);
-    f0 = max(sink_tiles, (max(0, qw0 + 31 - p.W + 1) + TK - 1) / TK + off);
-    f1 = max(f0, (qw0 + 1) / TK + off);
+    const int32_t first = pos_of(qw0), last = pos_of(qw0 + 31);
+    v0 = max(sink_tiles, max(0, first - p.W + 1) / TK + off);
+    v1 = max(v0, max(0, min(last, len - 1) + TK) / TK + off);
+    f0 = max(sink_tiles, (max(0, last - p.W + 1) + TK - 1) / TK + off);
+    f1 = max(f0, max(0, min(first + 1, len)) / TK + off);
+  }
+  // Over a cache: one byte per 16 tokens, 1 where their page is there. If one
+  // in sight is not, every tile is masked.
+  const uint32_t *links = nullptr;
+  if constexpr (PAGED) {
+    links = reinterpret_cast<const uint32_t *>(p.st.links + (int64_t)slot * (p.st.cap / 16));
+    bool gap = false;
+    for (int32_t it = lane; it < n_tiles; it += 64) gap |= links[key_at(tile_base(it)) / TK] != 0x01010101u;
+    if (__any(gap)) f1 = f0;
   }
   auto sees = [&](int32_t it) { return it < sink_tiles ? any : it >= v0 && it < v1; };
 
   // Register r of block blk holds key tb + 32 blk + 8 (r / 4) + 4 hl + r % 4.
   auto apply_mask = [&](f32x16_t (&s)[2], int32_t tb) __attribute__((always_inline)) {
     const int32_t key0 = tb + 4 * hl;
-    const int32_t last = q_ok ? qi - key0 : -1, first = qi - p.W + 1 - key0, sink = p.sinks - key0;
+    const int32_t last = q_ok ? min(qp, len - 1) - key0 : -1, first = qp - p.W + 1 - key0, sink = p.sinks - key0;
+    const uint32_t link = PAGED ? links[key_at(tb) / TK] : 0x01010101u;
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int32_t c = 32 * blk + 8 * (r >> 2) + (r & 3);
-        s[blk][r] = (c <= last) & ((c >= first) | (c < sink)) ? s[blk][r] : -INFINITY;
+      for (int half = 0; half < 2; ++half) {
+        const int32_t end = !PAGED || ((link >> (16 * blk + 8 * half)) & 1) ? last : -1;
+#pragma unroll
+        for (int r = 8 * half; r < 8 * half + 8; ++r) {
+          const int32_t c = 32 * blk + 8 * (r >> 2) + (r & 3);
+          s[blk][r] = (c <= end) & ((c >= first) | (c < sink)) ? s[blk][r] : -INFINITY;
+        }
       }
   };
   auto row_max = [&](const f32x16_t (&s)[2]) __attribute__((always_inline)) {
@@ -551,8 +587,9 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
       const int32_t tb = tile_base(i);
 #pragma unroll 1
       for (int32_t key = tb; key < min(tb + TK, len); ++key) {
-        const uint16_t *row = reinterpret_cast<const uint16_t *>(v_base + (int64_t)key * v_rb) + 4 * hl;
-        const bool see = q_ok && key <= qi && (key < p.sinks || key > qi - p.W);
+        if (PAGED && p.st.links[(int64_t)slot * (p.st.cap / 16) + key_at(key) / 16] == 0) continue;
+        const uint16_t *row = reinterpret_cast<const uint16_t *>(v_base + (int64_t)key_at(key) * v_rb) + 4 * hl;
+        const bool see = q_ok && key <= qp && (key < p.sinks || key > qp - p.W);
 #pragma unroll
         for (int r = 0; r < 16 * NDB; ++r) {
           const uint16_t bits = row[8 * (r >> 2) + (r & 3)];
@@ -565,7 +602,12 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
   const float l = xor32_sum(lsum + lsum1);
   if (!q_ok) return;
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-  uint16_t *dst = p.out + (int64_t)(s0 + qi) * p.o_ts + h * p.o_hs + 4 * hl;
+  // (The row is worked out again from the lane: held through the tiles it spills.)
+  int32_t row = qw0 + (int32_t)(__lane_id() & 31);
+  asm volatile("" : "+v"(row));
+  const int32_t row_tok = p.by_g(row);
+  uint16_t *dst = p.out + (int64_t)(seq.start + row_tok) * p.o_ts + ((int64_t)kvh * p.G + row - row_tok * p.G) * p.o_hs +
+                  4 * hl;
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -575,10 +617,43 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
                    E::pack(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv)};
 }
 
+// Tiles of T tokens in B sequences, at most.
+static int64_t most_tiles(int64_t T, int64_t B, int64_t G) { return (T * G + 127 * std::min(B, T)) / 128; }
+
 template <class E, int D>
 static void launch_prompt(const PromptParams &p, hipStream_t stream) {
-  const int64_t tiles = ((int64_t)p.T + 127LL * std::min(p.B, p.T)) / 128;
-  hipLaunchKernelGGL((prompt_kernel<E, D, 4>), dim3((unsigned)(tiles * p.Hq)), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((prompt_kernel<E, D, 4, false>), dim3((unsigned)(most_tiles(p.T, p.B, p.G) * p.Hk)), dim3(256), 0,
+                     stream, p);
+}
+
+int launch_paged_tiles(const PagedTiles &d, hipStream_t stream) {
+  PromptParams p = {};
+  p.q = (const uint16_t *)d.q;
+  p.out = (uint16_t *)d.out;
+  p.q_ts = d.q_ts;
+  p.q_hs = d.q_hs;
+  p.o_ts = d.o_ts;
+  p.o_hs = d.o_hs;
+  p.k = (const uint16_t *)d.st.k;
+  p.v = (const uint16_t *)d.st.v;
+  p.k_hs = p.v_hs = d.D;
+  p.k_ts = p.v_ts = (int64_t)d.Hk * d.D;
+  p.starts = d.starts;
+  p.ctx = d.ctx;
+  p.T = d.T;
+  p.B = d.B;
+  p.Hk = d.Hk;
+  p.G = d.G;
+  p.by_g = Divisor::of((uint32_t)d.G);
+  p.W = d.W;
+  p.sinks = d.sinks;
+  p.max_tokens = d.max_tokens;
+  p.qk_scale_log2 = d.qk_scale_log2;
+  p.st = d.st;
+  const dim3 grid((unsigned)(most_tiles(d.T, std::min(d.B, d.st.slots), d.G) * d.Hk));
+  if (d.D == 128) hipLaunchKernelGGL((prompt_kernel<Fp16, 128, 4, true>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((prompt_kernel<Fp16, 64, 4, true>), grid, dim3(256), 0, stream, p);
+  return check_launch("packed_attention(tiles)");
 }
 
 }  // namespace memopt
@@ -610,7 +685,7 @@ extern "C" int memopt_prompt_attention(const memopt_prompt_desc *desc, void *str
   auto in_range = [&](int64_t ts) { return ts >= d.head_dim && ts < (1LL << 23); };
   MEMOPT_REQUIRE(in_range(d.k_token_stride) && in_range(d.v_token_stride), MEMOPT_ERR_UNSUPPORTED,
                  "prompt_attention: key and value token strides must be head_dim to 2^23 - 1 elements");
-  PromptParams p;
+  PromptParams p = {};
   p.q = (const uint16_t *)d.query;
   p.k = (const uint16_t *)d.key;
   p.v = (const uint16_t *)d.value;
@@ -623,16 +698,18 @@ extern "C" int memopt_prompt_attention(const memopt_prompt_desc *desc, void *str
   p.v_hs = d.v_head_stride;
   p.o_ts = d.o_token_stride;
   p.o_hs = d.o_head_stride;
-  p.cu = d.query_starts;
+  p.starts = d.query_starts;
   p.T = d.tokens;
   p.B = d.batch;
-  p.Hq = d.num_heads;
   p.Hk = d.num_kv_heads;
+  p.G = d.num_heads / d.num_kv_heads;
+  p.by_g = Divisor::of((uint32_t)p.G);
   p.W = d.window_size <= 0 ? 1 << 30 : std::min(d.window_size, 1 << 30);  // (position - W stays in 32 bits)
   p.sinks = std::max(0, d.num_sink_tokens);
   p.qk_scale_log2 = 1.4426950408889634f / sqrtf((float)d.head_dim);
-  MEMOPT_REQUIRE(((int64_t)d.tokens / 32 + d.batch) * d.num_heads < (1LL << 31), MEMOPT_ERR_UNSUPPORTED,
-                 "prompt_attention: too many query tiles");
+  MEMOPT_REQUIRE((int64_t)d.tokens * d.num_heads < (1LL << 31) &&
+                     most_tiles(d.tokens, d.batch, p.G) * d.num_kv_heads < (1LL << 31),
+                 MEMOPT_ERR_UNSUPPORTED, "prompt_attention: too many query rows");
   hipStream_t s = (hipStream_t)stream;
   if (d.dtype == MEMOPT_FP16) {
     if (d.head_dim == 128) launch_prompt<Fp16, 128>(p, s);

@@ -34,7 +34,7 @@ def attend(q, k, v, pos, window, sinks, live=None):
     return o, a, e
 
 
-def tolerance(o, a, e, keys, D, out_dtype, p_dtype, v_rounded):
+def tolerance(o, a, e, keys, D, out_dtype, p_dtype, v_rounded, scores=0.0):
     """What the kernels' roundings may add up to, element by element.
 
     * the output: half a step of its type;
@@ -43,12 +43,23 @@ def tolerance(o, a, e, keys, D, out_dtype, p_dtype, v_rounded):
     * v_rounded: V itself is rounded once to fp16 (code * scale): half a step of a;
     * scores: D products summed in 32 bits, two fused scalings and the running maximum: D + 16 roundings of
       e at 2^-24, which move every weight by that much relative (natural exponent), numerator and sum: twice;
+    * scores: what else moves a score, absolute (quantized_scores): twice a's share again;
     * exp2 itself: 2^-22 relative, twice; the sums over the keys: at most keys 32-bit additions each.
     """
     u = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
     t = u[out_dtype] * o.abs() + 2 * u[p_dtype] * a + (2.0 ** -11 * a if v_rounded else 0)
-    t = t + 2 * (D + 16) * 2.0 ** -24 * e * a + (2 * 2.0 ** -22 + 2 * keys * 2.0 ** -24) * a
+    t = t + 2 * (D + 16) * 2.0 ** -24 * e * a + 2 * scores * a + (2 * 2.0 ** -22 + 2 * keys * 2.0 ** -24) * a
     return t + 2.0 ** -24 + keys * 2.0 ** -32 * a  # (2^-24: half a step of fp16's subnormals)
+
+
+def quantized_scores(q, e, scale, staged):
+    """By how much scores over INT4 keys may be off beyond the sums' own roundings, for q [n, Hq, D] and scales up
+    to ``scale``. Staged chunks read keys rounded to fp16: half a step of every product, so 2^-11 e. Others sum
+    codes that stand 1032 (or 72) too high, so that a partial sum is up to (1032 + 7) sum_d |q_d| before the scale,
+    with D + 16 roundings of it at 2^-24."""
+    n, Hq, D = q.shape
+    biased = 1039.0 * (D + 16) * 2.0 ** -24 * scale / D ** 0.5 * q.double().cpu().abs().sum(-1, keepdim=True)
+    return 2.0 ** -11 * e if staged else biased
 
 
 def check(got, want, tol, what=""):

@@ -5,11 +5,13 @@ import pytest
 import torch
 
 from gpu_helpers import dev, memopt_C
-from packed_reference import attend, check, starts, tolerance
+from packed_reference import attend, check, quantized_scores, starts, tolerance
 
 pytestmark = pytest.mark.gpu
 
 FORMATS = ["int4", "fp16"]
+STAGED = 512  # rows (tokens times query heads per key head) from which a chunk attends from a staged copy
+FILL = 128 * 256  # and rows of the whole batch over all key heads: a tile of 128 for each compute unit
 
 
 class Case:
@@ -60,11 +62,19 @@ class Case:
             pages = torch.from_numpy(self.tables[b, :-(-m // self.bs)]).long()
             live = (pages >= 0) & (pages < self.k.shape[0])
             k, v = (x[pages.clamp(0, self.k.shape[0] - 1)].flatten(0, 1)[:m] for x in (self.kval, self.vval))
-            o, w, e = attend(self.q[a:a + n], k, v, np.arange(c - n, c), window, sinks,
+            some = np.arange(n)
+            if n > 150:  # the first and last rows, and some of those between
+                some = np.unique(np.concatenate([np.arange(20), n - 1 - np.arange(20), np.random.default_rng(n).integers(0, n, 30)]))
+            o, w, e = attend(self.q[a:a + n][some], k, v, (c - n) + some, window, sinks,
                              live.repeat_interleave(self.bs)[:m])
-            tol = tolerance(o, w, e, m, self.D, torch.float16, torch.float16, self.fmt == "int4")
-            r = slice(None) if rows is None else rows[a:a + n]
-            check(out[a:a + n].cpu()[r], o[r], tol[r], f"sequence {b}")
+            scores = 0.0
+            if self.fmt == "int4":
+                G = self.q.shape[1] // self.k.shape[2]
+                staged = n * G >= STAGED and self.q.shape[0] * self.q.shape[1] >= FILL
+                scores = quantized_scores(self.q[a:a + n][some], e, float(self.kval.abs().max()) / 7, staged)
+            tol = tolerance(o, w, e, m, self.D, torch.float16, torch.float16, self.fmt == "int4", scores)
+            r = slice(None) if rows is None else rows[a:a + n][some]
+            check(out[a:a + n].cpu()[some][r], o[r], tol[r], f"sequence {b}")
             a += n
 
 
@@ -136,6 +146,118 @@ def test_unlinked_pages_and_entries_past_the_pool(fmt, D):
     out = memopt_C.packed_attention(*c.args())
     c.check(out)
     assert bool((out[-1] == 0).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("Hq,Hk,D,ctx,qn", [(64, 1, 128, [200, 700, 65, 300], [192, 7, 65, 250]),
+                                            (32, 2, 64, [640, 400, 333, 40], [640, 400, 31, 32]),
+                                            (30, 10, 64, [1, 300, 5, 1000], [1, 171, 5, 920]),
+                                            (32, 8, 128, [900, 127, 128, 5], [897, 127, 128, 1])])
+def test_long_chunks(fmt, Hq, Hk, D, ctx, qn):
+    """Chunks on both sides of the length from which they attend from a staged copy, beside single tokens."""
+    c = Case(fmt, ctx, qn, Hq, Hk, D, seed=Hq + qn[0])
+    assert sum(qn) * Hq >= FILL
+    plan = memopt_C.PreparedPackedAttention(*c.args())
+    for _ in range(2):
+        plan.out.fill_(float("nan"))
+        c.check(plan())
+    c.check(memopt_C.packed_attention(*c.args(window=90), num_sink_tokens=7), 90, 7)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("window,sinks", [(1, 0), (64, 0), (63, 64), (130, 65), (17, 200), (5, 2 ** 31 - 1),
+                                          (2 ** 31 - 1, 3)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_chunks_windows_and_sinks(fmt, window, sinks, D):
+    c = Case(fmt, [640, 90, 250], [300, 4, 220], 64, 1, D, seed=window % 100 + sinks % 7)
+    out = memopt_C.packed_attention(*c.args(window=window), num_sink_tokens=sinks)
+    c.check(out, min(window, c.M * 16), sinks)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_chunks_unlinked_pages(fmt, D):
+    c = Case(fmt, [500, 320, 100, 257], [250, 100, 1, 257], 64, 1, D, seed=3)
+    c.tables[0, 3] = c.tables[0, 20] = c.tables[0, 31] = -1
+    c.tables[1, :5] = 10 ** 6
+    c.tables[3, :] = -7  # nothing left: zeros
+    c.load()
+    out = memopt_C.packed_attention(*c.args())
+    c.check(out)
+    assert bool((out[-257:] == 0).all())
+    c.check(memopt_C.packed_attention(*c.args(window=70), num_sink_tokens=60), 70, 60)
+
+
+@pytest.mark.parametrize("bs", [32, 48, 64])
+def test_long_chunks_fp16_page_sizes(bs):
+    c = Case("fp16", [830, 297, 200], [730, 297, 1], 32, 2, 64, seed=bs, bs=bs)
+    c.check(memopt_C.packed_attention(*c.args()))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_long_chunks_outside_the_block_table(fmt):
+    """More queries than context, and contexts past the table: the keys that the table holds."""
+    c = Case(fmt, [64, 64, 20], [200, 200, 200], 64, 1, 64, seed=3, M=4)
+    c.ctx = [70, 1000, -3]
+    c.load()
+    c.check(memopt_C.packed_attention(*c.args()[:7], 2000, -1), 2000, 0)
+    c.ctx = [300, 150, 201]
+    c.load()
+    c.check(memopt_C.packed_attention(*c.args()[:7], 2000, 100), 100, 0)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_long_chunks_among_many_sequences(fmt):
+    qn = [1 + 59 * (i % 5 == 1) for i in range(70)]
+    c = Case(fmt, [100 + 3 * (i % 11) for i in range(70)], qn, 64, 2, 64, seed=9)
+    c.check(memopt_C.packed_attention(*c.args()))
+    qn = [1] * 290 + [120, 0, 140]
+    c = Case(fmt, [2] * 290 + [120, 9, 333], qn, 64, 2, 64, seed=9)
+    c.check(memopt_C.packed_attention(*c.args()))
+
+
+def test_long_chunks_of_more_sequences_than_are_staged():
+    """Block tables of 2^20 tokens leave room for copies of four sequences: only chunks that must be among four."""
+    for qn in ([100] * 6, [100, 97, 300, 100, 1, 1]):
+        c = Case("int4", [320, 100, 310, 100, 100, 101], qn, 64, 2, 64, seed=4, M=65536)
+        c.check(memopt_C.packed_attention(*c.args()))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("window,sinks", [(-1, 0), (70, 3)])
+def test_long_chunks_odd_values_reach_only_the_rows_that_see_them(fmt, window, sinks):
+    def case():
+        return Case(fmt, [600, 70], [510, 10], 64, 1, 64, seed=11)
+
+    good, lay = case(), memopt_C.int4_layout(64)
+    W = window if window > 0 else good.M * 16
+    pos = torch.arange(90, 600)
+    for token, bad, where in [(160, float("nan"), "v"), (599, float("inf"), "v"), (95, float("nan"), "k"),
+                              (64, float("nan"), "kv"), (0, float("nan"), "v"), (128, float("nan"), "v")]:
+        c = case()
+        page, row = c.tables[0, token // 16], token % 16
+        for x in where:
+            if fmt == "fp16":
+                (c.kc if x == "k" else c.vc)[page, row, :, 33] = bad
+            else:
+                c.kc.view(torch.float16)[page, :, lay[x + "scales"] // 2 + 2 * (row % 8) + row // 8] = bad
+        out = memopt_C.packed_attention(*c.args(window=window), num_sink_tokens=sinks)
+        see = (token <= pos) & ((pos - token < window) | (token < sinks)) if window > 0 else token <= pos
+        see = torch.cat([see, torch.zeros(10, dtype=torch.bool)])
+        good.check(out, W, sinks, ~see)
+        hit = out[see.to(dev())]
+        if hit.numel():
+            assert bool((~hit[..., 33].isfinite()).all()), (token, bad, where)
+    # behind the context
+    want = memopt_C.packed_attention(*good.args(window=window), num_sink_tokens=sinks)
+    tail = good.tables[0, 600 // 16]
+    if fmt == "fp16":
+        good.kc[tail, 600 % 16:] = good.vc[tail, 600 % 16:] = float("nan")
+    else:
+        for x in ("kscales", "vscales"):
+            for row in range(600 % 16, 16):
+                good.kc.view(torch.float16)[tail, :, lay[x] // 2 + 2 * (row % 8) + row // 8] = float("nan")
+    assert torch.equal(memopt_C.packed_attention(*good.args(window=window), num_sink_tokens=sinks), want)
 
 
 @pytest.mark.parametrize("bs", [16, 32, 48, 64])
@@ -263,7 +385,8 @@ def test_pool_views_are_taken(fmt):
         assert torch.equal(memopt_C.packed_attention(q, buf, buf, bt, cl, cu, 1, 112), out)
         k, v = (x[1:].flatten(0, 1)[:100] for x in page_values(buf.cpu().numpy(), 64))
     o, w, e = attend(q, k, v, [99], -1, 0)
-    check(out, o, tolerance(o, w, e, 100, 64, torch.float16, torch.float16, fmt == "int4"))
+    scores = quantized_scores(q, e, float(k.abs().max()) / 7, False) if fmt == "int4" else 0.0
+    check(out, o, tolerance(o, w, e, 100, 64, torch.float16, torch.float16, fmt == "int4", scores))
 
 
 def test_same_heads_agree_with_the_paged_attention():
