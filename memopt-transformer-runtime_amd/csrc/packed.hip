@@ -856,7 +856,8 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
 // takes tiles i, i + gridDim, ..., each wave 16 tokens of them, which lie in
 // one page. A wave reads a block of a page as it is (lane l: the 16 dims (D =
 // 64: 8) of tokens p = l / 8 and p + 8 that start at D / 8 * (l % 8)) and writes
-// fp16((code - 8) * scale): one rounding, as in the V operands above.
+// V as fp16((code - 8) * scale), one rounding, as in the operands above, and K
+// as codes with their factors.
 template <int D, int FMT>
 __global__ __launch_bounds__(256) void stage_kernel(const PackedParams p, const int32_t *__restrict__ starts,
                                                     const int32_t *__restrict__ ctxs,
@@ -916,22 +917,40 @@ __global__ __launch_bounds__(256) void stage_kernel(const PackedParams p, const 
           ks = *reinterpret_cast<const uint32_t *>(blk + f.kscales + 2 * f.scale_idx(t, d0 / 64));
           vs = *reinterpret_cast<const uint32_t *>(blk + f.vscales + 2 * f.scale_idx(t, d0 / 64));
         }
-        auto unpack = [&](uint32_t w, uint32_t s, uint32_t (&y)[4]) __attribute__((always_inline)) {
+        auto unpack = [&](uint32_t w, uint32_t (&y)[4]) __attribute__((always_inline)) {
           const half2_t b1032 = {(half_t)1032.0f, (half_t)1032.0f}, b72 = {(half_t)72.0f, (half_t)72.0f};
           const uint32_t w8 = w >> 8;
-          y[0] = as_u32((as_half2((w & 0x000F000Fu) | 0x64006400u) - b1032) * as_half2(s));
-          y[1] = as_u32((as_half2((w & 0x00F000F0u) | 0x54005400u) - b72) * as_half2(s));
-          y[2] = as_u32((as_half2((w8 & 0x000F000Fu) | 0x64006400u) - b1032) * as_half2(s));
-          y[3] = as_u32((as_half2((w8 & 0x00F000F0u) | 0x54005400u) - b72) * as_half2(s));
+          y[0] = as_u32(as_half2((w & 0x000F000Fu) | 0x64006400u) - b1032);
+          y[1] = as_u32(as_half2((w & 0x00F000F0u) | 0x54005400u) - b72);
+          y[2] = as_u32(as_half2((w8 & 0x000F000Fu) | 0x64006400u) - b1032);
+          y[3] = as_u32(as_half2((w8 & 0x00F000F0u) | 0x54005400u) - b72);
         };
+        auto scaled = [&](uint32_t w, uint32_t (&y)[4]) __attribute__((always_inline)) {
+          unpack(w, y);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = as_u32(as_half2(y[i]) * as_half2(vs));
+        };
+        if (lane < 16) {  // token `lane`
+          float first = 0.0f, last = 0.0f;
+          if (ok) {
+            const half_t *sc = reinterpret_cast<const half_t *>(p.k + (int64_t)phys * p.kv_ps + kvh * p.kv_hs + f.kscales);
+            first = (float)sc[f.scale_idx(lane, 0)];
+            last = (float)sc[f.scale_idx(lane, D / 64 - 1)];
+          }
+          // (a scale of 0 makes zeros of its codes below; if the last is, the first serves both)
+          float *const dst = p.st.factors + ((int64_t)slot * p.Hk + kvh) * 2 * p.st.cap + row + lane;
+          dst[0] = last == 0.0f ? 1.0f : first / last;
+          dst[p.st.cap] = (last == 0.0f ? first : last) * p.qk_scale_log2;
+        }
         constexpr uint32_t LO = 0x05040100u, HI = 0x07060302u;
         half_t *const ko = p.st.k + out + t * ts + d0, *const vo = p.st.v + out + t * ts + d0;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          const bool gone = ((h ? ks >> 16 : ks) & 0x7FFFu) == 0;
 #pragma unroll
           for (int j = 0; j < W; ++j) {
             uint32_t y[4];
-            unpack(kw[h][j], __builtin_amdgcn_perm(ks, ks, h ? 0x03020302u : 0x01000100u), y);
+            unpack(gone ? 0x88888888u : kw[h][j], y);
             *reinterpret_cast<u32x4_t *>(ko + 8 * h * ts + 8 * j) =
                 u32x4_t{__builtin_amdgcn_perm(y[1], y[0], LO), __builtin_amdgcn_perm(y[3], y[2], LO),
                         __builtin_amdgcn_perm(y[1], y[0], HI), __builtin_amdgcn_perm(y[3], y[2], HI)};
@@ -940,8 +959,8 @@ __global__ __launch_bounds__(256) void stage_kernel(const PackedParams p, const 
 #pragma unroll
         for (int j = 0; j < W; ++j) {
           uint32_t y[4], z[4];
-          unpack(vw[2 * j], vs, y);
-          unpack(vw[2 * j + 1], vs, z);
+          scaled(vw[2 * j], y);
+          scaled(vw[2 * j + 1], z);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t sel = h ? HI : LO;
@@ -1037,7 +1056,7 @@ static PackedPlan packed_plan(const memopt_packed_desc &d) {
 }
 
 struct PackedWorkspace {
-  int64_t counters, ml, links, k, v, total;  // bytes of the counters; offsets of the (m, l) pairs and the staged copies
+  int64_t counters, ml, links, factors, k, v, total;  // bytes of the counters; offsets of the (m, l) pairs and the staged copies
 };
 static PackedWorkspace packed_workspace(const memopt_packed_desc &d, const PackedPlan &pl) {
   PackedWorkspace w;
@@ -1046,7 +1065,9 @@ static PackedWorkspace packed_workspace(const memopt_packed_desc &d, const Packe
   w.ml = w.counters + rows * d.head_dim * 4;
   auto up256 = [](int64_t x) { return (x + 255) / 256 * 256; };
   w.links = up256(w.ml + rows * 8);
-  w.k = up256(w.links + pl.slots * pl.cap / 16);
+  w.factors = up256(w.links + pl.slots * pl.cap / 16);
+  w.k = w.factors;
+  if (d.kv_format == MEMOPT_KV_INT4) w.k = up256(w.factors + pl.slots * pl.cap * d.num_kv_heads * 8);
   const int64_t staged = pl.slots * pl.cap * d.num_kv_heads * d.head_dim * 2;
   w.v = w.k + staged;
   w.total = w.v + staged;
@@ -1173,7 +1194,8 @@ extern "C" int memopt_packed_attention(const memopt_packed_desc *desc, void *str
   if (pl.slots > 0) {
     uint8_t *const ws = (uint8_t *)d.workspace;
     p.st = {pl.min_rows, std::min(d.max_query_len, d.tokens), pl.slots, (int32_t)pl.cap, (half_t *)(ws + w.k),
-            (half_t *)(ws + w.v), ws + w.links};
+            (half_t *)(ws + w.v), ws + w.links,
+            d.kv_format == MEMOPT_KV_INT4 ? (float *)(ws + w.factors) : nullptr};
     const unsigned wgs = (unsigned)std::max<int64_t>(1, std::min<int64_t>(8LL * compute_units() / p.Hk, pl.slots * pl.cap / 64));
     const dim3 grid(wgs * p.Hk);
     if (d.head_dim == 128) launch_stage<128>(p, d, grid, s);

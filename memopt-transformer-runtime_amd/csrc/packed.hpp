@@ -37,11 +37,17 @@ __device__ __forceinline__ Rows rows_of(const int32_t *starts, int32_t T, int32_
 // K and V as fp16 [slot][cap tokens][Hk][D], slot = the sequence's rank among
 // them. Tokens [0, sinks) and the window lie one behind the other, each from a
 // multiple of 64; links has one byte per 16 tokens, 1 where their page is there.
+// From INT4 pages, K are the codes less 8, which fp16 holds exactly; factors
+// [slot][Hk][2][cap] make scores of their sums: the scale of a key's first
+// group over that of its last (D = 64 has one group: not used), and the last
+// one's scale times qk_scale_log2. (Rounding K to fp16 instead was the largest
+// error of the operator, 6.7e-4 of the output's norm; 3.0e-4 is left.)
 struct Staged {
   int32_t min_rows, max_query;  // rows from which a sequence is staged; queries a slot has room for
   int32_t slots, cap;           // sequences, tokens per slot (a multiple of 64)
   half_t *k, *v;
   uint8_t *links;
+  float *factors;  // null: K holds values
 };
 __device__ __forceinline__ bool is_staged(const Staged &s, int32_t n, int32_t G) {
   return s.slots > 0 && (int64_t)n * G >= s.min_rows && n <= s.max_query;

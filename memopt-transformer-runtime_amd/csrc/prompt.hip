@@ -20,6 +20,7 @@ namespace memopt {
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4p_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2p_t __attribute__((ext_vector_type(2)));
+typedef float f32x4p_t __attribute__((ext_vector_type(4)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 
 struct PromptParams {
@@ -198,14 +199,22 @@ struct IntConst {
 // MFMA, 0x100 LDS read, 0x400 transcendental).
 #define SCHED(mask, n) __builtin_amdgcn_sched_group_barrier(mask, n, 0)
 
-template <class E, int D, int NW, bool PAGED>
+// Where keys and values come from: the packed rows themselves, or for chunks
+// over a cache their staged copies, of fp16 values or of codes and factors.
+enum Source { kPacked, kStagedRows, kStagedCodes };
+
+template <class E, int D, int NW, Source FROM>
 __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p) {
+  constexpr bool PAGED = FROM != kPacked, CODES = FROM == kStagedCodes;
   constexpr int TK = 64, R = 32 * NW;             // keys per tile, query rows per workgroup
   constexpr int RB = 2 * D, CPR = RB / 16;         // bytes and 16-byte pieces of an LDS row
   constexpr int NCH = D / 16, NDB = D / 32;
   constexpr int RPC = 1024 / RB, NC = TK / RPC / NW;  // rows per copy; copies per wave of K (and of V)
   __shared__ __attribute__((aligned(16))) uint8_t lds_k0[TK * RB], lds_k1[TK * RB], lds_v0[TK * RB],
       lds_v1[TK * RB];
+  // Codes: per key of a tile the factors' ratio, then the second factor (Staged::factors).
+  constexpr int FB = 2 * TK * 4;
+  __shared__ __attribute__((aligned(16))) uint8_t lds_f[CODES ? 2 * FB : 16];
 
   const int lane = threadIdx.x & 63, n = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -276,6 +285,14 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
   };
   auto load_k = [&](int32_t it, int buf) __attribute__((always_inline)) {
     lds_dma_range<0, NC>(rows_at(k_base, k_rb, tile_base(it)), mk[buf], k_off, 0);
+    if constexpr (CODES) {
+      if (wave == buf && lane < FB / 16) {  // (either buffer's by one wave; both lists of a tile in one copy)
+        const float *f = p.st.factors + ((int64_t)slot * p.Hk + kvh) * 2 * p.st.cap + key_at(tile_base(it));
+        const uint32_t off[1] = {(lane < FB / 32 ? 0u : 4u * p.st.cap - FB / 2) + 16u * lane};
+        lds_dma<0, 1>(__builtin_amdgcn_make_buffer_rsrc((void *)f, (short)0, (int)(4 * p.st.cap + FB / 2), 0x00020000),
+                      lds_u32(lds_f) + buf * FB, off, 0);
+      }
+    }
   };
   auto load_v = [&](int32_t it, int buf) __attribute__((always_inline)) {
     lds_dma_range<0, NC>(rows_at(v_base, v_rb, tile_base(it)), mv[buf], v_off, 0);
@@ -347,9 +364,33 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
     for (int r = 0; r < 16; ++r) t = fmaxf(t, s[1][r]);
     return both_halves_max(t);
   };
-  auto to_x = [&](f32x16_t &s) __attribute__((always_inline)) {
+  // Four keys' factors: list 0 or 1 of buffer fb, registers 4 i .. 4 i + 3 of block blk.
+  auto factors = [&](int fb, int list, int blk, int i) __attribute__((always_inline)) {
+    return *reinterpret_cast<const f32x4p_t *>(lds_f + fb * FB + list * (FB / 2) + 4 * (32 * blk + 8 * i + 4 * hl));
+  };
+  auto to_x = [&](f32x16_t &s, int fb, int blk) __attribute__((always_inline)) {
+    if constexpr (CODES) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], p.qk_scale_log2, ncm);
+      for (int i = 0; i < 4; ++i) {
+        const f32x4p_t f = factors(fb, 1, blk, i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[4 * i + j] = fmaf(s[4 * i + j], f[j], ncm);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], p.qk_scale_log2, ncm);
+    }
+  };
+  // Codes of two scale groups (D = 128): the first group's sum is brought to
+  // the second's factor before that group is added to it.
+  constexpr bool SPLIT = CODES && D == 128;
+  auto to_second = [&](f32x16_t &s, int fb, int blk) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4p_t f = factors(fb, 0, blk, i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[4 * i + j] *= f[j];
+    }
   };
   auto raise_max = [&](float t, f32x16_t (&s)[2]) __attribute__((always_inline)) {
     if (__any(t > thr)) {
@@ -398,6 +439,32 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
     for (int c = 0; c < NCH; ++c)
       acc = E::mfma((decltype(prec)::value && c < 4) ? pre[c] : kfrag(kt, blk, c), qf[c], c == 0 ? (f32x16_t){} : acc);
   };
+  // Half of both blocks' products: scale group G of both.
+  auto qk_group = [&](const uint8_t *kt, auto group, f32x16_t (&acc)[2], const u32x4p_t (&pre)[4])
+                      __attribute__((always_inline)) {
+    constexpr int G = decltype(group)::value;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int blk = i / (NCH / 2), c = G * (NCH / 2) + i % (NCH / 2);
+      acc[blk] = E::mfma(G == 1 && i < 4 ? pre[i] : kfrag(kt, blk, c), qf[c], c == 0 ? (f32x16_t){} : acc[blk]);
+    }
+  };
+  auto scores = [&](const uint8_t *kt, int fb, f32x16_t (&s)[2]) __attribute__((always_inline)) {
+    u32x4p_t pre[4] = {};
+    if constexpr (SPLIT) {
+      qk_group(kt, IntConst<0>{}, s, pre);
+      to_second(s[0], fb, 0);
+      to_second(s[1], fb, 1);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) pre[c] = kfrag(kt, 0, NCH / 2 + c);
+      qk_group(kt, IntConst<1>{}, s, pre);
+    } else {
+      qk_block(kt, 0, s[0], IntConst<0>{}, pre);
+      qk_block(kt, 1, s[1], IntConst<0>{}, pre);
+    }
+    to_x(s[0], fb, 0);
+    to_x(s[1], fb, 1);
+  };
   auto pv_block = [&](const uint8_t *vt, int blk, const u32x4p_t (&pb)[2], const u32x4p_t (&pre)[4])
                       __attribute__((always_inline)) {
 #pragma unroll
@@ -425,11 +492,12 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
     u32x4p_t pre_k[4], pre_a[4], pre_b[4], pa[2], pb[2];
     if (it + 2 < n_tiles) load_k(it + 2, P);
     __builtin_amdgcn_s_setprio(1);
-    // QK(it + 1) block 0 | maximum of x(it)
-    qk_block(kt, 0, sn[0], IntConst<0>{}, none);
+    // QK(it + 1) block 0 (or group 0) | maximum of x(it)
+    if constexpr (SPLIT) qk_group(kt, IntConst<0>{}, sn, none);
+    else qk_block(kt, 0, sn[0], IntConst<0>{}, none);
     const float t = row_max(sc);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) pre_k[c] = kfrag(kt, 1, c);
+    for (int c = 0; c < 4; ++c) pre_k[c] = SPLIT ? kfrag(kt, 0, NCH / 2 + c) : kfrag(kt, 1, c);
     SCHED(0x100, 4);
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
@@ -439,8 +507,15 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
     }
     __builtin_amdgcn_sched_barrier(0);
     raise_max(t, sc);
-    // QK(it + 1) block 1 | probabilities of block 0
-    qk_block(kt, 1, sn[1], IntConst<1>{}, pre_k);
+    // QK(it + 1) block 1 (or group 1) | probabilities of block 0
+    if constexpr (SPLIT) {
+      to_second(sn[0], P ^ 1, 0);
+      to_second(sn[1], P ^ 1, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      qk_group(kt, IntConst<1>{}, sn, pre_k);
+    } else {
+      qk_block(kt, 1, sn[1], IntConst<1>{}, pre_k);
+    }
     probs(sc[0], pa, lsum);
 #pragma unroll
     for (int i = 0; i < 4; ++i) pre_a[i] = vfrag(vt, 0, i);
@@ -471,12 +546,13 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
     __builtin_amdgcn_sched_barrier(0);
     // PV(it) block 1 | x(it + 1)
     pv_block(vt, 1, pb, pre_b);
-    to_x(sn[0]);
-    to_x(sn[1]);
+    to_x(sn[0], P ^ 1, 0);
+    to_x(sn[1], P ^ 1, 1);
 #pragma unroll
     for (int c = 0; c < 2 * NDB; ++c) {
       SCHED(0x008, 1);
       if (c < 2 * NDB - 4) SCHED(0x100, 2);
+      if (CODES) SCHED(0x100, 8 / (2 * NDB));
       SCHED(0x002, 32 / (2 * NDB));
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -489,7 +565,6 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
   auto iter_edge = [&](int32_t it, f32x16_t (&sc)[2], f32x16_t (&sn)[2], auto pc) __attribute__((always_inline)) {
     constexpr int P = decltype(pc)::value;
     const uint8_t *const kt = P ? lds_k0 : lds_k1, *const vt = P ? lds_v1 : lds_v0;
-    const u32x4p_t none[4] = {};
     if (it + 2 < n_tiles) load_k(it + 2, P);
     if (it + 1 < n_tiles) load_v(it + 1, P ^ 1);
     if (sees(it)) {
@@ -516,10 +591,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
       }
     }
     if (it + 1 < n_tiles && sees(it + 1)) {
-      qk_block(kt, 0, sn[0], IntConst<0>{}, none);
-      qk_block(kt, 1, sn[1], IntConst<0>{}, none);
-      to_x(sn[0]);
-      to_x(sn[1]);
+      scores(kt, P ^ 1, sn);
     } else {
       sn[0] = (f32x16_t){};
       sn[1] = (f32x16_t){};
@@ -533,12 +605,8 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
     load_v(0, 0);
     if (n_tiles > 1) load_k(1, 1);
     publish();
-    const u32x4p_t none[4] = {};
     if (sees(0)) {
-      qk_block(lds_k0, 0, sx[0], IntConst<0>{}, none);
-      qk_block(lds_k0, 1, sx[1], IntConst<0>{}, none);
-      to_x(sx[0]);
-      to_x(sx[1]);
+      scores(lds_k0, 0, sx);
     } else {
       sx[0] = (f32x16_t){};
       sx[1] = (f32x16_t){};
@@ -622,7 +690,7 @@ static int64_t most_tiles(int64_t T, int64_t B, int64_t G) { return (T * G + 127
 
 template <class E, int D>
 static void launch_prompt(const PromptParams &p, hipStream_t stream) {
-  hipLaunchKernelGGL((prompt_kernel<E, D, 4, false>), dim3((unsigned)(most_tiles(p.T, p.B, p.G) * p.Hk)), dim3(256), 0,
+  hipLaunchKernelGGL((prompt_kernel<E, D, 4, kPacked>), dim3((unsigned)(most_tiles(p.T, p.B, p.G) * p.Hk)), dim3(256), 0,
                      stream, p);
 }
 
@@ -651,8 +719,13 @@ int launch_paged_tiles(const PagedTiles &d, hipStream_t stream) {
   p.qk_scale_log2 = d.qk_scale_log2;
   p.st = d.st;
   const dim3 grid((unsigned)(most_tiles(d.T, std::min(d.B, d.st.slots), d.G) * d.Hk));
-  if (d.D == 128) hipLaunchKernelGGL((prompt_kernel<Fp16, 128, 4, true>), grid, dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((prompt_kernel<Fp16, 64, 4, true>), grid, dim3(256), 0, stream, p);
+  if (d.st.factors) {
+    if (d.D == 128) hipLaunchKernelGGL((prompt_kernel<Fp16, 128, 4, kStagedCodes>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((prompt_kernel<Fp16, 64, 4, kStagedCodes>), grid, dim3(256), 0, stream, p);
+  } else {
+    if (d.D == 128) hipLaunchKernelGGL((prompt_kernel<Fp16, 128, 4, kStagedRows>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((prompt_kernel<Fp16, 64, 4, kStagedRows>), grid, dim3(256), 0, stream, p);
+  }
   return check_launch("packed_attention(tiles)");
 }
 

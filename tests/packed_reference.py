@@ -52,14 +52,14 @@ def tolerance(o, a, e, keys, D, out_dtype, p_dtype, v_rounded, scores=0.0):
     return t + 2.0 ** -24 + keys * 2.0 ** -32 * a  # (2^-24: half a step of fp16's subnormals)
 
 
-def quantized_scores(q, e, scale, staged):
+def quantized_scores(q, scale, staged):
     """By how much scores over INT4 keys may be off beyond the sums' own roundings, for q [n, Hq, D] and scales up
-    to ``scale``. Staged chunks read keys rounded to fp16: half a step of every product, so 2^-11 e. Others sum
-    codes that stand 1032 (or 72) too high, so that a partial sum is up to (1032 + 7) sum_d |q_d| before the scale,
-    with D + 16 roundings of it at 2^-24."""
-    n, Hq, D = q.shape
+    to ``scale``. Staged chunks sum exact codes, and their factors add three roundings to those counted for the
+    sums. Others sum codes that stand 1032 (or 72) too high, so that a partial sum is up to (1032 + 7) sum_d |q_d|
+    before the scale, with D + 16 roundings of it at 2^-24."""
+    D = q.shape[2]
     biased = 1039.0 * (D + 16) * 2.0 ** -24 * scale / D ** 0.5 * q.double().cpu().abs().sum(-1, keepdim=True)
-    return 2.0 ** -11 * e if staged else biased
+    return 0.0 if staged else biased
 
 
 def check(got, want, tol, what=""):

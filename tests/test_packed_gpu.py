@@ -71,7 +71,7 @@ class Case:
             if self.fmt == "int4":
                 G = self.q.shape[1] // self.k.shape[2]
                 staged = n * G >= STAGED and self.q.shape[0] * self.q.shape[1] >= FILL
-                scores = quantized_scores(self.q[a:a + n][some], e, float(self.kval.abs().max()) / 7, staged)
+                scores = quantized_scores(self.q[a:a + n][some], float(self.kval.abs().max()) / 7, staged)
             tol = tolerance(o, w, e, m, self.D, torch.float16, torch.float16, self.fmt == "int4", scores)
             r = slice(None) if rows is None else rows[a:a + n][some]
             check(out[a:a + n].cpu()[some][r], o[r], tol[r], f"sequence {b}")
@@ -343,6 +343,26 @@ def test_evicted_rows_and_extreme_scales(D):
     c.check(memopt_C.packed_attention(*c.args()))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_chunks_evicted_rows_and_extreme_scales(D):
+    """Scales of 0 in one group or all, the largest beside the smallest: what the staged keys' factors hold."""
+    c = Case("int4", [540, 64], [510, 5], 64, 1, D, seed=5)
+    c.k[:] *= np.float16(0.25)
+    c.k[::5, ..., D // 2:] *= np.float16(2.0 ** -12)
+    c.k[1::5, ..., :D // 2] *= np.float16(2.0 ** -12)
+    c.v[:] *= np.float16(3000)
+    c.load()
+    pages = c.kc.cpu().numpy()
+    lay = memopt_C.int4_layout(D)
+    sc = pages[..., lay["kscales"]:lay["kscales"] + 32 * (D // 64)].view(np.float16)
+    sc[::2, :, 3::5] = 0
+    sc[1::4, :, :4] = 0
+    sc[2::4, :, -7:] = 0
+    c.kc = c.vc = torch.from_numpy(pages).to(dev())
+    c.kval, c.vval = page_values(pages, D)
+    c.check(memopt_C.packed_attention(*c.args()))
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_strides_padding_and_out(fmt):
     c = Case(fmt, [60, 200], [4, 30], 6, 2, 64, seed=2)
@@ -385,7 +405,7 @@ def test_pool_views_are_taken(fmt):
         assert torch.equal(memopt_C.packed_attention(q, buf, buf, bt, cl, cu, 1, 112), out)
         k, v = (x[1:].flatten(0, 1)[:100] for x in page_values(buf.cpu().numpy(), 64))
     o, w, e = attend(q, k, v, [99], -1, 0)
-    scores = quantized_scores(q, e, float(k.abs().max()) / 7, False) if fmt == "int4" else 0.0
+    scores = quantized_scores(q, float(k.abs().max()) / 7, False) if fmt == "int4" else 0.0
     check(out, o, tolerance(o, w, e, 100, 64, torch.float16, torch.float16, fmt == "int4", scores))
 
 
