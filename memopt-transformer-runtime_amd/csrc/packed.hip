@@ -36,13 +36,15 @@
 //    n, k-group g of the B operand of O^T += V^T P^T, so probabilities stay in
 //    their lane, and a page's V word unpacks into one register of four
 //    operands.
-// Output row rr of V^T product i is dim (D / 16) rr + i.
+//  * V enters as exact codes, too: the products of a scale group take the
+//    weights times that group's scale per token. So a page's only rounding to
+//    16 bits is that of weight times scale.
 //
 // Bound by vector instructions: about 200 per step of 32 tokens and 16 rows
 // (D = 128, INT4), four cycles each, most of them the unpacking of V; a copy
 // without them streams 131072 tokens of 8 key heads in 18 us, the kernel takes
-// 35. 32 sequences of 2700 to 8192 tokens, 32 query over 8 key heads: 48 us, 4.1
-// TB/s of pages; one of 131072: 35 us, 4.0 TB/s. A card's large copy reaches
+// 35. 32 sequences of 2700 to 8192 tokens, 32 query over 8 key heads: 47 us, 4.2
+// TB/s of pages; one of 131072: 35 us, 4.1 TB/s. A card's large copy reaches
 // 5.1.
 #include <algorithm>
 #include <cmath>
@@ -150,8 +152,8 @@ template <int D, int FMT>
 struct PackedV;
 template <int D>
 struct PackedV<D, MEMOPT_KV_INT4> {
-  uint32_t w[4][D / 64];  // [p_i][unit]
-  u32x4_t sc;             // pair (p_i, p_i + 8) in word i
+  uint32_t w[4][D / 64];  // [p_i][group]
+  u32x4_t sc[D / 64];     // of a group: pair (p_i, p_i + 8) in word i
 };
 template <int D>
 struct PackedV<D, MEMOPT_KV_FP16> {
@@ -334,7 +336,7 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
       copy_block(offset_of(e.b, 0), ring + stage * STG + BLK);
     };
     // K of a step: lane row r is tokens r % 8 and r % 8 + 8 of chunk r / 8.
-    // V: lane (r, g) holds dims [D/16 r, D/16 (r + 1)) of its score tokens.
+    // V: lane (r, g) holds four dims from 64 u + 4 r (fp16: [D/16 r, D/16 (r + 1))) of its score tokens.
     auto read_k = [&](int stage) __attribute__((always_inline)) {
       if constexpr (PAGES) {
         const uint32_t at = ring + stage * STG;
@@ -355,16 +357,13 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
         const uint32_t tb = ring + stage * STG + (g < 2 ? 0 : BLK);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t src = tb + (uint32_t)f.vcodes + 8 * (p0 + i) * (D / 8) + (D / 16) * r;
-          if constexpr (D == 128) {
-            const u32x2_t x = lds_at<u32x2_t>(src);
-            vr.w[i][0] = x[0];
-            vr.w[i][1] = x[1];
-          } else {
-            vr.w[i][0] = lds_at<uint32_t>(src);
-          }
+#pragma unroll
+          for (int u = 0; u < D / 64; ++u)
+            vr.w[i][u] = lds_at<uint32_t>(tb + (uint32_t)f.vcodes + 8 * (p0 + i) * (D / 8) + 64 * u + 4 * r);
         }
-        vr.sc = lds_at<u32x4_t>(tb + (uint32_t)f.vscales + 2 * ((r * (D / 16) / 64) * 16 + 2 * p0));
+#pragma unroll
+        for (int u = 0; u < D / 64; ++u)
+          vr.sc[u] = lds_at<u32x4_t>(tb + (uint32_t)f.vscales + 2 * (16 * u + 2 * p0));
       }
     };
     // fp16 pools: the same from global memory into registers.
@@ -517,21 +516,45 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
       const int32_t ta = 16 * logical(2 * e.i), tb = 16 * logical(2 * e.i + 1);
       const int32_t key0 = (g < 2 ? ta : tb) + 4 * (g & 1);
       const bool c_ok = g < 2 ? ok_a : ok_b;
-      h8_t pf[QB];
+      h8_t pf[QB][NG];
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
+        u32x4_t vs[NG];
+        if constexpr (PAGES) {
+#pragma unroll
+          for (int u = 0; u < NG; ++u) vs[u] = vr.sc[u];
+        }
         if (!full) {
           const int32_t last = c_ok ? min(row_pos[qb], kv_lim - 1) - key0 : -1;
           const int32_t first_w = row_pos[qb] - p.W + 1 - key0, end_s = p.sinks - key0;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int32_t c = (e >> 1) + 8 * (e & 1);
-            x[qb][e] = (c <= last) & ((c >= first_w) | (c < end_s)) ? x[qb][e] : -INFINITY;
+            const bool seen = (c <= last) & ((c >= first_w) | (c < end_s));
+            x[qb][e] = seen ? x[qb][e] : -INFINITY;
+            if constexpr (PAGES) {  // (a weight of 0 must not meet a scale that is inf or NaN)
+#pragma unroll
+              for (int u = 0; u < NG; ++u) vs[u][e >> 1] &= seen ? ~0u : (e & 1) ? 0x0000FFFFu : 0xFFFF0000u;
+            }
           }
         }
         float t = x[qb][0];
 #pragma unroll
         for (int e = 1; e < 8; ++e) t = fmaxf(t, x[qb][e]);
+        if constexpr (PAGES) {
+          // The weights enter the second product times their token's scale, so
+          // what the running maximum bounds is that product: x plus the log2 of
+          // the largest scale here, read off its bits (2^(bits / 1024 - 15), too
+          // small by 0.09 at most).
+          typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+          u16x2 m = {0, 0};
+#pragma unroll
+          for (int i = 0; i < 4 * NG; ++i) {
+            const uint32_t w = vs[i / 4][i % 4];  // (a bit cast of the vector's element itself takes its element 0)
+            m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w));
+          }
+          t += fmaf((float)max((uint32_t)m[0], (uint32_t)m[1]), 1.0f / 1024.0f, -15.0f);
+        }
         if (__any(t > thr[qb])) {  // wave-uniform, rare after the first steps
           // the row's four lanes agree on the new maximum
           auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(t), __float_as_uint(t), false, false);
@@ -549,35 +572,43 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
           ncm[qb] -= shift;
           thr[qb] = (first && !found) ? thr[qb] : kTop + 8.0f;
         }
-        uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[qb][e] = fast_exp2(x[qb][e]);
+        u32x4_t w;
+        if constexpr (PAGES) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          w[i] = as_u32(half2_t{(half_t)x[qb][2 * i], (half_t)x[qb][2 * i + 1]});
-          lsum[qb] = __builtin_amdgcn_fdot2(as_half2(w[i]), ones, lsum[qb], false);
+          for (int e = 0; e < 8; ++e) lsum[qb] += x[qb][e];
+#pragma unroll
+          for (int u = 0; u < NG; ++u) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)  // (one mixed-precision instruction for each half)
+              w[i] = as_u32(half2_t{(half_t)fmaf(x[qb][2 * i], (float)as_half2(vs[u][i])[0], 0.0f),
+                                    (half_t)fmaf(x[qb][2 * i + 1], (float)as_half2(vs[u][i])[1], 0.0f)});
+            pf[qb][u] = __builtin_bit_cast(h8_t, w);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            w[i] = as_u32(half2_t{(half_t)x[qb][2 * i], (half_t)x[qb][2 * i + 1]});
+            lsum[qb] = __builtin_amdgcn_fdot2(as_half2(w[i]), ones, lsum[qb], false);
+          }
+          pf[qb][0] = __builtin_bit_cast(h8_t, w);
         }
-        pf[qb] = __builtin_bit_cast(h8_t, u32x4_t{w[0], w[1], w[2], w[3]});
       }
 
-      // A weight of 0 must not meet an inf or NaN of V. Tokens that no row of the
-      // block sees (behind the context, unlinked, outside the window) become
-      // zeros; so do inf and NaN among those that only some rows see, which
-      // get them back at the end (`odd`).
-      if (!full) {
-        const int32_t last = c_ok ? min(pos_hi, kv_lim - 1) - key0 : -1;
-        const int32_t first_w = pos_lo - p.W + 1 - key0, end_s = p.sinks - key0;
-        const bool several = pos_lo != pos_hi;
+      // fp16: a weight of 0 must not meet an inf or NaN of V. Tokens that no row
+      // of the block sees (behind the context, unlinked, outside the window)
+      // become zeros; so do inf and NaN among those that only some rows see,
+      // which get them back at the end (`odd`).
+      if constexpr (!PAGES) {
+        if (!full) {
+          const int32_t last = c_ok ? min(pos_hi, kv_lim - 1) - key0 : -1;
+          const int32_t first_w = pos_lo - p.W + 1 - key0, end_s = p.sinks - key0;
+          const bool several = pos_lo != pos_hi;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int32_t c = (e >> 1) + 8 * (e & 1);
-          const bool live = (c <= last) & ((c >= first_w) | (c < end_s));
-          if constexpr (PAGES) {
-            const uint32_t half = (e & 1) ? 0xFFFF0000u : 0x0000FFFFu;
-            const bool bad = several && live && (vr.sc[e >> 1] & half & 0x7C007C00u) == (half & 0x7C007C00u);
-            odd |= bad ? 1u : 0u;
-            vr.sc[e >> 1] &= live && !bad ? ~0u : ~half;
-          } else {
+          for (int e = 0; e < 8; ++e) {
+            const int32_t c = (e >> 1) + 8 * (e & 1);
+            const bool live = (c <= last) & ((c >= first_w) | (c < end_s));
 #pragma unroll
             for (int j = 0; j < D / 32; ++j) {
               uint32_t w = live ? vr.w[e][j] : 0u;
@@ -594,18 +625,14 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
       auto pv = [&](int i, u32x4_t a) __attribute__((always_inline)) {
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb)
-          o[qb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), pf[qb], o[qb][i], 0, 0, 0);
+          o[qb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), pf[qb][i / (ND / NG)], o[qb][i], 0, 0, 0);
       };
       if constexpr (PAGES) {
 #pragma unroll
         for (int u = 0; u < D / 64; ++u) {
           u32x4_t y[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            y[i] = codes(vr.w[i][u]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[i][j] = as_u32(as_half2(y[i][j]) * as_half2(vr.sc[i]));
-          }
+          for (int i = 0; i < 4; ++i) y[i] = codes(vr.w[i][u]);
 #pragma unroll
           for (int j = 0; j < 4; ++j) pv(4 * u + j, u32x4_t{y[0][j], y[1][j], y[2][j], y[3][j]});
         }
@@ -671,40 +698,35 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
       }
     }
 
-    if (__any(odd != 0)) {
-      // Rows that see an inf or NaN of V have inf or NaN in its column whatever
-      // its weight; a lane looks through its quarter of the dims.
+    if constexpr (!PAGES) {
+      if (__any(odd != 0)) {
+        // Rows that see an inf or NaN of V have inf or NaN in its column whatever
+        // its weight; a lane looks through its quarter of the dims.
 #pragma unroll 1
-      for (int32_t i = begin + wave; i < end; i += NW) {
-        if (i >= full0 && i < full1) continue;  // (a whole chunk there is unlinked: all zeros)
-        const Step e = fetch(i);
+        for (int32_t i = begin + wave; i < end; i += NW) {
+          if (i >= full0 && i < full1) continue;  // (a whole chunk there is unlinked: all zeros)
+          const Step e = fetch(i);
 #pragma unroll 1
-        for (int tk = 0; tk < 32; ++tk) {
-          const int32_t phys = tk < 16 ? e.a : e.b, lc = logical(2 * i + (tk >> 4)), t = tk & 15, key = 16 * lc + t;
-          if (!mapped(phys) || key >= kv_lim) continue;
-          const int64_t at = offset_of(phys, lc);
+          for (int tk = 0; tk < 32; ++tk) {
+            const int32_t phys = tk < 16 ? e.a : e.b, lc = logical(2 * i + (tk >> 4)), t = tk & 15, key = 16 * lc + t;
+            if (!mapped(phys) || key >= kv_lim) continue;
+            const half_t *row = reinterpret_cast<const half_t *>(vbase + offset_of(phys, lc) + (int64_t)t * p.kv_ts);
 #pragma unroll
-          for (int d = 0; d < D / 4; ++d) {
-            const int dim = (D / 4) * g + d;
-            float y;
-            if constexpr (PAGES) {
-              const uint8_t *blk = kbase + at;
-              const half_t sv = reinterpret_cast<const half_t *>(blk + f.vscales)[f.scale_idx(t, dim / 64)];
-              y = ((float)((blk[f.vcodes + f.v_byte(t, dim)] >> (4 * (dim & 1))) & 15) - 8.0f) * (float)sv;
-            } else {
-              y = (float)reinterpret_cast<const half_t *>(vbase + at + (int64_t)t * p.kv_ts)[dim];
+            for (int d = 0; d < D / 4; ++d) {
+              const float y = (float)row[(D / 4) * g + d];
+              const bool bad = (__float_as_uint(y) & 0x7F800000u) == 0x7F800000u;
+#pragma unroll
+              for (int qb = 0; qb < QB; ++qb)
+                if (bad && key <= row_pos[qb] && (key < p.sinks || key >= row_pos[qb] - p.W + 1))
+                  o[qb][d % ND][d / ND] += y;
             }
-            const bool bad = (__float_as_uint(y) & 0x7F800000u) == 0x7F800000u;
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb)
-              if (bad && key <= row_pos[qb] && (key < p.sinks || key >= row_pos[qb] - p.W + 1)) o[qb][d % ND][d / ND] += y;
           }
         }
       }
     }
 
-    // Merge of the waves. Lane (n, g) holds dims [D/4 g, D/4 (g + 1)) of row n:
-    // row 4 g + reg of V^T product i is dim D/16 (4 g + reg) + i.
+    // Merge of the waves. Row 4 g + reg of V^T product i is dim 64 (i / 4) + 4 (4 g
+    // + reg) + i % 4 over pages, D/16 (4 g + reg) + i over fp16 pools.
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
       const float l = xor32_sum(xor16_sum(lsum[qb]));
@@ -714,7 +736,7 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
       for (int reg = 0; reg < 4; ++reg)
 #pragma unroll
         for (int i = 0; i < ND; i += 4)
-          *reinterpret_cast<f32x4_t *>(&s_o[wave][row][ND * (4 * g + reg) + i]) =
+          *reinterpret_cast<f32x4_t *>(&s_o[wave][row][PAGES ? 16 * i + 4 * (4 * g + reg) : ND * (4 * g + reg) + i]) =
               f32x4_t{o[qb][i][reg], o[qb][i + 1][reg], o[qb][i + 2][reg], o[qb][i + 3][reg]};
       if (g == 0) {
         s_ml[wave][row][0] = thr[qb] == -INFINITY ? -INFINITY : -ncm[qb];

@@ -34,12 +34,15 @@ def attend(q, k, v, pos, window, sinks, live=None):
     return o, a, e
 
 
-def tolerance(o, a, e, keys, D, out_dtype, p_dtype, v_rounded, scores=0.0):
+def tolerance(o, a, e, keys, D, out_dtype, p_dtype, v_rounded, scores=0.0, v_scale=0.0):
     """What the kernels' roundings may add up to, element by element.
 
     * the output: half a step of its type;
     * the probabilities are rounded to p_dtype in numerator and row sum: each half a step, so 2 u a at most;
       those below 2^-21 of the largest (fp16 subnormals) are off by 2^-32 of it, keys of them;
+    * v_scale (over INT4 pages, up to that): what is rounded is probability times scale, and only in the
+      numerator, so u a less; but relative to the largest such product, at 2^7 or more: its subnormals are off by
+      2^-25 each, times a code of up to 8, over a row sum of 2^7 / v_scale or more: 2^-29 v_scale for each key;
     * v_rounded: V itself is rounded once to fp16 (code * scale): half a step of a;
     * scores: D products summed in 32 bits, two fused scalings and the running maximum: D + 16 roundings of
       e at 2^-24, which move every weight by that much relative (natural exponent), numerator and sum: twice;
@@ -49,6 +52,7 @@ def tolerance(o, a, e, keys, D, out_dtype, p_dtype, v_rounded, scores=0.0):
     u = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
     t = u[out_dtype] * o.abs() + 2 * u[p_dtype] * a + (2.0 ** -11 * a if v_rounded else 0)
     t = t + 2 * (D + 16) * 2.0 ** -24 * e * a + 2 * scores * a + (2 * 2.0 ** -22 + 2 * keys * 2.0 ** -24) * a
+    t = t - (u[p_dtype] * a if v_scale else 0) + keys * 2.0 ** -29 * v_scale
     return t + 2.0 ** -24 + keys * 2.0 ** -32 * a  # (2^-24: half a step of fp16's subnormals)
 
 

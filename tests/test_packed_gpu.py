@@ -67,12 +67,13 @@ class Case:
                 some = np.unique(np.concatenate([np.arange(20), n - 1 - np.arange(20), np.random.default_rng(n).integers(0, n, 30)]))
             o, w, e = attend(self.q[a:a + n][some], k, v, (c - n) + some, window, sinks,
                              live.repeat_interleave(self.bs)[:m])
-            scores = 0.0
+            scores, staged, v_scale = 0.0, False, 0.0
             if self.fmt == "int4":
                 G = self.q.shape[1] // self.k.shape[2]
                 staged = n * G >= STAGED and self.q.shape[0] * self.q.shape[1] >= FILL
                 scores = quantized_scores(self.q[a:a + n][some], float(self.kval.abs().max()) / 7, staged)
-            tol = tolerance(o, w, e, m, self.D, torch.float16, torch.float16, self.fmt == "int4", scores)
+                v_scale = 0.0 if staged else float(self.vval.abs().max()) / 7
+            tol = tolerance(o, w, e, m, self.D, torch.float16, torch.float16, staged, scores, v_scale)
             r = slice(None) if rows is None else rows[a:a + n][some]
             check(out[a:a + n].cpu()[some][r], o[r], tol[r], f"sequence {b}")
             a += n
@@ -406,7 +407,8 @@ def test_pool_views_are_taken(fmt):
         k, v = (x[1:].flatten(0, 1)[:100] for x in page_values(buf.cpu().numpy(), 64))
     o, w, e = attend(q, k, v, [99], -1, 0)
     scores = quantized_scores(q, float(k.abs().max()) / 7, False) if fmt == "int4" else 0.0
-    check(out, o, tolerance(o, w, e, 100, 64, torch.float16, torch.float16, fmt == "int4", scores))
+    v_scale = float(v.abs().max()) / 7 if fmt == "int4" else 0.0
+    check(out, o, tolerance(o, w, e, 100, 64, torch.float16, torch.float16, False, scores, v_scale))
 
 
 def test_same_heads_agree_with_the_paged_attention():
