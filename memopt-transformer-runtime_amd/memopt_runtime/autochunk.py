@@ -54,7 +54,8 @@ def autochunk_prefill(cache: PagedKVCache, seq_id: int, query: torch.Tensor, key
     """Prefill ``S`` new tokens of one sequence in chunks; returns fp16 ``[S, H, D]``.
 
     ``query``/``keys``/``values``: fp16 ``[S, H, D]``, the positions that
-    follow the sequence's current length. The chunk size is ``chunk_tokens``
+    follow the sequence's current length; ``query`` may have a multiple of
+    the cache's heads (grouped heads). The chunk size is ``chunk_tokens``
     or, with ``budget_bytes``, :func:`chunk_tokens_for_budget`; with neither
     the whole prompt is one chunk.
     """
@@ -79,18 +80,26 @@ def autochunk_prefill(cache: PagedKVCache, seq_id: int, query: torch.Tensor, key
     except RuntimeError:
         n_fit = _whole_chunks(cache, seq_id, rows, chunk_tokens)
         cache.reserve(seq_id, n_fit)
-    index = cache.prompt_indices(seq_id, n_fit, [start + min(rows, s0 + chunk_tokens) for s0 in
-                                                 range(0, S if n_fit == rows else n_fit, chunk_tokens)])
+    starts = range(0, S if n_fit == rows else n_fit, chunk_tokens)
+    ends = [start + min(rows, s0 + chunk_tokens) for s0 in starts]
+    grouped = H != cache.num_heads
+    if grouped:  # and the packed calls' two sequence starts, chunk by chunk
+        ends += [x for s0 in starts for x in (0, min(S, s0 + chunk_tokens) - s0)]
+    index = cache.prompt_indices(seq_id, n_fit, ends)
     for i, s0 in enumerate(range(0, S, chunk_tokens)):
         s1 = min(S, s0 + chunk_tokens)
         cache.reserve(seq_id, min(s1, rows) - min(s0, rows))  # raises at the first chunk past n_fit
         n = start + s1
         cache.write_rows([seq_id], keys[s0:s1], values[s0:s1], index.slots[s0:s1])
+        table, lens = index.table[:, :pages_needed(n, cache.block_size)], index.lens[i:i + 1]
+        if grouped:
+            cu = index.lens[len(starts) + 2 * i:][:2]
+            memopt_C.packed_attention(query[s0:s1], k_pool, v_pool, table, lens, cu, s1 - s0, n, window_size,
+                                      num_sink_tokens=num_sink_tokens, out=out[s0:s1])
+            continue
         with memopt_C._on(k_pool.device):  # (a plan launches on the current device)
-            memopt_C.PreparedAttention(query[s0:s1].unsqueeze(0), k_pool, v_pool,
-                                       index.table[:, :pages_needed(n, cache.block_size)], index.lens[i:i + 1], n,
-                                       window_size, num_sink_tokens=num_sink_tokens, causal=True,
-                                       out=out[s0:s1].unsqueeze(0))()
+            memopt_C.PreparedAttention(query[s0:s1].unsqueeze(0), k_pool, v_pool, table, lens, n, window_size,
+                                       num_sink_tokens=num_sink_tokens, causal=True, out=out[s0:s1].unsqueeze(0))()
     return out
 
 

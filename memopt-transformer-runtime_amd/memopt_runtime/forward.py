@@ -26,11 +26,12 @@ from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import Optional, Sequence, Tuple
 
+import numpy as np
 import torch
 
 import memopt_C
 
-from .kv_cache import PagedKVCache
+from .kv_cache import PagedKVCache, upload_indices
 
 
 @dataclass(frozen=True)
@@ -87,7 +88,9 @@ class PolicyForward:
         """Append the new tokens, attend, then evict under the current policy.
 
         ``query``/``keys``/``values``: fp16 ``[B, T, H, D]`` (T new tokens
-        per sequence; T = 1 for decode). ``scores``: optional f32
+        per sequence; T = 1 for decode); ``query`` may have a multiple of the
+        cache's heads (grouped: query head h reads cache head ``h //
+        (Hq / H)``). ``scores``: optional f32
         ``[B, H, L]`` per-token scores used for eviction when
         ``retain_ratio < 1``. Returns fp16 ``[B, T, H, D]``.
         """
@@ -101,13 +104,18 @@ class PolicyForward:
         return out
 
     def attend(self, seq_ids: Sequence[int], query: torch.Tensor) -> torch.Tensor:
-        """Attention of ``query`` ``[B, T, H, D]`` (the last T positions of each
-        sequence) over the paged cache."""
-        T = query.shape[1]
+        """Attention of ``query`` ``[B, T, Hq, D]`` (the last T positions of each
+        sequence) over the paged cache; Hq is the cache's heads or a multiple."""
+        B, T, Hq, D = query.shape
         bt = self.cache.block_tables(seq_ids)
         ctx = self.cache.context_lens(seq_ids)
         max_len = max(self.cache.length(s) for s in seq_ids)
         k, v = self.cache.key_value_pools()
+        if Hq != self.cache.num_heads:
+            cu = upload_indices(np.arange(B + 1) * T, query.device)
+            out = memopt_C.packed_attention(query.reshape(B * T, Hq, D), k, v, bt, ctx, cu, T, max_len,
+                                            self.window_size, num_sink_tokens=self.num_sink_tokens)
+            return out.view(B, T, Hq, D)
         return memopt_C.dynamic_sparse_attention(query, k, v, bt, ctx, max_len, self.window_size,
                                                  num_sink_tokens=self.num_sink_tokens, causal=T > 1)
 
