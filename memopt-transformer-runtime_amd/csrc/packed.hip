@@ -1175,7 +1175,7 @@ extern "C" int memopt_packed_attention(const memopt_packed_desc *desc, void *str
   const PackedWorkspace w = packed_workspace(d, pl);
   MEMOPT_REQUIRE(d.workspace && d.workspace_bytes >= w.total, MEMOPT_ERR_INVALID,
                  "packed_attention: workspace needs " + std::to_string(w.total) + " bytes");
-  MEMOPT_REQUIRE((int64_t)d.tokens * d.num_heads < (1LL << 31) && pl.blocks * packed_steps(d) < (1LL << 31),
+  MEMOPT_REQUIRE((int64_t)d.tokens * d.num_heads <= INT32_MAX - 255 && pl.blocks * packed_steps(d) < (1LL << 31),
                  MEMOPT_ERR_UNSUPPORTED, "packed_attention: too many (row, page) pairs for one call");
   PackedParams p = {};
   p.q = (const half_t *)d.query;

@@ -124,7 +124,8 @@ def test_windows_and_sinks(fmt, window, sinks, D):
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("Hq,Hk,D,ctx,qn", [(8, 2, 64, [3000], [1]), (8, 1, 128, [5000, 100, 2500], [1, 1, 1]),
                                             (20, 1, 128, [2100], [3]), (32, 8, 128, [1500], [1]),
-                                            (4, 2, 64, [2500, 600], [40, 1])])
+                                            (4, 2, 64, [2500, 600], [40, 1]), (8, 2, 64, [6100], [1]),
+                                            (8, 4, 64, [4000, 9000], [1, 2]), (32, 8, 128, [7000], [1])])
 def test_long_contexts_in_splits(fmt, Hq, Hk, D, ctx, qn):
     c = Case(fmt, ctx, qn, Hq, Hk, D, seed=7)
     plan = memopt_C.PreparedPackedAttention(*c.args())
@@ -448,6 +449,31 @@ def test_plans_on_two_streams_and_in_graphs():
         for c, p in zip(cases, plans):
             c.check(p.out)
             assert torch.equal(p.out, memopt_C.packed_attention(*c.args()))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_captured_long_chunks_follow_the_lengths_on_the_device(fmt):
+    """One captured plan, replayed as chunks grow and shrink across the length from which they are staged; and eager
+    calls of another shape in between."""
+    c = Case(fmt, [700, 300, 90], [500, 20, 10], 64, 1, 64, seed=21, spare=2)
+    plan = memopt_C.PreparedPackedAttention(*c.args(most=530))
+    plan()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan()
+    other = Case(fmt, [100, 40], [1, 1], 8, 2, 64, seed=2)
+    for ctx, qn in [([700, 300, 90], [500, 20, 10]), ([530, 1, 90], [530, 0, 0]), ([8, 300, 90], [8, 250, 7]),
+                    ([690, 299, 0], [265, 265, 0]), ([700, 300, 90], [500, 20, 10])]:
+        c.ctx, c.qn = ctx, qn
+        c.cl.copy_(torch.tensor(ctx, dtype=torch.int32))
+        c.cu.copy_(torch.from_numpy(starts(qn)))
+        for _ in range(2):
+            plan.out.fill_(9.0)
+            graph.replay()
+            other.check(memopt_C.packed_attention(*other.args()))
+            c.check(plan.out[:sum(qn)])
+            assert bool((plan.out[sum(qn):] == 9).all())
 
 
 def test_refusals():
