@@ -385,11 +385,14 @@ int memopt_packed_attention(const memopt_packed_desc *desc, void *stream);
 #define MEMOPT_STEP_NO_ROWS  4
 /* A request that is not served stays as it was and gets no rows. At most 4096
  * requests; calls on one batch must not overlap. */
-int memopt_advance_batch(const int32_t *new_tokens, const int32_t *context_lens, int32_t num_requests,
-                         int32_t *block_tables, int32_t max_blocks_per_seq, const int32_t *free_pages,
-                         int32_t num_free_pages, const int32_t *free_span, int32_t block_size, int32_t num_rows,
-                         int32_t *context_lens_out, int32_t *free_span_out, int32_t *query_starts, int32_t *slots,
-                         int32_t *positions, int32_t *status, void *stream);
+typedef struct memopt_advance_desc {
+  const int32_t *new_tokens, *context_lens;  /* [num_requests]                 */
+  int32_t *block_tables;                     /* [num_requests, max_blocks_per_seq] */
+  const int32_t *free_pages, *free_span;     /* [num_free_pages], [2]          */
+  int32_t *context_lens_out, *free_span_out, *query_starts, *slots, *positions, *status;
+  int32_t num_requests, max_blocks_per_seq, num_free_pages, block_size, num_rows;
+} memopt_advance_desc;
+int memopt_advance_batch(const memopt_advance_desc *desc, void *stream);
 
 #ifdef __cplusplus
 }

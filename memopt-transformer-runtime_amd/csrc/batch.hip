@@ -179,28 +179,30 @@ __global__ __launch_bounds__(256) void advance_rows_kernel(const AdvanceParams p
 
 using namespace memopt;
 
-extern "C" int memopt_advance_batch(const int32_t *new_tokens, const int32_t *context_lens, int32_t num_requests,
-                                    int32_t *block_tables, int32_t max_blocks_per_seq, const int32_t *free_pages,
-                                    int32_t num_free_pages, const int32_t *free_span, int32_t block_size,
-                                    int32_t num_rows, int32_t *context_lens_out, int32_t *free_span_out,
-                                    int32_t *query_starts, int32_t *slots, int32_t *positions, int32_t *status,
-                                    void *stream) {
-  MEMOPT_REQUIRE(num_requests > 0 && max_blocks_per_seq > 0 && num_free_pages > 0 && block_size > 0 && num_rows >= 0,
+extern "C" int memopt_advance_batch(const memopt_advance_desc *desc, void *stream) {
+  MEMOPT_REQUIRE(desc, MEMOPT_ERR_INVALID, "advance_batch: null descriptor");
+  const memopt_advance_desc &d = *desc;
+  MEMOPT_REQUIRE(d.num_requests > 0 && d.max_blocks_per_seq > 0 && d.num_free_pages > 0 && d.block_size > 0 &&
+                     d.num_rows >= 0,
                  MEMOPT_ERR_INVALID, "advance_batch: sizes must be positive");
-  MEMOPT_REQUIRE(num_requests <= kMaxRequests, MEMOPT_ERR_UNSUPPORTED,
+  MEMOPT_REQUIRE(d.num_requests <= kMaxRequests, MEMOPT_ERR_UNSUPPORTED,
                  "advance_batch: more than " + std::to_string(kMaxRequests) + " requests");
-  MEMOPT_REQUIRE((int64_t)max_blocks_per_seq * block_size < (1LL << 31), MEMOPT_ERR_UNSUPPORTED,
+  MEMOPT_REQUIRE((int64_t)d.max_blocks_per_seq * d.block_size < (1LL << 31), MEMOPT_ERR_UNSUPPORTED,
                  "advance_batch: a block table of 2^31 tokens and more");
-  MEMOPT_REQUIRE(new_tokens && context_lens && block_tables && free_pages && free_span && context_lens_out &&
-                     free_span_out && query_starts && status && (num_rows == 0 || (slots && positions)),
+  MEMOPT_REQUIRE(d.new_tokens && d.context_lens && d.block_tables && d.free_pages && d.free_span &&
+                     d.context_lens_out && d.free_span_out && d.query_starts && d.status &&
+                     (d.num_rows == 0 || (d.slots && d.positions)),
                  MEMOPT_ERR_INVALID, "advance_batch: null pointer");
-  const AdvanceParams p = {new_tokens, context_lens, num_requests, block_tables, max_blocks_per_seq, free_pages,
-                           num_free_pages, free_span, block_size, num_rows, context_lens_out, free_span_out,
-                           query_starts, slots, positions, status};
+  const int32_t num_requests = d.num_requests, num_rows = d.num_rows;
+  const AdvanceParams p = {d.new_tokens, d.context_lens, num_requests, d.block_tables, d.max_blocks_per_seq,
+                           d.free_pages, d.num_free_pages, d.free_span, d.block_size, num_rows, d.context_lens_out,
+                           d.free_span_out, d.query_starts, d.slots, d.positions, d.status};
   hipStream_t s = (hipStream_t)stream;
   const int fill = num_rows <= kOneLaunchRows;
-  if (num_requests <= 256 && num_rows <= 1024) hipLaunchKernelGGL(advance_kernel<256>, dim3(1), dim3(256), 0, s, p, fill);
-  else hipLaunchKernelGGL(advance_kernel<1024>, dim3(1), dim3(1024), 0, s, p, fill);
+  if (num_requests <= 256 && num_rows <= 1024)
+    hipLaunchKernelGGL(advance_kernel<256>, dim3(1), dim3(256), 0, s, p, fill);
+  else
+    hipLaunchKernelGGL(advance_kernel<1024>, dim3(1), dim3(1024), 0, s, p, fill);
   int rc = check_launch("advance_batch");
   if (rc != MEMOPT_OK || fill) return rc;
   const int64_t wgs = ((int64_t)num_rows + 255) / 256;

@@ -34,6 +34,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import struct
 import threading
 from typing import List, Optional, Sequence, Tuple
 
@@ -142,8 +143,7 @@ _c_prompt = _sig("memopt_prompt_attention", [ctypes.POINTER(PromptDesc), _vp])
 _c_packed_ws = _sig("memopt_packed_workspace_size",
                     [ctypes.POINTER(PackedDesc), ctypes.POINTER(_i64), ctypes.POINTER(_i64)])
 _c_packed = _sig("memopt_packed_attention", [ctypes.POINTER(PackedDesc), _vp])
-_c_advance = _sig("memopt_advance_batch",
-                  [_vp, _vp, _i32, _vp, _i32, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp])
+_c_advance = _sig("memopt_advance_batch", [ctypes.c_char_p, _vp])
 
 KV_FP16, KV_INT4, KV_INT4_ROWS = 0, 1, 2
 _FORMATS = {"fp16": KV_FP16, "int4": KV_INT4}
@@ -779,13 +779,13 @@ class PreparedAttention:
 # (On the smallest calls the host side takes longer than the kernels, so the
 # checks below read each property of a tensor once and format messages only
 # when they raise.)
-def _device_tensors(fn: str, device: torch.device, **tensors) -> None:
-    """Raises for the first of ``tensors`` that is not a CUDA tensor on ``device``."""
-    for n, t in tensors.items():
-        if not (isinstance(t, torch.Tensor) and t.is_cuda):
-            raise RuntimeError(f"{fn}: {n} must be a CUDA tensor")
-        if t.device != device:
-            raise RuntimeError(f"{fn}: {n} on a different device")
+def _device_tensors(fn: str, device: torch.device, names: Tuple[str, ...], *tensors) -> None:
+    """Raises for the first of ``tensors`` that is not a CUDA tensor on ``device`` (one of CUDA)."""
+    for i, t in enumerate(tensors):
+        if not (isinstance(t, torch.Tensor) and t.device == device):
+            if not (isinstance(t, torch.Tensor) and t.is_cuda):
+                raise RuntimeError(f"{fn}: {names[i]} must be a CUDA tensor")
+            raise RuntimeError(f"{fn}: {names[i]} on a different device")
 
 
 def _int32(fn: str, t: torch.Tensor, name: str, shape: Tuple[int, ...]) -> None:
@@ -793,8 +793,8 @@ def _int32(fn: str, t: torch.Tensor, name: str, shape: Tuple[int, ...]) -> None:
         raise RuntimeError(f"{fn}: {name} must be a contiguous int32 tensor of shape {list(shape)}")
 
 
-def _no_grad(fn: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+def _no_grad(fn: str, requires_grad: bool) -> None:
+    if requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{fn}: no gradients are computed; call it under torch.no_grad()")
 
 
@@ -813,9 +813,10 @@ def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int, int, int]:
 def _out_rows(fn: str, out: Optional[torch.Tensor], query: torch.Tensor) -> Tuple[torch.Tensor, int, int, int]:
     """(out, address, token stride, head stride); a fresh tensor for ``None``."""
     if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-        return out, out.data_ptr(), out.shape[1] * out.shape[2], out.shape[2]
-    _device_tensors(fn, query.device, out=out)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)  # (half the time of torch.empty)
+        _, H, D = out.shape
+        return out, out.data_ptr(), H * D, D
+    _device_tensors(fn, query.device, ("out",), out)
     if not (out.shape == query.shape and out.dtype == query.dtype):
         raise RuntimeError(f"{fn}: out must be shaped like query, with its dtype")
     ts, hs, ds = out.stride()
@@ -825,6 +826,20 @@ def _out_rows(fn: str, out: Optional[torch.Tensor], query: torch.Tensor) -> Tupl
                                                                                      out.shape[1] == 1)):
         raise RuntimeError(f"{fn}: out must have contiguous 16-byte aligned rows that do not overlap")
     return out, p, ts, hs
+
+
+# Descriptors as bytes, in native alignment (a quarter of the time that ctypes structures take):
+# memopt_prompt_desc and memopt_advance_desc.
+_PROMPT = struct.Struct("@4P6i8qP2i")
+_ADVANCE = struct.Struct("@11P5i")
+_c_prompt_bytes = _lib["memopt_prompt_attention"]
+_c_prompt_bytes.argtypes = [ctypes.c_char_p, _vp]
+_c_prompt_bytes.restype = _i32
+
+
+def _count32(n: int) -> int:
+    """``n`` as an int32, where any negative number means the same and any past 2^31 - 1 as that."""
+    return min(max(int(n), -1), 2 ** 31 - 1)
 
 
 def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -847,8 +862,8 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     if not (isinstance(query, torch.Tensor) and query.is_cuda):
         raise RuntimeError(f"{fn}: query must be a CUDA tensor")
     device, dtype, shape = query.device, query.dtype, query.shape
-    _device_tensors(fn, device, keys=keys, values=values, cu_seqlens=cu_seqlens)
-    _no_grad(fn, query, keys, values)
+    _device_tensors(fn, device, ("keys", "values", "cu_seqlens"), keys, values, cu_seqlens)
+    _no_grad(fn, query.requires_grad or keys.requires_grad or values.requires_grad)
     kshape = keys.shape
     if not (len(shape) == 3 and len(kshape) == 3 and values.dim() == 3):
         raise RuntimeError(f"{fn}: query, keys and values must be 3-D [tokens, heads, head_dim]")
@@ -861,18 +876,22 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     if not (kshape == (T, Hk, D) and values.shape == kshape):
         raise RuntimeError(f"{fn}: keys and values must be [{T}, kv heads, {D}], got {list(kshape)} and "
                            f"{list(values.shape)}")
-    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
+    cshape = cu_seqlens.shape
+    if len(cshape) != 1 or cshape[0] < 1:
         raise RuntimeError(f"{fn}: cu_seqlens must be 1-D [batch + 1]")
-    n = cu_seqlens.shape[0]
-    _int32(fn, cu_seqlens, "cu_seqlens", (n,))
+    _int32(fn, cu_seqlens, "cu_seqlens", cshape)
     with _on(device):
         out, po, ots, ohs = _out_rows(fn, out, query)
         q, pq, qts, qhs = _rows(query)
         k, pk, kts, khs = _rows(keys)
         v, pv, vts, vhs = _rows(values)
-        d = PromptDesc(pq, pk, pv, po, 1 if dtype is torch.bfloat16 else 0, T, n - 1, Hq, Hk, D, qts, qhs, kts, khs,
-                       vts, vhs, ots, ohs, cu_seqlens.data_ptr(), int(window_size), int(num_sink_tokens))
-        _check(_c_prompt(ctypes.byref(d), _stream(query)))
+        try:
+            d = _PROMPT.pack(pq, pk, pv, po, 1 if dtype is torch.bfloat16 else 0, T, cshape[0] - 1, Hq, Hk, D, qts, qhs,
+                             kts, khs, vts, vhs, ots, ohs, cu_seqlens.data_ptr(), _count32(window_size),
+                             _count32(num_sink_tokens))
+        except struct.error:
+            raise RuntimeError(f"{fn}: sizes must fit 32 bits") from None
+        _check(_c_prompt_bytes(d, torch._C._cuda_getCurrentRawStream(device.index)))
     return out
 
 
@@ -880,9 +899,9 @@ def _packed_desc(query, key_cache, value_cache, block_tables, context_lens, cu_s
                  window_size, num_sink_tokens, out):
     """Validated PackedDesc: (desc, out, workspace, keepalive)."""
     fn = "packed_attention"
-    _device_tensors(fn, query.device, key_cache=key_cache, value_cache=value_cache, block_tables=block_tables,
-                    context_lens=context_lens, cu_seqlens=cu_seqlens)
-    _no_grad(fn, query)
+    _device_tensors(fn, query.device, ("key_cache", "value_cache", "block_tables", "context_lens", "cu_seqlens"),
+                    key_cache, value_cache, block_tables, context_lens, cu_seqlens)
+    _no_grad(fn, query.requires_grad)
     _require(query.dim() == 3, "packed_attention: query must be 3-D [tokens, heads, head_dim]")
     _require(query.dtype == torch.float16, "packed_attention: query must be fp16")
     T, Hq, D = query.shape
@@ -918,8 +937,7 @@ def _packed_desc(query, key_cache, value_cache, block_tables, context_lens, cu_s
     # (the C side holds 32-bit sizes)
     d = PackedDesc(pq, po, T, B, Hq, Hk, D, qts, qhs, ots, ohs, fmt, base_k, base_v, bs, nb, block_tables.data_ptr(),
                    block_tables.shape[1], context_lens.data_ptr(), cu_seqlens.data_ptr(),
-                   min(int(max_query_len), 2 ** 31 - 1), min(int(max_seq_len), 2 ** 31 - 1), int(window_size),
-                   int(num_sink_tokens))
+                   _count32(max_query_len), _count32(max_seq_len), _count32(window_size), _count32(num_sink_tokens))
     need, zeroed = _i64(), _i64()
     _check(_c_packed_ws(ctypes.byref(d), ctypes.byref(need), ctypes.byref(zeroed)))
     ws = None
@@ -999,13 +1017,14 @@ class BatchStep:
         fn = "advance_batch"
         tensors = (context_lens, free_span, cu_seqlens, slots, positions, status)
         self.device = getattr(context_lens, "device", None)
-        _device_tensors(fn, self.device, **dict(zip(self.FIELDS, tensors)))
+        _require(getattr(context_lens, "is_cuda", False), "advance_batch: context_lens must be a CUDA tensor")
+        _device_tensors(fn, self.device, self.FIELDS, *tensors)
         _require(context_lens.dim() == 1 and slots.dim() == 1, "advance_batch: context_lens and slots must be 1-D")
         B, rows = context_lens.shape[0], slots.shape[0]
         for n, t, k in zip(self.FIELDS, tensors, (B, 2, B + 1, rows, rows, B)):
             _int32(fn, t, n, (k,))
             setattr(self, n, t)
-        self._args = (rows, *(t.data_ptr() for t in tensors))
+        self._args = tuple(t.data_ptr() for t in tensors)
 
     def replace(self, **tensors) -> "BatchStep":
         """The same buffers with some of them exchanged."""
@@ -1043,26 +1062,30 @@ def advance_batch(new_tokens: torch.Tensor, context_lens: torch.Tensor, block_ta
     if not (isinstance(new_tokens, torch.Tensor) and new_tokens.is_cuda):
         raise RuntimeError(f"{fn}: new_tokens must be a CUDA tensor")
     device = new_tokens.device
-    _device_tensors(fn, device, context_lens=context_lens, block_tables=block_tables, free_pages=free_pages,
-                    free_span=free_span)
-    if not (new_tokens.dim() == 1 and block_tables.dim() == 2 and free_pages.dim() == 1):
+    _device_tensors(fn, device, ("context_lens", "block_tables", "free_pages", "free_span"), context_lens, block_tables,
+                    free_pages, free_span)
+    nshape, tshape, fshape = new_tokens.shape, block_tables.shape, free_pages.shape
+    if not (len(nshape) == 1 and len(tshape) == 2 and len(fshape) == 1):
         raise RuntimeError(f"{fn}: new_tokens and free_pages must be 1-D, block_tables 2-D")
-    B, M, C = new_tokens.shape[0], block_tables.shape[1], free_pages.shape[0]
-    _int32(fn, new_tokens, "new_tokens", (B,))
-    _int32(fn, context_lens, "context_lens", (B,))
+    if not (0 < block_size < 2 ** 31 and fshape[0] < 2 ** 31):
+        raise RuntimeError(f"{fn}: sizes must be positive and fit 32 bits")
+    B, = nshape
+    M, C = tshape[1], fshape[0]
+    _int32(fn, new_tokens, "new_tokens", nshape)
+    _int32(fn, context_lens, "context_lens", nshape)
     _int32(fn, block_tables, "block_tables", (B, M))
-    _int32(fn, free_pages, "free_pages", (C,))
+    _int32(fn, free_pages, "free_pages", fshape)
     _int32(fn, free_span, "free_span", (2,))
     if out is None:
         _require(num_rows is not None and num_rows >= 0, "advance_batch: num_rows or out must be given")
         out = advance_batch_buffers(B, num_rows, device)
-    rows, *pointers = out._args
+    rows, = out.slots.shape
     if num_rows is not None and num_rows != rows:
         raise RuntimeError(f"{fn}: num_rows differs from out's rows")
-    if out.device != device or out.context_lens.shape[0] != B:
+    if out.device != device or out.context_lens.shape != nshape:
         raise RuntimeError(f"{fn}: out holds buffers of another device or number of requests")
     with _on(device):
-        _check(_c_advance(new_tokens.data_ptr(), context_lens.data_ptr(), B, block_tables.data_ptr(), M,
-                          free_pages.data_ptr(), C, free_span.data_ptr(), int(block_size), rows, *pointers,
-                          _stream(new_tokens)))
+        d = _ADVANCE.pack(new_tokens.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), free_pages.data_ptr(),
+                          free_span.data_ptr(), *out._args, B, M, C, block_size, rows)
+        _check(_c_advance(d, torch._C._cuda_getCurrentRawStream(device.index)))
     return out

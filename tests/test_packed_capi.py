@@ -46,6 +46,13 @@ def test_prompt_null_and_empty(C):
     assert prompt(C, tokens=0) == OK and prompt(C, batch=0, query_starts=None) == OK
 
 
+def test_prompt_bytes_are_the_descriptor(C):
+    """The bytes that memopt_C packs are those of the ctypes mirror."""
+    args = (1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 16, 17, 18, 19, -1, 21)
+    assert C._PROMPT.pack(*args) == bytes(C.PromptDesc(*args))
+    assert [C._count32(n) for n in (-2 ** 40, -1, 0, 7, 2 ** 40)] == [-1, -1, 0, 7, 2 ** 31 - 1]
+
+
 def packed(C, call=True, **kw):
     d = C.PackedDesc(P, P, 8, 8, 8, 2, 64, 512, 64, 512, 64, 1, P, None, 16, 100, P, 20, P, P, 1, 320, -1, 0, P, 1 << 40)
     for k, v in kw.items():
@@ -109,10 +116,12 @@ def test_packed_workspace(C):
 
 
 @pytest.mark.parametrize("text,code,at,value", [
-    ("positive", INVALID, 2, 0), ("4096", UNSUPPORTED, 2, 4097), ("positive", INVALID, 4, 0), ("positive", INVALID, 6, 0),
-    ("positive", INVALID, 8, 0), ("positive", INVALID, 9, -1), ("2^31", UNSUPPORTED, 4, 2 ** 27),
-] + [("null", INVALID, i, None) for i in (0, 1, 3, 5, 7, 10, 11, 12, 13, 14, 15)])
+    ("positive", INVALID, 11, 0), ("4096", UNSUPPORTED, 11, 4097), ("positive", INVALID, 12, 0),
+    ("positive", INVALID, 13, 0), ("positive", INVALID, 14, 0), ("positive", INVALID, 15, -1),
+    ("2^31", UNSUPPORTED, 12, 2 ** 27),
+] + [("null", INVALID, i, 0) for i in range(11)])
 def test_advance_refusals(C, text, code, at, value):
-    args = [P, P, 4, P, 8, P, 32, P, 16, 4, P, P, P, P, P, P, None]
+    args = [P] * 11 + [4, 8, 32, 16, 4]
     args[at] = value
-    refused(C, C._c_advance(*args), code, text)
+    refused(C, C._c_advance(C._ADVANCE.pack(*args), None), code, text)
+    refused(C, C._c_advance(None, None), INVALID, "null")
