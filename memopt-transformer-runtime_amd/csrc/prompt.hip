@@ -47,10 +47,11 @@ struct Fp16 {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return as_u32(half2_t{(half_t)a, (half_t)b}); }
-  static __device__ __forceinline__ float add2(uint32_t w, float s) {
-    return __builtin_amdgcn_fdot2(as_half2(w), half2_t{(half_t)1.0f, (half_t)1.0f}, s, false);
+  static __device__ __forceinline__ float dot2(uint32_t w, uint32_t y, float s) {
+    return __builtin_amdgcn_fdot2(as_half2(w), as_half2(y), s, false);
   }
   static __device__ __forceinline__ float value(uint16_t x) { return (float)__builtin_bit_cast(half_t, x); }
+  static constexpr uint32_t kOnes = 0x3C003C00u;
   static constexpr uint32_t kExponent = 0x7C00u;
 };
 struct Bf16 {
@@ -62,10 +63,11 @@ struct Bf16 {
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, x2{(__bf16)a, (__bf16)b});
   }
-  static __device__ __forceinline__ float add2(uint32_t w, float s) {
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(x2, w), __builtin_bit_cast(x2, 0x3F803F80u), s, false);
+  static __device__ __forceinline__ float dot2(uint32_t w, uint32_t y, float s) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(x2, w), __builtin_bit_cast(x2, y), s, false);
   }
   static __device__ __forceinline__ float value(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
+  static constexpr uint32_t kOnes = 0x3F803F80u;
   static constexpr uint32_t kExponent = 0x7F80u;
 };
 
@@ -232,17 +234,16 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
   const Rows seq = rows_of(p.starts, p.T, b);
   const int32_t rows = seq.n * p.G, ctx = PAGED ? p.ctx[b] : seq.n, pos0 = ctx - seq.n;
   const int32_t len = PAGED ? min(ctx, p.max_tokens) : seq.n;  // keys
-  const int32_t q0 = R * __builtin_amdgcn_readfirstlane(tile.t), qw0 = q0 + 32 * wave, qi = qw0 + n;
-  const bool q_ok = qi < rows;
-  const int32_t tok = p.by_g(min(qi, rows - 1)), qp = pos0 + tok;
-  const int64_t q_head = (int64_t)kvh * p.G + (min(qi, rows - 1) - tok * p.G);
+  const int32_t q0 = R * __builtin_amdgcn_readfirstlane(tile.t), qw0 = q0 + 32 * wave;
   auto pos_of = [&](int32_t row) { return pos0 + p.by_g(min(row, rows - 1)); };
 
   u32x4p_t qf[NCH];
 #pragma unroll
   for (int c = 0; c < NCH; ++c) qf[c] = (u32x4p_t){};
-  if (q_ok) {
-    const uint16_t *src = p.q + (int64_t)(seq.start + tok) * p.q_ts + q_head * p.q_hs + 8 * hl;
+  if (qw0 + n < rows) {
+    const int32_t tok = p.by_g(qw0 + n);
+    const uint16_t *src = p.q + (int64_t)(seq.start + tok) * p.q_ts +
+                          ((int64_t)kvh * p.G + qw0 + n - tok * p.G) * p.q_hs + 8 * hl;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) qf[c] = *reinterpret_cast<const u32x4p_t *>(src + 16 * c);
   }
@@ -320,12 +321,14 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
   // those, iterations [f0, f1) hold window tiles that all its rows see whole.
   const bool any = qw0 < rows;
   int32_t v0 = sink_tiles, v1 = sink_tiles, f0 = 0, f1 = 0;
+  int32_t first_whole = 0;  // keys from here on are in every row's window, as far as it reaches
   if (any) {
     const int32_t off = sink_tiles - t_first;  // iteration of tile t: t + off
     const int32_t first = pos_of(qw0), last = pos_of(qw0 + 31);
+    first_whole = max(0, last - p.W + 1);
     v0 = max(sink_tiles, max(0, first - p.W + 1) / TK + off);
     v1 = max(v0, max(0, min(last, len - 1) + TK) / TK + off);
-    f0 = max(sink_tiles, (max(0, last - p.W + 1) + TK - 1) / TK + off);
+    f0 = max(sink_tiles, (first_whole + TK - 1) / TK + off);
     f1 = max(f0, max(0, min(first + 1, len)) / TK + off);
   }
   // Over a cache: one byte per 16 tokens, 1 where their page is there. If one
@@ -340,10 +343,30 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
   auto sees = [&](int32_t it) { return it < sink_tiles ? any : it >= v0 && it < v1; };
 
   // Register r of block blk holds key tb + 32 blk + 8 (r / 4) + 4 hl + r % 4.
+  // (The row is worked out again from the lane: held through the tiles it spills.)
+  auto lane_row = [&]() __attribute__((always_inline)) {
+    int32_t row = qw0 + (int32_t)(__lane_id() & 31);
+    asm volatile("" : "+v"(row));
+    return row;
+  };
   auto apply_mask = [&](f32x16_t (&s)[2], int32_t tb) __attribute__((always_inline)) {
-    const int32_t key0 = tb + 4 * hl;
-    const int32_t last = q_ok ? min(qp, len - 1) - key0 : -1, first = qp - p.W + 1 - key0, sink = p.sinks - key0;
+    const int32_t key0 = tb + 4 * hl, row = lane_row(), qp = pos_of(row);
+    const bool q_ok = row < rows;
+    const int32_t last = q_ok ? min(qp, len - 1) - key0 : -1;
     const uint32_t link = PAGED ? links[key_at(tb) / TK] : 0x01010101u;
+    if (tb >= first_whole) {  // (wave-uniform) no row's window begins behind the tile's first key
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int32_t end = !PAGED || ((link >> (16 * blk + 8 * half)) & 1) ? last : -1;
+#pragma unroll
+          for (int r = 8 * half; r < 8 * half + 8; ++r)
+            s[blk][r] = 32 * blk + 8 * (r >> 2) + (r & 3) <= end ? s[blk][r] : -INFINITY;
+        }
+      return;
+    }
+    const int32_t first = qp - p.W + 1 - key0, sink = p.sinks - key0;
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
@@ -421,7 +444,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
       pb[i >> 2][i & 3] = E::pack(s[2 * i], s[2 * i + 1]);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = E::add2(pb[i >> 2][i & 3], sum);
+    for (int i = 0; i < 8; ++i) sum = E::dot2(pb[i >> 2][i & 3], E::kOnes, sum);
   };
   // Operands: K piece c of a 32-key block; V of 16 keys (half i % 2 of a
   // 32-key block) and dims 32 (i / 2) .. + 31, transposed from four-row reads.
@@ -581,10 +604,19 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
 #pragma unroll
         for (int c = 0; c < 4; ++c) vf[c] = vfrag(vt, c >> 1, 2 * db + (c & 1));
         if (!full) {
+          // A weight of 0 must not meet an inf or NaN. Few tiles hold one, and
+          // a sum of zero times every element tells with a quarter of the work.
+          float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) vf[c][i] = tame<E>(vf[c][i], odd);
+            for (int i = 0; i < 4; ++i) z[c] = E::dot2(vf[c][i], 0, z[c]);
+          if (__any(!((z[0] + z[1]) + (z[2] + z[3]) == 0.0f))) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) vf[c][i] = tame<E>(vf[c][i], odd);
+          }
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[db] = E::mfma(vf[c], pf[c >> 1][c & 1], o[db]);
@@ -646,9 +678,10 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
   }
 
   if (__any(odd != 0)) {
-    // inf and NaN in V entered the masked tiles as finite values, since the
-    // weight 0 of a row that does not see them would make NaN of them. Rows
-    // that do see one have inf or NaN in that column whatever its weight.
+    // inf and NaN in V entered the masked tiles as finite values. Rows that do
+    // see one have inf or NaN in that column whatever its weight.
+    const int32_t qp = pos_of(lane_row());
+    const bool q_ok = lane_row() < rows;
 #pragma unroll 1
     for (int32_t i = 0; i < n_tiles; ++i) {
       if (!sees(i) || (i >= f0 && i < f1)) continue;
@@ -668,11 +701,9 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
   }
 
   const float l = xor32_sum(lsum + lsum1);
-  if (!q_ok) return;
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-  // (The row is worked out again from the lane: held through the tiles it spills.)
-  int32_t row = qw0 + (int32_t)(__lane_id() & 31);
-  asm volatile("" : "+v"(row));
+  const int32_t row = lane_row();
+  if (row >= rows) return;
   const int32_t row_tok = p.by_g(row);
   uint16_t *dst = p.out + (int64_t)(seq.start + row_tok) * p.o_ts + ((int64_t)kvh * p.G + row - row_tok * p.G) * p.o_hs +
                   4 * hl;
