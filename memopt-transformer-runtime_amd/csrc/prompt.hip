@@ -8,6 +8,17 @@
 // which is the causal rule of the paged attention (attention.hpp key_range).
 // One pass over the keys with a running maximum m and sum; a later, larger
 // maximum scales what was summed before it.
+//
+// Bound by the matrix instructions and the softmax between them: 4 D flops per
+// visible pair and query head. A workgroup takes 128 rows (32 per wave, as
+// v_mfma_f32_32x32x16 has columns) against 64-key tiles: that reads K and V
+// once per 128 rows, and two workgroups (64 KiB of LDS and 252 registers each)
+// fit a CU. The softmax of one tile runs beside the products of the next, in
+// one wave, since two waves per SIMD do not cover it by themselves (16384
+// tokens, window 4096, 32 query over 8 key heads of 128: 1068 us one behind the
+// other, 941 now, 1.02 PFLOP/s; a library product of 8192^3 reaches 1.24).
+// Three prompts of up to 9000 tokens, 40 heads: 839 us, 1.03 PFLOP/s; 24 of 20
+// to 2500 tokens: 195 us, 0.77, with half of each diagonal tile hidden.
 #include <algorithm>
 #include <cmath>
 
