@@ -160,28 +160,38 @@ struct PackedV<D, MEMOPT_KV_FP16> {
   uint32_t w[8][D / 32];  // token e: D / 16 halves
 };
 
-// 16 bytes per lane from buffer offset IMM + off into LDS byte m0v + IMM + 16 *
-// lane, not waited for (the compiler does not track it; the immediate counts
-// for both addresses, and the s_nop is the wait state between a write of m0
-// and its use, as in lds_dma.hpp). STREAM: data read once per launch
-// (kStreamLoad).
-template <bool STREAM, int IMM>
-__device__ __forceinline__ void ring_copy(__amdgpu_buffer_rsrc_t r, uint32_t m0v, uint32_t off) {
-  static_assert(IMM < 4096, "immediate offsets are 12 bits");
-  if constexpr (STREAM)
-    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen offset:%3 nt lds"
-                 ::"v"(off), "s"(r), "{m0}"(m0v), "i"(IMM) : "memory");
+// A block of BLK bytes (1 or 2 KiB and a tail) into LDS at m0v, 16 bytes per
+// lane (lane16 = 16 * lane), not waited for: the compiler does not track it.
+// The immediate offsets count for both addresses, the s_nop is the wait state
+// between a write of m0 and its use, as in lds_dma.hpp, and the tail's lanes are
+// chosen in here (a branch around them costs six scalar instructions). STREAM:
+// data read once per launch (kStreamLoad).
+#define MEMOPT_COPY(OFF, NT) "buffer_load_dwordx4 %1, %2, 0 offen offset:" OFF NT " lds\n\t"
+#define MEMOPT_COPY_TAIL(LANES, OFF, NT) \
+  "s_mov_b64 %0, exec\n\ts_and_b64 exec, exec, " LANES "\n\t" MEMOPT_COPY(OFF, NT) "s_mov_b64 exec, %0"
+template <bool STREAM, int BLK>
+__device__ __forceinline__ void block_copy(__amdgpu_buffer_rsrc_t r, uint32_t m0v, uint32_t lane16) {
+  static_assert(BLK == 2048 + 8 * 16 || BLK == 1024 + 4 * 16, "tails of 8 and 4 lanes");
+  uint64_t lanes;
+#define MEMOPT_COPY_ASM(TEXT) \
+  asm volatile("s_nop 0\n\t" TEXT : "=&s"(lanes) : "v"(lane16), "s"(r), "{m0}"(m0v) : "memory", "scc")
+  if constexpr (BLK == 2176 && STREAM)
+    MEMOPT_COPY_ASM(MEMOPT_COPY("0", " nt") MEMOPT_COPY("1024", " nt") MEMOPT_COPY_TAIL("0xff", "2048", " nt"));
+  else if constexpr (BLK == 2176)
+    MEMOPT_COPY_ASM(MEMOPT_COPY("0", "") MEMOPT_COPY("1024", "") MEMOPT_COPY_TAIL("0xff", "2048", ""));
+  else if constexpr (STREAM)
+    MEMOPT_COPY_ASM(MEMOPT_COPY("0", " nt") MEMOPT_COPY_TAIL("0xf", "1024", " nt"));
   else
-    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen offset:%3 lds"
-                 ::"v"(off), "s"(r), "{m0}"(m0v), "i"(IMM) : "memory");
+    MEMOPT_COPY_ASM(MEMOPT_COPY("0", "") MEMOPT_COPY_TAIL("0xf", "1024", ""));
+#undef MEMOPT_COPY_ASM
 }
+#undef MEMOPT_COPY
+#undef MEMOPT_COPY_TAIL
 
 template <typename T>
 __device__ __forceinline__ T lds_at(uint32_t a) {
   return *(const __attribute__((address_space(3))) T *)(uintptr_t)a;
 }
-
-static constexpr int kRingSteps = 2;
 
 // Workgroups per CU that the kernels' registers and LDS are meant for.
 __host__ __device__ static constexpr int resident(int NW, int QB) { return QB == 2 ? 2 : NW == 4 ? 3 : 1; }
@@ -196,7 +206,7 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
   constexpr int OS = D + 4;               // row stride of s_o: 16 rows of D floats would share a bank
   // Pages stream through a ring of raw blocks per wave (see copy_step), which
   // the merge of the waves takes over when the steps are done.
-  constexpr int BLK = 16 * D + 64 * (D / 64), STG = 2 * BLK, NS = kRingSteps;
+  constexpr int BLK = 16 * D + 64 * (D / 64), STG = 2 * BLK, NS = 2;
   constexpr int OBYTES = NW * QN * OS * 4, RBYTES = PAGES ? NW * NS * STG : 0, MBYTES = QN * kMaxParts * 4 + NT * 16;
   __shared__ __attribute__((aligned(16))) uint8_t smem[std::max({OBYTES, RBYTES, MBYTES})];
   float(*const s_o)[QN][OS] = reinterpret_cast<float(*)[QN][OS]>(smem);
@@ -293,26 +303,34 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
     auto logical = [&](int32_t i) { return i + (i < sc ? 0 : skip); };
     const int32_t full0 = (max(skip > 0 ? sc : 0, ((max(0, pos_hi - p.W + 1) + 15) >> 4) - skip) + 1) >> 1;
     const int32_t full1 = ((max(0, min(kv_lim, pos_lo + 1)) >> 4) - skip) >> 1;
-    struct Step {  // its block-table entries, not yet waited for
-      int32_t i, a, b;
-    };
-    auto fetch = [&](int32_t i) __attribute__((always_inline)) {
-      Step e;
-      e.i = i;
-      const int32_t ca = 2 * i, cb = 2 * i + 1;
-      const int32_t la = ca < n_vis ? logical(ca) : 0, lb = cb < n_vis ? logical(cb) : 0;  // (a row has an entry 0)
-      e.a = btrow[cpp == 1 ? la : la / cpp];
-      e.b = btrow[cpp == 1 ? lb : lb / cpp];
-      if (cb >= n_vis) e.b = -1;
-      return e;
-    };
-    auto mapped = [&](int32_t phys) { return phys >= 0 && phys < nb32; };
-    // Byte offset of chunk `lc` (chunk 0 of page 0, always mapped, if its page is not).
-    auto offset_of = [&](int32_t phys, int32_t lc) __attribute__((always_inline)) {
-      const bool ok = mapped(phys);
+    // This wave's steps are begin + wave + j NW, j < mine. Their block-table
+    // entries are looked up 32 steps at a time, lane l for chunk l % 2 of step
+    // at0 + l / 2: byte offset of the chunk (chunk 0 of page 0 if its page is not
+    // there), whether it is there, and whether the step needs no mask. (Entry
+    // by entry, in scalar loads, they took half as many scalar instructions
+    // per step as it has vector ones, and every wait for LDS waited for them.)
+    const int32_t mine = max(0, end - begin - wave + NW - 1) / NW;
+    int32_t at0 = 0;
+    uint32_t off_lo = 0, off_hi = 0;
+    uint64_t there = 0, whole = 0;
+    auto look_up = [&](int32_t j0) __attribute__((always_inline)) {
+      at0 = j0;
+      const int32_t i = begin + wave + (j0 + (lane >> 1)) * NW, c = 2 * i + (lane & 1), lc = logical(c);
+      const bool in = i < end && c < n_vis;
+      const int32_t phys = in ? btrow[cpp == 1 ? lc : lc / cpp] : -1;
+      const bool ok = phys >= 0 && phys < nb32;
       int64_t x = (int64_t)(ok ? phys : 0) * p.kv_ps;
       if constexpr (!PAGES) x += (int64_t)(ok ? 16 * (lc - lc / cpp * cpp) : 0) * p.kv_ts;
-      return x;
+      off_lo = (uint32_t)x;
+      off_hi = (uint32_t)((uint64_t)x >> 32);
+      there = __ballot(ok);
+      whole = there & (there >> 1) & __ballot(i >= full0 && i < full1);  // (even bits count)
+    };
+    auto step_at = [&](int32_t j) { return begin + wave + j * NW; };
+    auto offset_of = [&](int32_t j, int chunk) __attribute__((always_inline)) {
+      const int32_t l = 2 * (j - at0) + chunk;
+      return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)off_hi, l) << 32 |
+                       (uint32_t)__builtin_amdgcn_readlane((int)off_lo, l));
     };
 
     const Int4Page f(D);
@@ -320,20 +338,17 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
     PackedV<D, FMT> vr;
     const int p0 = 4 * (g & 1);  // this lane's score tokens: p0 + i and p0 + i + 8 of chunk g / 2
     // Pages: the two blocks of a step as they are, 1 KiB per copy, straight into
-    // the wave's ring: kRingSteps steps are in flight without holding registers.
+    // the wave's ring: NS steps are in flight without holding registers.
     const uint32_t ring = lds_u32(smem) + wave * NS * STG;
     const uint8_t *const kbase = p.k + (int64_t)kvh * p.kv_hs, *const vbase = p.v + (int64_t)kvh * p.kv_hs;
     auto copy_block = [&](int64_t kv, uint32_t dst) __attribute__((always_inline)) {
       const __amdgpu_buffer_rsrc_t rs =
           __builtin_amdgcn_make_buffer_rsrc((void *)(kbase + kv), (short)0, BLK, 0x00020000);
-      constexpr int TAIL = BLK / 1024 * 1024;
-      ring_copy<QB == 1, 0>(rs, dst, 16 * lane);
-      if constexpr (D == 128) ring_copy<QB == 1, 1024>(rs, dst, 16 * lane);
-      if (lane < (BLK - TAIL) / 16) ring_copy<QB == 1, TAIL>(rs, dst, 16 * lane);
+      block_copy<QB == 1, BLK>(rs, dst, 16 * lane);
     };
-    auto copy_step = [&](const Step &e, int stage) __attribute__((always_inline)) {
-      copy_block(offset_of(e.a, 0), ring + stage * STG);
-      copy_block(offset_of(e.b, 0), ring + stage * STG + BLK);
+    auto copy_step = [&](int32_t j, int stage) __attribute__((always_inline)) {
+      copy_block(offset_of(j, 0), ring + stage * STG);
+      copy_block(offset_of(j, 1), ring + stage * STG + BLK);
     };
     // K of a step: lane row r is tokens r % 8 and r % 8 + 8 of chunk r / 8.
     // V: lane (r, g) holds four dims from 64 u + 4 r (fp16: [D/16 r, D/16 (r + 1))) of its score tokens.
@@ -367,9 +382,10 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
       }
     };
     // fp16 pools: the same from global memory into registers.
-    auto load_k = [&](const Step &e) __attribute__((always_inline)) {
+    auto load_k = [&](int32_t j) __attribute__((always_inline)) {
       if constexpr (!PAGES) {
-        const uint8_t *base = kbase + (r < 8 ? offset_of(e.a, logical(2 * e.i)) : offset_of(e.b, logical(2 * e.i + 1)));
+        const int64_t xa = offset_of(j, 0), xb = offset_of(j, 1);
+        const uint8_t *base = kbase + (r < 8 ? xa : xb);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -378,9 +394,10 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
                                                              2 * (32 * kk + 8 * g));
       }
     };
-    auto load_v = [&](const Step &e) __attribute__((always_inline)) {
+    auto load_v = [&](int32_t j) __attribute__((always_inline)) {
       if constexpr (!PAGES) {
-        const uint8_t *base = vbase + (g < 2 ? offset_of(e.a, logical(2 * e.i)) : offset_of(e.b, logical(2 * e.i + 1)));
+        const int64_t xa = offset_of(j, 0), xb = offset_of(j, 1);
+        const uint8_t *base = vbase + (g < 2 ? xa : xb);
 #pragma unroll
         for (int x = 0; x < 8; ++x) {  // element 2 i + t: token p0 + i + 8 t
           const uint8_t *src = base + (int64_t)(p0 + (x >> 1) + 8 * (x & 1)) * p.kv_ts + (D / 8) * r;
@@ -482,7 +499,7 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
     constexpr float kTop = 7.0f;
     uint32_t odd = 0;  // nonzero: a masked step held inf or NaN in V
     // One step; `between` runs when K has been used and V has not.
-    auto step = [&](const Step &e, auto between) __attribute__((always_inline)) {
+    auto step = [&](int32_t j, auto between) __attribute__((always_inline)) {
       f32x4_t s[QB][NG][2];
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
@@ -509,13 +526,12 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
           }
           x[qb][e] = fmaf(y, p.qk_scale_log2, ncm[qb]);
         }
+      const int32_t bit = 2 * (j - at0);
+      const bool full = (whole >> bit) & 1;  // (wave-uniform)
+      const bool c_ok = (there >> (bit + (g >> 1))) & 1;
+      const int32_t key0 = 16 * logical(2 * step_at(j) + (g >> 1)) + 4 * (g & 1);
       between();
 
-      const bool ok_a = mapped(e.a), ok_b = mapped(e.b);
-      const bool full = e.i >= full0 && e.i < full1 && ok_a && ok_b;  // (wave-uniform)
-      const int32_t ta = 16 * logical(2 * e.i), tb = 16 * logical(2 * e.i + 1);
-      const int32_t key0 = (g < 2 ? ta : tb) + 4 * (g & 1);
-      const bool c_ok = g < 2 ? ok_a : ok_b;
       h8_t pf[QB][NG];
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
@@ -651,50 +667,42 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
     // Wave w takes steps begin + w, begin + w + NW, ...
     if constexpr (PAGES) {
       constexpr int CPS = 2 * ((BLK + 1023) / 1024);  // copies per step
-      Step queue[NS];                                 // the steps in flight, then the next
+      look_up(0);
 #pragma unroll
-      for (int k = 0; k < NS; ++k) {
-        queue[k] = fetch(begin + wave + k * NW);
-        if (queue[k].i < end) copy_step(queue[k], k);
-      }
-      Step next = fetch(begin + wave + NS * NW);
+      for (int k = 0; k < NS; ++k)
+        if (k < mine) copy_step(k, k);
       load_q();  // (behind the first copies, which take longer)
       int stage = 0;
 #pragma unroll 1
-      for (int32_t round = begin; round < end; round += NW) {
-        if (queue[0].i >= end) continue;
-        // this step's copies are the oldest: wait until no more than the later steps' are left
-        if (queue[NS - 1].i < end) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * CPS) : "memory");
+      for (int32_t j = 0; j < mine; ++j) {
+        if (j + NS - at0 >= 32) look_up(j);
+        // this step's copies are the oldest: wait until no more than the later step's are left
+        static_assert(NS == 2, "one later step");
+        if (j + 1 < mine) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CPS) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        const Step e = queue[0];
         read_k(stage);
-        step(e, [&]() __attribute__((always_inline)) {
+        step(j, [&]() __attribute__((always_inline)) {
           read_v(stage);
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the stage is filled again
-          if (next.i < end) copy_step(next, stage);
-#pragma unroll
-          for (int k = 0; k + 1 < NS; ++k) queue[k] = queue[k + 1];
-          queue[NS - 1] = next;
-          next = fetch(next.i + NW);
+          if (j + NS < mine) copy_step(j + NS, stage);
         });
-        stage = stage + 1 == NS ? 0 : stage + 1;
+        stage ^= 1;
       }
       __syncthreads();  // every wave has read its ring: the sums take its place
     } else {
-      Step e = fetch(begin + wave), next = fetch(begin + wave + NW);
-      if (e.i < end) {
-        load_k(e);
-        load_v(e);
+      look_up(0);
+      if (0 < mine) {
+        load_k(0);
+        load_v(0);
       }
       load_q();
-      while (e.i < end) {
-        const Step after = fetch(next.i + NW);
-        step(e, [&]() __attribute__((always_inline)) {
-          if (next.i < end) load_k(next);
+#pragma unroll 1
+      for (int32_t j = 0; j < mine; ++j) {
+        if (j + 1 - at0 >= 32) look_up(j);
+        step(j, [&]() __attribute__((always_inline)) {
+          if (j + 1 < mine) load_k(j + 1);
         });
-        if (next.i < end) load_v(next);
-        e = next;
-        next = after;
+        if (j + 1 < mine) load_v(j + 1);
       }
     }
 
@@ -703,14 +711,14 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
         // Rows that see an inf or NaN of V have inf or NaN in its column whatever
         // its weight; a lane looks through its quarter of the dims.
 #pragma unroll 1
-        for (int32_t i = begin + wave; i < end; i += NW) {
-          if (i >= full0 && i < full1) continue;  // (a whole chunk there is unlinked: all zeros)
-          const Step e = fetch(i);
+        for (int32_t j = 0; j < mine; ++j) {
+          if (j < at0 || j >= at0 + 32) look_up(j);
+          if (step_at(j) >= full0 && step_at(j) < full1) continue;  // (a whole chunk there is unlinked: all zeros)
 #pragma unroll 1
           for (int tk = 0; tk < 32; ++tk) {
-            const int32_t phys = tk < 16 ? e.a : e.b, lc = logical(2 * i + (tk >> 4)), t = tk & 15, key = 16 * lc + t;
-            if (!mapped(phys) || key >= kv_lim) continue;
-            const half_t *row = reinterpret_cast<const half_t *>(vbase + offset_of(phys, lc) + (int64_t)t * p.kv_ts);
+            const int32_t t = tk & 15, key = 16 * logical(2 * step_at(j) + (tk >> 4)) + t;
+            if (!((there >> (2 * (j - at0) + (tk >> 4))) & 1) || key >= kv_lim) continue;
+            const half_t *row = reinterpret_cast<const half_t *>(vbase + offset_of(j, tk >> 4) + (int64_t)t * p.kv_ts);
 #pragma unroll
             for (int d = 0; d < D / 4; ++d) {
               const float y = (float)row[(D / 4) * g + d];
@@ -759,7 +767,7 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
     // A run holds at most two blocks in part: one that began before it (slot 0),
     // one that begins in it and goes on behind it (slot 1).
     auto partial_slot = [&](int32_t w) { return ((int64_t)w * 2 + (w == w0 ? 1 : 0)) * p.Hk + kvh; };
-    const int64_t mine = partial_slot(wg) * QN;
+    const int64_t own_part = partial_slot(wg) * QN;
     for (int idx = tid; idx < live * (D / 4); idx += NT) {
       const int row = idx / (D / 4), d = 4 * (idx % (D / 4));
       float mx = s_ml[0][row][0];
@@ -777,13 +785,13 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
         write_row(row, d, x, l);
       } else {
         // (agent scope: the other workgroups of the block may run on other XCDs)
-        uint64_t *dst = reinterpret_cast<uint64_t *>(p.ws_o + (mine + row) * D + d);
+        uint64_t *dst = reinterpret_cast<uint64_t *>(p.ws_o + (own_part + row) * D + d);
         __hip_atomic_store(dst, __builtin_bit_cast(uint64_t, u32x2_t{__float_as_uint(x[0]), __float_as_uint(x[1])}),
                            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __hip_atomic_store(dst + 1, __builtin_bit_cast(uint64_t, u32x2_t{__float_as_uint(x[2]), __float_as_uint(x[3])}),
                            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if (d == 0)
-          __hip_atomic_store(reinterpret_cast<uint64_t *>(p.ws_ml + 2 * (mine + row)),
+          __hip_atomic_store(reinterpret_cast<uint64_t *>(p.ws_ml + 2 * (own_part + row)),
                              __builtin_bit_cast(uint64_t, u32x2_t{__float_as_uint(mx), __float_as_uint(l)}),
                              __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }

@@ -125,7 +125,8 @@ def test_windows_and_sinks(fmt, window, sinks, D):
 @pytest.mark.parametrize("Hq,Hk,D,ctx,qn", [(8, 2, 64, [3000], [1]), (8, 1, 128, [5000, 100, 2500], [1, 1, 1]),
                                             (20, 1, 128, [2100], [3]), (32, 8, 128, [1500], [1]),
                                             (4, 2, 64, [2500, 600], [40, 1]), (8, 2, 64, [6100], [1]),
-                                            (8, 4, 64, [4000, 9000], [1, 2]), (32, 8, 128, [7000], [1])])
+                                            (8, 4, 64, [4000, 9000], [1, 2]), (32, 8, 128, [7000], [1]),
+                                            (16, 1, 64, [6100], [1]), (10, 1, 128, [5300, 4700], [1, 1])])
 def test_long_contexts_in_splits(fmt, Hq, Hk, D, ctx, qn):
     c = Case(fmt, ctx, qn, Hq, Hk, D, seed=7)
     plan = memopt_C.PreparedPackedAttention(*c.args())
