@@ -22,10 +22,11 @@
 // Work: QN = 16 * QB rows of one (sequence, key head) are a block; a wave takes
 // two 16-token chunks (32 tokens) of a block's visible ones per step. The steps
 // of all blocks of a key head form one list, which is dealt to its workgroups
-// of 4 waves in equal runs, whatever the sequences' lengths (by sequence and
-// split, a batch of 2700 to 8192 tokens ran as long as its longest part). A
-// block whose steps fall to one workgroup is finished there; else each
-// leaves partial sums, and the last to arrive adds them up. Layout, as in direct.hip:
+// of 4 waves in runs that are equal but for a few steps around block ends,
+// whatever the sequences' lengths (by sequence and split, a batch of 2700 to
+// 8192 tokens ran as long as its longest part). A block whose steps fall to
+// one workgroup is finished there; else each leaves partial sums, and the last
+// to arrive adds them up. Layout, as in direct.hip:
 //  * S^T = K Q^T on v_mfma_f32_16x16x32_f16, one product per token half t: row
 //    r of the A operand is token r % 8 + 8 t of chunk r / 8, which is how a
 //    page interleaves its tokens. Over pages each product covers dims of one
@@ -40,12 +41,13 @@
 //    weights times that group's scale per token. So a page's only rounding to
 //    16 bits is that of weight times scale.
 //
-// Bound by vector instructions: about 200 per step of 32 tokens and 16 rows
-// (D = 128, INT4), four cycles each, most of them the unpacking of V; a copy
-// without them streams 131072 tokens of 8 key heads in 18 us, the kernel takes
-// 35. 32 sequences of 2700 to 8192 tokens, 32 query over 8 key heads: 47 us, 4.2
-// TB/s of pages; one of 131072: 35 us, 4.1 TB/s. A card's large copy reaches
-// 5.1.
+// Bound by the stream of pages and 7 us around it: a copy of the kernel without
+// its arithmetic takes 41.5 us where it takes 46.7 (32 sequences of 2700 to 8192
+// tokens, 32 query over 8 key heads: 4.2 TB/s of pages), one without the copies
+// 37; one sequence of 131072 tokens 30 and 29 of 34.5 (4.1 TB/s). A large copy
+// reaches 5.1 on the card. One sequence of 1024: 8.6 us, a chain of the list of
+// sequences (1.0), queries (0.8), two steps (1.8), the waves' merge (0.7), the
+// arrival (0.6) and the workgroups' merge (2.5).
 #include <algorithm>
 #include <cmath>
 
@@ -219,7 +221,7 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
 
   // The list's length; then the sequence that holds this workgroup's first
   // place. Lane i takes sequence b0 + i; up to 64 sequences are counted once.
-  uint32_t sum = 0, c = 0, nb = 0;
+  uint32_t sum = 0, blocks_sum = 0, c = 0, nb = 0;
   auto count = [&](int32_t b0) __attribute__((always_inline)) {
     c = nb = 0;
     if (b0 + lane < p.B) {
@@ -231,6 +233,7 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
   for (int32_t b0 = 0; b0 < p.B; b0 += 64) {
     count(b0);
     sum = __builtin_elementwise_add_sat(sum, (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(c), 63));
+    blocks_sum = __builtin_elementwise_add_sat(blocks_sum, (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(nb), 63));
   }
   // (past 2^31 only where sequences overlap: nothing is computed then)
   const int32_t total = (int32_t)sum;
@@ -238,14 +241,22 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
   const int32_t wgs = min(p.wgs, max(1, total / NW));
   if (total <= 0 || wg >= wgs) return;
   const int32_t run = total / wgs, longer = total - run * wgs;  // the first `longer` runs have one place more
-  const int32_t first = wg * run + min(wg, longer);
+  auto start_of = [&](int32_t w) { return w * run + min(w, longer); };
+  const int32_t first = start_of(wg), next = start_of(wg + 1);
   int32_t at = first;
-  const int32_t stop = at + run + (wg < longer ? 1 : 0);
   auto wg_of = [&](int32_t x) {
     const int32_t edge = longer * (run + 1);
     const bool head = x < edge;
     return (head ? 0 : longer) + (head ? x : x - edge) / (head ? run + 1 : run);
   };
+  // A run that would begin within `snap` places of a block's end begins there: a
+  // block in two workgroups costs a start and a merge more, about as long as
+  // that many steps of one; the more, the fewer workgroups there are for each
+  // block. (Us with 0, 8 and 16, 32 query over 8 key heads, 96 workgroups: 64
+  // sequences of 300 tokens 22.3, 13.1, 13.0; 64 of 1000 28.1, 26.4, 22.5; 128 of
+  // 100 to 3000 57.7, 53.9, 51.0; 32 of 2700 to 8192 45.6, 42.2, 42.6; 8 of 100 to
+  // 2000 17.4, 12.3, 13.6; 4 of 1000 11.2, 11.3, 12.7.)
+  const int32_t snap = blocks_sum <= 1 ? 0 : 2 * blocks_sum >= (uint32_t)wgs ? 16 : 8;
   int32_t seq_at = 0, seq_blocks = 0, b = 0;  // places and blocks before sequence b
   for (int32_t b0 = 0; b0 < p.B; b0 += 64) {
     if (p.B > 64) count(b0);
@@ -264,22 +275,30 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
 
   // Block by block of this workgroup's run.
   Seq seq = sequence<QN>(p, starts, ctxs, b);
-  while (at < stop) {
-    while (at >= seq_at + seq.blocks * seq.steps) {  // (sequences without rows take no place)
-      seq_at += seq.blocks * seq.steps;
-      seq_blocks += seq.blocks;
-      seq = sequence<QN>(p, starts, ctxs, ++b);
-    }
-    const int32_t block = seq.blocks == 1 ? 0 : (at - seq_at) / seq.steps;
+  for (;;) {
+    int32_t block, block_at, w0, w1;
+    do {
+      while (at >= seq_at + seq.blocks * seq.steps) {  // (sequences without rows take no place)
+        seq_at += seq.blocks * seq.steps;
+        seq_blocks += seq.blocks;
+        seq = sequence<QN>(p, starts, ctxs, ++b);
+      }
+      block = seq.blocks == 1 ? 0 : (at - seq_at) / seq.steps;
+      block_at = seq_at + block * seq.steps;
+      at = block_at + seq.steps;
+      const int32_t s = min(snap, seq.steps >> 1), x0 = block_at + s, x1 = at - max(s, 1);
+      w0 = x0 >= first && x0 < next ? wg : wg_of(x0);
+      w1 = x1 >= first && x1 < next ? wg : wg_of(x1);
+    } while (wg > w1 && at < total);  // (a run that begins behind its first place)
+    if (wg < w0 || wg > w1) return;
     if (seq_blocks + block >= p.blocks) return;  // sequences overlap: past the counters
-    const int32_t block_at = seq_at + block * seq.steps;
     const int32_t row0 = block * QN, rows = seq.n * p.G, ctx = seq.ctx, kv_lim = seq.kv_lim;
     const int32_t pos0 = ctx - seq.n;  // position of the sequence's first query
     const int32_t pos_lo = pos0 + p.by_g(row0), pos_hi = pos0 + p.by_g(min(row0 + QN, rows) - 1);
     const Visible vis = visible_chunks(p, kv_lim, pos_lo, pos_hi);
     const int32_t sc = vis.sc, wc0 = vis.wc0, n_vis = vis.n;
-    const int32_t begin = at - block_at, end = min(min(stop - block_at, seq.steps), (n_vis + 1) >> 1);
-    at = min(stop, block_at + seq.steps);
+    const int32_t begin = wg == w0 ? 0 : first - block_at;
+    const int32_t end = min(wg == w1 ? seq.steps : next - block_at, (n_vis + 1) >> 1);
 
     f32x4_t o[QB][ND];
     float ncm[QB], thr[QB], lsum[QB];
@@ -478,8 +497,10 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
 #pragma unroll
             for (int kk = j * (KK / NG); kk < (j + 1) * (KK / NG); ++kk) {
               const u32x4_t y = __builtin_bit_cast(u32x4_t, qf[qb][kk]);
-              even = __builtin_amdgcn_fdot2(as_half2(y[2]), ones, __builtin_amdgcn_fdot2(as_half2(y[0]), ones, even, false), false);
-              odd_q = __builtin_amdgcn_fdot2(as_half2(y[3]), ones, __builtin_amdgcn_fdot2(as_half2(y[1]), ones, odd_q, false), false);
+              even = __builtin_amdgcn_fdot2(as_half2(y[0]), ones, even, false);
+              even = __builtin_amdgcn_fdot2(as_half2(y[2]), ones, even, false);
+              odd_q = __builtin_amdgcn_fdot2(as_half2(y[1]), ones, odd_q, false);
+              odd_q = __builtin_amdgcn_fdot2(as_half2(y[3]), ones, odd_q, false);
             }
             x = xor32_sum(xor16_sum(-1032.0f * even - 72.0f * odd_q));
           }
@@ -641,7 +662,8 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
       auto pv = [&](int i, u32x4_t a) __attribute__((always_inline)) {
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb)
-          o[qb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), pf[qb][i / (ND / NG)], o[qb][i], 0, 0, 0);
+          o[qb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), pf[qb][i / (ND / NG)], o[qb][i],
+                                                            0, 0, 0);
       };
       if constexpr (PAGES) {
 #pragma unroll
@@ -753,8 +775,6 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
     }
     __syncthreads();
     // A block whose steps lie in one run is finished here.
-    const int32_t w0 = block_at >= first ? wg : wg_of(block_at);
-    const int32_t w1 = block_at + seq.steps <= stop ? wg : wg_of(block_at + seq.steps - 1);
     const int32_t live = min(QN, rows - row0);
     auto write_row = [&](int row, int d, f32x4_t x, float l) __attribute__((always_inline)) {
       const float inv = l > 0.0f ? 1.0f / l : 0.0f;
@@ -877,6 +897,7 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
         }
       }
     }
+    if (wg < w1 || at >= total) return;
     __syncthreads();  // s_o and s_ml are free for the next block
   }
 }
@@ -1072,7 +1093,8 @@ static PackedPlan packed_plan(const memopt_packed_desc &d) {
   pl.wgs = wgs(pl.waves);
   pl.min_rows = kStagedRows;
   if (most >= pl.min_rows && (int64_t)d.tokens * d.num_heads >= 128LL * compute_units()) {
-    const int64_t W = std::min(effective_window(d.window_size, d.max_seq_len), 1 << 30), sinks = std::max(0, d.num_sink_tokens);
+    const int64_t W = std::min(effective_window(d.window_size, d.max_seq_len), 1 << 30);
+    const int64_t sinks = std::max(0, d.num_sink_tokens);
     auto up64 = [](int64_t x) { return (x + 63) / 64 * 64; };
     pl.cap = std::min(up64((int64_t)d.max_blocks_per_seq * d.block_size),
                       up64(W + std::min(d.max_query_len, d.tokens)) + 128 + up64(sinks));
@@ -1086,7 +1108,8 @@ static PackedPlan packed_plan(const memopt_packed_desc &d) {
 }
 
 struct PackedWorkspace {
-  int64_t counters, ml, links, factors, k, v, total;  // bytes of the counters; offsets of the (m, l) pairs and the staged copies
+  // Bytes of the counters; offsets of the (m, l) pairs and of the staged copies' parts.
+  int64_t counters, ml, links, factors, k, v, total;
 };
 static PackedWorkspace packed_workspace(const memopt_packed_desc &d, const PackedPlan &pl) {
   PackedWorkspace w;
@@ -1226,8 +1249,8 @@ extern "C" int memopt_packed_attention(const memopt_packed_desc *desc, void *str
     p.st = {pl.min_rows, std::min(d.max_query_len, d.tokens), pl.slots, (int32_t)pl.cap, (half_t *)(ws + w.k),
             (half_t *)(ws + w.v), ws + w.links,
             d.kv_format == MEMOPT_KV_INT4 ? (float *)(ws + w.factors) : nullptr};
-    const unsigned wgs = (unsigned)std::max<int64_t>(1, std::min<int64_t>(8LL * compute_units() / p.Hk, pl.slots * pl.cap / 64));
-    const dim3 grid(wgs * p.Hk);
+    const int64_t wgs = std::min<int64_t>(8LL * compute_units() / p.Hk, pl.slots * pl.cap / 64);
+    const dim3 grid((unsigned)(std::max<int64_t>(1, wgs) * p.Hk));
     if (d.head_dim == 128) launch_stage<128>(p, d, grid, s);
     else launch_stage<64>(p, d, grid, s);
     if ((rc = check_launch("packed_attention(stage)")) != MEMOPT_OK) return rc;

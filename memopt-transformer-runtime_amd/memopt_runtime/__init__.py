@@ -19,6 +19,6 @@ from .kv_cache import PagedKVCache, pages_needed, slots_for
 from .packed import PackedBatch
 from .policy import ThresholdPolicy, vram_utilization
 
-__all__ = ["PagedKVCache", "PackedBatch", "PolicyForward", "Policy", "read_policy", "attention_inputs", "autochunk_prefill",
-           "chunk_tokens_for_budget", "chunk_call_bytes", "pages_needed", "slots_for", "ThresholdPolicy",
-           "vram_utilization"]
+__all__ = ["PagedKVCache", "PackedBatch", "PolicyForward", "Policy", "read_policy", "attention_inputs",
+           "autochunk_prefill", "chunk_tokens_for_budget", "chunk_call_bytes", "pages_needed", "slots_for",
+           "ThresholdPolicy", "vram_utilization"]
