@@ -221,19 +221,22 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
 
   // The list's length; then the sequence that holds this workgroup's first
   // place. Lane i takes sequence b0 + i; up to 64 sequences are counted once.
-  uint32_t sum = 0, blocks_sum = 0, c = 0, nb = 0;
+  uint32_t sum = 0, blocks_sum = 0, c = 0, nb = 0, c_to = 0, nb_to = 0;  // places, blocks; up to this lane's end
+  Seq lane_seq = {};
   auto count = [&](int32_t b0) __attribute__((always_inline)) {
     c = nb = 0;
     if (b0 + lane < p.B) {
-      const Seq q = sequence<QN>(p, starts, ctxs, b0 + lane);
-      nb = q.blocks;
-      c = nb * (uint32_t)q.steps;
+      lane_seq = sequence<QN>(p, starts, ctxs, b0 + lane);
+      nb = lane_seq.blocks;
+      c = nb * (uint32_t)lane_seq.steps;
     }
+    c_to = wave_scan(c);
+    nb_to = wave_scan(nb);
   };
   for (int32_t b0 = 0; b0 < p.B; b0 += 64) {
     count(b0);
-    sum = __builtin_elementwise_add_sat(sum, (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(c), 63));
-    blocks_sum = __builtin_elementwise_add_sat(blocks_sum, (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(nb), 63));
+    sum = __builtin_elementwise_add_sat(sum, (uint32_t)__builtin_amdgcn_readlane((int)c_to, 63));
+    blocks_sum = __builtin_elementwise_add_sat(blocks_sum, (uint32_t)__builtin_amdgcn_readlane((int)nb_to, 63));
   }
   // (past 2^31 only where sequences overlap: nothing is computed then)
   const int32_t total = (int32_t)sum;
@@ -258,23 +261,25 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
   // 2000 17.4, 12.3, 13.6; 4 of 1000 11.2, 11.3, 12.7.)
   const int32_t snap = blocks_sum <= 1 ? 0 : 2 * blocks_sum >= (uint32_t)wgs ? 16 : 8;
   int32_t seq_at = 0, seq_blocks = 0, b = 0;  // places and blocks before sequence b
+  Seq seq = {};
   for (int32_t b0 = 0; b0 < p.B; b0 += 64) {
     if (p.B > 64) count(b0);
-    const int32_t incl = (int32_t)wave_scan(c), blocks = (int32_t)wave_scan(nb);
-    const int32_t sum64 = __builtin_amdgcn_readlane(incl, 63);
+    const int32_t sum64 = __builtin_amdgcn_readlane((int)c_to, 63);
     if (at < seq_at + sum64) {
-      const int src = __builtin_ctzll(__ballot(at < seq_at + incl));
+      const int src = __builtin_ctzll(__ballot(at < seq_at + (int32_t)c_to));
+      auto from = [&](int32_t v) { return __builtin_amdgcn_readlane(v, src); };
       b = b0 + src;
-      seq_at += __builtin_amdgcn_readlane(incl, src) - __builtin_amdgcn_readlane((int)c, src);
-      seq_blocks += __builtin_amdgcn_readlane(blocks, src) - __builtin_amdgcn_readlane((int)nb, src);
+      seq_at += from((int32_t)(c_to - c));
+      seq_blocks += from((int32_t)(nb_to - nb));
+      seq = {from(lane_seq.start), from(lane_seq.n),      from(lane_seq.ctx),
+             from(lane_seq.kv_lim), from(lane_seq.blocks), from(lane_seq.steps)};
       break;
     }
     seq_at += sum64;
-    seq_blocks += __builtin_amdgcn_readlane(blocks, 63);
+    seq_blocks += __builtin_amdgcn_readlane((int)nb_to, 63);
   }
 
   // Block by block of this workgroup's run.
-  Seq seq = sequence<QN>(p, starts, ctxs, b);
   for (;;) {
     int32_t block, block_at, w0, w1;
     do {
@@ -460,33 +465,37 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
     h8_t qf[QB][KK];
     f32x4_t kstart[QB][NG];
     int32_t row_pos[QB];
+    // Q as the B operand: column r = row, k-group g; dims of product kk as the K
+    // operand holds them (pages: 16 g + 8 (kk % 2) of scale group kk / 2, in
+    // nibble-unpack order; fp16: 32 kk + 8 g). Loaded ahead of the first pages,
+    // used behind their copies.
     auto load_q = [&]() __attribute__((always_inline)) {
-      // Q as the B operand: column r = row, k-group g; dims of product kk as the K
-      // operand holds them (pages: 16 g + 8 (kk % 2) of scale group kk / 2, in
-      // nibble-unpack order; fp16: 32 kk + 8 g).
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
         const int32_t row = row0 + 16 * qb + r, tok = p.by_g(row);
         row_pos[qb] = pos0 + tok;
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          h8_t x = {};
-          if (row < rows) {
-            const int d0 = PAGES ? 64 * (kk >> 1) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g;
-            const h8_t y = __builtin_bit_cast(
-                h8_t, *reinterpret_cast<const u32x4_t *>(p.q + (int64_t)(seq.start + tok) * p.q_ts +
-                                                         (int64_t)(kvh * p.G + row - tok * p.G) * p.q_hs + d0));
-            if (PAGES) {
-              x[0] = y[0]; x[1] = y[4]; x[2] = y[1]; x[3] = y[5];
-              x[4] = y[2]; x[5] = y[6]; x[6] = y[3]; x[7] = y[7];
-            } else {
-              x = y;
-            }
-          }
-          qf[qb][kk] = x;
+        for (int kk = 0; kk < KK; ++kk) qf[qb][kk] = (h8_t){};
+        if (row < rows) {
+          const half_t *src = p.q + (int64_t)(seq.start + tok) * p.q_ts +
+                              (int64_t)(kvh * p.G + row - tok * p.G) * p.q_hs + (PAGES ? 16 * g : 8 * g);
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk)
+            qf[qb][kk] = __builtin_bit_cast(
+                h8_t, *reinterpret_cast<const u32x4_t *>(src + (PAGES ? 64 * (kk >> 1) + 8 * (kk & 1) : 32 * kk)));
         }
       }
-
+    };
+    auto prepare_q = [&]() __attribute__((always_inline)) {
+      if constexpr (PAGES) {
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) {
+            const h8_t y = qf[qb][kk];
+            qf[qb][kk] = h8_t{y[0], y[4], y[1], y[5], y[2], y[6], y[3], y[7]};
+          }
+      }
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
@@ -689,11 +698,12 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
     // Wave w takes steps begin + w, begin + w + NW, ...
     if constexpr (PAGES) {
       constexpr int CPS = 2 * ((BLK + 1023) / 1024);  // copies per step
+      load_q();
       look_up(0);
 #pragma unroll
       for (int k = 0; k < NS; ++k)
         if (k < mine) copy_step(k, k);
-      load_q();  // (behind the first copies, which take longer)
+      prepare_q();
       int stage = 0;
 #pragma unroll 1
       for (int32_t j = 0; j < mine; ++j) {
@@ -712,12 +722,13 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
       }
       __syncthreads();  // every wave has read its ring: the sums take its place
     } else {
+      load_q();
       look_up(0);
       if (0 < mine) {
         load_k(0);
         load_v(0);
       }
-      load_q();
+      prepare_q();
 #pragma unroll 1
       for (int32_t j = 0; j < mine; ++j) {
         if (j + 1 - at0 >= 32) look_up(j);
