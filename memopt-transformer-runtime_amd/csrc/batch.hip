@@ -21,7 +21,7 @@
 // two block-wide scans, the ring's pages, then the slots from LDS. 8 requests:
 // 3.1 us (256 threads); 512: 6.4 (1024 threads); 260 with 48000 new rows: 6.4
 // and 2.2 for the rows, whose launch of their own spreads them over the GPU.
-#include "common.hpp"
+#include "packed.hpp"
 
 namespace memopt {
 
@@ -53,11 +53,7 @@ __device__ __forceinline__ Sums sat_add(Sums x, Sums y) {
 template <int NT>
 __device__ __forceinline__ Sums block_scan(Sums v, Sums *s_part, Sums &total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const Sums u = {(uint32_t)__shfl_up((int)v.a, off, 64), (uint32_t)__shfl_up((int)v.b, off, 64)};
-    if (lane >= off) v = sat_add(v, u);
-  }
+  v = {wave_scan(v.a), wave_scan(v.b)};
   __syncthreads();  // s_part is free
   if (lane == 63) s_part[wave] = v;
   __syncthreads();
@@ -85,11 +81,12 @@ __device__ __forceinline__ int32_t owner_of(const int32_t *start, int32_t n, int
 // Slot and position of row t (-1 behind the last row). A page whose slots pass
 // 32 bits gives -1 too: the writers skip it, where a wrapped slot would be
 // somebody else's.
-__device__ __forceinline__ void place_row(const AdvanceParams &p, const int32_t *s_cu, int32_t rows, int32_t t) {
+template <class Ctx>
+__device__ __forceinline__ void place_row(const AdvanceParams &p, const int32_t *s_cu, Ctx ctx, int32_t rows, int32_t t) {
   int32_t slot = -1, pos = -1;
   if (t < rows) {
     const int32_t b = owner_of(s_cu, p.B, t);
-    pos = p.ctx_out[b] - (s_cu[b + 1] - t);
+    pos = ctx(b) - (s_cu[b + 1] - t);
     const int64_t x = (int64_t)p.tables[(int64_t)b * p.M + pos / p.bs] * p.bs + pos % p.bs;
     slot = x >= 0 && x <= INT32_MAX ? (int32_t)x : -1;
   }
@@ -99,7 +96,8 @@ __device__ __forceinline__ void place_row(const AdvanceParams &p, const int32_t 
 
 template <int NT>
 __global__ __launch_bounds__(NT) void advance_kernel(const AdvanceParams p, const int fill) {
-  __shared__ int32_t s_cu[kMaxRequests + 1], s_first[kMaxRequests + 1];  // first row, first page of each request
+  // First row, first page and new context of each request.
+  __shared__ int32_t s_cu[kMaxRequests + 1], s_first[kMaxRequests + 1], s_ctx[kMaxRequests];
   __shared__ Sums s_part[NT / 64];
   const int tid = threadIdx.x;
   int32_t head = p.span[0] % p.C;
@@ -140,7 +138,7 @@ __global__ __launch_bounds__(NT) void advance_kernel(const AdvanceParams p, cons
       s_cu[b] = (int32_t)got.b - n;
       s_first[b] = (int32_t)got.a - need;
       p.cu[b + 1] = (int32_t)got.b;
-      p.ctx_out[b] = c + n;
+      s_ctx[b] = p.ctx_out[b] = c + n;
       p.status[b] = st;
     }
   }
@@ -154,17 +152,16 @@ __global__ __launch_bounds__(NT) void advance_kernel(const AdvanceParams p, cons
   }
   __syncthreads();
   // Pages: the j-th of the step belongs to the request whose range holds j,
-  // behind the pages its old context has. (ctx_out is what this workgroup
-  // wrote above: new context, rows in s_cu.)
+  // behind the pages its old context has.
   for (int32_t j = tid; j < pages; j += NT) {
     const int32_t b = owner_of(s_first, p.B, j);
-    const int32_t c = p.ctx_out[b] - (s_cu[b + 1] - s_cu[b]);
+    const int32_t c = s_ctx[b] - (s_cu[b + 1] - s_cu[b]);
     const int32_t have = (int32_t)(((int64_t)c + p.bs - 1) / p.bs);
     p.tables[(int64_t)b * p.M + have + j - s_first[b]] = p.ring[(int32_t)(((int64_t)head + j) % p.C)];
   }
   if (!fill) return;
   __syncthreads();
-  for (int32_t t = tid; t < p.rows; t += NT) place_row(p, s_cu, rows, t);
+  for (int32_t t = tid; t < p.rows; t += NT) place_row(p, s_cu, [&](int32_t b) { return s_ctx[b]; }, rows, t);
 }
 
 // Slots and positions from the step's query starts, context lengths and tables.
@@ -174,7 +171,7 @@ __global__ __launch_bounds__(256) void advance_rows_kernel(const AdvanceParams p
   __syncthreads();
   const int32_t rows = s_cu[p.B];
   for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < p.rows; t += (int64_t)gridDim.x * 256)
-    place_row(p, s_cu, rows, (int32_t)t);
+    place_row(p, s_cu, [&](int32_t b) { return p.ctx_out[b]; }, rows, (int32_t)t);
 }
 
 }  // namespace memopt

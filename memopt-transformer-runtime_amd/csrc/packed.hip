@@ -85,21 +85,6 @@ struct PackedParams {
 // Workgroups per key head, so partial sums of a block, at most.
 static constexpr int kMaxParts = 256;
 
-// Inclusive prefix sum over the wave (DPP row shifts, then row broadcasts),
-// saturating: query starts that do not ascend can count rows more than once.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t scan_step(uint32_t v) {
-  return __builtin_elementwise_add_sat(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, ROWS == 0xF));
-}
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-  v = scan_step<0x111, 0xF>(v);
-  v = scan_step<0x112, 0xF>(v);
-  v = scan_step<0x114, 0xF>(v);
-  v = scan_step<0x118, 0xF>(v);
-  v = scan_step<0x142, 0xA>(v);
-  return scan_step<0x143, 0xC>(v);
-}
-
 // What rows at positions pos_lo .. pos_hi of a context see, in 16-token
 // chunks: the sinks [0, sc), then the window [wc0, wc0 + n - sc).
 struct Visible {

@@ -21,6 +21,22 @@ struct Divisor {
   }
 };
 
+// Inclusive prefix sum over the wave (DPP row shifts, then row broadcasts),
+// saturating: neither query starts that do not ascend nor counts that a user
+// asks for can wrap it.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t scan_step(uint32_t v) {
+  return __builtin_elementwise_add_sat(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, ROWS == 0xF));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v = scan_step<0x111, 0xF>(v);
+  v = scan_step<0x112, 0xF>(v);
+  v = scan_step<0x114, 0xF>(v);
+  v = scan_step<0x118, 0xF>(v);
+  v = scan_step<0x142, 0xA>(v);
+  return scan_step<0x143, 0xC>(v);
+}
+
 // Rows of sequence b: G query heads per key head make each token G rows.
 struct Rows {
   int32_t start, n;  // first token row, tokens
