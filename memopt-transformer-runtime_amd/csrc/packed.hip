@@ -19,7 +19,7 @@
 // prompt.hip): a block of 32 rows unpacks each page once more, and from 512
 // rows on that costs more than writing the copy. What follows is the rest.
 //
-// Work: QN = 16 * QB rows of one (sequence, key head) are a block; a wave takes
+// Work: QN = 8, 16 or 32 rows of one (sequence, key head) are a block; a wave takes
 // two 16-token chunks (32 tokens) of a block's visible ones per step. The steps
 // of all blocks of a key head form one list, which is dealt to its workgroups
 // of 4 waves in runs that are equal but for a few steps around block ends,
@@ -39,15 +39,16 @@
 //    operands.
 //  * V enters as exact codes, too: the products of a scale group take the
 //    weights times that group's scale per token. So a page's only rounding to
-//    16 bits is that of weight times scale.
+//    16 bits is that of weight times scale, and up to 16 rows what that loses
+//    is a second operand (HALVES, REST).
 //
 // Bound by the stream of pages and 7 us around it: a copy of the kernel without
-// its arithmetic takes 41.5 us where it takes 46.7 (32 sequences of 2700 to 8192
-// tokens, 32 query over 8 key heads: 4.2 TB/s of pages), one without the copies
-// 37; one sequence of 131072 tokens 30 and 29 of 34.5 (4.1 TB/s). A large copy
-// reaches 5.1 on the card. One sequence of 1024: 8.6 us, a chain of the list of
-// sequences (1.0), queries (0.8), two steps (1.8), the waves' merge (0.7), the
-// arrival (0.6) and the workgroups' merge (2.5).
+// its arithmetic took 41.5 us where it took 46.7 (32 sequences of 2700 to 8192
+// tokens, 32 query over 8 key heads; 44.6 now, 4.4 TB/s of pages), one without
+// the copies 37; one sequence of 131072 tokens 30 and 29 of 34.5 (34.2 now, 4.2
+// TB/s). A large copy reaches 5.1 on the card. One sequence of 1024: 6.8 us, a
+// chain of the list of sequences, the table, two steps, the waves' merge, the
+// arrival and the workgroups' merge.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -181,15 +182,23 @@ __device__ __forceinline__ T lds_at(uint32_t a) {
 }
 
 // Workgroups per CU that the kernels' registers and LDS are meant for.
-__host__ __device__ static constexpr int resident(int NW, int QB) { return QB == 2 ? 2 : NW == 4 ? 3 : 1; }
+__host__ __device__ static constexpr int resident(int NW, int QN) { return QN == 32 ? 2 : NW == 4 ? 3 : 1; }
 
-template <int D, int FMT, int QB, int NW>
-__global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_kernel(
+template <int D, int FMT, int QN, int NW>
+__global__ __launch_bounds__(64 * NW, NW * resident(NW, QN) / 4) void packed_kernel(
     const PackedParams p, const int32_t *__restrict__ starts, const int32_t *__restrict__ ctxs,
     const int32_t *__restrict__ tables) {
-  constexpr int NT = 64 * NW, KK = D / 32, ND = D / 16, QN = 16 * QB;
+  constexpr int NT = 64 * NW, KK = D / 32, ND = D / 16, QB = QN == 32 ? 2 : 1;
   constexpr bool PAGES = FMT == MEMOPT_KV_INT4;
   constexpr int NG = PAGES ? D / 64 : 1;  // score sums per (row, token)
+  // Decode over pages: a weight enters the second product as the sum of two
+  // 16-bit operands, itself and what its rounding lost. One rounding of a weight
+  // that makes up much of a row is an error of that whole row: up to 4.8e-4 of
+  // the output's norm, where two operands leave the output's own 2e-4. Up to 8
+  // rows, the rest takes the other 8 columns of the same instructions (HALVES:
+  // columns n and n + 8 are the same row); up to 16 an instruction of its own.
+  // (131072 tokens, 5 rows: 33.1 us without, 37.7 as instructions of its own.)
+  constexpr bool HALVES = QN == 8, REST = PAGES && QN == 16;
   constexpr int OS = D + 4;               // row stride of s_o: 16 rows of D floats would share a bank
   // Pages stream through a ring of raw blocks per wave (see copy_step), which
   // the merge of the waves takes over when the steps are done.
@@ -447,6 +456,7 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
       return u32x4_t{(w & m_lo) | e1024, (w & m_hi) | e64, (w8 & m_lo) | e1024, (w8 & m_hi) | e64};
     };
     const half2_t ones = {(half_t)1.0f, (half_t)1.0f};
+    const uint32_t second_half = r < 8 ? 0u : ~0u;
     h8_t qf[QB][KK];
     f32x4_t kstart[QB][NG];
     int32_t row_pos[QB];
@@ -457,7 +467,7 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
     auto load_q = [&]() __attribute__((always_inline)) {
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
-        const int32_t row = row0 + 16 * qb + r, tok = p.by_g(row);
+        const int32_t row = row0 + 16 * qb + (HALVES ? r & 7 : r), tok = p.by_g(row);
         row_pos[qb] = pos0 + tok;
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) qf[qb][kk] = (h8_t){};
@@ -547,7 +557,7 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
       const int32_t key0 = 16 * logical(2 * step_at(j) + (g >> 1)) + 4 * (g & 1);
       between();
 
-      h8_t pf[QB][NG];
+      h8_t pf[QB][NG], pf_rest[QB][NG];
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
         u32x4_t vs[NG];
@@ -615,7 +625,23 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
             for (int i = 0; i < 4; ++i)  // (one mixed-precision instruction for each half)
               w[i] = as_u32(half2_t{(half_t)fmaf(x[qb][2 * i], (float)as_half2(vs[u][i])[0], 0.0f),
                                     (half_t)fmaf(x[qb][2 * i + 1], (float)as_half2(vs[u][i])[1], 0.0f)});
+            if constexpr (HALVES) {  // lanes n >= 8: what the rounding of their twin lost
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const half2_t twin = as_half2(w[i] & second_half);
+                w[i] = as_u32(half2_t{(half_t)fmaf(x[qb][2 * i], (float)as_half2(vs[u][i])[0], -(float)twin[0]),
+                                      (half_t)fmaf(x[qb][2 * i + 1], (float)as_half2(vs[u][i])[1], -(float)twin[1])});
+              }
+            }
             pf[qb][u] = __builtin_bit_cast(h8_t, w);
+            if constexpr (REST) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                w[i] = as_u32(half2_t{
+                    (half_t)fmaf(x[qb][2 * i], (float)as_half2(vs[u][i])[0], -(float)pf[qb][u][2 * i]),
+                    (half_t)fmaf(x[qb][2 * i + 1], (float)as_half2(vs[u][i])[1], -(float)pf[qb][u][2 * i + 1])});
+              pf_rest[qb][u] = __builtin_bit_cast(h8_t, w);
+            }
           }
         } else {
 #pragma unroll
@@ -655,9 +681,12 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
       }
       auto pv = [&](int i, u32x4_t a) __attribute__((always_inline)) {
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb)
-          o[qb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), pf[qb][i / (ND / NG)], o[qb][i],
-                                                            0, 0, 0);
+        for (int qb = 0; qb < QB; ++qb) {
+          const h8_t v = __builtin_bit_cast(h8_t, a);
+          o[qb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf[qb][i / (ND / NG)], o[qb][i], 0, 0, 0);
+          if constexpr (REST)
+            o[qb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf_rest[qb][i / (ND / NG)], o[qb][i], 0, 0, 0);
+        }
       };
       if constexpr (PAGES) {
 #pragma unroll
@@ -704,6 +733,15 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
           if (j + NS < mine) copy_step(j + NS, stage);
         });
         stage ^= 1;
+      }
+      if constexpr (HALVES) {  // both columns of a row
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+#pragma unroll
+          for (int reg = 0; reg < 4; ++reg) {
+            const uint32_t v = __float_as_uint(o[0][i][reg]);
+            o[0][i][reg] += __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xF, 0xF, true));
+          }
       }
       __syncthreads();  // every wave has read its ring: the sums take its place
     } else {
@@ -757,7 +795,7 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QB) / 4) void packed_ker
     for (int qb = 0; qb < QB; ++qb) {
       const float l = xor32_sum(xor16_sum(lsum[qb]));
       const int row = 16 * qb + r;
-      if (row0 + row >= rows) continue;
+      if (row0 + row >= rows || (HALVES && r >= 8)) continue;
 #pragma unroll
       for (int reg = 0; reg < 4; ++reg)
 #pragma unroll
@@ -1072,7 +1110,7 @@ static constexpr int64_t kStagedBytes = 2LL << 30;
 static PackedPlan packed_plan(const memopt_packed_desc &d) {
   PackedPlan pl = {};
   const int64_t G = d.num_heads / d.num_kv_heads, most = (int64_t)std::min(d.max_query_len, d.tokens) * G;
-  pl.qn = most <= 16 ? 16 : 32;
+  pl.qn = most > 16 ? 32 : most > 8 || d.kv_format == MEMOPT_KV_FP16 ? 16 : 8;
   // sum over the sequences of ceil(rows / qn)
   pl.blocks = (d.tokens * G + (int64_t)(pl.qn - 1) * std::min(d.batch, d.tokens)) / pl.qn;
   // Workgroups of 4 waves, three to a CU: they hide each other's starts and
@@ -1083,11 +1121,11 @@ static PackedPlan packed_plan(const memopt_packed_desc &d) {
   // 8192: 47.9 with 4 waves, 51.9 with 12; one of 1024: 8.7 and 11.6). fp16
   // rows take their registers from the ring's share: 8 waves, one workgroup.
   auto wgs = [&](int waves) {
-    const int64_t n = (int64_t)resident(waves, pl.qn / 16) * compute_units() / d.num_kv_heads;
+    const int64_t n = (int64_t)resident(waves, pl.qn) * compute_units() / d.num_kv_heads;
     return (int32_t)std::max<int64_t>(1, std::min<int64_t>(n, kMaxParts));
   };
   pl.waves = pl.qn == 32 ? 4 : d.kv_format == MEMOPT_KV_FP16 ? 8 : 4;
-  if (pl.waves == 4 && pl.qn == 16 && std::min<int64_t>(wgs(4), packed_steps(d) * d.batch / 4) > 24LL * d.batch)
+  if (pl.waves == 4 && pl.qn <= 16 && std::min<int64_t>(wgs(4), packed_steps(d) * d.batch / 4) > 24LL * d.batch)
     pl.waves = 12;
   pl.wgs = wgs(pl.waves);
   pl.min_rows = kStagedRows;
@@ -1149,20 +1187,22 @@ static int validate_packed(const memopt_packed_desc &d) {
   return MEMOPT_OK;
 }
 
-template <int D, int FMT, int QB, int NW>
+template <int D, int FMT, int QN, int NW>
 static void launch_packed(const PackedParams &p, const memopt_packed_desc &d, hipStream_t stream) {
-  hipLaunchKernelGGL((packed_kernel<D, FMT, QB, NW>), dim3((unsigned)((int64_t)p.wgs * p.Hk)), dim3(64 * NW), 0, stream,
+  hipLaunchKernelGGL((packed_kernel<D, FMT, QN, NW>), dim3((unsigned)((int64_t)p.wgs * p.Hk)), dim3(64 * NW), 0, stream,
                      p, d.query_starts, d.context_lens, d.block_tables);
 }
 template <int D>
 static void launch_packed(const PackedParams &p, const memopt_packed_desc &d, const PackedPlan &pl, hipStream_t s) {
   if (d.kv_format == MEMOPT_KV_INT4) {
-    if (pl.qn == 32) launch_packed<D, MEMOPT_KV_INT4, 2, 4>(p, d, s);
-    else if (pl.waves == 12) launch_packed<D, MEMOPT_KV_INT4, 1, 12>(p, d, s);
-    else launch_packed<D, MEMOPT_KV_INT4, 1, 4>(p, d, s);
+    if (pl.qn == 32) launch_packed<D, MEMOPT_KV_INT4, 32, 4>(p, d, s);
+    else if (pl.qn == 16 && pl.waves == 12) launch_packed<D, MEMOPT_KV_INT4, 16, 12>(p, d, s);
+    else if (pl.qn == 16) launch_packed<D, MEMOPT_KV_INT4, 16, 4>(p, d, s);
+    else if (pl.waves == 12) launch_packed<D, MEMOPT_KV_INT4, 8, 12>(p, d, s);
+    else launch_packed<D, MEMOPT_KV_INT4, 8, 4>(p, d, s);
   } else {
-    if (pl.qn == 32) launch_packed<D, MEMOPT_KV_FP16, 2, 4>(p, d, s);
-    else launch_packed<D, MEMOPT_KV_FP16, 1, 8>(p, d, s);
+    if (pl.qn == 32) launch_packed<D, MEMOPT_KV_FP16, 32, 4>(p, d, s);
+    else launch_packed<D, MEMOPT_KV_FP16, 16, 8>(p, d, s);
   }
 }
 

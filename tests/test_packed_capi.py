@@ -97,10 +97,11 @@ def test_packed_workspace(C):
 
     need, zeroed = size()
     assert zeroed == 256  # 8 sequences x 2 key heads x 4 bytes, rounded up
-    partials = 256 * 2 * 2 * 16 * (64 + 2) * 4  # kMaxParts workgroups, two blocks of 16 rows each, 2 key heads
+    partials = 256 * 2 * 2 * 8 * (64 + 2) * 4  # kMaxParts workgroups, two blocks of 8 rows each, 2 key heads
     assert need - zeroed == partials
-    # 33 rows of 4 heads per sequence: blocks of 32 rows, two workgroups to a CU
-    assert size(max_query_len=8, tokens=64)[0] - size(max_query_len=8, tokens=64)[1] == 2 * partials
+    # 32 rows (8 tokens x 4 heads) per sequence: blocks of 32 rows; 16 rows: of 16
+    assert size(max_query_len=8, tokens=64)[0] - size(max_query_len=8, tokens=64)[1] == 4 * partials
+    assert size(max_query_len=4, tokens=32)[0] - size(max_query_len=4, tokens=32)[1] == 2 * partials
     # chunks of 512 rows (128 tokens), 8 query heads: staged from 128 x 256 / 8 tokens on
     chunks = dict(max_query_len=512, max_seq_len=4096, max_blocks_per_seq=256)
     small, full = size(tokens=4095, **chunks)[0], size(tokens=4096, **chunks)[0]
