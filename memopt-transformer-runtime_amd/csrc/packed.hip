@@ -1114,18 +1114,19 @@ static PackedPlan packed_plan(const memopt_packed_desc &d) {
   // sum over the sequences of ceil(rows / qn)
   pl.blocks = (d.tokens * G + (int64_t)(pl.qn - 1) * std::min(d.batch, d.tokens)) / pl.qn;
   // Workgroups of 4 waves, three to a CU: they hide each other's starts and
-  // ends. Where a sequence would fall to more than 24 of them, its last
-  // workgroup adds up as many partial sums one round trip after another: there
-  // 12 waves in one workgroup per CU leave a third as many (one sequence of
-  // 131072 tokens x 8 key heads: 42.0 us, now 35.4; 32 sequences of 2700 to
-  // 8192: 47.9 with 4 waves, 51.9 with 12; one of 1024: 8.7 and 11.6). fp16
-  // rows take their registers from the ring's share: 8 waves, one workgroup.
+  // ends. Where a sequence falls to more than 8 of them and there is enough to
+  // read, 12 waves in one workgroup per CU, a third as many partial sums, are
+  // faster (us with 4 and 12 waves, 32 query over 8 key heads of 128: one sequence
+  // of 131072 tokens 40.0 and 35.1, one of 8000 17.6 and 15.3, 4 of 8000 20.8 and
+  // 15.1, 8 of 16000 35.3 and 32.5; but one of 4000 12.6 and 14.1, 4 of 1000 9.5
+  // and 12.4, 32 of 2700 to 8192 43.3 and 46.0). fp16 rows take their registers
+  // from the ring's share: 8 waves, one workgroup.
   auto wgs = [&](int waves) {
     const int64_t n = (int64_t)resident(waves, pl.qn) * compute_units() / d.num_kv_heads;
     return (int32_t)std::max<int64_t>(1, std::min<int64_t>(n, kMaxParts));
   };
   pl.waves = pl.qn == 32 ? 4 : d.kv_format == MEMOPT_KV_FP16 ? 8 : 4;
-  if (pl.waves == 4 && pl.qn <= 16 && std::min<int64_t>(wgs(4), packed_steps(d) * d.batch / 4) > 24LL * d.batch)
+  if (pl.waves == 4 && pl.qn <= 16 && wgs(4) > 8LL * d.batch && packed_steps(d) * d.batch * d.head_dim >= 32000)
     pl.waves = 12;
   pl.wgs = wgs(pl.waves);
   pl.min_rows = kStagedRows;
