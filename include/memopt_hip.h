@@ -343,7 +343,7 @@ int memopt_prompt_attention(const memopt_prompt_desc *desc, void *stream);
  * contiguous MEMOPT_KV_FP16 pools with block_size a multiple of 16, both with
  * num_kv_heads heads; head_dim 64 or 128; INT4 values are (code - 8) * scale.
  * max_query_len bounds the rows of any one sequence (rows past it may be left
- * unwritten). */
+ * unwritten). Block tables hold up to 2^30 tokens. */
 typedef struct memopt_packed_desc {
   const void *query;                 /* fp16 [tokens, num_heads, head_dim]     */
   void *out;                         /* fp16 [tokens, num_heads, head_dim]     */

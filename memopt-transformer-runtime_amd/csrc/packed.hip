@@ -1240,8 +1240,8 @@ extern "C" int memopt_packed_attention(const memopt_packed_desc *desc, void *str
   MEMOPT_REQUIRE(d.query && d.out && d.key_cache && (d.value_cache || d.kv_format == MEMOPT_KV_INT4) &&
                      d.block_tables && d.context_lens && d.query_starts,
                  MEMOPT_ERR_INVALID, "packed_attention: null pointer");
-  MEMOPT_REQUIRE((int64_t)d.max_blocks_per_seq * d.block_size <= INT32_MAX - 127, MEMOPT_ERR_UNSUPPORTED,
-                 "packed_attention: positions must fit 32 bits");
+  MEMOPT_REQUIRE((int64_t)d.max_blocks_per_seq * d.block_size <= 1 << 30, MEMOPT_ERR_UNSUPPORTED,
+                 "packed_attention: positions less a window must fit 32 bits: block tables of up to 2^30 tokens");
   const PackedPlan pl = packed_plan(d);
   const PackedWorkspace w = packed_workspace(d, pl);
   MEMOPT_REQUIRE(d.workspace && d.workspace_bytes >= w.total, MEMOPT_ERR_INVALID,

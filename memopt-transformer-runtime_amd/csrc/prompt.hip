@@ -822,7 +822,7 @@ extern "C" int memopt_prompt_attention(const memopt_prompt_desc *desc, void *str
   p.W = d.window_size <= 0 ? 1 << 30 : std::min(d.window_size, 1 << 30);  // (position - W stays in 32 bits)
   p.sinks = std::max(0, d.num_sink_tokens);
   p.qk_scale_log2 = 1.4426950408889634f / sqrtf((float)d.head_dim);
-  MEMOPT_REQUIRE((int64_t)d.tokens * d.num_heads <= INT32_MAX - 255 &&
+  MEMOPT_REQUIRE(d.tokens <= 1 << 30 && (int64_t)d.tokens * d.num_heads <= INT32_MAX - 255 &&
                      most_tiles(d.tokens, d.batch, p.G) * d.num_kv_heads < (1LL << 31),
                  MEMOPT_ERR_UNSUPPORTED, "prompt_attention: too many query rows");
   hipStream_t s = (hipStream_t)stream;

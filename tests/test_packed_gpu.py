@@ -367,6 +367,23 @@ def test_long_chunks_evicted_rows_and_extreme_scales(D):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("Hq,qn", [(4, [1, 2]), (64, [520, 3])], ids=["decode", "long chunk"])
+def test_pages_past_4_gib(fmt, Hq, qn):
+    """Byte offsets past 32 bits: the same pages at the end of a pool of more than 4 GiB."""
+    c = Case(fmt, [600, 77], qn, Hq, 1, 128, seed=6)
+    want = memopt_C.packed_attention(*c.args())
+    nb = c.kc.shape[0]
+    first = 2 ** 32 // (2176 if fmt == "int4" else 4096) + 5
+    pools = []
+    for x in ([c.kc] if fmt == "int4" else [c.kc, c.vc]):
+        pools.append(torch.empty((first + nb, *x.shape[1:]), dtype=x.dtype, device=dev()))
+        pools[-1][first:] = x
+    c.kc, c.vc = pools[0], pools[-1]
+    c.bt = torch.where(c.bt >= 0, c.bt + first, c.bt)
+    assert torch.equal(memopt_C.packed_attention(*c.args()), want)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_strides_padding_and_out(fmt):
     c = Case(fmt, [60, 200], [4, 30], 6, 2, 64, seed=2)
     want = memopt_C.packed_attention(*c.args())
