@@ -105,7 +105,7 @@ __global__ __launch_bounds__(NT) void advance_kernel(const AdvanceParams p, cons
   const int32_t count = min(max(p.span[1], 0), p.C);
   const int64_t most = (int64_t)p.M * p.bs;
 
-  Sums asked = {0, 0}, served = {0, 0};  // pages, rows of the requests before this round's
+  Sums asked = {0, 0}, served = {0, 0};  // pages, rows of the requests already looked at
   for (int32_t b0 = 0; b0 < p.B; b0 += NT) {
     const int32_t b = b0 + tid;
     int32_t c = 0, n = 0, st = 0, have = 0, need = 0;

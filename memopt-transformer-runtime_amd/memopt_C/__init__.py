@@ -781,11 +781,12 @@ class PreparedAttention:
 # when they raise.)
 def _device_tensors(fn: str, device: torch.device, names: Tuple[str, ...], *tensors) -> None:
     """Raises for the first of ``tensors`` that is not a CUDA tensor on ``device`` (one of CUDA)."""
-    for i, t in enumerate(tensors):
+    for t in tensors:
         if not (isinstance(t, torch.Tensor) and t.device == device):
+            name = next(n for n, x in zip(names, tensors) if x is t)
             if not (isinstance(t, torch.Tensor) and t.is_cuda):
-                raise RuntimeError(f"{fn}: {names[i]} must be a CUDA tensor")
-            raise RuntimeError(f"{fn}: {names[i]} on a different device")
+                raise RuntimeError(f"{fn}: {name} must be a CUDA tensor")
+            raise RuntimeError(f"{fn}: {name} on a different device")
 
 
 def _int32(fn: str, t: torch.Tensor, name: str, shape: Tuple[int, ...]) -> None:
@@ -839,7 +840,7 @@ _c_prompt_bytes.restype = _i32
 
 def _count32(n: int) -> int:
     """``n`` as an int32, where any negative number means the same and any past 2^31 - 1 as that."""
-    return min(max(int(n), -1), 2 ** 31 - 1)
+    return n if n.__class__ is int and -1 <= n < 2 ** 31 else min(max(int(n), -1), 2 ** 31 - 1)
 
 
 def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -861,10 +862,15 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     fn = "prompt_attention"
     if not (isinstance(query, torch.Tensor) and query.is_cuda):
         raise RuntimeError(f"{fn}: query must be a CUDA tensor")
-    device, dtype, shape = query.device, query.dtype, query.shape
+    device, dtype = query.device, query.dtype
+    index = device.index
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(device):
+            return prompt_attention(query, keys, values, cu_seqlens, window_size, num_sink_tokens=num_sink_tokens,
+                                    out=out)
     _device_tensors(fn, device, ("keys", "values", "cu_seqlens"), keys, values, cu_seqlens)
     _no_grad(fn, query.requires_grad or keys.requires_grad or values.requires_grad)
-    kshape = keys.shape
+    shape, kshape, cshape = query.shape, keys.shape, cu_seqlens.shape
     if not (len(shape) == 3 and len(kshape) == 3 and values.dim() == 3):
         raise RuntimeError(f"{fn}: query, keys and values must be 3-D [tokens, heads, head_dim]")
     T, Hq, D = shape
@@ -876,22 +882,20 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     if not (kshape == (T, Hk, D) and values.shape == kshape):
         raise RuntimeError(f"{fn}: keys and values must be [{T}, kv heads, {D}], got {list(kshape)} and "
                            f"{list(values.shape)}")
-    cshape = cu_seqlens.shape
     if len(cshape) != 1 or cshape[0] < 1:
         raise RuntimeError(f"{fn}: cu_seqlens must be 1-D [batch + 1]")
     _int32(fn, cu_seqlens, "cu_seqlens", cshape)
-    with _on(device):
-        out, po, ots, ohs = _out_rows(fn, out, query)
-        q, pq, qts, qhs = _rows(query)
-        k, pk, kts, khs = _rows(keys)
-        v, pv, vts, vhs = _rows(values)
-        try:
-            d = _PROMPT.pack(pq, pk, pv, po, 1 if dtype is torch.bfloat16 else 0, T, cshape[0] - 1, Hq, Hk, D, qts, qhs,
-                             kts, khs, vts, vhs, ots, ohs, cu_seqlens.data_ptr(), _count32(window_size),
-                             _count32(num_sink_tokens))
-        except struct.error:
-            raise RuntimeError(f"{fn}: sizes must fit 32 bits") from None
-        _check(_c_prompt_bytes(d, torch._C._cuda_getCurrentRawStream(device.index)))
+    out, po, ots, ohs = _out_rows(fn, out, query)
+    q, pq, qts, qhs = _rows(query)
+    k, pk, kts, khs = _rows(keys)
+    v, pv, vts, vhs = _rows(values)
+    try:
+        d = _PROMPT.pack(pq, pk, pv, po, 1 if dtype is torch.bfloat16 else 0, T, cshape[0] - 1, Hq, Hk, D, qts, qhs, kts,
+                         khs, vts, vhs, ots, ohs, cu_seqlens.data_ptr(), _count32(window_size),
+                         _count32(num_sink_tokens))
+    except struct.error:
+        raise RuntimeError(f"{fn}: sizes must fit 32 bits") from None
+    _check(_c_prompt_bytes(d, torch._C._cuda_getCurrentRawStream(index)))
     return out
 
 
@@ -1062,6 +1066,11 @@ def advance_batch(new_tokens: torch.Tensor, context_lens: torch.Tensor, block_ta
     if not (isinstance(new_tokens, torch.Tensor) and new_tokens.is_cuda):
         raise RuntimeError(f"{fn}: new_tokens must be a CUDA tensor")
     device = new_tokens.device
+    index = device.index
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(device):
+            return advance_batch(new_tokens, context_lens, block_tables, free_pages, free_span, block_size, num_rows,
+                                 out=out)
     _device_tensors(fn, device, ("context_lens", "block_tables", "free_pages", "free_span"), context_lens, block_tables,
                     free_pages, free_span)
     nshape, tshape, fshape = new_tokens.shape, block_tables.shape, free_pages.shape
@@ -1084,8 +1093,7 @@ def advance_batch(new_tokens: torch.Tensor, context_lens: torch.Tensor, block_ta
         raise RuntimeError(f"{fn}: num_rows differs from out's rows")
     if out.device != device or out.context_lens.shape != nshape:
         raise RuntimeError(f"{fn}: out holds buffers of another device or number of requests")
-    with _on(device):
-        d = _ADVANCE.pack(new_tokens.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), free_pages.data_ptr(),
-                          free_span.data_ptr(), *out._args, B, M, C, block_size, rows)
-        _check(_c_advance(d, torch._C._cuda_getCurrentRawStream(device.index)))
+    d = _ADVANCE.pack(new_tokens.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), free_pages.data_ptr(),
+                      free_span.data_ptr(), *out._args, B, M, C, block_size, rows)
+    _check(_c_advance(d, torch._C._cuda_getCurrentRawStream(index)))
     return out
