@@ -1088,7 +1088,7 @@ static int64_t packed_steps(const memopt_packed_desc &d) {
   return ((int64_t)d.max_blocks_per_seq * d.block_size + 31) / 32;
 }
 
-// Query rows per block: 16 where a sequence has no more than that.
+// Query rows per block: 8 or 16 where no sequence has more.
 struct PackedPlan {
   int32_t qn, waves, wgs;
   int64_t blocks;  // at most this many
@@ -1096,14 +1096,18 @@ struct PackedPlan {
   int64_t cap;
 };
 
-// Rows from which a sequence's chunk attends from a staged copy, and rows of
-// the whole batch and all key heads, as tiles of 128, from which any does: one
-// per CU, since those tiles are not split along the keys (some 17 us for 1024
-// of them) as the blocks here are. 32 query over 8 key heads of 128, us staged
-// and not: 8 chunks of 1024 rows over contexts of 4096 162 and 262; 8 of 512
-// (256 tiles) 110 and 133; 32 of 512 455 and 521; but 32 of 256 314 and 264,
-// one of 1024 (64 tiles) 72 and 53.
-static constexpr int kStagedRows = 512;
+// Rows from which a sequence's chunk attends from a staged copy, by the rows of
+// the whole batch and all key heads as tiles of 128, which are not split along
+// the keys (some 17 us for 1024 of them) as the blocks here are: 512 where there
+// are two tiles for each CU, 1024 where there is one, none below. 32 query over 8
+// key heads of 128, us staged and not: 32 chunks of 512 rows over contexts of 4096
+// 472 and 509, 16 of 512 over 1024 66 and 86; 8 of 1024 over 4096 182 and 263, 2 of
+// 2048 (256 tiles) 111 and 130; but 8 of 512 (256 tiles) over 16384 558 and 475, 32 of
+// 256 over 4096 320 and 258, one of 1024 (64 tiles) 95 and 45.
+static int32_t staged_rows(int64_t rows) {
+  const int64_t per_cu = rows / (128LL * compute_units());
+  return per_cu >= 2 ? 512 : per_cu >= 1 ? 1024 : INT32_MAX;
+}
 // Of staged copies at most this much.
 static constexpr int64_t kStagedBytes = 2LL << 30;
 
@@ -1129,8 +1133,8 @@ static PackedPlan packed_plan(const memopt_packed_desc &d) {
   if (pl.waves == 4 && pl.qn <= 16 && wgs(4) > 8LL * d.batch && packed_steps(d) * d.batch * d.head_dim >= 32000)
     pl.waves = 12;
   pl.wgs = wgs(pl.waves);
-  pl.min_rows = kStagedRows;
-  if (most >= pl.min_rows && (int64_t)d.tokens * d.num_heads >= 128LL * compute_units()) {
+  pl.min_rows = staged_rows((int64_t)d.tokens * d.num_heads);
+  if (most >= pl.min_rows) {
     const int64_t W = std::min(effective_window(d.window_size, d.max_seq_len), 1 << 30);
     const int64_t sinks = std::max(0, d.num_sink_tokens);
     auto up64 = [](int64_t x) { return (x + 63) / 64 * 64; };

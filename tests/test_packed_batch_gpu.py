@@ -118,20 +118,26 @@ def test_pages_that_do_not_last():
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-def test_captured_step(fmt):
-    """advance_batch, write_cache and a plan in one graph, replayed as the requests grow across pages."""
+@pytest.mark.parametrize("planned", [True, False])
+def test_captured_step(fmt, planned):
+    """advance_batch, write_cache and a plan (or the eager call) in one graph, replayed as the requests grow across
+    pages."""
     n, Hq, Hk, D = 5, 8, 2, 64
     batch = R().PackedBatch(60, Hk, D, n, 160, n, kv_format=fmt)
     host = Host(n, Hk, D)
     rng = torch.Generator().manual_seed(1)
     q, k, v = (torch.empty((n, h, D), dtype=torch.float16, device=dev()) for h in (Hq, Hk, Hk))
     new = torch.zeros(n, dtype=torch.int32, device=dev())
-    plan = batch.attend_plan(q, max_new=2)
+    out = torch.empty_like(q)
+    plan = batch.attend_plan(q, max_new=2, out=out)
 
     def work():
         batch.advance(new)
-        memopt_C.write_cache(k, v, None, batch.state.slots, validate_slots=False)
-        plan()
+        if planned:
+            memopt_C.write_cache(k, v, None, batch.state.slots, validate_slots=False)
+            assert plan() is out
+        else:
+            batch.attend(q, k, v, max_new=2, out=out)
 
     work()  # (nothing new: no rows)
     torch.cuda.synchronize()
@@ -153,7 +159,7 @@ def test_captured_step(fmt):
             a, b, first = cu[r], cu[r + 1], len(host.k[r])
             host.extend(r, k[a:b], v[a:b])
             if b > a and i % 6 == 0:
-                compare(plan.out[a:b], q[a:b], host.k[r], host.v[r], first, fmt, -1, 0, f"replay {i} request {r}")
+                compare(out[a:b], q[a:b], host.k[r], host.v[r], first, fmt, -1, 0, f"replay {i} request {r}")
     assert batch.state.context_lens.tolist() == [len(x) for x in host.k]
 
 

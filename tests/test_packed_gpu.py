@@ -10,8 +10,12 @@ from packed_reference import attend, check, quantized_scores, starts, tolerance
 pytestmark = pytest.mark.gpu
 
 FORMATS = ["int4", "fp16"]
-STAGED = 512  # rows (tokens times query heads per key head) from which a chunk attends from a staged copy
-FILL = 128 * 256  # and rows of the whole batch over all key heads: a tile of 128 for each compute unit
+FILL = 128 * 256  # rows of the whole batch over all key heads that give each compute unit a tile of 128
+
+
+def staged_rows(T, Hq):
+    """Rows (tokens times query heads per key head) from which a chunk attends from a staged copy."""
+    return 512 if T * Hq >= 2 * FILL else 1024 if T * Hq >= FILL else 2 ** 31
 
 
 class Case:
@@ -70,7 +74,7 @@ class Case:
             scores, staged, v_scale = 0.0, False, 0.0
             if self.fmt == "int4":
                 G = self.q.shape[1] // self.k.shape[2]
-                staged = n * G >= STAGED and self.q.shape[0] * self.q.shape[1] >= FILL
+                staged = n * G >= staged_rows(*self.q.shape[:2])
                 scores = quantized_scores(self.q[a:a + n][some], float(self.kval.abs().max()) / 7, staged)
                 v_scale = 0.0 if staged else float(self.vval.abs().max()) / 7
             tol = tolerance(o, w, e, m, self.D, torch.float16, torch.float16, staged, scores, v_scale)
@@ -153,9 +157,10 @@ def test_unlinked_pages_and_entries_past_the_pool(fmt, D):
 
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("Hq,Hk,D,ctx,qn", [(64, 1, 128, [200, 700, 65, 300], [192, 7, 65, 250]),
-                                            (32, 2, 64, [640, 400, 333, 40], [640, 400, 31, 32]),
-                                            (30, 10, 64, [1, 300, 5, 1000], [1, 171, 5, 920]),
-                                            (32, 8, 128, [900, 127, 128, 5], [897, 127, 128, 1])])
+                                            (32, 2, 64, [640, 400, 333, 64], [640, 400, 63, 64]),
+                                            (30, 10, 64, [1, 400, 350, 600], [1, 342, 341, 500]),
+                                            (32, 8, 128, [900, 255, 256, 5], [897, 255, 256, 1]),
+                                            (64, 1, 128, [600, 500, 8, 70], [600, 430, 8, 7])])
 def test_long_chunks(fmt, Hq, Hk, D, ctx, qn):
     """Chunks on both sides of the length from which they attend from a staged copy, beside single tokens."""
     c = Case(fmt, ctx, qn, Hq, Hk, D, seed=Hq + qn[0])
