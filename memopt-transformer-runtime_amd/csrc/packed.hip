@@ -39,7 +39,7 @@
 //    operands.
 //  * V enters as exact codes, too: the products of a scale group take the
 //    weights times that group's scale per token. So a page's only rounding to
-//    16 bits is that of weight times scale, and up to 16 rows what that loses
+//    16 bits is that of weight times scale, and up to 128 rows what that loses
 //    is a second operand (HALVES, REST).
 //
 // Bound by the stream of pages and 7 us around it: a copy of the kernel without
@@ -184,21 +184,23 @@ __device__ __forceinline__ T lds_at(uint32_t a) {
 // Workgroups per CU that the kernels' registers and LDS are meant for.
 __host__ __device__ static constexpr int resident(int NW, int QN) { return QN == 32 ? 2 : NW == 4 ? 3 : 1; }
 
-template <int D, int FMT, int QN, int NW>
+template <int D, int FMT, int QN, int NW, bool REST>
 __global__ __launch_bounds__(64 * NW, NW * resident(NW, QN) / 4) void packed_kernel(
     const PackedParams p, const int32_t *__restrict__ starts, const int32_t *__restrict__ ctxs,
     const int32_t *__restrict__ tables) {
   constexpr int NT = 64 * NW, KK = D / 32, ND = D / 16, QB = QN == 32 ? 2 : 1;
   constexpr bool PAGES = FMT == MEMOPT_KV_INT4;
   constexpr int NG = PAGES ? D / 64 : 1;  // score sums per (row, token)
-  // Decode over pages: a weight enters the second product as the sum of two
-  // 16-bit operands, itself and what its rounding lost. One rounding of a weight
-  // that makes up much of a row is an error of that whole row: up to 4.8e-4 of
-  // the output's norm, where two operands leave the output's own 2e-4. Up to 8
-  // rows, the rest takes the other 8 columns of the same instructions (HALVES:
-  // columns n and n + 8 are the same row); up to 16 an instruction of its own.
-  // (131072 tokens, 5 rows: 33.1 us without, 37.7 as instructions of its own.)
-  constexpr bool HALVES = QN == 8, REST = PAGES && QN == 16;
+  // Over pages, up to 128 rows: a weight enters the second product as the sum of
+  // two 16-bit operands, itself and what its rounding lost. One rounding of a
+  // weight that makes up much of a row is an error of that whole row: up to
+  // 4.8e-4 of the output's norm, where two operands leave the output's own 2e-4.
+  // Up to 8 rows, the rest takes the other 8 columns of the same instructions
+  // (HALVES: columns n and n + 8 are the same row); else instructions of its own
+  // (REST). (131072 tokens, 5 rows: 33.1 us without, 34.2 in columns, 37.7 as
+  // instructions; 8 sequences of 4096 tokens and 64 rows 34.3 without, 38.8 with,
+  // of 256 rows 73 and 89: there errors average out, to 3.0e-4.)
+  constexpr bool HALVES = QN == 8;
   constexpr int OS = D + 4;               // row stride of s_o: 16 rows of D floats would share a bank
   // Pages stream through a ring of raw blocks per wave (see copy_step), which
   // the merge of the waves takes over when the steps are done.
@@ -1091,6 +1093,7 @@ static int64_t packed_steps(const memopt_packed_desc &d) {
 // Query rows per block: 8 or 16 where no sequence has more.
 struct PackedPlan {
   int32_t qn, waves, wgs;
+  bool rest;       // see REST
   int64_t blocks;  // at most this many
   int32_t min_rows, slots;  // staged sequences
   int64_t cap;
@@ -1115,6 +1118,7 @@ static PackedPlan packed_plan(const memopt_packed_desc &d) {
   PackedPlan pl = {};
   const int64_t G = d.num_heads / d.num_kv_heads, most = (int64_t)std::min(d.max_query_len, d.tokens) * G;
   pl.qn = most > 16 ? 32 : most > 8 || d.kv_format == MEMOPT_KV_FP16 ? 16 : 8;
+  pl.rest = most <= 128;
   // sum over the sequences of ceil(rows / qn)
   pl.blocks = (d.tokens * G + (int64_t)(pl.qn - 1) * std::min(d.batch, d.tokens)) / pl.qn;
   // Workgroups of 4 waves, three to a CU: they hide each other's starts and
@@ -1192,22 +1196,23 @@ static int validate_packed(const memopt_packed_desc &d) {
   return MEMOPT_OK;
 }
 
-template <int D, int FMT, int QN, int NW>
+template <int D, int FMT, int QN, int NW, bool REST>
 static void launch_packed(const PackedParams &p, const memopt_packed_desc &d, hipStream_t stream) {
-  hipLaunchKernelGGL((packed_kernel<D, FMT, QN, NW>), dim3((unsigned)((int64_t)p.wgs * p.Hk)), dim3(64 * NW), 0, stream,
+  hipLaunchKernelGGL((packed_kernel<D, FMT, QN, NW, REST>), dim3((unsigned)((int64_t)p.wgs * p.Hk)), dim3(64 * NW), 0, stream,
                      p, d.query_starts, d.context_lens, d.block_tables);
 }
 template <int D>
 static void launch_packed(const PackedParams &p, const memopt_packed_desc &d, const PackedPlan &pl, hipStream_t s) {
   if (d.kv_format == MEMOPT_KV_INT4) {
-    if (pl.qn == 32) launch_packed<D, MEMOPT_KV_INT4, 32, 4>(p, d, s);
-    else if (pl.qn == 16 && pl.waves == 12) launch_packed<D, MEMOPT_KV_INT4, 16, 12>(p, d, s);
-    else if (pl.qn == 16) launch_packed<D, MEMOPT_KV_INT4, 16, 4>(p, d, s);
-    else if (pl.waves == 12) launch_packed<D, MEMOPT_KV_INT4, 8, 12>(p, d, s);
-    else launch_packed<D, MEMOPT_KV_INT4, 8, 4>(p, d, s);
+    if (pl.qn == 32 && pl.rest) launch_packed<D, MEMOPT_KV_INT4, 32, 4, true>(p, d, s);
+    else if (pl.qn == 32) launch_packed<D, MEMOPT_KV_INT4, 32, 4, false>(p, d, s);
+    else if (pl.qn == 16 && pl.waves == 12) launch_packed<D, MEMOPT_KV_INT4, 16, 12, true>(p, d, s);
+    else if (pl.qn == 16) launch_packed<D, MEMOPT_KV_INT4, 16, 4, true>(p, d, s);
+    else if (pl.waves == 12) launch_packed<D, MEMOPT_KV_INT4, 8, 12, false>(p, d, s);
+    else launch_packed<D, MEMOPT_KV_INT4, 8, 4, false>(p, d, s);
   } else {
-    if (pl.qn == 32) launch_packed<D, MEMOPT_KV_FP16, 32, 4>(p, d, s);
-    else launch_packed<D, MEMOPT_KV_FP16, 16, 8>(p, d, s);
+    if (pl.qn == 32) launch_packed<D, MEMOPT_KV_FP16, 32, 4, false>(p, d, s);
+    else launch_packed<D, MEMOPT_KV_FP16, 16, 8, false>(p, d, s);
   }
 }
 
