@@ -656,11 +656,12 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const PromptParams p
     }
     __syncthreads();  // K(0)'s buffer is refilled by the first iteration
   }
-  // Iterations [m0, m1) are pipelined: this tile seen whole, the next seen.
-  // Two iterations per trip keep buffers and score registers constant. (One
+  // Iterations [m0, m1) are pipelined: this tile seen whole, the next seen (and
+  // in the list: where the context passes the block table, a wave's positions
+  // can lie behind its last tile). Two iterations per trip keep buffers and score registers constant. (One
   // loop for the plain iterations before and behind, with the buffer as a
   // variable, spilled operand addresses into the pipelined loop: twice as long.)
-  const int32_t m0 = min(n_tiles, f0 + (f0 & 1)), m1 = max(m0, min(f1, v1 - 1));
+  const int32_t m0 = min(n_tiles, f0 + (f0 & 1)), m1 = max(m0, min(min(f1, v1 - 1), n_tiles - 1));
   int32_t it = 0;
   for (; it < m0; it += 2) {
     iter_edge(it, sx, sy, IntConst<0>{});

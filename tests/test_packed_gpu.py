@@ -215,6 +215,25 @@ def test_long_chunks_outside_the_block_table(fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,ctx,M,window,sinks", [(1162, 4511, 55, 500, 0), (1162, 4511, 55, 500, 70), (1162, 2000, 55, 64, 0),
+                                                  (1100, 1500, 55, 300, 200), (1100, 1300, 82, -1, 0),
+                                                  (1100, 1300, 82, 100, 4)])
+def test_long_chunks_of_one_query_head_per_key_head(fmt, D, n, ctx, M, window, sinks):
+    """A tile of 128 rows spans 128 positions: its last wave can see nothing where its first one does, in particular
+    behind the block table by more than the window (such rows give 0)."""
+    c = Case(fmt, [min(ctx, 16 * M)], [n], 32, 32, D, seed=n, M=M)
+    assert n * 32 >= FILL and n >= staged_rows(n, 32)
+    c.ctx = [ctx]
+    c.load()
+    out = memopt_C.packed_attention(*c.args()[:7], 5000, window, num_sink_tokens=sinks)
+    c.check(out, window, sinks)
+    if window > 0 and sinks == 0:
+        dark = torch.arange(ctx - n, ctx) - window + 1 >= 16 * M
+        assert bool((out[dark.to(dev())] == 0).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_long_chunks_among_many_sequences(fmt):
     qn = [1 + 59 * (i % 5 == 1) for i in range(70)]
     c = Case(fmt, [100 + 3 * (i % 11) for i in range(70)], qn, 64, 2, 64, seed=9)
