@@ -907,9 +907,11 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QN) / 4) void packed_ker
               x *= again;
 #pragma unroll
               for (int k = 0; k < R; ++k) {
-                const float f = i0 + k * groups >= parts || ml[k].x == -INFINITY ? 0.0f : fast_exp2(ml[k].x - mx);
+                const bool past = i0 + k * groups >= parts;
+                const float f = past || ml[k].x == -INFINITY ? 0.0f : fast_exp2(ml[k].x - mx);
                 l += f * ml[k].y;
-                x += f32x4_t{y[k][0].x, y[k][0].y, y[k][1].x, y[k][1].y} * f;
+                const f32x4_t z = f32x4_t{y[k][0].x, y[k][0].y, y[k][1].x, y[k][1].y} * f;
+                x += past ? f32x4_t{} : z;  // (no weight must not meet its inf again)
               }
             }
             if (groups > 1) {

@@ -355,6 +355,25 @@ def test_odd_values_reach_only_the_rows_that_see_them(fmt, D, window, sinks):
 
 
 @pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("ctx,qn", [(3000, 1), (3000, 5), (3000, 40), (420, 40), (20000, 1)])
+def test_infinities_pass_the_merge(D, ctx, qn):
+    """A column in which every row sees one inf of V is that inf, in whatever part of a split block it lies; the
+    others are what they were."""
+    c = Case("fp16", [ctx], [qn], 8, 2, D, seed=ctx)
+    want = memopt_C.packed_attention(*c.args()).cpu()
+    for token in (0, ctx // 3, ctx // 2, ctx - qn):
+        for bad in (float("inf"), float("-inf")):
+            page = int(c.tables[0, token // 16])
+            keep = c.vc[page, token % 16, :, 5].clone()
+            c.vc[page, token % 16, :, 5] = bad
+            out = memopt_C.packed_attention(*c.args()).cpu()
+            c.vc[page, token % 16, :, 5] = keep
+            assert bool((out[..., 5] == bad).all()), (token, bad)
+            out[..., 5] = want[..., 5]
+            assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("D", [64, 128])
 def test_evicted_rows_and_extreme_scales(D):
     """Scale 0 (rows that eviction removed), the largest scales of the format, and tiny ones."""
     c = Case("int4", [100, 64], [1, 5], 4, 2, D, seed=5)
