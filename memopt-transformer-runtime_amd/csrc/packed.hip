@@ -771,7 +771,7 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QN) / 4) void packed_ker
 #pragma unroll 1
         for (int32_t j = 0; j < mine; ++j) {
           if (j < at0 || j >= at0 + 32) look_up(j);
-          if (step_at(j) >= full0 && step_at(j) < full1) continue;  // (a whole chunk there is unlinked: all zeros)
+          if ((whole >> (2 * (j - at0))) & 1) continue;  // (its V went in as it is)
 #pragma unroll 1
           for (int tk = 0; tk < 32; ++tk) {
             const int32_t t = tk & 15, key = 16 * logical(2 * step_at(j) + (tk >> 4)) + t;

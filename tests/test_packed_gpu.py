@@ -374,6 +374,28 @@ def test_infinities_pass_the_merge(D, ctx, qn):
 
 
 @pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(-1, 0), (200, 40)])
+@pytest.mark.parametrize("qn", [1, 3, 40])
+def test_odd_values_beside_an_unlinked_page(D, window, sinks, qn):
+    """inf and NaN of V in the linked half of a 32-token step whose other page is gone, where every row sees it."""
+    for token, gone in ((40, 3), (329, 21), (385, 25)):
+        c = Case("fp16", [420], [qn], 8, 2, D, seed=token)
+        c.tables[0, gone] = -1
+        c.load()
+        want = memopt_C.packed_attention(*c.args(window=window), num_sink_tokens=sinks)
+        c.check(want, window, sinks)
+        pos = torch.arange(420 - qn, 420)
+        see = (token <= pos) & ((pos - token < window) | (token < sinks)) if window > 0 else token <= pos
+        for bad in (float("inf"), float("nan"), float("-inf")):
+            c.vc[c.tables[0, token // 16], token % 16, :, 5] = bad
+            out = memopt_C.packed_attention(*c.args(window=window), num_sink_tokens=sinks).cpu()
+            where = out[..., 5]
+            assert bool((where[see].isnan() if bad != bad else where[see] == bad).all()), (token, bad)
+            out[..., 5][see] = want.cpu()[..., 5][see]
+            assert torch.equal(out, want.cpu())
+
+
+@pytest.mark.parametrize("D", [64, 128])
 def test_evicted_rows_and_extreme_scales(D):
     """Scale 0 (rows that eviction removed), the largest scales of the format, and tiny ones."""
     c = Case("int4", [100, 64], [1, 5], 4, 2, D, seed=5)
