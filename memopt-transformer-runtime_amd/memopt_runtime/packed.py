@@ -12,7 +12,7 @@ over the cache else.
 """
 from __future__ import annotations
 
-from typing import Optional, Sequence
+from typing import List, Optional, Sequence
 
 import torch
 
@@ -111,20 +111,59 @@ class PackedBatch:
                                                 self.num_rows if max_new is None else max_new, self.max_tokens,
                                                 self.window_size, num_sink_tokens=self.num_sink_tokens, out=out)
 
+    def evict(self, requests: Sequence[int], scores: torch.Tensor, retain_ratio: float,
+              num_sink_tokens: int = 4) -> List[int]:
+        """Ada-KV eviction of the requests' tokens; pages that it unlinks go back to the ring.
+
+        ``scores``: f32 ``[requests, num_kv_heads, L]`` over the first L
+        positions, which every one of them holds (``evict_tokens``). Unlinked
+        pages stay as holes (-1) in the block tables, which attention skips.
+        Returns the freed pages, in ring order. (Waits for the device.
+        ``free_evicted_blocks`` would give them to the pool's own free list,
+        which this class does not use.)
+        """
+        requests = self._known(requests)
+        if len(set(requests)) != len(requests):
+            raise RuntimeError("PackedBatch: a request is named twice")
+        if scores.dim() != 3 or scores.shape[0] != len(requests):
+            raise RuntimeError(f"PackedBatch: scores must be [{len(requests)}, kv heads, positions]")
+        if not requests:
+            return []
+        rows = torch.tensor(requests, dtype=torch.int64, device=self.tables.device)
+        least = int(self.state.context_lens[rows].min())
+        if scores.shape[2] > least:
+            raise RuntimeError(f"PackedBatch: scores of {scores.shape[2]} positions, where a request holds {least}")
+        tables = self.tables[rows]
+        votes = torch.zeros_like(self.free_pages)
+        memopt_C.evict_tokens(scores, tables, votes, retain_ratio, num_sink_tokens)
+        self.tables[rows] = tables
+        freed = torch.nonzero(votes == scores.shape[1]).flatten().tolist()
+        self._give_back(freed)
+        return freed
+
     def release(self, requests: Sequence[int]) -> None:
-        """Return the requests' pages to the ring; their indices are free for
-        new requests. (Waits for the device: the pages are read back.)"""
-        requests = list(dict.fromkeys(int(r) for r in requests))
-        if any(not 0 <= r < self.tables.shape[0] for r in requests):
-            raise RuntimeError("PackedBatch: no such request")
+        """Return the requests' linked pages to the ring; their indices are free
+        for new requests. (Waits for the device: the pages are read back.)"""
+        requests = list(dict.fromkeys(self._known(requests)))
         if not requests:
             return
         rows = torch.tensor(requests, dtype=torch.int64, device=self.tables.device)
         tables, lens = self.tables[rows].cpu(), self.state.context_lens[rows].cpu()
-        pages = [p for t, n in zip(tables.tolist(), lens.tolist()) for p in t[:pages_needed(n, self.block_size)]]
-        head, count = self.state.free_span.tolist()
-        at = (head + count + torch.arange(len(pages))) % self.free_pages.shape[0]
-        self.free_pages[at.to(rows.device)] = torch.tensor(pages, dtype=torch.int32, device=rows.device)
-        self.state.free_span[1] = count + len(pages)
+        self._give_back([p for t, n in zip(tables.tolist(), lens.tolist())
+                         for p in t[:pages_needed(n, self.block_size)] if p >= 0])
         self.tables[rows] = -1
         self.state.context_lens[rows] = 0
+
+    def _known(self, requests: Sequence[int]) -> List[int]:
+        requests = [int(r) for r in requests]
+        if any(not 0 <= r < self.tables.shape[0] for r in requests):
+            raise RuntimeError("PackedBatch: no such request")
+        return requests
+
+    def _give_back(self, pages: List[int]) -> None:
+        """Append ``pages`` to the ring."""
+        head, count = self.state.free_span.tolist()
+        at = (head + count + torch.arange(len(pages))) % self.free_pages.shape[0]
+        dev = self.free_pages.device
+        self.free_pages[at.to(dev)] = torch.tensor(pages, dtype=torch.int32, device=dev)
+        self.state.free_span[1] = count + len(pages)

@@ -117,6 +117,90 @@ def test_pages_that_do_not_last():
         batch.release([3])
 
 
+def ring(batch):
+    """The free pages, front first."""
+    head, count = batch.state.free_span.tolist()
+    pages = batch.free_pages.tolist()
+    return [pages[(head + i) % len(pages)] for i in range(count)]
+
+
+class Evicting:
+    """Requests of 90 and 40 tokens over 12 pages, and scores that evict tokens 16 .. 47 of the first in every head."""
+
+    def __init__(self, fmt):
+        self.fmt, self.rng = fmt, torch.Generator().manual_seed(8)
+        self.batch = R().PackedBatch(12, 2, 64, 3, 112, 96 + 44, kv_format=fmt)
+        self.host = Host(3, 2, 64)
+        self.live = [np.ones(112, bool) for _ in range(3)]
+        self.step({0: 90, 1: 40})
+        self.scores = torch.arange(90, 0, -1, dtype=torch.float32, device=dev()).repeat(1, 2, 1)
+        self.scores[:, :, 16:48] -= 200
+        self.ratio = 0.64  # ceil(57.6) = 58 of 90 stay
+
+    def step(self, want):
+        b = self.batch
+        s = b.advance(torch.tensor([want.get(r, 0) for r in range(3)], dtype=torch.int32, device=dev()))
+        assert s.status.tolist() == [0, 0, 0]
+        q, k, v = (torch.randn((b.num_rows, h, 64), generator=self.rng).half().to(dev()) for h in (8, 2, 2))
+        out, cu = b.attend(q, k, v), s.cu_seqlens.tolist()
+        for r in want:
+            x, y, first = cu[r], cu[r + 1], len(self.host.k[r])
+            self.host.extend(r, k[x:y], v[x:y])
+            n = len(self.host.k[r])
+            (kk, ks), (vv, vs) = cached(self.host.k[r], self.fmt), cached(self.host.v[r], self.fmt)
+            o, a, e = attend(q[x:y], kk, vv, np.arange(first, n), -1, 0, torch.from_numpy(self.live[r][:n]))
+            scores = quantized_scores(q[x:y], ks, False) if self.fmt == "int4" else 0.0
+            check(out[x:y], o, tolerance(o, a, e, n, 64, torch.float16, torch.float16, False, scores, vs), f"request {r}")
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_release_of_a_request_with_evicted_pages(fmt):
+    """The holes that eviction leaves in a block table are no pages to give back."""
+    e = Evicting(fmt)
+    held = [p for p in e.batch.tables[0].tolist() if p >= 0]
+    votes = torch.zeros(12, dtype=torch.int32, device=dev())
+    memopt_C.evict_tokens(e.scores, e.batch.tables[:1], votes, e.ratio, 0)
+    assert e.batch.tables[0].tolist() == [held[0], -1, -1, *held[3:], -1]
+    before = ring(e.batch)
+    e.batch.release([0])
+    assert ring(e.batch) == before + [held[0], *held[3:]]
+    e.host.k[0], e.host.v[0] = e.host.k[0][:0], e.host.v[0][:0]
+    e.step({2: 112, 1: 1})  # all seven pages
+    assert ring(e.batch) == [] and int(e.batch.tables[2].min()) >= 0
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_evict_release_and_admit_again(fmt):
+    """Pages that PackedBatch.evict frees are in the ring once, and serve other requests."""
+    e = Evicting(fmt)
+    held = e.batch.tables[0].tolist()
+    before = ring(e.batch)
+    assert e.batch.evict([0], e.scores, e.ratio) == sorted(held[1:3])
+    assert ring(e.batch) == before + sorted(held[1:3])
+    assert e.batch.tables[0].tolist() == [held[0], -1, -1, *held[3:]]
+    e.live[0][16:48] = False
+    e.step({0: 7, 1: 1})    # (request 0 goes on: 97 tokens, one page more)
+    e.step({2: 60, 0: 1})   # the ring's last two, and the two that were freed
+    assert sorted(ring(e.batch)) == [] and set(held[1:3]) <= set(e.batch.tables[2].tolist())
+    e.batch.release([0])
+    e.host.k[0], e.host.v[0] = e.host.k[0][:0], e.host.v[0][:0]
+    e.live[0][:] = True
+    e.step({0: 70, 1: 1, 2: 1})
+    e.batch.release([0, 1, 2])
+    assert sorted(ring(e.batch)) == list(range(12))
+
+
+def test_evict_refusals():
+    e = Evicting("int4")
+    for match, requests, scores in [("no such request", [3], e.scores), ("twice", [0, 0], e.scores.repeat(2, 1, 1)),
+                                    ("scores", [0, 1], e.scores), ("scores", [1], e.scores), ("scores", [2], e.scores),
+                                    ("scores", [0], e.scores[0])]:
+        with pytest.raises(RuntimeError, match=match):
+            e.batch.evict(requests, scores, 0.5)
+    assert e.batch.evict([], e.scores[:0], 0.5) == []
+    assert len(ring(e.batch)) == 3
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("planned", [True, False])
 def test_captured_step(fmt, planned):
