@@ -979,10 +979,13 @@ def packed_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
 class PreparedPackedAttention:
     """A validated ``packed_attention`` call bound to fixed tensors.
 
-    Construction checks the arguments and allocates the workspace; each call
-    launches on the current stream and returns ``out`` (overwritten in place).
-    For loops in which only the tensors' contents change. Calls of one plan
-    share its workspace and must not overlap.
+    Construction checks the arguments, allocates the workspace and waits until
+    its counters are cleared, so that calls may come on any stream; each call
+    launches on the current stream (or the raw handle ``stream``) and returns
+    ``out`` (overwritten in place). For loops in which only the tensors'
+    contents change. Calls of one plan share its workspace and must not
+    overlap. A plan made while a stream is captured has its counters cleared
+    by that graph: it is for calls in that graph.
     """
 
     def __init__(self, query, key_cache, value_cache, block_tables, context_lens, cu_seqlens, max_query_len,
@@ -995,6 +998,8 @@ class PreparedPackedAttention:
             self._d, self.out, self._ws, self._keep = _packed_desc(
                 query, key_cache, value_cache, block_tables, context_lens, cu_seqlens, max_query_len, max_seq_len,
                 window_size, num_sink_tokens, out)
+            if self._ws is not None and not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream().synchronize()
         self._dp = ctypes.byref(self._d)
 
     @property

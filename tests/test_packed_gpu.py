@@ -534,6 +534,33 @@ def test_plans_on_two_streams_and_in_graphs():
             assert torch.equal(p.out, memopt_C.packed_attention(*c.args()))
 
 
+@pytest.mark.parametrize("explicit", [True, False])
+def test_first_call_of_a_plan_on_another_stream(explicit):
+    """A plan made behind queued work of one stream is ready for a call on another, whatever its memory held."""
+    c = Case("int4", [3000, 2500], [1, 1], 8, 2, 64, seed=31)
+    want = memopt_C.packed_attention(*c.args())
+    c.check(want)
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    busy = torch.ones((4096, 4096), device=dev())
+    size = memopt_C.PreparedPackedAttention(*c.args()).workspace_bytes
+    for _ in range(5):
+        dirty = torch.full((size,), 0xFF, dtype=torch.uint8, device=dev())  # (its memory is the next plan's)
+        del dirty
+        out = torch.zeros_like(c.q)
+        other.wait_stream(torch.cuda.current_stream())
+        for _ in range(20):
+            busy = busy @ busy * 0
+        plan = memopt_C.PreparedPackedAttention(*c.args(), out=out)
+        if explicit:
+            plan(other.cuda_stream)
+        else:
+            with torch.cuda.stream(other):
+                plan()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_captured_long_chunks_follow_the_lengths_on_the_device(fmt):
     """One captured plan, replayed as chunks grow and shrink across the length from which they are staged; and eager
