@@ -184,22 +184,29 @@ __device__ __forceinline__ T lds_at(uint32_t a) {
 // Workgroups per CU that the kernels' registers and LDS are meant for.
 __host__ __device__ static constexpr int resident(int NW, int QN) { return QN == 32 ? 2 : NW == 4 ? 3 : 1; }
 
-template <int D, int FMT, int QN, int NW, bool REST>
+// Where the rest of the weights is a second operand (see REST below): for no
+// row, for all, or for those of sequences with up to kRestRows rows.
+enum Rest { kNoRest, kAllRest, kShortRest };
+static constexpr int kRestRows = 128;
+
+template <int D, int FMT, int QN, int NW, Rest REST>
 __global__ __launch_bounds__(64 * NW, NW * resident(NW, QN) / 4) void packed_kernel(
     const PackedParams p, const int32_t *__restrict__ starts, const int32_t *__restrict__ ctxs,
     const int32_t *__restrict__ tables) {
   constexpr int NT = 64 * NW, KK = D / 32, ND = D / 16, QB = QN == 32 ? 2 : 1;
   constexpr bool PAGES = FMT == MEMOPT_KV_INT4;
   constexpr int NG = PAGES ? D / 64 : 1;  // score sums per (row, token)
-  // Over pages, up to 128 rows: a weight enters the second product as the sum of
-  // two 16-bit operands, itself and what its rounding lost. One rounding of a
-  // weight that makes up much of a row is an error of that whole row: up to
-  // 4.8e-4 of the output's norm, where two operands leave the output's own 2e-4.
-  // Up to 8 rows, the rest takes the other 8 columns of the same instructions
-  // (HALVES: columns n and n + 8 are the same row); else instructions of its own
-  // (REST). (131072 tokens, 5 rows: 33.1 us without, 34.2 in columns, 37.7 as
-  // instructions; 8 sequences of 4096 tokens and 64 rows 34.3 without, 38.8 with,
-  // of 256 rows 73 and 89: there errors average out, to 3.0e-4.)
+  // Over pages, in sequences of up to 128 rows: a weight enters the second product
+  // as the sum of two 16-bit operands, itself and what its rounding lost. One
+  // rounding of a weight that makes up much of a row is an error of that whole
+  // row: up to 4.8e-4 of the output's norm, where two operands leave the output's
+  // own 2e-4. Up to 8 rows, the rest takes the other 8 columns of the same
+  // instructions (HALVES: columns n and n + 8 are the same row); else
+  // instructions of its own (REST), by sequence where a batch has longer ones, so
+  // that what a request gets does not hang on its neighbours. (131072 tokens, 5
+  // rows: 33.1 us without, 34.2 in columns, 37.7 as instructions; 8 sequences of
+  // 4096 tokens and 64 rows 34.3 without, 38.8 with, of 256 rows 73 and 89: there
+  // errors average out, to 3.0e-4.)
   constexpr bool HALVES = QN == 8;
   constexpr int OS = D + 4;               // row stride of s_o: 16 rows of D floats would share a bank
   // Pages stream through a ring of raw blocks per wave (see copy_step), which
@@ -526,7 +533,8 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QN) / 4) void packed_ker
     constexpr float kTop = 7.0f;
     uint32_t odd = 0;  // nonzero: a masked step held inf or NaN in V
     // One step; `between` runs when K has been used and V has not.
-    auto step = [&](int32_t j, auto between) __attribute__((always_inline)) {
+    auto step = [&](int32_t j, auto rest, auto between) __attribute__((always_inline)) {
+      constexpr bool R = decltype(rest)::value;
       f32x4_t s[QB][NG][2];
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
@@ -636,7 +644,7 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QN) / 4) void packed_ker
               }
             }
             pf[qb][u] = __builtin_bit_cast(h8_t, w);
-            if constexpr (REST) {
+            if constexpr (R) {
 #pragma unroll
               for (int i = 0; i < 4; ++i)
                 w[i] = as_u32(half2_t{
@@ -686,7 +694,7 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QN) / 4) void packed_ker
         for (int qb = 0; qb < QB; ++qb) {
           const h8_t v = __builtin_bit_cast(h8_t, a);
           o[qb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf[qb][i / (ND / NG)], o[qb][i], 0, 0, 0);
-          if constexpr (REST)
+          if constexpr (R)
             o[qb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf_rest[qb][i / (ND / NG)], o[qb][i], 0, 0, 0);
         }
       };
@@ -720,21 +728,29 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QN) / 4) void packed_ker
       for (int k = 0; k < NS; ++k)
         if (k < mine) copy_step(k, k);
       prepare_q();
-      int stage = 0;
+      auto walk = [&](auto rest) __attribute__((always_inline)) {
+        int stage = 0;
 #pragma unroll 1
-      for (int32_t j = 0; j < mine; ++j) {
-        if (j + NS - at0 >= 32) look_up(j);
-        // this step's copies are the oldest: wait until no more than the later step's are left
-        static_assert(NS == 2, "one later step");
-        if (j + 1 < mine) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CPS) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        read_k(stage);
-        step(j, [&]() __attribute__((always_inline)) {
-          read_v(stage);
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the stage is filled again
-          if (j + NS < mine) copy_step(j + NS, stage);
-        });
-        stage ^= 1;
+        for (int32_t j = 0; j < mine; ++j) {
+          if (j + NS - at0 >= 32) look_up(j);
+          // this step's copies are the oldest: wait until no more than the later step's are left
+          static_assert(NS == 2, "one later step");
+          if (j + 1 < mine) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CPS) : "memory");
+          else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          read_k(stage);
+          step(j, rest, [&]() __attribute__((always_inline)) {
+            read_v(stage);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the stage is filled again
+            if (j + NS < mine) copy_step(j + NS, stage);
+          });
+          stage ^= 1;
+        }
+      };
+      if constexpr (REST == kShortRest) {
+        if (rows <= kRestRows) walk(std::true_type{});
+        else walk(std::false_type{});
+      } else {
+        walk(std::integral_constant<bool, REST == kAllRest>{});
       }
       if constexpr (HALVES) {  // both columns of a row
 #pragma unroll
@@ -757,7 +773,7 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QN) / 4) void packed_ker
 #pragma unroll 1
       for (int32_t j = 0; j < mine; ++j) {
         if (j + 1 - at0 >= 32) look_up(j);
-        step(j, [&]() __attribute__((always_inline)) {
+        step(j, std::false_type{}, [&]() __attribute__((always_inline)) {
           if (j + 1 < mine) load_k(j + 1);
         });
         if (j + 1 < mine) load_v(j + 1);
@@ -1095,7 +1111,7 @@ static int64_t packed_steps(const memopt_packed_desc &d) {
 // Query rows per block: 8 or 16 where no sequence has more.
 struct PackedPlan {
   int32_t qn, waves, wgs;
-  bool rest;       // see REST
+  bool rest;       // no sequence has more than kRestRows
   int64_t blocks;  // at most this many
   int32_t min_rows, slots;  // staged sequences
   int64_t cap;
@@ -1120,7 +1136,7 @@ static PackedPlan packed_plan(const memopt_packed_desc &d) {
   PackedPlan pl = {};
   const int64_t G = d.num_heads / d.num_kv_heads, most = (int64_t)std::min(d.max_query_len, d.tokens) * G;
   pl.qn = most > 16 ? 32 : most > 8 || d.kv_format == MEMOPT_KV_FP16 ? 16 : 8;
-  pl.rest = most <= 128;
+  pl.rest = most <= kRestRows;
   // sum over the sequences of ceil(rows / qn)
   pl.blocks = (d.tokens * G + (int64_t)(pl.qn - 1) * std::min(d.batch, d.tokens)) / pl.qn;
   // Workgroups of 4 waves, three to a CU: they hide each other's starts and
@@ -1198,7 +1214,7 @@ static int validate_packed(const memopt_packed_desc &d) {
   return MEMOPT_OK;
 }
 
-template <int D, int FMT, int QN, int NW, bool REST>
+template <int D, int FMT, int QN, int NW, Rest REST>
 static void launch_packed(const PackedParams &p, const memopt_packed_desc &d, hipStream_t stream) {
   hipLaunchKernelGGL((packed_kernel<D, FMT, QN, NW, REST>), dim3((unsigned)((int64_t)p.wgs * p.Hk)), dim3(64 * NW), 0, stream,
                      p, d.query_starts, d.context_lens, d.block_tables);
@@ -1206,15 +1222,15 @@ static void launch_packed(const PackedParams &p, const memopt_packed_desc &d, hi
 template <int D>
 static void launch_packed(const PackedParams &p, const memopt_packed_desc &d, const PackedPlan &pl, hipStream_t s) {
   if (d.kv_format == MEMOPT_KV_INT4) {
-    if (pl.qn == 32 && pl.rest) launch_packed<D, MEMOPT_KV_INT4, 32, 4, true>(p, d, s);
-    else if (pl.qn == 32) launch_packed<D, MEMOPT_KV_INT4, 32, 4, false>(p, d, s);
-    else if (pl.qn == 16 && pl.waves == 12) launch_packed<D, MEMOPT_KV_INT4, 16, 12, true>(p, d, s);
-    else if (pl.qn == 16) launch_packed<D, MEMOPT_KV_INT4, 16, 4, true>(p, d, s);
-    else if (pl.waves == 12) launch_packed<D, MEMOPT_KV_INT4, 8, 12, false>(p, d, s);
-    else launch_packed<D, MEMOPT_KV_INT4, 8, 4, false>(p, d, s);
+    if (pl.qn == 32 && pl.rest) launch_packed<D, MEMOPT_KV_INT4, 32, 4, kAllRest>(p, d, s);
+    else if (pl.qn == 32) launch_packed<D, MEMOPT_KV_INT4, 32, 4, kShortRest>(p, d, s);
+    else if (pl.qn == 16 && pl.waves == 12) launch_packed<D, MEMOPT_KV_INT4, 16, 12, kAllRest>(p, d, s);
+    else if (pl.qn == 16) launch_packed<D, MEMOPT_KV_INT4, 16, 4, kAllRest>(p, d, s);
+    else if (pl.waves == 12) launch_packed<D, MEMOPT_KV_INT4, 8, 12, kNoRest>(p, d, s);
+    else launch_packed<D, MEMOPT_KV_INT4, 8, 4, kNoRest>(p, d, s);
   } else {
-    if (pl.qn == 32) launch_packed<D, MEMOPT_KV_FP16, 32, 4, false>(p, d, s);
-    else launch_packed<D, MEMOPT_KV_FP16, 16, 8, false>(p, d, s);
+    if (pl.qn == 32) launch_packed<D, MEMOPT_KV_FP16, 32, 4, kNoRest>(p, d, s);
+    else launch_packed<D, MEMOPT_KV_FP16, 16, 8, kNoRest>(p, d, s);
   }
 }
 

@@ -115,6 +115,28 @@ def test_mixed_query_counts(fmt, Hq, Hk, D, ctx, qn):
     c.check(memopt_C.packed_attention(*c.args(most=10 ** 6)))
 
 
+@pytest.mark.parametrize("Hq,Hk,D,qn", [(8, 2, 64, [1, 40, 32, 1, 3, 33, 1]), (32, 8, 128, [33, 1, 32, 2, 200]),
+                                        (12, 1, 128, [1, 11, 10, 1]), (64, 1, 64, [600, 2, 1, 3, 1]),
+                                        (64, 1, 128, [1, 2, 600])])
+def test_short_sequences_beside_long_ones_keep_what_a_weight_rounding_loses(Hq, Hk, D, qn):
+    """Over pages, sequences of up to 128 rows (tokens times query heads per key head) hold their weights in two 16-bit
+    operands, whatever else the batch brings. A window of one token makes each row its own value: it is off by the
+    output's rounding, 2^-11, by the 2^-22 that two operands leave, and by a few roundings in 32 bits (less than 2^-20
+    in all), or by half a step of fp16's subnormals. (A single operand is off by 2^-11 more.)"""
+    c = Case("int4", [n + 40 + 3 * i for i, n in enumerate(qn)], qn, Hq, Hk, D, seed=D + len(qn))
+    G = Hq // Hk
+    out = memopt_C.packed_attention(*c.args(window=1)).double().cpu()
+    c.check(out.half(), 1, 0)
+    at = 0
+    for b, (ctx, n) in enumerate(zip(c.ctx, c.qn)):
+        pages = torch.from_numpy(c.tables[b, :-(-ctx // 16)]).long()
+        v = c.vval[pages].flatten(0, 1)[ctx - n:ctx].repeat_interleave(G, 1)
+        if n * G <= 128:
+            off = (out[at:at + n] - v).abs()
+            assert bool((off <= (2.0 ** -11 + 2.0 ** -20) * v.abs() + 2.0 ** -25).all()), (b, float((off / v.abs()).nan_to_num().max()))
+        at += n
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("window,sinks", [(1, 0), (16, 0), (17, 3), (100, 16), (100, 33), (5, 400), (2 ** 31 - 1, 2 ** 31 - 1),
                                           (0, 3)])
