@@ -807,7 +807,9 @@ def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int, int, int]:
     p = t.data_ptr()
     if ds == 1 and not (ts % 8 or hs % 8 or p % 16) and ts >= t.shape[2]:
         return t, p, ts, hs
-    t = t.contiguous()
+    t = t.contiguous()  # (itself, where it is that already but off the alignment)
+    if t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
     return t, t.data_ptr(), t.shape[1] * t.shape[2], t.shape[2]
 
 

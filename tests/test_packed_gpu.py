@@ -497,6 +497,18 @@ def test_strides_padding_and_out(fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+def test_contiguous_queries_off_the_alignment_are_copied(fmt):
+    c = Case(fmt, [60, 200], [4, 30], 6, 2, 64, seed=2)
+    want = memopt_C.packed_attention(*c.args())
+    flat = torch.empty(c.q.numel() + 8, dtype=c.q.dtype, device=dev())[4:4 + c.q.numel()]
+    c.q = flat.view(c.q.shape).copy_(c.q)
+    assert c.q.is_contiguous() and c.q.data_ptr() % 16 == 8
+    assert torch.equal(memopt_C.packed_attention(*c.args()), want)
+    with pytest.raises(RuntimeError, match="read in place"):
+        memopt_C.PreparedPackedAttention(*c.args())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_pool_views_are_taken(fmt):
     """The live pool's views, written by write_cache."""
     g = torch.Generator(device=dev()).manual_seed(0)

@@ -86,6 +86,23 @@ def test_strides_that_are_read_in_place_and_others():
     assert torch.equal(buf[..., 64:], want) and bool((buf[..., :64] == 7).all())
 
 
+def shifted(t):
+    """A contiguous tensor with t's values at an address that no 16 divide."""
+    flat = torch.empty(t.numel() + 8, dtype=t.dtype, device=t.device)[4:4 + t.numel()]
+    assert flat.data_ptr() % 16 == 8
+    return flat.view(t.shape).copy_(t)
+
+
+def test_contiguous_inputs_off_the_alignment_are_copied():
+    lens = [90, 45]
+    q, k, v = make(135, 4, 2, 64, torch.float16, 9)
+    want = memopt_C.prompt_attention(q, k, v, cu_of(lens))
+    for i in range(3):
+        ins = [shifted(t) if i == j else t for j, t in enumerate((q, k, v))]
+        assert torch.equal(memopt_C.prompt_attention(*ins, cu_of(lens)), want)
+    assert torch.equal(memopt_C.prompt_attention(*(shifted(t) for t in (q, k, v)), cu_of(lens)), want)
+
+
 def test_rows_of_no_sequence_stay_as_they_are():
     """Padding before, between (none can be) and behind the sequences is neither read nor written."""
     lens, first, T = [40, 100], 7, 160
