@@ -320,7 +320,8 @@ int memopt_multi_query_path(int32_t path);
  * sequence sees its rows j <= i with j < num_sink_tokens or j > i -
  * window_size (window_size <= 0: all j <= i), scale 1/sqrt(head_dim).
  * Elements of hidden rows never reach a result, inf and NaN included.
- * head_dim 64 or 128. `out` must not overlap the inputs. */
+ * head_dim 64 or 128; key and value token strides from head_dim to 2^23 - 1.
+ * `out` must not overlap the inputs. */
 typedef struct memopt_prompt_desc {
   const void *query, *key, *value;   /* [tokens, heads, head_dim]              */
   void *out;                         /* [tokens, num_heads, head_dim]          */

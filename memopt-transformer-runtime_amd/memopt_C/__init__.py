@@ -799,13 +799,17 @@ def _no_grad(fn: str, requires_grad: bool) -> None:
         raise RuntimeError(f"{fn}: no gradients are computed; call it under torch.no_grad()")
 
 
-def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int, int, int]:
+_FAR = 2 ** 23  # token stride from which the prompt kernel's 31-bit tile ranges no longer hold keys and values
+
+
+def _rows(t: torch.Tensor, far: int = 2 ** 63) -> Tuple[torch.Tensor, int, int, int]:
     """(tensor, address, token stride, head stride) of ``t`` itself where its
-    last dimension is contiguous and its rows are 16-byte aligned (views of a
-    fused projection are), else of a contiguous copy."""
+    last dimension is contiguous, its rows are 16-byte aligned (views of a
+    fused projection are) and its tokens less than ``far`` elements apart,
+    else of a contiguous copy."""
     ts, hs, ds = t.stride()
     p = t.data_ptr()
-    if ds == 1 and not (ts % 8 or hs % 8 or p % 16) and ts >= t.shape[2]:
+    if ds == 1 and not (ts % 8 or hs % 8 or p % 16) and t.shape[2] <= ts < far:
         return t, p, ts, hs
     t = t.contiguous()  # (itself, where it is that already but off the alignment)
     if t.data_ptr() % 16:
@@ -853,7 +857,8 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     ``query`` ``[T, Hq, D]``, ``keys`` / ``values`` ``[T, Hkv, D]``: fp16 or
     bf16, D 64 or 128, Hq a multiple of Hkv (query head h reads key head
     ``h // (Hq / Hkv)``); any strides whose rows are contiguous and 16-byte
-    aligned, such as views of a fused projection, are read in place.
+    aligned, such as views of a fused projection, are read in place (keys and
+    values less than 2^23 elements apart), others are copied.
     ``cu_seqlens``: int32 ``[B + 1]`` on the device, ascending; sequence b is
     rows ``cu_seqlens[b] .. cu_seqlens[b + 1] - 1``. Row i of a sequence sees
     its rows ``j <= i`` with ``j < num_sink_tokens`` or ``j > i -
@@ -889,8 +894,8 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     _int32(fn, cu_seqlens, "cu_seqlens", cshape)
     out, po, ots, ohs = _out_rows(fn, out, query)
     q, pq, qts, qhs = _rows(query)
-    k, pk, kts, khs = _rows(keys)
-    v, pv, vts, vhs = _rows(values)
+    k, pk, kts, khs = _rows(keys, _FAR)
+    v, pv, vts, vhs = _rows(values, _FAR)
     try:
         d = _PROMPT.pack(pq, pk, pv, po, 1 if dtype is torch.bfloat16 else 0, T, cshape[0] - 1, Hq, Hk, D, qts, qhs, kts,
                          khs, vts, vhs, ots, ohs, cu_seqlens.data_ptr(), _count32(window_size),

@@ -103,6 +103,17 @@ def test_contiguous_inputs_off_the_alignment_are_copied():
     assert torch.equal(memopt_C.prompt_attention(*(shifted(t) for t in (q, k, v)), cu_of(lens)), want)
 
 
+def test_token_strides_past_the_kernels_range():
+    """Rows 2^23 elements apart and more (a position of a [tokens, positions, heads, head_dim] buffer)."""
+    lens = [2, 1]
+    q, k, v = make(3, 4, 2, 64, torch.float16, 9)
+    want = memopt_C.prompt_attention(q, k, v, cu_of(lens))
+    for stride in (2 ** 23 - 8, 2 ** 23, 2 ** 23 + 8):
+        far = [torch.empty(3 * stride, dtype=t.dtype, device=dev()).as_strided(t.shape, (stride, 64, 1)).copy_(t)
+               for t in (q, k, v)]
+        assert torch.equal(memopt_C.prompt_attention(*far, cu_of(lens)), want)
+
+
 def test_rows_of_no_sequence_stay_as_they_are():
     """Padding before, between (none can be) and behind the sequences is neither read nor written."""
     lens, first, T = [40, 100], 7, 160
