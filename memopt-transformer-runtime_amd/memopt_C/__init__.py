@@ -828,9 +828,10 @@ def _out_rows(fn: str, out: Optional[torch.Tensor], query: torch.Tensor) -> Tupl
         raise RuntimeError(f"{fn}: out must be shaped like query, with its dtype")
     ts, hs, ds = out.stride()
     p = out.data_ptr()
-    # (a row stride of 0 would have rows overwrite each other)
-    if not (ds == 1 and not (ts % 8 or hs % 8 or p % 16) and ts >= out.shape[2] and (hs >= out.shape[2] or
-                                                                                     out.shape[1] == 1)):
+    T, H, D = out.shape
+    # (rows lie token by token or head by head: others would overwrite each other)
+    if not (ds == 1 and not (ts % 8 or hs % 8 or p % 16) and ts >= D and (
+            H == 1 or hs >= D and (ts >= (H - 1) * hs + D or hs >= (T - 1) * ts + D))):
         raise RuntimeError(f"{fn}: out must have contiguous 16-byte aligned rows that do not overlap")
     return out, p, ts, hs
 

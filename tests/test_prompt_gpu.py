@@ -114,6 +114,28 @@ def test_token_strides_past_the_kernels_range():
         assert torch.equal(memopt_C.prompt_attention(*far, cu_of(lens)), want)
 
 
+def test_outputs_whose_rows_overlap_are_refused():
+    """Every (token, head) row has a place of its own in ``out``, in whichever order tokens and heads lie."""
+    lens = [9, 11]
+    q, k, v = make(20, 4, 2, 64, torch.float16, 9)
+    want = memopt_C.prompt_attention(q, k, v, cu_of(lens))
+    for strides in ((256, 64), (64, 1280), (512, 128), (72, 1440), (320, 80), (64, 1288), (256, 64 * 20 * 4)):
+        out = torch.empty(2 ** 15, dtype=q.dtype, device=dev()).as_strided(q.shape, (*strides, 1))
+        assert torch.equal(memopt_C.prompt_attention(q, k, v, cu_of(lens), out=out), want)
+    for strides in ((64, 64), (64, 128), (128, 64), (248, 64), (64, 1272), (192, 128), (64, 0)):
+        out = torch.empty(2 ** 15, dtype=q.dtype, device=dev()).as_strided(q.shape, (*strides, 1))
+        with pytest.raises(RuntimeError, match="overlap"):
+            memopt_C.prompt_attention(q, k, v, cu_of(lens), out=out)
+    one = torch.empty(2 ** 12, dtype=q.dtype, device=dev())
+    for shape, strides in (((1, 4, 64), (64, 64)), ((20, 1, 64), (64, 8)), ((1, 1, 64), (64, 0))):
+        t, h, _ = shape
+        n = [t]
+        a, b, c = q[:t, :h].contiguous(), k[:t, :1].contiguous(), v[:t, :1].contiguous()
+        out = one.as_strided(shape, (*strides, 1))
+        assert torch.equal(memopt_C.prompt_attention(a, b, c, cu_of(n), out=out),
+                           memopt_C.prompt_attention(a, b, c, cu_of(n)))
+
+
 def test_rows_of_no_sequence_stay_as_they_are():
     """Padding before, between (none can be) and behind the sequences is neither read nor written."""
     lens, first, T = [40, 100], 7, 160
