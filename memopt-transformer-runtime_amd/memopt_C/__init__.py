@@ -1025,7 +1025,8 @@ class BatchStep:
     """What ``advance_batch`` writes (int32, contiguous, on one device):
     ``context_lens`` ``[B]``, ``free_span`` ``[2]``, ``cu_seqlens`` ``[B +
     1]``, ``slots`` and ``positions`` ``[rows]``, ``status`` ``[B]``. The
-    tensors are checked here once, and kept."""
+    tensors are checked here once, and kept: another set is another step
+    (``replace``)."""
 
     FIELDS = ("context_lens", "free_span", "cu_seqlens", "slots", "positions", "status")
     __slots__ = FIELDS + ("device", "_args")
@@ -1033,15 +1034,19 @@ class BatchStep:
     def __init__(self, context_lens, free_span, cu_seqlens, slots, positions, status):
         fn = "advance_batch"
         tensors = (context_lens, free_span, cu_seqlens, slots, positions, status)
-        self.device = getattr(context_lens, "device", None)
+        keep = super().__setattr__
+        keep("device", getattr(context_lens, "device", None))
         _require(getattr(context_lens, "is_cuda", False), "advance_batch: context_lens must be a CUDA tensor")
         _device_tensors(fn, self.device, self.FIELDS, *tensors)
         _require(context_lens.dim() == 1 and slots.dim() == 1, "advance_batch: context_lens and slots must be 1-D")
         B, rows = context_lens.shape[0], slots.shape[0]
         for n, t, k in zip(self.FIELDS, tensors, (B, 2, B + 1, rows, rows, B)):
             _int32(fn, t, n, (k,))
-            setattr(self, n, t)
-        self._args = tuple(t.data_ptr() for t in tensors)
+            keep(n, t)
+        keep("_args", tuple(t.data_ptr() for t in tensors))
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"BatchStep: {name} cannot be assigned; replace({name}=...) gives another step")
 
     def replace(self, **tensors) -> "BatchStep":
         """The same buffers with some of them exchanged."""

@@ -158,3 +158,18 @@ def test_refusals():
             memopt_C.advance_batch_buffers(3, 5, dev()).replace(**{field: t})
     with pytest.raises(TypeError):
         memopt_C.advance_batch_buffers(3, 5, dev()).replace(rows=z(5))
+
+
+def test_a_step_s_tensors_are_exchanged_by_replace_alone():
+    """The addresses are taken when the step is made, so a field that could be assigned would not be written to."""
+    step = memopt_C.advance_batch_buffers(3, 8, dev())
+    for name in memopt_C.BatchStep.FIELDS + ("device",):
+        with pytest.raises(AttributeError):
+            setattr(step, name, getattr(step, name))
+    slots = torch.full((8,), 7, dtype=torch.int32, device=dev())
+    other = step.replace(slots=slots)
+    assert other.slots is slots and step.slots is not slots and other.cu_seqlens is step.cu_seqlens
+    i32 = dict(dtype=torch.int32, device=dev())
+    memopt_C.advance_batch(torch.tensor([2, 0, 1], **i32), torch.zeros(3, **i32), torch.full((3, 2), -1, **i32),
+                           torch.arange(4, **i32), torch.tensor([0, 4], **i32), 16, out=other)
+    assert slots.tolist() == [0, 1, 16, -1, -1, -1, -1, -1]
