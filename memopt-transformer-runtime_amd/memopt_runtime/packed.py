@@ -63,7 +63,10 @@ class PackedBatch:
         self.tables = torch.full((num_requests, pages_needed(max_tokens, block_size)), -1, dtype=torch.int32, device=dev)
         # context_lens and free_span are advanced in place.
         self.state = memopt_C.advance_batch_buffers(num_requests, num_rows, dev)
-        self.state.context_lens.zero_()
+        for t in (self.state.context_lens, self.state.cu_seqlens, self.state.status):
+            t.zero_()
+        for t in (self.state.slots, self.state.positions):
+            t.fill_(-1)
         self.state.free_span.copy_(torch.tensor([0, num_blocks], dtype=torch.int32))
 
     @property

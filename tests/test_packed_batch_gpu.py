@@ -280,6 +280,23 @@ def test_grouped_heads_through_the_runtime(fmt, window, sinks):
         forward.attend([0, 1], rand(2, 1, 3, D))
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_attend_before_the_first_advance(fmt):
+    """No request has rows yet: nothing is written, whatever the step's memory held."""
+    dirty = [torch.ones(n, dtype=torch.int32, device=dev()) for n in (3, 2, 4, 8, 8, 3) * 4]
+    del dirty
+    batch = R().PackedBatch(4, 1, 64, 3, 32, 8, kv_format=fmt)
+    assert batch.state.cu_seqlens.tolist() == [0] * 4 and batch.state.context_lens.tolist() == [0] * 3
+    assert batch.state.slots.tolist() == [-1] * 8 and batch.state.positions.tolist() == [-1] * 8
+    pages = [x.clone() for x in (memopt_C.get_key_pool(), memopt_C.get_value_pool())]
+    q = torch.randn((8, 4, 64), device=dev()).half()
+    out = torch.full_like(q, 7.0)
+    for prompts in (False, True):
+        batch.attend(q, q[:, :1], q[:, 1:2], prompts=prompts, out=out)
+    assert bool((out == 7).all())
+    assert all(torch.equal(a, b) for a, b in zip(pages, (memopt_C.get_key_pool(), memopt_C.get_value_pool())))
+
+
 def test_refusals():
     for match, kw in [("2\\^31", dict(num_blocks=2 ** 28)), ("2\\^31", dict(num_blocks=0)), ("4096", dict(num_requests=4097)),
                       ("4096", dict(num_requests=0)), ("positive", dict(max_tokens=0)), ("positive", dict(num_rows=0)),
