@@ -45,7 +45,7 @@ __all__ = [
     "get_key_pool", "get_value_pool", "get_pool_scales", "get_int4_pages", "int4_layout", "free_blocks_count",
     "write_cache", "evict_cache", "evict_tokens", "free_evicted_blocks",
     "dynamic_sparse_attention", "PreparedAttention", "quantize_kv_cache_int4", "dequantize_kv_cache_int4",
-    "prompt_attention", "packed_attention", "PreparedPackedAttention", "advance_batch", "advance_batch_buffers",
+    "prompt_attention", "packed_attention", "packed_workspace_bytes", "PreparedPackedAttention", "advance_batch", "advance_batch_buffers",
     "BatchStep", "library_path",
 ]
 
@@ -905,6 +905,21 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
         raise RuntimeError(f"{fn}: sizes must fit 32 bits") from None
     _check(_c_prompt_bytes(d, torch._C._cuda_getCurrentRawStream(index)))
     return out
+
+
+def packed_workspace_bytes(tokens: int, batch: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                           max_query_len: int, max_seq_len: int, max_blocks_per_seq: int, window_size: int = -1, *,
+                           num_sink_tokens: int = 0, block_size: int = 16, kv_format: str = "int4") -> int:
+    """Device workspace bytes a ``packed_attention`` call of these sizes
+    allocates (``memopt_packed_workspace_size``); "int4" counts page buffers."""
+    fmt = _FORMATS.get(kv_format)
+    _require(fmt is not None, f"packed_workspace_bytes: kv_format must be one of {sorted(_FORMATS)}")
+    d = PackedDesc(None, None, tokens, batch, num_heads, num_kv_heads, head_dim, 0, 0, 0, 0, fmt, None, None, block_size,
+                   1, None, max_blocks_per_seq, None, None, _count32(max_query_len), _count32(max_seq_len),
+                   _count32(window_size), _count32(num_sink_tokens))
+    need, zeroed = _i64(), _i64()
+    _check(_c_packed_ws(ctypes.byref(d), ctypes.byref(need), ctypes.byref(zeroed)))
+    return need.value
 
 
 def _packed_desc(query, key_cache, value_cache, block_tables, context_lens, cu_seqlens, max_query_len, max_seq_len,

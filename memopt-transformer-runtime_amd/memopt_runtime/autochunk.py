@@ -22,26 +22,43 @@ import memopt_C
 from .kv_cache import PagedKVCache, pages_needed
 
 STAGED_BYTES_PER_TOKEN_HEAD_DIM = 4  # fp16 K + fp16 V of one (token, head, dim) in the staging workspace
+STAGED_BYTES = 2 << 30  # of such copies packed_attention makes at most this much
 
 
-def chunk_call_bytes(chunk: int, context_tokens: int, num_heads: int, head_dim: int, window: int = -1) -> int:
+def chunk_call_bytes(chunk: int, context_tokens: int, num_heads: int, head_dim: int, window: int = -1,
+                     num_kv_heads: Optional[int] = None, *, num_sink_tokens: int = 0, block_size: int = 16,
+                     kv_format: str = "int4") -> int:
     """Device bytes of one chunk call over ``chunk`` queries at the end of
     ``context_tokens``: fp16 queries and outputs (2 * C * H * D * 2) and the
     staged fp16 K/V of the keys the call can see (min(context, C + window)
-    tokens; the whole context without a window), 4 * H * D bytes each."""
+    tokens; the whole context without a window), 4 * H * D bytes each.
+
+    With fewer key heads (``num_kv_heads``), queries, outputs and the most
+    workspace that ``packed_attention`` asks for over contexts up to
+    ``context_tokens``; the arguments behind it count for that alone."""
     hd = num_heads * head_dim
+    if num_kv_heads is not None and num_kv_heads != num_heads:
+        # (staged copies that would pass the operator's limit are left out, so a shorter context can take more)
+        n = min(context_tokens, STAGED_BYTES // (STAGED_BYTES_PER_TOKEN_HEAD_DIM * num_kv_heads * head_dim))
+        return 2 * chunk * hd * 2 + max(memopt_C.packed_workspace_bytes(
+            chunk, 1, num_heads, num_kv_heads, head_dim, chunk, m, pages_needed(m, block_size), window,
+            num_sink_tokens=num_sink_tokens, block_size=block_size, kv_format=kv_format)
+            for m in {max(1, n), max(1, context_tokens)})
     seen = min(context_tokens, chunk + window) if window > 0 else context_tokens
     return 2 * chunk * hd * 2 + STAGED_BYTES_PER_TOKEN_HEAD_DIM * hd * seen
 
 
 def chunk_tokens_for_budget(budget_bytes: int, context_tokens: int, num_heads: int, head_dim: int,
-                            window: int = -1, multiple: int = 128, minimum: int = 16) -> int:
+                            window: int = -1, multiple: int = 128, minimum: int = 16,
+                            num_kv_heads: Optional[int] = None, **packed) -> int:
     """Largest chunk (a multiple of ``multiple``, at most the context) whose
-    :func:`chunk_call_bytes` fit ``budget_bytes``; ``minimum`` if none does."""
+    :func:`chunk_call_bytes` fit ``budget_bytes``; ``minimum`` if none does.
+    ``num_kv_heads`` and what follows are those of ``chunk_call_bytes``."""
     lo, hi = 0, max(0, context_tokens // multiple)
     while lo < hi:  # chunk_call_bytes grows with the chunk: largest feasible count of `multiple`s
         mid = (lo + hi + 1) // 2
-        if chunk_call_bytes(mid * multiple, context_tokens, num_heads, head_dim, window) <= budget_bytes:
+        if chunk_call_bytes(mid * multiple, context_tokens, num_heads, head_dim, window, num_kv_heads,
+                            **packed) <= budget_bytes:
             lo = mid
         else:
             hi = mid - 1
@@ -62,7 +79,9 @@ def autochunk_prefill(cache: PagedKVCache, seq_id: int, query: torch.Tensor, key
     S, H, D = query.shape
     start = cache.length(seq_id)
     if chunk_tokens is None:
-        chunk_tokens = (chunk_tokens_for_budget(budget_bytes, start + S, H, D, window_size)
+        chunk_tokens = (chunk_tokens_for_budget(budget_bytes, start + S, H, D, window_size, num_kv_heads=cache.num_heads,
+                                                num_sink_tokens=num_sink_tokens, block_size=cache.block_size,
+                                                kv_format=cache.kv_format)
                         if budget_bytes is not None else S)
     if chunk_tokens <= 0:
         raise RuntimeError("autochunk_prefill: chunk_tokens must be positive")

@@ -281,6 +281,25 @@ def test_grouped_heads_through_the_runtime(fmt, window, sinks):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+def test_grouped_prefill_stays_within_its_budget(fmt):
+    """Memory that a chunk call takes beside the prompt's own tensors, and its queries and outputs, fit the budget."""
+    Hq, Hk, D, S, budget = 32, 8, 128, 512, 20 << 20
+    cache = R().PagedKVCache(S // 16 + 2, Hk, D, kv_format=fmt)
+    cache.add_sequence(0)
+    q, k, v = (torch.randn((S, h, D), device=dev()).half() for h in (Hq, Hk, Hk))
+    chunk = R().chunk_tokens_for_budget(budget, S, Hq, D, num_kv_heads=Hk, kv_format=fmt)
+    assert chunk < S
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = R().autochunk_prefill(cache, 0, q, k, v, budget_bytes=budget)
+    taken = torch.cuda.max_memory_allocated() - before - out.numel() * 2
+    assert taken + 4 * chunk * Hq * D <= budget + 65536  # (the index tensors)
+    first = S - 40
+    compare(out[first:], q[first:], k.cpu().numpy(), v.cpu().numpy(), first, fmt, -1, 0, "the last rows")
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_attend_before_the_first_advance(fmt):
     """No request has rows yet: nothing is written, whatever the step's memory held."""
     dirty = [torch.ones(n, dtype=torch.int32, device=dev()) for n in (3, 2, 4, 8, 8, 3) * 4]

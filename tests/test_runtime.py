@@ -36,6 +36,32 @@ def test_chunk_size_fits_budget():
     assert R.chunk_tokens_for_budget(1 << 40, 16384, H, D) == 16384  # whole prompt
 
 
+@pytest.mark.parametrize("Hq,Hk,D", [(32, 8, 128), (8, 2, 64), (64, 1, 128)])
+@pytest.mark.parametrize("fmt", ["int4", "fp16"])
+@pytest.mark.parametrize("window,sinks", [(-1, 0), (1024, 4)])
+def test_chunk_size_of_grouped_heads_fits_budget(Hq, Hk, D, fmt, window, sinks):
+    """Every call of a prefill in chunks of the chosen size: queries, outputs and the workspace the call asks for."""
+    import memopt_C
+
+    def call(chunk, n):
+        pages = R.pages_needed(n, 16)
+        return 4 * chunk * Hq * D + memopt_C.packed_workspace_bytes(chunk, 1, Hq, Hk, D, chunk, n, pages, window,
+                                                                     num_sink_tokens=sinks, kv_format=fmt)
+
+    kw = dict(num_kv_heads=Hk, kv_format=fmt, num_sink_tokens=sinks)
+    for S in (512, 16384, 10 ** 6):
+        for budget in (1 << 20, 20 << 20, 64 << 20, 512 << 20, 3 << 30):
+            c = R.chunk_tokens_for_budget(budget, S, Hq, D, window, **kw)
+            starts = list(range(0, S, c))
+            if len(starts) > 100:  # the first and last, and some between
+                starts = starts[:30] + starts[30:-30:len(starts) // 40] + starts[-30:]
+            most = max(call(min(c, S - s), min(S, s + c)) for s in starts)
+            assert most <= R.chunk_call_bytes(c, S, Hq, D, window, **kw)
+            if c != 16:
+                assert most <= budget and c % 128 == 0
+    assert R.chunk_call_bytes(256, 4096, 8, 64, num_kv_heads=8) == R.chunk_call_bytes(256, 4096, 8, 64)
+
+
 class _Scheduler:
     """MemoryScheduler's policy fields behind its non-reentrant lock
     (src/memopt/scheduler.py:151-172, :212-233)."""
