@@ -824,8 +824,8 @@ extern "C" int memopt_prompt_attention(const memopt_prompt_desc *desc, void *str
   p.sinks = std::max(0, d.num_sink_tokens);
   p.qk_scale_log2 = 1.4426950408889634f / sqrtf((float)d.head_dim);
   MEMOPT_REQUIRE(d.tokens <= 1 << 30 && (int64_t)d.tokens * d.num_heads <= INT32_MAX - 255 &&
-                     most_tiles(d.tokens, d.batch, p.G) * d.num_kv_heads < (1LL << 31),
-                 MEMOPT_ERR_UNSUPPORTED, "prompt_attention: too many query rows");
+                     most_tiles(d.tokens, d.batch, p.G) * d.num_kv_heads < (1LL << 24),
+                 MEMOPT_ERR_UNSUPPORTED, "prompt_attention: too many query rows");  // (a launch holds 2^32 - 1 threads)
   hipStream_t s = (hipStream_t)stream;
   if (d.dtype == MEMOPT_FP16) {
     if (d.head_dim == 128) launch_prompt<Fp16, 128>(p, s);

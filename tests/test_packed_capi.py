@@ -41,6 +41,13 @@ def test_prompt_refusals(C, text, code, change):
     refused(C, prompt(C, **change), code, text)
 
 
+def test_prompt_launches_of_too_many_threads(C):
+    """Tiles are counted as if every sequence but the empty ones left one part full: 2^24 tiles of 256 threads are more
+    than a launch holds."""
+    refused(C, prompt(C, tokens=2 ** 20, batch=2 ** 20, num_heads=32, num_kv_heads=32), UNSUPPORTED, "too many")
+    refused(C, prompt(C, tokens=2 ** 19, batch=2 ** 20, num_heads=32, num_kv_heads=32), UNSUPPORTED, "too many")
+
+
 def test_prompt_null_and_empty(C):
     refused(C, C._c_prompt(None, None), INVALID, "null")
     assert prompt(C, tokens=0) == OK and prompt(C, batch=0, query_starts=None) == OK
