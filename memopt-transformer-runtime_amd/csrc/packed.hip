@@ -83,7 +83,8 @@ struct PackedParams {
   Staged st;                     // sequences that attend from a staged copy instead
 };
 
-// Workgroups per key head, so partial sums of a block, at most.
+// Workgroups per key head, so partial sums of a block, at most. (Reached with one
+// or two key heads on 256 CUs, where it leaves room for more workgroups.)
 static constexpr int kMaxParts = 256;
 
 // What rows at positions pos_lo .. pos_hi of a context see, in 16-token
@@ -206,7 +207,8 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QN) / 4) void packed_ker
   // that what a request gets does not hang on its neighbours. (131072 tokens, 5
   // rows: 33.1 us without, 34.2 in columns, 37.7 as instructions; 8 sequences of
   // 4096 tokens and 64 rows 34.3 without, 38.8 with, of 256 rows 73 and 89: there
-  // errors average out, to 3.0e-4.)
+  // errors average out, to 3.0e-4. 12 single tokens of 4 rows beside 4 chunks of
+  // 512 tokens: 2.9e-4 and 18.2 us without, 2.1e-4 and 20.4 with.)
   constexpr bool HALVES = QN == 8;
   constexpr int OS = D + 4;               // row stride of s_o: 16 rows of D floats would share a bank
   // Pages stream through a ring of raw blocks per wave (see copy_step), which
@@ -964,8 +966,9 @@ __global__ __launch_bounds__(64 * NW, NW * resident(NW, QN) / 4) void packed_ker
 // takes tiles i, i + gridDim, ..., each wave 16 tokens of them, which lie in
 // one page. A wave reads a block of a page as it is (lane l: the 16 dims (D =
 // 64: 8) of tokens p = l / 8 and p + 8 that start at D / 8 * (l % 8)) and writes
-// V as fp16((code - 8) * scale), one rounding, as in the operands above, and K
-// as codes with their factors.
+// V as fp16((code - 8) * scale), one rounding that the kernel above does not
+// make (there V enters as codes, and the weights carry its scales), and K as
+// codes with their factors.
 template <int D, int FMT>
 __global__ __launch_bounds__(256) void stage_kernel(const PackedParams p, const int32_t *__restrict__ starts,
                                                     const int32_t *__restrict__ ctxs,
@@ -1129,7 +1132,7 @@ static int32_t staged_rows(int64_t rows) {
   const int64_t per_cu = rows / (128LL * compute_units());
   return per_cu >= 2 ? 512 : per_cu >= 1 ? 1024 : INT32_MAX;
 }
-// Of staged copies at most this much.
+// Of staged copies at most this much (a prefill budget counts on it: autochunk.py).
 static constexpr int64_t kStagedBytes = 2LL << 30;
 
 static PackedPlan packed_plan(const memopt_packed_desc &d) {
