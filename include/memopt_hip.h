@@ -395,6 +395,36 @@ typedef struct memopt_advance_desc {
 } memopt_advance_desc;
 int memopt_advance_batch(const memopt_advance_desc *desc, void *stream);
 
+/* Attention weights per cached token: out[b, h, j] = scores[b, h, j] + the sum
+ * of the softmax weights that sequence b's query rows, in the num_heads /
+ * num_kv_heads heads of key head h, give token j; the rows, masks and caches
+ * are memopt_packed_attention's, and a row that sees nothing adds nothing. The
+ * order of all sums is fixed. Tokens from max_seq_len on are not looked at;
+ * weights of tokens from scores_len on are not written. `scores` may be null
+ * (zeros) or `out` itself. Query rows: 31 token strides and a group's head
+ * strides together less than 2^29 elements. */
+typedef struct memopt_scores_desc {
+  const void *query;                 /* fp16 [tokens, num_heads, head_dim]     */
+  const float *scores;               /* [batch, num_kv_heads, scores_len]      */
+  float *out;                        /* the same                               */
+  int32_t tokens, batch, num_heads, num_kv_heads, head_dim;
+  int64_t q_token_stride, q_head_stride;
+  int32_t kv_format;                 /* MEMOPT_KV_FP16 / MEMOPT_KV_INT4        */
+  const void *key_cache;             /* fp16 keys, or INT4 pages               */
+  int32_t block_size;
+  int64_t num_kv_blocks;
+  const int32_t *block_tables;       /* [batch, max_blocks_per_seq]            */
+  int32_t max_blocks_per_seq;
+  const int32_t *context_lens;       /* [batch]                                */
+  const int32_t *query_starts;       /* [batch + 1]                            */
+  int32_t max_query_len, max_seq_len, window_size, num_sink_tokens, scores_len;
+  void *workspace;                   /* >= memopt_scores_workspace_size bytes, 16-byte aligned, any content */
+  int64_t workspace_bytes;
+} memopt_scores_desc;
+/* Calls sharing a workspace must not overlap. */
+int memopt_scores_workspace_size(const memopt_scores_desc *desc, int64_t *bytes);
+int memopt_attention_scores(const memopt_scores_desc *desc, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

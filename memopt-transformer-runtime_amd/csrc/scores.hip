@@ -1,0 +1,613 @@
+// scores.hip — attention weights added up per cached token, the scores that
+// eviction goes by (gfx950 matrix cores).
+//
+// For sequence b, key head h and token j, over the sequence's query rows r and
+// the G query heads g of the group:
+//   out[b,h,j] = scores[b,h,j] + sum_{r,g} exp(q_rg . k_hj / sqrt(D) - lse_rg),
+//   lse_rg = log sum_{j' visible} exp(q_rg . k_hj' / sqrt(D))
+// with the masks of packed_attention. A weight needs its row's sum over all
+// keys, so there are two passes with a sum between. In both, keys stay in
+// registers (a wave's 64 as matrix operands, unpacked once) and query rows
+// stream past, so that a key's total is one lane's sum, in a fixed order, and
+// needs no atomics.
+//
+// INT4 keys enter the products as exact codes (code - 8, which fp16 holds) and
+// the sums of each 64-dim group are scaled in 32 bits: nothing is rounded to
+// fewer bits on the way from the cache to the result.
+#include <algorithm>
+#include <cmath>
+
+#include "lds_dma.hpp"
+#include "page_format.hpp"
+#include "tiles.hpp"
+
+namespace memopt {
+
+typedef _Float16 f16x8s_t __attribute__((ext_vector_type(8)));
+
+struct ScoresParams {
+  const uint16_t *q;
+  int64_t q_ts, q_hs;
+  const uint8_t *k;
+  int64_t k_ps, k_hs, k_ts;  // bytes: page, head, token (fp16)
+  const int32_t *bt, *ctx, *starts;
+  int64_t nb;
+  const float *scores;  // null: zeros
+  float *out;
+  int32_t T, B, Hk, G, M, bs, W, sinks, L;
+  int32_t max_keys, max_rows;  // tokens that are looked at; rows of a sequence and key head
+  int32_t kts;                 // key tiles of kTileKeys
+  Divisor by_g, by_chunks;     // by_chunks: 16-token chunks of a page
+  float qk_scale_log2;
+  float2 *ml;    // few rows: [B][Hk][kts][max_rows]; chunks: [Hk][kts][T G]
+  float *probs;  // few rows: [B][Hk][max_rows][kts * kTileKeys]
+  float *lse;    // chunks: [Hk][T G]
+};
+
+static constexpr int kTileKeys = 256;  // keys of a workgroup: 64 per wave
+static constexpr int kFewRows = 16;
+
+// A sequence as one key head sees it.
+struct ScoredSeq {
+  int32_t start, rows, pos0, len;  // first token row; rows; position of the first; keys
+};
+__device__ __forceinline__ ScoredSeq scored_seq(const ScoresParams &p, int32_t b) {
+  const Rows r = rows_of(p.starts, p.T, b);
+  const int32_t ctx = p.ctx[b];
+  return {r.start, min(r.n, p.max_rows / p.G) * p.G, ctx - r.n, max(0, min(ctx, p.max_keys))};
+}
+// Whether a query at position pos can see a key of [k0, k1).
+__device__ __forceinline__ bool meets(const ScoresParams &p, int32_t pos, int32_t k0, int32_t k1) {
+  return k0 <= pos && (k0 < p.sinks || k1 > pos - p.W + 1);
+}
+// Token range [lo, hi) of the sequence's queries that can see a key of [k0, k1).
+__device__ __forceinline__ void queries_of(const ScoresParams &p, const ScoredSeq &s, int32_t n, int32_t k0, int32_t k1,
+                                           int32_t &lo, int32_t &hi) {
+  lo = min(max(k0 - s.pos0, 0), n);
+  hi = k0 < p.sinks ? n : (int32_t)min(max((int64_t)k1 + p.W - 1 - s.pos0, (int64_t)0), (int64_t)n);
+  if (k0 >= s.len) hi = lo;
+}
+
+__device__ __forceinline__ float max_over_quarters(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return both_halves_max(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+}
+__device__ __forceinline__ float sum_over_quarters(float v) { return xor32_sum(xor16_sum(v)); }
+
+// Eight codes less 8 as exact fp16 values, in the order of their dims.
+__device__ __forceinline__ u32x4p_t codes_to_half(uint32_t w) {
+  const uint32_t lo = w & 0x0F0F0F0Fu, hi = (w >> 4) & 0x0F0F0F0Fu;
+  u32x4p_t r;
+  // bytes (code 2i, 0, code 2i + 1, 0); 1024 + code is 0x6400 | code in fp16
+  constexpr uint32_t sel[4] = {0x0C000C04u, 0x0C010C05u, 0x0C020C06u, 0x0C030C07u};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = __builtin_amdgcn_perm(lo, hi, sel[i]) | 0x64006400u;
+    r[i] = as_u32(as_half2(x) - half2_t{(half_t)1032.0f, (half_t)1032.0f});
+  }
+  return r;
+}
+
+// 64 keys of one head as operands of v_mfma_f32_16x16x32: page g's keys are
+// the rows of operand a[g][.]; lane l holds key l % 16 and of every 64 dims
+// the 16 from 16 (l / 16) on, in two operands. Products come out with the
+// query row in the lane's column l % 16 and keys 4 (l / 16) + r in register r.
+template <int FMT, int D>
+struct Keys {
+  static constexpr int NCH = D / 32, NG = D / 64;
+  static constexpr bool CODES = FMT == MEMOPT_KV_INT4;
+  u32x4p_t a[4][NCH];
+  f32x4p_t f[CODES ? 4 : 1][CODES ? NG : 1];  // factors of the register's keys: scale times qk_scale_log2
+  uint32_t linked;                            // bit g: page g is there
+
+  __device__ __forceinline__ void load(const ScoresParams &p, int32_t b, int32_t h, int32_t key0, int32_t len) {
+    const int lane = threadIdx.x & 63, t = lane & 15, kq = lane >> 4;
+    linked = 0;
+    const uint8_t *at[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int32_t key = key0 + 16 * g;
+      int32_t page = -1, first = 0;
+      if (key < len) {
+        const int32_t c = key >> 4, e = CODES ? c : p.by_chunks(c);
+        first = CODES ? 0 : 16 * (c - e * (int32_t)p.by_chunks.d);
+        page = __builtin_amdgcn_readfirstlane(p.bt[(int64_t)b * p.M + e]);
+      }
+      const bool ok = page >= 0 && page < p.nb;
+      linked |= (ok ? 1u : 0u) << g;
+      at[g] = ok ? p.k + (int64_t)page * p.k_ps + h * p.k_hs + first * p.k_ts : nullptr;
+    }
+    constexpr int BPL = D / 8;
+    uint32_t w[4][NCH];
+    uint4 sc[4][NG];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      if (!((linked >> g) & 1)) {
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+          if constexpr (CODES) w[g][c] = 0x88888888u;
+          else a[g][c] = (u32x4p_t){};
+        }
+        if constexpr (CODES)
+#pragma unroll
+          for (int i = 0; i < NG; ++i) sc[g][i] = uint4{0, 0, 0, 0};
+      } else if constexpr (CODES) {
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          if constexpr (D == 128) {
+            const uint2 x = *reinterpret_cast<const uint2 *>(at[g] + (8 * (t & 7) + 4 * i + kq) * BPL + (t >> 3) * 8);
+            w[g][2 * i] = x.x;
+            w[g][2 * i + 1] = x.y;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              w[g][j] = *reinterpret_cast<const uint32_t *>(at[g] + (8 * (t & 7) + 2 * kq + j) * BPL + (t >> 3) * 4);
+          }
+          sc[g][i] = *reinterpret_cast<const uint4 *>(at[g] + 16 * D + 32 * i + 16 * (kq & 1));
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < NCH; ++c)
+          a[g][c] = *reinterpret_cast<const u32x4p_t *>(at[g] + t * p.k_ts + 2 * (64 * (c >> 1) + 16 * kq + 8 * (c & 1)));
+      }
+    }
+    if constexpr (CODES) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) a[g][c] = codes_to_half(w[g][c]);
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          const uint32_t s[4] = {sc[g][i].x, sc[g][i].y, sc[g][i].z, sc[g][i].w};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const half2_t pair = as_half2(s[r]);
+            f[g][i][r] = (float)(kq >> 1 ? pair.y : pair.x) * p.qk_scale_log2;
+          }
+        }
+      }
+    }
+  }
+  // Scores in log2 units of page g's keys against 16 query rows.
+  __device__ __forceinline__ f32x4p_t scores(int g, const u32x4p_t (&q)[NCH], float scale) const {
+    f32x4p_t c[NG];
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      c[i] = (f32x4p_t){};
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        f32x4p_t &acc = CODES ? c[i] : c[0];
+        if (!CODES && i == 0 && j == 0) acc = (f32x4p_t){};
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8s_t, a[g][2 * i + j]),
+                                                     __builtin_bit_cast(f16x8s_t, q[2 * i + j]), acc, 0, 0, 0);
+      }
+    }
+    f32x4p_t x;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if constexpr (!CODES) x[r] = c[0][r] * scale;
+      else if constexpr (NG == 1) x[r] = c[0][r] * f[g][0][r];
+      else x[r] = fmaf(c[1][r], f[g][1][r], c[0][r] * f[g][0][r]);
+    }
+    return x;
+  }
+};
+
+// Hides what a row at position `pos` does not see of page g's keys (key: the
+// lane's first); ok: the row exists.
+__device__ __forceinline__ f32x4p_t hide(const ScoresParams &p, f32x4p_t x, int32_t key, int32_t pos, int32_t len, bool ok) {
+  const int32_t last = ok ? min(pos, len - 1) : -1;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int32_t j = key + r;
+    x[r] = (j <= last) & ((j > pos - p.W) | (j < p.sinks)) ? x[r] : -INFINITY;
+  }
+  return x;
+}
+
+// ---------------------------------------------------------------------------
+// Few rows (decode): up to kFewRows rows per sequence and key head
+// ---------------------------------------------------------------------------
+// The weights relative to the tile's maximum are kept instead of reading the
+// keys again: 8 bytes per row and key against D / 2 + 2 D / 64 of INT4.
+
+template <int FMT, int D>
+__global__ __launch_bounds__(256) void few_rows_kernel(const ScoresParams p) {
+  using K = Keys<FMT, D>;
+  __shared__ float s_m[4][kFewRows], s_l[4][kFewRows];
+  const int32_t h = (int32_t)(blockIdx.x % p.Hk), kt = (int32_t)(blockIdx.x / p.Hk), b = blockIdx.y;
+  const int lane = threadIdx.x & 63, n = lane & 15, kq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const ScoredSeq s = scored_seq(p, b);
+  int32_t lo, hi;
+  queries_of(p, s, s.rows / p.G, kt * kTileKeys, (kt + 1) * kTileKeys, lo, hi);
+  if (hi <= lo) return;
+  const int32_t key0 = kt * kTileKeys + 64 * wave;
+  K keys;
+  keys.load(p, b, h, key0, s.len);
+  const bool ok = n < s.rows;
+  const int32_t tok = p.by_g(min(n, s.rows - 1)), pos = s.pos0 + tok;
+  u32x4p_t q[K::NCH];
+  const uint16_t *src = p.q + (int64_t)(s.start + tok) * p.q_ts + ((int64_t)h * p.G + min(n, s.rows - 1) - tok * p.G) * p.q_hs;
+#pragma unroll
+  for (int c = 0; c < K::NCH; ++c)
+    q[c] = *reinterpret_cast<const u32x4p_t *>(src + 64 * (c >> 1) + 16 * kq + 8 * (c & 1));
+  f32x4p_t x[4];
+  float m = -INFINITY;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    x[g] = hide(p, keys.scores(g, q, p.qk_scale_log2), key0 + 16 * g + 4 * kq, pos, s.len, ok && ((keys.linked >> g) & 1));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) m = fmaxf(m, x[g][r]);
+  }
+  m = max_over_quarters(m);
+  if (kq == 0) s_m[wave][n] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_m[0][n], s_m[1][n]), fmaxf(s_m[2][n], s_m[3][n]));
+  const float ref = m == -INFINITY ? 0.0f : m;
+  const int64_t unit = (int64_t)b * p.Hk + h;
+  float l = 0.0f;
+  float *dst = p.probs + (unit * p.max_rows + n) * ((int64_t)p.kts * kTileKeys) + key0 + 4 * kq;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      x[g][r] = fast_exp2(x[g][r] - ref);
+      l += x[g][r];
+    }
+    if (ok) *reinterpret_cast<f32x4p_t *>(dst + 16 * g) = x[g];
+  }
+  l = sum_over_quarters(l);
+  if (kq == 0) s_l[wave][n] = l;
+  __syncthreads();
+  if (threadIdx.x < (unsigned)s.rows)
+    p.ml[(unit * p.kts + kt) * p.max_rows + n] = float2{m, (s_l[0][n] + s_l[1][n]) + (s_l[2][n] + s_l[3][n])};
+}
+
+// out = scores + the rows' weights: a thread per key. Also the whole of a
+// call without rows.
+__global__ __launch_bounds__(256) void finish_kernel(const ScoresParams p) {
+  __shared__ float s_f[kFewRows];
+  const int32_t h = (int32_t)(blockIdx.x % p.Hk), kt = (int32_t)(blockIdx.x / p.Hk), b = blockIdx.y;
+  const ScoredSeq s = scored_seq(p, b);
+  const int64_t unit = (int64_t)b * p.Hk + h;
+  const int32_t j = kt * kTileKeys + (int32_t)threadIdx.x;
+  const float before = p.scores && j < p.L ? p.scores[unit * p.L + j] : 0.0f;
+  int32_t lo, hi;
+  queries_of(p, s, s.rows / p.G, kt * kTileKeys, (kt + 1) * kTileKeys, lo, hi);
+  float w = 0.0f;
+  if (hi > lo) {
+    // Row threadIdx / 16's maximum and sum, by 16 lanes over the key tiles.
+    const int32_t row = threadIdx.x >> 4;
+    float m = -INFINITY, l = 0.0f;
+    if (row < s.rows) {
+      const int32_t tiles = (s.len + kTileKeys - 1) / kTileKeys;
+      for (int32_t t = threadIdx.x & 15; t < tiles; t += 16) {
+        int32_t a, z;
+        queries_of(p, s, s.rows / p.G, t * kTileKeys, (t + 1) * kTileKeys, a, z);
+        if (z <= a) continue;
+        const float2 x = p.ml[(unit * p.kts + t) * p.max_rows + row];
+        const float top = fmaxf(m, x.x);
+        if (top == -INFINITY) continue;
+        l = l * fast_exp2(m - top) + x.y * fast_exp2(x.x - top);
+        m = top;
+      }
+    }
+    float top = fmaxf(m, xor1(m));
+    top = fmaxf(top, xor2(top));
+    top = fmaxf(top, half_mirror(top));
+    top = fmaxf(top, dpp_f32<0x140>(top));
+    l = m == -INFINITY ? 0.0f : l * fast_exp2(m - top);
+    l += xor1(l);
+    l += xor2(l);
+    l += half_mirror(l);
+    l += dpp_f32<0x140>(l);
+    if ((threadIdx.x & 15) == 0 && row < s.rows) {
+      const float here = p.ml[(unit * p.kts + kt) * p.max_rows + row].x;
+      // (a tile without a visible key of this row has the reference 0 and zeros)
+      s_f[row] = l == 0.0f || here == -INFINITY ? 0.0f : fast_exp2(here - top) / l;
+    }
+    __syncthreads();
+    if (j < s.len) {
+      const float *src = p.probs + unit * p.max_rows * ((int64_t)p.kts * kTileKeys) + j;
+      for (int32_t r = 0; r < s.rows; ++r) w = fmaf(src[(int64_t)r * p.kts * kTileKeys], s_f[r], w);
+    }
+  }
+  if (j < p.L) p.out[unit * p.L + j] = before + w;
+}
+
+// ---------------------------------------------------------------------------
+// Chunks: rows stream past the keys twice
+// ---------------------------------------------------------------------------
+
+// SUM = false: every row's maximum and sum over the tile's keys; true: every
+// key's weights, with the rows' lse known, and the result.
+template <int FMT, int D, bool SUM>
+__global__ __launch_bounds__(256, 2) void chunk_rows_kernel(const ScoresParams p) {
+  using K = Keys<FMT, D>;
+  constexpr int NCH = K::NCH, TR = 32, RB = 2 * D, CPR = RB / 16, RPC = 1024 / RB, NC = TR / RPC / 4;
+  __shared__ __attribute__((aligned(16))) uint8_t lds_q[2][TR * RB];
+  __shared__ float2 s_ml[2][4][TR];
+  const int32_t h = (int32_t)(blockIdx.x % p.Hk), kt = (int32_t)(blockIdx.x / p.Hk), b = blockIdx.y;
+  const int lane = threadIdx.x & 63, n = lane & 15, kq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const ScoredSeq s = scored_seq(p, b);
+  const int32_t key0 = kt * kTileKeys + 64 * wave;
+  int32_t lo, hi;
+  queries_of(p, s, s.rows / p.G, kt * kTileKeys, (kt + 1) * kTileKeys, lo, hi);
+  f32x4p_t w[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) w[g] = (f32x4p_t){};
+  if (hi > lo) {
+    K keys;
+    keys.load(p, b, h, key0, s.len);
+    // Tiles of TR rows from the first that sees a key to the last.
+    const int32_t t0 = lo * p.G / TR, t1 = (hi * p.G + TR - 1) / TR;
+    const int64_t row_base = (int64_t)s.start * p.G;
+    auto q_swz = [](int row) { return CPR == 16 ? row & 15 : (row >> 1) & 7; };
+    // Rows past the last are copies of it: their weights are zeros.
+    auto load_q = [&](int32_t t, int buf) __attribute__((always_inline)) {
+      const int32_t tok0 = p.by_g(t * TR);
+      const uint8_t *base = reinterpret_cast<const uint8_t *>(p.q + (int64_t)(s.start + tok0) * p.q_ts + (int64_t)h * p.G * p.q_hs);
+      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)uniform_ptr(base), (short)0, 0x7FFFFFFF, 0x00020000);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int lrow = (wave * NC + c) * RPC + lane / CPR;
+        const int32_t row = min(t * TR + lrow, s.rows - 1), tok = p.by_g(row);
+        const uint32_t off[1] = {(uint32_t)(2 * ((tok - tok0) * (int32_t)p.q_ts + (row - tok * p.G) * (int32_t)p.q_hs) +
+                                            16 * ((lane % CPR) ^ q_swz(lrow)))};
+        lds_dma<0, 1>(rsrc, lds_u32(lds_q[buf]) + (uint32_t)(wave * NC + c) * 1024, off, 0);
+      }
+    };
+    auto load_lse = [&](int32_t t, float (&v)[2]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int32_t row = t * TR + 16 * i + n;
+        v[i] = SUM && row < s.rows ? p.lse[(int64_t)h * p.T * p.G + row_base + row] : INFINITY;
+      }
+    };
+    auto publish = [&]() __attribute__((always_inline)) {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __syncthreads();
+    };
+    float lse[2], lse_next[2];
+    load_q(t0, 0);
+    load_lse(t0, lse_next);
+    publish();
+    for (int32_t t = t0; t < t1; ++t) {
+      const int buf = (t - t0) & 1;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) lse[i] = lse_next[i];
+      if (t + 1 < t1) {
+        load_lse(t + 1, lse_next);
+        load_q(t + 1, buf ^ 1);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int32_t r0 = t * TR + 16 * i, row = r0 + n;
+        const int32_t pos = s.pos0 + p.by_g(min(row, s.rows - 1));
+        const int32_t first = s.pos0 + p.by_g(min(r0, s.rows - 1)), last = s.pos0 + p.by_g(min(r0 + 15, s.rows - 1));
+        const bool full = r0 + 15 < s.rows && key0 + 63 <= first && key0 + 64 <= s.len && keys.linked == 15u &&
+                          (key0 > last - p.W || key0 + 64 <= p.sinks);
+        u32x4p_t q[NCH];
+#pragma unroll
+        for (int c = 0; c < NCH; ++c)
+          q[c] = *reinterpret_cast<const u32x4p_t *>(lds_q[buf] + (16 * i + n) * RB +
+                                                     16 * ((8 * (c >> 1) + 2 * kq + (c & 1)) ^ q_swz(16 * i + n)));
+        f32x4p_t x[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          x[g] = keys.scores(g, q, p.qk_scale_log2);
+          if (!full) x[g] = hide(p, x[g], key0 + 16 * g + 4 * kq, pos, s.len, row < s.rows && ((keys.linked >> g) & 1));
+        }
+        if constexpr (SUM) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) w[g][r] += fast_exp2(x[g][r] - lse[i]);
+        } else {
+          float m = x[0][0], l = 0.0f;
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) m = fmaxf(m, x[g][r]);
+          m = max_over_quarters(m);
+          const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) l += fast_exp2(x[g][r] - ref);
+          l = sum_over_quarters(l);
+          if (kq == 0) s_ml[buf][wave][16 * i + n] = float2{m, l};
+        }
+      }
+      publish();
+      if (!SUM && threadIdx.x < TR && t * TR + (int32_t)threadIdx.x < s.rows) {
+        float m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = fmaxf(m, s_ml[buf][i][threadIdx.x].x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 v = s_ml[buf][i][threadIdx.x];
+          if (v.x != -INFINITY) l += v.y * fast_exp2(v.x - m);
+        }
+        p.ml[((int64_t)h * p.kts + kt) * p.T * p.G + row_base + t * TR + threadIdx.x] = float2{m, l};
+      }
+    }
+  }
+  if constexpr (SUM) {
+    const int64_t unit = (int64_t)b * p.Hk + h;
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float v = w[g][r];
+        v += xor1(v);
+        v += xor2(v);
+        v += half_mirror(v);
+        v += dpp_f32<0x140>(v);
+        const int32_t j = key0 + 16 * g + 4 * kq + r;
+        if (n == 0 && j < p.L) p.out[unit * p.L + j] = (p.scores ? p.scores[unit * p.L + j] : 0.0f) + v;
+      }
+  }
+}
+
+// lse of every row: a thread per row and key head.
+__global__ __launch_bounds__(256) void lse_kernel(const ScoresParams p) {
+  const int32_t h = (int32_t)(blockIdx.x % p.Hk), row = (int32_t)(blockIdx.x / p.Hk) * 256 + (int32_t)threadIdx.x;
+  const ScoredSeq s = scored_seq(p, blockIdx.y);
+  if (row >= s.rows) return;
+  const int32_t pos = s.pos0 + p.by_g(row), tiles = (min(s.len, pos + 1) + kTileKeys - 1) / kTileKeys;
+  const float2 *src = p.ml + (int64_t)h * p.kts * p.T * p.G + (int64_t)s.start * p.G + row;
+  float m = -INFINITY, l = 0.0f;
+  for (int32_t t = 0; t < tiles; ++t) {
+    if (!meets(p, pos, t * kTileKeys, (t + 1) * kTileKeys)) continue;
+    const float2 x = src[(int64_t)t * p.T * p.G];
+    const float top = fmaxf(m, x.x);
+    if (top == -INFINITY) continue;
+    l = l * fast_exp2(m - top) + x.y * fast_exp2(x.x - top);
+    m = top;
+  }
+  p.lse[(int64_t)h * p.T * p.G + (int64_t)s.start * p.G + row] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+struct ScoresPlan {
+  bool few;
+  int32_t max_rows, kts;
+  int64_t second, total;  // offset of probs or lse behind ml
+};
+static int64_t scored_keys(const memopt_scores_desc &d) {
+  return std::min<int64_t>((int64_t)d.max_blocks_per_seq * d.block_size, std::max(0, d.max_seq_len));
+}
+static ScoresPlan scores_plan(const memopt_scores_desc &d) {
+  const int64_t G = d.num_heads / d.num_kv_heads, rows = (int64_t)std::min(d.max_query_len, d.tokens) * G;
+  ScoresPlan pl = {};
+  pl.few = rows <= kFewRows;
+  pl.max_rows = (int32_t)rows;
+  pl.kts = (int32_t)((scored_keys(d) + kTileKeys - 1) / kTileKeys);
+  const int64_t ml = 8 * (int64_t)pl.kts * d.num_kv_heads * (pl.few ? d.batch * rows : d.tokens * G);
+  pl.second = (ml + 255) / 256 * 256;
+  pl.total = pl.second + (pl.few ? 4 * (int64_t)d.batch * d.num_kv_heads * rows * pl.kts * kTileKeys
+                                 : 4 * (int64_t)d.num_kv_heads * d.tokens * G);
+  if (rows == 0 || pl.kts == 0) pl.total = 0;
+  return pl;
+}
+
+static int validate_scores(const memopt_scores_desc &d) {
+  MEMOPT_REQUIRE(d.tokens >= 0 && d.batch >= 0 && d.max_query_len >= 0 && d.scores_len >= 0, MEMOPT_ERR_INVALID,
+                 "attention_scores: negative size");
+  MEMOPT_REQUIRE(d.num_heads > 0 && d.num_kv_heads > 0 && d.num_heads % d.num_kv_heads == 0, MEMOPT_ERR_INVALID,
+                 "attention_scores: num_heads must be a positive multiple of num_kv_heads");
+  MEMOPT_REQUIRE(d.kv_format == MEMOPT_KV_FP16 || d.kv_format == MEMOPT_KV_INT4, MEMOPT_ERR_UNSUPPORTED,
+                 "attention_scores: the cache must be an fp16 pool or INT4 pages");
+  MEMOPT_REQUIRE(d.head_dim == 64 || d.head_dim == 128, MEMOPT_ERR_UNSUPPORTED,
+                 "attention_scores: head_dim must be 64 or 128");
+  MEMOPT_REQUIRE(d.num_kv_blocks > 0 && d.max_blocks_per_seq > 0 && d.block_size > 0, MEMOPT_ERR_INVALID,
+                 "attention_scores: empty cache or block table");
+  MEMOPT_REQUIRE(d.kv_format == MEMOPT_KV_FP16 ? d.block_size % 16 == 0 : d.block_size == 16, MEMOPT_ERR_UNSUPPORTED,
+                 "attention_scores: pages must hold 16 tokens (fp16 pools: a multiple of 16)");
+  MEMOPT_REQUIRE((int64_t)d.max_blocks_per_seq * d.block_size <= 1 << 30 && d.scores_len <= 1 << 30,
+                 MEMOPT_ERR_UNSUPPORTED, "attention_scores: block tables and scores of up to 2^30 tokens");
+  const int64_t G = d.num_heads / d.num_kv_heads;
+  const int64_t tiles = (std::max<int64_t>(scored_keys(d), d.scores_len) + kTileKeys - 1) / kTileKeys;
+  MEMOPT_REQUIRE((int64_t)d.tokens * d.num_heads <= INT32_MAX - 255 && d.batch <= 65535 &&
+                     tiles * d.num_kv_heads * std::max(1, d.batch) < (1LL << 24) &&
+                     ((int64_t)d.tokens * G + 255) / 256 * d.num_kv_heads * std::max(1, d.batch) < (1LL << 24),
+                 MEMOPT_ERR_UNSUPPORTED, "attention_scores: too many (row, token) tiles for one call");
+  MEMOPT_REQUIRE(d.q_token_stride >= 0 && d.q_head_stride >= 0 &&
+                     d.q_token_stride < (1LL << 30) && d.q_head_stride < (1LL << 30) &&
+                     31 * d.q_token_stride + (G - 1) * d.q_head_stride < (1LL << 29),
+                 MEMOPT_ERR_UNSUPPORTED, "attention_scores: query rows lie too far apart");
+  MEMOPT_REQUIRE(((uintptr_t)d.query & 15) == 0 && d.q_token_stride % 8 == 0 && d.q_head_stride % 8 == 0 &&
+                     ((uintptr_t)d.key_cache & 15) == 0 && ((uintptr_t)d.workspace & 15) == 0,
+                 MEMOPT_ERR_INVALID, "attention_scores: rows, cache and workspace must be 16-byte aligned");
+  return MEMOPT_OK;
+}
+
+template <int FMT, int D>
+static int launch_scores(const ScoresParams &p, const ScoresPlan &pl, hipStream_t s) {
+  const unsigned tiles = (unsigned)((std::max<int64_t>(p.max_keys, p.L) + kTileKeys - 1) / kTileKeys);
+  const dim3 over_keys((unsigned)pl.kts * p.Hk, p.B), over_scores(tiles * p.Hk, p.B);
+  int rc;
+  if (pl.total == 0) {
+    hipLaunchKernelGGL(finish_kernel, over_scores, dim3(256), 0, s, p);
+    return check_launch("attention_scores");
+  }
+  if (pl.few) {
+    hipLaunchKernelGGL((few_rows_kernel<FMT, D>), over_keys, dim3(256), 0, s, p);
+    if ((rc = check_launch("attention_scores(rows)")) != MEMOPT_OK) return rc;
+    hipLaunchKernelGGL(finish_kernel, over_scores, dim3(256), 0, s, p);
+    return check_launch("attention_scores(finish)");
+  }
+  hipLaunchKernelGGL((chunk_rows_kernel<FMT, D, false>), over_keys, dim3(256), 0, s, p);
+  if ((rc = check_launch("attention_scores(maxima)")) != MEMOPT_OK) return rc;
+  hipLaunchKernelGGL(lse_kernel, dim3((unsigned)((p.max_rows + 255) / 256 * p.Hk), p.B), dim3(256), 0, s, p);
+  if ((rc = check_launch("attention_scores(lse)")) != MEMOPT_OK) return rc;
+  hipLaunchKernelGGL((chunk_rows_kernel<FMT, D, true>), over_scores, dim3(256), 0, s, p);
+  return check_launch("attention_scores(sums)");
+}
+
+}  // namespace memopt
+
+using namespace memopt;
+
+extern "C" int memopt_scores_workspace_size(const memopt_scores_desc *desc, int64_t *bytes) {
+  MEMOPT_REQUIRE(desc && bytes, MEMOPT_ERR_INVALID, "scores_workspace_size: null pointer");
+  *bytes = 0;
+  int rc = validate_scores(*desc);
+  if (rc != MEMOPT_OK || desc->batch == 0 || desc->scores_len == 0) return rc;
+  *bytes = scores_plan(*desc).total;
+  return MEMOPT_OK;
+}
+
+extern "C" int memopt_attention_scores(const memopt_scores_desc *desc, void *stream) {
+  MEMOPT_REQUIRE(desc, MEMOPT_ERR_INVALID, "attention_scores: null descriptor");
+  const memopt_scores_desc &d = *desc;
+  int rc = validate_scores(d);
+  if (rc != MEMOPT_OK || d.batch == 0 || d.scores_len == 0) return rc;
+  const ScoresPlan pl = scores_plan(d);
+  MEMOPT_REQUIRE(d.out && d.context_lens && d.query_starts && (pl.total == 0 || (d.query && d.key_cache && d.block_tables)),
+                 MEMOPT_ERR_INVALID, "attention_scores: null pointer");
+  MEMOPT_REQUIRE(pl.total == 0 || (d.workspace && d.workspace_bytes >= pl.total), MEMOPT_ERR_INVALID,
+                 "attention_scores: workspace needs " + std::to_string(pl.total) + " bytes");
+  ScoresParams p = {};
+  p.q = (const uint16_t *)d.query;
+  p.q_ts = d.q_token_stride;
+  p.q_hs = d.q_head_stride;
+  p.k = (const uint8_t *)d.key_cache;
+  p.T = pl.total == 0 ? 0 : d.tokens;
+  p.B = d.batch;
+  p.Hk = d.num_kv_heads;
+  p.G = d.num_heads / d.num_kv_heads;
+  p.by_g = Divisor::of((uint32_t)p.G);
+  p.by_chunks = Divisor::of((uint32_t)d.block_size / 16);
+  if (d.kv_format == MEMOPT_KV_INT4) {
+    p.k_hs = Int4Page(d.head_dim).block;
+    p.k_ps = p.Hk * p.k_hs;
+  } else {
+    p.k_hs = 2 * d.head_dim;
+    p.k_ts = p.Hk * p.k_hs;
+    p.k_ps = d.block_size * p.k_ts;
+  }
+  p.bt = d.block_tables;
+  p.ctx = d.context_lens;
+  p.starts = d.query_starts;
+  p.nb = d.num_kv_blocks;
+  p.scores = d.scores;
+  p.out = d.out;
+  p.M = d.max_blocks_per_seq;
+  p.bs = d.block_size;
+  p.W = std::min(effective_window(d.window_size, d.max_seq_len), 1 << 30);  // (position - W stays in 32 bits)
+  p.sinks = std::max(0, d.num_sink_tokens);
+  p.L = d.scores_len;
+  p.max_keys = (int32_t)scored_keys(d);
+  p.max_rows = pl.max_rows;
+  p.kts = pl.kts;
+  p.qk_scale_log2 = 1.4426950408889634f / sqrtf((float)d.head_dim);
+  p.ml = (float2 *)d.workspace;
+  (pl.few ? p.probs : p.lse) = (float *)((uint8_t *)d.workspace + pl.second);
+  hipStream_t s = (hipStream_t)stream;
+  if (d.kv_format == MEMOPT_KV_INT4)
+    return d.head_dim == 128 ? launch_scores<MEMOPT_KV_INT4, 128>(p, pl, s) : launch_scores<MEMOPT_KV_INT4, 64>(p, pl, s);
+  return d.head_dim == 128 ? launch_scores<MEMOPT_KV_FP16, 128>(p, pl, s) : launch_scores<MEMOPT_KV_FP16, 64>(p, pl, s);
+}

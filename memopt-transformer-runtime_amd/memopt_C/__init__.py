@@ -46,7 +46,7 @@ __all__ = [
     "write_cache", "evict_cache", "evict_tokens", "free_evicted_blocks",
     "dynamic_sparse_attention", "PreparedAttention", "quantize_kv_cache_int4", "dequantize_kv_cache_int4",
     "prompt_attention", "packed_attention", "packed_workspace_bytes", "PreparedPackedAttention", "advance_batch", "advance_batch_buffers",
-    "BatchStep", "library_path",
+    "BatchStep", "attention_scores", "library_path",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -144,6 +144,8 @@ _c_packed_ws = _sig("memopt_packed_workspace_size",
                     [ctypes.POINTER(PackedDesc), ctypes.POINTER(_i64), ctypes.POINTER(_i64)])
 _c_packed = _sig("memopt_packed_attention", [ctypes.POINTER(PackedDesc), _vp])
 _c_advance = _sig("memopt_advance_batch", [ctypes.c_char_p, _vp])
+_c_scores_ws = _sig("memopt_scores_workspace_size", [ctypes.c_char_p, ctypes.POINTER(_i64)])
+_c_scores = _sig("memopt_attention_scores", [ctypes.c_char_p, _vp])
 
 KV_FP16, KV_INT4, KV_INT4_ROWS = 0, 1, 2
 _FORMATS = {"fp16": KV_FP16, "int4": KV_INT4}
@@ -1130,3 +1132,127 @@ def advance_batch(new_tokens: torch.Tensor, context_lens: torch.Tensor, block_ta
                       free_span.data_ptr(), *out._args, B, M, C, block_size, rows)
     _check(_c_advance(d, torch._C._cuda_getCurrentRawStream(index)))
     return out
+
+
+# ---------------------------------------------------------------------------
+# A cache that is kept small: weights per token, compaction (no counterparts in
+# the reference)
+# ---------------------------------------------------------------------------
+
+_SCORES = struct.Struct("@3P5i2qiPiqPiPP5iPq")  # memopt_scores_desc
+
+
+def _paged_call(fn: str, query, context_lens, cu_seqlens, block_tables) -> Tuple[int, int]:
+    """(batch, max_blocks_per_seq) of the checked index tensors of packed queries over pages."""
+    if not (cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1):
+        raise RuntimeError(f"{fn}: cu_seqlens must be 1-D [batch + 1]")
+    if block_tables.dim() != 2:
+        raise RuntimeError(f"{fn}: block_tables must be 2-D [batch, max_blocks_per_seq]")
+    B, M = cu_seqlens.shape[0] - 1, block_tables.shape[1]
+    _int32(fn, cu_seqlens, "cu_seqlens", (B + 1,))
+    _int32(fn, context_lens, "context_lens", (B,))
+    _int32(fn, block_tables, "block_tables", (B, M))
+    return B, M
+
+
+def _near_rows(t: torch.Tensor, group: int) -> Tuple[torch.Tensor, int, int, int]:
+    """``_rows`` of ``t``, copied too where 31 token strides and ``group`` head strides pass 2^29 elements."""
+    r = _rows(t)
+    if 31 * r[2] + group * r[3] >= 2 ** 29:
+        r = _rows(t.clone(memory_format=torch.contiguous_format))
+    return r
+
+
+def attention_scores(query: torch.Tensor, key_cache: torch.Tensor, block_tables: torch.Tensor,
+                     context_lens: torch.Tensor, cu_seqlens: torch.Tensor, max_query_len: int, max_seq_len: int,
+                     window_size: int = -1, *, num_sink_tokens: int = 0, scores: Optional[torch.Tensor] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention weights that packed queries give the cached tokens, added up; returns f32 ``[B, Hkv, L]``.
+
+    ``out[b, h, j] = scores[b, h, j]`` plus the softmax weights of token j in
+    sequence b, summed over the sequence's query rows and the query heads of
+    key head h: the scores that ``evict_tokens`` and ``compact_cache`` go by.
+    ``query``, index tensors and masks are those of ``packed_attention``;
+    ``key_cache``: INT4 pages (the pool's key view or a page buffer) or the
+    fp16 key pool. A row that sees no key adds nothing. ``scores``: f32
+    ``[B, Hkv, L]``, contiguous (``None``: zeros, L = ``max_seq_len``);
+    ``out`` may be ``scores`` itself, else must not overlap it. Tokens from
+    ``max_seq_len`` on are not looked at. The sums' order is fixed.
+    """
+    fn = "attention_scores"
+    if not (isinstance(query, torch.Tensor) and query.is_cuda):
+        raise RuntimeError(f"{fn}: query must be a CUDA tensor")
+    device = query.device
+    index = device.index
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(device):
+            return attention_scores(query, key_cache, block_tables, context_lens, cu_seqlens, max_query_len, max_seq_len,
+                                    window_size, num_sink_tokens=num_sink_tokens, scores=scores, out=out)
+    _device_tensors(fn, device, ("key_cache", "block_tables", "context_lens", "cu_seqlens"), key_cache, block_tables,
+                    context_lens, cu_seqlens)
+    _no_grad(fn, query.requires_grad)
+    if query.dim() != 3 or query.dtype is not torch.float16:
+        raise RuntimeError(f"{fn}: query must be fp16 [tokens, heads, head_dim]")
+    T, Hq, D = query.shape
+    B, M = _paged_call(fn, query, context_lens, cu_seqlens, block_tables)
+    if max_query_len < 0 or max_seq_len < 0:
+        raise RuntimeError(f"{fn}: max_query_len and max_seq_len must not be negative")
+    if key_cache.dtype is torch.uint8:
+        if D not in (64, 128):
+            raise RuntimeError(f"{fn}: head_dim must be 64 or 128")
+        if not (key_cache.dim() == 3 and key_cache.shape[1] > 0):
+            raise RuntimeError(f"{fn}: INT4 caches are the pool's key view or its page buffer [pages, heads, bytes]")
+        Hk = key_cache.shape[1]
+        pages = _int4_pages_base(key_cache, key_cache, Hk, D)
+        if pages is None:
+            raise RuntimeError(f"{fn}: not an INT4 page buffer of this head_dim")
+        pk, nb, _ = pages
+        fmt, bs = KV_INT4, 16
+    else:
+        if key_cache.dtype is not torch.float16:
+            raise RuntimeError(f"{fn}: key_cache must be fp16 or INT4 pages")
+        if not (key_cache.dim() == 4 and key_cache.shape[3] == D and key_cache.is_contiguous()):
+            raise RuntimeError(f"{fn}: key_cache must be contiguous [num_kv_blocks, block_size, kv heads, {D}]")
+        nb, bs, Hk = key_cache.shape[:3]
+        fmt, pk = KV_FP16, key_cache.data_ptr()
+    if scores is not None:
+        _device_tensors(fn, device, ("scores",), scores)
+        if not (scores.dim() == 3 and scores.shape[:2] == (B, Hk) and scores.dtype is torch.float32 and
+                scores.is_contiguous()):
+            raise RuntimeError(f"{fn}: scores must be contiguous f32 [{B}, {Hk}, positions]")
+        _no_grad(fn, scores.requires_grad)
+        L = scores.shape[2]
+    else:
+        L = max_seq_len if out is None else out.shape[-1]
+    if out is None:
+        out = torch.empty((B, Hk, L), dtype=torch.float32, device=device)
+    else:
+        _device_tensors(fn, device, ("out",), out)
+        if not (out.shape == (B, Hk, L) and out.dtype is torch.float32 and out.is_contiguous()):
+            raise RuntimeError(f"{fn}: out must be contiguous f32 {[B, Hk, L]}")
+        _no_grad(fn, out.requires_grad)
+    q, pq, qts, qhs = _near_rows(query, Hq // max(1, Hk))
+    head = (pq, None if scores is None else scores.data_ptr(), out.data_ptr(), T, B, Hq, Hk, D, qts, qhs, fmt, pk, bs, nb,
+            block_tables.data_ptr(), M, context_lens.data_ptr(), cu_seqlens.data_ptr(), _count32(max_query_len),
+            _count32(max_seq_len), _count32(window_size), _count32(num_sink_tokens), L)
+    _launch(fn, _SCORES, head, _c_scores_ws, _c_scores, device)
+    return out
+
+
+def _launch(fn: str, packed: struct.Struct, head: tuple, size, call, device: torch.device) -> None:
+    """One call of a C entry whose descriptor ends in a workspace: ``head`` and then a fresh one of ``size``'s bytes
+    (any content) from torch's caching allocator, on the current stream of ``device``, which is current."""
+    try:
+        d = packed.pack(*(x or 0 for x in head), 0, 0)
+    except struct.error:
+        raise RuntimeError(f"{fn}: sizes must fit 32 bits") from None
+    need = _i64()
+    _check(size(d, ctypes.byref(need)))
+    n = need.value
+    if n:
+        ws = torch.empty(n, dtype=torch.uint8, device=device)
+        d = d[:-16] + _WORKSPACE.pack(ws.data_ptr(), n)
+    _check(call(d, torch._C._cuda_getCurrentRawStream(device.index)))
+
+
+_WORKSPACE = struct.Struct("@Pq")
