@@ -425,6 +425,50 @@ typedef struct memopt_scores_desc {
 int memopt_scores_workspace_size(const memopt_scores_desc *desc, int64_t *bytes);
 int memopt_attention_scores(const memopt_scores_desc *desc, void *stream);
 
+/* Tokens of least weight leave the cache. Of request b's context_lens[b]
+ * tokens, n = min(keep[b], those whose pages are linked) stay in every key
+ * head: the first num_sink_tokens, the last num_recent_tokens (as far as n
+ * reaches, the sinks first), and of the others those with the largest
+ * scores[b, h] (ties: the first; NaN counts as the lowest). They keep their
+ * order and become tokens 0 .. n - 1: their rows are copied, bit for bit, into
+ * fresh pages from the front of the ring of free pages (memopt_advance_batch),
+ * and the old linked pages go to its end, both in request order. Nothing else
+ * of the cache changes, rows of the fresh pages behind token n - 1 included.
+ *
+ * Written for every request: block_tables_out (the fresh pages, -1 behind),
+ * context_lens_out, scores_out (the kept tokens' scores, 0 behind), kept (old
+ * positions, -1 behind), status; a request that is not compacted keeps its
+ * tables, length and scores, and its `kept` are -1. free_span_out may be
+ * free_span; the other results must not overlap the inputs. At most 4096
+ * requests; calls on one batch must not overlap. Status: */
+#define MEMOPT_COMPACT_DONE     0
+#define MEMOPT_COMPACT_INVALID  1  /* a length past the table or scores_len, or keep past max_keep  */
+#define MEMOPT_COMPACT_LEFT     2  /* it may keep all it has (negative keep: always)                */
+#define MEMOPT_COMPACT_NO_PAGES 3  /* the free pages, or the ring's room for the old ones, did not  */
+                                   /* last (sums over all that ask so far, as in advance_batch);    */
+                                   /* pages that this call gives back serve the next one            */
+#define MEMOPT_COMPACT_SHARED   4  /* one of its pages is listed twice in this call's tables        */
+typedef struct memopt_compact_desc {
+  const float *scores;               /* [num_requests, num_kv_heads, scores_len] */
+  float *scores_out;                 /* the same                               */
+  int32_t *kept;                     /* [num_requests, num_kv_heads, max_keep] */
+  int32_t kv_format;                 /* MEMOPT_KV_FP16 / MEMOPT_KV_INT4        */
+  void *key_cache, *value_cache;     /* (value_cache unused for INT4 pages)    */
+  int64_t num_kv_blocks;
+  const int32_t *block_tables, *context_lens, *keep;
+  int32_t *block_tables_out, *context_lens_out, *status;
+  int32_t *free_pages;               /* [num_free_pages]; written at the end of the span */
+  const int32_t *free_span;
+  int32_t *free_span_out;
+  int32_t num_requests, num_kv_heads, head_dim, max_blocks_per_seq, block_size, num_free_pages, scores_len, max_keep;
+  int32_t num_sink_tokens, num_recent_tokens;
+  void *workspace;                   /* >= memopt_compact_workspace_size bytes, 16-byte aligned, any content */
+  int64_t workspace_bytes;
+} memopt_compact_desc;
+/* Calls sharing a workspace must not overlap. */
+int memopt_compact_workspace_size(const memopt_compact_desc *desc, int64_t *bytes);
+int memopt_compact_cache(const memopt_compact_desc *desc, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -46,7 +46,7 @@ __all__ = [
     "write_cache", "evict_cache", "evict_tokens", "free_evicted_blocks",
     "dynamic_sparse_attention", "PreparedAttention", "quantize_kv_cache_int4", "dequantize_kv_cache_int4",
     "prompt_attention", "packed_attention", "packed_workspace_bytes", "PreparedPackedAttention", "advance_batch", "advance_batch_buffers",
-    "BatchStep", "attention_scores", "library_path",
+    "BatchStep", "attention_scores", "compact_cache", "compact_cache_buffers", "CompactStep", "library_path",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -146,6 +146,8 @@ _c_packed = _sig("memopt_packed_attention", [ctypes.POINTER(PackedDesc), _vp])
 _c_advance = _sig("memopt_advance_batch", [ctypes.c_char_p, _vp])
 _c_scores_ws = _sig("memopt_scores_workspace_size", [ctypes.c_char_p, ctypes.POINTER(_i64)])
 _c_scores = _sig("memopt_attention_scores", [ctypes.c_char_p, _vp])
+_c_compact_ws = _sig("memopt_compact_workspace_size", [ctypes.c_char_p, ctypes.POINTER(_i64)])
+_c_compact = _sig("memopt_compact_cache", [ctypes.c_char_p, _vp])
 
 KV_FP16, KV_INT4, KV_INT4_ROWS = 0, 1, 2
 _FORMATS = {"fp16": KV_FP16, "int4": KV_INT4}
@@ -1256,3 +1258,138 @@ def _launch(fn: str, packed: struct.Struct, head: tuple, size, call, device: tor
 
 
 _WORKSPACE = struct.Struct("@Pq")
+
+
+class CompactStep:
+    """What ``compact_cache`` writes (contiguous, on one device; int32 but for
+    ``scores``, f32): ``block_tables`` ``[N, M]``, ``context_lens`` ``[N]``,
+    ``free_span`` ``[2]``, ``scores`` ``[N, Hkv, L]``, ``kept`` ``[N, Hkv,
+    max_keep]``, ``status`` ``[N]``. The tensors are checked here once, and kept."""
+
+    FIELDS = ("block_tables", "context_lens", "free_span", "scores", "kept", "status")
+    __slots__ = FIELDS + ("device", "_args", "_sizes")
+
+    def __init__(self, block_tables, context_lens, free_span, scores, kept, status):
+        fn = "compact_cache"
+        tensors = (block_tables, context_lens, free_span, scores, kept, status)
+        keep = super().__setattr__
+        keep("device", getattr(block_tables, "device", None))
+        _require(getattr(block_tables, "is_cuda", False), "compact_cache: block_tables must be a CUDA tensor")
+        _device_tensors(fn, self.device, self.FIELDS, *tensors)
+        _require(block_tables.dim() == 2 and scores.dim() == 3 and kept.dim() == 3,
+                 "compact_cache: block_tables must be 2-D, scores and kept 3-D")
+        N, M = block_tables.shape
+        Hk, L, K = scores.shape[1], scores.shape[2], kept.shape[2]
+        for n, t, shape in zip(self.FIELDS, tensors, ((N, M), (N,), (2,), None, (N, Hk, K), (N,))):
+            if shape is not None:
+                _int32(fn, t, n, shape)
+            elif not (t.dtype is torch.float32 and t.is_contiguous() and t.shape[0] == N):
+                raise RuntimeError(f"{fn}: scores must be contiguous f32 [{N}, kv heads, positions]")
+            keep(n, t)
+        keep("_sizes", (N, Hk, M, L, K))
+        keep("_args", tuple(t.data_ptr() for t in tensors))
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"CompactStep: {name} cannot be assigned")
+
+
+def compact_cache_buffers(num_requests: int, num_kv_heads: int, max_blocks_per_seq: int, scores_len: int, max_keep: int,
+                          device) -> CompactStep:
+    """Buffers for ``compact_cache(..., out=)``."""
+    def i32(*shape):
+        return torch.empty(shape, dtype=torch.int32, device=device)
+
+    N, Hk = num_requests, num_kv_heads
+    return CompactStep(i32(N, max_blocks_per_seq), i32(N), i32(2),
+                       torch.empty((N, Hk, scores_len), dtype=torch.float32, device=device), i32(N, Hk, max_keep), i32(N))
+
+
+_COMPACT = struct.Struct("@3Pi2Pq9P10iPq")  # memopt_compact_desc
+
+
+def compact_cache(scores: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_tables: torch.Tensor,
+                  context_lens: torch.Tensor, keep: torch.Tensor, free_pages: torch.Tensor, free_span: torch.Tensor, *,
+                  num_sink_tokens: int = 4, num_recent_tokens: int = 0, max_keep: Optional[int] = None,
+                  out: Optional[CompactStep] = None) -> CompactStep:
+    """Tokens of least weight leave the cache; the others move to fresh pages and the old pages come back.
+
+    Request b's ``context_lens[b]`` tokens lie in the pages of
+    ``block_tables[b]`` (int32 ``[N, M]``). Every key head keeps ``n =
+    min(keep[b], linked tokens)`` of them: the first ``num_sink_tokens``, the
+    last ``num_recent_tokens``, and of the others those with the largest
+    ``scores[b, h]`` (f32 ``[N, Hkv, L]``, L at least the longest context;
+    ties: the first; NaN: last). They keep their order, as tokens ``0 .. n -
+    1`` of pages from the front of the ring ``free_pages`` / ``free_span``
+    (``advance_batch``); the old pages go to its end, in place. Unlike
+    ``evict_tokens``, which zeroes rows, this takes them out of every later
+    softmax. Queries after it stand at positions from n on: rotary positions
+    are the caller's (``kept`` has the old ones).
+
+    Caches: INT4 pages (the pool's code views, or a page buffer passed as
+    both) or fp16 pools, changed in place (only in fresh pages). Results are
+    new tensors, or ``out``'s (``compact_cache_buffers``), which must not be
+    the inputs but for ``free_span``; ``status``: 0 compacted, 1 invalid
+    (length past table or scores, ``keep`` past ``max_keep``), 2 left (it may
+    keep all it has; a negative ``keep``: always), 3 pages did not last (what
+    a call gives back serves the next one), 4 a page is listed twice.
+    ``max_keep`` is needed without ``out``. Calls on one batch must not
+    overlap.
+    """
+    fn = "compact_cache"
+    if not (isinstance(scores, torch.Tensor) and scores.is_cuda):
+        raise RuntimeError(f"{fn}: scores must be a CUDA tensor")
+    device = scores.device
+    if torch._C._cuda_getDevice() != device.index:
+        with torch.cuda.device(device):
+            return compact_cache(scores, key_cache, value_cache, block_tables, context_lens, keep, free_pages, free_span,
+                                 num_sink_tokens=num_sink_tokens, num_recent_tokens=num_recent_tokens, max_keep=max_keep,
+                                 out=out)
+    _device_tensors(fn, device, ("key_cache", "value_cache", "block_tables", "context_lens", "keep", "free_pages",
+                                 "free_span"), key_cache, value_cache, block_tables, context_lens, keep, free_pages,
+                    free_span)
+    if not (scores.dim() == 3 and scores.dtype is torch.float32 and scores.is_contiguous()):
+        raise RuntimeError(f"{fn}: scores must be contiguous f32 [requests, kv heads, positions]")
+    if block_tables.dim() != 2 or free_pages.dim() != 1:
+        raise RuntimeError(f"{fn}: block_tables must be 2-D, free_pages 1-D")
+    N, Hk, L = scores.shape
+    M, C = block_tables.shape[1], free_pages.shape[0]
+    _int32(fn, block_tables, "block_tables", (N, M))
+    _int32(fn, context_lens, "context_lens", (N,))
+    _int32(fn, keep, "keep", (N,))
+    _int32(fn, free_pages, "free_pages", (C,))
+    _int32(fn, free_span, "free_span", (2,))
+    if key_cache.dtype is torch.uint8:
+        if not (key_cache.dim() == 3 and value_cache.dim() == 3 and key_cache.shape[1] == Hk):
+            raise RuntimeError(f"{fn}: INT4 caches are the pool's code views or its page buffer [pages, {Hk}, bytes]")
+        pages = None
+        for D in (64, 128):
+            pages = pages or _int4_pages_base(key_cache, value_cache, Hk, D)
+            if pages is not None:
+                break
+        if pages is None:
+            raise RuntimeError(f"{fn}: not an INT4 page buffer of head_dim 64 or 128")
+        pk, nb, _ = pages
+        fmt, bs, pv = KV_INT4, 16, 0
+    else:
+        if not (key_cache.dtype is torch.float16 and value_cache.dtype is torch.float16):
+            raise RuntimeError(f"{fn}: caches must be fp16 or INT4 pages")
+        if not (key_cache.dim() == 4 and key_cache.shape == value_cache.shape and key_cache.shape[2] == Hk and
+                key_cache.is_contiguous() and value_cache.is_contiguous()):
+            raise RuntimeError(f"{fn}: caches must be contiguous [num_kv_blocks, block_size, {Hk}, head_dim]")
+        nb, bs, _, D = key_cache.shape
+        fmt, pk, pv = KV_FP16, key_cache.data_ptr(), value_cache.data_ptr()
+    if out is None:
+        if max_keep is None or max_keep < 0:
+            raise RuntimeError(f"{fn}: max_keep or out must be given")
+        out = compact_cache_buffers(N, Hk, M, L, max_keep, device)
+    K = out.kept.shape[2]
+    if max_keep is not None and max_keep != K:
+        raise RuntimeError(f"{fn}: max_keep differs from out's")
+    if out.device != device or out._sizes[:4] != (N, Hk, M, L):
+        raise RuntimeError(f"{fn}: out holds buffers of another device or of other sizes")
+    bt_o, cl_o, span_o, sc_o, kept, status = out._args
+    head = (scores.data_ptr(), sc_o, kept, fmt, pk, pv, nb, block_tables.data_ptr(), context_lens.data_ptr(),
+            keep.data_ptr(), bt_o, cl_o, status, free_pages.data_ptr(), free_span.data_ptr(), span_o, N, Hk, D, M, bs, C, L,
+            K, _count32(num_sink_tokens), _count32(num_recent_tokens))
+    _launch(fn, _COMPACT, head, _c_compact_ws, _c_compact, device)
+    return out
