@@ -469,6 +469,47 @@ typedef struct memopt_compact_desc {
 int memopt_compact_workspace_size(const memopt_compact_desc *desc, int64_t *bytes);
 int memopt_compact_cache(const memopt_compact_desc *desc, void *stream);
 
+/* Attention over a paged cache of one vector per token for all heads (latent
+ * attention, absorbed form): cache [num_kv_blocks, block_size, rank +
+ * rope_dim], contiguous; keys are its whole rows, values their first `rank`
+ * elements:
+ *   out[t, h] = sum_j softmax_j(scale query[t, h] . cache_j) cache_j[: rank]
+ * Packed rows, positions, windows, sinks, unlinked pages and rows that see
+ * nothing are memopt_packed_attention's. Elements of hidden tokens never reach
+ * a result, inf and NaN included. Tokens from max_seq_len on are not looked
+ * at; rows past max_query_len of a sequence may be left unwritten. dtype is
+ * that of query, cache and out; rank 128, 256 or 512, rope_dim 32 or 64,
+ * block_size a multiple of 16. */
+typedef struct memopt_latent_desc {
+  const void *query;                 /* [tokens, num_heads, rank + rope_dim]   */
+  const void *cache;
+  void *out;                         /* [tokens, num_heads, rank]              */
+  int32_t dtype;                     /* MEMOPT_FP16 / MEMOPT_BF16              */
+  int32_t tokens, batch, num_heads, rank, rope_dim;
+  int64_t q_token_stride, q_head_stride, o_token_stride, o_head_stride;
+  int32_t block_size;
+  int64_t num_kv_blocks;
+  const int32_t *block_tables;       /* [batch, max_blocks_per_seq]            */
+  int32_t max_blocks_per_seq;
+  const int32_t *context_lens;       /* [batch]                                */
+  const int32_t *query_starts;       /* [batch + 1]                            */
+  int32_t max_query_len, max_seq_len, window_size, num_sink_tokens;
+  float scale;
+  void *workspace;                   /* >= memopt_latent_workspace_size bytes, 16-byte aligned, any content */
+  int64_t workspace_bytes;
+} memopt_latent_desc;
+/* Calls sharing a workspace must not overlap. */
+int memopt_latent_workspace_size(const memopt_latent_desc *desc, int64_t *bytes);
+int memopt_latent_attention(const memopt_latent_desc *desc, void *stream);
+
+/* Rows of the latent cache from their two parts: token t's latents [rank] and
+ * rotary keys [rope_dim] (16-bit elements, strides in elements, rows 16-byte
+ * aligned) go to row slots[t] of the cache's num_slots; slots outside are
+ * skipped. Two tokens of one slot: either's elements. */
+int memopt_write_latent(const void *latents, int64_t latent_stride, const void *rope_keys, int64_t rope_stride,
+                        int32_t num_tokens, int32_t rank, int32_t rope_dim, const int32_t *slots, void *cache,
+                        int64_t num_slots, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

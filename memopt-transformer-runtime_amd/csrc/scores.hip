@@ -260,8 +260,9 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const ScoresParams p) {
   l = sum_over_quarters(l);
   if (kq == 0) s_l[wave][n] = l;
   __syncthreads();
-  if (threadIdx.x < (unsigned)s.rows)
-    p.ml[(unit * p.kts + kt) * p.max_rows + n] = float2{m, (s_l[0][n] + s_l[1][n]) + (s_l[2][n] + s_l[3][n])};
+  l = (s_l[0][n] + s_l[1][n]) + (s_l[2][n] + s_l[3][n]);
+  // (a tile without a maximum adds nothing, unless all that the row sees in it is NaN)
+  if (threadIdx.x < (unsigned)s.rows) p.ml[(unit * p.kts + kt) * p.max_rows + n] = float2{l == 0.0f ? m : fmaxf(m, -3e38f), l};
 }
 
 // out = scores + the rows' weights: a thread per key. Also the whole of a
@@ -310,7 +311,10 @@ __global__ __launch_bounds__(256) void finish_kernel(const ScoresParams p) {
     __syncthreads();
     if (j < s.len) {
       const float *src = p.probs + unit * p.max_rows * ((int64_t)p.kts * kTileKeys) + j;
-      for (int32_t r = 0; r < s.rows; ++r) w = fmaf(src[(int64_t)r * p.kts * kTileKeys], s_f[r], w);
+      for (int32_t r = 0; r < s.rows; ++r) {
+        const float x = src[(int64_t)r * p.kts * kTileKeys];
+        w = x == 0.0f ? w : fmaf(x, s_f[r], w);  // (a hidden key takes no part in a row of NaN)
+      }
     }
   }
   if (j < p.L) p.out[unit * p.L + j] = before + w;
@@ -404,7 +408,10 @@ __global__ __launch_bounds__(256, 2) void chunk_rows_kernel(const ScoresParams p
 #pragma unroll
           for (int g = 0; g < 4; ++g)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) w[g][r] += fast_exp2(x[g][r] - lse[i]);
+            for (int r = 0; r < 4; ++r) {
+              const float y = fast_exp2(x[g][r] - lse[i]);
+              w[g][r] += !full && x[g][r] == -INFINITY ? 0.0f : y;  // (a hidden key takes no part in a row of NaN)
+            }
         } else {
           float m = x[0][0], l = 0.0f;
 #pragma unroll
@@ -418,7 +425,8 @@ __global__ __launch_bounds__(256, 2) void chunk_rows_kernel(const ScoresParams p
 #pragma unroll
             for (int r = 0; r < 4; ++r) l += fast_exp2(x[g][r] - ref);
           l = sum_over_quarters(l);
-          if (kq == 0) s_ml[buf][wave][16 * i + n] = float2{m, l};
+          // (keys without a maximum add nothing, unless all that the row sees of them is NaN)
+          if (kq == 0) s_ml[buf][wave][16 * i + n] = float2{l == 0.0f ? m : fmaxf(m, -3e38f), l};
         }
       }
       publish();

@@ -46,7 +46,8 @@ __all__ = [
     "write_cache", "evict_cache", "evict_tokens", "free_evicted_blocks",
     "dynamic_sparse_attention", "PreparedAttention", "quantize_kv_cache_int4", "dequantize_kv_cache_int4",
     "prompt_attention", "packed_attention", "packed_workspace_bytes", "PreparedPackedAttention", "advance_batch", "advance_batch_buffers",
-    "BatchStep", "attention_scores", "compact_cache", "compact_cache_buffers", "CompactStep", "library_path",
+    "BatchStep", "attention_scores", "compact_cache", "compact_cache_buffers", "CompactStep", "write_latent", "latent_attention",
+    "latent_prompt_attention", "library_path",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -148,6 +149,9 @@ _c_scores_ws = _sig("memopt_scores_workspace_size", [ctypes.c_char_p, ctypes.POI
 _c_scores = _sig("memopt_attention_scores", [ctypes.c_char_p, _vp])
 _c_compact_ws = _sig("memopt_compact_workspace_size", [ctypes.c_char_p, ctypes.POINTER(_i64)])
 _c_compact = _sig("memopt_compact_cache", [ctypes.c_char_p, _vp])
+_c_latent_ws = _sig("memopt_latent_workspace_size", [ctypes.c_char_p, ctypes.POINTER(_i64)])
+_c_latent = _sig("memopt_latent_attention", [ctypes.c_char_p, _vp])
+_c_write_latent = _sig("memopt_write_latent", [_vp, _i64, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _i64, _vp])
 
 KV_FP16, KV_INT4, KV_INT4_ROWS = 0, 1, 2
 _FORMATS = {"fp16": KV_FP16, "int4": KV_INT4}
@@ -821,15 +825,20 @@ def _rows(t: torch.Tensor, far: int = 2 ** 63) -> Tuple[torch.Tensor, int, int, 
     return t, t.data_ptr(), t.shape[1] * t.shape[2], t.shape[2]
 
 
-def _out_rows(fn: str, out: Optional[torch.Tensor], query: torch.Tensor) -> Tuple[torch.Tensor, int, int, int]:
-    """(out, address, token stride, head stride); a fresh tensor for ``None``."""
+def _out_rows(fn: str, out: Optional[torch.Tensor], query: torch.Tensor,
+              width: Optional[int] = None) -> Tuple[torch.Tensor, int, int, int]:
+    """(out, address, token stride, head stride); a fresh tensor for ``None``. ``width``: its last dimension, where
+    that is not query's."""
+    if width is not None and width != query.shape[2]:
+        query = query[:, :, :width] if width < query.shape[2] else query.new_empty((1, 1, width)).expand(*query.shape[:2], width)
     if out is None:
         out = torch.empty_like(query, memory_format=torch.contiguous_format)  # (half the time of torch.empty)
         _, H, D = out.shape
         return out, out.data_ptr(), H * D, D
     _device_tensors(fn, query.device, ("out",), out)
     if not (out.shape == query.shape and out.dtype == query.dtype):
-        raise RuntimeError(f"{fn}: out must be shaped like query, with its dtype")
+        raise RuntimeError(f"{fn}: out must be shaped like query, with its dtype" if width is None else
+                           f"{fn}: out must be {list(query.shape)}, with query's dtype")
     ts, hs, ds = out.stride()
     p = out.data_ptr()
     T, H, D = out.shape
@@ -1392,4 +1401,106 @@ def compact_cache(scores: torch.Tensor, key_cache: torch.Tensor, value_cache: to
             keep.data_ptr(), bt_o, cl_o, status, free_pages.data_ptr(), free_span.data_ptr(), span_o, N, Hk, D, M, bs, C, L,
             K, _count32(num_sink_tokens), _count32(num_recent_tokens))
     _launch(fn, _COMPACT, head, _c_compact_ws, _c_compact, device)
+    return out
+
+
+# ---------------------------------------------------------------------------
+# Latent attention: one cached vector per token for all heads (no counterparts
+# in the reference)
+# ---------------------------------------------------------------------------
+
+_LATENT = struct.Struct("@3P6i4qiqPiPP4ifPq")  # memopt_latent_desc
+
+
+def _latent_cache(fn: str, cache: torch.Tensor, width: int) -> Tuple[int, int]:
+    """(pages, tokens per page) of a latent cache of rows of ``width`` elements."""
+    if not (cache.dim() == 3 and cache.shape[2] == width and cache.is_contiguous()):
+        raise RuntimeError(f"{fn}: cache must be contiguous [num_kv_blocks, block_size, {width}]")
+    return cache.shape[0], cache.shape[1]
+
+
+def write_latent(latents: torch.Tensor, rope_keys: torch.Tensor, slot_mapping: torch.Tensor, cache: torch.Tensor) -> None:
+    """Write tokens' latents ``[T, rank]`` and rotary keys ``[T, rope_dim]`` into a latent cache.
+
+    ``cache`` ``[num_kv_blocks, block_size, rank + rope_dim]`` (contiguous,
+    fp16 or bf16 like the rows); token t's row goes to slot
+    ``slot_mapping[t]`` (int32; page * block_size + offset, as for
+    ``write_cache``); slots outside the cache, -1 among them, are skipped.
+    ``rank`` and ``rope_dim`` are multiples of 8. Rows may be views (of a
+    fused projection): they are read in place where they are 16-byte aligned.
+    """
+    fn = "write_latent"
+    if not (isinstance(latents, torch.Tensor) and latents.is_cuda):
+        raise RuntimeError(f"{fn}: latents must be a CUDA tensor")
+    device, dtype = latents.device, latents.dtype
+    if torch._C._cuda_getDevice() != device.index:
+        with torch.cuda.device(device):
+            return write_latent(latents, rope_keys, slot_mapping, cache)
+    _device_tensors(fn, device, ("rope_keys", "slot_mapping", "cache"), rope_keys, slot_mapping, cache)
+    _no_grad(fn, latents.requires_grad or rope_keys.requires_grad)
+    if not (latents.dim() == 2 and rope_keys.dim() == 2 and latents.shape[0] == rope_keys.shape[0]):
+        raise RuntimeError(f"{fn}: latents and rope_keys must be 2-D [tokens, elements] of the same tokens")
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
+        raise RuntimeError(f"{fn}: latents must be fp16 or bf16")
+    if not (rope_keys.dtype is dtype and cache.dtype is dtype):
+        raise RuntimeError(f"{fn}: rope_keys and cache must have latents' dtype")
+    T, R = latents.shape
+    P = rope_keys.shape[1]
+    nb, bs = _latent_cache(fn, cache, R + P)
+    _int32(fn, slot_mapping, "slot_mapping", (T,))
+    c, pc, cts, _ = _rows(latents[:, None])
+    r, pr, rts, _ = _rows(rope_keys[:, None])
+    if T > 2 ** 31 - 1:
+        raise RuntimeError(f"{fn}: sizes must fit 32 bits")
+    _check(_c_write_latent(pc, cts, pr, rts, T, R, P, slot_mapping.data_ptr(), cache.data_ptr(), nb * bs,
+                           torch._C._cuda_getCurrentRawStream(device.index)))
+
+
+def latent_attention(query: torch.Tensor, cache: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor,
+                     cu_seqlens: torch.Tensor, max_query_len: int, max_seq_len: int, scale: float, rank: int,
+                     window_size: int = -1, *, num_sink_tokens: int = 0,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of packed queries over a paged latent cache (absorbed form); returns ``[T, Hq, rank]``.
+
+    ``cache`` ``[num_kv_blocks, block_size, rank + rope_dim]``: a token's one
+    row is the key of every head, its first ``rank`` elements the value.
+    ``query`` ``[T, Hq, rank + rope_dim]`` holds each head's query times its
+    key projection, then its rotary part; the caller multiplies the result
+    with the heads' value projections. Scores are multiplied by ``scale``
+    (one over the root of the width that a head's keys have when expanded).
+    fp16 or bf16, one type for all; ``rank`` 128, 256 or 512, ``rope_dim`` 32
+    or 64, pages of a multiple of 16 tokens. Index tensors, masks, strides and
+    rows of no sequence are as in ``packed_attention``; tokens from
+    ``max_seq_len`` on are not looked at. ``out`` must not overlap the inputs.
+    """
+    fn = "latent_attention"
+    if not (isinstance(query, torch.Tensor) and query.is_cuda):
+        raise RuntimeError(f"{fn}: query must be a CUDA tensor")
+    device, dtype = query.device, query.dtype
+    if torch._C._cuda_getDevice() != device.index:
+        with torch.cuda.device(device):
+            return latent_attention(query, cache, block_tables, context_lens, cu_seqlens, max_query_len, max_seq_len, scale,
+                                    rank, window_size, num_sink_tokens=num_sink_tokens, out=out)
+    _device_tensors(fn, device, ("cache", "block_tables", "context_lens", "cu_seqlens"), cache, block_tables, context_lens,
+                    cu_seqlens)
+    _no_grad(fn, query.requires_grad or cache.requires_grad)
+    if query.dim() != 3:
+        raise RuntimeError(f"{fn}: query must be 3-D [tokens, heads, rank + rope_dim]")
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
+        raise RuntimeError(f"{fn}: query must be fp16 or bf16")
+    if cache.dtype is not dtype:
+        raise RuntimeError(f"{fn}: cache must have query's dtype")
+    T, Hq, W = query.shape
+    if not 0 < rank < W:
+        raise RuntimeError(f"{fn}: rank must be less than the query's width {W}")
+    nb, bs = _latent_cache(fn, cache, W)
+    B, M = _paged_call(fn, query, context_lens, cu_seqlens, block_tables)
+    if max_query_len < 0 or max_seq_len < 0:
+        raise RuntimeError(f"{fn}: max_query_len and max_seq_len must not be negative")
+    out, po, ots, ohs = _out_rows(fn, out, query, rank)
+    q, pq, qts, qhs = _rows(query)
+    head = (pq, cache.data_ptr(), po, 1 if dtype is torch.bfloat16 else 0, T, B, Hq, rank, W - rank, qts, qhs, ots, ohs, bs,
+            nb, block_tables.data_ptr(), M, context_lens.data_ptr(), cu_seqlens.data_ptr(), _count32(max_query_len),
+            _count32(max_seq_len), _count32(window_size), _count32(num_sink_tokens), float(scale))
+    _launch(fn, _LATENT, head, _c_latent_ws, _c_latent, device)
     return out

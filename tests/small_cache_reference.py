@@ -129,3 +129,32 @@ def compact(scores, pools, fmt, tables, ctx, keep, ring, span, nb, bs, K, sinks,
         ctx_out[b] = n
         scores[b] = row
     return tables, ctx_out, np.array([(head + taken) % C, count - taken + back], np.int32), scores, kept, status, ring, pools
+
+
+def latent(q, c, pos, rank, scale, window, sinks, live=None):
+    """One sequence in float64: q [n, Hq, W] at positions pos, c [m, W]. (o [n, Hq, rank], sum_j p_j |c_j|, and the largest
+    scale sum_d |q_d c_jd| of each row, as packed_reference.tolerance takes them.) Hidden tokens take no part at all."""
+    n, Hq, W = q.shape
+    m = c.shape[0]
+    q, c = q.double().cpu(), c.double().cpu()
+    see = visible(pos, m, window, sinks, live)
+    c = torch.where(see.any(0)[:, None], c, 0.0) if m else c
+    o, a, e = (torch.zeros(n, Hq, rank, dtype=torch.float64) for _ in range(3))
+    for h in range(Hq):
+        if not m:
+            break
+        w = torch.zeros(n, m, dtype=torch.float64)
+        for i in range(n):
+            j = see[i].nonzero()[:, 0]
+            if j.numel():
+                w[i, j] = torch.softmax(scale * (c[j] @ q[i, h]), 0)
+                o[i, h], a[i, h] = w[i, j] @ c[j, :rank], w[i, j] @ c[j, :rank].abs()
+                e[i, h] = (abs(scale) * (c[j].abs() @ q[i, h].abs())).max()
+    return o, a, e
+
+
+def latent_tolerance(o, a, e, keys, W, dtype):
+    """packed_reference.tolerance with W products in a score; the kernel's merges of partial sums add one factor of an
+    exp2 (2^-22) and one rounding each to numerator and denominator, of at most `keys` / 64 parts."""
+    from packed_reference import tolerance
+    return tolerance(o, a, e, keys, W, dtype, dtype, False) + 2 * (2.0 ** -22 + (keys / 64 + 1) * 2.0 ** -24) * a

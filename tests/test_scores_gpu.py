@@ -174,6 +174,18 @@ def test_hidden_odd_keys_change_nothing(fmt, qn):
     assert bool(out[0, 0, 240:329 - qn[0]].isnan().all())
 
 
+@pytest.mark.parametrize("ctx,qn", [(257, 1), (65, 1), (257, 20), (321, 20), (3, 1)])
+def test_a_nan_alone_in_its_tile(ctx, qn):
+    """The last key is NaN: the one row that sees it (with nothing else of its tile, or nothing at all but it) adds NaN to
+    every key it sees, and so to all of its sequence."""
+    c = Case("fp16", [ctx, 40], [qn, 1], 4, 2, 64, seed=4)
+    c.kc[int(c.tables[0, (ctx - 1) // 16]), (ctx - 1) % 16, 0, 3] = float("nan")
+    out = run(c)
+    assert bool(out[0, 0, :ctx].isnan().all()) and not bool(out[0, 1].isnan().any()) and not bool(out[1].isnan().any())
+    out = run(c, window=1)
+    assert bool(out[0, 0, ctx - 1].isnan()) and int(out[0, 0].isnan().sum()) == 1
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("qn", [[1, 3], [30, 41]])
 def test_strided_and_far_query_rows(fmt, qn):
