@@ -510,6 +510,28 @@ int memopt_write_latent(const void *latents, int64_t latent_stride, const void *
                         int32_t num_tokens, int32_t rank, int32_t rope_dim, const int32_t *slots, void *cache,
                         int64_t num_slots, void *stream);
 
+/* Causal attention over whole packed prompts with keys of two parts, one per
+ * head and a rotary one shared by all heads (latent attention, expanded form):
+ *   score = scale (query[.. : head_dim] . key + query[head_dim ..] . rope_key)
+ * with values of head_dim elements. Rows, masks, strides and hidden elements
+ * as in memopt_prompt_attention; every head has keys and values of its own.
+ * head_dim 64 or 128, rope_dim 32 or 64. `out` must not overlap the inputs. */
+typedef struct memopt_latent_prompt_desc {
+  const void *query;                 /* [tokens, num_heads, head_dim + rope_dim] */
+  const void *key;                   /* [tokens, num_heads, head_dim]          */
+  const void *rope_key;              /* [tokens, rope_dim]                     */
+  const void *value;                 /* [tokens, num_heads, head_dim]          */
+  void *out;                         /* [tokens, num_heads, head_dim]          */
+  int32_t dtype;                     /* MEMOPT_FP16 / MEMOPT_BF16              */
+  int32_t tokens, batch, num_heads, head_dim, rope_dim;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, r_token_stride;
+  int64_t v_token_stride, v_head_stride, o_token_stride, o_head_stride;
+  const int32_t *query_starts;
+  int32_t window_size, num_sink_tokens;
+  float scale;
+} memopt_latent_prompt_desc;
+int memopt_latent_prompt_attention(const memopt_latent_prompt_desc *desc, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,7 +16,8 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "memopt_C", "libmemopt_hip.so")
 SOURCES = ["pool.cpp", "quant.hip", "evict.hip", "attention.hip", "decode_int4.hip", "decode_fp16.hip", "prefill.hip",
-           "direct.hip", "batch.hip", "prompt.hip", "packed.hip", "scores.hip", "compact.hip", "latent.hip"]
+           "direct.hip", "batch.hip", "prompt.hip", "packed.hip", "scores.hip", "compact.hip", "latent.hip",
+           "latent_prompt.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = os.environ.get("MEMOPT_ARCH", "gfx950")

@@ -219,8 +219,7 @@ __global__ __launch_bounds__(RW * 128, 1) void latent_kernel(const LatentParams 
         const bool there = (ok >> g) & 1;
         const uint8_t *base = reinterpret_cast<const uint8_t *>(p.c) + (there ? (int64_t)e : 0) * p.page_bytes +
                               (int64_t)(chunk - p.by_chunks(chunk) * (int32_t)p.by_chunks.d) * CB;
-        const int range = __builtin_amdgcn_readfirstlane(there ? max(0, min(16, s.len - key)) * RB : 0);
-        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)uniform_ptr(base), (short)0, range, 0x00020000);
+        const auto rsrc = uniform_rsrc(base, there ? max(0, min(16, s.len - key)) * RB : 0);
         const uint32_t to = lds_u32(lds) + buf * BUF + g * CB;
 #pragma unroll
         for (int c = 0; c < NCOPY; ++c) lds_dma<0, 1>(rsrc, to + c * 1024, off + c, 0);

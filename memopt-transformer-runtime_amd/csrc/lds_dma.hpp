@@ -53,6 +53,18 @@ __device__ __forceinline__ void lds_dma_range(__amdgpu_buffer_rsrc_t r, uint32_t
   }
 }
 
+// The descriptor of `range` bytes from a wave-uniform address for the copies
+// above, settled: a scalar register that a vector instruction wrote
+// (v_readfirstlane here) must not be read by a buffer instruction within five
+// wait states, which the compiler keeps for its own instructions but not for
+// those in inline assembly.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t uniform_rsrc(const void *base, int range) {
+  __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *)uniform_ptr((const uint8_t *)base), (short)0,
+                                                               __builtin_amdgcn_readfirstlane(range), 0x00020000);
+  asm volatile("s_nop 4" : "+s"(r));
+  return r;
+}
+
 // LDS byte address of a __shared__ object, wave-uniform.
 __device__ __forceinline__ uint32_t lds_u32(const void *p) {
   return __builtin_amdgcn_readfirstlane(

@@ -353,7 +353,7 @@ __global__ __launch_bounds__(256, 2) void chunk_rows_kernel(const ScoresParams p
     auto load_q = [&](int32_t t, int buf) __attribute__((always_inline)) {
       const int32_t tok0 = p.by_g(t * TR);
       const uint8_t *base = reinterpret_cast<const uint8_t *>(p.q + (int64_t)(s.start + tok0) * p.q_ts + (int64_t)h * p.G * p.q_hs);
-      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)uniform_ptr(base), (short)0, 0x7FFFFFFF, 0x00020000);
+      const auto rsrc = uniform_rsrc(base, 0x7FFFFFFF);
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         const int lrow = (wave * NC + c) * RPC + lane / CPR;

@@ -79,7 +79,8 @@ __device__ __forceinline__ bool find_tile(const Params &p, int32_t rank, Tile &o
   auto tiles_of = [&](int32_t b) {
     if (b >= p.B) return 0;
     const int32_t n = rows_of(p.starts, p.T, b).n;
-    if (PAGED && !is_staged(p.st, n, p.G)) return 0;
+    if constexpr (PAGED)
+      if (!is_staged(p.st, n, p.G)) return 0;
     return (n * p.G + R - 1) / R;
   };
   if (p.B == 1) {

@@ -151,6 +151,7 @@ _c_compact_ws = _sig("memopt_compact_workspace_size", [ctypes.c_char_p, ctypes.P
 _c_compact = _sig("memopt_compact_cache", [ctypes.c_char_p, _vp])
 _c_latent_ws = _sig("memopt_latent_workspace_size", [ctypes.c_char_p, ctypes.POINTER(_i64)])
 _c_latent = _sig("memopt_latent_attention", [ctypes.c_char_p, _vp])
+_c_latent_prompt = _sig("memopt_latent_prompt_attention", [ctypes.c_char_p, _vp])
 _c_write_latent = _sig("memopt_write_latent", [_vp, _i64, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _i64, _vp])
 
 KV_FP16, KV_INT4, KV_INT4_ROWS = 0, 1, 2
@@ -1503,4 +1504,60 @@ def latent_attention(query: torch.Tensor, cache: torch.Tensor, block_tables: tor
             nb, block_tables.data_ptr(), M, context_lens.data_ptr(), cu_seqlens.data_ptr(), _count32(max_query_len),
             _count32(max_seq_len), _count32(window_size), _count32(num_sink_tokens), float(scale))
     _launch(fn, _LATENT, head, _c_latent_ws, _c_latent, device)
+    return out
+
+
+_LATENT_PROMPT = struct.Struct("@5P6i9qP2if")  # memopt_latent_prompt_desc (4 bytes of padding follow)
+
+
+def latent_prompt_attention(query: torch.Tensor, keys: torch.Tensor, rope_keys: torch.Tensor, values: torch.Tensor,
+                            cu_seqlens: torch.Tensor, window_size: int = -1, *, num_sink_tokens: int = 0,
+                            scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention over whole packed prompts of a latent model (expanded form); returns ``[T, H, D]``.
+
+    Head h's key of a token is its row of ``keys`` ``[T, H, D]`` and, shared
+    by all heads, that of ``rope_keys`` ``[T, P]``; ``query`` ``[T, H, D +
+    P]`` holds the matching parts side by side, ``values`` are ``[T, H, D]``.
+    fp16 or bf16, D 64 or 128, P 32 or 64; ``scale`` defaults to one over the
+    root of D + P. Prompts, masks, strides and rows of no sequence are as in
+    ``prompt_attention``: views (of the up-projection's output, say) are read
+    in place. ``out`` must not overlap the inputs.
+    """
+    fn = "latent_prompt_attention"
+    if not (isinstance(query, torch.Tensor) and query.is_cuda):
+        raise RuntimeError(f"{fn}: query must be a CUDA tensor")
+    device, dtype = query.device, query.dtype
+    index = device.index
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(device):
+            return latent_prompt_attention(query, keys, rope_keys, values, cu_seqlens, window_size,
+                                           num_sink_tokens=num_sink_tokens, scale=scale, out=out)
+    _device_tensors(fn, device, ("keys", "rope_keys", "values", "cu_seqlens"), keys, rope_keys, values, cu_seqlens)
+    _no_grad(fn, query.requires_grad or keys.requires_grad or rope_keys.requires_grad or values.requires_grad)
+    if not (query.dim() == 3 and keys.dim() == 3 and rope_keys.dim() == 2 and values.dim() == 3):
+        raise RuntimeError(f"{fn}: query, keys and values must be 3-D [tokens, heads, elements], rope_keys 2-D")
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
+        raise RuntimeError(f"{fn}: query must be fp16 or bf16")
+    if not (keys.dtype is dtype and rope_keys.dtype is dtype and values.dtype is dtype):
+        raise RuntimeError(f"{fn}: keys, rope_keys and values must have query's dtype")
+    T, H, W = query.shape
+    D, P = keys.shape[2], rope_keys.shape[1]
+    if not (keys.shape == (T, H, D) and values.shape == keys.shape and rope_keys.shape[0] == T and D + P == W):
+        raise RuntimeError(f"{fn}: keys and values must be [{T}, {H}, D] and rope_keys [{T}, P] with D + P = {W}, got "
+                           f"{list(keys.shape)}, {list(values.shape)} and {list(rope_keys.shape)}")
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
+        raise RuntimeError(f"{fn}: cu_seqlens must be 1-D [batch + 1]")
+    _int32(fn, cu_seqlens, "cu_seqlens", cu_seqlens.shape)
+    out, po, ots, ohs = _out_rows(fn, out, query, D)
+    q, pq, qts, qhs = _rows(query)
+    k, pk, kts, khs = _rows(keys, _FAR)
+    r, pr, rts, _ = _rows(rope_keys[:, None], _FAR)
+    v, pv, vts, vhs = _rows(values, _FAR)
+    try:
+        d = _LATENT_PROMPT.pack(pq, pk, pr, pv, po, 1 if dtype is torch.bfloat16 else 0, T, cu_seqlens.shape[0] - 1, H, D, P,
+                                qts, qhs, kts, khs, rts, vts, vhs, ots, ohs, cu_seqlens.data_ptr(), _count32(window_size),
+                                _count32(num_sink_tokens), W ** -0.5 if scale is None else float(scale))
+    except struct.error:
+        raise RuntimeError(f"{fn}: sizes must fit 32 bits") from None
+    _check(_c_latent_prompt(d + b"\0\0\0\0", torch._C._cuda_getCurrentRawStream(index)))
     return out
