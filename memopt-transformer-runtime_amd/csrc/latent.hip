@@ -21,6 +21,8 @@
 
 namespace memopt {
 
+typedef float f32x2m_t __attribute__((ext_vector_type(2)));
+
 struct LatentParams {
   const uint16_t *q, *c;
   uint16_t *out;
@@ -123,7 +125,7 @@ struct LatentLds {
   static constexpr int weights = tiles, tops = weights + RW * 2 * 2048, bytes = tops + RW * 2 * 128;
 };
 template <class E, int R, int P, int RW>
-__global__ __launch_bounds__(RW * 128, 1) void latent_kernel(const LatentParams p) {
+__global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_kernel(const LatentParams p) {
   constexpr int W = R + P, RB = 2 * W, NCH = W / 16, NDB = R / 64, NW = 2 * RW, ROWS = 32 * RW;
   constexpr int CB = 16 * RB, NCOPY = CB / 1024, CPW = 4 / NW;  // a 16-token chunk's bytes and copies; chunks per wave
   constexpr int BUF = 4 * CB;
@@ -146,9 +148,11 @@ __global__ __launch_bounds__(RW * 128, 1) void latent_kernel(const LatentParams 
   // eight rows nor those of 32 bytes of four rows meet a bank twice (rows are
   // 32 banks apart where R + P is an odd multiple of 64).
   auto swz = [](int row) { return 2 * ((row >> 1) & 1) + ((row >> 2) & 1); };
-  uint32_t off[NCOPY];
+  // (copies of the chunk's second eight rows, where they begin a copy, differ from those of the first by an offset)
+  constexpr int NOFF = NCOPY % 2 ? NCOPY : NCOPY / 2;
+  uint32_t off[NOFF];
 #pragma unroll
-  for (int c = 0; c < NCOPY; ++c) {
+  for (int c = 0; c < NOFF; ++c) {
     const int piece = c * 64 + lane, row = piece / (RB / 16), j = piece % (RB / 16);
     off[c] = row * RB + 16 * (j ^ swz(row));
   }
@@ -188,41 +192,47 @@ __global__ __launch_bounds__(RW * 128, 1) void latent_kernel(const LatentParams 
 #pragma unroll
       for (int c = 0; c < NCH; ++c) qf[c] = *reinterpret_cast<const u32x4p_t *>(src + 16 * c);
     }
-    // (waited for here: the first product would wait for them, and with them for every copy before, in each iteration)
+    // Waited for here: the first product would wait for them, and with them for every copy before, in each iteration.
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    __builtin_amdgcn_sched_barrier(0);
+
+    // Most of them live in accumulation registers beside the sums (a hint, without which the loop spills at 512 + 64).
+    constexpr int kInAcc = (240 - 16 * NDB) / 4;
 #pragma unroll
-    for (int c = 0; c < NCH; ++c) asm volatile("" : "+v"(qf[c]));
+    for (int c = 0; c < (NCH < kInAcc ? NCH : kInAcc); ++c) asm volatile("" : "+a"(qf[c]));
 
     // Pages of a tile's four chunks, and its copies. An entry that is no page, and rows behind the context, read as zeros.
-    int32_t entry[4];
+    int32_t e0 = -1, e1 = -1, e2 = -1, e3 = -1;  // (no array: chosen from by wave, it would go through scratch memory)
+    auto entry_at = [&](int32_t key) __attribute__((always_inline)) {
+      return key < s.len ? uniform_entry(p.bt + (int64_t)b * p.M + p.by_chunks(key >> 4)) : -1;
+    };
     auto look_up = [&](int32_t it) __attribute__((always_inline)) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int32_t key = tile_base(it) + 16 * g;
-        entry[g] = key < s.len ? uniform_entry(p.bt + (int64_t)b * p.M + p.by_chunks(key >> 4)) : -1;
-      }
+      const int32_t key = tile_base(it);
+      e0 = entry_at(key);
+      e1 = entry_at(key + 16);
+      e2 = entry_at(key + 32);
+      e3 = entry_at(key + 48);
     };
     uint32_t links0 = 0, links1 = 0;  // bit g: chunk g of the tile in buffer 0 or 1 is there
     auto load = [&](int32_t it, int buf) __attribute__((always_inline)) {
-      uint32_t ok = 0;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) ok |= (entry[g] >= 0 && entry[g] < p.nb ? 1u : 0u) << g;
-      ok = __builtin_amdgcn_readfirstlane(ok);
+      auto there = [&](int32_t e) { return e >= 0 && e < p.nb; };
+      const uint32_t ok = __builtin_amdgcn_readfirstlane((there(e0) ? 1u : 0u) | (there(e1) ? 2u : 0u) | (there(e2) ? 4u : 0u) |
+                                                         (there(e3) ? 8u : 0u));
       links0 = buf ? links0 : ok;
       links1 = buf ? ok : links1;
 #pragma unroll
       for (int i = 0; i < CPW; ++i) {
         const int g = wave * CPW + i;
-        int32_t e = entry[0];
-#pragma unroll
-        for (int j = 1; j < 4; ++j) e = g == j ? entry[j] : e;
+        const int32_t e = CPW == 2 ? (wave == 0 ? (i ? e1 : e0) : (i ? e3 : e2))
+                                   : wave == 0 ? e0 : wave == 1 ? e1 : wave == 2 ? e2 : e3;
         const int32_t key = tile_base(it) + 16 * g, chunk = key >> 4;
-        const bool there = (ok >> g) & 1;
-        const uint8_t *base = reinterpret_cast<const uint8_t *>(p.c) + (there ? (int64_t)e : 0) * p.page_bytes +
+        const uint8_t *base = reinterpret_cast<const uint8_t *>(p.c) + (there(e) ? (int64_t)e : 0) * p.page_bytes +
                               (int64_t)(chunk - p.by_chunks(chunk) * (int32_t)p.by_chunks.d) * CB;
-        const auto rsrc = uniform_rsrc(base, there ? max(0, min(16, s.len - key)) * RB : 0);
+        const auto rsrc = uniform_rsrc(base, there(e) ? max(0, min(16, s.len - key)) * RB : 0);
         const uint32_t to = lds_u32(lds) + buf * BUF + g * CB;
 #pragma unroll
-        for (int c = 0; c < NCOPY; ++c) lds_dma<0, 1>(rsrc, to + c * 1024, off + c, 0);
+        for (int c = 0; c < NCOPY; ++c) lds_dma<0, 1>(rsrc, to + c * 1024, off + c % NOFF, c < NOFF ? 0 : 8 * RB);
       }
     };
 
@@ -233,7 +243,7 @@ __global__ __launch_bounds__(RW * 128, 1) void latent_kernel(const LatentParams 
     // and the next rescale comes past kTop + 8 (prompt.hip).
     constexpr float kTop = 7.0f;
     float ncm = 0.0f, thr = -INFINITY, lsum = 0.0f;
-    uint32_t odd = 0;
+    bool odd = false;  // a tile of this part held inf or NaN that was made finite
     const bool any = qw0 < s.rows;
     const int32_t pos_first = pos_of(qw0), pos_last = pos_of(qw0 + 31);
     // Whether all this wave's rows see the 32 keys from k0 on; whether any sees one.
@@ -249,9 +259,26 @@ __global__ __launch_bounds__(RW * 128, 1) void latent_kernel(const LatentParams 
     // Scores of this wave's 32 keys, in log2 units, hidden ones -inf.
     auto scores = [&](const uint8_t *kt, int32_t k0, uint32_t link, f32x16_t &x) __attribute__((always_inline)) {
       x = (f32x16_t){};
+      // Operands are read a group of products ahead: a wave has its SIMD to itself and nothing else hides an LDS read.
+      constexpr int GR = 4, NG = (NCH + GR - 1) / GR;
+      u32x4p_t f[2][GR];
+      auto read = [&](int g) __attribute__((always_inline)) {
 #pragma unroll
-      for (int c = 0; c < NCH; ++c)
-        x = E::mfma(*reinterpret_cast<const u32x4p_t *>(kt + ka[c & 1] + 64 * (c >> 1)), qf[c], x);
+        for (int i = 0; i < GR; ++i)
+          if (g * GR + i < NCH)
+            f[g & 1][i] = *reinterpret_cast<const u32x4p_t *>(kt + ka[i & 1] + 64 * ((g * GR + i) >> 1));
+      };
+      read(0);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (g + 1 < NG) read(g + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < GR; ++i)
+          if (g * GR + i < NCH) x = E::mfma(f[g & 1][i], qf[g * GR + i], x);
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], p.scale_log2, ncm);
       if (full(k0, link)) return;
@@ -286,29 +313,50 @@ __global__ __launch_bounds__(RW * 128, 1) void latent_kernel(const LatentParams 
       ncm -= shift;
       thr = (start && !found) ? thr : kTop + 8.0f;
     };
-    auto add_values = [&](const uint8_t *kt, bool whole, const u32x4p_t (&pb)[4]) __attribute__((always_inline)) {
+    // Values of 16 keys and 32 columns, transposed by the read.
+    auto values = [&](const uint8_t *kt, int db, int i) __attribute__((always_inline)) {
+      const uint8_t *src = kt + va + 64 * db + 16 * i * RB;
+      const u32x2p_t a = v_read(src, 0), b8 = v_read(src + 8 * RB, 0);
+      return u32x4p_t{a[0], a[1], b8[0], b8[1]};
+    };
+    // `first`: the values of the first 32 columns, read before the weights were there.
+    auto add_values = [&](const uint8_t *kt, const u32x4p_t (&pb)[4], const u32x4p_t (&first)[4]) __attribute__((always_inline)) {
+      u32x4p_t v[2][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[0][i] = first[i];
 #pragma unroll
       for (int db = 0; db < NDB; ++db) {
-        u32x4p_t v[4];
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint8_t *src = kt + va + 64 * db + 16 * i * RB;
-          const u32x2p_t a = v_read(src, 0), b8 = v_read(src + 8 * RB, 0);
-          v[i] = u32x4p_t{a[0], a[1], b8[0], b8[1]};
-        }
-        if (!whole) {
-          // A weight of 0 must not meet an inf or NaN: a sum of zero times every element tells.
-          float z = 0.0f;
+        for (int i = 0; i < 4; ++i)
+          if (db + 1 < NDB) v[(db + 1) & 1][i] = values(kt, db + 1, i);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) z = E::dot2(v[i >> 2][i & 3], 0, z);
-          if (__any(!(z == 0.0f))) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i >> 2][i & 3] = tame<E>(v[i >> 2][i & 3], odd);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[db] = E::mfma(v[i], pb[i], o[db]);
+        for (int i = 0; i < 4; ++i) o[db] = E::mfma(v[db & 1][i], pb[i], o[db]);
       }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    // A weight of 0 must not meet an inf or NaN. Where a tile has a token that
+    // some row of the workgroup does not see, such values become finite in LDS
+    // (after all scores were taken), and rows that do see one get it at the end.
+    const int32_t group_first = pos_of(q0), group_last = pos_of(q0 + ROWS - 1);
+    auto hides = [&](int32_t tb) {
+      return min(tb + kLatentKeys, s.len) - 1 > group_first || (tb <= group_last - p.W && tb + kLatentKeys > p.sinks);
+    };
+    auto tame_tile = [&](uint8_t *kt) __attribute__((always_inline)) {
+      uint32_t changed = 0;
+#pragma unroll 1
+      for (int i = threadIdx.x; i < kLatentKeys * (R / 8); i += 64 * NW) {
+        const int row = i / (R / 8), j = i % (R / 8);
+        u32x4p_t *const at = reinterpret_cast<u32x4p_t *>(kt + row * RB + 16 * (j ^ swz(row)));
+        u32x4p_t v = *at;
+        uint32_t odd = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = tame<E>(v[k], odd);
+        if (odd) *at = v;
+        changed |= odd;
+      }
+      return changed;
     };
 
     if (i0 < i1) {
@@ -340,7 +388,7 @@ __global__ __launch_bounds__(RW * 128, 1) void latent_kernel(const LatentParams 
         if (hl == 0) s_tops[32 * kw + n] = t;
       }
       __syncthreads();
-      u32x4p_t pb[4];
+      u32x4p_t pb[4], first[4];
       if (some) {
         raise_max(fmaxf(s_tops[n], s_tops[32 + n]), x);
         // Weights enter the second product in 16 bits, and so the row's sum.
@@ -352,42 +400,22 @@ __global__ __launch_bounds__(RW * 128, 1) void latent_kernel(const LatentParams 
 #pragma unroll
         for (int i = 0; i < 2; ++i) s_weights[128 * kw + 64 * i] = mine[i];
       }
+      if (hides(tb)) odd |= __syncthreads_or((int)tame_tile(lds + buf * BUF)) != 0;
+      if (some) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) first[i] = values(kt, 0, i);
+      }
       __syncthreads();
       if (some) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) pb[i] = s_weights[64 * i];
-        add_values(kt, full(tb, link & 3) && full(tb + 32, link >> 2), pb);
+        add_values(kt, pb, first);
       }
       __syncthreads();
       if (it + 2 < i1) {
         load(it + 2, buf);
         if (it + 3 < i1) look_up(it + 3);
       }
-    }
-
-    if (__any(odd != 0)) {
-      // inf and NaN entered the masked blocks as finite values: rows that do see one get it, whatever its weight.
-      const int32_t row = lane_row(), qp = pos_of(row);
-#pragma unroll 1
-      for (int32_t it = i0; it < i1; ++it) {
-          const int32_t k0 = tile_base(it);
-          if (!seen(k0) && !seen(k0 + 32)) continue;
-#pragma unroll 1
-          for (int32_t key = k0; key < min(k0 + kLatentKeys, s.len); ++key) {
-            const int32_t chunk = key >> 4, e = p.bt[(int64_t)b * p.M + p.by_chunks(chunk)];
-            if (e < 0 || e >= p.nb) continue;
-            const bool see = row < s.rows && key <= qp && (key < p.sinks || key > qp - p.W);
-            const uint16_t *src = reinterpret_cast<const uint16_t *>(
-                                      reinterpret_cast<const uint8_t *>(p.c) + (int64_t)e * p.page_bytes +
-                                      (int64_t)(chunk - p.by_chunks(chunk) * (int32_t)p.by_chunks.d) * CB + (key & 15) * RB) +
-                                  4 * hl + 32 * NDB * kw;
-#pragma unroll
-            for (int r = 0; r < 16 * NDB; ++r) {
-              const uint16_t bits = src[8 * (r >> 2) + (r & 3)];
-              if (see && (bits & E::kExponent) == E::kExponent) o[r >> 4][r & 15] += E::value(bits);
-            }
-          }
-        }
     }
 
     // The pair's row sums.
@@ -422,6 +450,34 @@ __global__ __launch_bounds__(RW * 128, 1) void latent_kernel(const LatentParams 
           *reinterpret_cast<f32x4p_t *>(dst + 32 * db + 8 * g) =
               f32x4p_t{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
     }
+    if (odd && row < s.rows) {
+      // Rows that see an inf or NaN that was made finite have it in that column whatever its weight.
+      const int32_t qp = pos_of(row), tok = p.by_h(row);
+      const bool direct = first_step == 0 && last_step == s.steps;
+      uint16_t *const out = p.out + (int64_t)(s.start + tok) * p.o_ts + (int64_t)(row - tok * p.H) * p.o_hs;
+      float *const part = p.ws_o + (((int64_t)w * 2 + (at == begin ? 0 : 1)) * ROWS + 32 * rw + n) * R;
+#pragma unroll 1
+      for (int32_t it = i0; it < i1; ++it) {
+        const int32_t tb = tile_base(it);
+        if (!hides(tb)) continue;
+#pragma unroll 1
+        for (int32_t key = tb; key < min(tb + kLatentKeys, s.len); ++key) {
+          const int32_t chunk = key >> 4, e = p.bt[(int64_t)b * p.M + p.by_chunks(chunk)];
+          if (e < 0 || e >= p.nb || key > qp || (key >= p.sinks && key <= qp - p.W)) continue;
+          const uint16_t *src = reinterpret_cast<const uint16_t *>(
+              reinterpret_cast<const uint8_t *>(p.c) + (int64_t)e * p.page_bytes +
+              (int64_t)(chunk - p.by_chunks(chunk) * (int32_t)p.by_chunks.d) * CB + (key & 15) * RB);
+#pragma unroll 1
+          for (int i = 0; i < 16 * NDB; ++i) {
+            const int d = 32 * NDB * kw + 8 * (i >> 2) + 4 * hl + (i & 3);
+            const uint16_t bits = src[d];
+            if ((bits & E::kExponent) != E::kExponent) continue;
+            if (direct) out[d] = (uint16_t)E::pack(E::value(out[d]) + E::value(bits), 0.0f);
+            else part[d] += E::value(bits);
+          }
+        }
+      }
+    }
     at += (uint32_t)(last_step - first_step);
     __syncthreads();  // the space is free for the next tiles
   }
@@ -444,20 +500,49 @@ __global__ __launch_bounds__(256) void latent_merge_kernel(const LatentParams p)
   if (w0 == w1) return;
   // The first of them began the unit behind its run's begin, or with it.
   auto slot_of = [&](uint32_t w) { return ((int64_t)w * 2 + (w == w0 && s0 != w * run ? 1 : 0)) * ROWS + r; };
+  // Maxima and sums 64 parts at a time, one per lane; then the parts' rows, four reads in flight.
+  const uint32_t parts = w1 - w0 + 1;
   float top = -INFINITY, l = 0.0f, acc[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) acc[i] = 0.0f;
-  for (uint32_t w = w0; w <= w1; ++w) top = fmaxf(top, p.ws_ml[slot_of(w)].x);
-  for (uint32_t w = w0; w <= w1; ++w) {
-    const int64_t slot = slot_of(w);
-    const float2 ml = p.ws_ml[slot];
-    if (ml.x == -INFINITY) continue;
-    const float f = fast_exp2(ml.x - top);
-    l = fmaf(ml.y, f, l);
-    const float *src = p.ws_o + slot * R + lane * PER;
+  for (uint32_t i0 = 0; i0 < parts; i0 += 64)
+    top = fmaxf(top, i0 + lane < parts ? p.ws_ml[slot_of(w0 + i0 + lane)].x : -INFINITY);
+  top = wave_max(top);
+  for (uint32_t i0 = 0; i0 < parts; i0 += 64) {
+    const float2 ml = i0 + lane < parts ? p.ws_ml[slot_of(w0 + i0 + lane)] : float2{-INFINITY, 0.0f};
+    const float f = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - top);
+    l += f == 0.0f ? 0.0f : ml.y * f;
+    const uint32_t n = min(64u, parts - i0);
+    for (uint32_t i = 0; i < n; i += 4) {
+      f32x4p_t v[4][PER / 4 ? PER / 4 : 1];
+      f32x2m_t v2[4];
+      float g[4];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = fmaf(src[i], f, acc[i]);
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t j = min(i + k, n - 1);
+        g[k] = i + k < n ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), j)) : 0.0f;
+        const float *src = p.ws_o + slot_of(w0 + i0 + j) * R + lane * PER;
+        if constexpr (PER == 2) v2[k] = *reinterpret_cast<const f32x2m_t *>(src);
+        else
+#pragma unroll
+          for (int x = 0; x < PER / 4; ++x) v[k][x] = *reinterpret_cast<const f32x4p_t *>(src + 4 * x);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (g[k] == 0.0f) continue;  // (nothing seen there: its row may hold anything)
+#pragma unroll
+        for (int x = 0; x < PER; ++x) {
+          if constexpr (PER == 2) acc[x] = fmaf(v2[k][x], g[k], acc[x]);
+          else acc[x] = fmaf(v[k][x / 4][x & 3], g[k], acc[x]);
+        }
+      }
+    }
   }
+  l += xor1(l);
+  l += xor2(l);
+  l += half_mirror(l);
+  l += dpp_f32<0x140>(l);
+  l = xor32_sum(xor16_sum(l));
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
   const int32_t tok = p.by_h(row);
   uint32_t *dst = reinterpret_cast<uint32_t *>(p.out + (int64_t)(s.start + tok) * p.o_ts + (int64_t)(row - tok * p.H) * p.o_hs +
