@@ -9,9 +9,14 @@
 // (in place, a row's new place is another row's old one, so one workgroup
 // would have to walk a whole sequence), and leaves the old pages whole.
 //
-// Three launches: what each request gets (one workgroup: prefix sums over the
-// requests, as in batch.hip), which tokens stay (one workgroup per request and
-// key head: radix selection), and the copies (one wave per page and head).
+// Three launches. The first counts each request's tokens (a workgroup each).
+// The second finds the tokens that stay (a workgroup per request and key head:
+// radix selection); the workgroup that ends last also says what each request
+// gets, by prefix sums over the requests as in batch.hip. The third copies (a
+// wave per 16 new tokens and head) and writes tables and ring.
+//
+// Bound by the copies where requests are long, else by the chain of launches
+// and of the selection's passes.
 #include <algorithm>
 
 #include "page_format.hpp"
@@ -28,73 +33,62 @@ struct CompactParams {
   int32_t N, Hk, D, M, bs, C, L, K, sinks, recent;
   const int32_t *bt, *ctx, *keep, *span;
   int32_t *bt_out, *ctx_out, *status, *ring, *span_out;
-  int32_t *stay;   // [N]: tokens that stay per head, -1 where the request is left as it is
-  int32_t *holes;  // [N]: 1 where a page of the context is not linked
-  int32_t *marks;  // [nb]
+  // workspace
+  int32_t *stay;    // [N]: tokens that stay per head, -1 where the request is left as it is
+  int32_t *holes;   // [N]: 1 where a page of the context is not linked
+  int32_t *back;    // [N]: linked pages; then the first place that they get at the ring's end
+  int32_t *fresh;   // [N]: the first fresh page's place in the ring, from its front
+  int32_t *state;   // [N]: MEMOPT_COMPACT_*, as far as it is known
+  int32_t *counts;  // [4]: workgroups of the second launch that ended; the ring's front and pages
+  int32_t *marks;   // [nb]
+  int32_t in_lds;   // tokens whose orders the selection keeps in LDS
 };
 
 static constexpr int32_t kMaxCompacted = 4096;
 
 __device__ __forceinline__ bool page_ok(const CompactParams &p, int32_t page) { return page >= 0 && page < p.nb; }
 
-// Live tokens of a row's first `have` pages, and whether a page is missing. One wave.
-__device__ __forceinline__ int32_t live_tokens(const CompactParams &p, int32_t b, int32_t c, int32_t have) {
-  const int lane = threadIdx.x & 63;
-  int32_t live = 0;
-  for (int32_t i = lane; i < have; i += 64)
-    if (page_ok(p, p.bt[(int64_t)b * p.M + i])) live += min(p.bs, c - i * p.bs);
-  return wave_sum(live);
+// What a request holds and asks for. A page that two entries list would go
+// back to the ring twice: each entry leaves its number at the page, and who
+// finds another's there (the second launch) tells both requests.
+__global__ __launch_bounds__(256) void compact_count_kernel(const CompactParams p) {
+  __shared__ int32_t s_part[2][4];
+  const int32_t b = blockIdx.x, c = p.ctx[b], keep = p.keep[b];
+  const bool bad = c < 0 || (int64_t)c > (int64_t)p.M * p.bs || c > p.L || keep > p.K;
+  const int32_t have = bad ? 0 : (c + p.bs - 1) / p.bs;
+  int32_t live = 0, back = 0;
+  for (int32_t i = threadIdx.x; i < have; i += 256) {
+    const int32_t page = p.bt[(int64_t)b * p.M + i];
+    if (!page_ok(p, page)) continue;
+    ++back;
+    live += min(p.bs, c - i * p.bs);
+    p.marks[page] = b * p.M + i;
+  }
+  live = wave_sum(live);
+  back = wave_sum(back);
+  if ((threadIdx.x & 63) == 0) {
+    s_part[0][threadIdx.x >> 6] = live;
+    s_part[1][threadIdx.x >> 6] = back;
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  live = s_part[0][0] + s_part[0][1] + s_part[0][2] + s_part[0][3];
+  back = s_part[1][0] + s_part[1][1] + s_part[1][2] + s_part[1][3];
+  const bool asks = !bad && keep >= 0 && live > keep;
+  p.stay[b] = asks ? keep : -1;
+  p.holes[b] = live < c;
+  p.back[b] = back;
+  p.state[b] = bad ? MEMOPT_COMPACT_INVALID : asks ? MEMOPT_COMPACT_DONE : MEMOPT_COMPACT_LEFT;
+  if (b == 0) p.counts[0] = 0;
 }
 
-// What each request gets: fresh pages in request order while they last.
-__global__ __launch_bounds__(1024) void compact_plan_kernel(const CompactParams p) {
-  __shared__ int32_t s_need[kMaxCompacted], s_back[kMaxCompacted], s_status[kMaxCompacted];
-  __shared__ uint32_t s_part[2][16];
+// What each request gets: sums of what is asked decide, sums of what is served
+// place; 1024 requests at a time. One workgroup of 1024 threads.
+__device__ __forceinline__ void plan_requests(const CompactParams &p, uint32_t (*s_part)[16]) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int32_t head = p.span[0] % p.C;
   if (head < 0) head += p.C;
   const int32_t count = min(max(p.span[1], 0), p.C);
-  // A page that two entries list would go back twice: each entry leaves its
-  // number at the page, and who finds another's tells both requests.
-  for (int32_t b = wave; b < p.N; b += 16) {
-    const int32_t c = p.ctx[b], keep = p.keep[b];
-    const bool bad = c < 0 || (int64_t)c > (int64_t)p.M * p.bs || c > p.L || keep > p.K;
-    const int32_t have = bad ? 0 : (c + p.bs - 1) / p.bs;
-    const int32_t live = live_tokens(p, b, c, have), n = min(keep, live);
-    const bool asks = !bad && keep >= 0 && live > keep;
-    int32_t back = 0;
-    for (int32_t i = lane; i < have; i += 64) {
-      const int32_t page = p.bt[(int64_t)b * p.M + i];
-      if (!page_ok(p, page)) continue;
-      ++back;
-      __hip_atomic_store(&p.marks[page], b * p.M + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    back = wave_sum(back);
-    if (lane == 0) {
-      s_status[b] = bad ? MEMOPT_COMPACT_INVALID : asks ? MEMOPT_COMPACT_DONE : MEMOPT_COMPACT_LEFT;
-      s_need[b] = asks ? (n + p.bs - 1) / p.bs : 0;
-      s_back[b] = asks ? back : 0;
-      p.stay[b] = asks ? n : -1;
-      p.holes[b] = live < c;
-    }
-  }
-  __threadfence();
-  __syncthreads();
-  for (int32_t b = wave; b < p.N; b += 16) {
-    if (s_status[b] == MEMOPT_COMPACT_INVALID) continue;
-    const int32_t have = (p.ctx[b] + p.bs - 1) / p.bs;
-    for (int32_t i = lane; i < have; i += 64) {
-      const int32_t page = p.bt[(int64_t)b * p.M + i];
-      if (!page_ok(p, page)) continue;
-      const int32_t id = __hip_atomic_load(&p.marks[page], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (id != b * p.M + i) {
-        atomicExch(&s_status[b], MEMOPT_COMPACT_SHARED);
-        atomicExch(&s_status[id / p.M], MEMOPT_COMPACT_SHARED);
-      }
-    }
-  }
-  __syncthreads();
-  // Requests in order, 1024 at a time: sums of what is asked decide, sums of what is served place.
   uint32_t asked_need = 0, asked_back = 0, got_need = 0, got_back = 0;
   auto scan = [&](uint32_t a, uint32_t z, uint32_t &ta, uint32_t &tz, uint32_t &ea, uint32_t &ez) {
     ea = wave_scan(a);
@@ -106,6 +100,7 @@ __global__ __launch_bounds__(1024) void compact_plan_kernel(const CompactParams 
     }
     __syncthreads();
     ta = tz = 0;
+#pragma unroll
     for (int w = 0; w < 16; ++w) {
       if (w == wave) {
         ea = __builtin_elementwise_add_sat(ea, ta);
@@ -117,11 +112,12 @@ __global__ __launch_bounds__(1024) void compact_plan_kernel(const CompactParams 
   };
   for (int32_t b0 = 0; b0 < p.N; b0 += 1024) {
     const int32_t b = b0 + (int32_t)threadIdx.x;
-    int32_t st = b < p.N ? s_status[b] : MEMOPT_COMPACT_INVALID;
+    int32_t st = b < p.N ? __hip_atomic_load(&p.state[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : MEMOPT_COMPACT_INVALID;
     uint32_t need = 0, back = 0, ta, tz, ea, ez;
+    const int32_t stay = b < p.N ? p.stay[b] : 0;
     if (st == MEMOPT_COMPACT_DONE) {
-      need = (uint32_t)s_need[b];
-      back = (uint32_t)s_back[b];
+      need = (uint32_t)((stay + p.bs - 1) / p.bs);
+      back = (uint32_t)p.back[b];
     }
     scan(need, back, ta, tz, ea, ez);
     if (st == MEMOPT_COMPACT_DONE && (__builtin_elementwise_add_sat(asked_need, ea) > (uint32_t)count ||
@@ -132,158 +128,159 @@ __global__ __launch_bounds__(1024) void compact_plan_kernel(const CompactParams 
     if (st != MEMOPT_COMPACT_DONE) need = back = 0;
     scan(need, back, ta, tz, ea, ez);
     if (b < p.N) {
-      const int32_t c = p.ctx[b];
-      if (st != MEMOPT_COMPACT_DONE) p.stay[b] = -1;
-      p.status[b] = s_status[b] = st;
-      p.ctx_out[b] = st == MEMOPT_COMPACT_DONE ? p.stay[b] : c;
-      s_need[b] = (int32_t)(got_need + ea - need);  // first fresh page, first place at the ring's end
-      s_back[b] = (int32_t)(got_back + ez - back);
+      p.status[b] = st;
+      p.ctx_out[b] = st == MEMOPT_COMPACT_DONE ? stay : p.ctx[b];
+      p.fresh[b] = (int32_t)(got_need + ea - need);
+      p.back[b] = (int32_t)(got_back + ez - back);
     }
     got_need += ta;
     got_back += tz;
   }
-  __syncthreads();
-  for (int32_t b = wave; b < p.N; b += 16) {
-    const int64_t row = (int64_t)b * p.M;
-    if (s_status[b] != MEMOPT_COMPACT_DONE) {
-      for (int32_t i = lane; i < p.M; i += 64) p.bt_out[row + i] = p.bt[row + i];
-      continue;
-    }
-    const int32_t need = (__hip_atomic_load(&p.stay[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + p.bs - 1) / p.bs;
-    const int32_t have = (p.ctx[b] + p.bs - 1) / p.bs;
-    for (int32_t i = lane; i < p.M; i += 64)
-      p.bt_out[row + i] = i < need ? p.ring[(int32_t)(((int64_t)head + s_need[b] + i) % p.C)] : -1;
-    int32_t at = s_back[b];
-    for (int32_t i0 = 0; i0 < have; i0 += 64) {
-      const int32_t page = i0 + lane < have ? p.bt[row + i0 + lane] : -1;
-      const uint64_t m = __ballot(page_ok(p, page));
-      if (page_ok(p, page))
-        p.ring[(int32_t)(((int64_t)head + count + at + __popcll(m & ((1ull << lane) - 1))) % p.C)] = page;
-      at += (int32_t)__popcll(m);
-    }
-  }
   if (threadIdx.x == 0) {
+    p.counts[1] = head;
+    p.counts[2] = count;
     p.span_out[0] = (int32_t)(((int64_t)head + got_need) % p.C);
     p.span_out[1] = count - (int32_t)got_need + (int32_t)got_back;
   }
 }
 
-// Scores as integers in their order; NaN lowest, both zeros alike.
+// Scores as integers in their order, above 0 and below ~0; NaN lowest, both zeros alike.
 __device__ __forceinline__ uint32_t order_of(float x) {
   uint32_t u = __float_as_uint(x);
   if ((u << 1) == 0) u = 0;
-  if ((u & 0x7FFFFFFFu) > 0x7F800000u) return 0;
+  if ((u & 0x7FFFFFFFu) > 0x7F800000u) return 1;
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+static constexpr uint32_t kGone = 0, kStays = 0xFFFFFFFFu;  // orders of tokens that no score decides about
 
-// The tokens that stay, per request and key head: the value of the last one
-// to stay is found digit by digit (11, 11 and 10 bits) from histograms, then
-// each wave lists its part of the row in order.
-__global__ __launch_bounds__(1024) void compact_select_kernel(const CompactParams p) {
+// The tokens that stay, per request and key head: the order of the last one
+// to stay is found digit by digit (8 bits each) from histograms, then
+// each wave lists its part of the row. Orders of rows of up to kInLds tokens
+// are worked out once and kept in LDS (in registers, the unrolled passes are
+// 80 KB of code, whose fetch took longer than they did: 1024 tokens 15 us);
+// longer rows are read in every pass. Lanes that meet in one bin or bank wait
+// for each other, and scores have few exponents: a bin has sixteen counters
+// side by side, for every sixteenth lane.
+static constexpr int kInLds = 28672;
+struct SelectShared {
+  uint4 hist[256][4];
+  uint32_t part[16], eq[16], gt[16], bin, above, safe;
+};
+template <bool LDS>
+__device__ __forceinline__ void select_row(const CompactParams &p, SelectShared &sh, uint32_t *s_key, int32_t b,
+                                           const float *src, float *dst, int32_t *kept, int32_t n) {
   constexpr int NW = 16;
-  __shared__ uint32_t s_hist[2048];
-  __shared__ uint32_t s_part[NW], s_eq[NW], s_gt[NW], s_bin, s_above, s_safe;
-  const int32_t h = blockIdx.x, b = blockIdx.y;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t unit = (int64_t)b * p.Hk + h;
-  const float *src = p.scores + unit * p.L;
-  float *dst = p.scores_out + unit * p.L;
-  int32_t *kept = p.kept + unit * p.K;
-  const int32_t n = p.stay[b];
-  if (n < 0) {
-    for (int32_t j = threadIdx.x; j < p.L; j += 1024) dst[j] = src[j];
-    for (int32_t j = threadIdx.x; j < p.K; j += 1024) kept[j] = -1;
-    return;
-  }
   const int32_t c = p.ctx[b], sinks = min(p.sinks, n), recent0 = c - min(p.recent, n - sinks);
   const bool holes = p.holes[b] != 0;
   auto live = [&](int32_t j) { return !holes || page_ok(p, p.bt[(int64_t)b * p.M + j / p.bs]); };
   auto safe = [&](int32_t j) { return j < sinks || j >= recent0; };
-
-  // Protected tokens.
-  if (threadIdx.x == 0) s_safe = 0;
-  __syncthreads();
-  if (holes) {
-    uint32_t x = 0;
-    for (int32_t j = threadIdx.x; j < c; j += 1024) x += safe(j) && live(j);
-    x = (uint32_t)wave_sum((int32_t)x);
-    if (lane == 0) atomicAdd(&s_safe, x);
-  } else if (threadIdx.x == 0) {
-    s_safe = (uint32_t)(sinks + c - recent0);  // (n <= c: they do not overlap)
-  }
-  __syncthreads();
-  uint32_t want = (uint32_t)n - s_safe;  // to be taken by score
-  uint32_t prefix = 0, mask = 0;
-  if (want > 0) {
-    constexpr int shifts[3] = {21, 10, 0}, widths[3] = {11, 11, 10};
-#pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-      const int shift = shifts[pass];
-      const uint32_t digits = (1u << widths[pass]) - 1;
-      for (int i = threadIdx.x; i < 2048; i += 1024) s_hist[i] = 0;
-      __syncthreads();
-      for (int32_t j = threadIdx.x; j < c; j += 1024) {
-        if (safe(j) || !live(j)) continue;
-        const uint32_t u = order_of(src[j]);
-        if ((u & mask) == prefix) atomicAdd(&s_hist[(u >> shift) & digits], 1u);
-      }
-      __syncthreads();
-      // Bins from the top: thread t holds bins 2047 - 2 t and 2046 - 2 t.
-      const int top = 2047 - 2 * (int)threadIdx.x;
-      const uint32_t x0 = s_hist[top], x1 = s_hist[top - 1], incl = wave_scan(x0 + x1);
-      if (lane == 63) s_part[wave] = incl;
-      __syncthreads();
-      uint32_t before = 0;
-      for (int w = 0; w < wave; ++w) before += s_part[w];
-      const uint32_t end = before + incl, begin = end - x0 - x1;
-      if (begin < want && want <= end) {  // (one thread: the last token to stay is in one of its bins)
-        const bool first = want <= begin + x0;
-        s_bin = (uint32_t)(first ? top : top - 1);
-        s_above = first ? begin : begin + x0;
-      }
-      __syncthreads();
-      prefix |= s_bin << shift;
-      mask |= digits << shift;
-      want -= s_above;
-      __syncthreads();
-    }
-  } else {
-    prefix = 0xFFFFFFFFu;  // (no score reaches it)
-  }
-  // `want` tokens of the value `prefix` stay, the first ones; all above it do.
+  auto order_at = [&](int32_t j, float x) { return !live(j) ? kGone : safe(j) ? kStays : order_of(x); };
+  // Wave w takes tokens [j0, j1), 64 at a time.
   const int32_t part = ((c + NW - 1) / NW + 63) / 64 * 64;
   const int32_t j0 = min(wave * part, c), j1 = min(j0 + part, c);
-  uint32_t gt = 0, eq = 0;
-  auto kind = [&](int32_t j, float &x) {  // 2: stays, 1: stays while there are ties to take
-    if (j >= j1) return 0;
-    x = src[j];
-    if (!live(j)) return 0;
-    if (safe(j)) return 2;
-    const uint32_t u = order_of(x);
-    return u > prefix ? 2 : u == prefix ? 1 : 0;
+  // Eight reads before the first is looked at, past the end the last token's: under a condition, or behind a store,
+  // each would be waited for by itself.
+  constexpr int U = 8;
+  auto each = [&](auto f) __attribute__((always_inline)) {  // f(token, score), all lanes together
+    for (int32_t base = j0; base < j1; base += 64 * U) {
+      float x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) x[u] = src[min(base + 64 * u + lane, c - 1)];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (base + 64 * u < j1) f(base + 64 * u + lane, x[u]);
+    }
   };
-  for (int32_t j = j0 + lane; j - lane < j1; j += 64) {
-    float x;
-    const int k = kind(j, x);
-    gt += (uint32_t)__popcll(__ballot(k == 2));
-    eq += (uint32_t)__popcll(__ballot(k == 1));
+  if constexpr (LDS)  // (each wave reads its own later)
+    each([&](int32_t j, float x) __attribute__((always_inline)) {
+      if (j < j1) s_key[j] = order_at(j, x);
+    });
+  auto each_key = [&](auto f) __attribute__((always_inline)) {  // f(order, of a token or kGone), all lanes together
+    if constexpr (LDS) {
+#pragma unroll 4
+      for (int32_t j = j0 + lane; j - lane < j1; j += 64) f(j < j1 ? s_key[j] : kGone);
+    } else {
+      each([&](int32_t j, float x) __attribute__((always_inline)) { f(j < j1 ? order_at(j, x) : kGone); });
+    }
+  };
+
+  // Protected tokens.
+  if (threadIdx.x == 0) sh.safe = 0;
+  __syncthreads();
+  if (holes) {
+    uint32_t k = 0;
+    for (int32_t j = threadIdx.x; j < c; j += 1024) k += safe(j) && live(j);
+    k = (uint32_t)wave_sum((int32_t)k);
+    if (lane == 0) atomicAdd(&sh.safe, k);
+  } else if (threadIdx.x == 0) {
+    sh.safe = (uint32_t)(sinks + c - recent0);  // (n <= c: they do not overlap)
   }
+  __syncthreads();
+  uint32_t want = (uint32_t)n - sh.safe;  // to be taken by score
+  uint32_t prefix = kStays - 1;           // (above every score's order)
+  if (want > 0) {
+    prefix = 0;
+    uint32_t mask = 0;
+#pragma unroll 1
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      (&sh.hist[0][0])[threadIdx.x] = uint4{0, 0, 0, 0};
+      __syncthreads();
+      each_key([&](uint32_t u) __attribute__((always_inline)) {
+        if (u != kGone && u != kStays && (u & mask) == prefix)
+          atomicAdd(reinterpret_cast<uint32_t *>(sh.hist[(u >> shift) & 255]) + (lane & 15), 1u);
+      });
+      __syncthreads();
+      // Bins from the top: thread t < 256 holds bin 255 - t.
+      const int bin = 255 - (int)threadIdx.x;
+      uint32_t held = 0, incl = 0;
+      if (wave < 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4 x = sh.hist[bin][i];
+          held += (x.x + x.y) + (x.z + x.w);
+        }
+        incl = wave_scan(held);
+        if (lane == 63) sh.part[wave] = incl;
+      }
+      __syncthreads();
+      if (wave < 4) {
+        uint32_t before = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) before += w < wave ? sh.part[w] : 0;
+        const uint32_t end = before + incl, begin = end - held;
+        if (begin < want && want <= end) {  // (one thread: the last token to stay is in its bin)
+          sh.bin = (uint32_t)bin;
+          sh.above = begin;
+        }
+      }
+      __syncthreads();
+      prefix |= sh.bin << shift;
+      mask |= 255u << shift;
+      want -= sh.above;
+    }
+  }
+  // `want` tokens of the order `prefix` stay, the first ones; all above it do.
+  uint32_t gt = 0, eq = 0;
+  each_key([&](uint32_t u) __attribute__((always_inline)) {
+    gt += (uint32_t)__popcll(__ballot(u > prefix));
+    eq += (uint32_t)__popcll(__ballot(u == prefix));
+  });
   if (lane == 0) {
-    s_gt[wave] = gt;
-    s_eq[wave] = eq;
+    sh.gt[wave] = gt;
+    sh.eq[wave] = eq;
   }
   __syncthreads();
   uint32_t at = 0, ties = 0;
   for (int w = 0; w < wave; ++w) {
-    at += s_gt[w] + min(s_eq[w], want - min(want, ties));
-    ties += s_eq[w];
+    at += sh.gt[w] + min(sh.eq[w], want - min(want, ties));
+    ties += sh.eq[w];
   }
   const uint64_t below = (1ull << lane) - 1;
-  for (int32_t j = j0 + lane; j - lane < j1; j += 64) {
-    float x;
-    const int k = kind(j, x);
-    const uint64_t tie = __ballot(k == 1);
-    const bool take = k == 2 || (k == 1 && ties + (uint32_t)__popcll(tie & below) < want);
+  each([&](int32_t j, float x) __attribute__((always_inline)) {
+    const uint32_t u = j >= j1 ? kGone : LDS ? s_key[j] : order_at(j, x);
+    const uint64_t tie = __ballot(u == prefix);
+    const bool take = u > prefix || (u == prefix && ties + (uint32_t)__popcll(tie & below) < want);
     const uint64_t all = __ballot(take);
     if (take) {
       const uint32_t i = at + (uint32_t)__popcll(all & below);
@@ -292,20 +289,97 @@ __global__ __launch_bounds__(1024) void compact_select_kernel(const CompactParam
     }
     at += (uint32_t)__popcll(all);
     ties += (uint32_t)__popcll(tie);
-  }
+  });
   for (int32_t j = n + (int32_t)threadIdx.x; j < p.L; j += 1024) dst[j] = 0.0f;
   for (int32_t j = n + (int32_t)threadIdx.x; j < p.K; j += 1024) kept[j] = -1;
+}
+
+// A row that stays as it is.
+__device__ __forceinline__ void leave_row(const CompactParams &p, int64_t unit, int32_t threads) {
+  for (int32_t j = threadIdx.x; j < p.L; j += threads) p.scores_out[unit * p.L + j] = p.scores[unit * p.L + j];
+  for (int32_t j = threadIdx.x; j < p.K; j += threads) p.kept[unit * p.K + j] = -1;
+}
+
+__global__ __launch_bounds__(1024) void compact_select_kernel(const CompactParams p) {
+  __shared__ SelectShared sh;
+  extern __shared__ uint32_t s_key[];  // [in_lds]
+  __shared__ uint32_t s_part[2][16];
+  __shared__ int32_t s_last;
+  const int32_t h = blockIdx.x, b = blockIdx.y;
+  const int64_t unit = (int64_t)b * p.Hk + h;
+  const int32_t n = p.stay[b], c = p.ctx[b];
+  if (h == 0 && p.state[b] != MEMOPT_COMPACT_INVALID) {
+    const int32_t have = (c + p.bs - 1) / p.bs;
+    for (int32_t i = threadIdx.x; i < have; i += 1024) {
+      const int32_t page = p.bt[(int64_t)b * p.M + i];
+      if (!page_ok(p, page)) continue;
+      const int32_t id = p.marks[page];
+      if (id == b * p.M + i) continue;
+      __hip_atomic_store(&p.state[b], MEMOPT_COMPACT_SHARED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(&p.state[id / p.M], MEMOPT_COMPACT_SHARED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  const float *src = p.scores + unit * p.L;
+  float *dst = p.scores_out + unit * p.L;
+  int32_t *kept = p.kept + unit * p.K;
+  if (n < 0) leave_row(p, unit, 1024);
+  else if (c <= p.in_lds) select_row<true>(p, sh, s_key, b, src, dst, kept, n);
+  else select_row<false>(p, sh, s_key, b, src, dst, kept, n);
+  // The last workgroup to get here has all states before it: they alone pass between workgroups, by agent-scope
+  // stores that have arrived once they are waited for (a fence would write the whole L2 back).
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0)
+    s_last = __hip_atomic_fetch_add(&p.counts[0], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == p.Hk * p.N - 1;
+  __syncthreads();
+  if (s_last) plan_requests(p, s_part);
+}
+
+// A request's tables and its old pages' places at the ring's end; what the
+// second launch wrote for one that is not served after all. One workgroup.
+__device__ __forceinline__ void write_tables(const CompactParams &p, int32_t b) {
+  __shared__ int32_t s_count[4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = (int64_t)b * p.M;
+  if (p.status[b] != MEMOPT_COMPACT_DONE) {
+    for (int32_t i = threadIdx.x; i < p.M; i += 256) p.bt_out[row + i] = p.bt[row + i];
+    if (p.stay[b] >= 0)
+      for (int32_t h = 0; h < p.Hk; ++h) leave_row(p, (int64_t)b * p.Hk + h, 256);
+    return;
+  }
+  const int32_t need = (p.stay[b] + p.bs - 1) / p.bs, have = (p.ctx[b] + p.bs - 1) / p.bs;
+  for (int32_t i = threadIdx.x; i < p.M; i += 256)
+    p.bt_out[row + i] = i < need ? p.ring[(int32_t)(((int64_t)p.counts[1] + p.fresh[b] + i) % p.C)] : -1;
+  int32_t at = p.back[b];
+  for (int32_t i0 = 0; i0 < have; i0 += 256) {
+    const int32_t i = i0 + (int32_t)threadIdx.x, page = i < have ? p.bt[row + i] : -1;
+    const uint64_t m = __ballot(page_ok(p, page));
+    if (lane == 0) s_count[wave] = (int32_t)__popcll(m);
+    __syncthreads();
+    int32_t before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      before += w < wave ? s_count[w] : 0;
+      all += s_count[w];
+    }
+    if (page_ok(p, page))
+      p.ring[(int32_t)(((int64_t)p.counts[1] + p.counts[2] + at + before + __popcll(m & ((1ull << lane) - 1))) % p.C)] = page;
+    at += all;
+    __syncthreads();
+  }
 }
 
 // The copies: a wave per 16 new tokens and head.
 template <int FMT, int D>
 __global__ __launch_bounds__(256) void compact_move_kernel(const CompactParams p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int32_t h = (int32_t)(blockIdx.x % p.Hk), chunk = (int32_t)(blockIdx.x / p.Hk) * 4 + wave, b = blockIdx.y;
+  if (blockIdx.x == 0) return write_tables(p, blockIdx.y);
+  const int32_t h = (int32_t)((blockIdx.x - 1) % p.Hk), chunk = (int32_t)((blockIdx.x - 1) / p.Hk) * 4 + wave, b = blockIdx.y;
   const int32_t n = p.stay[b], i0 = 16 * chunk;
-  if (i0 >= n) return;
+  if (i0 >= n || p.status[b] != MEMOPT_COMPACT_DONE) return;
   const int64_t unit = (int64_t)b * p.Hk + h;
-  const int32_t page = __builtin_amdgcn_readfirstlane(p.bt_out[(int64_t)b * p.M + i0 / p.bs]);
+  const int32_t page = __builtin_amdgcn_readfirstlane(
+      p.ring[(int32_t)(((int64_t)p.counts[1] + p.fresh[b] + i0 / p.bs) % p.C)]);
   if (!page_ok(p, page)) return;  // (the ring held something that is no page)
   // Old page and place of new token i0 + t, in lane t.
   const int32_t mine = i0 + (lane & 15) < n ? p.kept[unit * p.K + i0 + (lane & 15)] : -1;
@@ -360,8 +434,15 @@ __global__ __launch_bounds__(256) void compact_move_kernel(const CompactParams p
   }
 }
 
+// A call without requests: the ring stays, its span within its bounds.
+__global__ void compact_no_requests_kernel(const CompactParams p) {
+  const int32_t head = p.span[0] % p.C, count = min(max(p.span[1], 0), p.C);
+  p.span_out[0] = head < 0 ? head + p.C : head;
+  p.span_out[1] = count;
+}
+
 static int64_t compact_workspace(const memopt_compact_desc &d) {
-  return ((2 * (int64_t)d.num_requests + d.num_kv_blocks) * 4 + 255) / 256 * 256;
+  return ((5 * (int64_t)d.num_requests + 4 + d.num_kv_blocks) * 4 + 255) / 256 * 256;
 }
 
 static int validate_compact(const memopt_compact_desc &d) {
@@ -383,7 +464,8 @@ static int validate_compact(const memopt_compact_desc &d) {
                      (int64_t)d.num_requests * d.max_blocks_per_seq <= INT32_MAX,
                  MEMOPT_ERR_UNSUPPORTED,
                  "compact_cache: block tables and scores of up to 2^30 tokens, no more of them kept than there are scores");
-  MEMOPT_REQUIRE(d.num_kv_heads <= 65535 && ((int64_t)d.max_keep / 64 + 1) * d.num_kv_heads * std::max(1, d.num_requests) < (1LL << 24),
+  MEMOPT_REQUIRE(d.num_kv_heads <= 65535 && (((int64_t)d.max_keep / 64 + 1) * d.num_kv_heads + 1) * std::max(1, d.num_requests) < (1LL << 24) &&
+                     (int64_t)d.num_kv_heads * d.num_requests < (1LL << 22),
                  MEMOPT_ERR_UNSUPPORTED, "compact_cache: too many pages for one call");
   return MEMOPT_OK;
 }
@@ -450,14 +532,26 @@ extern "C" int memopt_compact_cache(const memopt_compact_desc *desc, void *strea
   p.span_out = d.free_span_out;
   p.stay = (int32_t *)d.workspace;
   p.holes = p.stay + p.N;
-  p.marks = p.holes + p.N;
+  p.back = p.holes + p.N;
+  p.fresh = p.back + p.N;
+  p.state = p.fresh + p.N;
+  p.counts = p.state + p.N;
+  p.marks = p.counts + 4;
   hipStream_t s = (hipStream_t)stream;
-  hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(1024), 0, s, p);
-  rc = check_launch("compact_cache(plan)");
-  if (rc != MEMOPT_OK || p.N == 0) return rc;
-  hipLaunchKernelGGL(compact_select_kernel, dim3(p.Hk, p.N), dim3(1024), 0, s, p);
-  if ((rc = check_launch("compact_cache(select)")) != MEMOPT_OK || p.K == 0) return rc;
-  const dim3 grid((unsigned)(((int64_t)p.K + 63) / 64 * p.Hk), p.N);
+  if (p.N == 0) {
+    hipLaunchKernelGGL(compact_no_requests_kernel, dim3(1), dim3(1), 0, s, p);
+    return check_launch("compact_cache");
+  }
+  hipLaunchKernelGGL(compact_count_kernel, dim3(p.N), dim3(256), 0, s, p);
+  if ((rc = check_launch("compact_cache(count)")) != MEMOPT_OK) return rc;
+  // (no request is longer than its table or its scores)
+  p.in_lds = (int32_t)std::min<int64_t>(kInLds, std::min<int64_t>((int64_t)p.M * p.bs, p.L));
+  static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(&compact_select_kernel),
+                                                    hipFuncAttributeMaxDynamicSharedMemorySize, 4 * kInLds);
+  MEMOPT_REQUIRE(set == hipSuccess, MEMOPT_ERR_HIP, std::string("compact_cache: ") + hipGetErrorString(set));
+  hipLaunchKernelGGL(compact_select_kernel, dim3(p.Hk, p.N), dim3(1024), 4 * p.in_lds, s, p);
+  if ((rc = check_launch("compact_cache(select)")) != MEMOPT_OK) return rc;
+  const dim3 grid((unsigned)(((int64_t)p.K + 63) / 64 * p.Hk + 1), p.N);
   if (d.kv_format == MEMOPT_KV_INT4) {
     if (p.D == 128) hipLaunchKernelGGL((compact_move_kernel<MEMOPT_KV_INT4, 128>), grid, dim3(256), 0, s, p);
     else hipLaunchKernelGGL((compact_move_kernel<MEMOPT_KV_INT4, 64>), grid, dim3(256), 0, s, p);
