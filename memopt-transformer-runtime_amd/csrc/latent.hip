@@ -108,12 +108,6 @@ __device__ __forceinline__ uint32_t latent_run(uint32_t total, int32_t wgs) {
   return max(1u, (total + (uint32_t)wgs - 1) / (uint32_t)wgs);
 }
 
-// A block-table entry through the scalar cache: a vector load would be waited
-// for together with the key tiles whose copies were issued before it.
-__device__ __forceinline__ int32_t uniform_entry(const int32_t *x) {
-  return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)uniform_ptr(x);
-}
-
 // Two waves share 32 rows: in the first product each takes 32 of a tile's keys,
 // in the second half of the latent's columns, over all keys, so that a wave
 // holds 8 (R + P) / 16 operand and R / 4 accumulator registers (272 at 512 +

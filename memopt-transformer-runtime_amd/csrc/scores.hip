@@ -39,7 +39,7 @@ struct ScoresParams {
   int32_t kts;                 // key tiles of kTileKeys
   Divisor by_g, by_chunks;     // by_chunks: 16-token chunks of a page
   float qk_scale_log2;
-  float2 *ml;    // few rows: [B][Hk][kts][max_rows]; chunks: [Hk][kts][T G]
+  float2 *ml;    // few rows: [B][Hk][kts][4][max_rows]; chunks: [Hk][kts][T G]
   float *probs;  // few rows: [B][Hk][max_rows][kts * kTileKeys]
   float *lse;    // chunks: [Hk][T G]
 };
@@ -74,59 +74,58 @@ __device__ __forceinline__ float max_over_quarters(float v) {
 }
 __device__ __forceinline__ float sum_over_quarters(float v) { return xor32_sum(xor16_sum(v)); }
 
-// Eight codes less 8 as exact fp16 values, in the order of their dims.
+// Eight codes less 8 as exact fp16 values, in the order 0 4 1 5 2 6 3 7 of
+// their dims: a nibble beside the exponent of 1024 (or 64) is that plus the
+// code. (In the dims' own order an operand takes half as many instructions
+// again, and unpacking is what bounds single tokens over INT4 pages.)
 __device__ __forceinline__ u32x4p_t codes_to_half(uint32_t w) {
-  const uint32_t lo = w & 0x0F0F0F0Fu, hi = (w >> 4) & 0x0F0F0F0Fu;
-  u32x4p_t r;
-  // bytes (code 2i, 0, code 2i + 1, 0); 1024 + code is 0x6400 | code in fp16
-  constexpr uint32_t sel[4] = {0x0C000C04u, 0x0C010C05u, 0x0C020C06u, 0x0C030C07u};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t x = __builtin_amdgcn_perm(lo, hi, sel[i]) | 0x64006400u;
-    r[i] = as_u32(as_half2(x) - half2_t{(half_t)1032.0f, (half_t)1032.0f});
-  }
-  return r;
+  const half2_t lo = {(half_t)1032.0f, (half_t)1032.0f}, hi = {(half_t)72.0f, (half_t)72.0f};
+  const uint32_t v = w >> 8;
+  return u32x4p_t{as_u32(as_half2(bfi(0x000F000Fu, w, 0x64006400u)) - lo),
+                  as_u32(as_half2(bfi(0x00F000F0u, w, 0x54005400u)) - hi),
+                  as_u32(as_half2(bfi(0x000F000Fu, v, 0x64006400u)) - lo),
+                  as_u32(as_half2(bfi(0x00F000F0u, v, 0x54005400u)) - hi)};
+}
+// Eight elements of a query row in that order.
+__device__ __forceinline__ u32x4p_t in_code_order(u32x4p_t q) {
+  return u32x4p_t{__builtin_amdgcn_perm(q[2], q[0], 0x05040100u), __builtin_amdgcn_perm(q[2], q[0], 0x07060302u),
+                  __builtin_amdgcn_perm(q[3], q[1], 0x05040100u), __builtin_amdgcn_perm(q[3], q[1], 0x07060302u)};
 }
 
 // 64 keys of one head as operands of v_mfma_f32_16x16x32: page g's keys are
-// the rows of operand a[g][.]; lane l holds key l % 16 and of every 64 dims
-// the 16 from 16 (l / 16) on, in two operands. Products come out with the
+// the rows of four (two) operands; lane l holds key l % 16 and of every 64
+// dims the 16 from 16 (l / 16) on, in two operands. Products come out with the
 // query row in the lane's column l % 16 and keys 4 (l / 16) + r in register r.
 template <int FMT, int D>
 struct Keys {
   static constexpr int NCH = D / 32, NG = D / 64;
   static constexpr bool CODES = FMT == MEMOPT_KV_INT4;
-  u32x4p_t a[4][NCH];
-  f32x4p_t f[CODES ? 4 : 1][CODES ? NG : 1];  // factors of the register's keys: scale times qk_scale_log2
-  uint32_t linked;                            // bit g: page g is there
+  uint32_t linked;  // bit g: page g is there
+  uint32_t w[CODES ? 4 : 1][NCH];
+  uint4 sc[CODES ? 4 : 1][NG];
+  u32x4p_t rows[CODES ? 1 : 4][NCH];
 
   __device__ __forceinline__ void load(const ScoresParams &p, int32_t b, int32_t h, int32_t key0, int32_t len) {
     const int lane = threadIdx.x & 63, t = lane & 15, kq = lane >> 4;
+    constexpr int BPL = D / 8;
     linked = 0;
     const uint8_t *at[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int32_t key = key0 + 16 * g;
-      int32_t page = -1, first = 0;
-      if (key < len) {
-        const int32_t c = key >> 4, e = CODES ? c : p.by_chunks(c);
-        first = CODES ? 0 : 16 * (c - e * (int32_t)p.by_chunks.d);
-        page = __builtin_amdgcn_readfirstlane(p.bt[(int64_t)b * p.M + e]);
-      }
+      const int32_t key = key0 + 16 * g, c = key >> 4, e = CODES ? c : p.by_chunks(c);
+      const int32_t first = CODES ? 0 : 16 * (c - e * (int32_t)p.by_chunks.d);
+      const int32_t page = key < len ? uniform_entry(p.bt + (int64_t)b * p.M + e) : -1;
       const bool ok = page >= 0 && page < p.nb;
       linked |= (ok ? 1u : 0u) << g;
       at[g] = ok ? p.k + (int64_t)page * p.k_ps + h * p.k_hs + first * p.k_ts : nullptr;
     }
-    constexpr int BPL = D / 8;
-    uint32_t w[4][NCH];
-    uint4 sc[4][NG];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       if (!((linked >> g) & 1)) {
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
           if constexpr (CODES) w[g][c] = 0x88888888u;
-          else a[g][c] = (u32x4p_t){};
+          else rows[g][c] = (u32x4p_t){};
         }
         if constexpr (CODES)
 #pragma unroll
@@ -148,47 +147,44 @@ struct Keys {
       } else {
 #pragma unroll
         for (int c = 0; c < NCH; ++c)
-          a[g][c] = *reinterpret_cast<const u32x4p_t *>(at[g] + t * p.k_ts + 2 * (64 * (c >> 1) + 16 * kq + 8 * (c & 1)));
-      }
-    }
-    if constexpr (CODES) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) a[g][c] = codes_to_half(w[g][c]);
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-          const uint32_t s[4] = {sc[g][i].x, sc[g][i].y, sc[g][i].z, sc[g][i].w};
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const half2_t pair = as_half2(s[r]);
-            f[g][i][r] = (float)(kq >> 1 ? pair.y : pair.x) * p.qk_scale_log2;
-          }
-        }
+          rows[g][c] = *reinterpret_cast<const u32x4p_t *>(at[g] + t * p.k_ts + 2 * (64 * (c >> 1) + 16 * kq + 8 * (c & 1)));
       }
     }
   }
-  // Scores in log2 units of page g's keys against 16 query rows.
-  __device__ __forceinline__ f32x4p_t scores(int g, const u32x4p_t (&q)[NCH], float scale) const {
+  // Page g's operands, and the factors of the register's keys.
+  __device__ __forceinline__ void operands(int g, u32x4p_t (&a)[NCH], f32x4p_t (&f)[NG]) const {
+    const int kq = (threadIdx.x & 63) >> 4, sh = 16 * (kq >> 1);
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      if constexpr (CODES) a[c] = codes_to_half(w[g][c]);
+      else a[c] = rows[g][c];
+    }
+    if constexpr (CODES) {
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        const uint32_t s[4] = {sc[g][i].x, sc[g][i].y, sc[g][i].z, sc[g][i].w};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) f[i][r] = (float)__builtin_bit_cast(half_t, (uint16_t)(s[r] >> sh));
+      }
+    }
+  }
+  // q . k of a page's keys against 16 query rows (INT4: q in_code_order).
+  static __device__ __forceinline__ f32x4p_t scores(const u32x4p_t (&a)[NCH], const f32x4p_t (&f)[NG], const u32x4p_t (&q)[NCH]) {
     f32x4p_t c[NG];
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
-      c[i] = (f32x4p_t){};
+      if (CODES || i == 0) c[i] = (f32x4p_t){};
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        f32x4p_t &acc = CODES ? c[i] : c[0];
-        if (!CODES && i == 0 && j == 0) acc = (f32x4p_t){};
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8s_t, a[g][2 * i + j]),
+        f32x4p_t &acc = c[CODES ? i : 0];
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8s_t, a[2 * i + j]),
                                                      __builtin_bit_cast(f16x8s_t, q[2 * i + j]), acc, 0, 0, 0);
       }
     }
+    if constexpr (!CODES) return c[0];
     f32x4p_t x;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if constexpr (!CODES) x[r] = c[0][r] * scale;
-      else if constexpr (NG == 1) x[r] = c[0][r] * f[g][0][r];
-      else x[r] = fmaf(c[1][r], f[g][1][r], c[0][r] * f[g][0][r]);
-    }
+    for (int r = 0; r < 4; ++r) x[r] = NG == 1 ? c[0][r] * f[0][r] : fmaf(c[NG - 1][r], f[NG - 1][r], c[0][r] * f[0][r]);
     return x;
   }
 };
@@ -212,88 +208,120 @@ __device__ __forceinline__ f32x4p_t hide(const ScoresParams &p, f32x4p_t x, int3
 // keys again: 8 bytes per row and key against D / 2 + 2 D / 64 of INT4.
 
 template <int FMT, int D>
-__global__ __launch_bounds__(256) void few_rows_kernel(const ScoresParams p) {
+__global__ __launch_bounds__(256, 4) void few_rows_kernel(const ScoresParams p, const int32_t tiles_each) {
   using K = Keys<FMT, D>;
-  __shared__ float s_m[4][kFewRows], s_l[4][kFewRows];
-  const int32_t h = (int32_t)(blockIdx.x % p.Hk), kt = (int32_t)(blockIdx.x / p.Hk), b = blockIdx.y;
+  const int32_t h = (int32_t)(blockIdx.x % p.Hk), b = blockIdx.y;
   const int lane = threadIdx.x & 63, n = lane & 15, kq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const ScoredSeq s = scored_seq(p, b);
-  int32_t lo, hi;
-  queries_of(p, s, s.rows / p.G, kt * kTileKeys, (kt + 1) * kTileKeys, lo, hi);
-  if (hi <= lo) return;
-  const int32_t key0 = kt * kTileKeys + 64 * wave;
-  K keys;
-  keys.load(p, b, h, key0, s.len);
+  const int32_t kt0 = (int32_t)(blockIdx.x / p.Hk) * tiles_each;
+  const int32_t kt1 = min(min(kt0 + tiles_each, p.kts), (s.len + kTileKeys - 1) / kTileKeys);
+  if (s.rows == 0 || kt0 >= kt1) return;
   const bool ok = n < s.rows;
-  const int32_t tok = p.by_g(min(n, s.rows - 1)), pos = s.pos0 + tok;
+  const int32_t tok = p.by_g(min(n, s.rows - 1)), pos = s.pos0 + tok, last = s.pos0 + s.rows / p.G - 1;
   u32x4p_t q[K::NCH];
   const uint16_t *src = p.q + (int64_t)(s.start + tok) * p.q_ts + ((int64_t)h * p.G + min(n, s.rows - 1) - tok * p.G) * p.q_hs;
 #pragma unroll
-  for (int c = 0; c < K::NCH; ++c)
+  for (int c = 0; c < K::NCH; ++c) {
     q[c] = *reinterpret_cast<const u32x4p_t *>(src + 64 * (c >> 1) + 16 * kq + 8 * (c & 1));
-  f32x4p_t x[4];
-  float m = -INFINITY;
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    x[g] = hide(p, keys.scores(g, q, p.qk_scale_log2), key0 + 16 * g + 4 * kq, pos, s.len, ok && ((keys.linked >> g) & 1));
-#pragma unroll
-    for (int r = 0; r < 4; ++r) m = fmaxf(m, x[g][r]);
+    if constexpr (K::CODES) q[c] = in_code_order(q[c]);
   }
-  m = max_over_quarters(m);
-  if (kq == 0) s_m[wave][n] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(s_m[0][n], s_m[1][n]), fmaxf(s_m[2][n], s_m[3][n]));
-  const float ref = m == -INFINITY ? 0.0f : m;
   const int64_t unit = (int64_t)b * p.Hk + h;
-  float l = 0.0f;
-  float *dst = p.probs + (unit * p.max_rows + n) * ((int64_t)p.kts * kTileKeys) + key0 + 4 * kq;
+  for (int32_t kt = kt0; kt < kt1; ++kt) {
+    int32_t lo, hi;
+    queries_of(p, s, s.rows / p.G, kt * kTileKeys, (kt + 1) * kTileKeys, lo, hi);
+    if (hi <= lo) continue;
+    const int32_t key0 = kt * kTileKeys + 64 * wave;
+    K keys;
+    keys.load(p, b, h, key0, s.len);
+    // (rows past the last are not stored: what their lanes hold does not matter)
+    const bool full = key0 + 63 <= s.pos0 && key0 + 64 <= s.len && keys.linked == 15u &&
+                      (key0 > last - p.W || key0 + 64 <= p.sinks);
+    f32x4p_t x[4];
+    float m = -INFINITY;
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
+    for (int g = 0; g < 4; ++g) {
+      u32x4p_t a[K::NCH];
+      f32x4p_t f[K::NG];
+      keys.operands(g, a, f);
+      x[g] = K::scores(a, f, q);
+      if (!full) x[g] = hide(p, x[g], key0 + 16 * g + 4 * kq, pos, s.len, (keys.linked >> g) & 1);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      x[g][r] = fast_exp2(x[g][r] - ref);
-      l += x[g][r];
+      for (int r = 0; r < 4; ++r) m = fmaxf(m, x[g][r]);
     }
-    if (ok) *reinterpret_cast<f32x4p_t *>(dst + 16 * g) = x[g];
+    // Weights are relative to the maximum of the wave's 64 keys: no wave waits for another.
+    m = max_over_quarters(m) * p.qk_scale_log2;
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    float *dst = p.probs + (unit * p.max_rows + n) * ((int64_t)p.kts * kTileKeys) + key0 + 4 * kq;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[g][r] = fast_exp2(fmaf(x[g][r], p.qk_scale_log2, -ref));
+        l += x[g][r];
+      }
+      if (ok) *reinterpret_cast<f32x4p_t *>(dst + 16 * g) = x[g];
+    }
+    l = sum_over_quarters(l);
+    // (keys without a maximum add nothing, unless all that the row sees of them is NaN)
+    if (ok && kq == 0) p.ml[((unit * p.kts + kt) * 4 + wave) * p.max_rows + n] = float2{l == 0.0f ? m : fmaxf(m, -3e38f), l};
   }
-  l = sum_over_quarters(l);
-  if (kq == 0) s_l[wave][n] = l;
-  __syncthreads();
-  l = (s_l[0][n] + s_l[1][n]) + (s_l[2][n] + s_l[3][n]);
-  // (a tile without a maximum adds nothing, unless all that the row sees in it is NaN)
-  if (threadIdx.x < (unsigned)s.rows) p.ml[(unit * p.kts + kt) * p.max_rows + n] = float2{l == 0.0f ? m : fmaxf(m, -3e38f), l};
 }
 
-// out = scores + the rows' weights: a thread per key. Also the whole of a
+// out = scores + the rows' weights: four keys a thread. Also the whole of a
 // call without rows.
+static constexpr int kFinishTiles = 4;
 __global__ __launch_bounds__(256) void finish_kernel(const ScoresParams p) {
-  __shared__ float s_f[kFewRows];
-  const int32_t h = (int32_t)(blockIdx.x % p.Hk), kt = (int32_t)(blockIdx.x / p.Hk), b = blockIdx.y;
+  __shared__ float s_f[kFewRows][4 * kFinishTiles];  // [row][64 keys]
+  const int32_t h = (int32_t)(blockIdx.x % p.Hk), kt0 = (int32_t)(blockIdx.x / p.Hk) * kFinishTiles, b = blockIdx.y;
   const ScoredSeq s = scored_seq(p, b);
   const int64_t unit = (int64_t)b * p.Hk + h;
-  const int32_t j = kt * kTileKeys + (int32_t)threadIdx.x;
-  const float before = p.scores && j < p.L ? p.scores[unit * p.L + j] : 0.0f;
-  int32_t lo, hi;
-  queries_of(p, s, s.rows / p.G, kt * kTileKeys, (kt + 1) * kTileKeys, lo, hi);
-  float w = 0.0f;
-  if (hi > lo) {
-    // Row threadIdx / 16's maximum and sum, by 16 lanes over the key tiles.
-    const int32_t row = threadIdx.x >> 4;
+  const int32_t key0 = kt0 * kTileKeys;
+  float before[kFinishTiles], w[kFinishTiles];
+#pragma unroll
+  for (int k = 0; k < kFinishTiles; ++k) {
+    const int32_t j = key0 + kTileKeys * k + (int32_t)threadIdx.x;
+    before[k] = p.scores && j < p.L ? p.scores[unit * p.L + j] : 0.0f;
+    w[k] = 0.0f;
+  }
+  if (s.rows > 0 && key0 < s.len) {
+    const int32_t tiles = (s.len + kTileKeys - 1) / kTileKeys;
+    auto met = [&](int32_t t) {
+      int32_t lo, hi;
+      queries_of(p, s, s.rows / p.G, t * kTileKeys, (t + 1) * kTileKeys, lo, hi);
+      return hi > lo;
+    };
+    // Weights of four rows at a time, all reads under way together, the first four while the sums are put together
+    // (tiles that no row met hold anything: their values are not used).
+    const float *src = p.probs + unit * p.max_rows * ((int64_t)p.kts * kTileKeys) + threadIdx.x;
+    float x[kFinishTiles][4];
+    auto read = [&](int32_t r0) __attribute__((always_inline)) {
+#pragma unroll
+      for (int k = 0; k < kFinishTiles; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          x[k][r] = src[(int64_t)min(r0 + r, s.rows - 1) * p.kts * kTileKeys + kTileKeys * min(kt0 + k, tiles - 1)];
+    };
+    read(0);
+    // Row threadIdx / 16's maximum and sum, by 16 lanes over the 64-key parts.
+    const int32_t row = threadIdx.x >> 4, lane16 = threadIdx.x & 15;
+    const float2 *ml = p.ml + unit * p.kts * 4 * p.max_rows + row;
     float m = -INFINITY, l = 0.0f;
-    if (row < s.rows) {
-      const int32_t tiles = (s.len + kTileKeys - 1) / kTileKeys;
-      for (int32_t t = threadIdx.x & 15; t < tiles; t += 16) {
-        int32_t a, z;
-        queries_of(p, s, s.rows / p.G, t * kTileKeys, (t + 1) * kTileKeys, a, z);
-        if (z <= a) continue;
-        const float2 x = p.ml[(unit * p.kts + t) * p.max_rows + row];
-        const float top = fmaxf(m, x.x);
-        if (top == -INFINITY) continue;
-        l = l * fast_exp2(m - top) + x.y * fast_exp2(x.x - top);
-        m = top;
+    if (row < s.rows)
+      for (int32_t t0 = lane16; t0 < 4 * tiles; t0 += 16 * 8) {
+        float2 x[8];  // (eight reads in flight)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = ml[(int64_t)min(t0 + 16 * i, 4 * tiles - 1) * p.max_rows];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int32_t t = t0 + 16 * i;
+          const float top = fmaxf(m, x[i].x);
+          if (t >= 4 * tiles || !met(t >> 2) || top == -INFINITY) continue;
+          l = l * fast_exp2(m - top) + x[i].y * fast_exp2(x[i].x - top);
+          m = top;
+        }
       }
-    }
     float top = fmaxf(m, xor1(m));
     top = fmaxf(top, xor2(top));
     top = fmaxf(top, half_mirror(top));
@@ -303,21 +331,35 @@ __global__ __launch_bounds__(256) void finish_kernel(const ScoresParams p) {
     l += xor2(l);
     l += half_mirror(l);
     l += dpp_f32<0x140>(l);
-    if ((threadIdx.x & 15) == 0 && row < s.rows) {
-      const float here = p.ml[(unit * p.kts + kt) * p.max_rows + row].x;
-      // (a tile without a visible key of this row has the reference 0 and zeros)
-      s_f[row] = l == 0.0f || here == -INFINITY ? 0.0f : fast_exp2(here - top) / l;
+    if (row < s.rows) {
+      const int32_t t = 4 * kt0 + lane16;
+      const float here = t < 4 * tiles && met(t >> 2) ? ml[(int64_t)t * p.max_rows].x : -INFINITY;
+      // (keys without a visible one of this row have the reference 0 and zeros)
+      s_f[row][lane16] = l == 0.0f || here == -INFINITY ? 0.0f : fast_exp2(here - top) / l;
     }
     __syncthreads();
-    if (j < s.len) {
-      const float *src = p.probs + unit * p.max_rows * ((int64_t)p.kts * kTileKeys) + j;
-      for (int32_t r = 0; r < s.rows; ++r) {
-        const float x = src[(int64_t)r * p.kts * kTileKeys];
-        w = x == 0.0f ? w : fmaf(x, s_f[r], w);  // (a hidden key takes no part in a row of NaN)
-      }
+    bool in[kFinishTiles];
+#pragma unroll
+    for (int k = 0; k < kFinishTiles; ++k)
+      in[k] = kt0 + k < tiles && met(kt0 + k) && key0 + kTileKeys * k + (int32_t)threadIdx.x < s.len;
+    for (int32_t r0 = 0;;) {
+#pragma unroll
+      for (int k = 0; k < kFinishTiles; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool use = in[k] && r0 + r < s.rows && x[k][r] != 0.0f;  // (a hidden key takes no part in a row of NaN)
+          w[k] = use ? fmaf(x[k][r], s_f[min(r0 + r, kFewRows - 1)][4 * k + (threadIdx.x >> 6)], w[k]) : w[k];
+        }
+      r0 += 4;
+      if (r0 >= s.rows) break;
+      read(r0);
     }
   }
-  if (j < p.L) p.out[unit * p.L + j] = before + w;
+#pragma unroll
+  for (int k = 0; k < kFinishTiles; ++k) {
+    const int32_t j = key0 + kTileKeys * k + (int32_t)threadIdx.x;
+    if (j < p.L) p.out[unit * p.L + j] = before[k] + w[k];
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -345,6 +387,11 @@ __global__ __launch_bounds__(256, 2) void chunk_rows_kernel(const ScoresParams p
   if (hi > lo) {
     K keys;
     keys.load(p, b, h, key0, s.len);
+    const uint32_t linked = keys.linked;
+    u32x4p_t a[4][NCH];
+    f32x4p_t f[4][K::NG];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) keys.operands(g, a[g], f[g]);
     // Tiles of TR rows from the first that sees a key to the last.
     const int32_t t0 = lo * p.G / TR, t1 = (hi * p.G + TR - 1) / TR;
     const int64_t row_base = (int64_t)s.start * p.G;
@@ -391,25 +438,28 @@ __global__ __launch_bounds__(256, 2) void chunk_rows_kernel(const ScoresParams p
         const int32_t r0 = t * TR + 16 * i, row = r0 + n;
         const int32_t pos = s.pos0 + p.by_g(min(row, s.rows - 1));
         const int32_t first = s.pos0 + p.by_g(min(r0, s.rows - 1)), last = s.pos0 + p.by_g(min(r0 + 15, s.rows - 1));
-        const bool full = r0 + 15 < s.rows && key0 + 63 <= first && key0 + 64 <= s.len && keys.linked == 15u &&
+        const bool full = r0 + 15 < s.rows && key0 + 63 <= first && key0 + 64 <= s.len && linked == 15u &&
                           (key0 > last - p.W || key0 + 64 <= p.sinks);
         u32x4p_t q[NCH];
 #pragma unroll
         for (int c = 0; c < NCH; ++c)
           q[c] = *reinterpret_cast<const u32x4p_t *>(lds_q[buf] + (16 * i + n) * RB +
                                                      16 * ((8 * (c >> 1) + 2 * kq + (c & 1)) ^ q_swz(16 * i + n)));
+        if constexpr (K::CODES)
+#pragma unroll
+          for (int c = 0; c < NCH; ++c) q[c] = in_code_order(q[c]);
         f32x4p_t x[4];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          x[g] = keys.scores(g, q, p.qk_scale_log2);
-          if (!full) x[g] = hide(p, x[g], key0 + 16 * g + 4 * kq, pos, s.len, row < s.rows && ((keys.linked >> g) & 1));
+          x[g] = K::scores(a[g], f[g], q);
+          if (!full) x[g] = hide(p, x[g], key0 + 16 * g + 4 * kq, pos, s.len, row < s.rows && ((linked >> g) & 1));
         }
         if constexpr (SUM) {
 #pragma unroll
           for (int g = 0; g < 4; ++g)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const float y = fast_exp2(x[g][r] - lse[i]);
+              const float y = fast_exp2(fmaf(x[g][r], p.qk_scale_log2, -lse[i]));
               w[g][r] += !full && x[g][r] == -INFINITY ? 0.0f : y;  // (a hidden key takes no part in a row of NaN)
             }
         } else {
@@ -418,12 +468,12 @@ __global__ __launch_bounds__(256, 2) void chunk_rows_kernel(const ScoresParams p
           for (int g = 0; g < 4; ++g)
 #pragma unroll
             for (int r = 0; r < 4; ++r) m = fmaxf(m, x[g][r]);
-          m = max_over_quarters(m);
+          m = max_over_quarters(m) * p.qk_scale_log2;
           const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
           for (int g = 0; g < 4; ++g)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) l += fast_exp2(x[g][r] - ref);
+            for (int r = 0; r < 4; ++r) l += fast_exp2(fmaf(x[g][r], p.qk_scale_log2, -ref));
           l = sum_over_quarters(l);
           // (keys without a maximum add nothing, unless all that the row sees of them is NaN)
           if (kq == 0) s_ml[buf][wave][16 * i + n] = float2{l == 0.0f ? m : fmaxf(m, -3e38f), l};
@@ -493,7 +543,7 @@ static ScoresPlan scores_plan(const memopt_scores_desc &d) {
   pl.few = rows <= kFewRows;
   pl.max_rows = (int32_t)rows;
   pl.kts = (int32_t)((scored_keys(d) + kTileKeys - 1) / kTileKeys);
-  const int64_t ml = 8 * (int64_t)pl.kts * d.num_kv_heads * (pl.few ? d.batch * rows : d.tokens * G);
+  const int64_t ml = 8 * (int64_t)pl.kts * d.num_kv_heads * (pl.few ? 4 * d.batch * rows : d.tokens * G);
   pl.second = (ml + 255) / 256 * 256;
   pl.total = pl.second + (pl.few ? 4 * (int64_t)d.batch * d.num_kv_heads * rows * pl.kts * kTileKeys
                                  : 4 * (int64_t)d.num_kv_heads * d.tokens * G);
@@ -536,15 +586,19 @@ template <int FMT, int D>
 static int launch_scores(const ScoresParams &p, const ScoresPlan &pl, hipStream_t s) {
   const unsigned tiles = (unsigned)((std::max<int64_t>(p.max_keys, p.L) + kTileKeys - 1) / kTileKeys);
   const dim3 over_keys((unsigned)pl.kts * p.Hk, p.B), over_scores(tiles * p.Hk, p.B);
+  const dim3 finish((tiles + kFinishTiles - 1) / kFinishTiles * p.Hk, p.B);
   int rc;
   if (pl.total == 0) {
-    hipLaunchKernelGGL(finish_kernel, over_scores, dim3(256), 0, s, p);
+    hipLaunchKernelGGL(finish_kernel, finish, dim3(256), 0, s, p);
     return check_launch("attention_scores");
   }
   if (pl.few) {
-    hipLaunchKernelGGL((few_rows_kernel<FMT, D>), over_keys, dim3(256), 0, s, p);
+    // Tiles of a workgroup: as many as leave each compute unit eight workgroups (four are resident), at most eight.
+    const int64_t each = std::min<int64_t>(8, std::max<int64_t>(1, (int64_t)pl.kts * p.Hk * p.B / (8 * compute_units())));
+    const dim3 grid((unsigned)((pl.kts + each - 1) / each * p.Hk), p.B);
+    hipLaunchKernelGGL((few_rows_kernel<FMT, D>), grid, dim3(256), 0, s, p, (int32_t)each);
     if ((rc = check_launch("attention_scores(rows)")) != MEMOPT_OK) return rc;
-    hipLaunchKernelGGL(finish_kernel, over_scores, dim3(256), 0, s, p);
+    hipLaunchKernelGGL(finish_kernel, finish, dim3(256), 0, s, p);
     return check_launch("attention_scores(finish)");
   }
   hipLaunchKernelGGL((chunk_rows_kernel<FMT, D, false>), over_keys, dim3(256), 0, s, p);

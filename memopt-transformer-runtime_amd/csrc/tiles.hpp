@@ -168,6 +168,13 @@ __device__ __forceinline__ uint32_t tame(uint32_t w, uint32_t &odd) {
   return y;
 }
 
+// A block-table entry (or another uniform word that no kernel of the launch
+// writes) through the scalar cache: a vector load would be waited for together
+// with every load and copy before it.
+__device__ __forceinline__ int32_t uniform_entry(const int32_t *x) {
+  return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)uniform_ptr(x);
+}
+
 template <int N>
 struct IntConst {
   static constexpr int value = N;
