@@ -8,7 +8,9 @@ starts and lengths, so nothing is built on the host, nothing is read back,
 and steps can be captured into a graph. Attention is packed (requests bring
 any number of new tokens each) and grouped (fewer key heads than query
 heads): ``prompt_attention`` where all requests are new, ``packed_attention``
-over the cache else.
+over the cache else. It can keep count of the attention weight that each
+cached token gets and take those of least weight out (``compact``).
+``LatentBatch`` is the same over a latent cache.
 """
 from __future__ import annotations
 
@@ -21,45 +23,15 @@ import memopt_C
 from .kv_cache import pages_needed
 
 
-class PackedBatch:
-    """``num_requests`` requests of one attention layer over the ``memopt_C`` pool.
+class _Requests:
+    """Block tables, lengths and the ring of free pages of ``num_requests`` requests, on the device."""
 
-    Args:
-        num_blocks, num_kv_heads, head_dim, block_size, kv_format: the pool
-            (``init_pool``); 64 or 128 dims, 16-token pages (fp16 pools: a
-            multiple of 16). Any pool before is dropped.
-        num_requests: requests, live or free, at most 4096; a request is an
-            index ``0 .. num_requests - 1``.
-        max_tokens: the longest context that a request may reach.
-        num_rows: new tokens that one step may bring, of all requests together.
-        window_size, num_sink_tokens: the layer's mask (``dynamic_sparse_attention``).
-
-    A step is ``advance(new_tokens)`` (which tokens of which requests come,
-    decided by the caller), then ``attend(query, keys, values)`` with their
-    rows. The pool is the process-wide one: one ``PackedBatch`` or
-    ``PagedKVCache`` at a time.
-    """
-
-    def __init__(self, num_blocks: int, num_kv_heads: int, head_dim: int, num_requests: int, max_tokens: int,
-                 num_rows: int, block_size: int = 16, kv_format: str = "int4", window_size: int = -1,
-                 num_sink_tokens: int = 0) -> None:
-        if num_blocks <= 0 or block_size <= 0 or num_blocks * block_size > 2 ** 31:
-            raise RuntimeError("PackedBatch: the pool must hold 1 to 2^31 tokens (slots are int32)")
-        if not 0 < num_requests <= 4096:
-            raise RuntimeError("PackedBatch: num_requests must be 1 to 4096")
-        if max_tokens <= 0 or num_rows <= 0:
-            raise RuntimeError("PackedBatch: max_tokens and num_rows must be positive")
-        if head_dim not in (64, 128) or block_size % 16 or (kv_format == "int4" and block_size != 16):
-            raise RuntimeError("PackedBatch: head_dim must be 64 or 128, pages 16 tokens (fp16: a multiple of 16)")
-        memopt_C.reset_pool()
-        memopt_C.init_pool(num_blocks, block_size, num_kv_heads, head_dim, kv_format=kv_format)
+    def _start(self, name: str, pages: Sequence[int], num_requests: int, max_tokens: int, num_rows: int, block_size: int,
+               dev: torch.device) -> None:
+        self._name = name
         self.block_size = block_size
         self.max_tokens = max_tokens
-        self.window_size = window_size
-        self.num_sink_tokens = num_sink_tokens
-        dev = memopt_C.get_key_pool().device
-        # The pages leave the host's free list for a ring on the device.
-        self.free_pages = torch.tensor(memopt_C.allocate_blocks(num_blocks), dtype=torch.int32, device=dev)
+        self.free_pages = torch.tensor(pages, dtype=torch.int32, device=dev)
         self.tables = torch.full((num_requests, pages_needed(max_tokens, block_size)), -1, dtype=torch.int32, device=dev)
         # context_lens and free_span are advanced in place.
         self.state = memopt_C.advance_batch_buffers(num_requests, num_rows, dev)
@@ -67,7 +39,16 @@ class PackedBatch:
             t.zero_()
         for t in (self.state.slots, self.state.positions):
             t.fill_(-1)
-        self.state.free_span.copy_(torch.tensor([0, num_blocks], dtype=torch.int32))
+        self.state.free_span.copy_(torch.tensor([0, len(pages)], dtype=torch.int32))
+
+    @staticmethod
+    def _check_sizes(name: str, num_blocks: int, block_size: int, num_requests: int, max_tokens: int, num_rows: int) -> None:
+        if num_blocks <= 0 or block_size <= 0 or num_blocks * block_size > 2 ** 31:
+            raise RuntimeError(f"{name}: the pool must hold 1 to 2^31 tokens (slots are int32)")
+        if not 0 < num_requests <= 4096:
+            raise RuntimeError(f"{name}: num_requests must be 1 to 4096")
+        if max_tokens <= 0 or num_rows <= 0:
+            raise RuntimeError(f"{name}: max_tokens and num_rows must be positive")
 
     @property
     def num_rows(self) -> int:
@@ -84,6 +65,77 @@ class PackedBatch:
         return memopt_C.advance_batch(new_tokens, self.state.context_lens, self.tables, self.free_pages,
                                       self.state.free_span, self.block_size, out=self.state)
 
+    def _rows_of(self, query: torch.Tensor) -> None:
+        if query.shape[0] != self.num_rows:
+            raise RuntimeError(f"{self._name}: query has {query.shape[0]} rows, not num_rows={self.num_rows}")
+
+    def release(self, requests: Sequence[int]) -> None:
+        """Return the requests' linked pages to the ring; their indices are free
+        for new requests. (Waits for the device: the pages are read back.)"""
+        requests = list(dict.fromkeys(self._known(requests)))
+        if not requests:
+            return
+        rows = torch.tensor(requests, dtype=torch.int64, device=self.tables.device)
+        tables, lens = self.tables[rows].cpu(), self.state.context_lens[rows].cpu()
+        self._give_back([p for t, n in zip(tables.tolist(), lens.tolist())
+                         for p in t[:pages_needed(n, self.block_size)] if p >= 0])
+        self.tables[rows] = -1
+        self.state.context_lens[rows] = 0
+
+    def _known(self, requests: Sequence[int]) -> List[int]:
+        requests = [int(r) for r in requests]
+        if any(not 0 <= r < self.tables.shape[0] for r in requests):
+            raise RuntimeError(f"{self._name}: no such request")
+        return requests
+
+    def _give_back(self, pages: List[int]) -> None:
+        """Append ``pages`` to the ring."""
+        head, count = self.state.free_span.tolist()
+        at = (head + count + torch.arange(len(pages))) % self.free_pages.shape[0]
+        dev = self.free_pages.device
+        self.free_pages[at.to(dev)] = torch.tensor(pages, dtype=torch.int32, device=dev)
+        self.state.free_span[1] = count + len(pages)
+
+
+class PackedBatch(_Requests):
+    """``num_requests`` requests of one attention layer over the ``memopt_C`` pool.
+
+    Args:
+        num_blocks, num_kv_heads, head_dim, block_size, kv_format: the pool
+            (``init_pool``); 64 or 128 dims, 16-token pages (fp16 pools: a
+            multiple of 16). Any pool before is dropped.
+        num_requests: requests, live or free, at most 4096; a request is an
+            index ``0 .. num_requests - 1``.
+        max_tokens: the longest context that a request may reach.
+        num_rows: new tokens that one step may bring, of all requests together.
+        window_size, num_sink_tokens: the layer's mask (``dynamic_sparse_attention``).
+        track_weights: keep ``weights`` f32 ``[num_requests, num_kv_heads,
+            positions]``, what ``accumulate`` adds up and ``compact`` goes by.
+
+    A step is ``advance(new_tokens)`` (which tokens of which requests come,
+    decided by the caller), then ``attend(query, keys, values)`` with their
+    rows. The pool is the process-wide one: one ``PackedBatch`` or
+    ``PagedKVCache`` at a time.
+    """
+
+    def __init__(self, num_blocks: int, num_kv_heads: int, head_dim: int, num_requests: int, max_tokens: int,
+                 num_rows: int, block_size: int = 16, kv_format: str = "int4", window_size: int = -1,
+                 num_sink_tokens: int = 0, track_weights: bool = False) -> None:
+        self._check_sizes("PackedBatch", num_blocks, block_size, num_requests, max_tokens, num_rows)
+        if head_dim not in (64, 128) or block_size % 16 or (kv_format == "int4" and block_size != 16):
+            raise RuntimeError("PackedBatch: head_dim must be 64 or 128, pages 16 tokens (fp16: a multiple of 16)")
+        memopt_C.reset_pool()
+        memopt_C.init_pool(num_blocks, block_size, num_kv_heads, head_dim, kv_format=kv_format)
+        self.window_size = window_size
+        self.num_sink_tokens = num_sink_tokens
+        dev = memopt_C.get_key_pool().device
+        # The pages leave the host's free list for a ring on the device.
+        self._start("PackedBatch", memopt_C.allocate_blocks(num_blocks), num_requests, max_tokens, num_rows, block_size, dev)
+        positions = self.tables.shape[1] * block_size
+        self.weights = torch.zeros((num_requests, num_kv_heads, positions), device=dev) if track_weights else None
+        # Tokens that compaction took out of each request: what its positions lack.
+        self.removed = torch.zeros(num_requests, dtype=torch.int32, device=dev)
+
     def attend(self, query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, max_new: Optional[int] = None,
                prompts: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Write the step's keys and values and attend; returns ``[num_rows, Hq, D]``.
@@ -95,8 +147,7 @@ class PackedBatch:
         ``prompts``: every request with rows is new, so attention reads the
         rows themselves, not their quantized copies.
         """
-        if query.shape[0] != self.num_rows:
-            raise RuntimeError(f"PackedBatch: query has {query.shape[0]} rows, not num_rows={self.num_rows}")
+        self._rows_of(query)
         memopt_C.write_cache(keys, values, None, self.state.slots, validate_slots=False)
         if prompts:
             return memopt_C.prompt_attention(query, keys, values, self.state.cu_seqlens, self.window_size,
@@ -144,29 +195,125 @@ class PackedBatch:
         self._give_back(freed)
         return freed
 
+    def accumulate(self, query: torch.Tensor, max_new: Optional[int] = None) -> torch.Tensor:
+        """Add to ``weights`` what the step's queries (as in ``attend``, which
+        comes first) give each cached token; returns it. Every step, or only
+        where a prompt ends, as the policy has it."""
+        if self.weights is None:
+            raise RuntimeError("PackedBatch: made without track_weights")
+        self._rows_of(query)
+        return memopt_C.attention_scores(query, memopt_C.get_key_pool(), self.tables, self.state.context_lens,
+                                         self.state.cu_seqlens, self.num_rows if max_new is None else max_new,
+                                         self.max_tokens, self.window_size, num_sink_tokens=self.num_sink_tokens,
+                                         scores=self.weights, out=self.weights)
+
+    def compact(self, requests: Sequence[int], keep: int, num_sink_tokens: int = 4, num_recent_tokens: int = 0) -> List[int]:
+        """Cut the requests to ``keep`` tokens per head, those of most weight (``compact_cache``); returns the
+        requests that now have their tokens in fresh pages.
+
+        Old pages go back to the ring. A request that has no more than
+        ``keep`` stays as it is. The fresh pages come from the ring while the
+        old ones are still taken: where they do not last for all, requests
+        are compacted one after another, and those for which even that does
+        not suffice stay. Tokens that come later stand behind the ``keep``
+        (``token_positions`` says where they stand in the text). (Waits for
+        the device.)
+        """
+        if self.weights is None:
+            raise RuntimeError("PackedBatch: made without track_weights")
+        requests = self._known(requests)
+        if len(set(requests)) != len(requests):
+            raise RuntimeError("PackedBatch: a request is named twice")
+        if keep < 0:
+            raise RuntimeError("PackedBatch: keep must not be negative")
+        done: List[int] = []
+        todo, limit = requests, min(keep, self.weights.shape[2])
+        while todo:
+            rows = torch.tensor(todo, dtype=torch.int64, device=self.tables.device)
+            want = torch.full((len(todo),), limit, dtype=torch.int32, device=self.tables.device)
+            lens = self.state.context_lens[rows]
+            r = memopt_C.compact_cache(self.weights[rows], memopt_C.get_key_pool(), memopt_C.get_value_pool(), self.tables[rows],
+                                       lens, want, self.free_pages, self.state.free_span, num_sink_tokens=num_sink_tokens,
+                                       num_recent_tokens=num_recent_tokens, max_keep=limit)
+            self.tables[rows] = r.block_tables
+            self.state.context_lens[rows] = r.context_lens
+            self.weights[rows] = r.scores
+            self.removed[rows] += lens - r.context_lens
+            self.state.free_span.copy_(r.free_span)
+            status = r.status.tolist()
+            served = [b for b, s in zip(todo, status) if s == 0]
+            done += served
+            short = [b for b, s in zip(todo, status) if s == 3]
+            # (sums over all that ask decide: behind one that is refused, another may still fit by itself)
+            todo = short if served else short[1:]
+        return done
+
+    def token_positions(self) -> torch.Tensor:
+        """Where the step's rows stand in their texts (int32 ``[num_rows]``): ``state.positions``, which count cached
+        tokens, plus the tokens that compaction took out before; -1 behind the last row."""
+        rows = torch.arange(self.num_rows, dtype=torch.int32, device=self.tables.device)
+        owner = torch.searchsorted(self.state.cu_seqlens, rows, right=True) - 1
+        at = self.state.positions + self.removed[owner.clamp(0, self.removed.shape[0] - 1)]
+        return torch.where(self.state.positions >= 0, at, -1)
+
     def release(self, requests: Sequence[int]) -> None:
-        """Return the requests' linked pages to the ring; their indices are free
-        for new requests. (Waits for the device: the pages are read back.)"""
-        requests = list(dict.fromkeys(self._known(requests)))
-        if not requests:
-            return
-        rows = torch.tensor(requests, dtype=torch.int64, device=self.tables.device)
-        tables, lens = self.tables[rows].cpu(), self.state.context_lens[rows].cpu()
-        self._give_back([p for t, n in zip(tables.tolist(), lens.tolist())
-                         for p in t[:pages_needed(n, self.block_size)] if p >= 0])
-        self.tables[rows] = -1
-        self.state.context_lens[rows] = 0
+        super().release(requests)
+        rows = torch.tensor(self._known(requests), dtype=torch.int64, device=self.tables.device)
+        self.removed[rows] = 0
+        if self.weights is not None:
+            self.weights[rows] = 0.0
 
-    def _known(self, requests: Sequence[int]) -> List[int]:
-        requests = [int(r) for r in requests]
-        if any(not 0 <= r < self.tables.shape[0] for r in requests):
-            raise RuntimeError("PackedBatch: no such request")
-        return requests
 
-    def _give_back(self, pages: List[int]) -> None:
-        """Append ``pages`` to the ring."""
-        head, count = self.state.free_span.tolist()
-        at = (head + count + torch.arange(len(pages))) % self.free_pages.shape[0]
-        dev = self.free_pages.device
-        self.free_pages[at.to(dev)] = torch.tensor(pages, dtype=torch.int32, device=dev)
-        self.state.free_span[1] = count + len(pages)
+class LatentBatch(_Requests):
+    """``num_requests`` requests of one layer of latent attention.
+
+    The cache is this object's own (``cache`` ``[num_blocks, block_size, rank
+    + rope_dim]``, one row per token for all heads), not the ``memopt_C`` pool.
+
+    Args:
+        num_blocks, rank, rope_dim, block_size, dtype, device: the cache; rank
+            128, 256 or 512, rope_dim 32 or 64, pages of a multiple of 16
+            tokens, fp16 or bf16 (device: the current one).
+        num_requests, max_tokens, num_rows, window_size, num_sink_tokens: as in ``PackedBatch``.
+
+    A step is ``advance(new_tokens)``, then ``attend`` (or, where every
+    request with rows is new, ``attend_prompts``) with their rows.
+    """
+
+    def __init__(self, num_blocks: int, rank: int, rope_dim: int, num_requests: int, max_tokens: int, num_rows: int,
+                 block_size: int = 16, dtype: torch.dtype = torch.bfloat16, window_size: int = -1,
+                 num_sink_tokens: int = 0, device: Optional[torch.device] = None) -> None:
+        self._check_sizes("LatentBatch", num_blocks, block_size, num_requests, max_tokens, num_rows)
+        if rank not in (128, 256, 512) or rope_dim not in (32, 64) or block_size % 16:
+            raise RuntimeError("LatentBatch: rank must be 128, 256 or 512, rope_dim 32 or 64, pages a multiple of 16 tokens")
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise RuntimeError("LatentBatch: dtype must be fp16 or bf16")
+        dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        self.rank = rank
+        self.window_size = window_size
+        self.num_sink_tokens = num_sink_tokens
+        self.cache = torch.zeros((num_blocks, block_size, rank + rope_dim), dtype=dtype, device=dev)
+        self._start("LatentBatch", range(num_blocks), num_requests, max_tokens, num_rows, block_size, dev)
+
+    def attend(self, query: torch.Tensor, latents: torch.Tensor, rope_keys: torch.Tensor, scale: float,
+               max_new: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Write the step's latents ``[num_rows, rank]`` and rotary keys
+        ``[num_rows, rope_dim]`` and attend over the cache (``latent_attention``);
+        returns ``[num_rows, Hq, rank]``. ``max_new``: at least the most rows
+        of a request (default: num_rows)."""
+        self._rows_of(query)
+        memopt_C.write_latent(latents, rope_keys, self.state.slots, self.cache)
+        return memopt_C.latent_attention(query, self.cache, self.tables, self.state.context_lens, self.state.cu_seqlens,
+                                         self.num_rows if max_new is None else max_new, self.max_tokens, scale, self.rank,
+                                         self.window_size, num_sink_tokens=self.num_sink_tokens, out=out)
+
+    def attend_prompts(self, query: torch.Tensor, keys: torch.Tensor, latents: torch.Tensor, rope_keys: torch.Tensor,
+                       values: torch.Tensor, scale: Optional[float] = None,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The same where every request with rows is new: attention from the
+        heads' own ``keys`` and ``values`` (``latent_prompt_attention``);
+        returns ``[num_rows, H, head_dim]``."""
+        self._rows_of(query)
+        memopt_C.write_latent(latents, rope_keys, self.state.slots, self.cache)
+        return memopt_C.latent_prompt_attention(query, keys, rope_keys, values, self.state.cu_seqlens, self.window_size,
+                                                num_sink_tokens=self.num_sink_tokens, scale=scale, out=out)
