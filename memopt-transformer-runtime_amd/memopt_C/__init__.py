@@ -830,16 +830,18 @@ def _out_rows(fn: str, out: Optional[torch.Tensor], query: torch.Tensor,
               width: Optional[int] = None) -> Tuple[torch.Tensor, int, int, int]:
     """(out, address, token stride, head stride); a fresh tensor for ``None``. ``width``: its last dimension, where
     that is not query's."""
-    if width is not None and width != query.shape[2]:
-        query = query[:, :, :width] if width < query.shape[2] else query.new_empty((1, 1, width)).expand(*query.shape[:2], width)
     if out is None:
-        out = torch.empty_like(query, memory_format=torch.contiguous_format)  # (half the time of torch.empty)
+        if width is None:
+            out = torch.empty_like(query, memory_format=torch.contiguous_format)  # (half the time of torch.empty)
+        else:
+            out = torch.empty((query.shape[0], query.shape[1], width), dtype=query.dtype, device=query.device)
         _, H, D = out.shape
         return out, out.data_ptr(), H * D, D
     _device_tensors(fn, query.device, ("out",), out)
-    if not (out.shape == query.shape and out.dtype == query.dtype):
+    shape = query.shape if width is None else query.shape[:2] + (width,)
+    if not (out.shape == shape and out.dtype == query.dtype):
         raise RuntimeError(f"{fn}: out must be shaped like query, with its dtype" if width is None else
-                           f"{fn}: out must be {list(query.shape)}, with query's dtype")
+                           f"{fn}: out must be {list(shape)}, with query's dtype")
     ts, hs, ds = out.stride()
     p = out.data_ptr()
     T, H, D = out.shape
@@ -1244,7 +1246,7 @@ def attention_scores(query: torch.Tensor, key_cache: torch.Tensor, block_tables:
             raise RuntimeError(f"{fn}: out must be contiguous f32 {[B, Hk, L]}")
         _no_grad(fn, out.requires_grad)
     q, pq, qts, qhs = _near_rows(query, Hq // max(1, Hk))
-    head = (pq, None if scores is None else scores.data_ptr(), out.data_ptr(), T, B, Hq, Hk, D, qts, qhs, fmt, pk, bs, nb,
+    head = (pq, 0 if scores is None else scores.data_ptr(), out.data_ptr(), T, B, Hq, Hk, D, qts, qhs, fmt, pk, bs, nb,
             block_tables.data_ptr(), M, context_lens.data_ptr(), cu_seqlens.data_ptr(), _count32(max_query_len),
             _count32(max_seq_len), _count32(window_size), _count32(num_sink_tokens), L)
     _launch(fn, _SCORES, head, _c_scores_ws, _c_scores, device)
@@ -1252,19 +1254,23 @@ def attention_scores(query: torch.Tensor, key_cache: torch.Tensor, block_tables:
 
 
 def _launch(fn: str, packed: struct.Struct, head: tuple, size, call, device: torch.device) -> None:
-    """One call of a C entry whose descriptor ends in a workspace: ``head`` and then a fresh one of ``size``'s bytes
-    (any content) from torch's caching allocator, on the current stream of ``device``, which is current."""
+    """One call of a C entry whose descriptor ends in a workspace: ``head`` (numbers) and then a fresh one of ``size``'s
+    bytes (any content) from torch's caching allocator, on the current stream of ``device``, which is current."""
     try:
-        d = packed.pack(*(x or 0 for x in head), 0, 0)
+        d = packed.pack(*head, 0, 0)
     except struct.error:
         raise RuntimeError(f"{fn}: sizes must fit 32 bits") from None
     need = _i64()
-    _check(size(d, ctypes.byref(need)))
+    rc = size(d, need)
+    if rc:
+        _check(rc)
     n = need.value
     if n:
         ws = torch.empty(n, dtype=torch.uint8, device=device)
         d = d[:-16] + _WORKSPACE.pack(ws.data_ptr(), n)
-    _check(call(d, torch._C._cuda_getCurrentRawStream(device.index)))
+    rc = call(d, torch._C._cuda_getCurrentRawStream(device.index))
+    if rc:
+        _check(rc)
 
 
 _WORKSPACE = struct.Struct("@Pq")
@@ -1551,7 +1557,10 @@ def latent_prompt_attention(query: torch.Tensor, keys: torch.Tensor, rope_keys: 
     out, po, ots, ohs = _out_rows(fn, out, query, D)
     q, pq, qts, qhs = _rows(query)
     k, pk, kts, khs = _rows(keys, _FAR)
-    r, pr, rts, _ = _rows(rope_keys[:, None], _FAR)
+    rts, rds = rope_keys.stride()
+    r, pr = rope_keys, rope_keys.data_ptr()
+    if not (rds == 1 and not (rts % 8 or pr % 16) and P <= rts < _FAR):
+        r, pr, rts, _ = _rows(rope_keys[:, None], _FAR)
     v, pv, vts, vhs = _rows(values, _FAR)
     try:
         d = _LATENT_PROMPT.pack(pq, pk, pr, pv, po, 1 if dtype is torch.bfloat16 else 0, T, cu_seqlens.shape[0] - 1, H, D, P,
