@@ -448,21 +448,33 @@ __global__ __launch_bounds__(256, 2) void chunk_rows_kernel(const ScoresParams p
         if constexpr (K::CODES)
 #pragma unroll
           for (int c = 0; c < NCH; ++c) q[c] = in_code_order(q[c]);
-        f32x4p_t x[4];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          x[g] = K::scores(a[g], f[g], q);
-          if (!full) x[g] = hide(p, x[g], key0 + 16 * g + 4 * kq, pos, s.len, row < s.rows && ((linked >> g) & 1));
-        }
         if constexpr (SUM) {
+          if (full) {
 #pragma unroll
-          for (int g = 0; g < 4; ++g)
+            for (int g = 0; g < 4; ++g) {
+              const f32x4p_t x = K::scores(a[g], f[g], q);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float y = fast_exp2(fmaf(x[g][r], p.qk_scale_log2, -lse[i]));
-              w[g][r] += !full && x[g][r] == -INFINITY ? 0.0f : y;  // (a hidden key takes no part in a row of NaN)
+              for (int r = 0; r < 4; ++r) w[g][r] += fast_exp2(fmaf(x[r], p.qk_scale_log2, -lse[i]));
             }
+          } else {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const f32x4p_t x = hide(p, K::scores(a[g], f[g], q), key0 + 16 * g + 4 * kq, pos, s.len,
+                                      row < s.rows && ((linked >> g) & 1));
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const float y = fast_exp2(fmaf(x[r], p.qk_scale_log2, -lse[i]));
+                w[g][r] += x[r] == -INFINITY ? 0.0f : y;  // (a hidden key takes no part in a row of NaN)
+              }
+            }
+          }
         } else {
+          f32x4p_t x[4];
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            x[g] = K::scores(a[g], f[g], q);
+            if (!full) x[g] = hide(p, x[g], key0 + 16 * g + 4 * kq, pos, s.len, row < s.rows && ((linked >> g) & 1));
+          }
           float m = x[0][0], l = 0.0f;
 #pragma unroll
           for (int g = 0; g < 4; ++g)
@@ -518,13 +530,18 @@ __global__ __launch_bounds__(256) void lse_kernel(const ScoresParams p) {
   const int32_t pos = s.pos0 + p.by_g(row), tiles = (min(s.len, pos + 1) + kTileKeys - 1) / kTileKeys;
   const float2 *src = p.ml + (int64_t)h * p.kts * p.T * p.G + (int64_t)s.start * p.G + row;
   float m = -INFINITY, l = 0.0f;
-  for (int32_t t = 0; t < tiles; ++t) {
-    if (!meets(p, pos, t * kTileKeys, (t + 1) * kTileKeys)) continue;
-    const float2 x = src[(int64_t)t * p.T * p.G];
-    const float top = fmaxf(m, x.x);
-    if (top == -INFINITY) continue;
-    l = l * fast_exp2(m - top) + x.y * fast_exp2(x.x - top);
-    m = top;
+  for (int32_t t0 = 0; t0 < tiles; t0 += 8) {
+    float2 x[8];  // (eight reads in flight)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = src[(int64_t)min(t0 + i, tiles - 1) * p.T * p.G];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int32_t t = t0 + i;
+      const float top = fmaxf(m, x[i].x);
+      if (t >= tiles || !meets(p, pos, t * kTileKeys, (t + 1) * kTileKeys) || top == -INFINITY) continue;
+      l = l * fast_exp2(m - top) + x[i].y * fast_exp2(x[i].x - top);
+      m = top;
+    }
   }
   p.lse[(int64_t)h * p.T * p.G + (int64_t)s.start * p.G + row] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
