@@ -282,8 +282,8 @@ __device__ __forceinline__ void select_row(const CompactParams &p, SelectShared 
     const uint64_t tie = __ballot(u == prefix);
     const bool take = u > prefix || (u == prefix && ties + (uint32_t)__popcll(tie & below) < want);
     const uint64_t all = __ballot(take);
-    if (take) {
-      const uint32_t i = at + (uint32_t)__popcll(all & below);
+    const uint32_t i = at + (uint32_t)__popcll(all & below);
+    if (take && i < (uint32_t)n) {  // (never past n, unless the scores change under the call)
       kept[i] = j;
       dst[i] = x;
     }
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(256) void compact_move_kernel(const CompactParams p
   if (!page_ok(p, page)) return;  // (the ring held something that is no page)
   // Old page and place of new token i0 + t, in lane t.
   const int32_t mine = i0 + (lane & 15) < n ? p.kept[unit * p.K + i0 + (lane & 15)] : -1;
-  const int32_t old = mine < 0 ? -1 : p.bt[(int64_t)b * p.M + mine / p.bs], at = mine < 0 ? 0 : mine % p.bs;
+  const int32_t old = mine < 0 || mine >= p.ctx[b] ? -1 : p.bt[(int64_t)b * p.M + mine / p.bs], at = mine < 0 ? 0 : mine % p.bs;
   if constexpr (FMT == MEMOPT_KV_INT4) {
     // Lane 8 q + c owns tokens q and q + 8 of the new block, as in page_format.hpp.
     constexpr int BPL = D / 8, G = D / 64, W = BPL / 4;  // bytes and words of a lane's K (and of its V)
@@ -546,8 +546,7 @@ extern "C" int memopt_compact_cache(const memopt_compact_desc *desc, void *strea
   if ((rc = check_launch("compact_cache(count)")) != MEMOPT_OK) return rc;
   // (no request is longer than its table or its scores)
   p.in_lds = (int32_t)std::min<int64_t>(kInLds, std::min<int64_t>((int64_t)p.M * p.bs, p.L));
-  static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(&compact_select_kernel),
-                                                    hipFuncAttributeMaxDynamicSharedMemorySize, 4 * kInLds);
+  const hipError_t set = allow_lds<&compact_select_kernel>(4 * kInLds);
   MEMOPT_REQUIRE(set == hipSuccess, MEMOPT_ERR_HIP, std::string("compact_cache: ") + hipGetErrorString(set));
   hipLaunchKernelGGL(compact_select_kernel, dim3(p.Hk, p.N), dim3(1024), 4 * p.in_lds, s, p);
   if ((rc = check_launch("compact_cache(select)")) != MEMOPT_OK) return rc;

@@ -133,7 +133,8 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
   uint32_t at = w * run;
   const uint32_t end = min(total, at + run), begin = at;
   if (at >= end) return;
-  LatentPlace place = latent_place<ROWS, false>(p, at, false);
+  const LatentPlace place = latent_place<ROWS, false>(p, at, false);
+  if (place.b < 0) return;
   int32_t b = __builtin_amdgcn_readfirstlane(place.b);
   uint32_t before = __builtin_amdgcn_readfirstlane(place.before);
 
@@ -162,7 +163,8 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
     LatentSeq s = uniform_seq<ROWS>(p, b);
     while (at >= before + (uint32_t)s.tiles * (uint32_t)s.steps) {
       before += (uint32_t)s.tiles * (uint32_t)s.steps;
-      s = uniform_seq<ROWS>(p, ++b);
+      if (++b >= p.B) return;  // (sequences that overlap: their steps may pass 32 bits)
+      s = uniform_seq<ROWS>(p, b);
     }
     const int32_t rt = (int32_t)((at - before) / (uint32_t)s.steps), first_step = (int32_t)((at - before) % (uint32_t)s.steps);
     const int32_t last_step = (int32_t)min((uint32_t)s.steps, (uint32_t)first_step + (end - at));
@@ -617,8 +619,7 @@ static int validate_latent(const memopt_latent_desc &d) {
 template <class E, int R, int P, int RW>
 static int launch_latent(const LatentParams &p, int64_t units, hipStream_t s) {
   constexpr int bytes = LatentLds<R, P, RW>::bytes;
-  static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(&latent_kernel<E, R, P, RW>),
-                                                    hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  const hipError_t set = allow_lds<&latent_kernel<E, R, P, RW>>(bytes);
   MEMOPT_REQUIRE(set == hipSuccess, MEMOPT_ERR_HIP, std::string("latent_attention: ") + hipGetErrorString(set));
   hipLaunchKernelGGL((latent_kernel<E, R, P, RW>), dim3((unsigned)p.wgs), dim3(128 * RW), bytes, s, p);
   int rc = check_launch("latent_attention");

@@ -2,6 +2,8 @@
 // the 16-bit operand types, transposed LDS reads, and the order in which
 // workgroups take the tiles of sequences of different lengths.
 #pragma once
+#include <atomic>
+
 #include "packed.hpp"
 
 namespace memopt {
@@ -173,6 +175,19 @@ __device__ __forceinline__ uint32_t tame(uint32_t w, uint32_t &odd) {
 // with every load and copy before it.
 __device__ __forceinline__ int32_t uniform_entry(const int32_t *x) {
   return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)uniform_ptr(x);
+}
+
+// More than 64 KiB of LDS is allowed per kernel and device: once for each.
+template <auto Kernel>
+static hipError_t allow_lds(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int device = 0;
+  hipError_t e = hipGetDevice(&device);
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (e != hipSuccess || (done.load(std::memory_order_relaxed) & bit)) return e;
+  e = hipFuncSetAttribute(reinterpret_cast<const void *>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 template <int N>

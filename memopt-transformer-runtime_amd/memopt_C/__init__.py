@@ -1433,6 +1433,7 @@ def write_latent(latents: torch.Tensor, rope_keys: torch.Tensor, slot_mapping: t
     fp16 or bf16 like the rows); token t's row goes to slot
     ``slot_mapping[t]`` (int32; page * block_size + offset, as for
     ``write_cache``); slots outside the cache, -1 among them, are skipped.
+    No two tokens may have one slot (pieces of both rows could stay).
     ``rank`` and ``rope_dim`` are multiples of 8. Rows may be views (of a
     fused projection): they are read in place where they are 16-byte aligned.
     """

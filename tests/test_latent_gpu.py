@@ -284,6 +284,23 @@ def test_captured_calls_and_other_streams():
     assert all(torch.equal(x, want) for x in got)
 
 
+@pytest.mark.parametrize("given,meant", [([-5, 3, 2 ** 31 - 1], [0, 3, 9]), ([2, 1, 5], [1, 1, 5]), ([9, -1, 9], [0, 0, 9]),
+                                         ([-2 ** 31, -1, 4], [0, 0, 4])])
+def test_starts_out_of_range_or_order(given, meant):
+    """Starts are held within the rows, and a sequence that would end before it begins has none."""
+    c = Case(torch.float16, [400, 90], [3, 6], 5, 128, 32, seed=2)
+    for most in (9, 2):
+        outs = []
+        for cu in (given, meant):
+            c.cu = torch.tensor(cu, dtype=torch.int32, device=dev())
+            outs.append(c.run(most=most, out=torch.full((9, 5, 128), 7.0, dtype=c.dtype, device=dev())))
+        first = [c.cu[0].item(), c.cu[1].item()]
+        rows = [r for b, a in enumerate(first) for r in range(a, min(a + most, c.cu[b + 1].item()))]
+        assert torch.equal(outs[0][rows], outs[1][rows])
+        rest = [r for r in range(9) if r not in rows]
+        assert torch.equal(outs[0][rest], torch.full_like(outs[0][rest], 7.0))
+
+
 def test_empty_calls():
     c = Case(torch.float16, [20, 30], [1, 1], 4, 128, 32)
     assert c.run(most=0).shape == (2, 4, 128)

@@ -125,6 +125,20 @@ def test_no_rows_leaves_scores(qn):
     assert none.shape == (0, 2, 96)
 
 
+@pytest.mark.parametrize("most", [1, 30])
+@pytest.mark.parametrize("given,meant", [([-5, 3, 2 ** 31 - 1], [0, 3, 30]), ([2, 1, 5], [1, 1, 5]), ([30, -1, 9], [0, 0, 9])])
+def test_starts_out_of_range_or_order(given, meant, most):
+    """Starts are held within the rows, and a sequence that would end before it begins has none."""
+    c = Case("int4", [400, 90], [3, 27], 8, 2, 64, seed=2)
+    outs = []
+    for cu in (given, meant):
+        c.cu = torch.tensor(cu, dtype=torch.int32, device=dev())
+        outs.append(run(c, most=most))
+    assert torch.equal(*outs)
+    if meant[1] == meant[0]:
+        assert not outs[0][0].any()
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("qn", [[1, 2, 1], [30, 20, 25]])
 def test_contexts_outside_the_block_table_and_past_max_seq_len(fmt, qn):
