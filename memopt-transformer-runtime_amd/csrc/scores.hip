@@ -105,16 +105,25 @@ struct Keys {
   uint4 sc[CODES ? 4 : 1][NG];
   u32x4p_t rows[CODES ? 1 : 4][NCH];
 
-  __device__ __forceinline__ void load(const ScoresParams &p, int32_t b, int32_t h, int32_t key0, int32_t len) {
+  // Block-table entries of the pages of 64 keys, -1 past the end.
+  static __device__ __forceinline__ int4 entries(const ScoresParams &p, int32_t b, int32_t key0, int32_t len) {
+    int32_t e[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int32_t key = key0 + 16 * g, c = key >> 4;
+      e[g] = key < len ? uniform_entry(p.bt + (int64_t)b * p.M + (CODES ? c : p.by_chunks(c))) : -1;
+    }
+    return int4{e[0], e[1], e[2], e[3]};
+  }
+  __device__ __forceinline__ void load(const ScoresParams &p, const int4 &pages, int32_t h, int32_t key0) {
     const int lane = threadIdx.x & 63, t = lane & 15, kq = lane >> 4;
     constexpr int BPL = D / 8;
     linked = 0;
     const uint8_t *at[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int32_t key = key0 + 16 * g, c = key >> 4, e = CODES ? c : p.by_chunks(c);
-      const int32_t first = CODES ? 0 : 16 * (c - e * (int32_t)p.by_chunks.d);
-      const int32_t page = key < len ? uniform_entry(p.bt + (int64_t)b * p.M + e) : -1;
+      const int32_t c = (key0 >> 4) + g, first = CODES ? 0 : 16 * (c - p.by_chunks(c) * (int32_t)p.by_chunks.d);
+      const int32_t page = g == 0 ? pages.x : g == 1 ? pages.y : g == 2 ? pages.z : pages.w;
       const bool ok = page >= 0 && page < p.nb;
       linked |= (ok ? 1u : 0u) << g;
       at[g] = ok ? p.k + (int64_t)page * p.k_ps + h * p.k_hs + first * p.k_ts : nullptr;
@@ -149,6 +158,51 @@ struct Keys {
         for (int c = 0; c < NCH; ++c)
           rows[g][c] = *reinterpret_cast<const u32x4p_t *>(at[g] + t * p.k_ts + 2 * (64 * (c >> 1) + 16 * kq + 8 * (c & 1)));
       }
+    }
+  }
+  // The same for codes by way of LDS, a tile ahead: fetch() starts copies of the four pages' codes into the wave's 4 KiB
+  // at `to` and a read of their scales, take() waits for them, page() brings page g's. A copy's lanes lie side by side;
+  // lanes that read the operand layout from memory, 128 bytes apart, take 64 accesses of the cache where a copy
+  // takes 16, which bounded the kernel (32 sequences of up to 8192 tokens: 17.3 M accesses and 42 us, now 4.4 M and
+  // 33). (16-byte pieces are swizzled by the token.)
+  uint32_t scales;  // lane 16 g + i: word i of page g's
+  __device__ __forceinline__ void fetch(const ScoresParams &p, const int4 &pages, int32_t h, const uint8_t *to) {
+    const int lane = threadIdx.x & 63;
+    constexpr int PPT = D / 16;  // pieces of a token pair
+    const int row = lane / PPT;
+    const uint32_t off[1] = {(uint32_t)(16 * (PPT * row + ((lane % PPT) ^ (row % PPT))))};
+    linked = 0;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int32_t page = g == 0 ? pages.x : g == 1 ? pages.y : g == 2 ? pages.z : pages.w;
+      const bool ok = page >= 0 && page < p.nb;
+      linked |= (ok ? 1u : 0u) << g;
+      lds_dma<0, 1>(uniform_rsrc(p.k + (int64_t)(ok ? page : 0) * p.k_ps + h * p.k_hs, ok ? 8 * D : 0),
+                    lds_u32(to) + 1024 * g, off, 0);
+    }
+    const int32_t mine = lane < 32 ? (lane < 16 ? pages.x : pages.y) : (lane < 48 ? pages.z : pages.w);
+    scales = *reinterpret_cast<const uint32_t *>(p.k + (int64_t)(mine >= 0 && mine < p.nb ? mine : 0) * p.k_ps + h * p.k_hs +
+                                                 16 * D + 4 * (lane % (8 * NG)));
+  }
+  __device__ __forceinline__ void take(uint32_t *s_scales) {
+    asm volatile("" : "+v"(scales) : : "memory");  // (the scales were read last: once they are here, the copies are)
+    s_scales[threadIdx.x & 63] = scales;
+  }
+  __device__ __forceinline__ void page(int g, const uint8_t *from, const uint32_t *s_scales) {
+    const int lane = threadIdx.x & 63, t = lane & 15, kq = lane >> 4;
+    const uint8_t *at = from + 1024 * g + (D == 128 ? 8 : 4) * (t >> 3);
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      if constexpr (D == 128) {
+        const uint2 x = *reinterpret_cast<const uint2 *>(at + 16 * (8 * (t & 7) + ((4 * i + kq) ^ (t & 7))));
+        w[g][2 * i] = x.x;
+        w[g][2 * i + 1] = x.y;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          w[g][j] = *reinterpret_cast<const uint32_t *>(at + 16 * (4 * (t & 7) + (kq ^ (t & 3))) + 8 * j);
+      }
+      sc[g][i] = *reinterpret_cast<const uint4 *>(s_scales + 16 * g + 8 * i + 4 * (kq & 1));
     }
   }
   // Page g's operands, and the factors of the register's keys.
@@ -204,8 +258,12 @@ __device__ __forceinline__ f32x4p_t hide(const ScoresParams &p, f32x4p_t x, int3
 // ---------------------------------------------------------------------------
 // Few rows (decode): up to kFewRows rows per sequence and key head
 // ---------------------------------------------------------------------------
-// The weights relative to the tile's maximum are kept instead of reading the
+// The weights relative to a wave's maximum are kept instead of reading the
 // keys again: 8 bytes per row and key against D / 2 + 2 D / 64 of INT4.
+// Bound by vector instructions (unpacking, scales and weights: 0.62 of the
+// units' time) and by the chain table, keys, weights of each tile: 32
+// sequences of up to 8192 tokens, 8 key heads of 4 rows, 128: 33 us of which
+// the bytes take 16, and 13 for the second launch.
 
 template <int FMT, int D>
 __global__ __launch_bounds__(256, 4) void few_rows_kernel(const ScoresParams p, const int32_t tiles_each) {
@@ -227,15 +285,38 @@ __global__ __launch_bounds__(256, 4) void few_rows_kernel(const ScoresParams p, 
     if constexpr (K::CODES) q[c] = in_code_order(q[c]);
   }
   const int64_t unit = (int64_t)b * p.Hk + h;
-  for (int32_t kt = kt0; kt < kt1; ++kt) {
+  auto met = [&](int32_t kt) {
     int32_t lo, hi;
     queries_of(p, s, s.rows / p.G, kt * kTileKeys, (kt + 1) * kTileKeys, lo, hi);
-    if (hi <= lo) continue;
-    const int32_t key0 = kt * kTileKeys + 64 * wave;
-    K keys;
-    keys.load(p, b, h, key0, s.len);
+    return kt < kt1 && hi > lo;
+  };
+  auto entries_at = [&](int32_t kt) { return K::entries(p, b, kt * kTileKeys + 64 * wave, met(kt) ? s.len : 0); };
+  __shared__ __attribute__((aligned(16))) uint8_t s_codes[K::CODES ? 4 : 1][2][K::CODES ? 4096 : 1];
+  __shared__ __attribute__((aligned(16))) uint32_t s_scales[4][64];
+  K keys;
+  int4 pages = entries_at(kt0);
+  if constexpr (K::CODES) {
+    keys.fetch(p, pages, h, s_codes[wave][0]);
+    pages = entries_at(kt0 + 1);
+  }
+  for (int32_t kt = kt0; kt < kt1; ++kt) {
+    const int32_t key0 = kt * kTileKeys + 64 * wave, buf = (kt - kt0) & 1;
+    uint32_t linked;
+    if constexpr (K::CODES) {
+      keys.take(s_scales[wave]);
+      linked = keys.linked;
+      if (kt + 1 < kt1) keys.fetch(p, pages, h, s_codes[wave][buf ^ 1]);
+      pages = entries_at(kt + 2);
+      if (!met(kt)) continue;
+    } else {
+      const int4 here = pages;
+      pages = entries_at(kt + 1);
+      if (!met(kt)) continue;
+      keys.load(p, here, h, key0);
+      linked = keys.linked;
+    }
     // (rows past the last are not stored: what their lanes hold does not matter)
-    const bool full = key0 + 63 <= s.pos0 && key0 + 64 <= s.len && keys.linked == 15u &&
+    const bool full = key0 + 63 <= s.pos0 && key0 + 64 <= s.len && linked == 15u &&
                       (key0 > last - p.W || key0 + 64 <= p.sinks);
     f32x4p_t x[4];
     float m = -INFINITY;
@@ -243,9 +324,10 @@ __global__ __launch_bounds__(256, 4) void few_rows_kernel(const ScoresParams p, 
     for (int g = 0; g < 4; ++g) {
       u32x4p_t a[K::NCH];
       f32x4p_t f[K::NG];
+      if constexpr (K::CODES) keys.page(g, s_codes[wave][buf], s_scales[wave]);
       keys.operands(g, a, f);
       x[g] = K::scores(a, f, q);
-      if (!full) x[g] = hide(p, x[g], key0 + 16 * g + 4 * kq, pos, s.len, (keys.linked >> g) & 1);
+      if (!full) x[g] = hide(p, x[g], key0 + 16 * g + 4 * kq, pos, s.len, (linked >> g) & 1);
 #pragma unroll
       for (int r = 0; r < 4; ++r) m = fmaxf(m, x[g][r]);
     }
@@ -386,7 +468,7 @@ __global__ __launch_bounds__(256, 2) void chunk_rows_kernel(const ScoresParams p
   for (int g = 0; g < 4; ++g) w[g] = (f32x4p_t){};
   if (hi > lo) {
     K keys;
-    keys.load(p, b, h, key0, s.len);
+    keys.load(p, K::entries(p, b, key0, s.len), h, key0);
     const uint32_t linked = keys.linked;
     u32x4p_t a[4][NCH];
     f32x4p_t f[4][K::NG];
@@ -610,8 +692,9 @@ static int launch_scores(const ScoresParams &p, const ScoresPlan &pl, hipStream_
     return check_launch("attention_scores");
   }
   if (pl.few) {
-    // Tiles of a workgroup: as many as leave each compute unit eight workgroups (four are resident), at most eight.
-    const int64_t each = std::min<int64_t>(8, std::max<int64_t>(1, (int64_t)pl.kts * p.Hk * p.B / (8 * compute_units())));
+    // Tiles of a workgroup: as many as leave each compute unit sixteen workgroups (four are resident), at most
+    // eight (32 sequences of up to 8192 tokens: four per unit 37.6 us, eight 35.1, sixteen 33.5, 32 36.9).
+    const int64_t each = std::min<int64_t>(8, std::max<int64_t>(1, (int64_t)pl.kts * p.Hk * p.B / (16 * compute_units())));
     const dim3 grid((unsigned)((pl.kts + each - 1) / each * p.Hk), p.B);
     hipLaunchKernelGGL((few_rows_kernel<FMT, D>), grid, dim3(256), 0, s, p, (int32_t)each);
     if ((rc = check_launch("attention_scores(rows)")) != MEMOPT_OK) return rc;
