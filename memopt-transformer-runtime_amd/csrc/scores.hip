@@ -42,6 +42,8 @@ struct ScoresParams {
   float2 *ml;    // few rows: [B][Hk][kts][4][max_rows]; chunks: [Hk][kts][T G]
   float *probs;  // few rows: [B][Hk][max_rows][kts * kTileKeys]
   float *lse;    // chunks: [Hk][T G]
+  int32_t parts;  // chunks: workgroups that share a key tile's rows
+  float *sums;    // chunks, parts > 1: [parts][B][Hk][kts * kTileKeys]
 };
 
 static constexpr int kTileKeys = 256;  // keys of a workgroup: 64 per wave
@@ -456,7 +458,8 @@ __global__ __launch_bounds__(256, 2) void chunk_rows_kernel(const ScoresParams p
   constexpr int NCH = K::NCH, TR = 32, RB = 2 * D, CPR = RB / 16, RPC = 1024 / RB, NC = TR / RPC / 4;
   __shared__ __attribute__((aligned(16))) uint8_t lds_q[2][TR * RB];
   __shared__ float2 s_ml[2][4][TR];
-  const int32_t h = (int32_t)(blockIdx.x % p.Hk), kt = (int32_t)(blockIdx.x / p.Hk), b = blockIdx.y;
+  const int32_t h = (int32_t)(blockIdx.x % p.Hk), tp = (int32_t)(blockIdx.x / p.Hk), kt = tp / p.parts, part = tp % p.parts;
+  const int32_t b = blockIdx.y;
   const int lane = threadIdx.x & 63, n = lane & 15, kq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const ScoredSeq s = scored_seq(p, b);
@@ -466,7 +469,10 @@ __global__ __launch_bounds__(256, 2) void chunk_rows_kernel(const ScoresParams p
   f32x4p_t w[4];
 #pragma unroll
   for (int g = 0; g < 4; ++g) w[g] = (f32x4p_t){};
-  if (hi > lo) {
+  // This workgroup's part of the tiles of TR rows from the first that sees a key to the last.
+  const int32_t ta = lo * p.G / TR, tn = (hi * p.G + TR - 1) / TR - ta;
+  const int32_t t0 = ta + (int32_t)((int64_t)tn * part / p.parts), t1 = ta + (int32_t)((int64_t)tn * (part + 1) / p.parts);
+  if (hi > lo && t1 > t0) {
     K keys;
     keys.load(p, K::entries(p, b, key0, s.len), h, key0);
     const uint32_t linked = keys.linked;
@@ -474,8 +480,6 @@ __global__ __launch_bounds__(256, 2) void chunk_rows_kernel(const ScoresParams p
     f32x4p_t f[4][K::NG];
 #pragma unroll
     for (int g = 0; g < 4; ++g) keys.operands(g, a[g], f[g]);
-    // Tiles of TR rows from the first that sees a key to the last.
-    const int32_t t0 = lo * p.G / TR, t1 = (hi * p.G + TR - 1) / TR;
     const int64_t row_base = (int64_t)s.start * p.G;
     auto q_swz = [](int row) { return CPR == 16 ? row & 15 : (row >> 1) & 7; };
     // Rows past the last are copies of it: their weights are zeros.
@@ -599,7 +603,8 @@ __global__ __launch_bounds__(256, 2) void chunk_rows_kernel(const ScoresParams p
         v += half_mirror(v);
         v += dpp_f32<0x140>(v);
         const int32_t j = key0 + 16 * g + 4 * kq + r;
-        if (n == 0 && j < p.L) p.out[unit * p.L + j] = (p.scores ? p.scores[unit * p.L + j] : 0.0f) + v;
+        if (n == 0 && p.parts > 1) p.sums[((int64_t)part * p.B * p.Hk + unit) * ((int64_t)p.kts * kTileKeys) + j] = v;
+        else if (n == 0 && j < p.L) p.out[unit * p.L + j] = (p.scores ? p.scores[unit * p.L + j] : 0.0f) + v;
       }
   }
 }
@@ -628,11 +633,25 @@ __global__ __launch_bounds__(256) void lse_kernel(const ScoresParams p) {
   p.lse[(int64_t)h * p.T * p.G + (int64_t)s.start * p.G + row] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
+// out = scores + the parts' sums, in their order.
+__global__ __launch_bounds__(256) void add_parts_kernel(const ScoresParams p) {
+  const int32_t h = (int32_t)(blockIdx.x % p.Hk), j = (int32_t)(blockIdx.x / p.Hk) * kTileKeys + (int32_t)threadIdx.x;
+  if (j >= p.L) return;
+  const int64_t unit = (int64_t)blockIdx.y * p.Hk + h, row = (int64_t)p.kts * kTileKeys;
+  const float *src = p.sums + unit * row + j;
+  float v = p.scores ? p.scores[unit * p.L + j] : 0.0f;
+  float w = 0.0f;
+  if (j < row)
+    for (int i = 0; i < p.parts; ++i) w += src[(int64_t)i * p.B * p.Hk * row];
+  p.out[unit * p.L + j] = v + w;
+}
+
 struct ScoresPlan {
   bool few;
-  int32_t max_rows, kts;
-  int64_t second, total;  // offset of probs or lse behind ml
+  int32_t max_rows, kts, parts;
+  int64_t second, third, total;  // offsets of probs or lse behind ml, and of the parts' sums
 };
+static constexpr int kMaxParts = 8;
 static int64_t scored_keys(const memopt_scores_desc &d) {
   return std::min<int64_t>((int64_t)d.max_blocks_per_seq * d.block_size, std::max(0, d.max_seq_len));
 }
@@ -644,8 +663,14 @@ static ScoresPlan scores_plan(const memopt_scores_desc &d) {
   pl.kts = (int32_t)((scored_keys(d) + kTileKeys - 1) / kTileKeys);
   const int64_t ml = 8 * (int64_t)pl.kts * d.num_kv_heads * (pl.few ? 4 * d.batch * rows : d.tokens * G);
   pl.second = (ml + 255) / 256 * 256;
-  pl.total = pl.second + (pl.few ? 4 * (int64_t)d.batch * d.num_kv_heads * rows * pl.kts * kTileKeys
-                                 : 4 * (int64_t)d.num_kv_heads * d.tokens * G);
+  const int64_t units = (int64_t)d.batch * d.num_kv_heads;
+  pl.third = pl.second + (pl.few ? 4 * units * rows * pl.kts * kTileKeys : (4 * d.num_kv_heads * d.tokens * G + 255) / 256 * 256);
+  // Workgroups that share a key tile's rows: as many as make sixteen for each compute unit, with 256 rows or more each
+  // (four prompts' last 512 tokens, 2.25 tiles of keys per unit, two resident: each whole 306 us, four for each unit
+  // 267, eight 244, sixteen 243, 32 247).
+  pl.parts = (int32_t)std::min<int64_t>({kMaxParts, std::max<int64_t>(1, rows / 256),
+                                         16 * compute_units() / std::max<int64_t>(1, pl.kts * units) + 1});
+  pl.total = pl.third + (pl.few || pl.parts == 1 ? 0 : 4 * pl.parts * units * pl.kts * kTileKeys);
   if (rows == 0 || pl.kts == 0) pl.total = 0;
   return pl;
 }
@@ -684,7 +709,7 @@ static int validate_scores(const memopt_scores_desc &d) {
 template <int FMT, int D>
 static int launch_scores(const ScoresParams &p, const ScoresPlan &pl, hipStream_t s) {
   const unsigned tiles = (unsigned)((std::max<int64_t>(p.max_keys, p.L) + kTileKeys - 1) / kTileKeys);
-  const dim3 over_keys((unsigned)pl.kts * p.Hk, p.B), over_scores(tiles * p.Hk, p.B);
+  const dim3 over_keys((unsigned)pl.kts * pl.parts * p.Hk, p.B), over_scores(tiles * p.Hk, p.B);
   const dim3 finish((tiles + kFinishTiles - 1) / kFinishTiles * p.Hk, p.B);
   int rc;
   if (pl.total == 0) {
@@ -705,8 +730,10 @@ static int launch_scores(const ScoresParams &p, const ScoresPlan &pl, hipStream_
   if ((rc = check_launch("attention_scores(maxima)")) != MEMOPT_OK) return rc;
   hipLaunchKernelGGL(lse_kernel, dim3((unsigned)((p.max_rows + 255) / 256 * p.Hk), p.B), dim3(256), 0, s, p);
   if ((rc = check_launch("attention_scores(lse)")) != MEMOPT_OK) return rc;
-  hipLaunchKernelGGL((chunk_rows_kernel<FMT, D, true>), over_scores, dim3(256), 0, s, p);
-  return check_launch("attention_scores(sums)");
+  hipLaunchKernelGGL((chunk_rows_kernel<FMT, D, true>), pl.parts > 1 ? over_keys : over_scores, dim3(256), 0, s, p);
+  if ((rc = check_launch("attention_scores(sums)")) != MEMOPT_OK || pl.parts == 1) return rc;
+  hipLaunchKernelGGL(add_parts_kernel, over_scores, dim3(256), 0, s, p);
+  return check_launch("attention_scores(parts)");
 }
 
 }  // namespace memopt
@@ -768,6 +795,8 @@ extern "C" int memopt_attention_scores(const memopt_scores_desc *desc, void *str
   p.qk_scale_log2 = 1.4426950408889634f / sqrtf((float)d.head_dim);
   p.ml = (float2 *)d.workspace;
   (pl.few ? p.probs : p.lse) = (float *)((uint8_t *)d.workspace + pl.second);
+  p.parts = pl.few ? 1 : pl.parts;
+  p.sums = (float *)((uint8_t *)d.workspace + pl.third);
   hipStream_t s = (hipStream_t)stream;
   if (d.kv_format == MEMOPT_KV_INT4)
     return d.head_dim == 128 ? launch_scores<MEMOPT_KV_INT4, 128>(p, pl, s) : launch_scores<MEMOPT_KV_INT4, 64>(p, pl, s);
