@@ -666,7 +666,7 @@ static ScoresPlan scores_plan(const memopt_scores_desc &d) {
   const int64_t units = (int64_t)d.batch * d.num_kv_heads;
   pl.third = pl.second + (pl.few ? 4 * units * rows * pl.kts * kTileKeys : (4 * d.num_kv_heads * d.tokens * G + 255) / 256 * 256);
   // Workgroups that share a key tile's rows: as many as make sixteen for each compute unit, with 256 rows or more each
-  // (four prompts' last 512 tokens, 2.25 tiles of keys per unit, two resident: each whole 306 us, four for each unit
+  // (four prompts' last 512 tokens, 2.25 key tiles with keys for each unit: whole 306 us, four workgroups for each unit
   // 267, eight 244, sixteen 243, 32 247).
   pl.parts = (int32_t)std::min<int64_t>({kMaxParts, std::max<int64_t>(1, rows / 256),
                                          16 * compute_units() / std::max<int64_t>(1, pl.kts * units) + 1});
