@@ -15,8 +15,14 @@
 // gets, by prefix sums over the requests as in batch.hip. The third copies (a
 // wave per 16 new tokens and head) and writes tables and ring.
 //
-// Bound by the copies where requests are long, else by the chain of launches
-// and of the selection's passes.
+// Measured (medians): one request of 1024 tokens, two heads: 2.5 + 10 + 4 us,
+// a chain of launches, reads and barriers (the call's host side takes 16). 16
+// requests of up to 8192 tokens, 8 heads, 2048 kept, INT4: 4 + 17.4 + 20.4 us:
+// the copies' 71 MB at 3.5 TB/s; the selection's fixed 9 us (four passes of
+// five barriers, the plan) and 1 us per 1024 tokens, one workgroup a row. One
+// request of 16384 tokens, 8192 kept, fp16: 2.5 + 24 + 13.5 us: eight rows
+// leave 248 compute units idle in the selection, and a selection shared by
+// several workgroups would need a launch per pass.
 #include <algorithm>
 
 #include "page_format.hpp"

@@ -10,6 +10,13 @@
 // workgroup takes 128 rows of a head (32 per wave, the columns of both
 // products) against tiles of 64 keys in LDS. The shared part is copied into
 // every head's tile, so that no head's keys are ever joined in memory.
+//
+// Measured (128 + 64; medians): three prompts of up to 9000 tokens, 32 heads,
+// fp16: 0.90-0.92 ms, 0.95 PFLOP/s, 0.77 of the library's rate on a large product: a
+// wave's softmax stands between its two products, and the other workgroup on
+// the compute unit fills in. 24 prompts of 20 to 2500 tokens, 16 heads, bf16:
+// 136-146 us, 0.65 PFLOP/s of what the mask leaves: masked tiles are whole
+// products, and 2016 workgroups are four rounds of the GPU.
 #include <algorithm>
 #include <cmath>
 

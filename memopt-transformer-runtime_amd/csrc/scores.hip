@@ -449,6 +449,10 @@ __global__ __launch_bounds__(256) void finish_kernel(const ScoresParams p) {
 // ---------------------------------------------------------------------------
 // Chunks: rows stream past the keys twice
 // ---------------------------------------------------------------------------
+// Bound by vector instructions: the softmax's exponentials and sums, 0.75 of
+// the units' time in the first pass and 0.60 in the second, the matrix units
+// 0.31. The last 512 tokens of four prompts of up to 6000 tokens, 32 heads
+// over 8, 128, fp16: 120 + 6 + 123 + 5 us (passes, rows' sums, parts).
 
 // SUM = false: every row's maximum and sum over the tile's keys; true: every
 // key's weights, with the rows' lse known, and the result.

@@ -24,7 +24,12 @@ reference behaviour):
     reference documents but never implements (src/csrc/kv_cache.cu:1033-1036);
   * ``prompt_attention``, ``packed_attention`` / ``PreparedPackedAttention``
     and ``advance_batch`` — packed batches with grouped heads: whole prompts
-    straight from q, k and v, the paged cache, and a step's index tensors.
+    straight from q, k and v, the paged cache, and a step's index tensors;
+  * ``attention_scores`` and ``compact_cache`` — attention weights added up
+    per cached token, and the tokens of least weight taken out of the cache;
+  * ``write_latent``, ``latent_attention`` and ``latent_prompt_attention`` —
+    a cache of one latent row per token for all heads, attention over it, and
+    over whole prompts from the expanded keys and values.
 
 The library is loaded at import; a missing or unloadable library raises
 ``ImportError`` naming the path (there is no CPU fallback).
