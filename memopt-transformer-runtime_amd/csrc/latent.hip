@@ -140,10 +140,12 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
   // Workgroup i runs on XCD i % 8: an XCD takes neighbouring runs, whose tiles of rows read the same keys.
   const uint32_t w = (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
   const uint32_t total = latent_place<ROWS, false>(p, 0, true).total, run = latent_run(total, p.wgs);
-  uint32_t at = w * run;
-  const uint32_t end = min(total, at + run), begin = at;
-  if (at >= end) return;
-  const LatentPlace place = latent_place<ROWS, false>(p, at, false);
+  const uint32_t begin = w * run;
+  uint32_t end = min(total, begin + run);  // of the steps that are left
+  if (begin >= end) return;
+  // A run's tiles of rows from the last back: its first keys, then others' last ones. Workgroups that begin together
+  // so meet the same keys together, in their XCD's L2.
+  const LatentPlace place = latent_place<ROWS, false>(p, end - 1, false);
   if (place.b < 0) return;
   int32_t b = __builtin_amdgcn_readfirstlane(place.b);
   uint32_t before = __builtin_amdgcn_readfirstlane(place.before);
@@ -169,15 +171,16 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
   u32x4p_t *const s_weights = reinterpret_cast<u32x4p_t *>(lds + L::weights) + rw * 256 + lane;  // [half][register quad][lane]
   float *const s_tops = reinterpret_cast<float *>(lds + L::tops) + rw * 64;                      // [half][row]
 
-  while (at < end) {
+  while (begin < end) {
     LatentSeq s = uniform_seq<ROWS>(p, b);
-    while (at >= before + (uint32_t)s.tiles * (uint32_t)s.steps) {
-      before += (uint32_t)s.tiles * (uint32_t)s.steps;
-      if (++b >= p.B) return;  // (sequences that overlap: their steps may pass 32 bits)
+    while (before >= end) {
+      if (--b < 0) return;  // (sequences that overlap: their steps may pass 32 bits)
       s = uniform_seq<ROWS>(p, b);
+      before -= (uint32_t)s.tiles * (uint32_t)s.steps;
     }
-    const int32_t rt = (int32_t)((at - before) / (uint32_t)s.steps), first_step = (int32_t)((at - before) % (uint32_t)s.steps);
-    const int32_t last_step = (int32_t)min((uint32_t)s.steps, (uint32_t)first_step + (end - at));
+    const int32_t rt = (int32_t)((end - 1 - before) / (uint32_t)s.steps);
+    const uint32_t unit = before + (uint32_t)rt * (uint32_t)s.steps, at = max(begin, unit);
+    const int32_t first_step = (int32_t)(at - unit), last_step = (int32_t)(end - unit);
     const int32_t q0 = ROWS * rt, qw0 = q0 + 32 * rw;
     auto pos_of = [&](int32_t row) { return s.pos0 + p.by_h(min(row, s.rows - 1)); };
 
@@ -220,13 +223,15 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
       e2 = entry_at(key + 32);
       e3 = entry_at(key + 48);
     };
-    uint32_t links0 = 0, links1 = 0;  // bit g: chunk g of the tile in buffer 0 or 1 is there
-    auto load = [&](int32_t it, int buf) __attribute__((always_inline)) {
-      auto there = [&](int32_t e) { return e >= 0 && e < p.nb; };
-      const uint32_t ok = __builtin_amdgcn_readfirstlane((there(e0) ? 1u : 0u) | (there(e1) ? 2u : 0u) | (there(e2) ? 4u : 0u) |
-                                                         (there(e3) ? 8u : 0u));
-      links0 = buf ? links0 : ok;
-      links1 = buf ? ok : links1;
+    // A tile's copies are set up together (no tile: of nothing) and issued one by one between the matrix instructions of
+    // the tile before: all at once they keep a wave waiting for the queue (3400 of a tile's 9000 clocks).
+    uint32_t link_next = 0;  // bit g: chunk g is there
+    __amdgpu_buffer_rsrc_t next[CPW];
+    constexpr int N = NCOPY * CPW;
+    auto prepare = [&](int32_t it, bool some) __attribute__((always_inline)) {
+      auto there = [&](int32_t e) { return some && e >= 0 && e < p.nb; };
+      link_next = __builtin_amdgcn_readfirstlane((there(e0) ? 1u : 0u) | (there(e1) ? 2u : 0u) | (there(e2) ? 4u : 0u) |
+                                                 (there(e3) ? 8u : 0u));
 #pragma unroll
       for (int i = 0; i < CPW; ++i) {
         const int g = wave * CPW + i;
@@ -235,10 +240,15 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
         const int32_t key = tile_base(it) + 16 * g, chunk = key >> 4;
         const uint8_t *base = reinterpret_cast<const uint8_t *>(p.c) + (there(e) ? (int64_t)e : 0) * p.page_bytes +
                               (int64_t)(chunk - p.by_chunks(chunk) * (int32_t)p.by_chunks.d) * CB;
-        const auto rsrc = uniform_rsrc(base, there(e) ? max(0, min(16, s.len - key)) * RB : 0);
-        const uint32_t to = lds_u32(lds) + buf * BUF + g * CB;
+        next[i] = uniform_rsrc(base, there(e) ? max(0, min(16, s.len - key)) * RB : 0);
+      }
+    };
+    auto issue = [&](int buf, int from, int to) __attribute__((always_inline)) {  // copies [from, to) of N
 #pragma unroll
-        for (int c = 0; c < NCOPY; ++c) lds_dma<0, 1>(rsrc, to + c * 1024, off + c % NOFF, c < NOFF ? 0 : 8 * RB);
+      for (int k = 0; k < N; ++k) {
+        if (k < from || k >= to) continue;
+        const int i = k / NCOPY, c = k % NCOPY;
+        lds_dma<0, 1>(next[i], lds_u32(lds) + buf * BUF + (wave * CPW + i) * CB + c * 1024, off + c % NOFF, c < NOFF ? 0 : 8 * RB);
       }
     };
 
@@ -263,7 +273,8 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
     auto lane_row = [&]() { return qw0 + n; };
 
     // Scores of this wave's 32 keys, in log2 units, hidden ones -inf.
-    auto scores = [&](const uint8_t *kt, int32_t k0, uint32_t link, f32x16_t &x) __attribute__((always_inline)) {
+    constexpr int NSC = (2 * N + 2) / 3;  // copies beside the first product; the others go beside the second
+    auto scores = [&](const uint8_t *kt, int32_t k0, uint32_t link, int next_buf, f32x16_t &x) __attribute__((always_inline)) {
       x = (f32x16_t){};
       // Operands are read a group of products ahead: a wave has its SIMD to itself and nothing else hides an LDS read.
       constexpr int GR = 4, NG = (NCH + GR - 1) / GR;
@@ -280,6 +291,7 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
         __builtin_amdgcn_sched_barrier(0);
         if (g + 1 < NG) read(g + 1);
         __builtin_amdgcn_sched_barrier(0);
+        issue(next_buf, NSC * g / NG, NSC * (g + 1) / NG);
 #pragma unroll
         for (int i = 0; i < GR; ++i)
           if (g * GR + i < NCH) x = E::mfma(f[g & 1][i], qf[g * GR + i], x);
@@ -326,7 +338,9 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
       return u32x4p_t{a[0], a[1], b8[0], b8[1]};
     };
     // `first`: the values of the first 32 columns, read before the weights were there.
-    auto add_values = [&](const uint8_t *kt, const u32x4p_t (&pb)[4], const u32x4p_t (&first)[4]) __attribute__((always_inline)) {
+    auto add_values = [&](const uint8_t *kt, const u32x4p_t (&pb)[4], const u32x4p_t (&first)[4],
+                          int next_buf) __attribute__((always_inline)) {
+      constexpr int G = (3 * NDB + 3) / 4;  // (none in the last quarter: they have to arrive)
       u32x4p_t v[2][4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[0][i] = first[i];
@@ -337,6 +351,7 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
         for (int i = 0; i < 4; ++i)
           if (db + 1 < NDB) v[(db + 1) & 1][i] = values(kt, db + 1, i);
         __builtin_amdgcn_sched_barrier(0);
+        if (db < G) issue(next_buf, NSC + (N - NSC) * db / G, NSC + (N - NSC) * (db + 1) / G);
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[db] = E::mfma(v[db & 1][i], pb[i], o[db]);
       }
@@ -365,33 +380,34 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
       return changed;
     };
 
+    uint32_t link = 0;
     if (i0 < i1) {
       look_up(i0);
-      load(i0, 0);
-      if (i0 + 1 < i1) {
-        look_up(i0 + 1);
-        load(i0 + 1, 1);
-        if (i0 + 2 < i1) look_up(i0 + 2);
-      }
+      prepare(i0, true);
+      issue(0, 0, N);
+      if (i0 + 1 < i1) look_up(i0 + 1);
     }
     for (int32_t it = i0; it < i1; ++it) {
       const int buf = (it - i0) & 1;
-      // This wave's copies of the tile have arrived (the next tile's may be on their way); the barrier says so for all.
-      if (it + 1 < i1) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(NCOPY * CPW) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      link = link_next;
+      prepare(it + 1, it + 1 < i1);
+      if (it + 2 < i1) look_up(it + 2);
+      // This wave's copies of the tile have arrived; the barrier says so for all.
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
       const int32_t tb = tile_base(it), k0 = tb + 32 * kw;
       const uint8_t *const kt = lds + buf * BUF;
-      const uint32_t link = buf ? links1 : links0;
       const bool some = seen(tb) || seen(tb + 32);  // (the same for both waves of the pair)
       f32x16_t x;
       if (some) {
-        scores(kt + 2 * kw * CB, k0, (link >> (2 * kw)) & 3, x);
+        scores(kt + 2 * kw * CB, k0, (link >> (2 * kw)) & 3, buf ^ 1, x);
         float t = x[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) t = fmaxf(t, x[r]);
         t = both_halves_max(t);
         if (hl == 0) s_tops[32 * kw + n] = t;
+      } else {
+        issue(buf ^ 1, 0, N);
       }
       __syncthreads();
       u32x4p_t pb[4], first[4];
@@ -415,14 +431,11 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
       if (some) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) pb[i] = s_weights[64 * i];
-        add_values(kt, pb, first);
+        add_values(kt, pb, first, buf ^ 1);
       }
       __syncthreads();
-      if (it + 2 < i1) {
-        load(it + 2, buf);
-        if (it + 3 < i1) look_up(it + 3);
-      }
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the last tile's copies of nothing)
 
     // The pair's row sums.
     float l = xor32_sum(lsum);
@@ -484,7 +497,7 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
         }
       }
     }
-    at += (uint32_t)(last_step - first_step);
+    end = at;
     __syncthreads();  // the space is free for the next tiles
   }
 }
