@@ -29,13 +29,16 @@ DEVICE = [
     # Packed FP32 instructions are kept out of the generated code.
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
+# Matrix instructions with their sums in vector registers: the compiler's choice for a wave of more than 256 registers,
+# accumulation registers, has the sums of latent_kernel copied there and back for every tile.
+FILE_FLAGS = {"latent.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _compile(src: str, verbose: bool) -> str:
     obj = os.path.join(BUILD, os.path.splitext(src)[0] + ".o")
     path = os.path.join(CSRC, src)
     if src.endswith(".hip"):
-        cmd = [HIPCC, *COMMON, *DEVICE, "-x", "hip", "-c", path, "-o", obj]
+        cmd = [HIPCC, *COMMON, *DEVICE, *FILE_FLAGS.get(src, []), "-x", "hip", "-c", path, "-o", obj]
     else:
         cmd = [HIPCC, *COMMON, "-c", path, "-o", obj]
     if verbose:

@@ -14,15 +14,15 @@
 // in its lane, and the weights leave one product in the layout in which the
 // other takes them. One pass with a running maximum and sum.
 //
-// Measured (rank 512 + 64, bf16; medians): 32 single tokens of 16 heads over
-// up to 8192 tokens: 57-62 us, 3.5 TB/s of rows read once (the copies without
-// the arithmetic: 41-48); 6 more for the merge. 16 single tokens of 128 heads:
-// 66 us and 8: each 64-row tile reads all keys, so a head count of 128 reads
-// them twice. Three chunks of 256 tokens, 16 heads, beside nine single tokens:
-// 218 us, 0.6 PFLOP/s and 13 for the merge: of a tile's 9000 clocks 3400 wait
-// for its 72 KiB (4.7 TB/s out of L2 and the last-level cache), the first
-// product takes 2250 (1152 of matrix instructions), the softmax 800, the
-// second product 1550 (1024).
+// Measured (rank 512 + 64, bf16): 32 single tokens of 16 heads over up to 8192
+// tokens: 60 us with the merge's 6, 3.9 TB/s of rows read once (the copies
+// without the arithmetic: 41-48). 16 single tokens of 128 heads: 65 us with
+// the merge's 8: each 64-row tile reads all keys, so a head count of 128 reads them
+// twice. Three chunks of 256 tokens, 16 heads, beside nine single tokens: 197
+// us with the merge's 13, 0.71 PFLOP/s: of a tile's 6400 clocks the first
+// product takes 2900 (1152 of matrix instructions, the rest the issue of
+// copies and operand reads), the softmax 500, the second product 1850 (1024),
+// barriers and the next tile's pages 1100.
 #include <algorithm>
 #include <cmath>
 
@@ -192,6 +192,14 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
     const int32_t i0 = min(first_step, n_tiles), i1 = min(last_step, n_tiles);
     auto tile_base = [&](int32_t it) { return (it < sink_tiles ? it : t_first + (it - sink_tiles)) * kLatentKeys; };
 
+    // Block-table entries of the 64 chunks of 16 tiles from `it` on, one a lane; -1 behind the context or the last tile.
+    // (Scalar loads would be waited for with every LDS read: 2000 clocks and more a tile.)
+    auto entries_of = [&](int32_t it) __attribute__((always_inline)) {
+      const int32_t t = it + (lane >> 2), key = tile_base(t) + 16 * (lane & 3);
+      return t < i1 && key < s.len ? p.bt[(int64_t)b * p.M + p.by_chunks(key >> 4)] : -1;
+    };
+    int32_t entries = entries_of(i0), entries_next = -1;
+
     u32x4p_t qf[NCH];
 #pragma unroll
     for (int c = 0; c < NCH; ++c) qf[c] = (u32x4p_t){};
@@ -206,41 +214,31 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
     __builtin_amdgcn_sched_barrier(0);
 
-    // Most of them live in accumulation registers beside the sums (a hint, without which the loop spills at 512 + 64).
-    constexpr int kInAcc = (240 - 16 * NDB) / 4;
+    // They live in accumulation registers, where matrix instructions take operands from; the sums, which a new maximum
+    // scales, in the others. (A hint: without it some of them move about in the loop, 213 against 197 us for chunks.)
 #pragma unroll
-    for (int c = 0; c < (NCH < kInAcc ? NCH : kInAcc); ++c) asm volatile("" : "+a"(qf[c]));
+    for (int c = 0; c < NCH; ++c) asm volatile("" : "+a"(qf[c]));
 
-    // Pages of a tile's four chunks, and its copies. An entry that is no page, and rows behind the context, read as zeros.
-    int32_t e0 = -1, e1 = -1, e2 = -1, e3 = -1;  // (no array: chosen from by wave, it would go through scratch memory)
-    auto entry_at = [&](int32_t key) __attribute__((always_inline)) {
-      return key < s.len ? uniform_entry(p.bt + (int64_t)b * p.M + p.by_chunks(key >> 4)) : -1;
-    };
-    auto look_up = [&](int32_t it) __attribute__((always_inline)) {
-      const int32_t key = tile_base(it);
-      e0 = entry_at(key);
-      e1 = entry_at(key + 16);
-      e2 = entry_at(key + 32);
-      e3 = entry_at(key + 48);
-    };
-    // A tile's copies are set up together (no tile: of nothing) and issued one by one between the matrix instructions of
+    // A tile's copies are set up together (of nothing, where no tile follows) and issued one by one between the matrix instructions of
     // the tile before: all at once they keep a wave waiting for the queue (3400 of a tile's 9000 clocks).
-    uint32_t link_next = 0;  // bit g: chunk g is there
+    // An entry that is no page, and rows behind the context, read as zeros.
+    auto pages_of = [&](int32_t e) { return __ballot(e >= 0 && e < p.nb); };
+    uint64_t linked = pages_of(entries);  // of the lanes
+    uint32_t link_next = 0;               // bit g: chunk g is there
     __amdgpu_buffer_rsrc_t next[CPW];
     constexpr int N = NCOPY * CPW;
-    auto prepare = [&](int32_t it, bool some) __attribute__((always_inline)) {
-      auto there = [&](int32_t e) { return some && e >= 0 && e < p.nb; };
-      link_next = __builtin_amdgcn_readfirstlane((there(e0) ? 1u : 0u) | (there(e1) ? 2u : 0u) | (there(e2) ? 4u : 0u) |
-                                                 (there(e3) ? 8u : 0u));
+    auto prepare = [&](int32_t it) __attribute__((always_inline)) {
+      const int32_t first = 4 * ((it - i0) & 15);
+      link_next = (uint32_t)(linked >> first) & 15;
 #pragma unroll
       for (int i = 0; i < CPW; ++i) {
         const int g = wave * CPW + i;
-        const int32_t e = CPW == 2 ? (wave == 0 ? (i ? e1 : e0) : (i ? e3 : e2))
-                                   : wave == 0 ? e0 : wave == 1 ? e1 : wave == 2 ? e2 : e3;
+        const int32_t e = __builtin_amdgcn_readlane(entries, first + g);
+        const bool there = (link_next >> g) & 1;
         const int32_t key = tile_base(it) + 16 * g, chunk = key >> 4;
-        const uint8_t *base = reinterpret_cast<const uint8_t *>(p.c) + (there(e) ? (int64_t)e : 0) * p.page_bytes +
+        const uint8_t *base = reinterpret_cast<const uint8_t *>(p.c) + (there ? (int64_t)e : 0) * p.page_bytes +
                               (int64_t)(chunk - p.by_chunks(chunk) * (int32_t)p.by_chunks.d) * CB;
-        next[i] = uniform_rsrc(base, there(e) ? max(0, min(16, s.len - key)) * RB : 0);
+        next[i] = uniform_rsrc(base, there ? max(0, min(16, s.len - key)) * RB : 0);
       }
     };
     auto issue = [&](int buf, int from, int to) __attribute__((always_inline)) {  // copies [from, to) of N
@@ -380,21 +378,22 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
       return changed;
     };
 
-    uint32_t link = 0;
     if (i0 < i1) {
-      look_up(i0);
-      prepare(i0, true);
+      prepare(i0);
       issue(0, 0, N);
-      if (i0 + 1 < i1) look_up(i0 + 1);
     }
     for (int32_t it = i0; it < i1; ++it) {
       const int buf = (it - i0) & 1;
-      link = link_next;
-      prepare(it + 1, it + 1 < i1);
-      if (it + 2 < i1) look_up(it + 2);
       // This wave's copies of the tile have arrived; the barrier says so for all.
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
+      const uint32_t link = link_next;
+      if (((it + 1 - i0) & 15) == 0) {
+        entries = entries_next;
+        linked = pages_of(entries);
+      }
+      prepare(it + 1);
+      if (((it + 2 - i0) & 15) == 0) entries_next = entries_of(it + 2);
       const int32_t tb = tile_base(it), k0 = tb + 32 * kw;
       const uint8_t *const kt = lds + buf * BUF;
       const bool some = seen(tb) || seen(tb + 32);  // (the same for both waves of the pair)
