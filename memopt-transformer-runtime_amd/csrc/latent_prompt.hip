@@ -14,7 +14,8 @@
 // Measured (128 + 64; medians): three prompts of up to 9000 tokens, 32 heads,
 // fp16: 0.90-0.92 ms, 0.95 PFLOP/s, 0.77 of the library's rate on a large product: a
 // wave's softmax stands between its two products, and the other workgroup on
-// the compute unit fills in. 24 prompts of 20 to 2500 tokens, 16 heads, bf16:
+// the compute unit fills in (of 256 registers 234 are taken: neither a second
+// set of scores nor copies dealt over the products fit without spills). 24 prompts of 20 to 2500 tokens, 16 heads, bf16:
 // 136-146 us, 0.65 PFLOP/s of what the mask leaves: masked tiles are whole
 // products, and 2016 workgroups are four rounds of the GPU.
 #include <algorithm>
