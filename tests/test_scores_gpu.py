@@ -223,6 +223,22 @@ def test_strided_and_far_query_rows(fmt, qn):
     assert torch.equal(run(c), want)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("Hq,Hk,D", [(8, 2, 64), (16, 1, 128), (3, 3, 128)])
+@pytest.mark.parametrize("window,sinks", [(-1, 0), (90, 20)])
+def test_rows_shared_by_workgroups(fmt, Hq, Hk, D, window, sinks):
+    """256 rows and more per key head and few key tiles: parts of the rows are added up; adding in place, and to more
+    and fewer positions than there are tiles for."""
+    c = Case(fmt, [700, 513, 90, 0], [700, 300, 1, 0], Hq, Hk, D, seed=Hq + D)
+    check_scores(c, run(c, window, sinks), window, sinks)
+    for L in (100, 1500):
+        before = torch.rand(4, Hk, L, device=dev())
+        out = run(c, window, sinks, scores=before)
+        check_scores(c, out, window, sinks, before=before)
+        assert torch.equal(run(c, window, sinks, scores=before), out)
+        assert torch.equal(run(c, window, sinks, scores=before, out=before), out)
+
+
 def test_keys_past_4_gib():
     """Pages behind 4 GiB of the pool."""
     nb = 2 ** 32 // (16 * 1 * 128 * 2) + 40
