@@ -187,7 +187,7 @@ struct Keys {
                                                  16 * D + 4 * (lane % (8 * NG)));
   }
   __device__ __forceinline__ void take(uint32_t *s_scales) {
-    asm volatile("" : "+v"(scales) : : "memory");  // (the scales were read last: once they are here, the copies are)
+    asm volatile("s_waitcnt vmcnt(0)" : "+v"(scales) : : "memory");
     s_scales[threadIdx.x & 63] = scales;
   }
   __device__ __forceinline__ void page(int g, const uint8_t *from, const uint32_t *s_scales) {
