@@ -528,8 +528,12 @@ __global__ __launch_bounds__(256) void latent_merge_kernel(const LatentParams p)
   top = wave_max(top);
   for (uint32_t i0 = 0; i0 < parts; i0 += 64) {
     const float2 ml = i0 + lane < parts ? p.ws_ml[slot_of(w0 + i0 + lane)] : float2{-INFINITY, 0.0f};
-    const float f = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - top);
-    l += f == 0.0f ? 0.0f : ml.y * f;
+    // A part of a maximum of -inf saw nothing, and its row may hold anything. Every other part counts, also where its
+    // factor is 0: 0 times the NaN or inf that it may hold is the row's NaN.
+    const bool seen = ml.x != -INFINITY;
+    const uint64_t parts_seen = __ballot(seen);
+    const float f = seen ? fast_exp2(ml.x - top) : 0.0f;
+    l += seen ? ml.y * f : 0.0f;
     const uint32_t n = min(64u, parts - i0);
     for (uint32_t i = 0; i < n; i += 4) {
       f32x4p_t v[4][PER / 4 ? PER / 4 : 1];
@@ -538,7 +542,7 @@ __global__ __launch_bounds__(256) void latent_merge_kernel(const LatentParams p)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint32_t j = min(i + k, n - 1);
-        g[k] = i + k < n ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), j)) : 0.0f;
+        g[k] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), j));
         const float *src = p.ws_o + slot_of(w0 + i0 + j) * R + lane * PER;
         if constexpr (PER == 2) v2[k] = *reinterpret_cast<const f32x2m_t *>(src);
         else
@@ -547,7 +551,7 @@ __global__ __launch_bounds__(256) void latent_merge_kernel(const LatentParams p)
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (g[k] == 0.0f) continue;  // (nothing seen there: its row may hold anything)
+        if (i + k >= n || !((parts_seen >> (i + k)) & 1)) continue;
 #pragma unroll
         for (int x = 0; x < PER; ++x) {
           if constexpr (PER == 2) acc[x] = fmaf(v2[k][x], g[k], acc[x]);

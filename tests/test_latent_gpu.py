@@ -207,6 +207,43 @@ def test_infinite_values_of_weight():
     c.check(c.run())
 
 
+def _steep(dtype, ctx, qn, low, high=40.0):
+    """A case whose scores the first rotary element alone sets: keys lie at the level `low`, from the last 64 on at
+    `high`, which is (high - low) 64 scale log2(e), more than 250 powers of two at the defaults, above them."""
+    c = Case(dtype, [ctx], [qn], 16, seed=4)
+    c.q.zero_()
+    c.q[:, :, 512] = 64
+    pages = c.bt[0, :-(-ctx // 16)].long()
+    x = c.c[pages].flatten(0, 1)
+    x[:, 512:] = 0
+    x[:, 512] = low
+    x[64:128, 512] = high
+    c.c[pages] = x.view(-1, 16, 576)
+    return c
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("qn", [1, 70])
+@pytest.mark.parametrize("token", [10, 1500, 1800])
+def test_a_nan_far_below_the_other_parts(dtype, qn, token):
+    """A row that sees a NaN is NaN, however small the weights of the part of its keys in which the NaN lies."""
+    c = _steep(dtype, 2000, qn, -40.0)
+    good = c.run()
+    c.check(good)
+    c.c[c.tables[0, token // 16], token % 16, 3] = float("nan")
+    assert bool(c.run().isnan().all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_part_of_nothing_but_nan(dtype):
+    """Beside parts whose scores lie far above or below 0."""
+    for low, high in ((0.0, 40.0), (-40.0, 40.0), (-80.0, -40.0)):
+        c = _steep(dtype, 2000, 1, low, high)
+        c.check(c.run())
+        c.c[c.bt[0, 4 * 9:4 * 10].long()] = float("nan")  # (keys 576 to 639)
+        assert bool(c.run().isnan().all()), (low, high)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_queries_that_are_not_finite_stay_in_their_rows(dtype):
     c = Case(dtype, [100, 80], [5, 1], 16, 256, 64, seed=5)
