@@ -245,6 +245,30 @@ def test_a_part_of_nothing_but_nan(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ctx,qn", [(200, 100), (2000, 70), (2000, 1)])
+@pytest.mark.parametrize("back", [2, 40, 64])
+def test_infinite_elements_of_weight_zero(dtype, ctx, qn, back):
+    """A key with an inf where the queries are negative has the score -inf: rows that see it have 0 inf = NaN or inf in
+    that column, and everywhere else what the other keys give; the other rows nothing of it."""
+    c = Case(dtype, [ctx], [qn], 4, 128, 32, seed=5)
+    c.q[:, :, 7] = -1
+    token = ctx - back
+    c.c[c.tables[0, token // 16], token % 16, 7] = float("inf")
+    out = c.run().cpu()
+    pages = torch.from_numpy(c.tables[0, :-(-ctx // 16)]).long()
+    x, live = c.c.cpu()[pages].flatten(0, 1)[:ctx], torch.ones(ctx, dtype=torch.bool)
+    live[token] = False
+    pos = ctx - qn + np.arange(qn)
+    o, w, e = latent(c.q, x, pos, 128, c.scale, -1, 0, live)
+    tol = latent_tolerance(o, w, e, ctx, 160, dtype)
+    see = torch.from_numpy(pos >= token)
+    other = torch.arange(128) != 7
+    check(out[~see], o[~see], tol[~see], "rows before it")
+    check(out[see][:, :, other], o[see][:, :, other], tol[see][:, :, other], "its rows' other columns")
+    assert not bool(out[see][:, :, 7].isfinite().any())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_queries_that_are_not_finite_stay_in_their_rows(dtype):
     c = Case(dtype, [100, 80], [5, 1], 16, 256, 64, seed=5)
     want = c.run()
