@@ -447,7 +447,8 @@ int memopt_attention_scores(const memopt_scores_desc *desc, void *stream);
 #define MEMOPT_COMPACT_NO_PAGES 3  /* the free pages, or the ring's room for the old ones, did not  */
                                    /* last (sums over all that ask so far, as in advance_batch);    */
                                    /* pages that this call gives back serve the next one            */
-#define MEMOPT_COMPACT_SHARED   4  /* one of its pages is listed twice in this call's tables        */
+#define MEMOPT_COMPACT_SHARED   4  /* one of its pages is listed twice in this call's contexts,     */
+                                   /* those of invalid requests that fit their tables among them    */
 typedef struct memopt_compact_desc {
   const float *scores;               /* [num_requests, num_kv_heads, scores_len] */
   float *scores_out;                 /* the same                               */

@@ -54,14 +54,20 @@ static constexpr int32_t kMaxCompacted = 4096;
 
 __device__ __forceinline__ bool page_ok(const CompactParams &p, int32_t page) { return page >= 0 && page < p.nb; }
 
+// Pages of request b's context: 0 where no table can hold that many tokens.
+__device__ __forceinline__ int32_t pages_held(const CompactParams &p, int32_t c) {
+  return c < 0 || (int64_t)c > (int64_t)p.M * p.bs ? 0 : (c + p.bs - 1) / p.bs;
+}
+
 // What a request holds and asks for. A page that two entries list would go
-// back to the ring twice: each entry leaves its number at the page, and who
-// finds another's there (the second launch) tells both requests.
+// back to the ring twice, or while the other request still has it: each entry
+// leaves its number at the page, and who finds another's there (the second
+// launch) tells both requests. Refused requests take part: they keep their pages.
 __global__ __launch_bounds__(256) void compact_count_kernel(const CompactParams p) {
   __shared__ int32_t s_part[2][4];
   const int32_t b = blockIdx.x, c = p.ctx[b], keep = p.keep[b];
   const bool bad = c < 0 || (int64_t)c > (int64_t)p.M * p.bs || c > p.L || keep > p.K;
-  const int32_t have = bad ? 0 : (c + p.bs - 1) / p.bs;
+  const int32_t have = pages_held(p, c);
   int32_t live = 0, back = 0;
   for (int32_t i = threadIdx.x; i < have; i += 256) {
     const int32_t page = p.bt[(int64_t)b * p.M + i];
@@ -314,15 +320,20 @@ __global__ __launch_bounds__(1024) void compact_select_kernel(const CompactParam
   const int32_t h = blockIdx.x, b = blockIdx.y;
   const int64_t unit = (int64_t)b * p.Hk + h;
   const int32_t n = p.stay[b], c = p.ctx[b];
-  if (h == 0 && p.state[b] != MEMOPT_COMPACT_INVALID) {
-    const int32_t have = (c + p.bs - 1) / p.bs;
+  if (h == 0) {
+    const int32_t have = pages_held(p, c);
+    // (a refused request stays one: whether it is does not change in this launch)
+    auto shares = [&](int32_t who) {
+      if (__hip_atomic_load(&p.state[who], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != MEMOPT_COMPACT_INVALID)
+        __hip_atomic_store(&p.state[who], MEMOPT_COMPACT_SHARED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    };
     for (int32_t i = threadIdx.x; i < have; i += 1024) {
       const int32_t page = p.bt[(int64_t)b * p.M + i];
       if (!page_ok(p, page)) continue;
       const int32_t id = p.marks[page];
       if (id == b * p.M + i) continue;
-      __hip_atomic_store(&p.state[b], MEMOPT_COMPACT_SHARED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __hip_atomic_store(&p.state[id / p.M], MEMOPT_COMPACT_SHARED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      shares(b);
+      shares(id / p.M);
     }
   }
   const float *src = p.scores + unit * p.L;

@@ -1352,7 +1352,8 @@ def compact_cache(scores: torch.Tensor, key_cache: torch.Tensor, value_cache: to
     the inputs but for ``free_span``; ``status``: 0 compacted, 1 invalid
     (length past table or scores, ``keep`` past ``max_keep``), 2 left (it may
     keep all it has; a negative ``keep``: always), 3 pages did not last (what
-    a call gives back serves the next one), 4 a page is listed twice.
+    a call gives back serves the next one), 4 a page is listed twice (by an
+    invalid request, whose status stays 1, too).
     ``max_keep`` is needed without ``out``. Calls on one batch must not
     overlap.
     """

@@ -181,6 +181,36 @@ def test_pages_listed_twice(fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("why", ["keep", "scores"])
+@pytest.mark.parametrize("refused", [0, 1])
+def test_pages_shared_with_a_refused_request(fmt, why, refused):
+    """A request whose `keep` or length the call does not take still holds its pages: who shares one keeps it too."""
+    ctx = [100, 100, 90]
+    ctx[refused] = 200
+    c = Cache(fmt, ctx, 2, 64, seed=6, L=250 if why == "keep" else 150)
+    other = 1 - refused
+    lost = int(c.tables[other, 3])
+    c.tables[other, 3] = c.tables[refused, 7]
+    keep = [40, 40, 40]
+    if why == "keep":
+        keep[refused] = 60
+    t = [torch.from_numpy(x.copy()).to(dev()) for x in c.pools]
+    ring, span, tables = (torch.from_numpy(x.copy()).to(dev()) for x in (c.ring, c.span, c.tables))
+    scores, lens = torch.from_numpy(c.scores).to(dev()), torch.from_numpy(c.ctx).to(dev())
+    r = memopt_C.compact_cache(scores, t[0], t[-1], tables, lens, torch.tensor(keep, dtype=torch.int32, device=dev()), ring,
+                               span, num_recent_tokens=4, max_keep=50)
+    status = [4, 4, 0]
+    status[refused] = 1
+    assert r.status.tolist() == status
+    assert torch.equal(r.block_tables[:2], tables[:2]) and torch.equal(r.scores[:2], scores[:2])
+    assert r.context_lens.tolist() == ctx[:2] + [40] and bool((r.kept[:2] == -1).all())
+    head, count = r.free_span.tolist()
+    free = ring[(head + torch.arange(count, device=dev())) % c.nb].tolist()
+    held = set(r.block_tables[r.block_tables >= 0].tolist())
+    assert not held & set(free) and held | set(free) | {lost} == set(range(c.nb)) and len(set(free)) == count
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_invalid_requests(fmt):
     c = Cache(fmt, [100, 200, 90, 60], 2, 64, seed=6, M=14, L=150)
     c.ctx[2] = -4
