@@ -400,7 +400,10 @@ __global__ __launch_bounds__(256) void compact_move_kernel(const CompactParams p
   if (!page_ok(p, page)) return;  // (the ring held something that is no page)
   // Old page and place of new token i0 + t, in lane t.
   const int32_t mine = i0 + (lane & 15) < n ? p.kept[unit * p.K + i0 + (lane & 15)] : -1;
-  const int32_t old = mine < 0 || mine >= p.ctx[b] ? -1 : p.bt[(int64_t)b * p.M + mine / p.bs], at = mine < 0 ? 0 : mine % p.bs;
+  // (Only tokens of linked pages are kept; where scores change under the call a place of the list may be left as it was,
+  // and hold any number.)
+  const int32_t entry = mine < 0 || mine >= p.ctx[b] ? -1 : p.bt[(int64_t)b * p.M + mine / p.bs];
+  const int32_t old = page_ok(p, entry) ? entry : -1, at = mine < 0 ? 0 : mine % p.bs;
   if constexpr (FMT == MEMOPT_KV_INT4) {
     // Lane 8 q + c owns tokens q and q + 8 of the new block, as in page_format.hpp.
     constexpr int BPL = D / 8, G = D / 64, W = BPL / 4;  // bytes and words of a lane's K (and of its V)
