@@ -216,8 +216,10 @@ class PackedBatch(_Requests):
         old ones are still taken: where they do not last for all, requests
         are compacted one after another, and those for which even that does
         not suffice stay. Tokens that come later stand behind the ``keep``
-        (``token_positions`` says where they stand in the text). (Waits for
-        the device.)
+        (``token_positions`` says where they stand in the text). It belongs
+        behind a step's ``attend`` and ``accumulate``, before the next
+        ``advance``: the step's slots lie in pages that it gives back. (Waits
+        for the device.)
         """
         if self.weights is None:
             raise RuntimeError("PackedBatch: made without track_weights")
@@ -249,12 +251,16 @@ class PackedBatch(_Requests):
         return done
 
     def token_positions(self) -> torch.Tensor:
-        """Where the step's rows stand in their texts (int32 ``[num_rows]``): ``state.positions``, which count cached
-        tokens, plus the tokens that compaction took out before; -1 behind the last row."""
+        """Where the rows of the last ``advance`` stand in their texts (int32 ``[num_rows]``): ``state.positions``, which
+        count cached tokens, plus the tokens that compaction had taken out by then; -1 behind the last row, and for rows
+        of requests released since."""
         rows = torch.arange(self.num_rows, dtype=torch.int32, device=self.tables.device)
-        owner = torch.searchsorted(self.state.cu_seqlens, rows, right=True) - 1
-        at = self.state.positions + self.removed[owner.clamp(0, self.removed.shape[0] - 1)]
-        return torch.where(self.state.positions >= 0, at, -1)
+        owner = (torch.searchsorted(self.state.cu_seqlens, rows, right=True) - 1).clamp(0, self.removed.shape[0] - 1)
+        # A text ends with its request's last row. Its length, what is cached and what was removed, is the same before and
+        # after a compaction; `positions` beside `removed` are not.
+        text = (self.state.context_lens + self.removed)[owner]
+        at = text - (self.state.cu_seqlens[1:][owner] - rows)
+        return torch.where((self.state.positions >= 0) & (at >= 0), at, -1)
 
     def release(self, requests: Sequence[int]) -> None:
         super().release(requests)

@@ -123,6 +123,27 @@ def test_compaction_where_pages_are_short():
     assert full.compact([0], 0) == [0] and full.state.free_span.tolist()[1] == 10
 
 
+def test_positions_outlast_a_compaction():
+    """Where the step's rows stand in their texts does not change when tokens before them leave, and neither do the next
+    rows' places; rows of a released request stand nowhere."""
+    batch = R().PackedBatch(60, 1, 64, 3, 320, 200, track_weights=True)
+    q, k = (torch.randn(200, h, 64, device=dev()).half() for h in (2, 1))
+    for new in ([101, 20, 7], [1, 3, 0], [2, 1, 4]):
+        batch.advance(ints(*new))
+        batch.attend(q, k, k, max_new=max(new))
+        batch.accumulate(q, max_new=max(new))
+        rows = sum(new)
+        want = batch.token_positions()
+        assert bool((want[rows:] == -1).all()) and bool((want[:rows] >= 0).all())
+        first = [int(n) for n in batch.state.context_lens + batch.removed]
+        assert want[:rows].tolist() == [p for f, m in zip(first, new) for p in range(f - m, f)]
+        batch.compact([0, 2], 5 if new[0] == 1 else 64, num_recent_tokens=1)
+        assert torch.equal(batch.token_positions(), want)
+    assert batch.removed.tolist()[0] > 0
+    batch.release([0])
+    assert batch.token_positions()[:rows].tolist() == [-1] * new[0] + want[new[0]:rows].tolist()
+
+
 def test_refusals():
     batch = R().PackedBatch(10, 1, 64, 2, 160, 20)
     q = torch.zeros(20, 1, 64, dtype=torch.float16, device=dev())
