@@ -213,9 +213,9 @@ class PackedBatch(_Requests):
 
         Old pages go back to the ring. A request that has no more than
         ``keep`` stays as it is. The fresh pages come from the ring while the
-        old ones are still taken: where they do not last for all, requests
-        are compacted one after another, and those for which even that does
-        not suffice stay. Tokens that come later stand behind the ``keep``
+        old ones are still taken: where they do not last for all, the others
+        are compacted into what the first gave back, and where they do not
+        last for one, all stay. Tokens that come later stand behind the ``keep``
         (``token_positions`` says where they stand in the text). It belongs
         behind a step's ``attend`` and ``accumulate``, before the next
         ``advance``: the step's slots lie in pages that it gives back. (Waits
@@ -245,9 +245,9 @@ class PackedBatch(_Requests):
             status = r.status.tolist()
             served = [b for b, s in zip(todo, status) if s == 0]
             done += served
-            short = [b for b, s in zip(todo, status) if s == 3]
-            # (sums over all that ask decide: behind one that is refused, another may still fit by itself)
-            todo = short if served else short[1:]
+            # Those refused are tried again over what the others gave back. All ask for as many fresh pages, and the ring
+            # takes any old ones: where the first finds no room, none does.
+            todo = [b for b, s in zip(todo, status) if s == 3] if served else []
         return done
 
     def token_positions(self) -> torch.Tensor:

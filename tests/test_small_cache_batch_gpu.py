@@ -144,6 +144,20 @@ def test_positions_outlast_a_compaction():
     assert batch.token_positions()[:rows].tolist() == [-1] * new[0] + want[new[0]:rows].tolist()
 
 
+def test_a_full_pool_is_tried_once(monkeypatch):
+    """All requests of a call keep the same number of tokens: where the first finds no room, none does."""
+    batch = R().PackedBatch(40, 1, 64, 4, 160, 640, track_weights=True)
+    batch.advance(ints(160, 160, 160, 160))
+    assert batch.state.status.tolist() == [0] * 4
+    calls, one = [], memopt_C.compact_cache
+    monkeypatch.setattr("memopt_C.compact_cache", lambda *a, **kw: calls.append(1) or one(*a, **kw))
+    assert batch.compact([2, 0, 1, 3], 20) == [] and len(calls) == 1
+    assert batch.state.context_lens.tolist() == [160] * 4 and batch.state.free_span.tolist()[1] == 0
+    batch.release([1])
+    calls.clear()
+    assert batch.compact([2, 0, 3], 20) == [2, 0, 3] and len(calls) == 1
+
+
 def test_refusals():
     batch = R().PackedBatch(10, 1, 64, 2, 160, 20)
     q = torch.zeros(20, 1, 64, dtype=torch.float16, device=dev())
