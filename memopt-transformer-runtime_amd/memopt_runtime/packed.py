@@ -263,8 +263,9 @@ class PackedBatch(_Requests):
         return torch.where((self.state.positions >= 0) & (at >= 0), at, -1)
 
     def release(self, requests: Sequence[int]) -> None:
+        requests = self._known(requests)  # (once: an iterator is spent then)
         super().release(requests)
-        rows = torch.tensor(self._known(requests), dtype=torch.int64, device=self.tables.device)
+        rows = torch.tensor(requests, dtype=torch.int64, device=self.tables.device)
         self.removed[rows] = 0
         if self.weights is not None:
             self.weights[rows] = 0.0

@@ -158,6 +158,22 @@ def test_a_full_pool_is_tried_once(monkeypatch):
     assert batch.compact([2, 0, 3], 20) == [2, 0, 3] and len(calls) == 1
 
 
+@pytest.mark.parametrize("name", ["list", "generator", "empty"])
+def test_released_requests_start_without_weights(name):
+    batch = R().PackedBatch(40, 1, 64, 2, 160, 100, track_weights=True)
+    x = torch.randn(100, 1, 64, device=dev()).half()
+    batch.advance(ints(60, 40))
+    batch.attend(x, x, x, max_new=60)
+    batch.accumulate(x, max_new=60)
+    batch.compact([0], 30)
+    before = batch.weights.clone()
+    batch.release({"list": [0, 0], "generator": (r for r in [0]), "empty": []}[name])
+    gone = name != "empty"
+    assert batch.removed.tolist() == [0 if gone else 30, 0]
+    assert bool((batch.weights[0] == 0).all()) == gone and torch.equal(batch.weights[1], before[1])
+    assert batch.state.context_lens.tolist() == [0 if gone else 30, 40]
+
+
 def test_refusals():
     batch = R().PackedBatch(10, 1, 64, 2, 160, 20)
     q = torch.zeros(20, 1, 64, dtype=torch.float16, device=dev())
