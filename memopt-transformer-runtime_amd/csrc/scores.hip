@@ -665,16 +665,16 @@ static ScoresPlan scores_plan(const memopt_scores_desc &d) {
   pl.few = rows <= kFewRows;
   pl.max_rows = (int32_t)rows;
   pl.kts = (int32_t)((scored_keys(d) + kTileKeys - 1) / kTileKeys);
-  const int64_t ml = 8 * (int64_t)pl.kts * d.num_kv_heads * (pl.few ? 4 * d.batch * rows : d.tokens * G);
+  const int64_t ml = 8LL * pl.kts * d.num_kv_heads * (pl.few ? 4LL * d.batch * rows : d.tokens * G);
   pl.second = (ml + 255) / 256 * 256;
   const int64_t units = (int64_t)d.batch * d.num_kv_heads;
-  pl.third = pl.second + (pl.few ? 4 * units * rows * pl.kts * kTileKeys : (4 * d.num_kv_heads * d.tokens * G + 255) / 256 * 256);
+  pl.third = pl.second + (pl.few ? 4LL * units * rows * pl.kts * kTileKeys : (4LL * d.num_kv_heads * d.tokens * G + 255) / 256 * 256);
   // Workgroups that share a key tile's rows: as many as make sixteen for each compute unit, with 256 rows or more each
   // (four prompts' last 512 tokens, 2.25 key tiles with keys for each unit: whole 306 us, four workgroups for each unit
   // 267, eight 244, sixteen 243, 32 247).
   pl.parts = (int32_t)std::min<int64_t>({kMaxParts, std::max<int64_t>(1, rows / 256),
                                          16 * compute_units() / std::max<int64_t>(1, pl.kts * units) + 1});
-  pl.total = pl.third + (pl.few || pl.parts == 1 ? 0 : 4 * pl.parts * units * pl.kts * kTileKeys);
+  pl.total = pl.third + (pl.few || pl.parts == 1 ? 0 : 4LL * pl.parts * units * pl.kts * kTileKeys);
   if (rows == 0 || pl.kts == 0) pl.total = 0;
   return pl;
 }

@@ -84,6 +84,15 @@ def test_scores_empty_calls_and_workspace(C):
     assert call(C, "scores", SCORES, size=True, tokens=4096) == call(C, "scores", SCORES, size=True)
 
 
+@pytest.mark.parametrize("tokens,heads", [(2 ** 26, 8), (2 ** 25, 32), (2 ** 24 + 3, 64), (2 ** 27, 4)])
+def test_scores_workspace_of_very_many_rows(C, tokens, heads):
+    """Sizes that pass 32 bits on the way: a maximum and a sum per row and key tile, and the rows' lse."""
+    need = call(C, "scores", SCORES, size=True, tokens=tokens, num_heads=heads, num_kv_heads=heads, batch=1, max_query_len=tokens,
+                q_ts=64 * heads, max_seq_len=256)
+    sums = 4 * 8 * heads * 256  # (of eight workgroups that may share a tile's rows)
+    assert need == 8 * heads * tokens + (4 * heads * tokens + 255) // 256 * 256 + sums
+
+
 @pytest.mark.parametrize("text,code,change", [
     ("negative", INVALID, dict(num_requests=-1)), ("negative", INVALID, dict(scores_len=-1)), ("negative", INVALID, dict(max_keep=-1)),
     ("empty cache", INVALID, dict(num_kv_heads=0)), ("empty cache", INVALID, dict(num_kv_blocks=0)),
