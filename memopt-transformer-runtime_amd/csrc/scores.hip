@@ -653,9 +653,15 @@ __global__ __launch_bounds__(256) void add_parts_kernel(const ScoresParams p) {
 struct ScoresPlan {
   bool few;
   int32_t max_rows, kts, parts;
+  int32_t group;  // few rows: sequences whose weights the workspace holds at once
   int64_t second, third, total;  // offsets of probs or lse behind ml, and of the parts' sums
 };
 static constexpr int kMaxParts = 8;
+// Weights of few rows are kept for as many sequences at a time as this holds, one at least: all of a batch would be
+// requests x rows x the longest context allowed, whatever the contexts are. (64 requests of 65536 tokens and 8 x 16
+// rows, 2.1 GB: all at once 1406 us, by 1 GiB 1423, 512 MiB 1470, 256 MiB 1495; the same with 20 live at 3000
+// tokens, where each group of sequences costs its launches: 100, 107, 147, 158.)
+static constexpr int64_t kMaxProbs = 1LL << 30;
 static int64_t scored_keys(const memopt_scores_desc &d) {
   return std::min<int64_t>((int64_t)d.max_blocks_per_seq * d.block_size, std::max(0, d.max_seq_len));
 }
@@ -665,10 +671,12 @@ static ScoresPlan scores_plan(const memopt_scores_desc &d) {
   pl.few = rows <= kFewRows;
   pl.max_rows = (int32_t)rows;
   pl.kts = (int32_t)((scored_keys(d) + kTileKeys - 1) / kTileKeys);
-  const int64_t ml = 8LL * pl.kts * d.num_kv_heads * (pl.few ? 4LL * d.batch * rows : d.tokens * G);
+  const int64_t probs = 4LL * d.num_kv_heads * rows * pl.kts * kTileKeys;  // of one sequence
+  pl.group = (int32_t)std::min<int64_t>(d.batch, std::max<int64_t>(1, kMaxProbs / std::max<int64_t>(1, probs)));
+  const int64_t ml = 8LL * pl.kts * d.num_kv_heads * (pl.few ? 4LL * pl.group * rows : d.tokens * G);
   pl.second = (ml + 255) / 256 * 256;
   const int64_t units = (int64_t)d.batch * d.num_kv_heads;
-  pl.third = pl.second + (pl.few ? 4LL * units * rows * pl.kts * kTileKeys : (4LL * d.num_kv_heads * d.tokens * G + 255) / 256 * 256);
+  pl.third = pl.second + (pl.few ? pl.group * probs : (4LL * d.num_kv_heads * d.tokens * G + 255) / 256 * 256);
   // Workgroups that share a key tile's rows: as many as make sixteen for each compute unit, with 256 rows or more each
   // (four prompts' last 512 tokens, 2.25 key tiles with keys for each unit: whole 306 us, four workgroups for each unit
   // 267, eight 244, sixteen 243, 32 247).
@@ -723,12 +731,22 @@ static int launch_scores(const ScoresParams &p, const ScoresPlan &pl, hipStream_
   if (pl.few) {
     // Tiles of a workgroup: as many as leave each compute unit sixteen workgroups (four are resident), at most
     // eight (32 sequences of up to 8192 tokens: four per unit 37.6 us, eight 35.1, sixteen 33.5, 32 36.9).
-    const int64_t each = std::min<int64_t>(8, std::max<int64_t>(1, (int64_t)pl.kts * p.Hk * p.B / (16 * compute_units())));
-    const dim3 grid((unsigned)((pl.kts + each - 1) / each * p.Hk), p.B);
-    hipLaunchKernelGGL((few_rows_kernel<FMT, D>), grid, dim3(256), 0, s, p, (int32_t)each);
-    if ((rc = check_launch("attention_scores(rows)")) != MEMOPT_OK) return rc;
-    hipLaunchKernelGGL(finish_kernel, finish, dim3(256), 0, s, p);
-    return check_launch("attention_scores(finish)");
+    const int64_t each = std::min<int64_t>(8, std::max<int64_t>(1, (int64_t)pl.kts * p.Hk * pl.group / (16 * compute_units())));
+    ScoresParams g = p;
+    for (int32_t b = 0; b < p.B; b += pl.group) {
+      const unsigned n = (unsigned)std::min(pl.group, p.B - b);
+      g.bt = p.bt + (int64_t)b * p.M;
+      g.ctx = p.ctx + b;
+      g.starts = p.starts + b;
+      g.scores = p.scores ? p.scores + (int64_t)b * p.Hk * p.L : nullptr;
+      g.out = p.out + (int64_t)b * p.Hk * p.L;
+      const dim3 grid((unsigned)((pl.kts + each - 1) / each * p.Hk), n);
+      hipLaunchKernelGGL((few_rows_kernel<FMT, D>), grid, dim3(256), 0, s, g, (int32_t)each);
+      if ((rc = check_launch("attention_scores(rows)")) != MEMOPT_OK) return rc;
+      hipLaunchKernelGGL(finish_kernel, dim3(finish.x, n), dim3(256), 0, s, g);
+      if ((rc = check_launch("attention_scores(finish)")) != MEMOPT_OK) return rc;
+    }
+    return MEMOPT_OK;
   }
   hipLaunchKernelGGL((chunk_rows_kernel<FMT, D, false>), over_keys, dim3(256), 0, s, p);
   if ((rc = check_launch("attention_scores(maxima)")) != MEMOPT_OK) return rc;

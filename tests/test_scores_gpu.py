@@ -251,6 +251,33 @@ def test_keys_past_4_gib():
     assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("qn", [0, 1])
+def test_batches_whose_weights_are_kept_in_groups(qn):
+    """600 requests of up to 4096 tokens and 16 rows per key head: 1.26 GB of weights, more than are kept at a time."""
+    rng = np.random.default_rng(3)
+    ctx = rng.integers(1, 60, 600).tolist()
+    ctx[3], ctx[500], ctx[599] = 1000, 700, 4096
+    n = [qn or int(b % 3 == 0) for b in range(600)]
+    c = Case("int4", ctx, n, 128, 8, 64, seed=5)
+    assert c.M == 256
+    before = torch.rand(600, 8, 4096, device=dev())
+    out = run(c, scores=before)
+    q, kc, _, bt, cl, cu = c.args()[:6]
+    for a, z in ((0, 200), (200, 600)):  # (each half's weights are kept at once)
+        first, last = sum(n[:a]), sum(n[:z])
+        part = memopt_C.attention_scores(q[first:last], kc, bt[a:z], cl[a:z], cu[a:z + 1] - first, 1, 4096, scores=before[a:z])
+        assert torch.equal(out[a:z], part)
+    for b in (3, 499, 500, 599):
+        first, m = sum(n[:b]), ctx[b]
+        k = c.kval[torch.from_numpy(c.tables[b, :-(-m // 16)]).long()].flatten(0, 1)[:m]
+        w, tol = weight_sums(c.q[first:first + n[b]], k, m - n[b] + np.arange(n[b]), -1, 0)
+        want = before[b].double().cpu()
+        want[:, :m] += w
+        tol = torch.nn.functional.pad(tol, (0, 4096 - m))
+        check(out[b], want, tol + 2.0 ** -23 * want.abs(), f"sequence {b}")
+    assert run(c, scores=before, out=before) is before and torch.equal(before, out)
+
+
 def test_pool_view_is_the_page_buffer():
     memopt_C.init_pool(20, 16, 2, 64, kv_format="int4")
     x = torch.randn(100, 2, 64, device=dev()).half()

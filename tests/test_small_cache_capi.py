@@ -93,6 +93,20 @@ def test_scores_workspace_of_very_many_rows(C, tokens, heads):
     assert need == 8 * heads * tokens + (4 * heads * tokens + 255) // 256 * 256 + sums
 
 
+@pytest.mark.parametrize("batch,heads,kv_heads,tokens", [(64, 128, 8, 65536), (1024, 32, 8, 8192), (4096, 32, 8, 8192),
+                                                         (8, 16, 1, 2 ** 20), (4096, 16, 2, 4096)])
+def test_scores_workspace_of_large_batches_of_single_tokens(C, batch, heads, kv_heads, tokens):
+    """The rows' weights are kept for some sequences at a time: 1 GiB of them, and their maxima and sums, at most."""
+    size = dict(tokens=batch, batch=batch, num_heads=heads, num_kv_heads=kv_heads, q_ts=64 * heads, max_blocks=tokens // 16,
+                max_seq_len=tokens, scores_len=tokens)
+    all_of_them = 4 * batch * heads * tokens
+    need = call(C, "scores", SCORES, size=True, **size)
+    assert min(all_of_them, 2 ** 30) * 0.9 < need < 2 ** 30 * (1 + 8 * 4 / (4 * 256)) + 512
+    one = 4 * heads * 2 ** 28  # (a sequence past the limit by itself: its own weights)
+    size.update(max_blocks=2 ** 24, max_seq_len=2 ** 28, scores_len=2 ** 28, batch=1)
+    assert one <= call(C, "scores", SCORES, size=True, **size) < one * 1.04
+
+
 @pytest.mark.parametrize("text,code,change", [
     ("negative", INVALID, dict(num_requests=-1)), ("negative", INVALID, dict(scores_len=-1)), ("negative", INVALID, dict(max_keep=-1)),
     ("empty cache", INVALID, dict(num_kv_heads=0)), ("empty cache", INVALID, dict(num_kv_blocks=0)),
