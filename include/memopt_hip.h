@@ -439,8 +439,8 @@ int memopt_attention_scores(const memopt_scores_desc *desc, void *stream);
  * context_lens_out, scores_out (the kept tokens' scores, 0 behind), kept (old
  * positions, -1 behind), status; a request that is not compacted keeps its
  * tables, length and scores, and its `kept` are -1. free_span_out may be
- * free_span; the other results must not overlap the inputs. At most 4096
- * requests; calls on one batch must not overlap. Status: */
+ * free_span; apart from that results must not overlap the inputs, nor each
+ * other. At most 4096 requests; calls on one batch must not overlap. Status: */
 #define MEMOPT_COMPACT_DONE     0
 #define MEMOPT_COMPACT_INVALID  1  /* a length past the table or scores_len, or keep past max_keep  */
 #define MEMOPT_COMPACT_LEFT     2  /* it may keep all it has (negative keep: always)                */

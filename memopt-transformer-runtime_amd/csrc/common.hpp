@@ -29,6 +29,16 @@ void clear_error();
 // Checks the launch that was just enqueued.
 int check_launch(const char *what);
 
+// Memory of a call's argument: whether two of them share a byte.
+struct Memory {
+  const void *at;
+  int64_t bytes;
+};
+inline bool overlap(const Memory &a, const Memory &b) {
+  const uintptr_t x = (uintptr_t)a.at, y = (uintptr_t)b.at;
+  return a.bytes > 0 && b.bytes > 0 && x < y + (uint64_t)b.bytes && y < x + (uint64_t)a.bytes;
+}
+
 // ---------------------------------------------------------------------------
 // Registered pool (host state; storage is owned by the caller)
 // ---------------------------------------------------------------------------

@@ -24,6 +24,7 @@
 // leave 248 compute units idle in the selection, and a selection shared by
 // several workgroups would need a launch per pass.
 #include <algorithm>
+#include <iterator>
 
 #include "page_format.hpp"
 #include "tiles.hpp"
@@ -465,6 +466,27 @@ static int64_t compact_workspace(const memopt_compact_desc &d) {
   return ((5 * (int64_t)d.num_requests + 4 + d.num_kv_blocks) * 4 + 255) / 256 * 256;
 }
 
+// Whether a result shares memory with an input or another result (free_span_out may be free_span itself).
+static bool compact_overlaps(const memopt_compact_desc &d) {
+  const int64_t N = d.num_requests, rows = N * d.num_kv_heads;
+  const int64_t cache = d.kv_format == MEMOPT_KV_INT4 ? d.num_kv_blocks * d.num_kv_heads * Int4Page(d.head_dim).block
+                                                      : d.num_kv_blocks * d.num_kv_heads * d.block_size * d.head_dim * 2;
+  const Memory out[] = {{d.scores_out, 4 * rows * d.scores_len}, {d.kept, 4 * rows * d.max_keep},
+                        {d.block_tables_out, 4 * N * d.max_blocks_per_seq}, {d.context_lens_out, 4 * N}, {d.status, 4 * N},
+                        {d.free_span_out, 8}};
+  const Memory in[] = {{d.scores, 4 * rows * d.scores_len}, {d.key_cache, cache},
+                       {d.value_cache, d.kv_format == MEMOPT_KV_INT4 ? 0 : cache}, {d.block_tables, 4 * N * d.max_blocks_per_seq},
+                       {d.context_lens, 4 * N}, {d.keep, 4 * N}, {d.free_pages, 4LL * d.num_free_pages},
+                       {d.free_span_out == d.free_span ? nullptr : d.free_span, d.free_span_out == d.free_span ? 0 : 8}};
+  for (size_t i = 0; i < std::size(out); ++i) {
+    for (const Memory &x : in)
+      if (overlap(out[i], x)) return true;
+    for (size_t k = 0; k < i; ++k)
+      if (overlap(out[i], out[k])) return true;
+  }
+  return false;
+}
+
 static int validate_compact(const memopt_compact_desc &d) {
   MEMOPT_REQUIRE(d.num_requests >= 0 && d.scores_len >= 0 && d.max_keep >= 0, MEMOPT_ERR_INVALID,
                  "compact_cache: negative size");
@@ -524,6 +546,8 @@ extern "C" int memopt_compact_cache(const memopt_compact_desc *desc, void *strea
   const int64_t need = d.num_requests == 0 ? 0 : compact_workspace(d);
   MEMOPT_REQUIRE(need == 0 || (d.workspace && d.workspace_bytes >= need), MEMOPT_ERR_INVALID,
                  "compact_cache: workspace needs " + std::to_string(need) + " bytes");
+  MEMOPT_REQUIRE(d.num_requests == 0 || !compact_overlaps(d), MEMOPT_ERR_INVALID,
+                 "compact_cache: results must not overlap the inputs, nor each other");
   CompactParams p = {};
   p.scores = d.scores;
   p.scores_out = d.scores_out;

@@ -1348,8 +1348,8 @@ def compact_cache(scores: torch.Tensor, key_cache: torch.Tensor, value_cache: to
 
     Caches: INT4 pages (the pool's code views, or a page buffer passed as
     both) or fp16 pools, changed in place (only in fresh pages). Results are
-    new tensors, or ``out``'s (``compact_cache_buffers``), which must not be
-    the inputs but for ``free_span``; ``status``: 0 compacted, 1 invalid
+    new tensors, or ``out``'s (``compact_cache_buffers``), which must not
+    overlap the inputs (but for ``free_span`` itself) nor each other; ``status``: 0 compacted, 1 invalid
     (length past table or scores, ``keep`` past ``max_keep``), 2 left (it may
     keep all it has; a negative ``keep``: always), 3 pages did not last (what
     a call gives back serves the next one), 4 a page is listed twice (by an

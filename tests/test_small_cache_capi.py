@@ -130,6 +130,25 @@ def test_compact_refusals(C, text, code, change):
     refused(C, call(C, "compact", COMPACT, **change), code, text)
 
 
+def test_compact_results_that_overlap(C):
+    """Results share no byte with an input, their last and first among them, nor with each other."""
+    need = call(C, "compact", COMPACT, size=True)
+    size = dict(scores=4 * 2 * 320 * 4, scores_out=4 * 2 * 320 * 4, kept=4 * 2 * 64 * 4, block_tables=4 * 20 * 4, context_lens=16,
+                keep=16, block_tables_out=4 * 20 * 4, context_lens_out=16, status=16, free_pages=400, free_span=8, free_span_out=8,
+                workspace=need)
+    at = {name: (i + 1) << 20 for i, name in enumerate(size)}
+    results = ("scores_out", "kept", "block_tables_out", "context_lens_out", "status", "free_span_out")
+    for fmt, caches in ((1, dict(key_cache=100 * 2 * 17 * 64)), (0, dict(key_cache=100 * 16 * 2 * 64 * 2, value_cache=100 * 16 * 2 * 64 * 2))):
+        place = {**COMPACT, **at, **{n: (100 + i) << 20 for i, n in enumerate(caches)}, "kv_format": fmt}
+        sizes = {**size, **caches}
+        for r in results:
+            for x in sizes:
+                if x == r or x == "workspace":
+                    continue
+                for where in (place[x] + sizes[x] - 4, place[x] - sizes[r] + 4):
+                    refused(C, call(C, "compact", {**place, r: where}), INVALID, "must not overlap")
+
+
 def test_compact_workspace(C):
     refused(C, C._c_compact(None, None), INVALID, "null")
     assert call(C, "compact", COMPACT, size=True, num_requests=0) == 0
