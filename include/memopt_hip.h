@@ -401,7 +401,7 @@ int memopt_advance_batch(const memopt_advance_desc *desc, void *stream);
  * are memopt_packed_attention's, and a row that sees nothing adds nothing. The
  * order of all sums is fixed. Tokens from max_seq_len on are not looked at;
  * weights of tokens from scores_len on are not written. `scores` may be null
- * (zeros) or `out` itself. Query rows: 31 token strides and a group's head
+ * (zeros) or `out` itself, else the two must not overlap. Query rows: 31 token strides and a group's head
  * strides together less than 2^29 elements. */
 typedef struct memopt_scores_desc {
   const void *query;                 /* fp16 [tokens, num_heads, head_dim]     */

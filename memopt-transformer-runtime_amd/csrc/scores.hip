@@ -781,6 +781,9 @@ extern "C" int memopt_attention_scores(const memopt_scores_desc *desc, void *str
                  MEMOPT_ERR_INVALID, "attention_scores: null pointer");
   MEMOPT_REQUIRE(pl.total == 0 || (d.workspace && d.workspace_bytes >= pl.total), MEMOPT_ERR_INVALID,
                  "attention_scores: workspace needs " + std::to_string(pl.total) + " bytes");
+  const int64_t sums = 4LL * d.batch * d.num_kv_heads * d.scores_len;
+  MEMOPT_REQUIRE(d.out == d.scores || !overlap({d.out, sums}, {d.scores, d.scores ? sums : 0}), MEMOPT_ERR_INVALID,
+                 "attention_scores: out must be scores, or not overlap it");
   ScoresParams p = {};
   p.q = (const uint16_t *)d.query;
   p.q_ts = d.q_token_stride;

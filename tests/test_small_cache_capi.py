@@ -84,6 +84,12 @@ def test_scores_empty_calls_and_workspace(C):
     assert call(C, "scores", SCORES, size=True, tokens=4096) == call(C, "scores", SCORES, size=True)
 
 
+def test_scores_that_overlap_out_in_part(C):
+    size = 4 * 8 * 2 * 320
+    for d in (4 - size, -256, 4, size - 4):
+        refused(C, call(C, "scores", SCORES, scores=2 ** 20 + d, out=2 ** 20), INVALID, "overlap")
+
+
 @pytest.mark.parametrize("tokens,heads", [(2 ** 26, 8), (2 ** 25, 32), (2 ** 24 + 3, 64), (2 ** 27, 4)])
 def test_scores_workspace_of_very_many_rows(C, tokens, heads):
     """Sizes that pass 32 bits on the way: a maximum and a sum per row and key tile, and the rows' lse."""
