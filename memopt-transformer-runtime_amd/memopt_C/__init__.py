@@ -605,9 +605,9 @@ def _int4_rows_layout(key_cache, key_scales, num_heads, head_dim):
     return bs, nb, kv, sc, 1 if key_scales.dtype == torch.float16 else 0
 
 
-def _int4_pages_base(key_cache, value_cache, num_heads, head_dim):
+def _int4_pages_base(key_cache, value_cache, num_heads, head_dim, fn="dynamic_sparse_attention"):
     """Base pointer and page count when the caches are the INT4 page buffer (or
-    its K/V code views from get_pool_tensors), else None."""
+    its K/V code views from get_pool_tensors), else None. fn: who refuses."""
     lay = int4_layout(head_dim)
     if _pool and _pool["fmt"] == KV_INT4 and _pool["d"] == head_dim and _pool["h"] == num_heads:
         base = _pool["pages"].data_ptr()
@@ -615,9 +615,10 @@ def _int4_pages_base(key_cache, value_cache, num_heads, head_dim):
                 value_cache.data_ptr() in (base, base + lay["vcodes"]):
             return base, _pool["nb"], _pool["pages"]
     if key_cache.dim() == 3 and key_cache.shape[1] == num_heads and key_cache.shape[2] == lay["block"]:
-        _require(key_cache.is_contiguous(), "INT4 page buffer must be contiguous")
-        _require(value_cache.data_ptr() == key_cache.data_ptr(),
-                 "dynamic_sparse_attention: pass the INT4 page buffer as both key_cache and value_cache")
+        if not key_cache.is_contiguous():
+            raise RuntimeError(f"{fn}: INT4 page buffer must be contiguous")
+        if value_cache.data_ptr() != key_cache.data_ptr():
+            raise RuntimeError(f"{fn}: pass the INT4 page buffer as both key_cache and value_cache")
         return key_cache.data_ptr(), key_cache.shape[0], key_cache
     return None
 
@@ -966,7 +967,7 @@ def _packed_desc(query, key_cache, value_cache, block_tables, context_lens, cu_s
         _require(key_cache.dim() == 3 and value_cache.dim() == 3 and key_cache.shape[1] > 0,
                  "packed_attention: INT4 caches are the pool's code views or its page buffer [pages, heads, bytes]")
         Hk = key_cache.shape[1]
-        pages = _int4_pages_base(key_cache, value_cache, Hk, D)
+        pages = _int4_pages_base(key_cache, value_cache, Hk, D, fn)
         _require(pages is not None, "packed_attention: not an INT4 page buffer of this head_dim")
         base_k, nb, buf = pages
         _require(buf.device == query.device, "packed_attention: key_cache on a different device")
@@ -1222,7 +1223,7 @@ def attention_scores(query: torch.Tensor, key_cache: torch.Tensor, block_tables:
         if not (key_cache.dim() == 3 and key_cache.shape[1] > 0):
             raise RuntimeError(f"{fn}: INT4 caches are the pool's key view or its page buffer [pages, heads, bytes]")
         Hk = key_cache.shape[1]
-        pages = _int4_pages_base(key_cache, key_cache, Hk, D)
+        pages = _int4_pages_base(key_cache, key_cache, Hk, D, fn)
         if pages is None:
             raise RuntimeError(f"{fn}: not an INT4 page buffer of this head_dim")
         pk, nb, _ = pages
@@ -1385,7 +1386,7 @@ def compact_cache(scores: torch.Tensor, key_cache: torch.Tensor, value_cache: to
             raise RuntimeError(f"{fn}: INT4 caches are the pool's code views or its page buffer [pages, {Hk}, bytes]")
         pages = None
         for D in (64, 128):
-            pages = pages or _int4_pages_base(key_cache, value_cache, Hk, D)
+            pages = pages or _int4_pages_base(key_cache, value_cache, Hk, D, fn)
             if pages is not None:
                 break
         if pages is None:

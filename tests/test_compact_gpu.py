@@ -343,3 +343,24 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="CUDA"):
         memopt_C.CompactStep(out.block_tables.cpu(), out.context_lens, out.free_span, out.scores, out.kept, out.status)
     call(out=memopt_C.CompactStep(out.block_tables, out.context_lens, span, out.scores, out.kept, out.status))
+
+
+def test_refusals_of_page_buffers_name_the_call():
+    """A page buffer that is not contiguous, or two of them, given to any operator over INT4 pages."""
+    c = Cache("int4", [90, 40], 2, 64)
+    wide = torch.zeros(c.nb, 2, 17 * 64 + 8, dtype=torch.uint8, device=dev())
+    pages = wide[:, :, :17 * 64].contiguous()
+    s, bt, cl, ring, span = (torch.from_numpy(x).to(dev()) for x in (c.scores, c.tables, c.ctx, c.ring, c.span))
+    keep, cu = (torch.tensor(x, dtype=torch.int32, device=dev()) for x in ([50, 20], [0, 1, 2]))
+    q = torch.zeros(2, 4, 64, dtype=torch.float16, device=dev())
+    calls = {"compact_cache": lambda k, v: memopt_C.compact_cache(s, k, v, bt, cl, keep, ring, span, max_keep=60),
+             "packed_attention": lambda k, v: memopt_C.packed_attention(q, k, v, bt, cl, cu, 1, 96),
+             "attention_scores": lambda k, v: memopt_C.attention_scores(q, k, bt, cl, cu, 1, 96),
+             "dynamic_sparse_attention": lambda k, v: memopt_C.dynamic_sparse_attention(
+                 q[:, None, :2].contiguous(), k, v, bt, cl, 96, -1)}
+    for name, call in calls.items():
+        with pytest.raises(RuntimeError, match=f"^{name}: INT4 page buffer must be contiguous"):
+            call(wide[:, :, :17 * 64], wide[:, :, :17 * 64])
+        if name != "attention_scores":
+            with pytest.raises(RuntimeError, match=f"^{name}: pass the INT4 page buffer as both"):
+                call(pages, pages.clone())
