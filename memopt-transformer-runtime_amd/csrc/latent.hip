@@ -156,12 +156,12 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
   // 32 banks apart where R + P is an odd multiple of 64).
   auto swz = [](int row) { return 2 * ((row >> 1) & 1) + ((row >> 2) & 1); };
   // (copies of the chunk's second eight rows, where they begin a copy, differ from those of the first by an offset)
-  constexpr int NOFF = NCOPY % 2 ? NCOPY : NCOPY / 2;
+  constexpr int NOFF = NCOPY % 2 ? NCOPY : NCOPY / 2, PAIRS = (NOFF + 1) / 2;
   uint32_t off[NOFF];
 #pragma unroll
   for (int c = 0; c < NOFF; ++c) {
     const int piece = c * 64 + lane, row = piece / (RB / 16), j = piece % (RB / 16);
-    off[c] = row * RB + 16 * (j ^ swz(row));
+    off[c] = row * RB + 16 * (j ^ swz(row)) - c % 2 * 1024;  // (of a pair, the second)
   }
   uint32_t ka[2];
 #pragma unroll
@@ -226,7 +226,7 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
     uint64_t linked = pages_of(entries);  // of the lanes
     uint32_t link_next = 0;               // bit g: chunk g is there
     __amdgpu_buffer_rsrc_t next[CPW];
-    constexpr int N = NCOPY * CPW;
+    constexpr int N = NCOPY / NOFF * PAIRS * CPW;
     auto prepare = [&](int32_t it) __attribute__((always_inline)) {
       const int32_t first = 4 * ((it - i0) & 15);
       link_next = (uint32_t)(linked >> first) & 15;
@@ -241,12 +241,14 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
         next[i] = uniform_rsrc(base, there ? max(0, min(16, s.len - key)) * RB : 0);
       }
     };
-    auto issue = [&](int buf, int from, int to) __attribute__((always_inline)) {  // copies [from, to) of N
+    auto issue = [&](int buf, int from, int to) __attribute__((always_inline)) {  // pairs of copies [from, to) of N
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         if (k < from || k >= to) continue;
-        const int i = k / NCOPY, c = k % NCOPY;
-        lds_dma<0, 1>(next[i], lds_u32(lds) + buf * BUF + (wave * CPW + i) * CB + c * 1024, off + c % NOFF, c < NOFF ? 0 : 8 * RB);
+        const int i = k * CPW / N, half = k / PAIRS % (NCOPY / NOFF), c = 2 * (k % PAIRS);
+        const uint32_t to_lds = lds_u32(lds) + buf * BUF + (wave * CPW + i) * CB + (half * NOFF + c) * 1024;
+        if (c + 1 < NOFF) lds_dma<0, 2>(next[i], to_lds, off + c, half * 8 * RB);
+        else lds_dma<0, 1>(next[i], to_lds, off + c, half * 8 * RB);
       }
     };
 

@@ -151,8 +151,8 @@ struct PackedV<D, MEMOPT_KV_FP16> {
 
 // A block of BLK bytes (1 or 2 KiB and a tail) into LDS at m0v, 16 bytes per
 // lane (lane16 = 16 * lane), not waited for: the compiler does not track it.
-// The immediate offsets count for both addresses, the s_nop is the wait state
-// between a write of m0 and its use, as in lds_dma.hpp, and the tail's lanes are
+// The immediate offsets count for both addresses, the s_nop are the wait states
+// between a write of m0 or of the descriptor and its use, as in lds_dma.hpp, and the tail's lanes are
 // chosen in here (a branch around them costs six scalar instructions). STREAM:
 // data read once per launch (kStreamLoad).
 #define MEMOPT_COPY(OFF, NT) "buffer_load_dwordx4 %1, %2, 0 offen offset:" OFF NT " lds\n\t"
@@ -163,7 +163,7 @@ __device__ __forceinline__ void block_copy(__amdgpu_buffer_rsrc_t r, uint32_t m0
   static_assert(BLK == 2048 + 8 * 16 || BLK == 1024 + 4 * 16, "tails of 8 and 4 lanes");
   uint64_t lanes;
 #define MEMOPT_COPY_ASM(TEXT) \
-  asm volatile("s_nop 0\n\t" TEXT : "=&s"(lanes) : "v"(lane16), "s"(r), "{m0}"(m0v) : "memory", "scc")
+  asm volatile("s_nop 4\n\t" TEXT : "=&s"(lanes) : "v"(lane16), "s"(r), "{m0}"(m0v) : "memory", "scc")
   if constexpr (BLK == 2176 && STREAM)
     MEMOPT_COPY_ASM(MEMOPT_COPY("0", " nt") MEMOPT_COPY("1024", " nt") MEMOPT_COPY_TAIL("0xff", "2048", " nt"));
   else if constexpr (BLK == 2176)
