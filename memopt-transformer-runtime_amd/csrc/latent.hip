@@ -257,7 +257,7 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
     for (int db = 0; db < NDB; ++db) o[db] = (f32x16_t){};
     // x = scale_log2 s + ncm is the exp2 argument; a new maximum lands at kTop
     // and the next rescale comes past kTop + 8 (prompt.hip).
-    constexpr float kTop = 7.0f;
+    constexpr float kTop = E::kTop;
     float ncm = 0.0f, thr = -INFINITY, lsum = 0.0f;
     bool odd = false;  // a tile of this part held inf or NaN that was made finite
     const bool any = qw0 < s.rows;

@@ -121,7 +121,7 @@ __global__ __launch_bounds__(256, 2) void latent_prompt_kernel(const ExpandedPar
   for (int db = 0; db < NDB; ++db) o[db] = (f32x16_t){};
   // x = scale_log2 s + ncm is the exp2 argument; a new maximum lands at kTop and
   // the next rescale comes past kTop + 8 (prompt.hip).
-  constexpr float kTop = 7.0f;
+  constexpr float kTop = E::kTop;
   float ncm = 0.0f, thr = -INFINITY, lsum = 0.0f;
   uint32_t odd = 0;  // nonzero where a masked tile's V held inf or NaN
   const int32_t last_row = min(qw0 + 31, len - 1);

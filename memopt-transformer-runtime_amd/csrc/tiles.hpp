@@ -30,6 +30,9 @@ struct Fp16 {
   static __device__ __forceinline__ float value(uint16_t x) { return (float)__builtin_bit_cast(half_t, x); }
   static constexpr uint32_t kOnes = 0x3C003C00u;
   static constexpr uint32_t kExponent = 0x7C00u;
+  // Where a row's maximum lands, as a power of two: weights reach 2^15 before the next rescale, and those down to 2^-21
+  // of the largest are normal numbers.
+  static constexpr float kTop = 7.0f;
 };
 struct Bf16 {
   typedef __bf16 x8 __attribute__((ext_vector_type(8)));
@@ -46,6 +49,9 @@ struct Bf16 {
   static __device__ __forceinline__ float value(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
   static constexpr uint32_t kOnes = 0x3F803F80u;
   static constexpr uint32_t kExponent = 0x7F80u;
+  // The type has 32 bits' range: weights stay under 2^-20, so that 2^20 of them times the largest value do not overflow
+  // the 32-bit sums (nor underflow with values down to 2^-98).
+  static constexpr float kTop = -28.0f;
 };
 
 __device__ __forceinline__ float both_halves_max(float v) {

@@ -268,6 +268,22 @@ def test_infinite_elements_of_weight_zero(dtype, ctx, qn, back):
     assert not bool(out[see][:, :, 7].isfinite().any())
 
 
+@pytest.mark.parametrize("power", [126, 100, -96])
+@pytest.mark.parametrize("ctx,qn", [([300, 70], [40, 1]), ([3000], [1])])
+def test_latents_of_bfloat16s_range(power, ctx, qn):
+    """Latents up to nearly the type's largest, all alike or of both signs, and small ones, where the rotary part alone
+    sets the scores: their means are in its range, and scaling by a power of two, exact, changes nothing else."""
+    c = Case(torch.bfloat16, ctx, qn, 16, 256, 64, seed=9)
+    c.q[:, :, :256] = 0
+    some = c.c[:, :, :256].clamp(-3.5, 3.5)
+    for latents in (torch.full_like(some, 3.5), some):
+        c.c[:, :, :256] = latents * 2.0 ** power
+        out = c.run()
+        assert bool(out.isfinite().all())
+        c.c[:, :, :256] = latents
+        c.check((out.double() * 2.0 ** -power).bfloat16())
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_queries_that_are_not_finite_stay_in_their_rows(dtype):
     c = Case(dtype, [100, 80], [5, 1], 16, 256, 64, seed=5)

@@ -238,3 +238,15 @@ def test_refusals():
     refused("gradients", q, k, r.clone().requires_grad_(), v, cu)
     with torch.no_grad():
         memopt_C.latent_prompt_attention(q, k, r.clone().requires_grad_(), v, cu)
+
+
+@pytest.mark.parametrize("power", [126, 100, -96])
+@pytest.mark.parametrize("lens", [[300, 70], [1500]], ids=str)
+def test_values_of_bfloat16s_range(power, lens):
+    """Values up to nearly the type's largest, all alike or of both signs, and small ones: their means are in its range,
+    and scaling by a power of two, exact, changes nothing else."""
+    q, k, r, v = make(sum(lens), 2, 128, 64, torch.bfloat16, 9)
+    for values in (torch.full_like(v, 3.5), v.clamp(-3.5, 3.5)):
+        out = memopt_C.latent_prompt_attention(q, k, r, values * 2.0 ** power, cu_of(lens))
+        assert bool(out.isfinite().all())
+        check_expanded((out.double() * 2.0 ** -power).bfloat16(), q, k, r, values, lens)
