@@ -319,7 +319,8 @@ int memopt_multi_query_path(int32_t path);
  * projections leave them (views of a fused projection included): row i of a
  * sequence sees its rows j <= i with j < num_sink_tokens or j > i -
  * window_size (window_size <= 0: all j <= i), scale 1/sqrt(head_dim).
- * Elements of hidden rows never reach a result, inf and NaN included.
+ * Elements of hidden rows never reach a result, inf and NaN included (bf16
+ * values from 2^112 on may overflow the sums).
  * head_dim 64 or 128; key and value token strides from head_dim to 2^23 - 1.
  * `out` must not overlap the inputs. */
 typedef struct memopt_prompt_desc {

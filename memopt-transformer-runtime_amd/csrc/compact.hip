@@ -16,13 +16,14 @@
 // wave per 16 new tokens and head) and writes tables and ring.
 //
 // Measured (medians): one request of 1024 tokens, two heads: 2.5 + 10 + 4 us,
-// a chain of launches, reads and barriers (the call's host side takes 16). 16
+// a chain of launches, reads and barriers (14.8 a call in a captured graph). 16
 // requests of up to 8192 tokens, 8 heads, 2048 kept, INT4: 4 + 17.4 + 20.4 us:
 // the copies' 71 MB at 3.5 TB/s; the selection's fixed 9 us (four passes of
-// five barriers, the plan) and 1 us per 1024 tokens, one workgroup a row. One
+// four barriers, the plan) and 1 us per 1024 tokens, one workgroup a row. One
 // request of 16384 tokens, 8192 kept, fp16: 2.5 + 24 + 13.5 us: eight rows
-// leave 248 compute units idle in the selection, and a selection shared by
-// several workgroups would need a launch per pass.
+// leave 248 compute units idle in the selection (sharing a row among several
+// workgroups, with a histogram in memory and a launch of 2.5 us per digit or a
+// last one to arrive, has not been built).
 #include <algorithm>
 #include <iterator>
 

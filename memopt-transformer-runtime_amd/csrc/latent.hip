@@ -16,13 +16,14 @@
 //
 // Measured (rank 512 + 64, bf16): 32 single tokens of 16 heads over up to 8192
 // tokens: 60 us with the merge's 6, 3.9 TB/s of rows read once (the copies
-// without the arithmetic: 41-48). 16 single tokens of 128 heads: 65 us with
-// the merge's 8: each 64-row tile reads all keys, so a head count of 128 reads them
-// twice. Three chunks of 256 tokens, 16 heads, beside nine single tokens: 197
+// without the arithmetic: 41-48). 16 single tokens of 128 heads: 63-66 us with
+// the merge's 9: each 64-row tile reads all keys, so a head count of 128 reads them
+// twice. Three chunks of 256 tokens, 16 heads, beside nine single tokens: 171-195
 // us with the merge's 13, 0.71 PFLOP/s: of a tile's 6400 clocks the first
 // product takes 2900 (1152 of matrix instructions, the rest the issue of
 // copies and operand reads), the softmax 500, the second product 1850 (1024),
-// barriers and the next tile's pages 1100.
+// barriers and the next tile's pages 1100. write_latent: a launch (2 us) up to
+// some 2048 tokens, 12.7 us for 32768 (150 MB, partly from the last-level cache).
 #include <algorithm>
 #include <cmath>
 
@@ -120,7 +121,7 @@ __device__ __forceinline__ uint32_t latent_run(uint32_t total, int32_t wgs) {
 
 // Two waves share 32 rows: in the first product each takes 32 of a tile's keys,
 // in the second half of the latent's columns, over all keys, so that a wave
-// holds 8 (R + P) / 16 operand and R / 4 accumulator registers (272 at 512 +
+// holds (R + P) / 4 operand and R / 4 accumulator registers (272 at 512 +
 // 64; a wave with whole rows would need 400 and spills). Between the products
 // they exchange their keys' maxima and weights through LDS. RW such pairs.
 template <int R, int P, int RW>
@@ -219,8 +220,8 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
 #pragma unroll
     for (int c = 0; c < NCH; ++c) asm volatile("" : "+a"(qf[c]));
 
-    // A tile's copies are set up together (of nothing, where no tile follows) and issued one by one between the matrix instructions of
-    // the tile before: all at once they keep a wave waiting for the queue (3400 of a tile's 9000 clocks).
+    // A tile's copies are set up together (of nothing, where no tile follows) and issued in pairs between the matrix
+    // instructions of the tile before: all at once they keep a wave waiting for the queue (3400 of a tile's 9000 clocks).
     // An entry that is no page, and rows behind the context, read as zeros.
     auto pages_of = [&](int32_t e) { return __ballot(e >= 0 && e < p.nb); };
     uint64_t linked = pages_of(entries);  // of the lanes
@@ -414,7 +415,9 @@ __global__ __launch_bounds__(RW * 128) __attribute__((amdgpu_waves_per_eu(1, 1))
       u32x4p_t pb[4], first[4];
       if (some) {
         raise_max(fmaxf(s_tops[n], s_tops[32 + n]), x);
-        // Weights enter the second product in 16 bits, and so the row's sum.
+        // Weights enter the second product in 16 bits, and so the row's sum. With what the rounding leaves as a second
+        // operand the result's error would be its own rounding alone (bf16 1.65e-3 for 1.91e-3, fp16 2.07e-4 for
+        // 2.27e-4 of its norm), for 64 instead of 60 us (32 single tokens), and 64-row tiles have no LDS for it.
         u32x4p_t mine[2];
 #pragma unroll
         for (int i = 0; i < 8; ++i) mine[i >> 2][i & 3] = E::pack(fast_exp2(x[2 * i]), fast_exp2(x[2 * i + 1]));
@@ -606,6 +609,10 @@ static int64_t latent_keys(const memopt_latent_desc &d) {
 static LatentPlan latent_plan(const memopt_latent_desc &d) {
   LatentPlan pl = {};
   const int64_t most = (int64_t)std::min(d.max_query_len, d.tokens) * d.num_heads;
+  // Tiles of 32 rows leave room for two workgroups on a compute unit at rank 128 (single tokens of 8 to 32 heads take 0.71
+  // to 0.95 of the time with 64) and at 256 + 32 (0.90 to 1.0 in batches, 1.4 for four sequences of 8192); elsewhere
+  // both take about the same (0.97 to 1.08), and 32 rows half the workspace. By the longest query of the call: the
+  // lengths are on the device.
   pl.rows = most <= 32 ? 32 : 64;
   // As many workgroups as are resident at once: the key tiles take 144 KiB of LDS at 576 elements.
   const int per_cu = std::max(1, std::min(2, 163840 / (8 * 16 * 2 * (d.rank + d.rope_dim) + pl.rows / 32 * 4352)));

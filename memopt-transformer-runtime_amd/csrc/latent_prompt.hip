@@ -12,11 +12,11 @@
 // every head's tile, so that no head's keys are ever joined in memory.
 //
 // Measured (128 + 64; medians): three prompts of up to 9000 tokens, 32 heads,
-// fp16: 0.90-0.92 ms, 0.95 PFLOP/s, 0.77 of the library's rate on a large product: a
+// fp16: 0.89-0.96 ms, 0.91-0.97 PFLOP/s, 0.74-0.79 of the library's rate on a large product: a
 // wave's softmax stands between its two products, and the other workgroup on
 // the compute unit fills in (of 256 registers 234 are taken: neither a second
 // set of scores nor copies dealt over the products fit without spills). 24 prompts of 20 to 2500 tokens, 16 heads, bf16:
-// 136-146 us, 0.65 PFLOP/s of what the mask leaves: masked tiles are whole
+// 138-148 us, 0.65 PFLOP/s of what the mask leaves: masked tiles are whole
 // products, and 2016 workgroups are four rounds of the GPU.
 #include <algorithm>
 #include <cmath>
@@ -189,7 +189,9 @@ __global__ __launch_bounds__(256, 2) void latent_prompt_kernel(const ExpandedPar
       ncm -= shift;
       thr = first && !found ? thr : kTop + 8.0f;
     }
-    // Weights enter the second product in 16 bits, and so the row's sum.
+    // Weights enter the second product in 16 bits, and so the row's sum. (What the rounding leaves, as a second operand,
+    // would bring the result's error from 1.96e-3 of its norm to its own rounding, 1.59e-3 (bf16), and the time of
+    // short prompts from 144 to 174 us, of long ones from 923 to 1203.)
     u32x4p_t pb[4];
 #pragma unroll
     for (int i = 0; i < 16; ++i)

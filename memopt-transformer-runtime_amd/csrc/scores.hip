@@ -47,7 +47,7 @@ struct ScoresParams {
 };
 
 static constexpr int kTileKeys = 256;  // keys of a workgroup: 64 per wave
-static constexpr int kFewRows = 16;
+static constexpr int kFewRows = 16;  // (the columns of one product)
 
 // A sequence as one key head sees it.
 struct ScoredSeq {
@@ -260,8 +260,13 @@ __device__ __forceinline__ f32x4p_t hide(const ScoresParams &p, f32x4p_t x, int3
 // ---------------------------------------------------------------------------
 // Few rows (decode): up to kFewRows rows per sequence and key head
 // ---------------------------------------------------------------------------
-// The weights relative to a wave's maximum are kept instead of reading the
-// keys again: 8 bytes per row and key against D / 2 + 2 D / 64 of INT4.
+// The weights relative to a wave's maximum are kept (8 bytes written and read
+// per row and key) instead of meeting the keys again in the form for chunks,
+// whose tiles have 32 rows. In us, here / there, 32 sequences of up to 8192
+// tokens, 8 key heads of 128: INT4 1 row 46 / 207, 4: 49 / 208, 8: 55 / 208,
+// 16: 72 / 203; fp16 101 / 203, 110 / 205, 117 / 205, 137 / 204; 2 key heads of
+// 64, 16 rows: 25 / 43 and 28 / 44. One sequence of 1024: 16 / 19. The form is the
+// call's, by its longest query: the lengths are on the device.
 // Bound by vector instructions (unpacking, scales and weights: 0.62 of the
 // units' time) and by the chain table, keys, weights of each tile: 32
 // sequences of up to 8192 tokens, 8 key heads of 4 rows, 128: 33 us of which

@@ -198,7 +198,9 @@ class PackedBatch(_Requests):
     def accumulate(self, query: torch.Tensor, max_new: Optional[int] = None) -> torch.Tensor:
         """Add to ``weights`` what the step's queries (as in ``attend``, which
         comes first) give each cached token; returns it. Every step, or only
-        where a prompt ends, as the policy has it."""
+        where a prompt ends, as the policy has it. ``max_new``: at least the
+        most rows of a request; steps of few tokens a request (16 rows per key
+        head) are two to four times as fast where it says so."""
         if self.weights is None:
             raise RuntimeError("PackedBatch: made without track_weights")
         self._rows_of(query)
